@@ -1,7 +1,7 @@
 """Backend selection for the functional ops (see the package docstring)."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -229,3 +229,89 @@ def lm_head_ce(x, w_head, targets, vocab: int, scale: float):
         from .native_ops import lm_head_ce as f
         return f(x, w_head, targets, vocab, scale)
     return ref.lm_head_ce(x, w_head, targets, vocab, scale)
+
+
+def embed_tokens(ids, table, scale: float = 1.0, out_dtype: Optional[torch.dtype] = None):
+    """``scale · table[ids]``: ``ids`` ``(...)`` int32 or int64, ``table`` ``(V, D)`` → ``(..., D)`` in ``out_dtype`` (the
+    table's by default).  Ids outside ``[0, V)`` give a row of zeros.  The table's gradient is dense, in its own type, and
+    summed in fp32 in an order that the ids alone fix."""
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"token ids are int32 or int64, got {ids.dtype}")
+    if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+        raise ValueError(f"the table is (rows, width), got {tuple(table.shape)}")
+    out_dtype = out_dtype or table.dtype
+    if not (table.dtype == out_dtype or table.dtype == torch.float32):
+        raise TypeError(f"a {table.dtype} table gives rows of its own type, not {out_dtype}")
+    if table.is_cuda and _BACKEND == "auto" and out_dtype in (torch.float32, torch.bfloat16, torch.float16):
+        from .embedding import embed_tokens as f
+        return f(ids, table, scale, out_dtype)
+    return ref.embed_tokens(ids, table, scale, out_dtype)
+
+
+def gated_recurrence(zgo, state=None, resets=None):
+    """``zgo`` ``(B, T, 3, D)``: candidates ``z``, gates ``g`` and output gates ``o`` of whole sequences (or of one step).
+    ``h_t = σ(g) h_{t-1} + (1 - σ(g)) z``, ``y = σ(o) h``.  ``state`` ``(B, D)`` fp32 is the ``h`` before the first step
+    (zeros by default); where ``resets`` ``(B, T)`` bool is set, a step starts a new sequence and drops ``h_{t-1}``.
+    Returns ``(y (B, T, D), state (B, D) fp32)``; sequences may be time-major views, which ``y`` then is too."""
+    if zgo.dim() != 4 or zgo.shape[2] != 3 or zgo.shape[3] == 0:
+        raise ValueError(f"the projections are (batch, steps, 3, width), got {tuple(zgo.shape)}")
+    b, t, _, d = zgo.shape
+    if state is not None and (state.shape != (b, d) or state.dtype != torch.float32):
+        raise ValueError(f"the state is fp32 {(b, d)}, got {state.dtype} {tuple(state.shape)}")
+    if resets is not None and (resets.shape != (b, t) or resets.dtype != torch.bool):
+        raise ValueError(f"the resets are bool {(b, t)}, got {resets.dtype} {tuple(resets.shape)}")
+    if b and t and _native(zgo):
+        from .recurrence import gated_recurrence as f
+        return f(zgo, state, resets)
+    return ref.gated_recurrence(zgo, state, resets)
+
+
+def gated_mlp(x, w_in, w_out, b_in=None, b_out=None, act: str = "gelu", residual=None):
+    """``(v · act(g)) W_outᵀ + b_out + residual`` with ``(v, g) = x W_inᵀ + b_in``.  ``x`` ``(..., D)``, ``w_in``
+    ``(2 F, D)`` with the value rows first and the gate rows behind them (the order of :func:`geglu`), ``w_out``
+    ``(D', F)``, ``residual`` ``(..., D')``; ``act``: ``"gelu"`` (exact) or ``"silu"``."""
+    if act not in ("gelu", "silu"):
+        raise ValueError(f"the gate's activation is 'gelu' or 'silu', got '{act}'")
+    if w_in.dim() != 2 or w_out.dim() != 2 or w_in.shape[0] != 2 * w_out.shape[1] or w_in.shape[1] != x.shape[-1] or 0 in w_in.shape:
+        raise ValueError(f"weights {tuple(w_in.shape)} and {tuple(w_out.shape)} do not make a gated block on rows of {x.shape[-1]}")
+    for name, bias, n in (("b_in", b_in, w_in.shape[0]), ("b_out", b_out, w_out.shape[0])):
+        if bias is not None and bias.shape != (n,):
+            raise ValueError(f"{name} is ({n},), got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != (*x.shape[:-1], w_out.shape[0]):
+        raise ValueError(f"the residual is {(*x.shape[:-1], w_out.shape[0])}, got {tuple(residual.shape)}")
+    if x.numel() and _native(x, family="gemm"):
+        from .feedforward import gated_mlp as f
+        return f(x, w_in, w_out, b_in, b_out, act, residual)
+    return ref.gated_mlp(x, w_in, w_out, b_in, b_out, act, residual)
+
+
+MAX_ALTERNATIVES = 32
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_ids: Optional[torch.Tensor]
+
+
+def token_logprobs(logits, targets=None, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+    """Of ``softmax(logits / temperature)`` over the last dimension: ``logprob (...)`` of ``targets (...)`` (None without),
+    ``entropy (...)`` in nats and the ``top`` most likely tokens, ``top_logprobs`` and ``top_ids`` ``(..., top)`` (None for
+    0), ties to the lowest id; all fp32 but the int64 ids.  ``logprob`` and ``entropy`` are differentiable in the logits.
+
+    A target outside the vocabulary (-1, -100) has log probability 0 and no gradient.  Logits of -inf have probability 0; a
+    row of nothing else has entropy 0, log probabilities of -inf and no gradient.  A NaN makes ``logprob`` and ``entropy`` of
+    its row NaN and counts as -inf among the alternatives."""
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"logits are (..., vocabulary), got {tuple(logits.shape)}")
+    if targets is not None and (targets.shape != logits.shape[:-1] or targets.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"targets are int32 or int64 {tuple(logits.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
+    if not 0 <= top <= min(MAX_ALTERNATIVES, logits.shape[-1]):
+        raise ValueError(f"between 0 and {min(MAX_ALTERNATIVES, logits.shape[-1])} alternatives of {logits.shape[-1]} tokens, got {top}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"the temperature is above 0 and finite, got {temperature}")
+    if logits.is_cuda and _BACKEND == "auto" and logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        from .logprobs import token_logprobs as f
+        return TokenLogprobs(*f(logits, targets, top, temperature))
+    return TokenLogprobs(*ref.token_logprobs(logits, targets, top, temperature))

@@ -131,3 +131,65 @@ def lm_head_ce(x: torch.Tensor, w_head: torch.Tensor, targets: torch.Tensor, voc
     Returns ``scale · Σ_rows CE`` (reference: ``src/main.cpp:1377-1463, 2428``)."""
     logits = (x.float() @ w_head.float().t())[:, :vocab]
     return cross_entropy_sum(logits, targets) * scale
+
+
+def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float, out_dtype: torch.dtype) -> torch.Tensor:
+    """``out[i] = scale · table[ids[i]]``; a row of zeros for ids outside the table."""
+    valid = (ids >= 0) & (ids < table.shape[0])
+    rows = table.float()[ids.clamp(0, table.shape[0] - 1).long()]
+    return torch.where(valid.unsqueeze(-1), rows * scale, 0.0).to(out_dtype)
+
+
+def gated_recurrence(zgo: torch.Tensor, state: Optional[torch.Tensor], resets: Optional[torch.Tensor]):
+    """``zgo`` ``(B, T, 3, D)``: candidates, gates, output gates.  ``h_t = f h_{t-1} + (1 - f) z`` with ``f = σ(g)``, where a
+    reset drops ``h_{t-1}``; ``y = σ(o) h``.  Returns ``y (B, T, D)`` and the last ``h`` in fp32."""
+    b, t_len, _, d = zgo.shape
+    z, g, o = zgo.float().unbind(2)
+    f, f1, s = torch.sigmoid(g), torch.sigmoid(-g), torch.sigmoid(o)
+    h = torch.zeros(b, d, dtype=torch.float32, device=zgo.device) if state is None else state
+    ys = []
+    for t in range(t_len):
+        if resets is not None:
+            h = torch.where(resets[:, t].bool().unsqueeze(1), 0.0, h)
+        h = f[:, t] * h + f1[:, t] * z[:, t]
+        ys.append(s[:, t] * h)
+    y = torch.stack(ys, 1) if ys else zgo.new_empty(b, 0, d).float()
+    return y.to(zgo.dtype), h
+
+
+def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor],
+              b_out: Optional[torch.Tensor], act: str, residual: Optional[torch.Tensor]) -> torch.Tensor:
+    """``(v · act(g)) W_outᵀ + b_out + residual`` with ``(v, g) = x W_inᵀ + b_in``: value half first."""
+    vg = x.float() @ w_in.float().t()
+    if b_in is not None:
+        vg = vg + b_in.float()
+    v, g = vg.chunk(2, dim=-1)
+    y = (v * (F.silu(g) if act == "silu" else F.gelu(g))) @ w_out.float().t()
+    if b_out is not None:
+        y = y + b_out.float()
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(x.dtype)
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], top: int, temperature: float):
+    """``(log p[target], entropy, top log p, top ids)`` of ``softmax(logits / temperature)``; ties go to the lowest id, a NaN
+    counts as -inf among the alternatives.  A target outside the vocabulary has 0 and no gradient; a row of -inf only has
+    entropy 0, log probabilities of -inf and no gradient."""
+    vocab = logits.shape[-1]
+    x = logits.float() / temperature
+    nothing = (x == float("-inf")).all(-1)
+    logp = torch.log_softmax(x.masked_fill(nothing.unsqueeze(-1), 0.0), dim=-1)
+    entropy = -(logp.exp() * logp.masked_fill(logp == float("-inf"), 0.0)).sum(-1).masked_fill(nothing, 0.0)
+    logp = logp.masked_fill(nothing.unsqueeze(-1), float("-inf"))
+    logprob = None
+    if targets is not None:
+        valid = (targets >= 0) & (targets < vocab)
+        logprob = logp.gather(-1, targets.clamp(0, vocab - 1).long().unsqueeze(-1)).squeeze(-1).masked_fill(~valid, 0.0)
+    if top == 0:
+        return logprob, entropy, None, None
+    with torch.no_grad():
+        order = logits.float()
+        order = torch.where(order.isnan(), float("-inf"), order)
+        ids = order.sort(dim=-1, descending=True, stable=True)[1][..., :top]
+        return logprob, entropy, logp.gather(-1, ids), ids
