@@ -3,19 +3,34 @@
 // and its gradient, with e_t = what step t hands to the step before it:
 //   dh_t = dy_t sigmoid(o_t) + e_{t+1}      e_t = (reset_t ? 0 : f_t) dh_t
 //   dz = (1 - f) dh     dg = (h_{t-1} - z) f (1 - f) dh     do = dy h sigmoid(o) (1 - sigmoid(o))
-// Both directions are scans of x -> a x + b: a warp takes 32 x VEC channels of kSteps consecutive steps, all warps of a CTA
-// take consecutive chunks, and what a chunk does to a value that comes in, (product of a, result from 0), is passed on in
-// shared memory before every warp walks its chunk again from the true value.  The state is fp32 throughout; the forward leaves
-// the state in front of every chunk for the backward, which rebuilds h from it in registers.
+// Both directions are scans of x -> a x + b.  A warp takes 64 channels of a chunk of consecutive steps, the warps of a CTA and the
+// CTAs of a cluster take consecutive chunks, and a cluster walks along its sequence.  What a chunk does to a value that comes
+// in, (product of a, result from 0), is a link; links are passed on before every warp walks its chunk again from the true
+// value: between warps in shared memory, between CTAs by asynchronous stores into each other's shared memory.  The state is
+// fp32 throughout; the forward leaves it in front of every eighth step for the backward, which rebuilds h from it.
+//
+// Bound: 8 bytes a value of h forward, 14 backward (16 bytes more for every 32 of them: the saved states).  The arithmetic is
+// close behind, four operations of the special-function units a value in either direction, so the two gates' exponentials and
+// reciprocals are formed once and everything else is packed.  Measured, bf16: 1 x 30011 x 2048 125 us forward (64 % of the
+// copy rate) and 207 us backward (66 %); 8 x 1024 x 1024 22 and 31 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "elem16.cuh"
 #include "gemm_tcgen05.h"
+#include "tc05.cuh"
+#include "tensor_map.h"
+
+extern int g_fbam_last_driver_error;   // defined in gemm_tcgen05.cu
 
 namespace {
 
-constexpr int kSteps = 16;        // steps of a chunk
+using namespace tc05;
+
+constexpr int kSaved = 8;         // the forward keeps the state in front of every eighth step
+constexpr int kFwdSteps = 16;     // of a chunk of the forward by TMA; all others have kSaved steps
+constexpr int kMaxCtas = 8;       // of a cluster
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -27,47 +42,104 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// sigmoid(x) and sigmoid(-x), both to full relative accuracy
-__device__ __forceinline__ void gate(float x, float& f, float& f1) {
-  const float e = ex2(-1.4426950408889634f * fabsf(x));
-  const float p = rcp(1.0f + e), q = e * p;
-  f = x >= 0.0f ? p : q;
-  f1 = x >= 0.0f ? q : p;
-  if (x != x) f = f1 = x;
+// A lane's channels: two packed values (sm_100 computes on two fp32 values per instruction) or one.
+template <int VEC>
+struct Vec;
+template <>
+struct Vec<1> {
+  float v;
+  __device__ __forceinline__ static Vec all(float a) { return {a}; }
+  __device__ __forceinline__ float get(int) const { return v; }
+};
+template <>
+struct Vec<2> {
+  float2 v;
+  __device__ __forceinline__ static Vec all(float a) { return {make_float2(a, a)}; }
+  __device__ __forceinline__ float get(int j) const { return j ? v.y : v.x; }
+};
+__device__ __forceinline__ Vec<1> fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Vec<2> fma(Vec<2> a, Vec<2> b, Vec<2> c) { return {__ffma2_rn(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Vec<1> operator*(Vec<1> a, Vec<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b) { return {__fmul2_rn(a.v, b.v)}; }
+__device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {a.v + b.v}; }
+__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b) { return {__fadd2_rn(a.v, b.v)}; }
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> operator-(Vec<VEC> a, Vec<VEC> b) { return fma(b, Vec<VEC>::all(-1.0f), a); }
+__device__ __forceinline__ Vec<1> ex2(Vec<1> a) { return {ex2(a.v)}; }
+__device__ __forceinline__ Vec<2> ex2(Vec<2> a) { return {make_float2(ex2(a.v.x), ex2(a.v.y))}; }
+__device__ __forceinline__ Vec<1> rcp(Vec<1> a) { return {rcp(a.v)}; }
+__device__ __forceinline__ Vec<2> rcp(Vec<2> a) { return {make_float2(rcp(a.v.x), rcp(a.v.y))}; }
+__device__ __forceinline__ Vec<1> pick(bool c, Vec<1> a, Vec<1> b) { return {c ? a.v : b.v}; }
+__device__ __forceinline__ Vec<2> pick(bool c, Vec<2> a, Vec<2> b) { return {make_float2(c ? a.v.x : b.v.x, c ? a.v.y : b.v.y)}; }
+
+// sigmoid(x) to full relative accuracy at both ends
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> sigmoid(Vec<VEC> x) {
+  return rcp(ex2(x * Vec<VEC>::all(-kLog2e)) + Vec<VEC>::all(1.0f));
+}
+// -sigmoid(-x), the same
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> minus_sigmoid_minus(Vec<VEC> x) {
+  return rcp(Vec<VEC>::all(-1.0f) - ex2(x * Vec<VEC>::all(kLog2e)));
+}
+__device__ __forceinline__ float below(float x, float most) {     // NaN stays NaN
+  float a;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(x), "f"(most));
+  return a;
+}
+__device__ __forceinline__ Vec<1> below(Vec<1> x, float most) { return {below(x.v, most)}; }
+__device__ __forceinline__ Vec<2> below(Vec<2> x, float most) { return {make_float2(below(x.v.x, most), below(x.v.y, most))}; }
+// f = sigmoid(x) and nf1 = -sigmoid(-x), both to full relative accuracy; exp is kept finite for its product with 0
+template <int VEC>
+__device__ __forceinline__ void gates(Vec<VEC> x, Vec<VEC>& f, Vec<VEC>& nf1) {
+  const Vec<VEC> e = ex2(below(x * Vec<VEC>::all(kLog2e), 126.0f));
+  const Vec<VEC> r = rcp(e + Vec<VEC>::all(1.0f));
+  f = e * r;
+  nf1 = r * Vec<VEC>::all(-1.0f);
 }
 
+// VEC elements as they lie in memory
 template <int VEC>
-struct Vec { float v[VEC]; };
-template <int VEC>
-__device__ __forceinline__ Vec<VEC> load(const elem_t* p) {
-  Vec<VEC> r;
-  if constexpr (VEC == 2) {
-    const float2 f = e22ff(*reinterpret_cast<const elem2_t*>(p));
-    r.v[0] = f.x; r.v[1] = f.y;
-  } else {
-    r.v[0] = e2f(*p);
+struct Raw {
+  uint32_t u;
+  __device__ __forceinline__ void load(const elem_t* p) {
+    if constexpr (VEC == 2) u = *reinterpret_cast<const uint32_t*>(p);
+    else u = *reinterpret_cast<const uint16_t*>(p);
   }
-  return r;
-}
+  __device__ __forceinline__ Vec<VEC> get() const {
+    if constexpr (VEC == 2) return {e22ff(*reinterpret_cast<const elem2_t*>(&u))};
+    else {
+      const uint16_t h = (uint16_t)u;
+      return {e2f(*reinterpret_cast<const elem_t*>(&h))};
+    }
+  }
+};
+__device__ __forceinline__ void store(elem_t* p, Vec<2> r) { *reinterpret_cast<elem2_t*>(p) = ff2e2(r.v.x, r.v.y); }
+__device__ __forceinline__ void store(elem_t* p, Vec<1> r) { *p = f2e(r.v); }
+__device__ __forceinline__ void store(float* p, Vec<2> r) { p[0] = r.v.x; p[1] = r.v.y; }
+__device__ __forceinline__ void store(float* p, Vec<1> r) { *p = r.v; }
 template <int VEC>
-__device__ __forceinline__ void store(elem_t* p, const Vec<VEC>& r) {
-  if constexpr (VEC == 2) *reinterpret_cast<elem2_t*>(p) = ff2e2(r.v[0], r.v[1]);
-  else *p = f2e(r.v[0]);
+__device__ __forceinline__ Vec<VEC> load(const float* p) {
+  if constexpr (VEC == 2) return {make_float2(p[0], p[1])};
+  else return {*p};
 }
 
 // What a chunk makes of a value that comes in.  A gain below 0 marks a chunk with a reset: nothing of what comes in goes on,
 // not even as a product of 0 with an infinity or a NaN of the sequence before.
 template <int VEC>
-__device__ __forceinline__ Vec<VEC> drops() {
-  Vec<VEC> r;
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) r.v[j] = -1.0f;
-  return r;
-}
-__device__ __forceinline__ float pass(float gain, float from0, float x) { return gain < 0.0f ? from0 : fmaf(gain, x, from0); }
+struct Link {
+  Vec<VEC> gain, from0;
+  __device__ __forceinline__ Vec<VEC> operator()(Vec<VEC> x) const {
+    return pick(gain.get(0) < 0.0f, from0, fma(gain, x, from0));      // a mark is in all of a lane's channels
+  }
+  // this one, then `next`
+  __device__ __forceinline__ Link then(const Link& next) const {
+    return {pick(gain.get(0) < 0.0f || next.gain.get(0) < 0.0f, Vec<VEC>::all(-1.0f), gain * next.gain), next(from0)};
+  }
+};
 
 struct Shape {
-  int batch, steps, dim, chunks;
+  int batch, steps, dim, states;    // states: saved ones of a sequence
   long long zb, zt, zk;             // strides of zgo: sequence, step, member
   long long yb, yt;                 // of y, or of dy in the backward
   long long rb, rt;                 // of the resets
@@ -81,245 +153,574 @@ __device__ __forceinline__ uint32_t reset_bits(const uint8_t* resets, const Shap
   return __ballot_sync(0xffffffffu, r);
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Sends a link to the same place in the shared memory of CTA `rank`, counted on the barrier at the same place there.
+__device__ __forceinline__ void push(const Link<2>* place, uint64_t* bar, uint32_t rank, const Link<2>& l) {
+  uint32_t at, at_bar;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(place)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_bar) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "f"(l.gain.v.x),
+               "f"(l.gain.v.y), "f"(l.from0.v.x), "f"(l.from0.v.y), "r"(at_bar) : "memory");
+}
+__device__ __forceinline__ void push(const Link<1>* place, uint64_t* bar, uint32_t rank, const Link<1>& l) {
+  uint32_t at, at_bar;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(place)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_bar) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(at), "f"(l.gain.v), "f"(l.from0.v),
+               "r"(at_bar) : "memory");
+}
+
+// The links of a walk step: of the warps of this CTA, and of the CTAs of the cluster, each sent there by its CTA.  Two sets take
+// turns: whoever writes a set again has passed the step between, to which every reader of the set has contributed.
+template <int VEC, int WARPS>
+struct __align__(16) Exchange {
+  Link<VEC> warps[2][WARPS][32], ctas[2][kMaxCtas][32];
+  uint64_t arrived[2];
+  // before the first exchange
+  __device__ __forceinline__ void init() {
+    if (cluster_size() == 1) return;
+    if (threadIdx.x == 0) {
+      mbar_init(&arrived[0], 1);
+      mbar_init(&arrived[1], 1);
+      mbar_fence_init();
+    }
+    cluster_sync();
+  }
+};
+
+// Passes `mine` on and returns what comes in to this warp's chunk; `carry` is what comes in to the cluster's first chunk, and
+// becomes what its last chunk hands on.  Chunks follow one another by (place of the CTA, place of the warp).  round: of this
+// launch, from 0.
+template <int VEC, int WARPS>
+__device__ __forceinline__ Vec<VEC> exchange(Exchange<VEC, WARPS>& ex, int round, const Link<VEC>& mine, int place, bool backwards,
+                                             Vec<VEC>& carry, int* status) {
+  Vec<VEC> in = carry;
+  if constexpr (WARPS == 1) {
+    carry = mine(carry);
+  } else {
+    const int lane = threadIdx.x % 32, turn = round & 1;
+    const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+    ex.warps[turn][place][lane] = mine;
+    __syncthreads();
+    if (ctas == 1) {
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == place) in = carry;
+        carry = ex.warps[turn][w][lane](carry);
+      }
+    } else {
+      Link<VEC> before{Vec<VEC>::all(1.0f), Vec<VEC>::all(0.0f)};     // of the warps before this one
+#pragma unroll
+      for (int w = 0; w < WARPS - 1; ++w)
+        if (w < place) before = before.then(ex.warps[turn][w][lane]);
+      const int here = backwards ? ctas - 1 - rank : rank;
+      if (place == WARPS - 1) {                                       // of the CTA as a whole
+        const Link<VEC> all = before.then(mine);
+        if (lane == 0) mbar_expect_tx(&ex.arrived[turn], ctas * 32 * (uint32_t)sizeof(Link<VEC>));
+        for (int c = 0; c < ctas; ++c) push(&ex.ctas[turn][here][lane], &ex.arrived[turn], c, all);
+      }
+      if (!mbar_wait(&ex.arrived[turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_EPILOGUE_TIMEOUT);
+#pragma unroll
+      for (int c = 0; c < kMaxCtas; ++c) {
+        if (c >= ctas) break;
+        if (c == here) in = carry;
+        carry = ex.ctas[turn][c][lane](carry);
+      }
+      in = before(in);
+    }
+  }
+  return in;
+}
+
+// The walks over a chunk of STEPS steps.  FAST: all of them are there and none is a reset.  z, g, o, d: functions of the step
+// that give the inputs (0 behind the end), put: one that takes an output.  nf1: -(1 - f).
+template <bool FAST, int STEPS, int VEC, typename Z, typename G>
+__device__ __forceinline__ void forward_in(Vec<VEC> (&nf1)[STEPS], Link<VEC>& link, int n, uint32_t bits, Z z, G g) {
+  using V = Vec<VEC>;
+  link.gain = V::all(1.0f);
+  link.from0 = V::all(0.0f);
+#pragma unroll
+  for (int t = 0; t < STEPS; ++t) {
+    nf1[t] = minus_sigmoid_minus<VEC>(g(t));
+    if (!FAST && t >= n) nf1[t] = V::all(0.0f);             // behind the end nothing changes
+    if (!FAST && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
+    // h - (1 - f) (h - z): 1 - f is known to its last bits where f is near 1
+    link.from0 = fma(nf1[t], link.from0 - z(t), link.from0);
+    link.gain = fma(nf1[t], link.gain, link.gain);
+  }
+  if (!FAST && bits) link.gain = V::all(-1.0f);
+}
+
+template <bool FAST, int STEPS, int VEC, typename Z, typename O, typename P>
+__device__ __forceinline__ void forward_out(const Vec<VEC> (&nf1)[STEPS], Vec<VEC>& h, float* saved, int dim, int n, uint32_t bits,
+                                            Z z, O o, P put) {
+  using V = Vec<VEC>;
+#pragma unroll
+  for (int t = 0; t < STEPS; ++t) {
+    if (t % kSaved == 0 && saved != nullptr && (FAST || t < n)) store(saved + t / kSaved * dim, h);
+    if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
+    h = fma(nf1[t], h - z(t), h);
+    put(t, sigmoid<VEC>(o(t)) * h);
+  }
+}
+
+// Forwards over the chunk from the state h in front of it, and with it the gradient of the output gate.  What is left for the
+// walk back: nf1, u (the factor of dg), and dh0 (the part of dh that a step's own y gives).
+template <bool FAST, int STEPS, int VEC, typename Z, typename G, typename O, typename D, typename P>
+__device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&u)[STEPS], Vec<VEC> (&dh0)[STEPS], Link<VEC>& link,
+                                            Vec<VEC> h, int n, uint32_t bits, Z z, G g, O o, D d, P put) {
+  using V = Vec<VEC>;
+#pragma unroll
+  for (int t = 0; t < STEPS; ++t) {
+    if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
+    V f, so, nso1;
+    gates<VEC>(g(t), f, nf1[t]);
+    gates<VEC>(o(t), so, nso1);
+    const V step = h - z(t);
+    u[t] = (step * f) * (nf1[t] * V::all(-1.0f));
+    h = fma(nf1[t], step, h);
+    dh0[t] = d(t) * so;
+    put(t, (dh0[t] * h) * (nso1 * V::all(-1.0f)));
+    if (!FAST && t >= n) nf1[t] = dh0[t] = V::all(0.0f);    // behind the end e passes unchanged
+  }
+  link.gain = V::all(1.0f);
+  link.from0 = V::all(0.0f);
+#pragma unroll
+  for (int t = STEPS - 1; t >= 0; --t) {
+    const V dh = link.from0 + dh0[t];
+    link.from0 = fma(nf1[t], dh, dh);
+    if (!FAST && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
+    link.gain = fma(nf1[t], link.gain, link.gain);
+  }
+  if (!FAST && bits) link.gain = V::all(-1.0f);
+}
+
+template <bool FAST, int STEPS, int VEC, typename P, typename Q>
+__device__ __forceinline__ void backward_out(const Vec<VEC> (&nf1)[STEPS], const Vec<VEC> (&u)[STEPS], const Vec<VEC> (&dh0)[STEPS],
+                                             Vec<VEC> e, uint32_t bits, P put_z, Q put_g) {
+  using V = Vec<VEC>;
+#pragma unroll
+  for (int t = STEPS - 1; t >= 0; --t) {
+    const V dh = e + dh0[t];
+    put_z(t, (nf1[t] * dh) * V::all(-1.0f));
+    put_g(t, u[t] * dh);
+    e = fma(nf1[t], dh, dh);
+    if (!FAST && ((bits >> t) & 1)) e = V::all(0.0f);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Any alignment, and a few steps: inputs in registers by plain loads
+// ---------------------------------------------------------------------------------------------------------------
+template <int VEC, int STEPS>
+__device__ __forceinline__ void fetch(Raw<VEC> (&r)[STEPS], const elem_t* p, long long step, int n) {
+#pragma unroll
+  for (int t = 0; t < STEPS; ++t) {
+    r[t] = Raw<VEC>{0};
+    if (t < n) r[t].load(p + t * step);
+  }
+}
+
 template <int VEC, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
 recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ state_in, const uint8_t* __restrict__ resets,
-                      elem_t* __restrict__ y, float* __restrict__ state_out, float* __restrict__ saved, const Shape s) {
-  __shared__ Vec<VEC> gain[WARPS][32], from0[WARPS][32];
+                      elem_t* __restrict__ y, float* __restrict__ state_out, float* __restrict__ saved, int* status, const Shape s) {
+  constexpr int STEPS = kSaved;
+  __shared__ Exchange<VEC, WARPS> ex;
+  ex.init();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int b = blockIdx.y, ch = (blockIdx.x * 32 + lane) * VEC;
-  const bool in = ch < s.dim;
-  const elem_t* src = zgo + b * s.zb + ch;
-  Vec<VEC> h_in = {};
-  if (in && state_in != nullptr) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) h_in.v[j] = state_in[(long long)b * s.dim + ch + j];
-  }
-  for (int c0 = 0; c0 < s.chunks; c0 += WARPS) {
-    const int chunk = c0 + warp, t0 = chunk * kSteps;
-    const int n = min(kSteps, s.steps - t0);                // may be below 0
+  const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+  const int b = blockIdx.y, own = (blockIdx.x / ctas * 32 + lane) * VEC;
+  const bool in = own < s.dim;
+  const int ch = in ? own : s.dim - VEC;                    // lanes behind the last channel compute it too
+  Vec<VEC> carry = state_in != nullptr ? load<VEC>(state_in + (long long)b * s.dim + ch) : Vec<VEC>::all(0.0f);
+  int round = 0;
+  for (int c0 = 0; c0 < s.states; c0 += ctas * WARPS, ++round) {
+    const int chunk = c0 + rank * WARPS + warp, t0 = chunk * STEPS;
+    const int n = min(STEPS, s.steps - t0);                 // may be below 0
     const uint32_t bits = reset_bits(resets, s, b, t0, n);
-    Vec<VEC> z[kSteps], q[kSteps], o[kSteps];
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      z[t] = q[t] = o[t] = Vec<VEC>{};
-      if (in && t < n) {
-        const elem_t* p = src + (t0 + t) * s.zt;
-        z[t] = load<VEC>(p);
-        q[t] = load<VEC>(p + s.zk);
-        o[t] = load<VEC>(p + 2 * s.zk);
-      }
-    }
-    Vec<VEC> a, h;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { a.v[j] = 1.0f; h.v[j] = 0.0f; }
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      const bool reset = (bits >> t) & 1;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float f, f1;
-        gate(q[t].v[j], f, f1);
-        if (t >= n) f1 = 0.0f;                              // steps behind the end change nothing
-        q[t].v[j] = f1;
-        // h - (1 - f) (h - z): 1 - f is known to its last bits where f is near 1
-        if (reset) h.v[j] = 0.0f;
-        h.v[j] = fmaf(f1, z[t].v[j] - h.v[j], h.v[j]);
-        a.v[j] = fmaf(-f1, a.v[j], a.v[j]);
-      }
-    }
-    gain[warp][lane] = bits ? drops<VEC>() : a;
-    from0[warp][lane] = h;
-    __syncthreads();
-    Vec<VEC> mine = h_in;
-    h = h_in;
-    for (int w = 0; w < WARPS; ++w) {
-      if (w == warp) mine = h;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) h.v[j] = pass(gain[w][lane].v[j], from0[w][lane].v[j], h.v[j]);
-    }
-    h_in = h;
-    __syncthreads();
-    h = mine;
-    if (in && saved != nullptr && n > 0) {
-      float* at = saved + ((long long)b * s.chunks + chunk) * s.dim + ch;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) at[j] = h.v[j];
-    }
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      Vec<VEC> out;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if ((bits >> t) & 1) h.v[j] = 0.0f;
-        h.v[j] = fmaf(q[t].v[j], z[t].v[j] - h.v[j], h.v[j]);
-        float f, f1;
-        gate(o[t].v[j], f, f1);
-        out.v[j] = f * h.v[j];
-      }
-      if (in && t < n) store<VEC>(y + b * s.yb + (t0 + t) * s.yt + ch, out);
-    }
-    if (in && t0 + kSteps >= s.steps && n > 0) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) state_out[(long long)b * s.dim + ch + j] = h.v[j];
-    }
+    const elem_t* src = zgo + b * s.zb + t0 * s.zt + ch;
+    Raw<VEC> z[STEPS], g[STEPS], o[STEPS];
+    fetch(g, src + s.zk, s.zt, n);
+    fetch(z, src, s.zt, n);
+    fetch(o, src + 2 * s.zk, s.zt, n);
+    Vec<VEC> nf1[STEPS];
+    Link<VEC> link;
+    forward_in<false>(nf1, link, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return g[t].get(); });
+    Vec<VEC> h = exchange<VEC, WARPS>(ex, round, link, warp, false, carry, status);
+    elem_t* out = y + b * s.yb + t0 * s.yt + ch;
+    float* at = saved != nullptr && in ? saved + ((long long)b * s.states + chunk) * s.dim + ch : nullptr;
+    forward_out<false>(nf1, h, at, s.dim, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return o[t].get(); },
+                       [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * s.yt, v); });
+    if (in && t0 + STEPS >= s.steps && n > 0) store(state_out + (long long)b * s.dim + ch, h);
   }
+  if (ctas > 1) cluster_sync();     // no CTA leaves while another may still read its links
 }
 
 template <int VEC, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
 recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict__ resets, const float* __restrict__ saved,
                       const elem_t* __restrict__ dy, const float* __restrict__ d_state_out, elem_t* __restrict__ d_zgo,
-                      float* __restrict__ d_state_in, const Shape s, long long db, long long dt) {
-  __shared__ Vec<VEC> gain[WARPS][32], from0[WARPS][32];
+                      float* __restrict__ d_state_in, int* status, const Shape s, long long db, long long dt) {
+  constexpr int STEPS = kSaved;
+  __shared__ Exchange<VEC, WARPS> ex;
+  ex.init();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int b = blockIdx.y, ch = (blockIdx.x * 32 + lane) * VEC;
-  const bool in = ch < s.dim;
-  const elem_t* src = zgo + b * s.zb + ch;
-  Vec<VEC> e_in = {};
-  if (in && d_state_out != nullptr) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) e_in.v[j] = d_state_out[(long long)b * s.dim + ch + j];
-  }
-  const int rounds = (s.chunks + WARPS - 1) / WARPS;
-  for (int round = rounds - 1; round >= 0; --round) {
-    const int chunk = round * WARPS + warp, t0 = chunk * kSteps;
-    const int n = min(kSteps, s.steps - t0);
+  const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+  const int b = blockIdx.y, own = (blockIdx.x / ctas * 32 + lane) * VEC;
+  const bool in = own < s.dim;
+  const int ch = in ? own : s.dim - VEC;
+  Vec<VEC> carry = d_state_out != nullptr ? load<VEC>(d_state_out + (long long)b * s.dim + ch) : Vec<VEC>::all(0.0f);
+  const int per_step = ctas * WARPS, rounds = (s.states + per_step - 1) / per_step;
+  for (int round = 0; round < rounds; ++round) {
+    const int chunk = (rounds - 1 - round) * per_step + rank * WARPS + warp, t0 = chunk * STEPS;
+    const int n = min(STEPS, s.steps - t0);
     const uint32_t bits = reset_bits(resets, s, b, t0, n);
-    Vec<VEC> h[kSteps], z[kSteps], q[kSteps], o[kSteps], d[kSteps], h0 = {};
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      z[t] = q[t] = o[t] = d[t] = Vec<VEC>{};
-      if (in && t < n) {
-        const elem_t* p = src + (t0 + t) * s.zt;
-        z[t] = load<VEC>(p);
-        q[t] = load<VEC>(p + s.zk);
-        o[t] = load<VEC>(p + 2 * s.zk);
-        d[t] = load<VEC>(dy + b * s.yb + (t0 + t) * s.yt + ch);
-      }
+    const elem_t* src = zgo + b * s.zb + t0 * s.zt + ch;
+    elem_t* out = d_zgo + b * db + t0 * dt + ch;
+    Raw<VEC> z[STEPS], g[STEPS], o[STEPS], d[STEPS];
+    fetch(g, src + s.zk, s.zt, n);
+    fetch(z, src, s.zt, n);
+    fetch(o, src + 2 * s.zk, s.zt, n);
+    fetch(d, dy + b * s.yb + t0 * s.yt + ch, s.yt, n);
+    const Vec<VEC> h = n > 0 ? load<VEC>(saved + ((long long)b * s.states + chunk) * s.dim + ch) : Vec<VEC>::all(0.0f);
+    Vec<VEC> nf1[STEPS], u[STEPS], dh0[STEPS];
+    Link<VEC> link;
+    backward_in<false>(nf1, u, dh0, link, h, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return g[t].get(); },
+                       [&](int t) { return o[t].get(); }, [&](int t) { return d[t].get(); },
+                       [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + 2 * s.dim, v); });
+    const Vec<VEC> e = exchange<VEC, WARPS>(ex, round, link, WARPS - 1 - warp, true, carry, status);
+    backward_out<false>(nf1, u, dh0, e, bits, [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt, v); },
+                        [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + s.dim, v); });
+  }
+  if (in && rank == 0 && warp == 0 && d_state_in != nullptr) store(d_state_in + (long long)b * s.dim + ch, carry);
+  if (ctas > 1) cluster_sync();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Rows of 16-byte pieces: tiles by TMA.  Each warp fetches the chunk of its next walk step while it works on this one, and
+// writes results over the inputs that it has read, from where they leave by TMA; what lies behind the last step or channel is
+// filled with zeros on the way in and clipped on the way out.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kWarps = 8, kSlab = 64;       // channels of a tile: two a lane
+
+struct Tile {
+  elem_t* at;                               // [members][STEPS][kSlab], this lane's two channels
+  int steps;
+  __device__ __forceinline__ Vec<2> get(int member, int t) const {
+    return {e22ff(*reinterpret_cast<const elem2_t*>(at + (member * steps + t) * kSlab))};
+  }
+  __device__ __forceinline__ void put(int member, int t, Vec<2> v) const { store(at + (member * steps + t) * kSlab, v); }
+};
+
+template <int STEPS>
+struct FwdSmem {
+  alignas(128) elem_t tiles[kWarps][2][3][STEPS][kSlab];
+  Exchange<2, kWarps> ex;
+  uint64_t full_zg[kWarps][2], full_o[kWarps][2];
+};
+
+template <int STEPS>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_y,
+                          const float* __restrict__ state_in, const uint8_t* __restrict__ resets, float* __restrict__ state_out,
+                          float* __restrict__ saved, int* status, const Shape s) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  FwdSmem<STEPS>& sm = *reinterpret_cast<FwdSmem<STEPS>*>(smem_raw);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+  const int b = blockIdx.y, ch0 = blockIdx.x / ctas * kSlab, ch = ch0 + 2 * lane;
+  const bool in = ch < s.dim;
+  if (lane == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.full_zg[warp][i], 1);
+      mbar_init(&sm.full_o[warp][i], 1);
     }
-    if (in && n > 0) {
-      const float* at = saved + ((long long)b * s.chunks + chunk) * s.dim + ch;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) h0.v[j] = at[j];
+    mbar_fence_init();
+  }
+  sm.ex.init();
+  __syncwarp();
+  auto issue_zg = [&](int t0, int buf) {                    // one lane
+    mbar_expect_tx(&sm.full_zg[warp][buf], 2 * STEPS * kSlab * 2);
+    for (int k = 0; k < 2; ++k) tma_load_4d(sm.tiles[warp][buf][k], &map_in, &sm.full_zg[warp][buf], ch0, k, t0, b);
+  };
+  auto issue_o = [&](int t0, int buf) {
+    mbar_expect_tx(&sm.full_o[warp][buf], STEPS * kSlab * 2);
+    tma_load_4d(sm.tiles[warp][buf][2], &map_in, &sm.full_o[warp][buf], ch0, 2, t0, b);
+  };
+  Vec<2> carry = Vec<2>::all(0.0f);
+  if (in && state_in != nullptr) carry = load<2>(state_in + (long long)b * s.dim + ch);
+  const int per_step = ctas * kWarps * STEPS;
+  int t0 = (rank * kWarps + warp) * STEPS;
+  if (lane == 0 && t0 < s.steps) {
+    issue_zg(t0, 0);
+    issue_o(t0, 0);
+  }
+  uint32_t next_bits = reset_bits(resets, s, b, t0, min(STEPS, s.steps - t0));
+  for (int base = 0, round = 0; base < s.steps; base += per_step, t0 += per_step, ++round) {
+    const int turn = round & 1;
+    const int n = min(STEPS, s.steps - t0);                 // may be below 0
+    const uint32_t bits = next_bits;
+    const bool fast = n == STEPS && bits == 0;
+    const Tile tile{&sm.tiles[warp][turn][0][0][2 * lane], STEPS};
+    const bool more = t0 + per_step < s.steps;
+    if (n > 0 && !mbar_wait(&sm.full_zg[warp][turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_PRODUCER_TIMEOUT);
+    if (more && lane == 0) issue_zg(t0 + per_step, turn ^ 1);
+    if (more) next_bits = reset_bits(resets, s, b, t0 + per_step, min(STEPS, s.steps - t0 - per_step));
+    auto z = [&](int t) { return tile.get(0, t); };
+    auto g = [&](int t) { return tile.get(1, t); };
+    auto o = [&](int t) { return tile.get(2, t); };
+    auto put = [&](int t, Vec<2> v) { tile.put(2, t, v); };
+    Vec<2> nf1[STEPS];
+    Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
+    if (fast) forward_in<true>(nf1, link, n, bits, z, g);
+    else if (n > 0) forward_in<false>(nf1, link, n, bits, z, g);
+    // Results go over the output gates that they come from.  The ones of the step before take a while to leave the other buffer,
+    // so its output gates, which are needed last, are fetched only now.
+    if (more && lane == 0) {
+      bulk_wait_group_read<0>();
+      issue_o(t0 + per_step, turn ^ 1);
     }
-    Vec<VEC> a, e = h0;
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if ((bits >> t) & 1) e.v[j] = 0.0f;
-        float f, f1;
-        gate(q[t].v[j], f, f1);
-        e.v[j] = fmaf(f1, z[t].v[j] - e.v[j], e.v[j]);
-        h[t].v[j] = e.v[j];
-      }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { a.v[j] = 1.0f; e.v[j] = 0.0f; }
-#pragma unroll
-    for (int t = kSteps - 1; t >= 0; --t)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (t >= n) continue;
-        float f, f1, so, so1;
-        gate(q[t].v[j], f, f1);
-        gate(o[t].v[j], so, so1);
-        e.v[j] = (bits >> t) & 1 ? 0.0f : f * fmaf(d[t].v[j], so, e.v[j]);
-        a.v[j] *= f;
-      }
-    gain[warp][lane] = bits ? drops<VEC>() : a;
-    from0[warp][lane] = e;
-    __syncthreads();
-    Vec<VEC> mine = e_in;
-    e = e_in;
-    for (int w = WARPS - 1; w >= 0; --w) {
-      if (w == warp) mine = e;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) e.v[j] = pass(gain[w][lane].v[j], from0[w][lane].v[j], e.v[j]);
-    }
-    e_in = e;
-    __syncthreads();
-    e = mine;
-#pragma unroll
-    for (int t = kSteps - 1; t >= 0; --t) {
-      if (t >= n) continue;
-      Vec<VEC> dz, dg, dout;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const bool reset = (bits >> t) & 1;
-        float f, f1, so, so1;
-        gate(q[t].v[j], f, f1);
-        gate(o[t].v[j], so, so1);
-        const float dh = fmaf(d[t].v[j], so, e.v[j]);
-        const float before = reset ? 0.0f : t > 0 ? h[t > 0 ? t - 1 : 0].v[j] : h0.v[j];
-        dz.v[j] = f1 * dh;
-        dg.v[j] = (before - z[t].v[j]) * f * f1 * dh;
-        dout.v[j] = d[t].v[j] * h[t].v[j] * so * so1;
-        e.v[j] = reset ? 0.0f : f * dh;
-      }
-      if (in) {
-        elem_t* p = d_zgo + b * db + (t0 + t) * dt + ch;
-        store<VEC>(p, dz);
-        store<VEC>(p + s.dim, dg);
-        store<VEC>(p + 2 * s.dim, dout);
-      }
+    __syncwarp();
+    Vec<2> h = exchange<2, kWarps>(sm.ex, round, link, warp, false, carry, status);
+    if (n <= 0) continue;
+    if (!mbar_wait(&sm.full_o[warp][turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_PRODUCER_TIMEOUT);
+    float* at = saved != nullptr && in ? saved + ((long long)b * s.states + t0 / kSaved) * s.dim + ch : nullptr;
+    if (fast) forward_out<true>(nf1, h, at, s.dim, n, bits, z, o, put);
+    else forward_out<false>(nf1, h, at, s.dim, n, bits, z, o, put);
+    if (in && t0 + STEPS >= s.steps) store(state_out + (long long)b * s.dim + ch, h);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(&map_y, sm.tiles[warp][turn][2], ch0, t0, b);
+      bulk_commit_group();
     }
   }
-  if (in && warp == 0 && d_state_in != nullptr) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) d_state_in[(long long)b * s.dim + ch + j] = e_in.v[j];
+  if (lane == 0) bulk_wait_group_all();
+  if (ctas > 1) cluster_sync();     // no CTA leaves while another may still read its links
+}
+
+template <int STEPS>
+struct BwdSmem {
+  alignas(128) elem_t tiles[kWarps][2][4][STEPS][kSlab];
+  alignas(128) elem_t results[kWarps][3][STEPS][kSlab];
+  alignas(128) float states[kWarps][2][kSlab];
+  Exchange<2, kWarps> ex;
+  uint64_t full[kWarps][2];
+};
+
+template <int STEPS>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_dy,
+                          const __grid_constant__ CUtensorMap map_out, const uint8_t* __restrict__ resets,
+                          const float* __restrict__ saved, const float* __restrict__ d_state_out, float* __restrict__ d_state_in,
+                          int* status, const Shape s) {
+  static_assert(STEPS == kSaved, "a chunk starts from a saved state");
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  BwdSmem<STEPS>& sm = *reinterpret_cast<BwdSmem<STEPS>*>(smem_raw);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+  const int b = blockIdx.y, ch0 = blockIdx.x / ctas * kSlab, ch = ch0 + 2 * lane;
+  const bool in = ch < s.dim;
+  if (lane == 0) {
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.full[warp][i], 1);
+    mbar_fence_init();
   }
+  sm.ex.init();
+  __syncwarp();
+  const int state_bytes = min(kSlab, s.dim - ch0) * 4;
+  auto issue = [&](int t0, int buf) {                       // one lane
+    mbar_expect_tx(&sm.full[warp][buf], 4 * STEPS * kSlab * 2 + state_bytes);
+    bulk_load(sm.states[warp][buf], saved + ((long long)b * s.states + t0 / kSaved) * s.dim + ch0, state_bytes, &sm.full[warp][buf]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) tma_load_4d(sm.tiles[warp][buf][k], &map_in, &sm.full[warp][buf], ch0, k, t0, b);
+    tma_load_3d(sm.tiles[warp][buf][3], &map_dy, &sm.full[warp][buf], ch0, t0, b);
+  };
+  Vec<2> carry = Vec<2>::all(0.0f);
+  if (in && d_state_out != nullptr) carry = load<2>(d_state_out + (long long)b * s.dim + ch);
+  const int per_step = ctas * kWarps * STEPS, rounds = (s.steps + per_step - 1) / per_step;
+  int t0 = (rounds - 1) * per_step + (rank * kWarps + warp) * STEPS;
+  if (lane == 0 && t0 < s.steps) issue(t0, 0);
+  uint32_t next_bits = reset_bits(resets, s, b, t0, min(STEPS, s.steps - t0));
+  uint32_t phases = 0;
+  for (int round = 0, stage = 0; round < rounds; ++round, t0 -= per_step, stage ^= 1) {
+    const int n = min(STEPS, s.steps - t0);
+    const uint32_t bits = next_bits;
+    const bool fast = n == STEPS && bits == 0;
+    const Tile tile{&sm.tiles[warp][stage][0][0][2 * lane], STEPS}, result{&sm.results[warp][0][0][2 * lane], STEPS};
+    if (n > 0) {
+      if (!mbar_wait(&sm.full[warp][stage], (phases >> stage) & 1) && lane == 0) atomicExch(status, GEMM_ERR_PRODUCER_TIMEOUT);
+      phases ^= 1u << stage;
+    }
+    if (round + 1 < rounds) {
+      if (lane == 0) issue(t0 - per_step, stage ^ 1);
+      next_bits = reset_bits(resets, s, b, t0 - per_step, min(STEPS, s.steps - t0 + per_step));
+    }
+    auto z = [&](int t) { return tile.get(0, t); };
+    auto g = [&](int t) { return tile.get(1, t); };
+    auto o = [&](int t) { return tile.get(2, t); };
+    auto d = [&](int t) { return tile.get(3, t); };
+    elem2_t dout[STEPS];
+    auto put_z = [&](int t, Vec<2> v) { result.put(0, t, v); };
+    auto put_g = [&](int t, Vec<2> v) { result.put(1, t, v); };
+    auto put_o = [&](int t, Vec<2> v) { dout[t] = ff2e2(v.v.x, v.v.y); };
+    Vec<2> nf1[STEPS], u[STEPS], dh0[STEPS];
+    Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
+    const Vec<2> h = load<2>(&sm.states[warp][stage][2 * lane]);
+    if (fast) backward_in<true>(nf1, u, dh0, link, h, n, bits, z, g, o, d, put_o);
+    else if (n > 0) backward_in<false>(nf1, u, dh0, link, h, n, bits, z, g, o, d, put_o);
+    const Vec<2> e = exchange<2, kWarps>(sm.ex, round, link, kWarps - 1 - warp, true, carry, status);
+    if (n <= 0) continue;
+    if (lane == 0) bulk_wait_group_read<0>();               // the results of the step before have left
+    __syncwarp();
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) *reinterpret_cast<elem2_t*>(result.at + (2 * STEPS + t) * kSlab) = dout[t];
+    if (fast) backward_out<true>(nf1, u, dh0, e, bits, put_z, put_g);
+    else backward_out<false>(nf1, u, dh0, e, bits, put_z, put_g);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) tma_store_4d(&map_out, sm.results[warp][k], ch0, k, t0, b);
+      bulk_commit_group();
+    }
+  }
+  if (in && rank == 0 && warp == 0 && d_state_in != nullptr) store(d_state_in + (long long)b * s.dim + ch, carry);
+  if (lane == 0) bulk_wait_group_all();
+  if (ctas > 1) cluster_sync();
 }
 
 // Two neighbouring channels per lane where they lie on 4-byte boundaries
 bool pairs(const void* p, int dim, long long a, long long b, long long c) {
   return dim % 2 == 0 && ((a | b | c) & 1) == 0 && (reinterpret_cast<uintptr_t>(p) & 3) == 0;
 }
-
-template <int VEC, int WARPS>
-int launch_fwd(const void* zgo, const float* state_in, const uint8_t* resets, void* y, float* state_out, float* saved,
-               const Shape& s, cudaStream_t stream) {
-  const dim3 grid((s.dim + 32 * VEC - 1) / (32 * VEC), s.batch);
-  recurrence_fwd_kernel<VEC, WARPS><<<grid, WARPS * 32, 0, stream>>>((const elem_t*)zgo, state_in, resets, (elem_t*)y, state_out, saved, s);
-  return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+// What a tensor map takes: rows and strides of 16-byte pieces
+bool pieces(const void* p, int dim, long long a, long long b, long long c) {
+  return dim % 8 == 0 && ((a | b | c) & 7) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && a > 0 && b > 0 && c > 0 &&
+         a < (1ll << 38) && b < (1ll << 38) && c < (1ll << 38);
 }
 
-template <int VEC, int WARPS>
-int launch_bwd(const void* zgo, const uint8_t* resets, const float* saved, const void* dy, const float* d_state_out,
-               void* d_zgo, float* d_state_in, const Shape& s, long long db, long long dt, cudaStream_t stream) {
-  const dim3 grid((s.dim + 32 * VEC - 1) / (32 * VEC), s.batch);
-  recurrence_bwd_kernel<VEC, WARPS><<<grid, WARPS * 32, 0, stream>>>((const elem_t*)zgo, resets, saved, (const elem_t*)dy, d_state_out,
-                                                                     (elem_t*)d_zgo, d_state_in, s, db, dt);
-  return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+// (batch, steps, members, dim), or (batch, steps, dim) with members = 0; boxes of `box` steps and kSlab channels
+int encode(CUtensorMap* map, const void* p, const Shape& s, long long sb, long long st, long long sk, int members, int box) {
+  auto enc = fbam_encode_tiled();
+  if (!enc) return GEMM_ERR_DRIVER;
+  fbam_bind_context_to_thread();
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  CUresult r;
+  if (members) {
+    const cuuint64_t dims[4] = {(cuuint64_t)s.dim, (cuuint64_t)members, (cuuint64_t)s.steps, (cuuint64_t)s.batch};
+    const cuuint64_t strides[3] = {(cuuint64_t)sk * 2, (cuuint64_t)st * 2, (cuuint64_t)sb * 2};
+    const cuuint32_t boxes[4] = {kSlab, 1, (cuuint32_t)box, 1};
+    r = enc(map, ELEM_TMAP, 4, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    const cuuint64_t dims[3] = {(cuuint64_t)s.dim, (cuuint64_t)s.steps, (cuuint64_t)s.batch};
+    const cuuint64_t strides[2] = {(cuuint64_t)st * 2, (cuuint64_t)sb * 2};
+    const cuuint32_t boxes[3] = {kSlab, (cuuint32_t)box, 1};
+    r = enc(map, ELEM_TMAP, 3, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  if (r != CUDA_SUCCESS) g_fbam_last_driver_error = (int)r;
+  return r == CUDA_SUCCESS ? 0 : GEMM_ERR_TENSORMAP;
+}
+
+// CTAs of a cluster: as many as the machine holds at once, two per SM, but no more than the sequence has chunks for.  A cluster
+// pays for its links once a walk step, so where there are enough sequences and channels it stays small.  us forward | backward
+// by cluster size, bf16 (batch x steps x channels):
+//   8 x 1024 x 1024    1: 25 | 38     2: 25 | 35     8: 36 | 50
+//   64 x 128 x 1024    1: 25 | 35     2: 25 | 49
+//   1 x 30011 x 2048   1: 488 | 857   2: 303 | 535   4: 156 | 283   8: 126 | 206
+//   16 x 4096 x 512    1: 74 | 126    2: 66 | 105    8: 84 | 129
+// (Sixteen, which a cluster may have on request: 1 x 60000 x 512 191 | 334 against 168 | 295 with eight.)
+int cluster_ctas(const Shape& s, int slabs, int steps) {
+  int ctas = 1;
+  while (ctas < kMaxCtas && ctas * steps < s.steps && 2ll * ctas * slabs * s.batch <= 2 * 148) ctas *= 2;
+  return ctas;
+}
+
+template <typename K, typename... Args>
+int launch(K kernel, int slab, int warps, int steps, int smem, const Shape& s, cudaStream_t stream, Args... args) {
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return GEMM_ERR_LAUNCH;
+  const int slabs = (s.dim + slab - 1) / slab, ctas = warps > 1 ? cluster_ctas(s, slabs, warps * steps) : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(slabs * ctas, s.batch);
+  cfg.blockDim = dim3(warps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {(unsigned)ctas, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }
 
 }  // namespace
 
-// Steps of a chunk: the forward's `saved` has [batch][ceil(steps / this)][dim] fp32 values (null where no backward follows).
-extern "C" int fbam_recurrence_chunk() { return kSteps; }
+// Steps from one saved state to the next: the forward's `saved` has [batch][ceil(steps / this)][dim] fp32 values (null where no
+// backward follows).
+extern "C" int fbam_recurrence_chunk() { return kSaved; }
 
 // zgo: strides zb, zt, zk (sequence, step, member; channels dense); y: yb, yt; resets (bytes, or null): rb, rt.  state_in
 // (batch, dim) fp32 or null for zeros.
 extern "C" int fbam_recurrence_fwd(const void* zgo, long long zb, long long zt, long long zk, const float* state_in,
                                    const uint8_t* resets, long long rb, long long rt, void* y, long long yb, long long yt,
-                                   float* state_out, float* saved, int batch, int steps, int dim, void* stream) {
+                                   float* state_out, float* saved, int batch, int steps, int dim, int* status, void* stream) {
   if (batch <= 0 || steps <= 0 || dim <= 0 || batch > 65535 || steps > 0x3fffffff) return GEMM_ERR_SHAPE;
-  const Shape s{batch, steps, dim, (steps + kSteps - 1) / kSteps, zb, zt, zk, yb, yt, rb, rt};
+  const Shape s{batch, steps, dim, (steps + kSaved - 1) / kSaved, zb, zt, zk, yb, yt, rb, rt};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (steps > kSaved && pieces(zgo, dim, zb, zt, zk) && pieces(y, dim, yb, yt, 8)) {
+    CUtensorMap in, out;
+    int e = encode(&in, zgo, s, zb, zt, zk, 3, kFwdSteps);
+    if (!e) e = encode(&out, y, s, yb, yt, 0, 0, kFwdSteps);
+    if (e) return e;
+    return launch(recurrence_fwd_tma_kernel<kFwdSteps>, kSlab, kWarps, kFwdSteps, (int)sizeof(FwdSmem<kFwdSteps>), s, st, in, out, state_in, resets,
+                  state_out, saved, status, s);
+  }
   const bool two = pairs(zgo, dim, zb, zt, zk) && pairs(y, dim, yb, yt, 0);
-  auto f = s.chunks == 1 ? (two ? launch_fwd<2, 1> : launch_fwd<1, 1>) : (two ? launch_fwd<2, 8> : launch_fwd<1, 8>);
-  return f(zgo, state_in, resets, y, state_out, saved, s, st);
+  auto go = [&](auto kernel, int vec, int warps) {
+    return launch(kernel, 32 * vec, warps, kSaved, 0, s, st, (const elem_t*)zgo, state_in, resets, (elem_t*)y, state_out, saved, status, s);
+  };
+  if (steps > kSaved) return go(recurrence_fwd_kernel<1, 8>, 1, 8);
+  return two ? go(recurrence_fwd_kernel<2, 1>, 2, 1) : go(recurrence_fwd_kernel<1, 1>, 1, 1);
 }
 
 // dy: strides yb, yt; d_zgo: db, dt and dense (3, dim) steps.  d_state_out and d_state_in (batch, dim) fp32 or null.
 extern "C" int fbam_recurrence_bwd(const void* zgo, long long zb, long long zt, long long zk, const uint8_t* resets,
                                    long long rb, long long rt, const float* saved, const void* dy, long long yb, long long yt,
                                    const float* d_state_out, void* d_zgo, long long db, long long dt, float* d_state_in,
-                                   int batch, int steps, int dim, void* stream) {
+                                   int batch, int steps, int dim, int* status, void* stream) {
   if (batch <= 0 || steps <= 0 || dim <= 0 || batch > 65535 || steps > 0x3fffffff) return GEMM_ERR_SHAPE;
-  const Shape s{batch, steps, dim, (steps + kSteps - 1) / kSteps, zb, zt, zk, yb, yt, rb, rt};
+  const Shape s{batch, steps, dim, (steps + kSaved - 1) / kSaved, zb, zt, zk, yb, yt, rb, rt};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (steps > kSaved && pieces(zgo, dim, zb, zt, zk) && pieces(dy, dim, yb, yt, 8) && pieces(d_zgo, dim, db, dt, 8) &&
+      (reinterpret_cast<uintptr_t>(saved) & 15) == 0) {
+    CUtensorMap in, d, out;
+    int e = encode(&in, zgo, s, zb, zt, zk, 3, kSaved);
+    if (!e) e = encode(&d, dy, s, yb, yt, 0, 0, kSaved);
+    if (!e) e = encode(&out, d_zgo, s, db, dt, dim, 3, kSaved);
+    if (e) return e;
+    return launch(recurrence_bwd_tma_kernel<kSaved>, kSlab, kWarps, kSaved, (int)sizeof(BwdSmem<kSaved>), s, st, in, d, out, resets, saved,
+                  d_state_out, d_state_in, status, s);
+  }
   const bool two = pairs(zgo, dim, zb, zt, zk) && pairs(dy, dim, yb, yt, 0) && pairs(d_zgo, dim, db, dt, 0);
-  auto f = s.chunks == 1 ? (two ? launch_bwd<2, 1> : launch_bwd<1, 1>) : (two ? launch_bwd<2, 8> : launch_bwd<1, 8>);
-  return f(zgo, resets, saved, dy, d_state_out, d_zgo, d_state_in, s, db, dt, st);
+  auto go = [&](auto kernel, int vec, int warps) {
+    return launch(kernel, 32 * vec, warps, kSaved, 0, s, st, (const elem_t*)zgo, resets, saved, (const elem_t*)dy, d_state_out,
+                  (elem_t*)d_zgo, d_state_in, status, s, db, dt);
+  };
+  if (steps > kSaved) return go(recurrence_bwd_kernel<1, 8>, 1, 8);
+  return two ? go(recurrence_bwd_kernel<2, 1>, 2, 1) : go(recurrence_bwd_kernel<1, 1>, 1, 1);
 }

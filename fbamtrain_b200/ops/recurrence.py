@@ -3,7 +3,7 @@ steps, so that a sequence is a scan instead of a chain.
 
 Projections of a whole sequence come as one tensor ``(B, T, 3, D)`` (candidates, gates, output gates), as
 ``attention_qkv`` takes its projections, and its gradient is one tensor too.  The forward keeps the fp32 state in front of
-every chunk of steps, a sixteenth of the sequence, and nothing else; the backward rebuilds the states in between.
+every eighth step and nothing else; the backward rebuilds the states in between.
 """
 from __future__ import annotations
 
@@ -44,7 +44,8 @@ class _GatedRecurrence(torch.autograd.Function):
             saved = torch.empty(b, (t + chunk - 1) // chunk, d, dtype=torch.float32, device=zgo.device)
         rs = (C.c_longlong(0), C.c_longlong(0)) if resets is None else _strides(resets, 0, 1)
         nv.check(lib.fbam_recurrence_fwd(nv.ptr(zgo), *_strides(zgo, 0, 1, 2), nv.ptr(state), nv.ptr(resets), *rs, nv.ptr(y),
-                                         *_strides(y, 0, 1), nv.ptr(out), nv.ptr(saved), b, t, d, nv.stream_ptr()),
+                                         *_strides(y, 0, 1), nv.ptr(out), nv.ptr(saved), b, t, d,
+                                         nv.ptr(nv.status_word(zgo.device)), nv.stream_ptr()),
                  "fbam_recurrence_fwd")
         ctx.save_for_backward(zgo, resets, saved)
         return y, out
@@ -64,7 +65,8 @@ class _GatedRecurrence(torch.autograd.Function):
         rs = (C.c_longlong(0), C.c_longlong(0)) if resets is None else _strides(resets, 0, 1)
         nv.check(nv.lib(zgo).fbam_recurrence_bwd(nv.ptr(zgo), *_strides(zgo, 0, 1, 2), nv.ptr(resets), *rs, nv.ptr(saved),
                                                  nv.ptr(dy), *_strides(dy, 0, 1), nv.ptr(d_out), nv.ptr(d_zgo),
-                                                 *_strides(d_zgo, 0, 1), nv.ptr(d_state), b, t, d, nv.stream_ptr()),
+                                                 *_strides(d_zgo, 0, 1), nv.ptr(d_state), b, t, d,
+                                                 nv.ptr(nv.status_word(zgo.device)), nv.stream_ptr()),
                  "fbam_recurrence_bwd")
         return d_zgo, d_state, None, None
 
