@@ -11,50 +11,55 @@ import torch
 
 from . import native as nv
 
+F32 = torch.float32
+
+
+def _forward(ids, flat, table, scale, out_dtype, elem):
+    vocab, dim = table.shape
+    out = torch.empty((*ids.shape, dim), dtype=out_dtype, device=table.device)
+    n = flat.numel()
+    if n:
+        nv.check(nv.lib(elem).fbam_embed_fwd(flat.data_ptr(), flat.dtype == torch.int64, table.data_ptr(), table.stride(0),
+                                             table.dtype == F32, out.data_ptr(), out_dtype == F32, n, vocab, dim, scale,
+                                             nv.stream()), "fbam_embed_fwd")
+    return out
+
 
 class _EmbedTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale, out_dtype):
-        vocab, dim = table.shape
-        flat = ids.reshape(-1)
-        if not flat.is_contiguous():
-            flat = flat.contiguous()
-        if table.stride(1) != 1:
-            table = table.contiguous()
-        n = flat.numel()
-        out = torch.empty(*ids.shape, dim, dtype=out_dtype, device=table.device)
-        elem = table.dtype if table.dtype != torch.float32 else out_dtype
-        if n:
-            nv.check(nv.lib(elem).fbam_embed_fwd(nv.ptr(flat), int(flat.dtype == torch.int64), nv.ptr(table),
-                                                 C.c_longlong(table.stride(0)), int(table.dtype == torch.float32), nv.ptr(out),
-                                                 int(out_dtype == torch.float32), C.c_longlong(n), vocab, dim, C.c_float(scale),
-                                                 nv.stream_ptr()), "fbam_embed_fwd")
+    def forward(ctx, ids, flat, table, scale, out_dtype, elem):
         ctx.save_for_backward(flat)
-        ctx.meta = (vocab, dim, table.dtype, elem, scale)
-        return out
+        ctx.meta = (*table.shape, table.dtype, elem, scale)
+        return _forward(ids, flat, table, scale, out_dtype, elem)
 
     @staticmethod
     def backward(ctx, d_out):
         (flat,) = ctx.saved_tensors
         vocab, dim, dtype, elem, scale = ctx.meta
-        n = flat.numel()
+        n, dev = flat.numel(), d_out.device
         if n == 0:
-            return None, torch.zeros(vocab, dim, dtype=dtype, device=d_out.device), None, None
+            return None, None, torch.zeros(vocab, dim, dtype=dtype, device=dev), None, None, None
         d_out = d_out.contiguous()
-        d_table = torch.empty(vocab, dim, dtype=dtype, device=d_out.device)
+        d_table = torch.empty(vocab, dim, dtype=dtype, device=dev)
         lib = nv.lib(elem)
         words, floats = C.c_longlong(), C.c_longlong()
-        lib.fbam_embed_bwd_workspace(C.c_longlong(n), dim, C.byref(words), C.byref(floats))
-        work = torch.empty(words.value, dtype=torch.int32, device=d_out.device)
-        partial = torch.empty(floats.value, dtype=torch.float32, device=d_out.device)
-        nv.check(lib.fbam_embed_bwd(nv.ptr(flat), int(flat.dtype == torch.int64), nv.ptr(d_out),
-                                    int(d_out.dtype == torch.float32), nv.ptr(d_table), int(dtype == torch.float32),
-                                    C.c_longlong(n), vocab, dim, C.c_float(scale), nv.ptr(work), nv.ptr(partial),
-                                    nv.stream_ptr()), "fbam_embed_bwd")
-        return None, d_table, None, None
+        lib.fbam_embed_bwd_workspace(n, dim, C.byref(words), C.byref(floats))
+        work = torch.empty(words.value, dtype=torch.int32, device=dev)
+        partial = torch.empty(floats.value, dtype=F32, device=dev)
+        nv.check(lib.fbam_embed_bwd(flat.data_ptr(), flat.dtype == torch.int64, d_out.data_ptr(), d_out.dtype == F32,
+                                    d_table.data_ptr(), dtype == F32, n, vocab, dim, scale, work.data_ptr(),
+                                    partial.data_ptr(), nv.stream()), "fbam_embed_bwd")
+        return None, None, d_table, None, None, None
 
 
 def embed_tokens(ids, table, scale, out_dtype):
-    if not ids.is_cuda or ids.device != table.device:
+    if ids.device != table.device:
         raise ValueError(f"ids are on {ids.device}, the table on {table.device}")
-    return _EmbedTokens.apply(ids, table, float(scale), out_dtype)
+    flat = ids.reshape(-1)
+    if not flat.is_contiguous():
+        flat = flat.contiguous()
+    if table.stride(1) != 1:
+        table = table.contiguous()
+    elem = table.dtype if table.dtype != F32 else out_dtype
+    run = _EmbedTokens.apply if table.requires_grad and torch.is_grad_enabled() else _forward
+    return run(ids, flat, table, float(scale), out_dtype, elem)

@@ -2,32 +2,39 @@
 (``csrc/logprobs.cu``)."""
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import native as nv
+
+F32 = torch.float32
+
+
+def _forward(logits, targets, top, inv_t, keep):
+    """``(logprob, entropy, top logprobs, top ids, stats)``; ``stats`` with ``keep``: what the backward needs."""
+    rows, vocab = logits.shape
+    dev = logits.device
+    logprob = None if targets is None else torch.empty(rows, dtype=F32, device=dev)
+    entropy = torch.empty(rows, dtype=F32, device=dev)
+    stats = torch.empty((rows, 2), dtype=F32, device=dev) if keep else None
+    top_lp = top_ids = None
+    if top:
+        top_lp = torch.empty((rows, top), dtype=F32, device=dev)
+        top_ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    if rows:
+        nv.check(nv.lib(logits).fbam_logprobs_fwd(logits.data_ptr(), logits.dtype == F32, logits.stride(0), nv.addr(targets),
+                                                  nv.addr(logprob), entropy.data_ptr(), nv.addr(stats), nv.addr(top_lp),
+                                                  nv.addr(top_ids), rows, vocab, top, inv_t, nv.stream()),
+                 "fbam_logprobs_fwd")
+    return logprob, entropy, top_lp, top_ids, stats
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, inv_t):
-        rows, vocab = logits.shape
-        dev = logits.device
         ctx.set_materialize_grads(False)
-        logprob = None if targets is None else torch.empty(rows, dtype=torch.float32, device=dev)
-        entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-        stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
-        top_lp = top_ids = None
+        logprob, entropy, top_lp, top_ids, stats = _forward(logits, targets, top, inv_t, True)
         if top:
-            top_lp = torch.empty(rows, top, dtype=torch.float32, device=dev)
-            top_ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
             ctx.mark_non_differentiable(top_lp, top_ids)
-        if rows:
-            nv.check(nv.lib(logits).fbam_logprobs_fwd(
-                nv.ptr(logits), int(logits.dtype == torch.float32), C.c_longlong(logits.stride(0)), nv.ptr(targets),
-                nv.ptr(logprob), nv.ptr(entropy), nv.ptr(stats), nv.ptr(top_lp), nv.ptr(top_ids), C.c_longlong(rows), vocab,
-                top, C.c_float(inv_t), nv.stream_ptr()), "fbam_logprobs_fwd")
         ctx.save_for_backward(logits, targets, stats, entropy)
         ctx.inv_t = inv_t
         return logprob, entropy, top_lp, top_ids
@@ -38,26 +45,33 @@ class _TokenLogprobs(torch.autograd.Function):
         rows, vocab = logits.shape
         d_logprob = None if d_logprob is None else d_logprob.contiguous()
         d_entropy = None if d_entropy is None else d_entropy.contiguous()
-        # rows of 16 bytes each, whatever the vocabulary
+        # rows of whole 16-byte pieces, whatever the vocabulary
         per = 16 // logits.element_size()
-        d = torch.empty(rows, (vocab + per - 1) // per * per, dtype=logits.dtype, device=logits.device)[:, :vocab]
+        width = (vocab + per - 1) // per * per
+        d = torch.empty((rows, width), dtype=logits.dtype, device=logits.device)
         if rows:
-            nv.check(nv.lib(logits).fbam_logprobs_bwd(
-                nv.ptr(logits), int(logits.dtype == torch.float32), C.c_longlong(logits.stride(0)), nv.ptr(targets),
-                nv.ptr(stats), nv.ptr(entropy), nv.ptr(d_logprob), nv.ptr(d_entropy), nv.ptr(d), C.c_longlong(d.stride(0)),
-                C.c_longlong(rows), vocab, C.c_float(ctx.inv_t), nv.stream_ptr()), "fbam_logprobs_bwd")
-        return d, None, None, None
+            nv.check(nv.lib(logits).fbam_logprobs_bwd(logits.data_ptr(), logits.dtype == F32, logits.stride(0), nv.addr(targets),
+                                                      stats.data_ptr(), entropy.data_ptr(), nv.addr(d_logprob),
+                                                      nv.addr(d_entropy), d.data_ptr(), width, rows, vocab, ctx.inv_t,
+                                                      nv.stream()), "fbam_logprobs_bwd")
+        return d if width == vocab else d[:, :vocab], None, None, None
 
 
 def token_logprobs(logits, targets, top, temperature):
     if targets is not None and targets.device != logits.device:
         raise ValueError(f"targets are on {targets.device}, the logits on {logits.device}")
     shape, vocab = logits.shape[:-1], logits.shape[-1]
-    flat = logits.reshape(-1, vocab)
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     if flat.stride(1) != 1:
         flat = flat.contiguous()
     if targets is not None:
         targets = targets.reshape(-1).long().contiguous()
-    logprob, entropy, top_lp, top_ids = _TokenLogprobs.apply(flat, targets, top, 1.0 / temperature)
+    if flat.requires_grad and torch.is_grad_enabled():
+        out = _TokenLogprobs.apply(flat, targets, top, 1.0 / temperature)
+    else:
+        out = _forward(flat, targets, top, 1.0 / temperature, False)[:4]
+    if logits.dim() == 2:
+        return out
+    logprob, entropy, top_lp, top_ids = out
     return (None if logprob is None else logprob.view(shape), entropy.view(shape),
             None if top_lp is None else top_lp.view(*shape, top), None if top_ids is None else top_ids.view(*shape, top))

@@ -99,6 +99,20 @@ def _check_struct_layout(library: C.CDLL, path: str) -> None:
                            f"{list(got)} vs {mine}); run `python -m fbamtrain_b200.build`")
 
 
+_P, _I, _L, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
+# Argument types of the token operators' entry points: with them ctypes takes plain integers and addresses, which is a third of
+# what an object for every argument costs, and these calls are short.
+_ARGTYPES = {
+    "fbam_embed_fwd": (_P, _I, _P, _L, _I, _P, _I, _L, _I, _I, _F, _P),
+    "fbam_embed_bwd": (_P, _I, _P, _I, _P, _I, _L, _I, _I, _F, _P, _P, _P),
+    "fbam_embed_bwd_workspace": (_L, _I, _P, _P),
+    "fbam_recurrence_fwd": (_P, _L, _L, _L, _P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _P, _P),
+    "fbam_recurrence_bwd": (_P, _L, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _P, _I, _I, _I, _P, _P),
+    "fbam_logprobs_fwd": (_P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _I, _I, _F, _P),
+    "fbam_logprobs_bwd": (_P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _L, _I, _F, _P),
+}
+
+
 def _load(path: str) -> C.CDLL:
     if not os.path.exists(path):
         raise RuntimeError(f"native kernel library missing: {path} (run `python -m fbamtrain_b200.build`)")
@@ -107,6 +121,8 @@ def _load(path: str) -> C.CDLL:
     for name in ("fbam_gemm", "fbam_conv", "fbam_conv_wgrad", "fbam_gemm2", "fbam_conv2",
                  "fbam_lstm_persistent_max_hidden", "fbam_lstm_fwd_ex", "fbam_lstm_bwd_ex", "fbam_elem_is_fp16"):
         getattr(library, name).restype = C.c_int
+    for name, types in _ARGTYPES.items():
+        getattr(library, name).argtypes = types
     return library
 
 
@@ -165,6 +181,16 @@ def stream_ptr() -> C.c_void_p:
     """The current stream of the current device (without the stream object that ``torch.cuda.current_stream`` builds,
     which is several times the cost of the launch that follows)."""
     return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+
+
+def stream() -> int:
+    """:func:`stream_ptr` for an entry point with argument types."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def addr(t: Optional[torch.Tensor]) -> int:
+    """:func:`ptr` for an entry point with argument types."""
+    return 0 if t is None else t.data_ptr()
 
 
 def ptr(t: Optional[torch.Tensor]) -> C.c_void_p:

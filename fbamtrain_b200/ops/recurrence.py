@@ -7,46 +7,46 @@ every eighth step and nothing else; the backward rebuilds the states in between.
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import native as nv
+
+F32 = torch.float32
 
 
 def _ordered_like(x: torch.Tensor, *inner: int) -> torch.Tensor:
     """An empty ``(B, T, *inner)`` tensor that is time-major in memory where ``x`` is."""
     b, t = x.shape[:2]
-    if x.stride(0) < x.stride(1) and b > 1:
-        return torch.empty(t, b, *inner, dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty(b, t, *inner, dtype=x.dtype, device=x.device)
+    if b > 1 and x.stride(0) < x.stride(1):
+        return torch.empty((t, b, *inner), dtype=x.dtype, device=x.device).transpose(0, 1)
+    return torch.empty((b, t, *inner), dtype=x.dtype, device=x.device)
 
 
-def _strides(t: torch.Tensor, *dims: int):
-    return tuple(C.c_longlong(t.stride(d)) for d in dims)
+def _forward(zgo, state, resets, keep):
+    """``(y, state, saved)``; ``saved`` with ``keep``: what the backward needs."""
+    b, t, _, d = zgo.shape
+    dev = zgo.device
+    y = _ordered_like(zgo, d)
+    out = torch.empty((b, d), dtype=F32, device=dev)
+    lib = nv.lib(zgo)
+    saved = None
+    if keep:
+        chunk = lib.fbam_recurrence_chunk()
+        saved = torch.empty((b, (t + chunk - 1) // chunk, d), dtype=F32, device=dev)
+    zb, zt, zk, _ = zgo.stride()
+    yb, yt, _ = y.stride()
+    rb, rt = (0, 0) if resets is None else resets.stride()
+    nv.check(lib.fbam_recurrence_fwd(zgo.data_ptr(), zb, zt, zk, nv.addr(state), nv.addr(resets), rb, rt, y.data_ptr(), yb, yt,
+                                     out.data_ptr(), nv.addr(saved), b, t, d, nv.status_word(dev).data_ptr(), nv.stream()),
+             "fbam_recurrence_fwd")
+    return y, out, saved
 
 
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, zgo, state, resets, keep):
-        b, t, _, d = zgo.shape
-        if zgo.stride(3) != 1:
-            zgo = zgo.contiguous()
-        if state is not None:
-            state = state.contiguous()
+    def forward(ctx, zgo, state, resets):
         ctx.set_materialize_grads(False)
-        y = _ordered_like(zgo, d)
-        out = torch.empty(b, d, dtype=torch.float32, device=zgo.device)
-        lib = nv.lib(zgo)
-        saved = None
-        if keep:
-            chunk = lib.fbam_recurrence_chunk()
-            saved = torch.empty(b, (t + chunk - 1) // chunk, d, dtype=torch.float32, device=zgo.device)
-        rs = (C.c_longlong(0), C.c_longlong(0)) if resets is None else _strides(resets, 0, 1)
-        nv.check(lib.fbam_recurrence_fwd(nv.ptr(zgo), *_strides(zgo, 0, 1, 2), nv.ptr(state), nv.ptr(resets), *rs, nv.ptr(y),
-                                         *_strides(y, 0, 1), nv.ptr(out), nv.ptr(saved), b, t, d,
-                                         nv.ptr(nv.status_word(zgo.device)), nv.stream_ptr()),
-                 "fbam_recurrence_fwd")
+        y, out, saved = _forward(zgo, state, resets, True)
         ctx.save_for_backward(zgo, resets, saved)
         return y, out
 
@@ -54,26 +54,34 @@ class _GatedRecurrence(torch.autograd.Function):
     def backward(ctx, dy, d_out):
         zgo, resets, saved = ctx.saved_tensors
         b, t, _, d = zgo.shape
+        dev = zgo.device
         if dy is None:
-            dy = torch.zeros(b, t, d, dtype=zgo.dtype, device=zgo.device)
+            dy = torch.zeros(b, t, d, dtype=zgo.dtype, device=dev)
         elif dy.stride(2) != 1:
             dy = dy.contiguous()
         if d_out is not None:
             d_out = d_out.contiguous()
         d_zgo = _ordered_like(zgo, 3, d)
-        d_state = torch.empty(b, d, dtype=torch.float32, device=zgo.device) if ctx.needs_input_grad[1] else None
-        rs = (C.c_longlong(0), C.c_longlong(0)) if resets is None else _strides(resets, 0, 1)
-        nv.check(nv.lib(zgo).fbam_recurrence_bwd(nv.ptr(zgo), *_strides(zgo, 0, 1, 2), nv.ptr(resets), *rs, nv.ptr(saved),
-                                                 nv.ptr(dy), *_strides(dy, 0, 1), nv.ptr(d_out), nv.ptr(d_zgo),
-                                                 *_strides(d_zgo, 0, 1), nv.ptr(d_state), b, t, d,
-                                                 nv.ptr(nv.status_word(zgo.device)), nv.stream_ptr()),
+        d_state = torch.empty((b, d), dtype=F32, device=dev) if ctx.needs_input_grad[1] else None
+        zb, zt, zk, _ = zgo.stride()
+        yb, yt, _ = dy.stride()
+        db, dt, _, _ = d_zgo.stride()
+        rb, rt = (0, 0) if resets is None else resets.stride()
+        nv.check(nv.lib(zgo).fbam_recurrence_bwd(zgo.data_ptr(), zb, zt, zk, nv.addr(resets), rb, rt, saved.data_ptr(),
+                                                 dy.data_ptr(), yb, yt, nv.addr(d_out), d_zgo.data_ptr(), db, dt,
+                                                 nv.addr(d_state), b, t, d, nv.status_word(dev).data_ptr(), nv.stream()),
                  "fbam_recurrence_bwd")
-        return d_zgo, d_state, None, None
+        return d_zgo, d_state, None
 
 
 def gated_recurrence(zgo, state, resets):
     for name, x in (("state", state), ("resets", resets)):
         if x is not None and x.device != zgo.device:
             raise ValueError(f"{name} is on {x.device}, the sequence on {zgo.device}")
-    keep = torch.is_grad_enabled() and (zgo.requires_grad or (state is not None and state.requires_grad))
-    return _GatedRecurrence.apply(zgo, state, resets, keep)
+    if zgo.stride(3) != 1:
+        zgo = zgo.contiguous()
+    if state is not None:
+        state = state.contiguous()
+    if torch.is_grad_enabled() and (zgo.requires_grad or (state is not None and state.requires_grad)):
+        return _GatedRecurrence.apply(zgo, state, resets)
+    return _forward(zgo, state, resets, False)[:2]

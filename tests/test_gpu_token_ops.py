@@ -522,3 +522,37 @@ def test_operators_are_captured_in_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(want, got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("vocab", [300, 4096, 70001, 262144])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_logprobs_more_equal_values_than_candidates(vocab, dtype):
+    """A few allowed tokens among masked ones, plateaus, and large values that all lie where one thread reads them."""
+    logits = torch.full((5, vocab), -INF, dtype=dtype, device="cuda")
+    logits[0, [vocab - 1, 3, vocab // 2]] = torch.tensor([1.0, 2.0, 1.0], device="cuda").to(dtype)
+    logits[1] = 0.5
+    logits[1, vocab // 3::7] = 0.75
+    logits[2, -40:] = -3.0
+    logits[3] = torch.arange(vocab, device="cuda") % 3
+    logits[4] = torch.randn(vocab, device="cuda").to(dtype)
+    logits[4].view(-1)[::128] += 10.0                         # stride of a few threads' vectors
+    for top in (1, 5, 32):
+        r = ops.token_logprobs(logits, None, top)
+        ids = oracle.alternatives(logits, top)
+        assert torch.equal(r.top_ids, ids)
+        _, _, logp, _ = oracle.logprobs(logits, torch.zeros(5, dtype=torch.int64, device="cuda"), 1.0)
+        oracle.within(r.top_logprobs, logp.gather(1, ids), F32, 1e-5)
+
+
+def test_logprobs_values_of_one_thread_only():
+    """More values above the k-th best thread's best than the list of candidates has room for."""
+    vocab = 262144
+    logits = torch.randn(1, vocab, device="cuda")
+    for dtype, vec in ((BF, 8), (F32, 4)):
+        x = logits.to(dtype)
+        for threads in (32, 128, 512, 4096):                  # of a row, in the launches that there are
+            y = x.clone().view(1, -1)
+            wide = y[:, : vocab // (threads * vec) * threads * vec].view(1, -1, threads, vec)
+            wide[:, :, 0] += 20.0
+            r = ops.token_logprobs(y, None, 32)
+            assert torch.equal(r.top_ids, oracle.alternatives(y, 32))
