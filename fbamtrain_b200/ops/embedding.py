@@ -43,8 +43,8 @@ class _EmbedTokens(torch.autograd.Function):
         d_table = torch.empty(vocab, dim, dtype=dtype, device=dev)
         lib = nv.lib(elem)
         words, floats = C.c_longlong(), C.c_longlong()
-        lib.fbam_embed_bwd_workspace(n, dim, C.byref(words), C.byref(floats))
-        work = torch.empty(words.value, dtype=torch.int32, device=dev)
+        lib.fbam_embed_bwd_workspace(n, vocab, dim, C.byref(words), C.byref(floats))
+        work = torch.empty(words.value, dtype=torch.int64, device=dev)
         partial = torch.empty(floats.value, dtype=F32, device=dev)
         nv.check(lib.fbam_embed_bwd(flat.data_ptr(), flat.dtype == torch.int64, d_out.data_ptr(), d_out.dtype == F32,
                                     d_table.data_ptr(), dtype == F32, n, vocab, dim, scale, work.data_ptr(),
