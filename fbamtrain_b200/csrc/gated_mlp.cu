@@ -1,54 +1,506 @@
-// Gated feed-forward block: h = v * act(g) with (v, g) = x W_inᵀ + b_in, value rows first, and its gradient
-//   dv = dh act(g)     dg = dh v act'(g).
+// Gated feed-forward block: the two projections, the activation and the product in one kernel,
+//   (v, g) = x W_inᵀ + b_in     h = v act(g)          W_in (2 F, D): value rows first, gate rows behind them
+// and its backward, the product of the output gradient with W_out and the derivative of the gating in one kernel,
+//   dh = dy W_out     dv = dh act(g)     dg = dh v act'(g).
+// The other products of the block are plain ones.
+//
+// Forward: the B tile of a CTA is the value rows and the gate rows of the same hidden columns, so a lane that reads an
+// accumulator row back finds both factors of its results there.  On a CTA pair (one 256 x 256 tile, tcgen05 cta_group::2) the
+// leader's half of B is the value rows and its peer's the gate rows; a single CTA loads both.  For a backward v and g are kept in
+// fp32: 16-bit ones would add as much error to dv and dg as the rounding of those does, and the extra bytes leave while the
+// tensor cores work.
+//
+// Backward: v and g come back through shared memory by TMA (a lane's own 128-byte rows through the load unit would take 32
+// look-ups per instruction), one chunk of 32 columns ahead in the epilogue warp that needs them.
+//
+// Epilogue values are fp32; h, dv and dg are rounded once.  What leaves goes through shared memory and TMA tiled stores, which
+// also clip rows and columns behind the end.
 #include <cuda_runtime.h>
+#include <stdlib.h>
 #include <stdint.h>
 
 #include "elem16.cuh"
 #include "gelu_math.cuh"
+#include "gemm_epilogue.cuh"
 #include "gemm_tcgen05.h"
+#include "tc05.cuh"
+#include "tc05_pair.cuh"
+#include "tensor_map.h"
+
+extern int g_fbam_reserved_sms;        // defined in gemm_tcgen05.cu
+extern int g_fbam_last_driver_error;   // defined in gemm_tcgen05.cu
 
 namespace {
 
+using namespace tc05;
+
 enum { GATE_GELU = 0, GATE_SILU = 1 };
+enum { FORWARD = 0, FORWARD_KEEP = 1, BACKWARD = 2 };
+
+constexpr int BM = 128, BK = 64, UMMA_K = 16;     // rows per CTA
+constexpr int kEpiWarps = 8, kThreads = 32 * (2 + kEpiWarps);
 
 // act(g) and act'(g) of two values
-__device__ __forceinline__ void gate2(float2 g, int act, float2& a, float2& da) {
+__device__ __forceinline__ float2 act2(float2 g, int act) {
+  if (act == GATE_GELU) return gelu_math::gelu2(g);
+  const float2 e = __fmul2_rn(g, gelu_math::f2(-1.4426950408889634f));
+  const float2 d = __fadd2_rn(make_float2(gelu_math::ex2_approx(e.x), gelu_math::ex2_approx(e.y)), gelu_math::f2(1.0f));
+  return __fmul2_rn(g, make_float2(gelu_math::rcp_approx(d.x), gelu_math::rcp_approx(d.y)));
+}
+__device__ __forceinline__ void act_and_grad2(float2 g, int act, float2& a, float2& da) {
   if (act == GATE_GELU) {
-    a = gelu_math::gelu2(g);
-    da = gelu_math::gelu_grad2(g);
+    float2 e;
+    const float2 er = gelu_math::erf_core2(g, e);
+    const float2 cdf = __ffma2_rn(er, gelu_math::f2(0.5f), gelu_math::f2(0.5f));
+    a = __fmul2_rn(g, cdf);
+    da = __ffma2_rn(__fmul2_rn(g, gelu_math::f2(0.3989422804014327f)), e, cdf);
   } else {
-    const float sx = gelu_math::rcp_approx(1.0f + gelu_math::ex2_approx(-1.4426950408889634f * g.x));
-    const float sy = gelu_math::rcp_approx(1.0f + gelu_math::ex2_approx(-1.4426950408889634f * g.y));
-    a = make_float2(g.x * sx, g.y * sy);
-    da = make_float2(sx * fmaf(g.x, 1.0f - sx, 1.0f), sy * fmaf(g.y, 1.0f - sy, 1.0f));
+    const float2 x = __fmul2_rn(g, gelu_math::f2(-1.4426950408889634f));
+    const float2 d = __fadd2_rn(make_float2(gelu_math::ex2_approx(x.x), gelu_math::ex2_approx(x.y)), gelu_math::f2(1.0f));
+    const float2 s = make_float2(gelu_math::rcp_approx(d.x), gelu_math::rcp_approx(d.y));
+    a = __fmul2_rn(g, s);
+    // s + a (1 - s)
+    da = __ffma2_rn(__fmul2_rn(a, gelu_math::f2(-1.0f)), s, __fadd2_rn(s, a));
   }
 }
 
-// vg (rows, 2 inner) fp32; h (rows, inner); with dh (rows, inner) fp32: d_vg (rows, 2 inner) instead.  inner % 8 == 0.
-__global__ void gated_act_kernel(const float* __restrict__ vg, const float* __restrict__ dh, elem_t* __restrict__ out, long long n,
-                                 int inner, int act) {
-  for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 2; i < n; i += (long long)gridDim.x * blockDim.x * 2) {
-    const long long r = i / inner, c = i % inner;
-    const float2 v = *reinterpret_cast<const float2*>(vg + r * 2 * inner + c);
-    const float2 g = *reinterpret_cast<const float2*>(vg + r * 2 * inner + inner + c);
-    float2 a, da;
-    gate2(g, act, a, da);
-    if (dh == nullptr) {
-      *reinterpret_cast<elem2_t*>(out + i) = ff2e2(v.x * a.x, v.y * a.y);
+struct Params {
+  const elem_t* bias;       // [2 inner], or null
+  int* status;
+  int rows, inner, depth;   // depth: the products' K
+  int act;
+};
+
+// BN: columns of the accumulator.  Forward: BN / 2 hidden columns, values then gates; backward: BN hidden columns.
+template <int BN, bool PAIR, int MODE>
+struct Smem {
+  static constexpr int kABytes = BM * BK * 2;
+  static constexpr int kBBytes = (PAIR ? BN / 2 : BN) * BK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  // per epilogue warp, chunks of 32 rows x 32 columns: h twice | v, g in fp32 and h | v, g in fp32 and dv, dg
+  static constexpr int kWarpStage = MODE == FORWARD ? 4096 : MODE == FORWARD_KEEP ? 10240 : 12288;
+  static constexpr int kFixed = kEpiWarps * kWarpStage + 512 + 1024;
+  static constexpr int kStages = (227 * 1024 - kFixed) / kStageBytes > 6 ? 6 : (227 * 1024 - kFixed) / kStageBytes;
+  static constexpr int kTotal = kStages * kStageBytes + kFixed;
+  static_assert(kStages >= 3, "");
+};
+
+// 32 fp32 values of this lane's row in the layout of CU_TENSOR_MAP_SWIZZLE_128B; the buffer is 1024-byte aligned.
+__device__ __forceinline__ void put_row128(uint8_t* buffer, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  float4* row = reinterpret_cast<float4*>(buffer + lane * 128);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) row[j ^ (lane & 7)] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+__device__ __forceinline__ void get_row128(const uint8_t* buffer, float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  const float4* row = reinterpret_cast<const float4*>(buffer + lane * 128);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 t = row[j ^ (lane & 7)];
+    v[4 * j] = t.x; v[4 * j + 1] = t.y; v[4 * j + 2] = t.z; v[4 * j + 3] = t.w;
+  }
+}
+
+// v += bias[n0 .. n0 + 32), of `left` columns that there are; the same addresses in all lanes
+__device__ __forceinline__ void add_bias(float (&v)[32], const elem_t* bias, int left) {
+  if (left >= 32 && (reinterpret_cast<uintptr_t>(bias) & 15) == 0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(bias) + q);
+      const elem2_t* h = reinterpret_cast<const elem2_t*>(&raw);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = e22ff(h[e]);
+        v[8 * q + 2 * e] += f.x;
+        v[8 * q + 2 * e + 1] += f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) v[j] += e2f(bias[j]);
+  }
+}
+
+// Forward: map_0 h, map_1 v, map_2 g (stores).  Backward: map_0 v, map_1 g (loads), map_2 dv, map_3 dg (stores).
+template <int BN, bool PAIR, int MODE>
+__device__ __forceinline__ void
+gated_body(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_0, const CUtensorMap& map_1,
+           const CUtensorMap& map_2, const CUtensorMap& map_3, const Params& p) {
+  using L = Smem<BN, PAIR, MODE>;
+  constexpr bool kBack = MODE == BACKWARD;
+  constexpr int kCols = kBack ? BN : BN / 2;           // hidden columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi_stage = smem + L::kStages * L::kStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(epi_stage + kEpiWarps * L::kWarpStage);
+  uint64_t* empty_bar = full_bar + L::kStages;
+  uint64_t* tmem_full = empty_bar + L::kStages;
+  uint64_t* tmem_empty = tmem_full + 2;
+  uint64_t* side_bar = tmem_empty + 2;                 // one for each epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(side_bar + kEpiWarps);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;  // 0 = leader
+  const int first_tile = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
+  constexpr int kTileRows = PAIR ? 2 * BM : BM;
+  const int tiles_m = (p.rows + kTileRows - 1) / kTileRows, tiles_n = (p.inner + kCols - 1) / kCols;
+  const int num_tiles = tiles_m * tiles_n, k_blocks = (p.depth + BK - 1) / BK;
+  constexpr uint32_t kTmemCols = 2 * BN;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_a);
+    prefetch_tensormap(&map_b);
+    for (int s = 0; s < L::kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tmem_full[a], 1);
+      mbar_init(&tmem_empty[a], (PAIR ? 2 : 1) * kEpiWarps);
+    }
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(&side_bar[w], 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc2(tmem_slot, kTmemCols);
+      tmem_relinquish2();
     } else {
-      const float2 d = *reinterpret_cast<const float2*>(dh + i);
-      *reinterpret_cast<elem2_t*>(out + r * 2 * inner + c) = ff2e2(d.x * a.x, d.y * a.y);
-      *reinterpret_cast<elem2_t*>(out + r * 2 * inner + inner + c) = ff2e2(d.x * v.x * da.x, d.y * v.y * da.y);
+      tmem_alloc(tmem_slot, kTmemCols);
+      tmem_relinquish();
     }
   }
+  fence_before_sync();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();
+  fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += stride) {
+        const int row0 = (tile / tiles_n) * kTileRows + rank * BM, n0 = (tile % tiles_n) * kCols;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1)) { ok = false; break; }
+          uint8_t* sa = smem + stage * L::kStageBytes;
+          uint8_t* sb = sa + L::kABytes;
+          if constexpr (PAIR) {
+            const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
+            if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * L::kStageBytes);
+            tma2_load_2d(sa, &map_a, bar, kb * BK, row0);
+            if constexpr (kBack) {
+#pragma unroll
+              for (int j = 0; j < BN / 128; ++j)
+                tma2_load_2d(sb + j * BK * 128, &map_b, bar, n0 + rank * (BN / 2) + j * 64, kb * BK);
+            } else {
+              tma2_load_2d(sb, &map_b, bar, kb * BK, rank * p.inner + n0);
+            }
+          } else {
+            mbar_expect_tx(&full_bar[stage], L::kStageBytes);
+            tma_load_2d(sa, &map_a, &full_bar[stage], kb * BK, row0);
+            if constexpr (kBack) {
+#pragma unroll
+              for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * BK * 128, &map_b, &full_bar[stage], n0 + j * 64, kb * BK);
+            } else {
+              tma_load_2d(sb, &map_b, &full_bar[stage], kb * BK, n0);
+              tma_load_2d(sb + kCols * 128, &map_b, &full_bar[stage], kb * BK, p.inner + n0);
+            }
+          }
+          if (++stage == L::kStages) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) atomicExch(p.status, GEMM_ERR_PRODUCER_TIMEOUT);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (of a pair: the leader)
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = make_idesc_f16kind(PAIR ? 256 : 128, BN, false, kBack);
+      constexpr uint32_t b_lbo = kBack ? BK * 128 : 16, b_kstep = kBack ? UMMA_K * 128 : UMMA_K * 2;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += stride) {
+        if (!mbar_wait(&tmem_empty[acc], acc_phase ^ 1)) { ok = false; break; }
+        fence_after_sync();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase)) { ok = false; break; }
+          fence_after_sync();
+          const uint32_t sa = smem_u32(smem + stage * L::kStageBytes), sb = sa + L::kABytes;
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k) {
+            const uint64_t da = make_smem_desc_sw128(sa + k * UMMA_K * 2, 16, 1024);
+            const uint64_t db = make_smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
+            if constexpr (PAIR) mma2_f16_ss(d_tmem, da, db, idesc, (kb | k) != 0);
+            else mma_f16_ss(d_tmem, da, db, idesc, (kb | k) != 0);
+          }
+          if constexpr (PAIR) mma2_commit_both(&empty_bar[stage]);
+          else mma_commit(&empty_bar[stage]);
+          if (++stage == L::kStages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        if constexpr (PAIR) mma2_commit_both(&tmem_full[acc]);
+        else mma_commit(&tmem_full[acc]);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      if (!ok) atomicExch(p.status, GEMM_ERR_MMA_TIMEOUT);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue warps: 32 rows, every other run of columns
+    const int lane_group = warp % 4, second = (warp - 2) / 4;
+    constexpr int kShare = kCols >= 64 ? kCols / 2 : kCols;         // columns of a warp; of 32 the second warp has none
+    const int c_first = second * kShare, c_last = c_first + kShare <= kCols ? c_first + kShare : c_first;
+    uint8_t* buf_0 = epi_stage + (warp - 2) * L::kWarpStage;
+    uint64_t* side = &side_bar[warp - 2];
+    int acc = 0;
+    uint32_t acc_phase = 0, side_phase = 0, turn = 0;
+    bool ok = true;
+
+    // backward: (tile, column) of the chunk whose v and g are fetched next
+    int ahead_tile = first_tile, ahead_c = c_first;
+    auto fetch_next = [&]() {
+      if constexpr (kBack) {
+        while (ahead_tile < num_tiles && (ahead_c >= c_last || (ahead_tile % tiles_n) * kCols + ahead_c >= p.inner)) {
+          ahead_tile += stride;
+          ahead_c = c_first;
+        }
+        if (ahead_tile >= num_tiles) return;
+        if (lane == 0) {
+          const int x = (ahead_tile % tiles_n) * kCols + ahead_c;
+          const int y = (ahead_tile / tiles_n) * kTileRows + rank * BM + lane_group * 32;
+          mbar_expect_tx(side, 8192);
+          tma_load_2d(buf_0, &map_0, side, x, y);
+          tma_load_2d(buf_0 + 4096, &map_1, side, x, y);
+        }
+        ahead_c += 32;
+      }
+    };
+    if (c_first < c_last) fetch_next();
+    for (int tile = first_tile; tile < num_tiles && ok; tile += stride) {
+      const int row0 = (tile / tiles_n) * kTileRows + rank * BM + lane_group * 32, col0 = (tile % tiles_n) * kCols;
+      const bool box_in = row0 < p.rows;                            // else there is nothing to store
+      if (!mbar_wait(&tmem_full[acc], acc_phase)) { ok = false; break; }
+      fence_after_sync();
+      const uint32_t taddr = tmem_base + (uint32_t(lane_group * 32) << 16) + acc * BN;
+#pragma unroll 1
+      for (int c = c_first; c < c_last; c += 32) {
+        const int n0 = col0 + c;
+        if (n0 >= p.inner) break;                                   // the same for the whole warp
+        if constexpr (kBack) {
+          if (!mbar_wait(side, side_phase)) { ok = false; break; }
+          side_phase ^= 1;
+          float v[32], g[32];
+          get_row128(buf_0, v);
+          get_row128(buf_0 + 4096, g);
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + c, r);
+          __syncwarp();
+          fetch_next();
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float2 a, da;
+            act_and_grad2(make_float2(g[j], g[j + 1]), p.act, a, da);
+            const float2 dh = make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+            const float2 dg = __fmul2_rn(__fmul2_rn(dh, make_float2(v[j], v[j + 1])), da);
+            const float2 dv = __fmul2_rn(dh, a);
+            v[j] = dv.x; v[j + 1] = dv.y;
+            g[j] = dg.x; g[j + 1] = dg.y;
+          }
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+          gemm_epi::stage_row64(buf_0 + 8192, v);
+          gemm_epi::stage_row64(buf_0 + 10240, g);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (box_in) {
+              tma_store_2d(&map_2, buf_0 + 8192, n0, row0);
+              tma_store_2d(&map_3, buf_0 + 10240, n0, row0);
+            }
+            bulk_commit_group();
+          }
+        } else {
+          float v[32], g[32], h[32];
+          {
+            uint32_t rv[32], rg[32];
+            tmem_ld_32x32(taddr + c, rv);
+            tmem_ld_32x32(taddr + kCols + c, rg);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              v[j] = __uint_as_float(rv[j]);
+              g[j] = __uint_as_float(rg[j]);
+            }
+          }
+          if (p.bias != nullptr) {
+            add_bias(v, p.bias + n0, p.inner - n0);
+            add_bias(g, p.bias + p.inner + n0, p.inner - n0);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 t = __fmul2_rn(make_float2(v[j], v[j + 1]), act2(make_float2(g[j], g[j + 1]), p.act));
+            h[j] = t.x;
+            h[j + 1] = t.y;
+          }
+          uint8_t* out = MODE == FORWARD ? buf_0 + (turn++ & 1) * 2048 : buf_0 + 8192;
+          if (lane == 0) {
+            if constexpr (MODE == FORWARD) bulk_wait_group_read<1>();
+            else bulk_wait_group_read<0>();
+          }
+          __syncwarp();
+          gemm_epi::stage_row64(out, h);
+          if constexpr (MODE == FORWARD_KEEP) {
+            put_row128(buf_0, v);
+            put_row128(buf_0 + 4096, g);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (box_in) {
+              tma_store_2d(&map_0, out, n0, row0);
+              if constexpr (MODE == FORWARD_KEEP) {
+                tma_store_2d(&map_1, buf_0, n0, row0);
+                tma_store_2d(&map_2, buf_0 + 4096, n0, row0);
+              }
+            }
+            bulk_commit_group();
+          }
+        }
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if (!PAIR || rank == 0) mbar_arrive(&tmem_empty[acc]);
+        else remote_arrive(map_to_cta(smem_u32(&tmem_empty[acc]), 0));
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+    if (!ok && lane == 0) atomicExch(p.status, GEMM_ERR_EPILOGUE_TIMEOUT);
+    if (lane == 0) bulk_wait_group_all();
+  }
+
+  fence_before_sync();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();              // neither CTA leaves while the other may still touch it
+  if (warp == 1) {
+    fence_after_sync();
+    if constexpr (PAIR) tmem_dealloc2(tmem_base, kTmemCols);
+    else tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+template <int BN, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+             const __grid_constant__ CUtensorMap map_0, const __grid_constant__ CUtensorMap map_1,
+             const __grid_constant__ CUtensorMap map_2, const __grid_constant__ CUtensorMap map_3, const Params p) {
+  gated_body<BN, false, MODE>(map_a, map_b, map_0, map_1, map_2, map_3, p);
+}
+template <int BN, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gated_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const __grid_constant__ CUtensorMap map_0, const __grid_constant__ CUtensorMap map_1,
+                  const __grid_constant__ CUtensorMap map_2, const __grid_constant__ CUtensorMap map_3, const Params p) {
+  gated_body<BN, true, MODE>(map_a, map_b, map_0, map_1, map_2, map_3, p);
+}
+
+// rows x cols of pitch ld; fp32 in boxes of 32 x 32 with 128-byte swizzle, elements in boxes of box_rows x box_cols with
+// box_cols * 2 bytes of swizzle
+int encode(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_rows, int box_cols, bool fp32) {
+  auto enc = fbam_encode_tiled();
+  if (!enc) return GEMM_ERR_DRIVER;
+  fbam_bind_context_to_thread();
+  const int size = fp32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (ld * size) % 16) return GEMM_ERR_ALIGNMENT;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  const CUresult r = enc(map, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : ELEM_TMAP, 2, const_cast<void*>(base), dims, strides, box, ones,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) g_fbam_last_driver_error = (int)r;
+  return r == CUDA_SUCCESS ? 0 : GEMM_ERR_TENSORMAP;
+}
+
+template <typename K>
+int launch(K kernel, int smem, bool pair, long long tiles, const CUtensorMap (&m)[6], const Params& p, cudaStream_t s) {
+  static int sms = 0;
+  if (sms == 0) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  }
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return GEMM_ERR_LAUNCH;
+  const int usable = sms - g_fbam_reserved_sms > 2 ? sms - g_fbam_reserved_sms : 2;
+  const long long slots = pair ? usable / 2 : usable, blocks = (tiles < slots ? tiles : slots) * (pair ? 2 : 1);
+  kernel<<<(unsigned)blocks, kThreads, smem, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
+  return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+}
+
+long long tiles_of(int rows, int tile_rows, int cols, int tile_cols) {
+  return (long long)((rows + tile_rows - 1) / tile_rows) * ((cols + tile_cols - 1) / tile_cols);
+}
+
+// Accumulator width and pairing: 0: single CTAs with 64 columns, 1: with 128, 2: pairs with 256.
+int pick(int rows, int inner, bool back) {
+  if (getenv("GM_PICK")) return atoi(getenv("GM_PICK"));
+  const int h = back ? 2 : 1;
+  if (tiles_of(rows, 256, inner, 128 * h) >= 74) return 2;
+  return tiles_of(rows, 128, inner, 64 * h) >= 148 ? 1 : 0;
+}
+
+template <int MODE>
+int run(int which, int rows, int inner, const CUtensorMap (&m)[6], const Params& p, cudaStream_t s) {
+  constexpr int h = MODE == BACKWARD ? 2 : 1;
+  if (which == 2)
+    return launch(gated_pair_kernel<256, MODE>, Smem<256, true, MODE>::kTotal, true, tiles_of(rows, 256, inner, 128 * h), m, p, s);
+  if (which == 1)
+    return launch(gated_kernel<128, MODE>, Smem<128, false, MODE>::kTotal, false, tiles_of(rows, 128, inner, 64 * h), m, p, s);
+  return launch(gated_kernel<64, MODE>, Smem<64, false, MODE>::kTotal, false, tiles_of(rows, 128, inner, 32 * h), m, p, s);
 }
 
 }  // namespace
 
-extern "C" int fbam_gated_act(const float* vg, const float* dh, void* out, long long rows, int inner, int act, void* stream) {
-  if (rows <= 0 || inner <= 0 || inner % 8 != 0 || act < 0 || act > 1) return GEMM_ERR_SHAPE;
-  const long long n = rows * inner, blocks = (n + 511) / 512;
-  gated_act_kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      vg, dh, (elem_t*)out, n, inner, act);
-  return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+// x (rows, depth) pitch ldx, w_in (2 inner, depth) pitch ldw, bias (2 inner) elements or null -> h (rows, inner) dense and, where v
+// is not null, v and g (rows, inner) dense fp32.  inner is a multiple of 8, all rows start on 16-byte boundaries.
+extern "C" int fbam_gated_fwd(const void* x, long long ldx, const void* w_in, long long ldw, const void* bias, void* h, float* v,
+                              float* g, int rows, int inner, int depth, int act, int* status, void* stream) {
+  if (rows <= 0 || inner <= 0 || depth <= 0 || inner % 8 != 0 || inner > 0x3fffffff || act < 0 || act > 1 || (v == nullptr) != (g == nullptr))
+    return GEMM_ERR_SHAPE;
+  const int which = pick(rows, inner, false), box = which == 2 ? 128 : which == 1 ? 64 : 32;
+  CUtensorMap m[6];
+  int e = encode(&m[0], x, rows, depth, ldx, BM, BK, false);
+  if (!e) e = encode(&m[1], w_in, 2ll * inner, depth, ldw, box, BK, false);
+  if (!e) e = encode(&m[2], h, rows, inner, inner, 32, 32, false);
+  if (!e && v) e = encode(&m[3], v, rows, inner, inner, 32, 32, true);
+  if (!e && v) e = encode(&m[4], g, rows, inner, inner, 32, 32, true);
+  if (e) return e;
+  if (!v) m[3] = m[4] = m[2];
+  m[5] = m[2];
+  const Params p{(const elem_t*)bias, status, rows, inner, depth, act};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return v ? run<FORWARD_KEEP>(which, rows, inner, m, p, s) : run<FORWARD>(which, rows, inner, m, p, s);
+}
+
+// dy (rows, depth) pitch ldy, w_out (depth, inner) pitch ldw, v and g as the forward left them -> d_vg (rows, 2 inner) dense.
+extern "C" int fbam_gated_bwd(const void* dy, long long ldy, const void* w_out, long long ldw, const float* v, const float* g, void* d_vg,
+                              int rows, int inner, int depth, int act, int* status, void* stream) {
+  if (rows <= 0 || inner <= 0 || depth <= 0 || inner % 8 != 0 || inner > 0x3fffffff || act < 0 || act > 1) return GEMM_ERR_SHAPE;
+  CUtensorMap m[6];
+  int e = encode(&m[0], dy, rows, depth, ldy, BM, BK, false);
+  if (!e) e = encode(&m[1], w_out, depth, inner, ldw, BK, 64, false);
+  if (!e) e = encode(&m[2], v, rows, inner, inner, 32, 32, true);
+  if (!e) e = encode(&m[3], g, rows, inner, inner, 32, 32, true);
+  if (!e) e = encode(&m[4], d_vg, rows, inner, 2ll * inner, 32, 32, false);
+  if (!e) e = encode(&m[5], (elem_t*)d_vg + inner, rows, inner, 2ll * inner, 32, 32, false);
+  if (e) return e;
+  const Params p{nullptr, status, rows, inner, depth, act};
+  return run<BACKWARD>(pick(rows, inner, true), rows, inner, m, p, reinterpret_cast<cudaStream_t>(stream));
 }

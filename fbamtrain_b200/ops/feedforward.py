@@ -3,12 +3,11 @@ with ``(v, g) = x W_inᵀ + b_in``; the first half of the projection is the valu
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
+from ..utils import flops
 from . import native as nv
-from .native_ops import _colsum, _need_elem, gemm, gemm_nn, gemm_tn, weight_grad_splits
+from .native_ops import _colsum, _need_elem, _tma_pitch, gemm, gemm_nn, gemm_tn, weight_grad_splits
 
 GATES = {"gelu": 0, "silu": 1}
 
@@ -45,58 +44,83 @@ def _bias_grad(d: torch.Tensor) -> torch.Tensor:
     return _colsum(d, d.dtype)
 
 
-def _gated_act(vg, dh, out, rows, inner, act):
-    nv.check(nv.lib(out).fbam_gated_act(nv.ptr(vg), nv.ptr(dh), nv.ptr(out), C.c_longlong(rows), inner, act, nv.stream_ptr()),
-             "fbam_gated_act")
-    return out
+def _project(x2, w1, b1, act, keep):
+    """``(h, vg)``: the gated hidden values and, with ``keep``, both factors before the activation, ``(2, rows, inner)`` fp32."""
+    rows, inner = x2.shape[0], w1.shape[0] // 2
+    x2, w1 = _tma_pitch(x2), _tma_pitch(w1)
+    h = torch.empty((rows, inner), dtype=x2.dtype, device=x2.device)
+    vg = torch.empty((2, rows, inner), dtype=torch.float32, device=x2.device) if keep else None
+    v, g = (vg[0].data_ptr(), vg[1].data_ptr()) if keep else (0, 0)
+    nv.check(nv.lib(x2).fbam_gated_fwd(x2.data_ptr(), x2.stride(0), w1.data_ptr(), w1.stride(0), nv.addr(b1), h.data_ptr(), v, g,
+                                       rows, inner, x2.shape[1], act, nv.status_word(x2.device).data_ptr(), nv.stream()),
+             "fbam_gated_fwd")
+    flops.add(4.0 * rows * inner * x2.shape[1])
+    return h, vg
+
+
+def _project_grad(dy2, w2, vg, act):
+    """The gradient of the projection ``(rows, 2 · inner)``, values first."""
+    _, rows, inner = vg.shape
+    dy2, w2 = _tma_pitch(dy2), _tma_pitch(w2)
+    d_vg = torch.empty((rows, 2 * inner), dtype=dy2.dtype, device=dy2.device)
+    nv.check(nv.lib(dy2).fbam_gated_bwd(dy2.data_ptr(), dy2.stride(0), w2.data_ptr(), w2.stride(0), vg[0].data_ptr(),
+                                        vg[1].data_ptr(), d_vg.data_ptr(), rows, inner, dy2.shape[1], act,
+                                        nv.status_word(dy2.device).data_ptr(), nv.stream()), "fbam_gated_bwd")
+    flops.add(2.0 * rows * inner * dy2.shape[1])
+    return d_vg
+
+
+def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
+    """``(y, x2, w1, w2, vg, h)``; the later ones for the backward."""
+    inner, dim = w_out.shape[1], w_out.shape[0]
+    x2 = _dense(x.reshape(-1, x.shape[-1]))
+    res2 = None if residual is None else _dense(residual.reshape(-1, dim))
+    w1, w2, b1, _ = _wider(_dense(w_in), _dense(w_out), None if b_in is None else _dense(b_in), inner)
+    h, vg = _project(x2, w1, b1, act, keep)
+    y = gemm(h, w2, bias=None if b_out is None else _dense(b_out), residual=res2)
+    return y.view(*x.shape[:-1], dim), x2, w1, w2, vg, h
 
 
 class _GatedMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, act, residual):
-        inner, dim = w_out.shape[1], w_out.shape[0]
-        x2 = _dense(x.reshape(-1, x.shape[-1]))
-        res2 = None if residual is None else _dense(residual.reshape(-1, dim))
-        w1, w2, b1, wide = _wider(_dense(w_in), _dense(w_out), b_in, inner)
-        rows = x2.shape[0]
-        vg = gemm(x2, w1, bias=b1, out_dtype=torch.float32)
-        h = _gated_act(vg, None, torch.empty(rows, wide, dtype=x.dtype, device=x.device), rows, wide, act)
-        y = gemm(h, w2, bias=b_out, residual=res2)
+        y, x2, w1, w2, vg, h = _forward(x, w_in, w_out, b_in, b_out, act, residual, True)
         ctx.save_for_backward(x2, w1, w2, vg, h)
-        ctx.meta = (x.shape, inner, act, b_in is not None, b_out is not None)
-        return y.view(*x.shape[:-1], dim)
+        ctx.meta = (x.shape, w_out.shape[1], act)
+        return y
 
     @staticmethod
     def backward(ctx, dy):
         x2, w1, w2, vg, h = ctx.saved_tensors
-        shape, inner, act, has_b_in, has_b_out = ctx.meta
+        shape, inner, act = ctx.meta
         need = ctx.needs_input_grad
-        rows, dim = x2.shape[0], w2.shape[0]
-        wide = w2.shape[1]
+        rows, wide = h.shape
+        dim = w2.shape[0]
         dy2 = _dense(dy.reshape(-1, dim))
         dx = dw_in = dw_out = db_in = db_out = None
         if need[0] or need[1] or need[3]:
-            dh = gemm_nn(dy2, w2, out_dtype=torch.float32)
-            dvg = _gated_act(vg, dh, torch.empty(rows, 2 * wide, dtype=dy.dtype, device=dy.device), rows, wide, act)
+            d_vg = _project_grad(dy2, w2, vg, act)
             if need[0]:
-                dx = gemm_nn(dvg, w1).view(shape)
+                dx = gemm_nn(d_vg, w1).view(shape)
             if need[1]:
-                dw_in = gemm_tn(dvg, x2, splits=weight_grad_splits(2 * wide, x2.shape[1], rows))
+                dw_in = gemm_tn(d_vg, x2, splits=weight_grad_splits(2 * wide, x2.shape[1], rows))
                 if wide != inner:
                     dw_in = dw_in.view(2, wide, -1)[:, :inner].reshape(2 * inner, -1)
-            if has_b_in and need[3]:
-                db_in = _bias_grad(dvg)
+            if need[3]:
+                db_in = _bias_grad(d_vg)
                 if wide != inner:
                     db_in = db_in.view(2, wide)[:, :inner].reshape(-1)
         if need[2]:
             dw_out = gemm_tn(dy2, h, splits=weight_grad_splits(dim, wide, rows))
             if wide != inner:
                 dw_out = dw_out[:, :inner].contiguous()
-        if has_b_out and need[4]:
+        if need[4]:
             db_out = _bias_grad(dy2)
         return dx, dw_in, dw_out, db_in, db_out, None, dy if need[6] else None
 
 
 def gated_mlp(x, w_in, w_out, b_in, b_out, act, residual):
     _need_elem(x, w_in, w_out, b_in, b_out, residual)
-    return _GatedMlp.apply(x, w_in, w_out, b_in, b_out, GATES[act], residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out, residual)):
+        return _GatedMlp.apply(x, w_in, w_out, b_in, b_out, GATES[act], residual)
+    return _forward(x, w_in, w_out, b_in, b_out, GATES[act], residual, False)[0]
