@@ -66,6 +66,7 @@ __device__ __forceinline__ void act_and_grad2(float2 g, int act, float2& a, floa
 
 struct Params {
   const elem_t* bias;       // [2 inner], or null
+  float* col_sums;          // backward: [rows / 32, upwards][2 inner] sums over 32 rows, or null
   int* status;
   int rows, inner, depth;   // depth: the products' K
   int act;
@@ -121,6 +122,16 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const elem_t* bias, int
     for (int j = 0; j < 32; ++j)
       if (j < left) v[j] += e2f(bias[j]);
   }
+}
+
+// Tiles in panels of kPanel columns of tiles, row by row inside a panel: what runs at the same time then shares few rows of A
+// and of B, which stay in L2 (8192 x 2048 x 8192, forward that keeps: 472 -> 401 us; without keeping 336 -> 318).
+constexpr int kPanel = 16;
+struct Tile { int m, n; };
+__device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
+  const int panel = t / (kPanel * tiles_m), in = t - panel * kPanel * tiles_m;
+  const int width = min(kPanel, tiles_n - panel * kPanel);
+  return {in / width, panel * kPanel + in % width};
 }
 
 // Forward: map_0 h, map_1 v, map_2 g (stores).  Backward: map_0 v, map_1 g (loads), map_2 dv, map_3 dg (stores).
@@ -185,7 +196,8 @@ gated_body(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = first_tile; tile < num_tiles && ok; tile += stride) {
-        const int row0 = (tile / tiles_n) * kTileRows + rank * BM, n0 = (tile % tiles_n) * kCols;
+        const Tile at = tile_at(tile, tiles_m, tiles_n);
+        const int row0 = at.m * kTileRows + rank * BM, n0 = at.n * kCols;
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1)) { ok = false; break; }
           uint8_t* sa = smem + stage * L::kStageBytes;
@@ -262,18 +274,19 @@ gated_body(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap
     uint32_t acc_phase = 0, side_phase = 0, turn = 0;
     bool ok = true;
 
-    // backward: (tile, column) of the chunk whose v and g are fetched next
+    // backward: tile and column of the chunk whose v and g are fetched next; behind the last one it stays where it is
     int ahead_tile = first_tile, ahead_c = c_first;
+    Tile ahead = tile_at(first_tile, tiles_m, tiles_n);
     auto fetch_next = [&]() {
       if constexpr (kBack) {
-        while (ahead_tile < num_tiles && (ahead_c >= c_last || (ahead_tile % tiles_n) * kCols + ahead_c >= p.inner)) {
+        while (ahead_c >= c_last || ahead.n * kCols + ahead_c >= p.inner) {
           ahead_tile += stride;
+          if (ahead_tile >= num_tiles) return;
+          ahead = tile_at(ahead_tile, tiles_m, tiles_n);
           ahead_c = c_first;
         }
-        if (ahead_tile >= num_tiles) return;
         if (lane == 0) {
-          const int x = (ahead_tile % tiles_n) * kCols + ahead_c;
-          const int y = (ahead_tile / tiles_n) * kTileRows + rank * BM + lane_group * 32;
+          const int x = ahead.n * kCols + ahead_c, y = ahead.m * kTileRows + rank * BM + lane_group * 32;
           mbar_expect_tx(side, 8192);
           tma_load_2d(buf_0, &map_0, side, x, y);
           tma_load_2d(buf_0 + 4096, &map_1, side, x, y);
@@ -283,7 +296,8 @@ gated_body(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap
     };
     if (c_first < c_last) fetch_next();
     for (int tile = first_tile; tile < num_tiles && ok; tile += stride) {
-      const int row0 = (tile / tiles_n) * kTileRows + rank * BM + lane_group * 32, col0 = (tile % tiles_n) * kCols;
+      const Tile at = tile_at(tile, tiles_m, tiles_n);
+      const int row0 = at.m * kTileRows + rank * BM + lane_group * 32, col0 = at.n * kCols;
       const bool box_in = row0 < p.rows;                            // else there is nothing to store
       if (!mbar_wait(&tmem_full[acc], acc_phase)) { ok = false; break; }
       fence_after_sync();
@@ -317,6 +331,15 @@ gated_body(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap
           __syncwarp();
           gemm_epi::stage_row64(buf_0 + 8192, v);
           gemm_epi::stage_row64(buf_0 + 10240, g);
+          if (p.col_sums != nullptr && box_in) {                    // rows behind the end are 0
+            float* sums = p.col_sums + (long long)(row0 / 32) * 2 * p.inner + n0;
+            gemm_epi::segment_sums<32>(v, nullptr);
+            gemm_epi::segment_sums<32>(g, nullptr);
+            if (n0 + lane < p.inner) {
+              sums[lane] = v[0];
+              sums[p.inner + lane] = g[0];
+            }
+          }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -396,6 +419,114 @@ gated_body(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// A few rows: the weights are streamed once, and a 128-row tile would be padding.  A CTA has 8 output columns (and, gated, the 8
+// gate columns of the same hidden ones), its warps take runs of 32 along K in turn; mma.sync.m16n8k16 with the 8 columns as N and
+// 16 rows as M.  The order of K inside a run does not matter to a product, so lane t of a quad takes K = 8 t .. 8 t + 7 of both
+// operands: one 16-byte load feeds two instructions.
+// ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." ELEM_PTX "." ELEM_PTX ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct FewParams {
+  const elem_t *x, *w, *bias, *residual;      // w: gated (2 cols, depth), else (cols, depth)
+  elem_t* out;                                // [rows][cols] dense
+  long long ldx, ldw, ldr;
+  int rows, cols, depth, act;                 // depth: a multiple of 8; all rows of x and w on 16-byte boundaries
+};
+
+// The second product's CTAs start while the first one's still run, fetch their first weights and wait for its results there.
+template <int MT, bool GATED>
+__global__ void __launch_bounds__(GATED ? 256 : 512)
+few_rows_kernel(const FewParams p) {
+  constexpr int kB = GATED ? 2 : 1, kAhead = 4, kFewWarps = GATED ? 8 : 16;
+  __shared__ float sums[kFewWarps][kB][MT][16][8];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane % 4, grp = lane / 4;
+  const int n0 = blockIdx.x * 8, n = n0 + grp;
+  const elem_t* w[kB];
+#pragma unroll
+  for (int i = 0; i < kB; ++i) w[i] = p.w + (long long)((n < p.cols ? n : p.cols - 1) + i * p.cols) * p.ldw;
+  const elem_t* x[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = m * 16 + i * 8 + grp;
+      x[m][i] = p.x + (long long)(row < p.rows ? row : p.rows - 1) * p.ldx;      // rows behind the last one are not stored
+    }
+  float acc[kB][MT][4] = {};
+  if constexpr (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  bool waited = GATED;
+  for (int k0 = warp * 32; k0 < p.depth; k0 += kFewWarps * 32 * kAhead) {
+    uint4 b[kAhead][kB];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int k = k0 + u * kFewWarps * 32 + quad * 8;
+#pragma unroll
+      for (int i = 0; i < kB; ++i)
+        b[u][i] = k < p.depth ? __ldcs(reinterpret_cast<const uint4*>(w[i] + k)) : make_uint4(0, 0, 0, 0);
+    }
+    if (!waited) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      waited = true;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int k = k0 + u * kFewWarps * 32 + quad * 8;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint4 a[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          a[i] = k < p.depth ? *reinterpret_cast<const uint4*>(x[m][i] + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+          mma_16x8x16(acc[i][m], a[0].x, a[1].x, a[0].y, a[1].y, b[u][i].x, b[u][i].y);
+          mma_16x8x16(acc[i][m], a[0].z, a[1].z, a[0].w, a[1].w, b[u][i].z, b[u][i].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kB; ++i)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sums[warp][i][m][grp + q / 2 * 8][quad * 2 + q % 2] = acc[i][m][q];
+  if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");      // a warp without a part of K
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * 128; o += kFewWarps * 32) {
+    const int row = o / 8, c = o % 8, col = n0 + c;
+    if (row >= p.rows || col >= p.cols) continue;
+    float s[kB] = {};
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+#pragma unroll
+      for (int v = 0; v < kFewWarps; ++v) s[i] += sums[v][i][row / 16][row % 16][c];
+      if (p.bias != nullptr) s[i] += e2f(p.bias[col + i * p.cols]);
+    }
+    if constexpr (GATED) s[0] *= act2(make_float2(s[1], 0.0f), p.act).x;
+    else if (p.residual != nullptr) s[0] += e2f(p.residual[row * p.ldr + col]);
+    p.out[(long long)row * p.cols + col] = f2e(s[0]);
+  }
+}
+
+template <bool GATED>
+int launch_few(const FewParams& p, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.cols + 7) / 8));
+  cfg.blockDim = dim3(GATED ? 256 : 512);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = GATED ? 0 : 1;
+  return cudaLaunchKernelEx(&cfg, p.rows <= 16 ? few_rows_kernel<1, GATED> : few_rows_kernel<2, GATED>, p) == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+}
+
 template <int BN, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -409,6 +540,24 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                   const __grid_constant__ CUtensorMap map_0, const __grid_constant__ CUtensorMap map_1,
                   const __grid_constant__ CUtensorMap map_2, const __grid_constant__ CUtensorMap map_3, const Params p) {
   gated_body<BN, true, MODE>(map_a, map_b, map_0, map_1, map_2, map_3, p);
+}
+
+// out[c] = sum over `parts` rows of part[r][c], in a fixed order: eight threads a column, every eighth row each.
+__global__ void __launch_bounds__(256) add_sums_kernel(const float* __restrict__ part, elem_t* __restrict__ out, int parts, int cols) {
+  __shared__ float sums[8][33];
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, r = threadIdx.x / 32;
+  float sum = 0.0f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int i = r; i < parts; i += 8) sum += part[(long long)i * cols + c];
+  }
+  sums[r][threadIdx.x % 32] = sum;
+  __syncthreads();
+  if (r == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += sums[i][threadIdx.x];
+    out[c] = f2e(sum);
+  }
 }
 
 // rows x cols of pitch ld; fp32 in boxes of 32 x 32 with 128-byte swizzle, elements in boxes of box_rows x box_cols with
@@ -484,15 +633,18 @@ extern "C" int fbam_gated_fwd(const void* x, long long ldx, const void* w_in, lo
   if (e) return e;
   if (!v) m[3] = m[4] = m[2];
   m[5] = m[2];
-  const Params p{(const elem_t*)bias, status, rows, inner, depth, act};
+  const Params p{(const elem_t*)bias, nullptr, status, rows, inner, depth, act};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return v ? run<FORWARD_KEEP>(which, rows, inner, m, p, s) : run<FORWARD>(which, rows, inner, m, p, s);
 }
 
-// dy (rows, depth) pitch ldy, w_out (depth, inner) pitch ldw, v and g as the forward left them -> d_vg (rows, 2 inner) dense.
+// dy (rows, depth) pitch ldy, w_out (depth, inner) pitch ldw, v and g as the forward left them -> d_vg (rows, 2 inner) dense, and
+// where col_sums is not null its column sums in db (2 inner) elements; col_sums is the workspace, 2 inner fp32 values for every 32 rows.
 extern "C" int fbam_gated_bwd(const void* dy, long long ldy, const void* w_out, long long ldw, const float* v, const float* g, void* d_vg,
-                              int rows, int inner, int depth, int act, int* status, void* stream) {
-  if (rows <= 0 || inner <= 0 || depth <= 0 || inner % 8 != 0 || inner > 0x3fffffff || act < 0 || act > 1) return GEMM_ERR_SHAPE;
+                              float* col_sums, void* db, int rows, int inner, int depth, int act, int* status, void* stream) {
+  if (rows <= 0 || inner <= 0 || depth <= 0 || inner % 8 != 0 || inner > 0x3fffffff || act < 0 || act > 1 ||
+      (col_sums == nullptr) != (db == nullptr))
+    return GEMM_ERR_SHAPE;
   CUtensorMap m[6];
   int e = encode(&m[0], dy, rows, depth, ldy, BM, BK, false);
   if (!e) e = encode(&m[1], w_out, depth, inner, ldw, BK, 64, false);
@@ -501,6 +653,28 @@ extern "C" int fbam_gated_bwd(const void* dy, long long ldy, const void* w_out, 
   if (!e) e = encode(&m[4], d_vg, rows, inner, 2ll * inner, 32, 32, false);
   if (!e) e = encode(&m[5], (elem_t*)d_vg + inner, rows, inner, 2ll * inner, 32, 32, false);
   if (e) return e;
-  const Params p{nullptr, status, rows, inner, depth, act};
-  return run<BACKWARD>(pick(rows, inner, true), rows, inner, m, p, reinterpret_cast<cudaStream_t>(stream));
+  const Params p{nullptr, col_sums, status, rows, inner, depth, act};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  e = run<BACKWARD>(pick(rows, inner, true), rows, inner, m, p, s);
+  if (e || db == nullptr) return e;
+  add_sums_kernel<<<(2 * inner + 31) / 32, 256, 0, s>>>(col_sums, (elem_t*)db, (rows + 31) / 32, 2 * inner);
+  return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+}
+
+// Up to 32 rows, the whole block: x (rows, depth) pitch ldx -> h (rows, inner), a workspace, -> y (rows, out_dim), both dense.
+// depth and inner are multiples of 8; rows of x, w_in and w_out start on 16-byte boundaries; biases and residual may be null.
+extern "C" int fbam_gated_few_rows(const void* x, long long ldx, const void* w_in, long long ld_in, const void* b_in, const void* w_out,
+                                   long long ld_out, const void* b_out, const void* residual, long long ldr, void* h, void* y, int rows,
+                                   int depth, int inner, int out_dim, int act, void* stream) {
+  if (rows <= 0 || rows > 32 || depth <= 0 || inner <= 0 || out_dim <= 0 || depth % 8 || inner % 8 || inner > 0x3fffffff || act < 0 || act > 1)
+    return GEMM_ERR_SHAPE;
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w_in) | reinterpret_cast<uintptr_t>(w_out) | reinterpret_cast<uintptr_t>(h)) & 15) ||
+      ((ldx | ld_in | ld_out) & 7))
+    return GEMM_ERR_ALIGNMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int e = launch_few<true>({(const elem_t*)x, (const elem_t*)w_in, (const elem_t*)b_in, nullptr, (elem_t*)h, ldx, ld_in, 0, rows,
+                                  inner, depth, act}, s);
+  if (e) return e;
+  return launch_few<false>({(const elem_t*)h, (const elem_t*)w_out, (const elem_t*)b_out, (const elem_t*)residual, (elem_t*)y, inner,
+                            ld_out, ldr, rows, out_dim, inner, act}, s);
 }

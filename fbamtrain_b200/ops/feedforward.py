@@ -58,27 +58,55 @@ def _project(x2, w1, b1, act, keep):
     return h, vg
 
 
-def _project_grad(dy2, w2, vg, act):
-    """The gradient of the projection ``(rows, 2 · inner)``, values first."""
+def _project_grad(dy2, w2, vg, act, sums):
+    """The gradient of the projection ``(rows, 2 · inner)``, values first, and with ``sums`` its column sums."""
     _, rows, inner = vg.shape
+    dev = dy2.device
     dy2, w2 = _tma_pitch(dy2), _tma_pitch(w2)
-    d_vg = torch.empty((rows, 2 * inner), dtype=dy2.dtype, device=dy2.device)
+    d_vg = torch.empty((rows, 2 * inner), dtype=dy2.dtype, device=dev)
+    work = torch.empty(((rows + 31) // 32, 2 * inner), dtype=torch.float32, device=dev) if sums else None
+    db = torch.empty(2 * inner, dtype=dy2.dtype, device=dev) if sums else None
     nv.check(nv.lib(dy2).fbam_gated_bwd(dy2.data_ptr(), dy2.stride(0), w2.data_ptr(), w2.stride(0), vg[0].data_ptr(),
-                                        vg[1].data_ptr(), d_vg.data_ptr(), rows, inner, dy2.shape[1], act,
-                                        nv.status_word(dy2.device).data_ptr(), nv.stream()), "fbam_gated_bwd")
+                                        vg[1].data_ptr(), d_vg.data_ptr(), nv.addr(work), nv.addr(db), rows, inner, dy2.shape[1],
+                                        act, nv.status_word(dev).data_ptr(), nv.stream()), "fbam_gated_bwd")
     flops.add(2.0 * rows * inner * dy2.shape[1])
-    return d_vg
+    return d_vg, db
+
+
+# Rows up to which the weights are streamed past the rows instead of tiled.
+FEW_ROWS = 32
+
+
+def _few_rows(x2, w1, w2, b1, b_out, act, res2):
+    """The block on up to ``FEW_ROWS`` rows, or None where a row does not start on a 16-byte boundary."""
+    rows, depth = x2.shape
+    dim, inner = w2.shape
+    if depth % 8 or (x2.data_ptr() | w1.data_ptr() | w2.data_ptr()) % 16:
+        return None
+    h = torch.empty((rows, inner), dtype=x2.dtype, device=x2.device)
+    y = torch.empty((rows, dim), dtype=x2.dtype, device=x2.device)
+    nv.check(nv.lib(x2).fbam_gated_few_rows(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b1), w2.data_ptr(), inner,
+                                            nv.addr(b_out), nv.addr(res2), dim, h.data_ptr(), y.data_ptr(), rows, depth, inner, dim,
+                                            act, nv.stream()), "fbam_gated_few_rows")
+    flops.add(2.0 * rows * inner * (2 * depth + dim))
+    return y
 
 
 def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
     """``(y, x2, w1, w2, vg, h)``; the later ones for the backward."""
     inner, dim = w_out.shape[1], w_out.shape[0]
-    x2 = _dense(x.reshape(-1, x.shape[-1]))
-    res2 = None if residual is None else _dense(residual.reshape(-1, dim))
+    x2 = _dense(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    res2 = None if residual is None else _dense(residual if residual.dim() == 2 else residual.reshape(-1, dim))
     w1, w2, b1, _ = _wider(_dense(w_in), _dense(w_out), None if b_in is None else _dense(b_in), inner)
-    h, vg = _project(x2, w1, b1, act, keep)
-    y = gemm(h, w2, bias=None if b_out is None else _dense(b_out), residual=res2)
-    return y.view(*x.shape[:-1], dim), x2, w1, w2, vg, h
+    if b_out is not None:
+        b_out = _dense(b_out)
+    y = h = vg = None
+    if not keep and x2.shape[0] <= FEW_ROWS:
+        y = _few_rows(x2, w1, w2, b1, b_out, act, res2)
+    if y is None:
+        h, vg = _project(x2, w1, b1, act, keep)
+        y = gemm(h, w2, bias=b_out, residual=res2)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], dim), x2, w1, w2, vg, h
 
 
 class _GatedMlp(torch.autograd.Function):
@@ -99,17 +127,15 @@ class _GatedMlp(torch.autograd.Function):
         dy2 = _dense(dy.reshape(-1, dim))
         dx = dw_in = dw_out = db_in = db_out = None
         if need[0] or need[1] or need[3]:
-            d_vg = _project_grad(dy2, w2, vg, act)
+            d_vg, db_in = _project_grad(dy2, w2, vg, act, need[3])
             if need[0]:
                 dx = gemm_nn(d_vg, w1).view(shape)
             if need[1]:
                 dw_in = gemm_tn(d_vg, x2, splits=weight_grad_splits(2 * wide, x2.shape[1], rows))
                 if wide != inner:
                     dw_in = dw_in.view(2, wide, -1)[:, :inner].reshape(2 * inner, -1)
-            if need[3]:
-                db_in = _bias_grad(d_vg)
-                if wide != inner:
-                    db_in = db_in.view(2, wide)[:, :inner].reshape(-1)
+            if need[3] and wide != inner:
+                db_in = db_in.view(2, wide)[:, :inner].reshape(-1)
         if need[2]:
             dw_out = gemm_tn(dy2, h, splits=weight_grad_splits(dim, wide, rows))
             if wide != inner:
