@@ -31,6 +31,7 @@
 // its matmul pass selects (src/passes/matmul_pass.cpp:2783-3468), and conv2d fprop / dgrad / wgrad with
 // accumulation (cutlass_codegen/conv2d_cutlass_kernel.cu, kernels/conv2d.py:72-190, kernels/conv2d_bwd.py:6-232;
 // dispatch in src/passes/conv2d_pass.cpp).
+#include <string.h>
 #include "gemm_tcgen05.h"
 #include "gemm_out_maps.h"
 #include <cstddef>
@@ -706,6 +707,41 @@ extern "C" int fbam_gemm(const void* A, long long lda, int a_mn_major, const voi
   else e = encode_2d(&mb, B, N, K, ldb, bn);
   if (e) return e;
   return dispatch(BM, bn, ma, mb, p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int fbam_gemm2(const void* A, long long lda, int a_mn_major, const void* B, long long ldb, int b_mn_major, int M, int N,
+                          int K, GemmParams* params, void* stream);                                  // gemm2_tcgen05.cu
+extern "C" int fbam_slab_reduce(const void* work, void* out, long long n, int slabs, int out_elem, void* stream);   // embconv.cu
+
+// A product of elements into elements with the launchers' own choices, for callers that take no other option: D = A Bᵀ + bias +
+// residual, or with splits > 1 split along K over `slabs` ([splits][M * N] fp32; then no bias or residual, D dense).
+extern "C" int fbam_product(const void* A, long long lda, int a_mn_major, const void* B, long long ldb, int b_mn_major, int M, int N,
+                            int K, void* D, long long ldd, const void* bias, const void* residual, long long ldr, float* slabs,
+                            int splits, int* status, void* stream) {
+  GemmParams p;
+  memset(&p, 0, sizeof(p));
+  p.status = status;
+  p.alpha = 1.0f;
+  p.residual_scale = 1.0f;
+  if (splits > 1) {
+    if (slabs == nullptr || bias != nullptr || residual != nullptr || ldd != N) return GEMM_ERR_SHAPE;
+    p.D = slabs;
+    p.ldd = N;
+    p.split_workspace = slabs;
+    p.split_stride = (long long)M * N;
+    p.out_fp32 = 1;
+    p.splits = splits;
+    const int e = fbam_gemm(A, lda, a_mn_major, B, ldb, b_mn_major, M, N, K, &p, stream);
+    return e ? e : fbam_slab_reduce(slabs, D, (long long)M * N, splits, 1, stream);
+  }
+  p.D = D;
+  p.ldd = ldd;
+  p.bias = bias;
+  p.residual = reinterpret_cast<const elem_t*>(residual);
+  p.ldr = ldr;
+  // pairs where 256-row tiles fill the machine
+  const bool pair = N >= 256 && N % 16 == 0 && (long long)((M + 255) / 256) * ((N + 255) / 256) >= 148;
+  return (pair ? fbam_gemm2 : fbam_gemm)(A, lda, a_mn_major, B, ldb, b_mn_major, M, N, K, &p, stream);
 }
 
 // Implicit-GEMM convolution pass.  `X` is the gathered NHWC tensor [batch, in_h, in_w, C]; `Wmat` is the
