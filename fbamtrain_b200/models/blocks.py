@@ -95,6 +95,19 @@ class Embedding(nn.Module):
         return out * valid.unsqueeze(-1).to(out.dtype)
 
 
+class TokenEmbedding(nn.Module):
+    """Scaled row lookup ``scale · weight[ids]`` on the sorted-gradient kernels; ids outside the table give zeros."""
+
+    def __init__(self, rows: int, dim: int, dtype: torch.dtype, seeds: SeedSequence, scale: float = 1.0):
+        super().__init__()
+        self.scale = scale
+        self.weight = nn.Parameter(torch.empty(rows, dim, dtype=dtype))
+        fill_uniform_fan_(self.weight.data, dim, seeds)
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return ops.embed_tokens(ids, self.weight, self.scale)
+
+
 class Mean(nn.Module):
     """Mean over one dimension with fp32 accumulation (reference: ``tensorlib/include/mean.h:13-138``)."""
 
@@ -114,6 +127,23 @@ class MlpBlock(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor = None) -> torch.Tensor:
         return self.fc2(self.fc1(x), residual)
+
+
+class GatedMlp(nn.Module):
+    """``W_out · (v · act(g))`` with ``(v, g) = W_in · x``; the value rows of ``w_in`` come first."""
+
+    def __init__(self, dim: int, inner: int, bias: bool, dtype: torch.dtype, seeds: SeedSequence, act: str = "gelu"):
+        super().__init__()
+        self.act = act
+        self.w_in = nn.Parameter(torch.empty(2 * inner, dim, dtype=dtype))
+        self.w_out = nn.Parameter(torch.empty(dim, inner, dtype=dtype))
+        fill_uniform_fan_(self.w_in.data, dim, seeds)
+        fill_uniform_fan_(self.w_out.data, inner, seeds)
+        self.b_in = nn.Parameter(torch.zeros(2 * inner, dtype=dtype)) if bias else None
+        self.b_out = nn.Parameter(torch.zeros(dim, dtype=dtype)) if bias else None
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor = None) -> torch.Tensor:
+        return ops.gated_mlp(x, self.w_in, self.w_out, self.b_in, self.b_out, self.act, residual)
 
 
 class FullMhaAttention(nn.Module):
