@@ -31,12 +31,12 @@ __device__ __forceinline__ float to_f(elem_t x) { return e2f(x); }
 __device__ __forceinline__ void from_f(float* p, float x) { *p = x; }
 __device__ __forceinline__ void from_f(elem_t* p, float x) { *p = f2e(x); }
 
-// VEC logits as they lie in memory: 16 bytes, or one.
+// VEC logits as they lie in memory, 16 bytes.
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Raw {
   T v[VEC];
   __device__ __forceinline__ void get(float (&x)[VEC]) const {
-    if constexpr (sizeof(T) == 2 && VEC == 8) {
+    if constexpr (sizeof(T) == 2) {
       const elem2_t* a = reinterpret_cast<const elem2_t*>(v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -50,7 +50,7 @@ struct alignas(sizeof(T) * VEC) Raw {
     }
   }
   __device__ __forceinline__ void set(const float (&x)[VEC]) {
-    if constexpr (sizeof(T) == 2 && VEC == 8) {
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) reinterpret_cast<elem2_t*>(v)[i] = ff2e2(x[2 * i], x[2 * i + 1]);
     } else {
@@ -61,7 +61,7 @@ struct alignas(sizeof(T) * VEC) Raw {
   // of two vectors, the larger of each place; a NaN is not taken where there is a number
   __device__ __forceinline__ Raw max(const Raw& o) const {
     Raw r;
-    if constexpr (sizeof(T) == 2 && VEC == 8) {
+    if constexpr (sizeof(T) == 2) {
       const elem2_t *a = reinterpret_cast<const elem2_t*>(v), *b = reinterpret_cast<const elem2_t*>(o.v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) reinterpret_cast<elem2_t*>(r.v)[i] = __hmax2(a[i], b[i]);
@@ -72,7 +72,7 @@ struct alignas(sizeof(T) * VEC) Raw {
     return r;
   }
   __device__ __forceinline__ float top() const {
-    if constexpr (sizeof(T) == 2 && VEC == 8) {
+    if constexpr (sizeof(T) == 2) {
       const elem2_t* a = reinterpret_cast<const elem2_t*>(v);
       const float2 f = e22ff(__hmax2(__hmax2(a[0], a[1]), __hmax2(a[2], a[3])));
       return fmaxf(f.x, f.y);
@@ -87,14 +87,18 @@ struct alignas(sizeof(T) * VEC) Raw {
 template <typename T, int VEC>
 __device__ __forceinline__ Raw<T, VEC> load_raw(const T* p) {
   Raw<T, VEC> r;
-  if constexpr (sizeof(T) * VEC == 16) *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
-  else r.v[0] = p[0];
+  *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
   return r;
 }
+// The same without a line in L1, which the forward's one reading of a row has no use for (1001 x 100003 fp32: 84 -> 76 us,
+// 16384 x 6000 80 -> 70; the backward is no faster with it).
 template <typename T, int VEC>
-__device__ __forceinline__ void store_raw(T* p, const Raw<T, VEC>& r) {
-  if constexpr (sizeof(T) * VEC == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
-  else p[0] = r.v[0];
+__device__ __forceinline__ Raw<T, VEC> stream_raw(const T* p) {
+  Raw<T, VEC> r;
+  uint4 t;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(t.x), "=r"(t.y), "=r"(t.z), "=r"(t.w) : "l"(p));
+  *reinterpret_cast<uint4*>(&r) = t;
+  return r;
 }
 
 // Packed pairs (sm_100 computes on two fp32 values per instruction)
@@ -131,17 +135,20 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
+// Vectors of a row start on 16-byte boundaries whatever the row's start: `lead` places of the first one lie in front of the row.
 template <typename T, int VEC>
 struct Row {
   const T* p;
-  int vocab;
-  // the VEC logits from j on; -inf behind the end of the row
+  int vocab, lead;
+  __device__ __forceinline__ Row(const T* row, int n) : p(row), vocab(n), lead((int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))) {}
+  __device__ __forceinline__ bool has(long long j) const { return j >= 0 && j < vocab; }
+  // the VEC logits from j on; -inf outside the row
   __device__ __forceinline__ Raw<T, VEC> load(long long j) const {
-    if (j + VEC <= vocab) return load_raw<T, VEC>(p + j);
+    if (j >= 0 && j + VEC <= vocab) return load_raw<T, VEC>(p + j);
     Raw<T, VEC> r;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      if (j + i < vocab) r.v[i] = p[j + i];
+      if (has(j + i)) r.v[i] = p[j + i];
       else from_f(&r.v[i], -INFINITY);
     }
     return r;
@@ -177,9 +184,8 @@ __device__ __forceinline__ unsigned long long cluster_read(const unsigned long l
   return v;
 }
 
-// Vectors that a thread has on their way at once: 32 logits, or 8 of an unaligned row.
 template <int VEC>
-constexpr int kBatchOf = VEC == 8 ? 4 : 8;
+constexpr int kBatchOf = 32 / VEC;  // vectors that a thread has on their way at once
 constexpr int kMaxTop = 32, kMaxCtas = 8;
 constexpr uint32_t kNothing = 0x007fffffu;    // order_key(-inf)
 
@@ -192,8 +198,8 @@ constexpr uint32_t kNothing = 0x007fffffu;    // order_key(-inf)
 // Where the list overflows, equal logits are taken in order, or each alternative is looked for in a pass of its own.
 //
 // Bound: reading the logits once, with the special-function unit close behind for 16-bit ones (one exponential a logit, 0.7 of
-// the time of the reading).  8192 x 4096 bf16 20 us (3.4 TB/s), 1001 x 100003 fp32 82 us (4.9 TB/s), 16384 x 6000 fp32 77 us
-// (5.1 TB/s).  Packed arithmetic, a whole batch of loads before the first use, 32 warps per SM; fetching a batch ahead in
+// the time of the reading).  8192 x 4096 bf16 20 us (3.4 TB/s), 1001 x 100003 fp32 72 us (5.5 TB/s), 16384 x 6000 fp32 66 us
+// (6.0 TB/s).  Packed arithmetic, a whole batch of loads before the first use, 32 warps per SM; fetching a batch ahead in
 // registers cost more warps than it hid (8192 x 4096: 24 -> 31).
 // With one warp a row, a CTA has ROWS rows, which share nothing.
 template <typename T, int VEC, int WARPS, int ROWS>
@@ -218,18 +224,18 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
   uint32_t* best_of = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned long long*>(smem_raw) + ROWS * (kMaxTop + candidates)) +
                       sub * batches * kThreads;               // [batches][kThreads]
   int& list_length = list_lengths[sub];
-  const Row<T, VEC> row{logits + r * ld, vocab};
+  const Row<T, VEC> row(logits + r * ld, vocab);
   const float c = inv_t * kLog2e;
   const long long hop = (long long)ctas * kThreads * VEC;     // from one vector of a thread to its next
-  const long long first = (long long)(rank * kThreads + tid) * VEC;
+  const long long first = (long long)(rank * kThreads + tid) * VEC - row.lead;
 
   Stats st{-INFINITY, 0.0f, 0.0f};
   uint32_t best = 0;
   auto fetch = [&](Raw<T, VEC> (&to)[kBatch], long long j) {
-    if (j + (kBatch - 1) * hop + VEC <= vocab) {
+    if (j >= 0 && j + (kBatch - 1) * hop + VEC <= vocab) {
       const T* p = row.p + j;
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) to[b] = load_raw<T, VEC>(p + b * hop);
+      for (int b = 0; b < kBatch; ++b) to[b] = stream_raw<T, VEC>(p + b * hop);
     } else {
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) to[b] = row.load(j + b * hop);
@@ -250,31 +256,22 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
     }
     if (top_x > st.m) st.move_to(top_x, c);
     const float m = fmaxf(st.m, kLowest);
-    if constexpr (VEC > 1) {
-      float2 s2 = both(0.0f), u2 = both(0.0f);
+    float2 s2 = both(0.0f), u2 = both(0.0f);
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        float x[VEC];
-        raw[b].get(x);
+    for (int b = 0; b < kBatch; ++b) {
+      float x[VEC];
+      raw[b].get(x);
 #pragma unroll
-        for (int q = 0; q < VEC; q += 2) {
-          const float2 d = __fadd2_rn(make_float2(x[q], x[q + 1]), both(-m));
-          const float2 w = __fmul2_rn(d, both(c));
-          const float2 e = make_float2(ex2(w.x), ex2(w.y));      // NaN for a NaN, 0 for -inf
-          s2 = __fadd2_rn(s2, e);
-          u2 = __ffma2_rn(e, make_float2(fmaxf(d.x, kFar), fmaxf(d.y, kFar)), u2);
-        }
-      }
-      st.s += s2.x + s2.y;
-      st.u += u2.x + u2.y;
-    } else {
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const float d = to_f(raw[b].v[0]) - m, e = ex2(d * c);
-        st.s += e;
-        st.u = fmaf(e, fmaxf(d, kFar), st.u);
+      for (int q = 0; q < VEC; q += 2) {
+        const float2 d = __fadd2_rn(make_float2(x[q], x[q + 1]), both(-m));
+        const float2 w = __fmul2_rn(d, both(c));
+        const float2 e = make_float2(ex2(w.x), ex2(w.y));        // NaN for a NaN, 0 for -inf
+        s2 = __fadd2_rn(s2, e);
+        u2 = __ffma2_rn(e, make_float2(fmaxf(d.x, kFar), fmaxf(d.y, kFar)), u2);
       }
     }
+    st.s += s2.x + s2.y;
+    st.u += u2.x + u2.y;
   }
   // of the warp: one move to its maximum, then sums
   float top_m = st.m;
@@ -358,8 +355,9 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
         raw[b].get(x);
 #pragma unroll
         for (int q = 0; q < VEC; ++q) reach |= x[q] >= least ? 1u << q : 0u;
-      } else if (j < vocab) {
-        reach = (1u << min((long long)VEC, vocab - j)) - 1;
+      } else {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) reach |= row.has(j + q) ? 1u << q : 0u;
       }
       while (reach != 0) {
         const int q = __ffs(reach) - 1;
@@ -398,7 +396,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
         row.load(j).get(x);
 #pragma unroll
         for (int q = 0; q < VEC; ++q)
-          if (j + q < vocab && order_key(x[q]) > bound) {
+          if (row.has(j + q) && order_key(x[q]) > bound) {
             const int at = atomicAdd(&list_length, 1);
             if (at < candidates) list[at] = entry(x[q], j + q);
           }
@@ -417,7 +415,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
         row.load(j).get(x);
         uint32_t equal = 0;
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) equal |= j + q < vocab && order_key(x[q]) == bound ? 1u << q : 0u;
+        for (int q = 0; q < VEC; ++q) equal |= row.has(j + q) && order_key(x[q]) == bound ? 1u << q : 0u;
         const int mine = __popc(equal);
         int upto = mine;                                      // of this warp's lanes up to this one
 #pragma unroll
@@ -450,7 +448,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
         row.load(j).get(x);
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-          const unsigned long long e = j + q < vocab ? entry(x[q], j + q) : 0;
+          const unsigned long long e = row.has(j + q) ? entry(x[q], j + q) : 0;
           if (e < last && e > mine) mine = e;
         }
       }
@@ -503,10 +501,10 @@ logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const long long*
   const unsigned long long w = ((unsigned long long)blockIdx.x * 256 + threadIdx.x) / 32;
   const long long r = w / parts;
   if (r >= rows) return;
-  const Row<T, VEC> row{logits + r * ld, vocab};
-  const int j0 = (int)(w % parts) * (32 * VEC * kBatch) + threadIdx.x % 32 * VEC;
+  const Row<T, VEC> row(logits + r * ld, vocab);
+  const int j0 = (int)(w % parts) * (32 * VEC * kBatch) + threadIdx.x % 32 * VEC - row.lead;
   Raw<T, VEC> raw[kBatch];
-  if (j0 + (kBatch - 1) * 32 * VEC + VEC <= vocab) {
+  if (j0 >= 0 && j0 + (kBatch - 1) * 32 * VEC + VEC <= vocab) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) raw[b] = load_raw<T, VEC>(row.p + j0 + b * 32 * VEC);
   } else {
@@ -514,6 +512,7 @@ logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const long long*
     for (int b = 0; b < kBatch; ++b) raw[b] = row.load(j0 + b * 32 * VEC);
   }
   T* out = d_logits + r * d_ld;
+  const bool whole = (reinterpret_cast<uintptr_t>(out - row.lead) & 15) == 0;      // its vectors lie as the logits' do
   const float c = inv_t * kLog2e, m = stats[2 * r], log2_s = stats[2 * r + 1];
   const bool nothing = m == -INFINITY && log2_s == 0.0f;
   const long long t = targets != nullptr ? targets[r] : -1;
@@ -530,7 +529,7 @@ logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const long long*
     if (nothing) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) x[i] = 0.0f;
-    } else if constexpr (VEC > 1) {
+    } else {
 #pragma unroll
       for (int i = 0; i < VEC; i += 2) {
         const float2 lp = __ffma2_rn(__fadd2_rn(make_float2(x[i], x[i + 1]), both(-mm)), both(c), both(-log2_s));
@@ -539,28 +538,29 @@ logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const long long*
         x[i] = g.x;
         x[i + 1] = g.y;
       }
-    } else {
-      const float lp = fmaf(x[0] - mm, c, -log2_s);
-      x[0] = ex2(lp) * fmaf(b2, fmaxf(lp, kFar), a);
     }
-    if (t - j < VEC && t >= j) {                              // t below 2^31, or outside
+    if (valid && t - j < VEC && t >= j) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
         if (t == j + i) x[i] += dl;
     }
     Raw<T, VEC> g;
     g.set(x);
-    if (j + VEC <= vocab) {
-      store_raw<T, VEC>(out + j, g);
+    if (whole && j >= 0 && j + VEC <= vocab) {
+      *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<const uint4*>(&g);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (j + i < vocab) out[j + i] = g.v[i];
+        if (row.has(j + i)) out[j + i] = g.v[i];
     }
   }
 }
 
-bool aligned16(const void* p, long long ld, int size) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * size % 16 == 0; }
+// The largest Row::lead
+template <typename T>
+int most_lead(const void* p, long long ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * sizeof(T) % 16 == 0 ? 0 : 16 / sizeof(T) - 1;
+}
 
 struct FwdArgs {
   const void* logits;
@@ -574,7 +574,7 @@ struct FwdArgs {
 
 template <typename T, int VEC, int WARPS, int ROWS>
 int launch_fwd_w(const FwdArgs& a, int ctas, cudaStream_t s) {
-  const long long step = (long long)ctas * WARPS * 32 * VEC * kBatchOf<VEC>, batches = (a.vocab + step - 1) / step;
+  const long long step = (long long)ctas * WARPS * 32 * VEC * kBatchOf<VEC>, batches = (a.vocab + most_lead<T>(a.logits, a.ld) + step - 1) / step;
   const long long candidates = ROWS > 1 ? 256 : 1024, blocks = ROWS > 1 ? (a.rows + ROWS - 1) / ROWS : a.rows * ctas;
   const long long smem = a.top > 0 ? ROWS * ((candidates + kMaxTop) * 8 + batches * WARPS * 32 * 4) : 0;
   if (blocks > 0x7fffffffll || smem > 220 * 1024) return GEMM_ERR_SHAPE;
@@ -603,6 +603,7 @@ int launch_fwd_w(const FwdArgs& a, int ctas, cudaStream_t s) {
 //   1001 x 100003 fp32    4: 86 | 104   16: 88 | 115
 //   400 x 250001 bf16     4: 80 | 104   16: 61 | 79
 //   16 x 262144 bf16      4: 63 | 84    16: 27 | 35    2 CTAs: 18 | 31    8 CTAs: 13 | 23
+// (all with the logits going through L1)
 template <typename T, int VEC>
 int launch_fwd(const FwdArgs& a, cudaStream_t s) {
   constexpr int unit = 32 * VEC * kBatchOf<VEC>;
@@ -619,7 +620,7 @@ template <typename T, int VEC>
 int launch_bwd(const void* logits, long long ld, const long long* targets, const float* stats, const float* entropy,
                const float* d_logprob, const float* d_entropy, void* d_logits, long long d_ld, long long rows, int vocab,
                float inv_t, cudaStream_t s) {
-  const long long parts = ((long long)vocab + 32 * VEC * 4 - 1) / (32 * VEC * 4), blocks = (rows * parts + 7) / 8;
+  const long long parts = ((long long)vocab + most_lead<T>(logits, ld) + 32 * VEC * 4 - 1) / (32 * VEC * 4), blocks = (rows * parts + 7) / 8;
   if (blocks > 0x7fffffffll) return GEMM_ERR_SHAPE;
   logprobs_bwd_kernel<T, VEC><<<(unsigned)blocks, 256, 0, s>>>((const T*)logits, ld, targets, stats, entropy, d_logprob, d_entropy,
                                                                (T*)d_logits, d_ld, rows, vocab, inv_t, (unsigned)parts);
@@ -635,8 +636,7 @@ extern "C" int fbam_logprobs_fwd(const void* logits, int fp32, long long ld, con
                                  int vocab, int top, float inv_temperature, void* stream) {
   if (rows <= 0 || rows > 0x7fffffffll || vocab <= 0 || vocab > 0x3fffffff || top < 0 || top > vocab || top > kMaxTop) return GEMM_ERR_SHAPE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const bool vec = aligned16(logits, ld, fp32 ? 4 : 2);
-  auto f = fp32 ? (vec ? launch_fwd<float, 4> : launch_fwd<float, 1>) : (vec ? launch_fwd<elem_t, 8> : launch_fwd<elem_t, 1>);
+  auto f = fp32 ? launch_fwd<float, 4> : launch_fwd<elem_t, 8>;
   return f({logits, ld, targets, logprob, entropy, stats, top_logprobs, top_ids, rows, vocab, top, inv_temperature}, s);
 }
 
@@ -645,7 +645,6 @@ extern "C" int fbam_logprobs_bwd(const void* logits, int fp32, long long ld, con
                                  long long d_ld, long long rows, int vocab, float inv_temperature, void* stream) {
   if (rows <= 0 || vocab <= 0 || vocab > 0x3fffffff) return GEMM_ERR_SHAPE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const bool vec = aligned16(logits, ld, fp32 ? 4 : 2) && aligned16(d_logits, d_ld, fp32 ? 4 : 2);
-  auto f = fp32 ? (vec ? launch_bwd<float, 4> : launch_bwd<float, 1>) : (vec ? launch_bwd<elem_t, 8> : launch_bwd<elem_t, 1>);
+  auto f = fp32 ? launch_bwd<float, 4> : launch_bwd<elem_t, 8>;
   return f(logits, ld, targets, stats, entropy, d_logprob, d_entropy, d_logits, d_ld, rows, vocab, inv_temperature, s);
 }

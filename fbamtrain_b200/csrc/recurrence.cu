@@ -342,7 +342,8 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
   ex.init();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-  const int b = blockIdx.y, own = (blockIdx.x / ctas * 32 + lane) * VEC;
+  const int slabs = (s.dim + 32 * VEC - 1) / (32 * VEC), unit = blockIdx.x / ctas;
+  const int b = unit / slabs, own = (unit % slabs * 32 + lane) * VEC;
   const bool in = own < s.dim;
   const int ch = in ? own : s.dim - VEC;                    // lanes behind the last channel compute it too
   Vec<VEC> carry = state_in != nullptr ? load<VEC>(state_in + (long long)b * s.dim + ch) : Vec<VEC>::all(0.0f);
@@ -379,7 +380,8 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
   ex.init();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-  const int b = blockIdx.y, own = (blockIdx.x / ctas * 32 + lane) * VEC;
+  const int slabs = (s.dim + 32 * VEC - 1) / (32 * VEC), unit = blockIdx.x / ctas;
+  const int b = unit / slabs, own = (unit % slabs * 32 + lane) * VEC;
   const bool in = own < s.dim;
   const int ch = in ? own : s.dim - VEC;
   Vec<VEC> carry = d_state_out != nullptr ? load<VEC>(d_state_out + (long long)b * s.dim + ch) : Vec<VEC>::all(0.0f);
@@ -441,7 +443,8 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
   FwdSmem<STEPS>& sm = *reinterpret_cast<FwdSmem<STEPS>*>(smem_raw);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-  const int b = blockIdx.y, ch0 = blockIdx.x / ctas * kSlab, ch = ch0 + 2 * lane;
+  const int slabs = (s.dim + kSlab - 1) / kSlab, unit = blockIdx.x / ctas;
+  const int b = unit / slabs, ch0 = unit % slabs * kSlab, ch = ch0 + 2 * lane;
   const bool in = ch < s.dim;
   if (lane == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -532,7 +535,8 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
   BwdSmem<STEPS>& sm = *reinterpret_cast<BwdSmem<STEPS>*>(smem_raw);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-  const int b = blockIdx.y, ch0 = blockIdx.x / ctas * kSlab, ch = ch0 + 2 * lane;
+  const int slabs = (s.dim + kSlab - 1) / kSlab, unit = blockIdx.x / ctas;
+  const int b = unit / slabs, ch0 = unit % slabs * kSlab, ch = ch0 + 2 * lane;
   const bool in = ch < s.dim;
   if (lane == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&sm.full[warp][i], 1);
@@ -656,7 +660,8 @@ int launch(K kernel, int slab, int warps, int steps, int smem, const Shape& s, c
     return GEMM_ERR_LAUNCH;
   const int slabs = (s.dim + slab - 1) / slab, ctas = warps > 1 ? cluster_ctas(s, slabs, warps * steps) : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(slabs * ctas, s.batch);
+  if ((long long)slabs * ctas * s.batch > 0x7fffffffll) return GEMM_ERR_SHAPE;
+  cfg.gridDim = dim3((unsigned)(slabs * ctas * s.batch));
   cfg.blockDim = dim3(warps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -679,7 +684,7 @@ extern "C" int fbam_recurrence_chunk() { return kSaved; }
 extern "C" int fbam_recurrence_fwd(const void* zgo, long long zb, long long zt, long long zk, const float* state_in,
                                    const uint8_t* resets, long long rb, long long rt, void* y, long long yb, long long yt,
                                    float* state_out, float* saved, int batch, int steps, int dim, int* status, void* stream) {
-  if (batch <= 0 || steps <= 0 || dim <= 0 || batch > 65535 || steps > 0x3fffffff) return GEMM_ERR_SHAPE;
+  if (batch <= 0 || steps <= 0 || dim <= 0 || steps > 0x3fffffff) return GEMM_ERR_SHAPE;
   const Shape s{batch, steps, dim, (steps + kSaved - 1) / kSaved, zb, zt, zk, yb, yt, rb, rt};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (steps > kSaved && pieces(zgo, dim, zb, zt, zk) && pieces(y, dim, yb, yt, 8)) {
@@ -703,7 +708,7 @@ extern "C" int fbam_recurrence_bwd(const void* zgo, long long zb, long long zt, 
                                    long long rb, long long rt, const float* saved, const void* dy, long long yb, long long yt,
                                    const float* d_state_out, void* d_zgo, long long db, long long dt, float* d_state_in,
                                    int batch, int steps, int dim, int* status, void* stream) {
-  if (batch <= 0 || steps <= 0 || dim <= 0 || batch > 65535 || steps > 0x3fffffff) return GEMM_ERR_SHAPE;
+  if (batch <= 0 || steps <= 0 || dim <= 0 || steps > 0x3fffffff) return GEMM_ERR_SHAPE;
   const Shape s{batch, steps, dim, (steps + kSaved - 1) / kSaved, zb, zt, zk, yb, yt, rb, rt};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (steps > kSaved && pieces(zgo, dim, zb, zt, zk) && pieces(dy, dim, yb, yt, 8) && pieces(d_zgo, dim, db, dt, 8) &&

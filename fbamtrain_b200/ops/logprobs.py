@@ -45,9 +45,9 @@ class _TokenLogprobs(torch.autograd.Function):
         rows, vocab = logits.shape
         d_logprob = None if d_logprob is None else d_logprob.contiguous()
         d_entropy = None if d_entropy is None else d_entropy.contiguous()
-        # rows of whole 16-byte pieces, whatever the vocabulary
+        # rows that lie in their 16-byte pieces as the logits' do: dense where those are, else whole pieces
         per = 16 // logits.element_size()
-        width = (vocab + per - 1) // per * per
+        width = vocab if logits.stride(0) == vocab else (vocab + per - 1) // per * per
         d = torch.empty((rows, width), dtype=logits.dtype, device=logits.device)
         if rows:
             nv.check(nv.lib(logits).fbam_logprobs_bwd(logits.data_ptr(), logits.dtype == F32, logits.stride(0), nv.addr(targets),

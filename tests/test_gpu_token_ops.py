@@ -197,6 +197,20 @@ def test_recurrence_extreme_gates():
     oracle.within(last, want_last, F32, 1e-5)
 
 
+def test_recurrence_of_many_sequences():
+    """More sequences than one dimension of a grid has places, of one step each."""
+    b, d = 70_000, 24
+    gen = _gen("many")
+    zgo, state = _randn(gen, b, 1, 3, d, dtype=BF).requires_grad_(), _randn(gen, b, d)
+    y, last = ops.gated_recurrence(zgo, state)
+    want_y, want_last, _, _ = oracle.recurrence(zgo.detach(), state, None)
+    oracle.within(y, want_y, BF, 1e-5)
+    oracle.within(last, want_last, F32, 1e-5)
+    dy = _randn(gen, b, 1, d, dtype=BF)
+    g, = torch.autograd.grad((y,), (zgo,), (dy,))
+    oracle.within(g, oracle.recurrence_grad(zgo.detach(), state, None, dy, None)[0], BF, 1e-4)
+
+
 def test_recurrence_without_steps():
     state = torch.randn(3, 8, device="cuda")
     y, last = ops.gated_recurrence(torch.empty(3, 0, 3, 8, dtype=BF, device="cuda"), state)
@@ -396,6 +410,28 @@ def test_logprobs_shapes_and_parts():
     g2, = torch.autograd.grad((r.entropy,), (logits,), (torch.ones(6, 4, device="cuda"),))
     assert torch.equal(g, g2)
     assert ops.token_logprobs(logits[:0], t[:0], 2).top_ids.shape == (0, 4, 2)
+
+
+@pytest.mark.parametrize("vocab", [1, 5, 8, 31, 257, 4099, 50257])
+@pytest.mark.parametrize("start", [0, 1, 3])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_logprobs_rows_that_start_anywhere(vocab, start, dtype):
+    """Dense rows of odd lengths and views at odd starts: 16-byte pieces of a row begin in front of it."""
+    gen = _gen("starts", vocab, start)
+    rows, top = 7, min(vocab, 4)
+    flat = _randn(gen, rows * vocab + 8, dtype=dtype, scale=3.0)
+    flat[:start] = flat[start + rows * vocab:] = 1e4                  # neighbours that must not count
+    logits = flat[start:start + rows * vocab].view(rows, vocab).requires_grad_()
+    t = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    r = ops.token_logprobs(logits, t, top)
+    held = logits.detach()
+    lp, entropy, logp, _ = oracle.logprobs(held, t, 1.0)
+    oracle.within(r.logprob, lp, F32, 1e-5)
+    oracle.within(r.entropy, entropy, F32, 1e-5)
+    assert torch.equal(r.top_ids, oracle.alternatives(held, top))
+    dl, dh = _randn(gen, rows), _randn(gen, rows)
+    g, = torch.autograd.grad((r.logprob, r.entropy), (logits,), (dl, dh))
+    oracle.within(g, oracle.logprobs_grad(held, t, 1.0, dl, dh), dtype, 1e-4)
 
 
 def test_logprobs_gradient_against_differences():
