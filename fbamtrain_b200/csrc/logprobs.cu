@@ -343,6 +343,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
   const float least = key_value(bound);                       // no logit that reaches the bound is below it
   for (int i = 0; i < batches; ++i) {
     if (best_of[i * kThreads + tid] < max(bound, 1u)) continue;
+    if (*reinterpret_cast<volatile int*>(&list_length) > candidates) break;    // too many anyway
     const long long j0 = first + (long long)i * kBatch * hop;
     Raw<T, VEC> raw[kBatch];
     fetch(raw, j0);
