@@ -16,7 +16,7 @@ F32 = torch.float32
 
 def _forward(ids, flat, table, scale, out_dtype, elem):
     vocab, dim = table.shape
-    out = torch.empty((*ids.shape, dim), dtype=out_dtype, device=table.device)
+    out = table.new_empty((*ids.shape, dim), dtype=out_dtype)
     n = flat.numel()
     if n:
         nv.check(nv.lib(elem).fbam_embed_fwd(flat.data_ptr(), flat.dtype == torch.int64, table.data_ptr(), table.stride(0),
@@ -36,16 +36,16 @@ class _EmbedTokens(torch.autograd.Function):
     def backward(ctx, d_out):
         (flat,) = ctx.saved_tensors
         vocab, dim, dtype, elem, scale = ctx.meta
-        n, dev = flat.numel(), d_out.device
+        n = flat.numel()
         if n == 0:
-            return None, None, torch.zeros(vocab, dim, dtype=dtype, device=dev), None, None, None
+            return None, None, d_out.new_zeros((vocab, dim), dtype=dtype), None, None, None
         d_out = d_out.contiguous()
-        d_table = torch.empty(vocab, dim, dtype=dtype, device=dev)
+        d_table = d_out.new_empty((vocab, dim), dtype=dtype)
         lib = nv.lib(elem)
         words, floats = C.c_longlong(), C.c_longlong()
         lib.fbam_embed_bwd_workspace(n, vocab, dim, C.byref(words), C.byref(floats))
-        work = torch.empty(words.value, dtype=torch.int64, device=dev)
-        partial = torch.empty(floats.value, dtype=F32, device=dev)
+        work = flat.new_empty(words.value, dtype=torch.int64)
+        partial = d_out.new_empty(floats.value, dtype=F32)
         nv.check(lib.fbam_embed_bwd(flat.data_ptr(), flat.dtype == torch.int64, d_out.data_ptr(), d_out.dtype == F32,
                                     d_table.data_ptr(), dtype == F32, n, vocab, dim, scale, work.data_ptr(),
                                     partial.data_ptr(), nv.stream()), "fbam_embed_bwd")
@@ -55,7 +55,7 @@ class _EmbedTokens(torch.autograd.Function):
 def embed_tokens(ids, table, scale, out_dtype):
     if ids.device != table.device:
         raise ValueError(f"ids are on {ids.device}, the table on {table.device}")
-    flat = ids.reshape(-1)
+    flat = ids if ids.dim() == 1 else ids.reshape(-1)
     if not flat.is_contiguous():
         flat = flat.contiguous()
     if table.stride(1) != 1:

@@ -51,17 +51,16 @@ def _product(a, b, m, n, a_mn=False, b_mn=False, bias=None, residual=None, split
         return gemm(a, b, a_mn=a_mn, b_mn=b_mn, bias=bias, residual=residual, splits=splits)
     a, b = _tma_pitch(a), _tma_pitch(b)
     k = a.shape[0] if a_mn else a.shape[1]
-    dev = a.device
-    out = torch.empty((m, n), dtype=a.dtype, device=dev)
+    out = a.new_empty((m, n))
     slabs = None
     splits = min(splits, (k + 63) // 64)
     if splits > 1 and m * n % 8 == 0:
-        slabs = torch.empty((splits, m, n), dtype=torch.float32, device=dev)
+        slabs = a.new_empty((splits, m, n), dtype=torch.float32)
     else:
         splits = 0
     nv.check(nv.lib(a).fbam_product(a.data_ptr(), a.stride(0), a_mn, b.data_ptr(), b.stride(0), b_mn, m, n, k, out.data_ptr(), n,
                                     nv.addr(bias), nv.addr(residual), n, nv.addr(slabs), splits,
-                                    nv.status_word(dev).data_ptr(), nv.stream()), "fbam_product")
+                                    nv.status_word(a.device).data_ptr(), nv.stream()), "fbam_product")
     flops.add(2.0 * m * n * k)
     return out
 
@@ -70,8 +69,8 @@ def _project(x2, w1, b1, act, keep):
     """``(h, vg)``: the gated hidden values and, with ``keep``, both factors before the activation, ``(2, rows, inner)`` fp32."""
     rows, inner = x2.shape[0], w1.shape[0] // 2
     x2, w1 = _tma_pitch(x2), _tma_pitch(w1)
-    h = torch.empty((rows, inner), dtype=x2.dtype, device=x2.device)
-    vg = torch.empty((2, rows, inner), dtype=torch.float32, device=x2.device) if keep else None
+    h = x2.new_empty((rows, inner))
+    vg = x2.new_empty((2, rows, inner), dtype=torch.float32) if keep else None
     v, g = (vg[0].data_ptr(), vg[1].data_ptr()) if keep else (0, 0)
     nv.check(nv.lib(x2).fbam_gated_fwd(x2.data_ptr(), x2.stride(0), w1.data_ptr(), w1.stride(0), nv.addr(b1), h.data_ptr(), v, g,
                                        rows, inner, x2.shape[1], act, nv.status_word(x2.device).data_ptr(), nv.stream()),
@@ -83,14 +82,13 @@ def _project(x2, w1, b1, act, keep):
 def _project_grad(dy2, w2, vg, act, sums):
     """The gradient of the projection ``(rows, 2 · inner)``, values first, and with ``sums`` its column sums."""
     _, rows, inner = vg.shape
-    dev = dy2.device
     dy2, w2 = _tma_pitch(dy2), _tma_pitch(w2)
-    d_vg = torch.empty((rows, 2 * inner), dtype=dy2.dtype, device=dev)
-    work = torch.empty(((rows + 31) // 32, 2 * inner), dtype=torch.float32, device=dev) if sums else None
-    db = torch.empty(2 * inner, dtype=dy2.dtype, device=dev) if sums else None
+    d_vg = dy2.new_empty((rows, 2 * inner))
+    work = vg.new_empty(((rows + 31) // 32, 2 * inner)) if sums else None
+    db = dy2.new_empty(2 * inner) if sums else None
     nv.check(nv.lib(dy2).fbam_gated_bwd(dy2.data_ptr(), dy2.stride(0), w2.data_ptr(), w2.stride(0), vg[0].data_ptr(),
                                         vg[1].data_ptr(), d_vg.data_ptr(), nv.addr(work), nv.addr(db), rows, inner, dy2.shape[1],
-                                        act, nv.status_word(dev).data_ptr(), nv.stream()), "fbam_gated_bwd")
+                                        act, nv.status_word(dy2.device).data_ptr(), nv.stream()), "fbam_gated_bwd")
     flops.add(2.0 * rows * inner * dy2.shape[1])
     return d_vg, db
 
@@ -105,8 +103,7 @@ def _few_rows(x2, w1, w2, b1, b_out, act, res2):
     dim, inner = w2.shape
     if depth % 8 or (x2.data_ptr() | w1.data_ptr() | w2.data_ptr()) % 16:
         return None
-    h = torch.empty((rows, inner), dtype=x2.dtype, device=x2.device)
-    y = torch.empty((rows, dim), dtype=x2.dtype, device=x2.device)
+    h, y = x2.new_empty((rows, inner)), x2.new_empty((rows, dim))
     nv.check(nv.lib(x2).fbam_gated_few_rows(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b1), w2.data_ptr(), inner,
                                             nv.addr(b_out), nv.addr(res2), dim, h.data_ptr(), y.data_ptr(), rows, depth, inner, dim,
                                             act, nv.stream()), "fbam_gated_few_rows")

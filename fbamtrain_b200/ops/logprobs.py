@@ -12,14 +12,13 @@ F32 = torch.float32
 def _forward(logits, targets, top, inv_t, keep):
     """``(logprob, entropy, top logprobs, top ids, stats)``; ``stats`` with ``keep``: what the backward needs."""
     rows, vocab = logits.shape
-    dev = logits.device
-    logprob = None if targets is None else torch.empty(rows, dtype=F32, device=dev)
-    entropy = torch.empty(rows, dtype=F32, device=dev)
-    stats = torch.empty((rows, 2), dtype=F32, device=dev) if keep else None
+    entropy = logits.new_empty(rows, dtype=F32)
+    logprob = None if targets is None else torch.empty_like(entropy)
+    stats = entropy.new_empty((rows, 2)) if keep else None
     top_lp = top_ids = None
     if top:
-        top_lp = torch.empty((rows, top), dtype=F32, device=dev)
-        top_ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        top_lp = entropy.new_empty((rows, top))
+        top_ids = entropy.new_empty((rows, top), dtype=torch.int64)
     if rows:
         nv.check(nv.lib(logits).fbam_logprobs_fwd(logits.data_ptr(), logits.dtype == F32, logits.stride(0), nv.addr(targets),
                                                   nv.addr(logprob), entropy.data_ptr(), nv.addr(stats), nv.addr(top_lp),
@@ -48,7 +47,7 @@ class _TokenLogprobs(torch.autograd.Function):
         # rows that lie in their 16-byte pieces as the logits' do: dense where those are, else whole pieces
         per = 16 // logits.element_size()
         width = vocab if logits.stride(0) == vocab else (vocab + per - 1) // per * per
-        d = torch.empty((rows, width), dtype=logits.dtype, device=logits.device)
+        d = logits.new_empty((rows, width))
         if rows:
             nv.check(nv.lib(logits).fbam_logprobs_bwd(logits.data_ptr(), logits.dtype == F32, logits.stride(0), nv.addr(targets),
                                                       stats.data_ptr(), entropy.data_ptr(), nv.addr(d_logprob),
@@ -64,7 +63,7 @@ def token_logprobs(logits, targets, top, temperature):
     flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     if flat.stride(1) != 1:
         flat = flat.contiguous()
-    if targets is not None:
+    if targets is not None and not (targets.dim() == 1 and targets.dtype == torch.int64 and targets.is_contiguous()):
         targets = targets.reshape(-1).long().contiguous()
     if flat.requires_grad and torch.is_grad_enabled():
         out = _TokenLogprobs.apply(flat, targets, top, 1.0 / temperature)

@@ -18,8 +18,8 @@ def _ordered_like(x: torch.Tensor, *inner: int) -> torch.Tensor:
     """An empty ``(B, T, *inner)`` tensor that is time-major in memory where ``x`` is."""
     b, t = x.shape[:2]
     if b > 1 and x.stride(0) < x.stride(1):
-        return torch.empty((t, b, *inner), dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty((b, t, *inner), dtype=x.dtype, device=x.device)
+        return x.new_empty((t, b, *inner)).transpose(0, 1)
+    return x.new_empty((b, t, *inner))
 
 
 def _forward(zgo, state, resets, keep):
@@ -27,12 +27,12 @@ def _forward(zgo, state, resets, keep):
     b, t, _, d = zgo.shape
     dev = zgo.device
     y = _ordered_like(zgo, d)
-    out = torch.empty((b, d), dtype=F32, device=dev)
+    out = zgo.new_empty((b, d), dtype=F32) if state is None else torch.empty_like(state)
     lib = nv.lib(zgo)
     saved = None
     if keep:
         chunk = lib.fbam_recurrence_chunk()
-        saved = torch.empty((b, (t + chunk - 1) // chunk, d), dtype=F32, device=dev)
+        saved = out.new_empty((b, (t + chunk - 1) // chunk, d))
     zb, zt, zk, _ = zgo.stride()
     yb, yt, _ = y.stride()
     rb, rt = (0, 0) if resets is None else resets.stride()
@@ -56,13 +56,13 @@ class _GatedRecurrence(torch.autograd.Function):
         b, t, _, d = zgo.shape
         dev = zgo.device
         if dy is None:
-            dy = torch.zeros(b, t, d, dtype=zgo.dtype, device=dev)
+            dy = zgo.new_zeros((b, t, d))
         elif dy.stride(2) != 1:
             dy = dy.contiguous()
         if d_out is not None:
             d_out = d_out.contiguous()
         d_zgo = _ordered_like(zgo, 3, d)
-        d_state = torch.empty((b, d), dtype=F32, device=dev) if ctx.needs_input_grad[1] else None
+        d_state = saved.new_empty((b, d)) if ctx.needs_input_grad[1] else None
         zb, zt, zk, _ = zgo.stride()
         yb, yt, _ = dy.stride()
         db, dt, _, _ = d_zgo.stride()
