@@ -678,3 +678,65 @@ extern "C" int fbam_gated_few_rows(const void* x, long long ldx, const void* w_i
   return launch_few<false>({(const elem_t*)h, (const elem_t*)w_out, (const elem_t*)b_out, (const elem_t*)residual, (elem_t*)y, inner,
                             ld_out, ldr, rows, out_dim, inner, act}, s);
 }
+
+extern "C" int fbam_product(const void* A, long long lda, int a_mn_major, const void* B, long long ldb, int b_mn_major, int M, int N,
+                            int K, void* D, long long ldd, const void* bias, const void* residual, long long ldr, float* slabs,
+                            int splits, int* status, void* stream);                                  // gemm_tcgen05.cu
+extern "C" int fbam_colsum_to(const void* x, const void* z, void* dz, void* out, int out_elem, float* work, long long rows, int cols,
+                              void* stream);                                                         // kernels_simt.cu
+
+// The block's forward: fbam_gated_fwd, and where y is not null y (rows, out_dim) = h W_outᵀ + b_out + residual, dense.
+extern "C" int fbam_gated_block_fwd(const void* x, long long ldx, const void* w_in, long long ld_in, const void* b_in, const void* w_out,
+                                    long long ld_out, const void* b_out, const void* residual, void* h, float* v, float* g, void* y,
+                                    int rows, int inner, int depth, int out_dim, int act, int* status, void* stream) {
+  const int e = fbam_gated_fwd(x, ldx, w_in, ld_in, b_in, h, v, g, rows, inner, depth, act, status, stream);
+  if (e || y == nullptr) return e;
+  return fbam_product(h, inner, 0, w_out, ld_out, 0, rows, out_dim, inner, y, out_dim, b_out, residual, out_dim, nullptr, 0, status, stream);
+}
+
+// The block's backward; a gradient whose pointer is null is not wanted.  hidden, the inner width without its padding, is the width
+// of d_w_out; dx has width columns of the depth.  slabs: [splits][..] fp32 for a weight gradient that is split along the rows.
+// d_b_out: out_dim rounded up to 8, dy then dense and that wide; col_work as fbam_colsum_partials says.
+extern "C" int fbam_gated_block_bwd(const void* dy, long long ldy, const void* x, long long ldx, const void* w_in, long long ld_in,
+                                    const void* w_out, long long ld_out, const float* v, const float* g, const void* h, void* d_vg,
+                                    float* col_sums, void* d_b_in, void* dx, void* d_w_in, void* d_w_out, void* d_b_out, float* col_work,
+                                    float* slabs_in, int splits_in, float* slabs_out, int splits_out, int rows, int inner, int hidden,
+                                    int depth, int width, int out_dim, int act, int* status, void* stream) {
+  int e = 0;
+  if (d_vg != nullptr)
+    e = fbam_gated_bwd(dy, ldy, w_out, ld_out, v, g, d_vg, col_sums, d_b_in, rows, inner, out_dim, act, status, stream);
+  if (!e && dx != nullptr)
+    e = fbam_product(d_vg, 2ll * inner, 0, w_in, ld_in, 1, rows, width, 2 * inner, dx, width, nullptr, nullptr, 0, nullptr, 0, status, stream);
+  if (!e && d_w_in != nullptr)
+    e = fbam_product(d_vg, 2ll * inner, 1, x, ldx, 1, 2 * inner, width, rows, d_w_in, width, nullptr, nullptr, 0, slabs_in, splits_in, status,
+                     stream);
+  if (!e && d_w_out != nullptr)
+    e = fbam_product(dy, ldy, 1, h, inner, 1, out_dim, hidden, rows, d_w_out, hidden, nullptr, nullptr, 0, slabs_out, splits_out, status,
+                     stream);
+  if (!e && d_b_out != nullptr) e = fbam_colsum_to(dy, nullptr, nullptr, d_b_out, 1, col_work, rows, (out_dim + 7) / 8 * 8, stream);
+  return e;
+}
+
+namespace {
+__global__ void __launch_bounds__(256)
+refit_kernel(const elem_t* __restrict__ src, long long ld, elem_t* __restrict__ dst, int src_rows, int src_cols, int dst_rows, int dst_cols,
+             long long total) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / dst_cols;
+    const int c = (int)(i - row * dst_cols);
+    const long long block = row / dst_rows;
+    const int r = (int)(row - block * dst_rows);
+    dst[i] = r < src_rows && c < src_cols ? src[(block * src_rows + r) * ld + c] : f2e(0.0f);
+  }
+}
+}  // namespace
+
+// blocks of src_rows x src_cols (pitch ld) -> dense blocks of dst_rows x dst_cols: padded with zeros, or cut.
+extern "C" int fbam_refit(const void* src, long long ld, void* dst, int blocks, int src_rows, int src_cols, int dst_rows, int dst_cols,
+                          void* stream) {
+  const long long total = (long long)blocks * dst_rows * dst_cols, need = (total + 255) / 256;
+  if (blocks <= 0 || src_rows < 0 || src_cols < 0 || dst_rows <= 0 || dst_cols <= 0) return GEMM_ERR_SHAPE;
+  refit_kernel<<<(unsigned)(need < 148 * 16 ? need : 148 * 16), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      (const elem_t*)src, ld, (elem_t*)dst, src_rows, src_cols, dst_rows, dst_cols, total);
+  return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+}

@@ -1,5 +1,8 @@
-"""Gated feed-forward block on the tcgen05 GEMMs (``csrc/gated_mlp.cu``): ``y = (v · act(g)) W_outᵀ + b_out + residual``
-with ``(v, g) = x W_inᵀ + b_in``; the first half of the projection is the value and the second the gate, as in ``geglu``.
+"""Gated feed-forward block on the tensor cores (``csrc/gated_mlp.cu``): ``y = (v · act(g)) W_outᵀ + b_out + residual`` with
+``(v, g) = x W_inᵀ + b_in``; the first half of the projection is the value and the second the gate, as in ``geglu``.
+
+Widths that are no multiple of 8 are refitted: rows of ``x``, the weights and ``dy`` get zeros up to the next one (tensor maps
+want 16-byte rows), which add nothing to any product.
 """
 from __future__ import annotations
 
@@ -8,124 +11,79 @@ import torch
 from ..utils import flops
 from . import native as nv
 from . import tuning
-from .native_ops import _colsum, _need_elem, _tma_pitch, gemm, weight_grad_splits
+from .native_ops import _need_elem, _sum_partials, gemm, weight_grad_splits
 
 GATES = {"gelu": 0, "silu": 1}
+F32 = torch.float32
+
+# Rows up to which the weights are streamed past the rows instead of tiled.  us, streamed | tiled: 8 x 1024 x 4096 17 | 36, 32 x
+# 1024 x 4096 24 | 34, 8 x 2048 x 8192 34 | 71, 32 x 2048 x 8192 54 | 60.
+FEW_ROWS = 32
+
+
+def _up8(n: int) -> int:
+    return (n + 7) // 8 * 8
 
 
 def _dense(x: torch.Tensor) -> torch.Tensor:
     return x if x.is_contiguous() else x.contiguous()
 
 
-def _wider(w_in, w_out, b_in, inner: int):
-    """The weights with the inner width padded to a multiple of 8 by zero rows and columns, which add nothing: 16-byte rows
-    for the tensor maps."""
-    wide = (inner + 7) // 8 * 8
-    if wide == inner:
-        return w_in, w_out, b_in, inner
-    dim = w_in.shape[1]
-    w1 = w_in.new_zeros(2, wide, dim)
-    w1[:, :inner] = w_in.view(2, inner, dim)
-    w2 = w_out.new_zeros(w_out.shape[0], wide)
-    w2[:, :inner] = w_out
-    if b_in is not None:
-        b1 = b_in.new_zeros(2, wide)
-        b1[:, :inner] = b_in.view(2, inner)
-        b_in = b1.view(-1)
-    return w1.view(2 * wide, dim), w2, b_in, wide
+def _flat(x: torch.Tensor) -> torch.Tensor:
+    """The rows of ``x``, dense, the first one on a 16-byte boundary."""
+    x = _dense(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    return x.clone() if x.data_ptr() % 16 else x
 
 
-def _bias_grad(d: torch.Tensor) -> torch.Tensor:
-    """Column sums; the kernel takes columns in eights."""
-    rows, cols = d.shape
-    if cols % 8:
-        wide = d.new_zeros(rows, (cols + 7) // 8 * 8)
-        wide[:, :cols] = d
-        return _colsum(wide, d.dtype)[:cols]
-    return _colsum(d, d.dtype)
-
-
-def _product(a, b, m, n, a_mn=False, b_mn=False, bias=None, residual=None, splits=0):
-    """:func:`gemm` with the launchers' own choices, which cost a short call less time to pass on."""
-    if tuning.active():
-        return gemm(a, b, a_mn=a_mn, b_mn=b_mn, bias=bias, residual=residual, splits=splits)
-    a, b = _tma_pitch(a), _tma_pitch(b)
-    k = a.shape[0] if a_mn else a.shape[1]
-    out = a.new_empty((m, n))
-    slabs = None
-    splits = min(splits, (k + 63) // 64)
-    if splits > 1 and m * n % 8 == 0:
-        slabs = a.new_empty((splits, m, n), dtype=torch.float32)
-    else:
-        splits = 0
-    nv.check(nv.lib(a).fbam_product(a.data_ptr(), a.stride(0), a_mn, b.data_ptr(), b.stride(0), b_mn, m, n, k, out.data_ptr(), n,
-                                    nv.addr(bias), nv.addr(residual), n, nv.addr(slabs), splits,
-                                    nv.status_word(a.device).data_ptr(), nv.stream()), "fbam_product")
-    flops.add(2.0 * m * n * k)
+def _refit(src: torch.Tensor, blocks: int, rows: int, cols: int) -> torch.Tensor:
+    """``src`` as ``blocks`` blocks of rows, each cut or padded with zeros to ``(rows, cols)``."""
+    out = src.new_empty((blocks * rows, cols))
+    nv.check(nv.lib(src).fbam_refit(src.data_ptr(), src.stride(0), out.data_ptr(), blocks, src.shape[0] // blocks, src.shape[1],
+                                    rows, cols, nv.stream()), "fbam_refit")
     return out
 
 
-def _project(x2, w1, b1, act, keep):
-    """``(h, vg)``: the gated hidden values and, with ``keep``, both factors before the activation, ``(2, rows, inner)`` fp32."""
-    rows, inner = x2.shape[0], w1.shape[0] // 2
-    x2, w1 = _tma_pitch(x2), _tma_pitch(w1)
-    h = x2.new_empty((rows, inner))
-    vg = x2.new_empty((2, rows, inner), dtype=torch.float32) if keep else None
-    v, g = (vg[0].data_ptr(), vg[1].data_ptr()) if keep else (0, 0)
-    nv.check(nv.lib(x2).fbam_gated_fwd(x2.data_ptr(), x2.stride(0), w1.data_ptr(), w1.stride(0), nv.addr(b1), h.data_ptr(), v, g,
-                                       rows, inner, x2.shape[1], act, nv.status_word(x2.device).data_ptr(), nv.stream()),
-             "fbam_gated_fwd")
-    flops.add(4.0 * rows * inner * x2.shape[1])
-    return h, vg
-
-
-def _project_grad(dy2, w2, vg, act, sums):
-    """The gradient of the projection ``(rows, 2 · inner)``, values first, and with ``sums`` its column sums."""
-    _, rows, inner = vg.shape
-    dy2, w2 = _tma_pitch(dy2), _tma_pitch(w2)
-    d_vg = dy2.new_empty((rows, 2 * inner))
-    work = vg.new_empty(((rows + 31) // 32, 2 * inner)) if sums else None
-    db = dy2.new_empty(2 * inner) if sums else None
-    nv.check(nv.lib(dy2).fbam_gated_bwd(dy2.data_ptr(), dy2.stride(0), w2.data_ptr(), w2.stride(0), vg[0].data_ptr(),
-                                        vg[1].data_ptr(), d_vg.data_ptr(), nv.addr(work), nv.addr(db), rows, inner, dy2.shape[1],
-                                        act, nv.status_word(dy2.device).data_ptr(), nv.stream()), "fbam_gated_bwd")
-    flops.add(2.0 * rows * inner * dy2.shape[1])
-    return d_vg, db
-
-
-# Rows up to which the weights are streamed past the rows instead of tiled.
-FEW_ROWS = 32
-
-
-def _few_rows(x2, w1, w2, b1, b_out, act, res2):
-    """The block on up to ``FEW_ROWS`` rows, or None where a row does not start on a 16-byte boundary."""
-    rows, depth = x2.shape
-    dim, inner = w2.shape
-    if depth % 8 or (x2.data_ptr() | w1.data_ptr() | w2.data_ptr()) % 16:
-        return None
-    h, y = x2.new_empty((rows, inner)), x2.new_empty((rows, dim))
-    nv.check(nv.lib(x2).fbam_gated_few_rows(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b1), w2.data_ptr(), inner,
-                                            nv.addr(b_out), nv.addr(res2), dim, h.data_ptr(), y.data_ptr(), rows, depth, inner, dim,
-                                            act, nv.stream()), "fbam_gated_few_rows")
-    flops.add(2.0 * rows * inner * (2 * depth + dim))
-    return y
-
-
 def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
-    """``(y, x2, w1, w2, vg, h)``; the later ones for the backward."""
-    inner, dim = w_out.shape[1], w_out.shape[0]
-    x2 = _dense(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
-    res2 = None if residual is None else _dense(residual if residual.dim() == 2 else residual.reshape(-1, dim))
-    w1, w2, b1, _ = _wider(_dense(w_in), _dense(w_out), None if b_in is None else _dense(b_in), inner)
-    if b_out is not None:
-        b_out = _dense(b_out)
-    y = h = vg = None
-    if not keep and x2.shape[0] <= FEW_ROWS:
-        y = _few_rows(x2, w1, w2, b1, b_out, act, res2)
-    if y is None:
-        h, vg = _project(x2, w1, b1, act, keep)
-        y = _product(h, w2, x2.shape[0], dim, bias=b_out, residual=res2)
+    """``(y, x2, w1, w2, vg, h)``; the later ones for the backward, in their padded widths."""
+    dim, inner = w_out.shape
+    depth, wide = _up8(x.shape[-1]), _up8(inner)
+    x2, w1, w2 = _flat(x), _flat(w_in), _flat(w_out)
+    rows = x2.shape[0]
+    if depth != x2.shape[1]:
+        x2 = _refit(x2, 1, rows, depth)
+    if depth != w1.shape[1] or wide != inner:
+        w1 = _refit(w1, 2, wide, depth)
+    if wide != inner:
+        w2 = _refit(w2, 1, dim, wide)
+        if b_in is not None:
+            b_in = _refit(_dense(b_in).view(2, inner), 2, 1, wide)
+    b_in = None if b_in is None else _dense(b_in)
+    b_out = None if b_out is None else _dense(b_out)
+    res2 = None if residual is None else _flat(residual)
+    lib = nv.lib(x2)
+    h = x2.new_empty((rows, wide))
+    if not keep and rows <= FEW_ROWS:
+        y, vg = x2.new_empty((rows, dim)), None
+        nv.check(lib.fbam_gated_few_rows(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide, nv.addr(b_out),
+                                         nv.addr(res2), dim, h.data_ptr(), y.data_ptr(), rows, depth, wide, dim, act, nv.stream()),
+                 "fbam_gated_few_rows")
+    else:
+        vg = x2.new_empty((2, rows, wide), dtype=F32) if keep else None
+        v = vg.data_ptr() if keep else 0
+        tuned = tuning.active()
+        y = None if tuned else x2.new_empty((rows, dim))
+        nv.check(lib.fbam_gated_block_fwd(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide, nv.addr(b_out),
+                                          nv.addr(res2), h.data_ptr(), v, v + 4 * rows * wide if keep else 0, nv.addr(y), rows, wide,
+                                          depth, dim, act, nv.status_word(x2.device).data_ptr(), nv.stream()), "fbam_gated_block_fwd")
+        if tuned:
+            y = gemm(h, w2, bias=b_out, residual=res2)
+    flops.add(2.0 * rows * inner * (2 * x.shape[-1] + dim))
     return y if x.dim() == 2 else y.view(*x.shape[:-1], dim), x2, w1, w2, vg, h
+
+
+def _slabs(like, splits, m, n):
+    """fp32 workspace of a weight gradient in ``splits`` parts, or None where it is not split."""
+    return like.new_empty((splits, m, n), dtype=F32) if splits > 1 and m * n % 8 == 0 else None
 
 
 class _GatedMlp(torch.autograd.Function):
@@ -140,34 +98,58 @@ class _GatedMlp(torch.autograd.Function):
     def backward(ctx, dy):
         x2, w1, w2, vg, h = ctx.saved_tensors
         shape, inner, act = ctx.meta
-        need = ctx.needs_input_grad
+        need_x, need_in, need_out, need_bin, need_bout, _, need_res = ctx.needs_input_grad
         rows, wide = h.shape
-        dim = w2.shape[0]
-        dy2 = _dense(dy if dy.dim() == 2 else dy.reshape(-1, dim))
-        dx = dw_in = dw_out = db_in = db_out = None
-        if need[0] or need[1] or need[3]:
-            d_vg, db_in = _project_grad(dy2, w2, vg, act, need[3])
-            if need[0]:
-                dx = _product(d_vg, w1, rows, w1.shape[1], b_mn=True)
-                if len(shape) != 2:
-                    dx = dx.view(shape)
-            if need[1]:
-                dw_in = _product(d_vg, x2, 2 * wide, x2.shape[1], True, True, splits=weight_grad_splits(2 * wide, x2.shape[1], rows))
-                if wide != inner:
-                    dw_in = dw_in.view(2, wide, -1)[:, :inner].reshape(2 * inner, -1)
-            if need[3] and wide != inner:
-                db_in = db_in.view(2, wide)[:, :inner].reshape(-1)
-        if need[2]:
-            dw_out = _product(dy2, h, dim, wide, True, True, splits=weight_grad_splits(dim, wide, rows))
-            if wide != inner:
-                dw_out = dw_out[:, :inner].contiguous()
-        if need[4]:
-            db_out = _bias_grad(dy2)
-        return dx, dw_in, dw_out, db_in, db_out, None, dy if need[6] else None
+        dim, width = w2.shape[0], shape[-1]
+        dy2 = _flat(dy)
+        if dim % 8:
+            dy2 = _refit(dy2, 1, rows, _up8(dim))
+        dx = dw_in = dw_out = db_in = db_out = d_vg = sums = work = slabs_in = slabs_out = None
+        splits_in = splits_out = 0
+        tuned = tuning.active()
+        if need_x or need_in or need_bin:
+            d_vg = h.new_empty((rows, 2 * wide))
+            if need_bin:
+                db_in, sums = h.new_empty(2 * wide), vg.new_empty(((rows + 31) // 32, 2 * wide))
+            if need_x:
+                dx = None if tuned else h.new_empty((rows, width))
+            if need_in and not tuned:
+                dw_in = h.new_empty((2 * wide, width))
+                splits_in = weight_grad_splits(2 * wide, width, rows)
+                slabs_in = _slabs(h, splits_in, 2 * wide, width)
+        if need_out and not tuned:
+            dw_out = h.new_empty((dim, inner))
+            splits_out = weight_grad_splits(dim, inner, rows)
+            slabs_out = _slabs(h, splits_out, dim, inner)
+        if need_bout:
+            db_out = h.new_empty(_up8(dim))
+            parts = _sum_partials("fbam_colsum_partials", rows, _up8(dim), 0)
+            work = vg.new_empty(parts * _up8(dim)) if parts else None
+        v = vg.data_ptr()
+        nv.check(nv.lib(h).fbam_gated_block_bwd(
+            dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), w1.data_ptr(), w1.stride(0), w2.data_ptr(), wide, v,
+            v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
+            nv.addr(dw_out), nv.addr(db_out), nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0,
+            nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, inner, x2.shape[1], width, dim, act,
+            nv.status_word(h.device).data_ptr(), nv.stream()), "fbam_gated_block_bwd")
+        flops.add(2.0 * rows * inner * (dim * ((d_vg is not None) + (dw_out is not None)) + 2 * width * ((dx is not None) + (dw_in is not None))))
+        if tuned:
+            dx = gemm(d_vg, w1[:, :width], b_mn=True) if need_x else None
+            dw_in = gemm(d_vg, x2[:, :width], a_mn=True, b_mn=True) if need_in else None
+            dw_out = gemm(dy2[:, :dim], h[:, :inner], a_mn=True, b_mn=True) if need_out else None
+        if wide != inner:
+            dw_in = None if dw_in is None else _refit(dw_in, 2, inner, width)
+            db_in = None if db_in is None else _refit(db_in.view(2, wide), 2, 1, inner).view(-1)
+        if db_out is not None and dim % 8:
+            db_out = db_out[:dim]
+        if dx is not None and len(shape) != 2:
+            dx = dx.view(shape)
+        return dx, dw_in, dw_out, db_in, db_out, None, dy if need_res else None
 
 
 def gated_mlp(x, w_in, w_out, b_in, b_out, act, residual):
     _need_elem(x, w_in, w_out, b_in, b_out, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad or
+                                    any(t is not None and t.requires_grad for t in (b_in, b_out, residual))):
         return _GatedMlp.apply(x, w_in, w_out, b_in, b_out, GATES[act], residual)
     return _forward(x, w_in, w_out, b_in, b_out, GATES[act], residual, False)[0]

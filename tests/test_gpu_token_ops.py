@@ -592,3 +592,38 @@ def test_logprobs_values_of_one_thread_only():
             wide[:, :, 0] += 20.0
             r = ops.token_logprobs(y, None, 32)
             assert torch.equal(r.top_ids, oracle.alternatives(y, 32))
+
+
+def test_gated_mlp_with_a_tile_table():
+    """A table of tuned tiles is used for the block's plain products, and nothing else changes."""
+    from fbamtrain_b200.ops import tuning
+    gen = _gen("tuned")
+    x, w_in, w_out = _randn(gen, 260, 72, dtype=BF), _randn(gen, 2 * 90, 72, dtype=BF, scale=0.1), _randn(gen, 66, 90, dtype=BF, scale=0.1)
+    dy = _randn(gen, 260, 66, dtype=BF)
+    named = [t.requires_grad_() for t in (x, w_in, w_out)]
+
+    def both():
+        y = ops.gated_mlp(x, w_in, w_out)
+        return [y.detach(), *torch.autograd.grad((y,), named, (dy,))]
+
+    plain = both()
+    with tuning.recording() as noted:
+        tuned = both()
+    assert len(noted) >= 3
+    for a, b in zip(plain, tuned):
+        # other tiles, other order of fp32 sums: at most one unit of the type apart
+        oracle.within(a, b.double(), BF, 2.0 ** -8 * b.double().abs() + 1e-3)
+
+
+@pytest.mark.parametrize("needs", ["x", "w_in", "w_out", "b_in", "b_out", "residual"])
+def test_gated_mlp_one_gradient_at_a_time(needs):
+    gen = _gen("needs")
+    named = {"x": _randn(gen, 50, 44, dtype=BF), "w_in": _randn(gen, 2 * 30, 44, dtype=BF, scale=0.1),
+             "w_out": _randn(gen, 20, 30, dtype=BF, scale=0.1), "b_in": _randn(gen, 60, dtype=BF), "b_out": _randn(gen, 20, dtype=BF),
+             "residual": _randn(gen, 50, 20, dtype=BF)}
+    dy = _randn(gen, 50, 20, dtype=BF)
+    want, size = oracle.mlp(*(named[k] for k in ("x", "w_in", "w_out", "b_in", "b_out")), "gelu", named["residual"], dy)
+    named[needs].requires_grad_()
+    y = ops.gated_mlp(named["x"], named["w_in"], named["w_out"], named["b_in"], named["b_out"], "gelu", named["residual"])
+    g, = torch.autograd.grad((y,), (named[needs],), (dy,))
+    oracle.within(g, want[needs], BF, (1.01 * 2.0 ** -8 + 1e-4) * size[needs] + 1e-6)
