@@ -10,6 +10,11 @@
 //                         Further CTAs write the rows that no id names;
 //   3. the same kernel on the partial sums, two entries a piece in the order of the pieces, until there is one piece.  However
 //      common an id is, its sum takes log32 of its count steps.
+//
+// Bound by memory, and below some ten thousand tokens by the latency of four launches.  Four rows are on their way at once in a
+// look-up (65536 rows of 2048 from fp32 to bf16: 85 us, 4.9 TB/s of DRAM traffic); a piece's keys and positions come through
+// shared memory so that eight rows can be (gradient of the same, 100003 rows of fp32: 186 us, 5.6 TB/s).  The partial sums, a
+// sixteenth of the rows at most, are taken 32 at a time by few CTAs (16 + 10 + 8 us there).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -152,7 +157,9 @@ __device__ __forceinline__ int cluster_read(const int* smem, uint32_t rank) {
 // Every warp owns a contiguous part of the input, so (CTA, warp, round, lane) is the input's order.  Per pass over `bits`
 // bits: count the digits of each warp's part, turn the counts into first output places (digits before, then CTAs before,
 // then warps before), and place the elements in order.  counts: [kSortWarps][bins] in shared memory.  A warp has the elements of
-// eight rounds on their way at once, and keeps them from the counting to the placing where that is all there are.
+// eight rounds on their way at once, and keeps them from the counting to the placing where that is all there are.  What takes
+// the time is placing single 8-byte entries from sixteen SMs (131072 ids of 262144: 35 us, with keys and positions apart and
+// eight CTAs 65).
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads, 1)
 embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint32_t* present, int n, int vocab, int bits, int passes) {
