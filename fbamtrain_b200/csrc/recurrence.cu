@@ -200,49 +200,63 @@ struct __align__(16) Exchange {
   }
 };
 
-// Passes `mine` on and returns what comes in to this warp's chunk; `carry` is what comes in to the cluster's first chunk, and
-// becomes what its last chunk hands on.  Chunks follow one another by (place of the CTA, place of the warp).  round: of this
-// launch, from 0.
+// Links are passed on in two halves, between which a warp has work that needs nothing from the others.  Chunks follow one another
+// by (place of the CTA, place of the warp); round: of this launch, from 0.
 template <int VEC, int WARPS>
-__device__ __forceinline__ Vec<VEC> exchange(Exchange<VEC, WARPS>& ex, int round, const Link<VEC>& mine, int place, bool backwards,
-                                             Vec<VEC>& carry, int* status) {
-  Vec<VEC> in = carry;
-  if constexpr (WARPS == 1) {
-    carry = mine(carry);
-  } else {
-    const int lane = threadIdx.x % 32, turn = round & 1;
-    const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-    ex.warps[turn][place][lane] = mine;
-    __syncthreads();
-    if (ctas == 1) {
+struct Passing {
+  Link<VEC> own, before;            // of this warp, and of the warps of the CTA before it
+
+  __device__ __forceinline__ void send(Exchange<VEC, WARPS>& ex, int round, const Link<VEC>& mine, int place, bool backwards) {
+    own = mine;
+    if constexpr (WARPS > 1) {
+      const int lane = threadIdx.x % 32, turn = round & 1;
+      const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+      ex.warps[turn][place][lane] = mine;
+      __syncthreads();
+      before = Link<VEC>{Vec<VEC>::all(1.0f), Vec<VEC>::all(0.0f)};
+      if (ctas > 1) {
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        if (w == place) in = carry;
-        carry = ex.warps[turn][w][lane](carry);
+        for (int w = 0; w < WARPS - 1; ++w)
+          if (w < place) before = before.then(ex.warps[turn][w][lane]);
+        if (place == WARPS - 1) {                                     // of the CTA as a whole
+          const Link<VEC> all = before.then(mine);
+          if (lane == 0) mbar_expect_tx(&ex.arrived[turn], ctas * 32 * (uint32_t)sizeof(Link<VEC>));
+          const int here = backwards ? ctas - 1 - rank : rank;
+          for (int c = 0; c < ctas; ++c) push(&ex.ctas[turn][here][lane], &ex.arrived[turn], c, all);
+        }
       }
-    } else {
-      Link<VEC> before{Vec<VEC>::all(1.0f), Vec<VEC>::all(0.0f)};     // of the warps before this one
-#pragma unroll
-      for (int w = 0; w < WARPS - 1; ++w)
-        if (w < place) before = before.then(ex.warps[turn][w][lane]);
-      const int here = backwards ? ctas - 1 - rank : rank;
-      if (place == WARPS - 1) {                                       // of the CTA as a whole
-        const Link<VEC> all = before.then(mine);
-        if (lane == 0) mbar_expect_tx(&ex.arrived[turn], ctas * 32 * (uint32_t)sizeof(Link<VEC>));
-        for (int c = 0; c < ctas; ++c) push(&ex.ctas[turn][here][lane], &ex.arrived[turn], c, all);
-      }
-      if (!mbar_wait(&ex.arrived[turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_EPILOGUE_TIMEOUT);
-#pragma unroll
-      for (int c = 0; c < kMaxCtas; ++c) {
-        if (c >= ctas) break;
-        if (c == here) in = carry;
-        carry = ex.ctas[turn][c][lane](carry);
-      }
-      in = before(in);
     }
   }
-  return in;
-}
+
+  // What comes in to this warp's chunk; `carry` is what comes in to the cluster's first chunk, and becomes what its last hands on.
+  __device__ __forceinline__ Vec<VEC> take(Exchange<VEC, WARPS>& ex, int round, int place, bool backwards, Vec<VEC>& carry, int* status) {
+    Vec<VEC> in = carry;
+    if constexpr (WARPS == 1) {
+      carry = own(carry);
+    } else {
+      const int lane = threadIdx.x % 32, turn = round & 1;
+      const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+      if (ctas == 1) {
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          if (w == place) in = carry;
+          carry = ex.warps[turn][w][lane](carry);
+        }
+      } else {
+        if (!mbar_wait(&ex.arrived[turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_EPILOGUE_TIMEOUT);
+        const int here = backwards ? ctas - 1 - rank : rank;
+#pragma unroll
+        for (int c = 0; c < kMaxCtas; ++c) {
+          if (c >= ctas) break;
+          if (c == here) in = carry;
+          carry = ex.ctas[turn][c][lane](carry);
+        }
+        in = before(in);
+      }
+    }
+    return in;
+  }
+};
 
 // The walks over a chunk of STEPS steps.  FAST: all of them are there and none is a reset.  z, g, o, d: functions of the step
 // that give the inputs (0 behind the end), put: one that takes an output.  nf1: -(1 - f).
@@ -263,36 +277,40 @@ __device__ __forceinline__ void forward_in(Vec<VEC> (&nf1)[STEPS], Link<VEC>& li
   if (!FAST && bits) link.gain = V::all(-1.0f);
 }
 
+// Output gates are formed while links are on their way, but only the first kAhead of a chunk: they lie in registers until h is
+// there.  us by kAhead, 16 steps to a chunk, bf16: 1 x 30011 x 2048  0: 123  4: 119  8: 120  16: 131; 1 x 60000 x 512  0: 158
+// 4: 150  8: 145  16: 156.
+constexpr int kAhead = 8;
+template <int VEC, typename O>
+__device__ __forceinline__ void forward_ahead(Vec<VEC> (&so)[kAhead], O o) {
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) so[t] = sigmoid<VEC>(o(t));
+}
+
 template <bool FAST, int STEPS, int VEC, typename Z, typename O, typename P>
-__device__ __forceinline__ void forward_out(const Vec<VEC> (&nf1)[STEPS], Vec<VEC>& h, float* saved, int dim, int n, uint32_t bits,
-                                            Z z, O o, P put) {
+__device__ __forceinline__ void forward_out(const Vec<VEC> (&nf1)[STEPS], const Vec<VEC> (&so)[kAhead], Vec<VEC>& h, float* saved, int dim,
+                                            int n, uint32_t bits, Z z, O o, P put) {
   using V = Vec<VEC>;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
     if (t % kSaved == 0 && saved != nullptr && (FAST || t < n)) store(saved + t / kSaved * dim, h);
     if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
     h = fma(nf1[t], h - z(t), h);
-    put(t, sigmoid<VEC>(o(t)) * h);
+    put(t, (t < kAhead ? so[t] : sigmoid<VEC>(o(t))) * h);
   }
 }
 
-// Forwards over the chunk from the state h in front of it, and with it the gradient of the output gate.  What is left for the
-// walk back: nf1, u (the factor of dg), and dh0 (the part of dh that a step's own y gives).
-template <bool FAST, int STEPS, int VEC, typename Z, typename G, typename O, typename D, typename P>
-__device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&u)[STEPS], Vec<VEC> (&dh0)[STEPS], Link<VEC>& link,
-                                            Vec<VEC> h, int n, uint32_t bits, Z z, G g, O o, D d, P put) {
+// What a link needs: nf1, f, so1 = 1 - sigmoid(o), and dh0, the part of dh that a step's own y gives.
+template <bool FAST, int STEPS, int VEC, typename G, typename O, typename D>
+__device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&f)[STEPS], Vec<VEC> (&nso1)[STEPS], Vec<VEC> (&dh0)[STEPS],
+                                            Link<VEC>& link, int n, uint32_t bits, G g, O o, D d) {
   using V = Vec<VEC>;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
-    if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
-    V f, so, nso1;
-    gates<VEC>(g(t), f, nf1[t]);
-    gates<VEC>(o(t), so, nso1);
-    const V step = h - z(t);
-    u[t] = (step * f) * (nf1[t] * V::all(-1.0f));
-    h = fma(nf1[t], step, h);
+    V so;
+    gates<VEC>(g(t), f[t], nf1[t]);
+    gates<VEC>(o(t), so, nso1[t]);
     dh0[t] = d(t) * so;
-    put(t, (dh0[t] * h) * (nso1 * V::all(-1.0f)));
     if (!FAST && t >= n) nf1[t] = dh0[t] = V::all(0.0f);    // behind the end e passes unchanged
   }
   link.gain = V::all(1.0f);
@@ -305,6 +323,21 @@ __device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&u
     link.gain = fma(nf1[t], link.gain, link.gain);
   }
   if (!FAST && bits) link.gain = V::all(-1.0f);
+}
+
+// Forwards over the chunk from the state h in front of it: the gradient of the output gates, and u, the factor of dg, over f.
+template <bool FAST, int STEPS, int VEC, typename Z, typename P>
+__device__ __forceinline__ void backward_states(const Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&f)[STEPS], const Vec<VEC> (&nso1)[STEPS],
+                                                const Vec<VEC> (&dh0)[STEPS], Vec<VEC> h, uint32_t bits, Z z, P put) {
+  using V = Vec<VEC>;
+#pragma unroll
+  for (int t = 0; t < STEPS; ++t) {
+    if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
+    const V step = h - z(t);
+    f[t] = (step * f[t]) * (nf1[t] * V::all(-1.0f));
+    h = fma(nf1[t], step, h);
+    put(t, (dh0[t] * h) * (nso1[t] * V::all(-1.0f)));
+  }
 }
 
 template <bool FAST, int STEPS, int VEC, typename P, typename Q>
@@ -360,10 +393,14 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
     Vec<VEC> nf1[STEPS];
     Link<VEC> link;
     forward_in<false>(nf1, link, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return g[t].get(); });
-    Vec<VEC> h = exchange<VEC, WARPS>(ex, round, link, warp, false, carry, status);
+    Passing<VEC, WARPS> passing;
+    passing.send(ex, round, link, warp, false);
+    Vec<VEC> so[kAhead];
+    forward_ahead(so, [&](int t) { return o[t].get(); });
+    Vec<VEC> h = passing.take(ex, round, warp, false, carry, status);
     elem_t* out = y + b * s.yb + t0 * s.yt + ch;
     float* at = saved != nullptr && in ? saved + ((long long)b * s.states + chunk) * s.dim + ch : nullptr;
-    forward_out<false>(nf1, h, at, s.dim, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return o[t].get(); },
+    forward_out<false>(nf1, so, h, at, s.dim, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return o[t].get(); },
                        [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * s.yt, v); });
     if (in && t0 + STEPS >= s.steps && n > 0) store(state_out + (long long)b * s.dim + ch, h);
   }
@@ -398,12 +435,15 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
     fetch(o, src + 2 * s.zk, s.zt, n);
     fetch(d, dy + b * s.yb + t0 * s.yt + ch, s.yt, n);
     const Vec<VEC> h = n > 0 ? load<VEC>(saved + ((long long)b * s.states + chunk) * s.dim + ch) : Vec<VEC>::all(0.0f);
-    Vec<VEC> nf1[STEPS], u[STEPS], dh0[STEPS];
+    Vec<VEC> nf1[STEPS], u[STEPS], nso1[STEPS], dh0[STEPS];
     Link<VEC> link;
-    backward_in<false>(nf1, u, dh0, link, h, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return g[t].get(); },
-                       [&](int t) { return o[t].get(); }, [&](int t) { return d[t].get(); },
-                       [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + 2 * s.dim, v); });
-    const Vec<VEC> e = exchange<VEC, WARPS>(ex, round, link, WARPS - 1 - warp, true, carry, status);
+    backward_in<false>(nf1, u, nso1, dh0, link, n, bits, [&](int t) { return g[t].get(); }, [&](int t) { return o[t].get(); },
+                       [&](int t) { return d[t].get(); });
+    Passing<VEC, WARPS> passing;
+    passing.send(ex, round, link, WARPS - 1 - warp, true);
+    backward_states<false>(nf1, u, nso1, dh0, h, bits, [&](int t) { return z[t].get(); },
+                           [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + 2 * s.dim, v); });
+    const Vec<VEC> e = passing.take(ex, round, WARPS - 1 - warp, true, carry, status);
     backward_out<false>(nf1, u, dh0, e, bits, [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt, v); },
                         [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + s.dim, v); });
   }
@@ -486,10 +526,12 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     auto g = [&](int t) { return tile.get(1, t); };
     auto o = [&](int t) { return tile.get(2, t); };
     auto put = [&](int t, Vec<2> v) { tile.put(2, t, v); };
-    Vec<2> nf1[STEPS];
+    Vec<2> nf1[STEPS], so[kAhead];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
     if (fast) forward_in<true>(nf1, link, n, bits, z, g);
     else if (n > 0) forward_in<false>(nf1, link, n, bits, z, g);
+    Passing<2, kWarps> passing;
+    passing.send(sm.ex, round, link, warp, false);
     // Results go over the output gates that they come from.  The ones of the step before take a while to leave the other buffer,
     // so its output gates, which are needed last, are fetched only now.
     if (more && lane == 0) {
@@ -497,12 +539,15 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
       issue_o(t0 + per_step, turn ^ 1);
     }
     __syncwarp();
-    Vec<2> h = exchange<2, kWarps>(sm.ex, round, link, warp, false, carry, status);
+    if (n > 0) {
+      if (!mbar_wait(&sm.full_o[warp][turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_PRODUCER_TIMEOUT);
+      forward_ahead(so, o);
+    }
+    Vec<2> h = passing.take(sm.ex, round, warp, false, carry, status);
     if (n <= 0) continue;
-    if (!mbar_wait(&sm.full_o[warp][turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_PRODUCER_TIMEOUT);
     float* at = saved != nullptr && in ? saved + ((long long)b * s.states + t0 / kSaved) * s.dim + ch : nullptr;
-    if (fast) forward_out<true>(nf1, h, at, s.dim, n, bits, z, o, put);
-    else forward_out<false>(nf1, h, at, s.dim, n, bits, z, o, put);
+    if (fast) forward_out<true>(nf1, so, h, at, s.dim, n, bits, z, o, put);
+    else forward_out<false>(nf1, so, h, at, s.dim, n, bits, z, o, put);
     if (in && t0 + STEPS >= s.steps) store(state_out + (long long)b * s.dim + ch, h);
     fence_proxy_async_smem();
     __syncwarp();
@@ -580,12 +625,16 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     auto put_z = [&](int t, Vec<2> v) { result.put(0, t, v); };
     auto put_g = [&](int t, Vec<2> v) { result.put(1, t, v); };
     auto put_o = [&](int t, Vec<2> v) { dout[t] = ff2e2(v.v.x, v.v.y); };
-    Vec<2> nf1[STEPS], u[STEPS], dh0[STEPS];
+    Vec<2> nf1[STEPS], u[STEPS], nso1[STEPS], dh0[STEPS];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
+    if (fast) backward_in<true>(nf1, u, nso1, dh0, link, n, bits, g, o, d);
+    else if (n > 0) backward_in<false>(nf1, u, nso1, dh0, link, n, bits, g, o, d);
+    Passing<2, kWarps> passing;
+    passing.send(sm.ex, round, link, kWarps - 1 - warp, true);
     const Vec<2> h = load<2>(&sm.states[warp][stage][2 * lane]);
-    if (fast) backward_in<true>(nf1, u, dh0, link, h, n, bits, z, g, o, d, put_o);
-    else if (n > 0) backward_in<false>(nf1, u, dh0, link, h, n, bits, z, g, o, d, put_o);
-    const Vec<2> e = exchange<2, kWarps>(sm.ex, round, link, kWarps - 1 - warp, true, carry, status);
+    if (fast) backward_states<true>(nf1, u, nso1, dh0, h, bits, z, put_o);
+    else if (n > 0) backward_states<false>(nf1, u, nso1, dh0, h, bits, z, put_o);
+    const Vec<2> e = passing.take(sm.ex, round, kWarps - 1 - warp, true, carry, status);
     if (n <= 0) continue;
     if (lane == 0) bulk_wait_group_read<0>();               // the results of the step before have left
     __syncwarp();
