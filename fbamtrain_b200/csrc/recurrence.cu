@@ -65,6 +65,8 @@ __device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {a.v + 
 __device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b) { return {__fadd2_rn(a.v, b.v)}; }
 template <int VEC>
 __device__ __forceinline__ Vec<VEC> operator-(Vec<VEC> a, Vec<VEC> b) { return fma(b, Vec<VEC>::all(-1.0f), a); }
+__device__ __forceinline__ Vec<1> minus(Vec<1> a) { return {-a.v}; }
+__device__ __forceinline__ Vec<2> minus(Vec<2> a) { return {make_float2(-a.v.x, -a.v.y)}; }
 __device__ __forceinline__ Vec<1> ex2(Vec<1> a) { return {ex2(a.v)}; }
 __device__ __forceinline__ Vec<2> ex2(Vec<2> a) { return {make_float2(ex2(a.v.x), ex2(a.v.y))}; }
 __device__ __forceinline__ Vec<1> rcp(Vec<1> a) { return {rcp(a.v)}; }
@@ -89,13 +91,20 @@ __device__ __forceinline__ float below(float x, float most) {     // NaN stays N
 }
 __device__ __forceinline__ Vec<1> below(Vec<1> x, float most) { return {below(x.v, most)}; }
 __device__ __forceinline__ Vec<2> below(Vec<2> x, float most) { return {make_float2(below(x.v.x, most), below(x.v.y, most))}; }
-// f = sigmoid(x) and nf1 = -sigmoid(-x), both to full relative accuracy; exp is kept finite for its product with 0
+// With e = exp(x), kept finite for its product with 0, to full relative accuracy at both ends:
+// nf = -sigmoid(x) and nf1 = -sigmoid(-x)
 template <int VEC>
-__device__ __forceinline__ void gates(Vec<VEC> x, Vec<VEC>& f, Vec<VEC>& nf1) {
+__device__ __forceinline__ void gates(Vec<VEC> x, Vec<VEC>& nf, Vec<VEC>& nf1) {
   const Vec<VEC> e = ex2(below(x * Vec<VEC>::all(kLog2e), 126.0f));
-  const Vec<VEC> r = rcp(e + Vec<VEC>::all(1.0f));
-  f = e * r;
-  nf1 = r * Vec<VEC>::all(-1.0f);
+  nf1 = rcp(Vec<VEC>::all(-1.0f) - e);
+  nf = e * nf1;
+}
+// s = sigmoid(x) and s1 = sigmoid(-x)
+template <int VEC>
+__device__ __forceinline__ void both_sigmoids(Vec<VEC> x, Vec<VEC>& s, Vec<VEC>& s1) {
+  const Vec<VEC> e = ex2(below(x * Vec<VEC>::all(-kLog2e), 126.0f));
+  s = rcp(e + Vec<VEC>::all(1.0f));
+  s1 = e * s;
 }
 
 // VEC elements as they lie in memory
@@ -300,16 +309,16 @@ __device__ __forceinline__ void forward_out(const Vec<VEC> (&nf1)[STEPS], const 
   }
 }
 
-// What a link needs: nf1, f, so1 = 1 - sigmoid(o), and dh0, the part of dh that a step's own y gives.
+// What a link needs: nf1, nf, so1 = 1 - sigmoid(o), and dh0, the part of dh that a step's own y gives.
 template <bool FAST, int STEPS, int VEC, typename G, typename O, typename D>
-__device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&f)[STEPS], Vec<VEC> (&nso1)[STEPS], Vec<VEC> (&dh0)[STEPS],
+__device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&nf)[STEPS], Vec<VEC> (&so1)[STEPS], Vec<VEC> (&dh0)[STEPS],
                                             Link<VEC>& link, int n, uint32_t bits, G g, O o, D d) {
   using V = Vec<VEC>;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
     V so;
-    gates<VEC>(g(t), f[t], nf1[t]);
-    gates<VEC>(o(t), so, nso1[t]);
+    gates<VEC>(g(t), nf[t], nf1[t]);
+    both_sigmoids<VEC>(o(t), so, so1[t]);
     dh0[t] = d(t) * so;
     if (!FAST && t >= n) nf1[t] = dh0[t] = V::all(0.0f);    // behind the end e passes unchanged
   }
@@ -325,18 +334,18 @@ __device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&f
   if (!FAST && bits) link.gain = V::all(-1.0f);
 }
 
-// Forwards over the chunk from the state h in front of it: the gradient of the output gates, and u, the factor of dg, over f.
+// Forwards over the chunk from the state h in front of it: the gradient of the output gates, and u, the factor of dg, over nf.
 template <bool FAST, int STEPS, int VEC, typename Z, typename P>
-__device__ __forceinline__ void backward_states(const Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&f)[STEPS], const Vec<VEC> (&nso1)[STEPS],
+__device__ __forceinline__ void backward_states(const Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&nf)[STEPS], const Vec<VEC> (&so1)[STEPS],
                                                 const Vec<VEC> (&dh0)[STEPS], Vec<VEC> h, uint32_t bits, Z z, P put) {
   using V = Vec<VEC>;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
     if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
     const V step = h - z(t);
-    f[t] = (step * f[t]) * (nf1[t] * V::all(-1.0f));
     h = fma(nf1[t], step, h);
-    put(t, (dh0[t] * h) * (nso1[t] * V::all(-1.0f)));
+    nf[t] = (step * nf[t]) * nf1[t];
+    put(t, (dh0[t] * h) * so1[t]);
   }
 }
 
@@ -347,7 +356,7 @@ __device__ __forceinline__ void backward_out(const Vec<VEC> (&nf1)[STEPS], const
 #pragma unroll
   for (int t = STEPS - 1; t >= 0; --t) {
     const V dh = e + dh0[t];
-    put_z(t, (nf1[t] * dh) * V::all(-1.0f));
+    put_z(t, minus(nf1[t] * dh));
     put_g(t, u[t] * dh);
     e = fma(nf1[t], dh, dh);
     if (!FAST && ((bits >> t) & 1)) e = V::all(0.0f);
@@ -435,13 +444,13 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
     fetch(o, src + 2 * s.zk, s.zt, n);
     fetch(d, dy + b * s.yb + t0 * s.yt + ch, s.yt, n);
     const Vec<VEC> h = n > 0 ? load<VEC>(saved + ((long long)b * s.states + chunk) * s.dim + ch) : Vec<VEC>::all(0.0f);
-    Vec<VEC> nf1[STEPS], u[STEPS], nso1[STEPS], dh0[STEPS];
+    Vec<VEC> nf1[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
     Link<VEC> link;
-    backward_in<false>(nf1, u, nso1, dh0, link, n, bits, [&](int t) { return g[t].get(); }, [&](int t) { return o[t].get(); },
+    backward_in<false>(nf1, u, so1, dh0, link, n, bits, [&](int t) { return g[t].get(); }, [&](int t) { return o[t].get(); },
                        [&](int t) { return d[t].get(); });
     Passing<VEC, WARPS> passing;
     passing.send(ex, round, link, WARPS - 1 - warp, true);
-    backward_states<false>(nf1, u, nso1, dh0, h, bits, [&](int t) { return z[t].get(); },
+    backward_states<false>(nf1, u, so1, dh0, h, bits, [&](int t) { return z[t].get(); },
                            [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + 2 * s.dim, v); });
     const Vec<VEC> e = passing.take(ex, round, WARPS - 1 - warp, true, carry, status);
     backward_out<false>(nf1, u, dh0, e, bits, [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt, v); },
@@ -458,14 +467,8 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kWarps = 8, kSlab = 64;       // channels of a tile: two a lane
 
-struct Tile {
-  elem_t* at;                               // [members][STEPS][kSlab], this lane's two channels
-  int steps;
-  __device__ __forceinline__ Vec<2> get(int member, int t) const {
-    return {e22ff(*reinterpret_cast<const elem2_t*>(at + (member * steps + t) * kSlab))};
-  }
-  __device__ __forceinline__ void put(int member, int t, Vec<2> v) const { store(at + (member * steps + t) * kSlab, v); }
-};
+// This lane's two channels of a row of a tile
+__device__ __forceinline__ Vec<2> get(const elem_t* row) { return {e22ff(*reinterpret_cast<const elem2_t*>(row))}; }
 
 template <int STEPS>
 struct FwdSmem {
@@ -517,15 +520,16 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     const int n = min(STEPS, s.steps - t0);                 // may be below 0
     const uint32_t bits = next_bits;
     const bool fast = n == STEPS && bits == 0;
-    const Tile tile{&sm.tiles[warp][turn][0][0][2 * lane], STEPS};
+    const elem_t *zs = &sm.tiles[warp][turn][0][0][2 * lane], *gs = &sm.tiles[warp][turn][1][0][2 * lane];
+    elem_t* oy = &sm.tiles[warp][turn][2][0][2 * lane];
     const bool more = t0 + per_step < s.steps;
     if (n > 0 && !mbar_wait(&sm.full_zg[warp][turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_PRODUCER_TIMEOUT);
     if (more && lane == 0) issue_zg(t0 + per_step, turn ^ 1);
     if (more) next_bits = reset_bits(resets, s, b, t0 + per_step, min(STEPS, s.steps - t0 - per_step));
-    auto z = [&](int t) { return tile.get(0, t); };
-    auto g = [&](int t) { return tile.get(1, t); };
-    auto o = [&](int t) { return tile.get(2, t); };
-    auto put = [&](int t, Vec<2> v) { tile.put(2, t, v); };
+    auto z = [&](int t) { return get(zs + t * kSlab); };
+    auto g = [&](int t) { return get(gs + t * kSlab); };
+    auto o = [&](int t) { return get(oy + t * kSlab); };
+    auto put = [&](int t, Vec<2> v) { store(oy + t * kSlab, v); };
     Vec<2> nf1[STEPS], so[kAhead];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
     if (fast) forward_in<true>(nf1, link, n, bits, z, g);
@@ -562,8 +566,9 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
 
 template <int STEPS>
 struct BwdSmem {
-  alignas(128) elem_t tiles[kWarps][2][4][STEPS][kSlab];
-  alignas(128) elem_t results[kWarps][3][STEPS][kSlab];
+  alignas(128) elem_t zgo[kWarps][2][STEPS][3][kSlab];
+  alignas(128) elem_t dy[kWarps][2][STEPS][kSlab];
+  alignas(128) elem_t results[kWarps][STEPS][3][kSlab];
   alignas(128) float states[kWarps][2][kSlab];
   Exchange<2, kWarps> ex;
   uint64_t full[kWarps][2];
@@ -590,12 +595,13 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
   sm.ex.init();
   __syncwarp();
   const int state_bytes = min(kSlab, s.dim - ch0) * 4;
-  auto issue = [&](int t0, int buf) {                       // one lane
+  // One lane.  A chunk's three members come and go as one copy: 1 x 30011 x 2048 189 us, 197 as one each.  (The forward, which
+  // fetches z and g as one copy and o as another, gains nothing: 119 | 119, and 1 x 60000 x 512 loses, 160 | 144.)
+  auto issue = [&](int t0, int buf) {
     mbar_expect_tx(&sm.full[warp][buf], 4 * STEPS * kSlab * 2 + state_bytes);
     bulk_load(sm.states[warp][buf], saved + ((long long)b * s.states + t0 / kSaved) * s.dim + ch0, state_bytes, &sm.full[warp][buf]);
-#pragma unroll
-    for (int k = 0; k < 3; ++k) tma_load_4d(sm.tiles[warp][buf][k], &map_in, &sm.full[warp][buf], ch0, k, t0, b);
-    tma_load_3d(sm.tiles[warp][buf][3], &map_dy, &sm.full[warp][buf], ch0, t0, b);
+    tma_load_4d(sm.zgo[warp][buf], &map_in, &sm.full[warp][buf], ch0, 0, t0, b);
+    tma_load_3d(sm.dy[warp][buf], &map_dy, &sm.full[warp][buf], ch0, t0, b);
   };
   Vec<2> carry = Vec<2>::all(0.0f);
   if (in && d_state_out != nullptr) carry = load<2>(d_state_out + (long long)b * s.dim + ch);
@@ -608,7 +614,8 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     const int n = min(STEPS, s.steps - t0);
     const uint32_t bits = next_bits;
     const bool fast = n == STEPS && bits == 0;
-    const Tile tile{&sm.tiles[warp][stage][0][0][2 * lane], STEPS}, result{&sm.results[warp][0][0][2 * lane], STEPS};
+    const elem_t *zgo = &sm.zgo[warp][stage][0][0][2 * lane], *dy = &sm.dy[warp][stage][0][2 * lane];
+    elem_t* result = &sm.results[warp][0][0][2 * lane];
     if (n > 0) {
       if (!mbar_wait(&sm.full[warp][stage], (phases >> stage) & 1) && lane == 0) atomicExch(status, GEMM_ERR_PRODUCER_TIMEOUT);
       phases ^= 1u << stage;
@@ -617,36 +624,35 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
       if (lane == 0) issue(t0 - per_step, stage ^ 1);
       next_bits = reset_bits(resets, s, b, t0 - per_step, min(STEPS, s.steps - t0 + per_step));
     }
-    auto z = [&](int t) { return tile.get(0, t); };
-    auto g = [&](int t) { return tile.get(1, t); };
-    auto o = [&](int t) { return tile.get(2, t); };
-    auto d = [&](int t) { return tile.get(3, t); };
+    auto z = [&](int t) { return get(zgo + 3 * t * kSlab); };
+    auto g = [&](int t) { return get(zgo + (3 * t + 1) * kSlab); };
+    auto o = [&](int t) { return get(zgo + (3 * t + 2) * kSlab); };
+    auto d = [&](int t) { return get(dy + t * kSlab); };
     elem2_t dout[STEPS];
-    auto put_z = [&](int t, Vec<2> v) { result.put(0, t, v); };
-    auto put_g = [&](int t, Vec<2> v) { result.put(1, t, v); };
+    auto put_z = [&](int t, Vec<2> v) { store(result + 3 * t * kSlab, v); };
+    auto put_g = [&](int t, Vec<2> v) { store(result + (3 * t + 1) * kSlab, v); };
     auto put_o = [&](int t, Vec<2> v) { dout[t] = ff2e2(v.v.x, v.v.y); };
-    Vec<2> nf1[STEPS], u[STEPS], nso1[STEPS], dh0[STEPS];
+    Vec<2> nf1[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
-    if (fast) backward_in<true>(nf1, u, nso1, dh0, link, n, bits, g, o, d);
-    else if (n > 0) backward_in<false>(nf1, u, nso1, dh0, link, n, bits, g, o, d);
+    if (fast) backward_in<true>(nf1, u, so1, dh0, link, n, bits, g, o, d);
+    else if (n > 0) backward_in<false>(nf1, u, so1, dh0, link, n, bits, g, o, d);
     Passing<2, kWarps> passing;
     passing.send(sm.ex, round, link, kWarps - 1 - warp, true);
     const Vec<2> h = load<2>(&sm.states[warp][stage][2 * lane]);
-    if (fast) backward_states<true>(nf1, u, nso1, dh0, h, bits, z, put_o);
-    else if (n > 0) backward_states<false>(nf1, u, nso1, dh0, h, bits, z, put_o);
+    if (fast) backward_states<true>(nf1, u, so1, dh0, h, bits, z, put_o);
+    else if (n > 0) backward_states<false>(nf1, u, so1, dh0, h, bits, z, put_o);
     const Vec<2> e = passing.take(sm.ex, round, kWarps - 1 - warp, true, carry, status);
     if (n <= 0) continue;
     if (lane == 0) bulk_wait_group_read<0>();               // the results of the step before have left
     __syncwarp();
 #pragma unroll
-    for (int t = 0; t < STEPS; ++t) *reinterpret_cast<elem2_t*>(result.at + (2 * STEPS + t) * kSlab) = dout[t];
+    for (int t = 0; t < STEPS; ++t) *reinterpret_cast<elem2_t*>(result + (3 * t + 2) * kSlab) = dout[t];
     if (fast) backward_out<true>(nf1, u, dh0, e, bits, put_z, put_g);
     else backward_out<false>(nf1, u, dh0, e, bits, put_z, put_g);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-#pragma unroll
-      for (int k = 0; k < 3; ++k) tma_store_4d(&map_out, sm.results[warp][k], ch0, k, t0, b);
+      tma_store_4d(&map_out, sm.results[warp], ch0, 0, t0, b);
       bulk_commit_group();
     }
   }
@@ -665,7 +671,7 @@ bool pieces(const void* p, int dim, long long a, long long b, long long c) {
          a < (1ll << 38) && b < (1ll << 38) && c < (1ll << 38);
 }
 
-// (batch, steps, members, dim), or (batch, steps, dim) with members = 0; boxes of `box` steps and kSlab channels
+// (batch, steps, 3, dim), or (batch, steps, dim) with members = 0, in boxes of `box` steps, `members` and kSlab channels
 int encode(CUtensorMap* map, const void* p, const Shape& s, long long sb, long long st, long long sk, int members, int box) {
   auto enc = fbam_encode_tiled();
   if (!enc) return GEMM_ERR_DRIVER;
@@ -673,9 +679,9 @@ int encode(CUtensorMap* map, const void* p, const Shape& s, long long sb, long l
   const cuuint32_t ones[4] = {1, 1, 1, 1};
   CUresult r;
   if (members) {
-    const cuuint64_t dims[4] = {(cuuint64_t)s.dim, (cuuint64_t)members, (cuuint64_t)s.steps, (cuuint64_t)s.batch};
+    const cuuint64_t dims[4] = {(cuuint64_t)s.dim, 3, (cuuint64_t)s.steps, (cuuint64_t)s.batch};
     const cuuint64_t strides[3] = {(cuuint64_t)sk * 2, (cuuint64_t)st * 2, (cuuint64_t)sb * 2};
-    const cuuint32_t boxes[4] = {kSlab, 1, (cuuint32_t)box, 1};
+    const cuuint32_t boxes[4] = {kSlab, (cuuint32_t)members, (cuuint32_t)box, 1};
     r = enc(map, ELEM_TMAP, 4, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   } else {
@@ -738,7 +744,7 @@ extern "C" int fbam_recurrence_fwd(const void* zgo, long long zb, long long zt, 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (steps > kSaved && pieces(zgo, dim, zb, zt, zk) && pieces(y, dim, yb, yt, 8)) {
     CUtensorMap in, out;
-    int e = encode(&in, zgo, s, zb, zt, zk, 3, kFwdSteps);
+    int e = encode(&in, zgo, s, zb, zt, zk, 1, kFwdSteps);
     if (!e) e = encode(&out, y, s, yb, yt, 0, 0, kFwdSteps);
     if (e) return e;
     return launch(recurrence_fwd_tma_kernel<kFwdSteps>, kSlab, kWarps, kFwdSteps, (int)sizeof(FwdSmem<kFwdSteps>), s, st, in, out, state_in, resets,
