@@ -11,10 +11,13 @@
 //
 // Bound: 8 bytes a value of h forward, 14 backward (16 bytes more for every 32 of them: the saved states).  The arithmetic is
 // close behind, four operations of the special-function units a value in either direction, so the two gates' exponentials and
-// reciprocals are formed once and everything else is packed.  Measured, bf16: 1 x 30011 x 2048 125 us forward (64 % of the
-// copy rate) and 207 us backward (66 %); 8 x 1024 x 1024 22 and 31 us.
+// reciprocals are formed once and everything else is packed.  Measured, bf16: 1 x 30011 x 2048 120 us forward (67 % of the
+// copy rate) and 194 us backward (70 %); 8 x 1024 x 1024 24 and 33 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
+#include <type_traits>
 
 #include "elem16.cuh"
 #include "gemm_tcgen05.h"
@@ -29,7 +32,7 @@ using namespace tc05;
 
 constexpr int kSaved = 8;         // the forward keeps the state in front of every eighth step
 constexpr int kFwdSteps = 16;     // of a chunk of the forward by TMA; all others have kSaved steps
-constexpr int kMaxCtas = 8;       // of a cluster
+constexpr int kMaxCtas = 16;      // of a cluster
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -195,8 +198,11 @@ __device__ __forceinline__ void push(const Link<1>* place, uint64_t* bar, uint32
 // turns: whoever writes a set again has passed the step between, to which every reader of the set has contributed.
 template <int VEC, int WARPS>
 struct __align__(16) Exchange {
-  Link<VEC> warps[2][WARPS][32], ctas[2][kMaxCtas][32];
-  uint64_t arrived[2];
+  Link<VEC> warps[2][WARPS][32];
+  uint64_t arrived[2];              // behind it in shared memory: the links of the cluster's CTAs
+  __device__ __forceinline__ Link<VEC>* cta(int turn, int c) {
+    return reinterpret_cast<Link<VEC>*>(this + 1) + (turn * (int)cluster_size() + c) * 32 + threadIdx.x % 32;
+  }
   // before the first exchange
   __device__ __forceinline__ void init() {
     if (cluster_size() == 1) return;
@@ -231,7 +237,7 @@ struct Passing {
           const Link<VEC> all = before.then(mine);
           if (lane == 0) mbar_expect_tx(&ex.arrived[turn], ctas * 32 * (uint32_t)sizeof(Link<VEC>));
           const int here = backwards ? ctas - 1 - rank : rank;
-          for (int c = 0; c < ctas; ++c) push(&ex.ctas[turn][here][lane], &ex.arrived[turn], c, all);
+          for (int c = 0; c < ctas; ++c) push(ex.cta(turn, here), &ex.arrived[turn], c, all);
         }
       }
     }
@@ -258,7 +264,7 @@ struct Passing {
         for (int c = 0; c < kMaxCtas; ++c) {
           if (c >= ctas) break;
           if (c == here) in = carry;
-          carry = ex.ctas[turn][c][lane](carry);
+          carry = (*ex.cta(turn, c))(carry);
         }
         in = before(in);
       }
@@ -376,11 +382,12 @@ __device__ __forceinline__ void fetch(Raw<VEC> (&r)[STEPS], const elem_t* p, lon
 }
 
 template <int VEC, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(WARPS * 32, 2)
 recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ state_in, const uint8_t* __restrict__ resets,
                       elem_t* __restrict__ y, float* __restrict__ state_out, float* __restrict__ saved, int* status, const Shape s) {
   constexpr int STEPS = kSaved;
-  __shared__ Exchange<VEC, WARPS> ex;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  Exchange<VEC, WARPS>& ex = *reinterpret_cast<Exchange<VEC, WARPS>*>(smem_raw);
   ex.init();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
@@ -417,12 +424,13 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
 }
 
 template <int VEC, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(WARPS * 32, 2)
 recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict__ resets, const float* __restrict__ saved,
                       const elem_t* __restrict__ dy, const float* __restrict__ d_state_out, elem_t* __restrict__ d_zgo,
                       float* __restrict__ d_state_in, int* status, const Shape s, long long db, long long dt) {
   constexpr int STEPS = kSaved;
-  __shared__ Exchange<VEC, WARPS> ex;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  Exchange<VEC, WARPS>& ex = *reinterpret_cast<Exchange<VEC, WARPS>*>(smem_raw);
   ex.init();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
@@ -473,8 +481,8 @@ __device__ __forceinline__ Vec<2> get(const elem_t* row) { return {e22ff(*reinte
 template <int STEPS>
 struct FwdSmem {
   alignas(128) elem_t tiles[kWarps][2][3][STEPS][kSlab];
-  Exchange<2, kWarps> ex;
   uint64_t full_zg[kWarps][2], full_o[kWarps][2];
+  Exchange<2, kWarps> ex;           // the last one
 };
 
 template <int STEPS>
@@ -570,8 +578,8 @@ struct BwdSmem {
   alignas(128) elem_t dy[kWarps][2][STEPS][kSlab];
   alignas(128) elem_t results[kWarps][STEPS][3][kSlab];
   alignas(128) float states[kWarps][2][kSlab];
-  Exchange<2, kWarps> ex;
   uint64_t full[kWarps][2];
+  Exchange<2, kWarps> ex;           // the last one
 };
 
 template <int STEPS>
@@ -661,6 +669,9 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
   if (ctas > 1) cluster_sync();
 }
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 // Two neighbouring channels per lane where they lie on 4-byte boundaries
 bool pairs(const void* p, int dim, long long a, long long b, long long c) {
   return dim % 2 == 0 && ((a | b | c) & 1) == 0 && (reinterpret_cast<uintptr_t>(p) & 3) == 0;
@@ -695,37 +706,60 @@ int encode(CUtensorMap* map, const void* p, const Shape& s, long long sb, long l
   return r == CUDA_SUCCESS ? 0 : GEMM_ERR_TENSORMAP;
 }
 
-// CTAs of a cluster: as many as the machine holds at once, two per SM, but no more than the sequence has chunks for.  A cluster
-// pays for its links once a walk step, so where there are enough sequences and channels it stays small.  us forward | backward
-// by cluster size, bf16 (batch x steps x channels):
-//   8 x 1024 x 1024    1: 25 | 38     2: 25 | 35     8: 36 | 50
-//   64 x 128 x 1024    1: 25 | 35     2: 25 | 49
-//   1 x 30011 x 2048   1: 488 | 857   2: 303 | 535   4: 156 | 283   8: 126 | 206
-//   16 x 4096 x 512    1: 74 | 126    2: 66 | 105    8: 84 | 129
-// (Sixteen, which a cluster may have on request: 1 x 60000 x 512 191 | 334 against 168 | 295 with eight.)
-int cluster_ctas(const Shape& s, int slabs, int steps) {
-  int ctas = 1;
-  while (ctas < kMaxCtas && ctas * steps < s.steps && 2ll * ctas * slabs * s.batch <= 2 * 148) ctas *= 2;
-  return ctas;
-}
-
-template <typename K, typename... Args>
-int launch(K kernel, int slab, int warps, int steps, int smem, const Shape& s, cudaStream_t stream, Args... args) {
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return GEMM_ERR_LAUNCH;
-  const int slabs = (s.dim + slab - 1) / slab, ctas = warps > 1 ? cluster_ctas(s, slabs, warps * steps) : 1;
-  cudaLaunchConfig_t cfg = {};
-  if ((long long)slabs * ctas * s.batch > 0x7fffffffll) return GEMM_ERR_SHAPE;
-  cfg.gridDim = dim3((unsigned)(slabs * ctas * s.batch));
-  cfg.blockDim = dim3(warps * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
+// A launch with the cluster that suits it: sequences and channels that do not fit on the machine at once run in waves, the larger
+// the cluster the more of them, each of as many rounds as its warps need for the sequence, and one for its start; a round with
+// links between CTAs takes half as long again.  us forward | backward by cluster size, bf16 (batch x steps x channels):
+//   8 x 1024 x 1024    1: 26 | 38     2: 25 | 33     4: 30 | 39     8: 35 | 49
+//   64 x 128 x 1024    1: 25 | 35     2: 47 | 49
+//   3 x 8192 x 1024    4: 63 | 102    5: 55 | 88     6: 72 | 119    8: 62 | 101
+//   1 x 16384 x 2368   6: 88 | 141    7: 80 | 124    8: 100 | 174
+//   1 x 30011 x 2048   4: 141 | 262   7: 135 | 215   8: 121 | 190
+//   1 x 60000 x 64     4: 270 | 510   8: 145 | 281   12: 107 | 203   16: 88 | 164
+template <auto KERNEL, int VEC, int WARPS, int STEPS, typename... Args>
+int launch(size_t smem, const Shape& s, cudaStream_t stream, Args... args) {
+  constexpr size_t cta_links = 2 * 32 * sizeof(Link<VEC>);
+  static std::atomic<int> held[kMaxCtas + 1];               // clusters of each size that the machine holds at once
+  const long long units = (long long)((s.dim + 32 * VEC - 1) / (32 * VEC)) * s.batch;
+  if (units * kMaxCtas > 0x7fffffffll) return GEMM_ERR_SHAPE;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {(unsigned)ctas, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+  auto clusters_of = [&](int ctas) {
+    cfg.gridDim = dim3((unsigned)(units * ctas));
+    cfg.dynamicSmemBytes = smem + ctas * cta_links;
+    attr.val.clusterDim = {(unsigned)ctas, 1, 1};
+  };
+  int best = 1;
+  if (WARPS > 1) {
+    if (held[1] == 0) {
+      if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(smem + kMaxCtas * cta_links)) != cudaSuccess ||
+          cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return GEMM_ERR_LAUNCH;
+      for (int ctas = kMaxCtas; ctas > 0; --ctas) {
+        int n = 0;
+        clusters_of(ctas);
+        if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) return GEMM_ERR_LAUNCH;
+        held[ctas] = n;
+      }
+    }
+    double least = 0;
+    for (int ctas = 1; ctas <= kMaxCtas && (ctas == 1 || (long long)(ctas - 1) * WARPS * STEPS < s.steps); ++ctas) {
+      const int n = held[ctas];
+      if (n == 0) continue;
+      const long long waves = (units + n - 1) / n, rounds = (s.steps + ctas * WARPS * STEPS - 1) / (ctas * WARPS * STEPS);
+      const double time = (double)waves * (rounds + 1) * (ctas > 1 ? 1.5 : 1.0);
+      if (ctas == 1 || time < least) {
+        best = ctas;
+        least = time;
+      }
+    }
+  }
+  clusters_of(best);
+  return cudaLaunchKernelEx(&cfg, KERNEL, args...) == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -747,15 +781,16 @@ extern "C" int fbam_recurrence_fwd(const void* zgo, long long zb, long long zt, 
     int e = encode(&in, zgo, s, zb, zt, zk, 1, kFwdSteps);
     if (!e) e = encode(&out, y, s, yb, yt, 0, 0, kFwdSteps);
     if (e) return e;
-    return launch(recurrence_fwd_tma_kernel<kFwdSteps>, kSlab, kWarps, kFwdSteps, (int)sizeof(FwdSmem<kFwdSteps>), s, st, in, out, state_in, resets,
-                  state_out, saved, status, s);
+    return launch<recurrence_fwd_tma_kernel<kFwdSteps>, 2, kWarps, kFwdSteps>(sizeof(FwdSmem<kFwdSteps>), s, st, in, out, state_in, resets,
+                                                                              state_out, saved, status, s);
   }
   const bool two = pairs(zgo, dim, zb, zt, zk) && pairs(y, dim, yb, yt, 0);
-  auto go = [&](auto kernel, int vec, int warps) {
-    return launch(kernel, 32 * vec, warps, kSaved, 0, s, st, (const elem_t*)zgo, state_in, resets, (elem_t*)y, state_out, saved, status, s);
+  auto go = [&](auto vec, auto warps) {
+    return launch<recurrence_fwd_kernel<vec(), warps()>, vec(), warps(), kSaved>(
+        sizeof(Exchange<vec(), warps()>), s, st, (const elem_t*)zgo, state_in, resets, (elem_t*)y, state_out, saved, status, s);
   };
-  if (steps > kSaved) return go(recurrence_fwd_kernel<1, 8>, 1, 8);
-  return two ? go(recurrence_fwd_kernel<2, 1>, 2, 1) : go(recurrence_fwd_kernel<1, 1>, 1, 1);
+  if (steps > kSaved) return go(Int<1>(), Int<kWarps>());
+  return two ? go(Int<2>(), Int<1>()) : go(Int<1>(), Int<1>());
 }
 
 // dy: strides yb, yt; d_zgo: db, dt and dense (3, dim) steps.  d_state_out and d_state_in (batch, dim) fp32 or null.
@@ -773,14 +808,15 @@ extern "C" int fbam_recurrence_bwd(const void* zgo, long long zb, long long zt, 
     if (!e) e = encode(&d, dy, s, yb, yt, 0, 0, kSaved);
     if (!e) e = encode(&out, d_zgo, s, db, dt, dim, 3, kSaved);
     if (e) return e;
-    return launch(recurrence_bwd_tma_kernel<kSaved>, kSlab, kWarps, kSaved, (int)sizeof(BwdSmem<kSaved>), s, st, in, d, out, resets, saved,
-                  d_state_out, d_state_in, status, s);
+    return launch<recurrence_bwd_tma_kernel<kSaved>, 2, kWarps, kSaved>(sizeof(BwdSmem<kSaved>), s, st, in, d, out, resets, saved,
+                                                                        d_state_out, d_state_in, status, s);
   }
   const bool two = pairs(zgo, dim, zb, zt, zk) && pairs(dy, dim, yb, yt, 0) && pairs(d_zgo, dim, db, dt, 0);
-  auto go = [&](auto kernel, int vec, int warps) {
-    return launch(kernel, 32 * vec, warps, kSaved, 0, s, st, (const elem_t*)zgo, resets, saved, (const elem_t*)dy, d_state_out,
-                  (elem_t*)d_zgo, d_state_in, status, s, db, dt);
+  auto go = [&](auto vec, auto warps) {
+    return launch<recurrence_bwd_kernel<vec(), warps()>, vec(), warps(), kSaved>(
+        sizeof(Exchange<vec(), warps()>), s, st, (const elem_t*)zgo, resets, saved, (const elem_t*)dy, d_state_out, (elem_t*)d_zgo,
+        d_state_in, status, s, db, dt);
   };
-  if (steps > kSaved) return go(recurrence_bwd_kernel<1, 8>, 1, 8);
-  return two ? go(recurrence_bwd_kernel<2, 1>, 2, 1) : go(recurrence_bwd_kernel<1, 1>, 1, 1);
+  if (steps > kSaved) return go(Int<1>(), Int<kWarps>());
+  return two ? go(Int<2>(), Int<1>()) : go(Int<1>(), Int<1>());
 }

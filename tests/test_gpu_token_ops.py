@@ -147,6 +147,26 @@ def test_recurrence(b, t, d, dtype, time_major, extras):
         oracle.within(grads[1], want[1], F32, bwd)
 
 
+# From one CTA to as many as a cluster has, whole and partial rounds of it
+@pytest.mark.parametrize("b,t,d", [(93, 200, 64), (1, 2100, 1300), (3, 700, 1024), (1, 600, 2368), (2, 900, 1416), (1, 2500, 960),
+                                   (1, 2500, 65), (1, 1025, 72), (300, 100, 40), (7, 260, 500)])
+def test_recurrence_over_clusters(b, t, d):
+    gen = _gen("clusters", b, t, d)
+    zgo, state = _randn(gen, b, t, 3, d, dtype=BF).requires_grad_(), _randn(gen, b, d).requires_grad_()
+    resets = torch.rand(b, t, generator=gen, device="cuda") < 0.01
+    dy, d_state = _randn(gen, b, t, d, dtype=BF), _randn(gen, b, d)
+    y, last = ops.gated_recurrence(zgo, state, resets)
+    grads = torch.autograd.grad((y, last), (zgo, state), (dy, d_state))
+    held = zgo.detach(), state.detach()
+    fwd, bwd = _recurrence_bounds(*held, resets, dy, d_state)
+    want_y, want_last, _, _ = oracle.recurrence(*held, resets)
+    oracle.within(y, want_y, BF, fwd)
+    oracle.within(last, want_last, F32, fwd)
+    want = oracle.recurrence_grad(*held, resets, dy, d_state)
+    oracle.within(grads[0], want[0], BF, bwd)
+    oracle.within(grads[1], want[1], F32, bwd)
+
+
 def test_recurrence_in_pieces_is_the_whole():
     """The carried state of one call starts the next, down to single steps."""
     gen = _gen("pieces")
