@@ -271,6 +271,7 @@ embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint32
     }
     if (ranks > 1) cluster_sync(); else __syncthreads();         // the next pass reads what all CTAs placed, and overwrites totals
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int i = rank * kSortThreads + threadIdx.x; i < n; i += ranks * kSortThreads) {
     const int k = __ldcg(list_a + i).x;
     if (k < vocab && (i == 0 || __ldcg(list_a + i - 1).x != k)) atomicOr(present + k / 32, 1u << k % 32);
@@ -289,6 +290,8 @@ template <typename I, typename T, int VEC, int AHEAD>
 __global__ void __launch_bounds__(kSumThreads)
 embed_sum_kernel(const int2* __restrict__ list, const I* __restrict__ in, T* __restrict__ d_table, float* __restrict__ partial,
                  int2* __restrict__ next, const uint32_t* __restrict__ present, int n, int vocab, int dim, float scale, int lanes, int piece_blocks) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");            // for the sort, or for the step before
   if ((int)blockIdx.x >= piece_blocks) {
     const int word = (int)blockIdx.x - piece_blocks;
     const uint32_t there = present[word];
@@ -437,31 +440,40 @@ int launch_sort(const void* ids, int2* list, int2* list_b, uint32_t* present, in
 
 // The sums of one step, and with `present` the rows of absent ids.
 template <typename I, typename T, int VEC, int AHEAD>
-void launch_step(const int2* list, const void* in, void* d_table, float* partial, int2* next, const uint32_t* present, int n, int vocab,
+cudaError_t launch_step(const int2* list, const void* in, void* d_table, float* partial, int2* next, const uint32_t* present, int n, int vocab,
                  int dim, float scale, cudaStream_t s) {
   int lanes = row_lanes((dim + VEC - 1) / VEC);
   lanes = lanes > kSumThreads ? kSumThreads : lanes < kMinLanes ? kMinLanes : lanes;
   const int pieces = (n + kPiece - 1) / kPiece, per_block = kSumThreads / lanes;
   const int piece_blocks = (pieces + per_block - 1) / per_block;
   const dim3 grid(piece_blocks + (present != nullptr ? (vocab + kZeroRows - 1) / kZeroRows : 0), (dim + lanes * VEC - 1) / (lanes * VEC));
-  embed_sum_kernel<I, T, VEC, AHEAD><<<grid, kSumThreads, 0, s>>>(list, (const I*)in, (T*)d_table, partial, pieces > 1 ? next : nullptr,
-                                                                  present, n, vocab, dim, scale, lanes, piece_blocks);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kSumThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;                        // starts while the kernel before it ends
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, embed_sum_kernel<I, T, VEC, AHEAD>, list, (const I*)in, (T*)d_table, partial, pieces > 1 ? next : nullptr,
+                            present, n, vocab, dim, scale, lanes, piece_blocks);
 }
 
 // Of the first step there is a machine full, of the later ones a few CTAs: those take a piece's entries all at once.
 template <typename O, typename T, int VEC>
 int launch_sums(const int2* list, const void* d_out, void* d_table, float* partial, int2* next, const uint32_t* present, int n, int vocab,
                 int dim, float scale, cudaStream_t s) {
-  launch_step<O, T, VEC, 8>(list, d_out, d_table, partial, next, present, n, vocab, dim, scale, s);
-  for (int pieces = (n + kPiece - 1) / kPiece; pieces > 1; pieces = (n + kPiece - 1) / kPiece) {
+  cudaError_t e = launch_step<O, T, VEC, 8>(list, d_out, d_table, partial, next, present, n, vocab, dim, scale, s);
+  for (int pieces = (n + kPiece - 1) / kPiece; pieces > 1 && e == cudaSuccess; pieces = (n + kPiece - 1) / kPiece) {
     n = 2 * pieces;
     const float* in = partial;
     partial += (long long)n * dim;
     list = next;
     next += n;
-    launch_step<float, T, VEC == 1 ? 1 : 4, kPiece>(list, in, d_table, partial, next, nullptr, n, vocab, dim, scale, s);
+    e = launch_step<float, T, VEC == 1 ? 1 : 4, kPiece>(list, in, d_table, partial, next, nullptr, n, vocab, dim, scale, s);
   }
-  return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+  return e == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }
 
 template <typename O, typename T>
