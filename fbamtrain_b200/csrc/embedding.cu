@@ -4,10 +4,10 @@
 // row of zeros and has no gradient.
 //
 // Gradient:
-//   1. embed_sort_kernel  stable radix sort of (id, position) by one cluster of CTAs, and one bit for every id that comes up;
+//   1. embed_sort_kernel  stable radix sort of (id, position) by one cluster of CTAs.  Meanwhile the other clusters of the same
+//                         launch write the rows that no id names;
 //   2. embed_sum_kernel   the sorted order is cut into pieces of kPiece entries; a piece sums its runs of equal ids.  A run
-//                         that lies inside the piece is the row's gradient, one that crosses an edge leaves a partial sum.
-//                         Further CTAs write the rows that no id names;
+//                         that lies inside the piece is the row's gradient, one that crosses an edge leaves a partial sum;
 //   3. the same kernel on the partial sums, two entries a piece in the order of the pieces, until there is one piece.  However
 //      common an id is, its sum takes log32 of its count steps.
 //
@@ -18,16 +18,18 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "elem16.cuh"
 #include "gemm_tcgen05.h"
 
 namespace {
 
 constexpr int kPiece = 32;        // sorted positions of one piece
-constexpr int kZeroRows = 32;     // table rows per CTA that writes absent ones: the bits of one word
 constexpr int kSumThreads = 128, kMinLanes = 8;
 constexpr int kDigitBits = 10;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxSortCtas = 16;
+constexpr int kAbsentWords = 4096;      // of 32 ids each, that a cluster looks for at once
 
 template <int N>
 struct Vals { float v[N]; };
@@ -154,6 +156,61 @@ __device__ __forceinline__ int cluster_read(const int* smem, uint32_t rank) {
   return v;
 }
 
+// Zeros for the rows of ids that do not come up, next to the sort and without anything of it.  Cluster c of `clusters` has words
+// c, c + clusters, ... of 32 ids (neighbouring ids are about as common as one another); each of its CTAs looks through its part of
+// the ids for them, and then writes its part of the rows that none of them has found.  ABSENT_FIGURES
+template <typename Id>
+__device__ __forceinline__ void absent_rows(const Id* __restrict__ ids, uint8_t* d_table, long long row_bytes, int n, int vocab, int cluster,
+                                            int clusters) {
+  __shared__ int found[kAbsentWords];                           // by this CTA
+  __shared__ uint32_t there[kAbsentWords];                      // of the words that this CTA writes the rows of
+  constexpr int kAhead = 16;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rank = (int)cluster_rank(), ranks = (int)cluster_size();
+  const int words = (vocab + 31) / 32, ours = (words - cluster + clusters - 1) / clusters;
+  const long long begin = (long long)n * rank / ranks, end = (long long)n * (rank + 1) / ranks;
+  for (int w0 = 0; w0 < ours; w0 += kAbsentWords) {
+    const int count = min(ours - w0, kAbsentWords);
+    for (int w = threadIdx.x; w < count; w += kSortThreads) found[w] = 0;
+    __syncthreads();
+    for (long long i0 = begin + threadIdx.x; i0 < end; i0 += kAhead * kSortThreads) {
+      int key[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const long long i = i0 + u * kSortThreads;
+        key[u] = i < end ? key_of(ids, i, vocab) : vocab;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t word = (uint32_t)key[u] / 32, turn = word / (uint32_t)clusters, w = turn - w0;
+        if (key[u] < vocab && word - turn * clusters == (uint32_t)cluster && w < (uint32_t)count) {
+          const int bit = 1 << key[u] % 32;
+          if (!(*(volatile int*)&found[w] & bit)) atomicOr(&found[w], bit);      // common ids come up again and again
+        }
+      }
+    }
+    cluster_sync();
+    const int mine = (count - rank + ranks - 1) / ranks;
+    for (int l = threadIdx.x; l < mine; l += kSortThreads) {
+      int any = 0;
+#pragma unroll 8
+      for (int r = 0; r < ranks; ++r) any |= cluster_read(&found[l * ranks + rank], r);
+      there[l] = any;
+    }
+    cluster_sync();                                             // and nobody reads `found` any more
+    for (int r = warp; r < mine * 32; r += kSortWarps) {
+      const long long v = ((long long)(w0 + r / 32 * ranks + rank) * clusters + cluster) * 32 + r % 32;
+      if (v >= vocab || (there[r / 32] >> r % 32 & 1)) continue;
+      uint8_t* row = d_table + v * row_bytes;
+      // up to the first 16-byte boundary, pieces of 16 bytes, and the rest
+      const long long lead = min((long long)(-reinterpret_cast<uintptr_t>(row) & 15), row_bytes), body = (row_bytes - lead) & ~15ll;
+      if (2 * lane < lead) *reinterpret_cast<uint16_t*>(row + 2 * lane) = 0;
+      for (long long at = lead + 16 * lane; at < lead + body; at += 16 * 32) *reinterpret_cast<uint4*>(row + at) = make_uint4(0, 0, 0, 0);
+      if (lead + body + 2 * lane < row_bytes) *reinterpret_cast<uint16_t*>(row + lead + body + 2 * lane) = 0;
+    }
+    __syncthreads();
+  }
+}
+
 // Every warp owns a contiguous part of the input, so (CTA, warp, round, lane) is the input's order.  Per pass over `bits`
 // bits: count the digits of each warp's part, turn the counts into first output places (digits before, then CTAs before,
 // then warps before), and place the elements in order.  counts: [kSortWarps][bins] in shared memory.  A warp has the elements of
@@ -162,7 +219,12 @@ __device__ __forceinline__ int cluster_read(const int* smem, uint32_t rank) {
 // eight CTAs 65).
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads, 1)
-embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint32_t* present, int n, int vocab, int bits, int passes) {
+embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint8_t* d_table, long long row_bytes, int n, int vocab, int bits,
+                  int passes) {
+  if (blockIdx.x >= cluster_size()) {
+    absent_rows(ids, d_table, row_bytes, n, vocab, (int)(blockIdx.x / cluster_size()) - 1, (int)(gridDim.x / cluster_size()) - 1);
+    return;
+  }
   extern __shared__ int counts[];
   __shared__ int totals[1 << kDigitBits];
   __shared__ int warp_sums[kSortWarps];
@@ -178,7 +240,6 @@ embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint32
   const bool kept = per_warp <= kRounds * 32;
   int* mine = counts + warp * bins;
   const uint32_t before = (1u << lane) - 1;
-  for (int w = rank * kSortThreads + threadIdx.x; w < (vocab + 31) / 32; w += ranks * kSortThreads) present[w] = 0;
 
   int2 entry[kRounds];              // key and position
   for (int pass = 0; pass < passes; ++pass) {
@@ -271,15 +332,10 @@ embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint32
     }
     if (ranks > 1) cluster_sync(); else __syncthreads();         // the next pass reads what all CTAs placed, and overwrites totals
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  for (int i = rank * kSortThreads + threadIdx.x; i < n; i += ranks * kSortThreads) {
-    const int k = __ldcg(list_a + i).x;
-    if (k < vocab && (i == 0 || __ldcg(list_a + i - 1).x != k)) atomicOr(present + k / 32, 1u << k % 32);
-  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// sums of the pieces, and the rows without an id
+// sums of the pieces
 // ---------------------------------------------------------------------------------------------------------------
 // Entries in the order of their keys: key, and the row of `in` that is added (below 0: none).  A CTA has kSumThreads / lanes
 // groups of `lanes` threads; a group takes one piece and VEC columns per thread of the CTA's column slab (blockIdx.y).
@@ -289,20 +345,9 @@ embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint32
 template <typename I, typename T, int VEC, int AHEAD>
 __global__ void __launch_bounds__(kSumThreads)
 embed_sum_kernel(const int2* __restrict__ list, const I* __restrict__ in, T* __restrict__ d_table, float* __restrict__ partial,
-                 int2* __restrict__ next, const uint32_t* __restrict__ present, int n, int vocab, int dim, float scale, int lanes, int piece_blocks) {
+                 int2* __restrict__ next, int n, int vocab, int dim, float scale, int lanes) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");            // for the sort, or for the step before
-  if ((int)blockIdx.x >= piece_blocks) {
-    const int word = (int)blockIdx.x - piece_blocks;
-    const uint32_t there = present[word];
-    const Vals<VEC> zero = {};
-    for (int r = blockIdx.y; r < kZeroRows; r += gridDim.y) {
-      const int v = word * kZeroRows + r;
-      if (v >= vocab || (there >> r & 1)) continue;
-      for (int c = threadIdx.x * VEC; c < dim; c += kSumThreads * VEC) store_vals<VEC>(d_table + (long long)v * dim + c, zero);
-    }
-    return;
-  }
   __shared__ int keys[kSumThreads / kMinLanes][kPiece + 2], rows[kSumThreads / kMinLanes][kPiece];
   const int groups = kSumThreads / lanes, group = threadIdx.x / lanes;
   for (int i = threadIdx.x; i < groups * (kPiece + 2); i += kSumThreads) {
@@ -397,91 +442,93 @@ void launch_fwd(const void* ids, const void* table, long long ld, void* out, lon
 }
 
 template <typename Id>
-int launch_sort(const void* ids, int2* list, int2* list_b, uint32_t* present, int n, int vocab, cudaStream_t s) {
+int launch_sort(const void* ids, int2* list, int2* list_b, void* d_table, long long row_bytes, int n, int vocab, cudaStream_t s) {
   int total_bits = 1;
   while ((1ll << total_bits) <= vocab) ++total_bits;      // keys run up to vocab
   const int passes = (total_bits + kDigitBits - 1) / kDigitBits, bits = (total_bits + passes - 1) / passes;
-  static int most = 0;                              // CTAs of a cluster: sixteen where the device has room for it, which it need not
-  const int smem_most = kSortWarps * (1 << kDigitBits) * (int)sizeof(int);
-  if (most == 0) {
-    if (cudaFuncSetAttribute(embed_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_most) != cudaSuccess)
-      return GEMM_ERR_LAUNCH;
-    int clusters = 0;
-    cudaLaunchConfig_t probe = {};
-    probe.gridDim = dim3(kMaxSortCtas);
-    probe.blockDim = dim3(kSortThreads);
-    probe.dynamicSmemBytes = smem_most;
-    cudaLaunchAttribute size;
-    size.id = cudaLaunchAttributeClusterDimension;
-    size.val.clusterDim = {kMaxSortCtas, 1, 1};
-    probe.attrs = &size;
-    probe.numAttrs = 1;
-    const bool wide = cudaFuncSetAttribute(embed_sort_kernel<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-                      cudaOccupancyMaxActiveClusters(&clusters, embed_sort_kernel<Id>, &probe) == cudaSuccess && clusters > 0;
-    if (!wide) cudaGetLastError();
-    most = wide ? kMaxSortCtas : 8;
-  }
-  int ctas = 1;
-  while (ctas < most && n > ctas * kSortThreads) ctas *= 2;       // one round per warp and pass where that is enough
-  const int smem = kSortWarps * (1 << bits) * (int)sizeof(int);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
+  static std::atomic<int> held[kMaxSortCtas + 1];   // clusters of 1, 2, 4, 8 and 16 CTAs that the machine holds at once; -1: none
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {(unsigned)ctas, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, embed_sort_kernel<Id>, (const Id*)ids, list, list_b, present, n, vocab, bits,
+  auto clusters_of = [&](int ctas, int clusters, int smem) {
+    cfg.gridDim = dim3((unsigned)(ctas * clusters));
+    cfg.dynamicSmemBytes = smem;
+    attr.val.clusterDim = {(unsigned)ctas, 1, 1};
+  };
+  if (held[1] == 0) {
+    const int most = kSortWarps * (1 << kDigitBits) * (int)sizeof(int);
+    if (cudaFuncSetAttribute(embed_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
+        cudaFuncSetAttribute(embed_sort_kernel<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return GEMM_ERR_LAUNCH;
+    for (int ctas = kMaxSortCtas; ctas > 0; ctas /= 2) {
+      int k = 0;
+      clusters_of(ctas, 1, most);
+      if (cudaOccupancyMaxActiveClusters(&k, embed_sort_kernel<Id>, &cfg) != cudaSuccess) return GEMM_ERR_LAUNCH;
+      held[ctas] = k > 0 ? k : -1;
+    }
+  }
+  int ctas = 1;
+  while (ctas < kMaxSortCtas && n > ctas * kSortThreads && held[2 * ctas] > 0) ctas *= 2;      // one round per warp and pass where that is enough
+  const int others = held[ctas] - 1, words = (vocab + 31) / 32;
+  clusters_of(ctas, 1 + (others < 1 ? 1 : others < words ? others : words), kSortWarps * (1 << bits) * (int)sizeof(int));
+  return cudaLaunchKernelEx(&cfg, embed_sort_kernel<Id>, (const Id*)ids, list, list_b, (uint8_t*)d_table, row_bytes, n, vocab, bits,
                             passes) == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }
 
-// The sums of one step, and with `present` the rows of absent ids.
-template <typename I, typename T, int VEC, int AHEAD>
-cudaError_t launch_step(const int2* list, const void* in, void* d_table, float* partial, int2* next, const uint32_t* present, int n, int vocab,
-                 int dim, float scale, cudaStream_t s) {
-  int lanes = row_lanes((dim + VEC - 1) / VEC);
-  lanes = lanes > kSumThreads ? kSumThreads : lanes < kMinLanes ? kMinLanes : lanes;
-  const int pieces = (n + kPiece - 1) / kPiece, per_block = kSumThreads / lanes;
-  const int piece_blocks = (pieces + per_block - 1) / per_block;
-  const dim3 grid(piece_blocks + (present != nullptr ? (vocab + kZeroRows - 1) / kZeroRows : 0), (dim + lanes * VEC - 1) / (lanes * VEC));
+// A launch that starts while the kernel before it ends
+template <typename K, typename... Args>
+cudaError_t launch_early(K kernel, dim3 grid, int threads, cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kSumThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = s;
-  cudaLaunchAttribute attr;                        // starts while the kernel before it ends
+  cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, embed_sum_kernel<I, T, VEC, AHEAD>, list, (const I*)in, (T*)d_table, partial, pieces > 1 ? next : nullptr,
-                            present, n, vocab, dim, scale, lanes, piece_blocks);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// The sums of one step
+template <typename I, typename T, int VEC, int AHEAD>
+cudaError_t launch_step(const int2* list, const void* in, void* d_table, float* partial, int2* next, int n, int vocab, int dim, float scale,
+                        cudaStream_t s) {
+  int lanes = row_lanes((dim + VEC - 1) / VEC);
+  lanes = lanes > kSumThreads ? kSumThreads : lanes < kMinLanes ? kMinLanes : lanes;
+  const int pieces = (n + kPiece - 1) / kPiece, per_block = kSumThreads / lanes;
+  const dim3 grid((pieces + per_block - 1) / per_block, (dim + lanes * VEC - 1) / (lanes * VEC));
+  return launch_early(embed_sum_kernel<I, T, VEC, AHEAD>, grid, kSumThreads, s, list, (const I*)in, (T*)d_table, partial,
+                      pieces > 1 ? next : nullptr, n, vocab, dim, scale, lanes);
 }
 
 // Of the first step there is a machine full, of the later ones a few CTAs: those take a piece's entries all at once.
 template <typename O, typename T, int VEC>
-int launch_sums(const int2* list, const void* d_out, void* d_table, float* partial, int2* next, const uint32_t* present, int n, int vocab,
-                int dim, float scale, cudaStream_t s) {
-  cudaError_t e = launch_step<O, T, VEC, 8>(list, d_out, d_table, partial, next, present, n, vocab, dim, scale, s);
+int launch_sums(const int2* list, const void* d_out, void* d_table, float* partial, int2* next, int n, int vocab, int dim,
+                float scale, cudaStream_t s) {
+  cudaError_t e = launch_step<O, T, VEC, 8>(list, d_out, d_table, partial, next, n, vocab, dim, scale, s);
   for (int pieces = (n + kPiece - 1) / kPiece; pieces > 1 && e == cudaSuccess; pieces = (n + kPiece - 1) / kPiece) {
     n = 2 * pieces;
     const float* in = partial;
     partial += (long long)n * dim;
     list = next;
     next += n;
-    e = launch_step<float, T, VEC == 1 ? 1 : 4, kPiece>(list, in, d_table, partial, next, nullptr, n, vocab, dim, scale, s);
+    e = launch_step<float, T, VEC == 1 ? 1 : 4, kPiece>(list, in, d_table, partial, next, n, vocab, dim, scale, s);
   }
   return e == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }
 
-template <typename O, typename T>
-int launch_sums_vec(const int2* list, const void* d_out, void* d_table, float* partial, int2* next, const uint32_t* present, int n,
-                    int vocab, int dim, float scale, cudaStream_t s) {
+template <typename Id, typename O, typename T>
+int backward(const void* ids, int2* list, int2* list_b, const void* d_out, void* d_table, float* partial, int2* next, int n, int vocab,
+             int dim, float scale, cudaStream_t s) {
+  if (const int e = launch_sort<Id>(ids, list, list_b, d_table, (long long)dim * (int)sizeof(T), n, vocab, s)) return e;
   const bool vec = dim % 8 == 0 && aligned16(d_out) && aligned16(d_table) && aligned16(partial);
-  return vec ? launch_sums<O, T, 16 / sizeof(O)>(list, d_out, d_table, partial, next, present, n, vocab, dim, scale, s)
-             : launch_sums<O, T, 1>(list, d_out, d_table, partial, next, present, n, vocab, dim, scale, s);
+  return vec ? launch_sums<O, T, 16 / sizeof(O)>(list, d_out, d_table, partial, next, n, vocab, dim, scale, s)
+             : launch_sums<O, T, 1>(list, d_out, d_table, partial, next, n, vocab, dim, scale, s);
 }
 
 }  // namespace
@@ -503,8 +550,8 @@ extern "C" int fbam_embed_fwd(const void* ids, int ids64, const void* table, lon
 }
 
 // 8-byte words and fp32 values of the workspaces of fbam_embed_bwd
-extern "C" void fbam_embed_bwd_workspace(long long n, int vocab, int dim, long long* words, long long* floats) {
-  *words = 2 * n + ((long long)vocab + 63) / 64;
+extern "C" void fbam_embed_bwd_workspace(long long n, int dim, long long* words, long long* floats) {
+  *words = 2 * n;
   *floats = 0;
   for (long long pieces = (n + kPiece - 1) / kPiece; pieces > 1; pieces = (2 * pieces + kPiece - 1) / kPiece) {
     *words += 2 * pieces;
@@ -516,12 +563,11 @@ extern "C" int fbam_embed_bwd(const void* ids, int ids64, const void* d_out, int
                               long long n, int vocab, int dim, float scale, void* words, float* partial, void* stream) {
   if (n <= 0 || vocab <= 0 || dim <= 0 || (out_fp32 && !table_fp32) || n > 0x3fffffffll || vocab > 0x3fffffff) return GEMM_ERR_SHAPE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  int2 *list = reinterpret_cast<int2*>(words), *list_b = list + n, *next = list_b + n + ((long long)vocab + 63) / 64;
-  uint32_t* present = reinterpret_cast<uint32_t*>(list_b + n);
-  const int e = ids64 ? launch_sort<long long>(ids, list, list_b, present, (int)n, vocab, s)
-                      : launch_sort<int>(ids, list, list_b, present, (int)n, vocab, s);
-  if (e) return e;
-  if (!table_fp32) return launch_sums_vec<elem_t, elem_t>(list, d_out, d_table, partial, next, present, (int)n, vocab, dim, scale, s);
-  if (out_fp32) return launch_sums_vec<float, float>(list, d_out, d_table, partial, next, present, (int)n, vocab, dim, scale, s);
-  return launch_sums_vec<elem_t, float>(list, d_out, d_table, partial, next, present, (int)n, vocab, dim, scale, s);
+  int2 *list = reinterpret_cast<int2*>(words), *list_b = list + n, *next = list_b + n;
+  auto go = [&](auto id) {
+    using Id = decltype(id);
+    const auto run = !table_fp32 ? backward<Id, elem_t, elem_t> : out_fp32 ? backward<Id, float, float> : backward<Id, elem_t, float>;
+    return run(ids, list, list_b, d_out, d_table, partial, next, (int)n, vocab, dim, scale, s);
+  };
+  return ids64 ? go((long long)0) : go(0);
 }

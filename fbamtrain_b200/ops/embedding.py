@@ -43,7 +43,7 @@ class _EmbedTokens(torch.autograd.Function):
         d_table = d_out.new_empty((vocab, dim), dtype=dtype)
         lib = nv.lib(elem)
         words, floats = C.c_longlong(), C.c_longlong()
-        lib.fbam_embed_bwd_workspace(n, vocab, dim, C.byref(words), C.byref(floats))
+        lib.fbam_embed_bwd_workspace(n, dim, C.byref(words), C.byref(floats))
         work = flat.new_empty(words.value, dtype=torch.int64)
         partial = d_out.new_empty(floats.value, dtype=F32)
         nv.check(lib.fbam_embed_bwd(flat.data_ptr(), flat.dtype == torch.int64, d_out.data_ptr(), d_out.dtype == F32,
