@@ -12,9 +12,10 @@
 //      common an id is, its sum takes log32 of its count steps.
 //
 // Bound by memory, and below some ten thousand tokens by the latency of four launches.  Four rows are on their way at once in a
-// look-up (65536 rows of 2048 from fp32 to bf16: 85 us, 4.9 TB/s of DRAM traffic); a piece's keys and positions come through
-// shared memory so that eight rows can be (gradient of the same, 100003 rows of fp32: 186 us, 5.6 TB/s).  The partial sums, a
-// sixteenth of the rows at most, are taken 32 at a time by few CTAs (16 + 10 + 8 us there).
+// look-up (65536 rows of 2048 from fp32 to bf16: 86 us, 4.9 TB/s of DRAM traffic); a piece's keys and positions come through
+// shared memory so that eight rows can be.  The gradient of the same, 100003 rows of fp32, takes 220 us: sort and 655 MB of zeros,
+// then the first sums (73 us: 270 MB read, 150 written) and their partial sums, a sixteenth of the rows at most and taken 32 at a
+// time by few CTAs (14 + 8 + 7 us).  Each step of the sums starts while the one before it ends.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -158,7 +159,8 @@ __device__ __forceinline__ int cluster_read(const int* smem, uint32_t rank) {
 
 // Zeros for the rows of ids that do not come up, next to the sort and without anything of it.  Cluster c of `clusters` has words
 // c, c + clusters, ... of 32 ids (neighbouring ids are about as common as one another); each of its CTAs looks through its part of
-// the ids for them, and then writes its part of the rows that none of them has found.  ABSENT_FIGURES
+// the ids for them, and then writes its part of the rows that none of them has found.
+// (By further CTAs of the first sums instead, from bits that the sort left: gradient of 131072 of 262144 x 768 bf16 201 us, not 161.)
 template <typename Id>
 __device__ __forceinline__ void absent_rows(const Id* __restrict__ ids, uint8_t* d_table, long long row_bytes, int n, int vocab, int cluster,
                                             int clusters) {
@@ -473,6 +475,11 @@ int launch_sort(const void* ids, int2* list, int2* list_b, void* d_table, long l
   }
   int ctas = 1;
   while (ctas < kMaxSortCtas && n > ctas * kSortThreads && held[2 * ctas] > 0) ctas *= 2;      // one round per warp and pass where that is enough
+  // Clusters of sixteen leave a third of the machine unused, so where the zeros that are certain to come take longer than the sort
+  // takes with eight CTAs (0.29 ns an entry and pass; sixteen's six other clusters write 4.8 TB/s), eight it is.  us of the gradient
+  // with 16 | 8: 65536 of 100003 x 2048 fp32 238 | 220; 30000 of 50021 x 1029 bf16 113 | 111; 131072 of 262144 x 768 bf16 161 | 205;
+  // 131072 of 4096 x 1024 bf16 120 | 142
+  if (ctas == kMaxSortCtas && held[ctas / 2] > 0 && (double)(vocab - n) * row_bytes > 1400.0 * passes * n) ctas /= 2;
   const int others = held[ctas] - 1, words = (vocab + 31) / 32;
   clusters_of(ctas, 1 + (others < 1 ? 1 : others < words ? others : words), kSortWarps * (1 << bits) * (int)sizeof(int));
   return cudaLaunchKernelEx(&cfg, embed_sort_kernel<Id>, (const Id*)ids, list, list_b, (uint8_t*)d_table, row_bytes, n, vocab, bits,
