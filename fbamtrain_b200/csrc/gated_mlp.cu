@@ -700,49 +700,74 @@ extern "C" int fbam_gated_block_fwd(const void* x, long long ldx, const void* w_
   return fbam_product(h, inner, 0, w_out, ld_out, 0, rows, out_dim, inner, y, out_dim, b_out, residual, out_dim, nullptr, 0, status, stream);
 }
 
-// The block's backward; a gradient whose pointer is null is not wanted.  hidden, the inner width without its padding, is the width
-// of d_w_out; dx has width columns of the depth.  slabs: [splits][..] fp32 for a weight gradient that is split along the rows.
-// d_b_out: out_dim rounded up to 8, dy then dense and that wide; col_work as fbam_colsum_partials says.
+// The block's backward; a gradient whose pointer is null is not wanted.  slabs: [splits][..] fp32 for a weight gradient
+// that is split along the rows.  d_b_out: out_dim rounded up to 8, dy then dense and that wide; col_work as fbam_colsum_partials says.
 extern "C" int fbam_gated_block_bwd(const void* dy, long long ldy, const void* x, long long ldx, const void* w_in, long long ld_in,
                                     const void* w_out, long long ld_out, const float* v, const float* g, const void* h, void* d_vg,
                                     float* col_sums, void* d_b_in, void* dx, void* d_w_in, void* d_w_out, void* d_b_out, float* col_work,
-                                    float* slabs_in, int splits_in, float* slabs_out, int splits_out, int rows, int inner, int hidden,
-                                    int depth, int width, int out_dim, int act, int* status, void* stream) {
+                                    float* slabs_in, int splits_in, float* slabs_out, int splits_out, int rows, int inner, int depth,
+                                    int out_dim, int act, int* status, void* stream) {
   int e = 0;
   if (d_vg != nullptr)
     e = fbam_gated_bwd(dy, ldy, w_out, ld_out, v, g, d_vg, col_sums, d_b_in, rows, inner, out_dim, act, status, stream);
   if (!e && dx != nullptr)
-    e = fbam_product(d_vg, 2ll * inner, 0, w_in, ld_in, 1, rows, width, 2 * inner, dx, width, nullptr, nullptr, 0, nullptr, 0, status, stream);
+    e = fbam_product(d_vg, 2ll * inner, 0, w_in, ld_in, 1, rows, depth, 2 * inner, dx, depth, nullptr, nullptr, 0, nullptr, 0, status, stream);
   if (!e && d_w_in != nullptr)
-    e = fbam_product(d_vg, 2ll * inner, 1, x, ldx, 1, 2 * inner, width, rows, d_w_in, width, nullptr, nullptr, 0, slabs_in, splits_in, status,
+    e = fbam_product(d_vg, 2ll * inner, 1, x, ldx, 1, 2 * inner, depth, rows, d_w_in, depth, nullptr, nullptr, 0, slabs_in, splits_in, status,
                      stream);
   if (!e && d_w_out != nullptr)
-    e = fbam_product(dy, ldy, 1, h, inner, 1, out_dim, hidden, rows, d_w_out, hidden, nullptr, nullptr, 0, slabs_out, splits_out, status,
+    e = fbam_product(dy, ldy, 1, h, inner, 1, out_dim, inner, rows, d_w_out, inner, nullptr, nullptr, 0, slabs_out, splits_out, status,
                      stream);
   if (!e && d_b_out != nullptr) e = fbam_colsum_to(dy, nullptr, nullptr, d_b_out, 1, col_work, rows, (out_dim + 7) / 8 * 8, stream);
   return e;
 }
 
 namespace {
+// U: elements a thread moves at once
+template <int U>
 __global__ void __launch_bounds__(256)
-refit_kernel(const elem_t* __restrict__ src, long long ld, elem_t* __restrict__ dst, int src_rows, int src_cols, int dst_rows, int dst_cols,
-             long long total) {
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long row = i / dst_cols;
-    const int c = (int)(i - row * dst_cols);
-    const long long block = row / dst_rows;
-    const int r = (int)(row - block * dst_rows);
-    dst[i] = r < src_rows && c < src_cols ? src[(block * src_rows + r) * ld + c] : f2e(0.0f);
+refit_kernel(const elem_t* __restrict__ src, uint32_t ld, elem_t* __restrict__ dst, uint32_t src_rows, uint32_t src_cols, uint32_t dst_rows,
+             uint32_t dst_cols, uint32_t units) {
+  struct alignas(2 * U) Unit { elem_t e[U]; };
+  constexpr int kAhead = 4;
+  const uint32_t across = dst_cols / U, step = gridDim.x * 256;
+  for (uint32_t i0 = blockIdx.x * 256 + threadIdx.x; i0 < units; i0 += kAhead * step) {
+    Unit x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const uint32_t i = i0 + k * step, row = i / across, c = (i - row * across) * U, block = row / dst_rows, r = row - block * dst_rows;
+#pragma unroll
+      for (int j = 0; j < U; ++j) x[k].e[j] = f2e(0.0f);
+      if (i < units && r < src_rows && c < src_cols)
+        x[k] = *reinterpret_cast<const Unit*>(src + (long long)(block * src_rows + r) * ld + c);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const uint32_t i = i0 + k * step;
+      if (i < units) *reinterpret_cast<Unit*>(dst + (long long)i * U) = x[k];
+    }
   }
 }
 }  // namespace
 
-// blocks of src_rows x src_cols (pitch ld) -> dense blocks of dst_rows x dst_cols: padded with zeros, or cut.
+// blocks of src_rows x src_cols (pitch ld) -> dense blocks of dst_rows x dst_cols: padded with zeros, or cut.  In pieces of 16, 8, 4
+// or 2 bytes, whichever all rows begin and end on: 5460 rows of 1000 bf16 to 5472 in
+// 6.4 us, 1000 of 2730 to 2736 in 6.5 (element by element, with a division of 64 bits for each, 24 and 14).
 extern "C" int fbam_refit(const void* src, long long ld, void* dst, int blocks, int src_rows, int src_cols, int dst_rows, int dst_cols,
                           void* stream) {
-  const long long total = (long long)blocks * dst_rows * dst_cols, need = (total + 255) / 256;
-  if (blocks <= 0 || src_rows < 0 || src_cols < 0 || dst_rows <= 0 || dst_cols <= 0) return GEMM_ERR_SHAPE;
-  refit_kernel<<<(unsigned)(need < 148 * 16 ? need : 148 * 16), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      (const elem_t*)src, ld, (elem_t*)dst, src_rows, src_cols, dst_rows, dst_cols, total);
+  const long long total = (long long)blocks * dst_rows * dst_cols;
+  if (blocks <= 0 || src_rows < 0 || src_cols < 0 || dst_rows <= 0 || dst_cols <= 0 || ld < 0 || ld > 0x7fffffff || total > 0x7fffffff ||
+      (long long)blocks * src_rows > 0x7fffffff)
+    return GEMM_ERR_SHAPE;
+  const uintptr_t odd = reinterpret_cast<uintptr_t>(src) / 2 | reinterpret_cast<uintptr_t>(dst) / 2 | (uintptr_t)ld | src_cols | dst_cols;
+  auto go = [&](auto kernel, int u) {
+    const long long units = total / u, need = (units + 1023) / 1024;
+    kernel<<<(unsigned)(need < 148 * 8 ? need : 148 * 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+        (const elem_t*)src, (uint32_t)ld, (elem_t*)dst, src_rows, src_cols, dst_rows, dst_cols, (uint32_t)units);
+  };
+  if (odd % 8 == 0) go(refit_kernel<8>, 8);
+  else if (odd % 4 == 0) go(refit_kernel<4>, 4);
+  else if (odd % 2 == 0) go(refit_kernel<2>, 2);
+  else go(refit_kernel<1>, 1);
   return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }

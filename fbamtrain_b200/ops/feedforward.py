@@ -2,7 +2,8 @@
 ``(v, g) = x W_inᵀ + b_in``; the first half of the projection is the value and the second the gate, as in ``geglu``.
 
 Widths that are no multiple of 8 are refitted: rows of ``x``, the weights and ``dy`` get zeros up to the next one (tensor maps
-want 16-byte rows), which add nothing to any product.
+want 16-byte rows), which add nothing to any product; gradients are formed in padded widths and cut, since a product that stores
+rows of other lengths stores them value by value (1000 x 2730 from 1001 rows: 56 us, padded and cut 29 + 6).
 """
 from __future__ import annotations
 
@@ -83,7 +84,7 @@ def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
 
 def _slabs(like, splits, m, n):
     """fp32 workspace of a weight gradient in ``splits`` parts, or None where it is not split."""
-    return like.new_empty((splits, m, n), dtype=F32) if splits > 1 and m * n % 8 == 0 else None
+    return like.new_empty((splits, m, n), dtype=F32) if splits > 1 else None
 
 
 class _GatedMlp(torch.autograd.Function):
@@ -100,7 +101,7 @@ class _GatedMlp(torch.autograd.Function):
         shape, inner, act = ctx.meta
         need_x, need_in, need_out, need_bin, need_bout, _, need_res = ctx.needs_input_grad
         rows, wide = h.shape
-        dim, width = w2.shape[0], shape[-1]
+        dim, width, depth = w2.shape[0], shape[-1], x2.shape[1]
         dy2 = _flat(dy)
         if dim % 8:
             dy2 = _refit(dy2, 1, rows, _up8(dim))
@@ -112,15 +113,15 @@ class _GatedMlp(torch.autograd.Function):
             if need_bin:
                 db_in, sums = h.new_empty(2 * wide), vg.new_empty(((rows + 31) // 32, 2 * wide))
             if need_x:
-                dx = None if tuned else h.new_empty((rows, width))
+                dx = None if tuned else h.new_empty((rows, depth))
             if need_in and not tuned:
-                dw_in = h.new_empty((2 * wide, width))
-                splits_in = weight_grad_splits(2 * wide, width, rows)
-                slabs_in = _slabs(h, splits_in, 2 * wide, width)
+                dw_in = h.new_empty((2 * wide, depth))
+                splits_in = weight_grad_splits(2 * wide, depth, rows)
+                slabs_in = _slabs(h, splits_in, 2 * wide, depth)
         if need_out and not tuned:
-            dw_out = h.new_empty((dim, inner))
-            splits_out = weight_grad_splits(dim, inner, rows)
-            slabs_out = _slabs(h, splits_out, dim, inner)
+            dw_out = h.new_empty((dim, wide))
+            splits_out = weight_grad_splits(dim, wide, rows)
+            slabs_out = _slabs(h, splits_out, dim, wide)
         if need_bout:
             db_out = h.new_empty(_up8(dim))
             parts = _sum_partials("fbam_colsum_partials", rows, _up8(dim), 0)
@@ -130,15 +131,19 @@ class _GatedMlp(torch.autograd.Function):
             dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), w1.data_ptr(), w1.stride(0), w2.data_ptr(), wide, v,
             v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
             nv.addr(dw_out), nv.addr(db_out), nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0,
-            nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, inner, x2.shape[1], width, dim, act,
+            nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, depth, dim, act,
             nv.status_word(h.device).data_ptr(), nv.stream()), "fbam_gated_block_bwd")
         flops.add(2.0 * rows * inner * (dim * ((d_vg is not None) + (dw_out is not None)) + 2 * width * ((dx is not None) + (dw_in is not None))))
         if tuned:
-            dx = gemm(d_vg, w1[:, :width], b_mn=True) if need_x else None
-            dw_in = gemm(d_vg, x2[:, :width], a_mn=True, b_mn=True) if need_in else None
-            dw_out = gemm(dy2[:, :dim], h[:, :inner], a_mn=True, b_mn=True) if need_out else None
+            dx = gemm(d_vg, w1, b_mn=True) if need_x else None
+            dw_in = gemm(d_vg, x2, a_mn=True, b_mn=True) if need_in else None
+            dw_out = gemm(dy2[:, :dim], h, a_mn=True, b_mn=True) if need_out else None
+        if depth != width and dx is not None:
+            dx = _refit(dx, 1, rows, width)
+        if (wide != inner or depth != width) and dw_in is not None:
+            dw_in = _refit(dw_in, 2, inner, width)
         if wide != inner:
-            dw_in = None if dw_in is None else _refit(dw_in, 2, inner, width)
+            dw_out = None if dw_out is None else _refit(dw_out, 1, dim, inner)
             db_in = None if db_in is None else _refit(db_in.view(2, wide), 2, 1, inner).view(-1)
         if db_out is not None and dim % 8:
             db_out = db_out[:dim]

@@ -110,7 +110,7 @@ _ARGTYPES = {
     "fbam_recurrence_bwd": (_P, _L, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _P, _I, _I, _I, _P, _P),
     "fbam_gated_block_fwd": (_P, _L, _P, _L, _P, _P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P),
     "fbam_gated_block_bwd": (_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I,
-                             _I, _I, _P, _P),
+                             _P, _P),
     "fbam_refit": (_P, _L, _P, _I, _I, _I, _I, _I, _P),
     "fbam_gated_few_rows": (_P, _L, _P, _L, _P, _P, _L, _P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _P),
     "fbam_logprobs_fwd": (_P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _I, _I, _F, _P),
