@@ -469,9 +469,13 @@ int launch_sort(const void* ids, int2* list, int2* list_b, void* d_table, long l
     for (int ctas = kMaxSortCtas; ctas > 0; ctas /= 2) {
       int k = 0;
       clusters_of(ctas, 1, most);
-      if (cudaOccupancyMaxActiveClusters(&k, embed_sort_kernel<Id>, &cfg) != cudaSuccess) return GEMM_ERR_LAUNCH;
+      if (cudaOccupancyMaxActiveClusters(&k, embed_sort_kernel<Id>, &cfg) != cudaSuccess) {      // sixteen are for the device to grant
+        cudaGetLastError();
+        k = 0;
+      }
       held[ctas] = k > 0 ? k : -1;
     }
+    if (held[1] < 0) return GEMM_ERR_LAUNCH;
   }
   int ctas = 1;
   while (ctas < kMaxSortCtas && n > ctas * kSortThreads && held[2 * ctas] > 0) ctas *= 2;      // one round per warp and pass where that is enough

@@ -742,9 +742,13 @@ int launch(size_t smem, const Shape& s, cudaStream_t stream, Args... args) {
       for (int ctas = kMaxCtas; ctas > 0; --ctas) {
         int n = 0;
         clusters_of(ctas);
-        if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) return GEMM_ERR_LAUNCH;
+        if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {      // more than eight are for the device to grant
+          cudaGetLastError();
+          n = 0;
+        }
         held[ctas] = n;
       }
+      if (held[1] == 0) return GEMM_ERR_LAUNCH;
     }
     double least = 0;
     for (int ctas = 1; ctas <= kMaxCtas && (ctas == 1 || (long long)(ctas - 1) * WARPS * STEPS < s.steps); ++ctas) {

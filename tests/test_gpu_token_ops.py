@@ -92,6 +92,26 @@ def test_embedding_of_one_token_only():
         assert not grad[0].any() and not grad[2].any()
 
 
+@pytest.mark.parametrize("n,vocab,dim,dtype", [(700, 300_007, 5, BF), (5000, 2_000_003, 3, F32), (20_000, 2_000_003, 9, HALF),
+                                               (3000, 100_003, 1029, BF)])
+@pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
+def test_embedding_writes_every_row_of_the_gradient(n, vocab, dim, dtype, ids_dtype):
+    """Large tables of which few rows come up, in memory that held something else; rows of no whole number of 16-byte pieces."""
+    gen = _gen("absent", n, vocab, dim)
+    table = torch.zeros(vocab, dim, dtype=dtype, device="cuda").requires_grad_()
+    ids = torch.randint(0, vocab, (n,), generator=gen, device="cuda").to(ids_dtype)
+    ids[:2] = torch.tensor([0, vocab - 1])
+    d_out = _randn(gen, n, dim, dtype=dtype)
+    out = ops.embed_tokens(ids, table)
+    stale = torch.full_like(table, math.nan)
+    del stale
+    grad, = torch.autograd.grad((out,), (table,), (d_out,))
+    want, size = oracle.embed_grad(ids.long(), d_out, vocab, 1.0)
+    count = torch.bincount(ids.long(), minlength=vocab).unsqueeze(1)
+    oracle.within(grad, want, dtype, (count + 2) * 2.0 ** -24 * size)
+    assert not grad[count[:, 0] == 0].any()
+
+
 def test_embedding_table_beyond_32_bit_offsets():
     vocab, dim = 600_000, 4096                                # 2.5e9 values
     table = torch.zeros(vocab, dim, dtype=BF, device="cuda").requires_grad_()
