@@ -372,14 +372,33 @@ __device__ __forceinline__ void backward_out(const Vec<VEC> (&nf1)[STEPS], const
 // ---------------------------------------------------------------------------------------------------------------
 // Any alignment, and a few steps: inputs in registers by plain loads
 // ---------------------------------------------------------------------------------------------------------------
-template <int VEC, int STEPS>
-__device__ __forceinline__ void fetch(Raw<VEC> (&r)[STEPS], const elem_t* p, long long step, int n) {
-#pragma unroll
-  for (int t = 0; t < STEPS; ++t) {
-    r[t] = Raw<VEC>{0};
-    if (t < n) r[t].load(p + t * step);
+// A lane's VEC channels in a row of them; a lane behind the last one computes it too, and stores nothing.
+template <int VEC>
+struct Channels {
+  int ch;
+  bool in;
+  __device__ __forceinline__ Channels(int slab, int dim) {
+    const int own = (slab * 32 + (int)threadIdx.x % 32) * VEC;
+    in = own < dim;
+    ch = in ? own : dim - VEC;
   }
-}
+  template <int STEPS>
+  __device__ __forceinline__ void fetch(Raw<VEC> (&r)[STEPS], const elem_t* row, long long step, int n) const {
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) {
+      r[t].u = 0;
+      if (t < n) r[t].load(row + t * step + ch);
+    }
+  }
+  __device__ __forceinline__ Vec<VEC> load(const float* row) const {
+    if constexpr (VEC == 1) return {row[ch]};
+    else return {make_float2(row[ch], row[ch + 1])};
+  }
+  template <typename T>
+  __device__ __forceinline__ void put(T* row, Vec<VEC> v) const {
+    if (in) store(row + ch, v);
+  }
+};
 
 template <int VEC, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 2)
@@ -389,23 +408,21 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Exchange<VEC, WARPS>& ex = *reinterpret_cast<Exchange<VEC, WARPS>*>(smem_raw);
   ex.init();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = threadIdx.x / 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-  const int slabs = (s.dim + 32 * VEC - 1) / (32 * VEC), unit = blockIdx.x / ctas;
-  const int b = unit / slabs, own = (unit % slabs * 32 + lane) * VEC;
-  const bool in = own < s.dim;
-  const int ch = in ? own : s.dim - VEC;                    // lanes behind the last channel compute it too
-  Vec<VEC> carry = state_in != nullptr ? load<VEC>(state_in + (long long)b * s.dim + ch) : Vec<VEC>::all(0.0f);
+  const int slabs = (s.dim + 32 * VEC - 1) / (32 * VEC), unit = blockIdx.x / ctas, b = unit / slabs;
+  const Channels<VEC> c(unit % slabs, s.dim);
+  Vec<VEC> carry = state_in != nullptr ? c.load(state_in + (long long)b * s.dim) : Vec<VEC>::all(0.0f);
   int round = 0;
   for (int c0 = 0; c0 < s.states; c0 += ctas * WARPS, ++round) {
     const int chunk = c0 + rank * WARPS + warp, t0 = chunk * STEPS;
     const int n = min(STEPS, s.steps - t0);                 // may be below 0
     const uint32_t bits = reset_bits(resets, s, b, t0, n);
-    const elem_t* src = zgo + b * s.zb + t0 * s.zt + ch;
+    const elem_t* src = zgo + b * s.zb + t0 * s.zt;
     Raw<VEC> z[STEPS], g[STEPS], o[STEPS];
-    fetch(g, src + s.zk, s.zt, n);
-    fetch(z, src, s.zt, n);
-    fetch(o, src + 2 * s.zk, s.zt, n);
+    c.fetch(g, src + s.zk, s.zt, n);
+    c.fetch(z, src, s.zt, n);
+    c.fetch(o, src + 2 * s.zk, s.zt, n);
     Vec<VEC> nf1[STEPS];
     Link<VEC> link;
     forward_in<false>(nf1, link, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return g[t].get(); });
@@ -414,11 +431,11 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
     Vec<VEC> so[kAhead];
     forward_ahead(so, [&](int t) { return o[t].get(); });
     Vec<VEC> h = passing.take(ex, round, warp, false, carry, status);
-    elem_t* out = y + b * s.yb + t0 * s.yt + ch;
-    float* at = saved != nullptr && in ? saved + ((long long)b * s.states + chunk) * s.dim + ch : nullptr;
+    elem_t* out = y + b * s.yb + t0 * s.yt;
+    float* at = saved != nullptr && c.in ? saved + ((long long)b * s.states + chunk) * s.dim + c.ch : nullptr;
     forward_out<false>(nf1, so, h, at, s.dim, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return o[t].get(); },
-                       [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * s.yt, v); });
-    if (in && t0 + STEPS >= s.steps && n > 0) store(state_out + (long long)b * s.dim + ch, h);
+                       [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * s.yt, v); });
+    if (t0 + STEPS >= s.steps && n > 0) c.put(state_out + (long long)b * s.dim, h);
   }
   if (ctas > 1) cluster_sync();     // no CTA leaves while another may still read its links
 }
@@ -432,26 +449,24 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Exchange<VEC, WARPS>& ex = *reinterpret_cast<Exchange<VEC, WARPS>*>(smem_raw);
   ex.init();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = threadIdx.x / 32;
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-  const int slabs = (s.dim + 32 * VEC - 1) / (32 * VEC), unit = blockIdx.x / ctas;
-  const int b = unit / slabs, own = (unit % slabs * 32 + lane) * VEC;
-  const bool in = own < s.dim;
-  const int ch = in ? own : s.dim - VEC;
-  Vec<VEC> carry = d_state_out != nullptr ? load<VEC>(d_state_out + (long long)b * s.dim + ch) : Vec<VEC>::all(0.0f);
+  const int slabs = (s.dim + 32 * VEC - 1) / (32 * VEC), unit = blockIdx.x / ctas, b = unit / slabs;
+  const Channels<VEC> c(unit % slabs, s.dim);
+  Vec<VEC> carry = d_state_out != nullptr ? c.load(d_state_out + (long long)b * s.dim) : Vec<VEC>::all(0.0f);
   const int per_step = ctas * WARPS, rounds = (s.states + per_step - 1) / per_step;
   for (int round = 0; round < rounds; ++round) {
     const int chunk = (rounds - 1 - round) * per_step + rank * WARPS + warp, t0 = chunk * STEPS;
     const int n = min(STEPS, s.steps - t0);
     const uint32_t bits = reset_bits(resets, s, b, t0, n);
-    const elem_t* src = zgo + b * s.zb + t0 * s.zt + ch;
-    elem_t* out = d_zgo + b * db + t0 * dt + ch;
+    const elem_t* src = zgo + b * s.zb + t0 * s.zt;
+    elem_t* out = d_zgo + b * db + t0 * dt;
     Raw<VEC> z[STEPS], g[STEPS], o[STEPS], d[STEPS];
-    fetch(g, src + s.zk, s.zt, n);
-    fetch(z, src, s.zt, n);
-    fetch(o, src + 2 * s.zk, s.zt, n);
-    fetch(d, dy + b * s.yb + t0 * s.yt + ch, s.yt, n);
-    const Vec<VEC> h = n > 0 ? load<VEC>(saved + ((long long)b * s.states + chunk) * s.dim + ch) : Vec<VEC>::all(0.0f);
+    c.fetch(g, src + s.zk, s.zt, n);
+    c.fetch(z, src, s.zt, n);
+    c.fetch(o, src + 2 * s.zk, s.zt, n);
+    c.fetch(d, dy + b * s.yb + t0 * s.yt, s.yt, n);
+    const Vec<VEC> h = n > 0 ? c.load(saved + ((long long)b * s.states + chunk) * s.dim) : Vec<VEC>::all(0.0f);
     Vec<VEC> nf1[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
     Link<VEC> link;
     backward_in<false>(nf1, u, so1, dh0, link, n, bits, [&](int t) { return g[t].get(); }, [&](int t) { return o[t].get(); },
@@ -459,12 +474,12 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
     Passing<VEC, WARPS> passing;
     passing.send(ex, round, link, WARPS - 1 - warp, true);
     backward_states<false>(nf1, u, so1, dh0, h, bits, [&](int t) { return z[t].get(); },
-                           [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + 2 * s.dim, v); });
+                           [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt + 2 * s.dim, v); });
     const Vec<VEC> e = passing.take(ex, round, WARPS - 1 - warp, true, carry, status);
-    backward_out<false>(nf1, u, dh0, e, bits, [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt, v); },
-                        [&](int t, Vec<VEC> v) { if (in && t < n) store(out + t * dt + s.dim, v); });
+    backward_out<false>(nf1, u, dh0, e, bits, [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt, v); },
+                        [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt + s.dim, v); });
   }
-  if (in && rank == 0 && warp == 0 && d_state_in != nullptr) store(d_state_in + (long long)b * s.dim + ch, carry);
+  if (rank == 0 && warp == 0 && d_state_in != nullptr) c.put(d_state_in + (long long)b * s.dim, carry);
   if (ctas > 1) cluster_sync();
 }
 
