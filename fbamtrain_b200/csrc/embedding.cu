@@ -40,9 +40,12 @@ template <typename T, int N>
 struct Raw {
   static constexpr int kWords = sizeof(T) * N / 16;
   uint4 w[kWords];
+  // SHARED: the memory is written while kernels that read it are already resident, so it is read from L2
+  template <bool SHARED = false>
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < kWords; ++i)
+      w[i] = SHARED ? __ldcg(reinterpret_cast<const uint4*>(p) + i) : __ldg(reinterpret_cast<const uint4*>(p) + i);
   }
   __device__ __forceinline__ Vals<N> get() const {
     Vals<N> r;
@@ -63,7 +66,8 @@ struct Raw {
 template <typename T>
 struct Raw<T, 1> {
   T v;
-  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  template <bool SHARED = false>
+  __device__ __forceinline__ void load(const T* p) { v = SHARED ? __ldcg(p) : __ldg(p); }
   __device__ __forceinline__ Vals<1> get() const {
     if constexpr (sizeof(T) == 2) return {{e2f(v)}};
     else return {{v}};
@@ -343,11 +347,12 @@ embed_sort_kernel(const Id* __restrict__ ids, int2* list_a, int2* list_b, uint8_
 // groups of `lanes` threads; a group takes one piece and VEC columns per thread of the CTA's column slab (blockIdx.y).
 // What crosses the edges of a piece is left as two entries of the next step, with their rows in `partial`: the run that came in,
 // and the run that begins here and goes on; a run that covers the piece from edge to edge is the former.
-// AHEAD: entries of a thread on their way at once.
-template <typename I, typename T, int VEC, int AHEAD>
+// AHEAD: entries of a thread on their way at once.  PARTIAL: `in` is the `partial` of the step before.  That and `list` are written
+// while this kernel is already resident, so they are read by loads that go to L2; only d_out is read-only for its whole life.
+template <typename I, typename T, int VEC, int AHEAD, bool PARTIAL>
 __global__ void __launch_bounds__(kSumThreads)
-embed_sum_kernel(const int2* __restrict__ list, const I* __restrict__ in, T* __restrict__ d_table, float* __restrict__ partial,
-                 int2* __restrict__ next, int n, int vocab, int dim, float scale, int lanes) {
+embed_sum_kernel(const int2* list, const I* in, T* d_table, float* partial, int2* next, int n, int vocab, int dim, float scale,
+                 int lanes) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");            // for the sort, or for the step before
   __shared__ int keys[kSumThreads / kMinLanes][kPiece + 2], rows[kSumThreads / kMinLanes][kPiece];
@@ -356,7 +361,7 @@ embed_sum_kernel(const int2* __restrict__ list, const I* __restrict__ in, T* __r
     const int g = i / (kPiece + 2), k = i % (kPiece + 2);
     const long long e = ((long long)blockIdx.x * groups + g) * kPiece + k - 1;
     const bool in_list = e >= 0 && e < n;
-    const int2 entry = in_list ? list[e] : make_int2(-1, -1);
+    const int2 entry = in_list ? __ldcg(list + e) : make_int2(-1, -1);
     keys[g][k] = entry.x;
     if (k >= 1 && k <= kPiece) rows[g][k - 1] = entry.y;
   }
@@ -401,7 +406,7 @@ embed_sum_kernel(const int2* __restrict__ list, const I* __restrict__ in, T* __r
       const bool valid = i0 + u < count && my_key[i0 + u] < vocab;
       k[u] = valid ? my_key[i0 + u] : -1;
       const int row = valid ? my_row[i0 + u] : -1;
-      if (row >= 0 && col < dim) x[u].load(in + (long long)row * dim + col);
+      if (row >= 0 && col < dim) x[u].template load<PARTIAL>(in + (long long)row * dim + col);
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
@@ -506,14 +511,14 @@ cudaError_t launch_early(K kernel, dim3 grid, int threads, cudaStream_t s, Args.
 }
 
 // The sums of one step
-template <typename I, typename T, int VEC, int AHEAD>
+template <typename I, typename T, int VEC, int AHEAD, bool PARTIAL>
 cudaError_t launch_step(const int2* list, const void* in, void* d_table, float* partial, int2* next, int n, int vocab, int dim, float scale,
                         cudaStream_t s) {
   int lanes = row_lanes((dim + VEC - 1) / VEC);
   lanes = lanes > kSumThreads ? kSumThreads : lanes < kMinLanes ? kMinLanes : lanes;
   const int pieces = (n + kPiece - 1) / kPiece, per_block = kSumThreads / lanes;
   const dim3 grid((pieces + per_block - 1) / per_block, (dim + lanes * VEC - 1) / (lanes * VEC));
-  return launch_early(embed_sum_kernel<I, T, VEC, AHEAD>, grid, kSumThreads, s, list, (const I*)in, (T*)d_table, partial,
+  return launch_early(embed_sum_kernel<I, T, VEC, AHEAD, PARTIAL>, grid, kSumThreads, s, list, (const I*)in, (T*)d_table, partial,
                       pieces > 1 ? next : nullptr, n, vocab, dim, scale, lanes);
 }
 
@@ -521,14 +526,14 @@ cudaError_t launch_step(const int2* list, const void* in, void* d_table, float* 
 template <typename O, typename T, int VEC>
 int launch_sums(const int2* list, const void* d_out, void* d_table, float* partial, int2* next, int n, int vocab, int dim,
                 float scale, cudaStream_t s) {
-  cudaError_t e = launch_step<O, T, VEC, 8>(list, d_out, d_table, partial, next, n, vocab, dim, scale, s);
+  cudaError_t e = launch_step<O, T, VEC, 8, false>(list, d_out, d_table, partial, next, n, vocab, dim, scale, s);
   for (int pieces = (n + kPiece - 1) / kPiece; pieces > 1 && e == cudaSuccess; pieces = (n + kPiece - 1) / kPiece) {
     n = 2 * pieces;
     const float* in = partial;
     partial += (long long)n * dim;
     list = next;
     next += n;
-    e = launch_step<float, T, VEC == 1 ? 1 : 4, kPiece>(list, in, d_table, partial, next, n, vocab, dim, scale, s);
+    e = launch_step<float, T, VEC == 1 ? 1 : 4, kPiece, true>(list, in, d_table, partial, next, n, vocab, dim, scale, s);
   }
   return e == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }
