@@ -31,7 +31,8 @@ def _dense(x: torch.Tensor) -> torch.Tensor:
 
 
 def _flat(x: torch.Tensor) -> torch.Tensor:
-    """The rows of ``x``, dense, the first one on a 16-byte boundary."""
+    """The rows of ``x``, dense, the first one on a 16-byte boundary.  The pitch is the width: a single row counts as dense
+    whatever its stride says."""
     x = _dense(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
     return x.clone() if x.data_ptr() % 16 else x
 
@@ -39,7 +40,7 @@ def _flat(x: torch.Tensor) -> torch.Tensor:
 def _refit(src: torch.Tensor, blocks: int, rows: int, cols: int) -> torch.Tensor:
     """``src`` as ``blocks`` blocks of rows, each cut or padded with zeros to ``(rows, cols)``."""
     out = src.new_empty((blocks * rows, cols))
-    nv.check(nv.lib(src).fbam_refit(src.data_ptr(), src.stride(0), out.data_ptr(), blocks, src.shape[0] // blocks, src.shape[1],
+    nv.check(nv.lib(src).fbam_refit(src.data_ptr(), src.shape[1], out.data_ptr(), blocks, src.shape[0] // blocks, src.shape[1],
                                     rows, cols, nv.stream()), "fbam_refit")
     return out
 
@@ -128,7 +129,7 @@ class _GatedMlp(torch.autograd.Function):
             work = vg.new_empty(parts * _up8(dim)) if parts else None
         v = vg.data_ptr()
         nv.check(nv.lib(h).fbam_gated_block_bwd(
-            dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), w1.data_ptr(), w1.stride(0), w2.data_ptr(), wide, v,
+            dy2.data_ptr(), dy2.shape[1], x2.data_ptr(), depth, w1.data_ptr(), depth, w2.data_ptr(), wide, v,
             v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
             nv.addr(dw_out), nv.addr(db_out), nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0,
             nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, depth, dim, act,

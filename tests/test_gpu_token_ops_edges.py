@@ -38,3 +38,53 @@ def test_embedding_sums_follow_one_another_in_used_memory(n, dim, dtype):
         grad, = torch.autograd.grad((ops.embed_tokens(ids, table),), (table,), (d_out,))
         want = torch.zeros(50, dim, dtype=torch.float64, device="cuda").index_add(0, ids, d_out.double())
         assert torch.equal(grad, want.to(dtype))
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# gated feed-forward block
+# ------------------------------------------------------------------------------------------------------------------
+def _mlp_check(rows, width, inner, out, dtype, act, extras, make=lambda t: t):
+    """All outputs against 64 bits, with the bound of test_gated_mlp; `make` lays an input out."""
+    gen = _gen("mlp", rows, width, inner, out, act)
+    named = {"x": _randn(gen, rows, width, dtype=dtype), "w_in": _randn(gen, 2 * inner, width, dtype=dtype, scale=width ** -0.5),
+             "w_out": _randn(gen, out, inner, dtype=dtype, scale=inner ** -0.5),
+             "b_in": _randn(gen, 2 * inner, dtype=dtype, scale=0.1) if extras else None,
+             "b_out": _randn(gen, out, dtype=dtype, scale=0.1) if extras else None,
+             "residual": _randn(gen, rows, out, dtype=dtype) if extras else None}
+    dy = make(_randn(gen, rows, out, dtype=dtype, scale=0.5))
+    named = {k: make(v) if v is not None and v.dim() == 2 else v for k, v in named.items()}
+    for v in named.values():
+        if v is not None:
+            v.requires_grad_()
+    y = ops.gated_mlp(*(named[k] for k in ("x", "w_in", "w_out", "b_in", "b_out")), act, named["residual"])
+    names = [k for k, v in named.items() if v is not None]
+    grads = dict(zip(names, torch.autograd.grad((y,), [named[k] for k in names], (dy,))))
+    with torch.no_grad():
+        want, size = oracle.mlp(*(named[k] for k in ("x", "w_in", "w_out", "b_in", "b_out")), act, named["residual"], dy)
+    relative = 1.01 * oracle.UNIT[dtype] + 8 * (rows + width + inner + 64) * 2.0 ** -24
+    for name, got in [("y", y)] + list(grads.items()):
+        oracle.within(got, want[name], dtype, relative * size[name] + 1e-6)
+
+
+@pytest.mark.parametrize("rows,width,inner,out", [(1, 1000, 40, 1000), (1, 64, 1, 8), (4, 64, 24, 1), (1, 77, 51, 35), (1, 8, 8, 1)])
+def test_gated_mlp_rows_of_any_pitch(rows, width, inner, out):
+    """Slices of rows of odd lengths.  A single row counts as dense whatever its pitch is."""
+    def sliced(t):
+        wide = torch.zeros(t.shape[0] + 1, t.shape[1] + 1, dtype=t.dtype, device="cuda")
+        wide[:-1, :-1] = t
+        return wide[:-1, :-1].detach()
+    _mlp_check(rows, width, inner, out, BF, "gelu", True, sliced)
+    _mlp_check(rows, width, inner, out, HALF, "silu", False, sliced)
+
+
+def test_gated_mlp_one_row_in_front_of_an_odd_width():
+    """The gradient of a row that is joined with an odd number of columns comes as a slice of the joined row."""
+    gen = _gen("joined")
+    x, w_in, w_out = _randn(gen, 1, 64, dtype=BF), _randn(gen, 96, 64, dtype=BF, scale=0.1), _randn(gen, 40, 48, dtype=BF, scale=0.1)
+    d = _randn(gen, 1, 43, dtype=BF)
+    y = ops.gated_mlp(x.requires_grad_(), w_in, w_out)
+    joined = torch.cat([y, torch.zeros(1, 3, dtype=BF, device="cuda")], 1)
+    grad, = torch.autograd.grad((joined,), (x,), (d,))
+    with torch.no_grad():
+        want, size = oracle.mlp(x, w_in, w_out, None, None, "gelu", None, d[:, :40])
+    oracle.within(grad, want["x"], BF, (1.01 * 2.0 ** -8 + 1e-4) * size["x"] + 1e-6)
