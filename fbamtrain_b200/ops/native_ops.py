@@ -33,8 +33,8 @@ USE_MN_MAJOR = True
 
 
 def _need_elem(*ts) -> torch.dtype:
-    """All given tensors must share one 16-bit element type (bf16 or half); returns it."""
-    dtype = None
+    """All given tensors must share one 16-bit element type (bf16 or half) and one device; returns the type."""
+    dtype = device = None
     for t in ts:
         if t is None:
             continue
@@ -42,7 +42,9 @@ def _need_elem(*ts) -> torch.dtype:
             raise TypeError(f"native kernels take bf16 or fp16 tensors, got {t.dtype}")
         if dtype is not None and t.dtype != dtype:
             raise TypeError(f"native kernels take operands of one 16-bit type, got {dtype} and {t.dtype}")
-        dtype = t.dtype
+        if device is not None and t.device != device:
+            raise ValueError(f"native kernels take operands on one device, got {device} and {t.device}")
+        dtype, device = t.dtype, t.device
     return dtype
 
 

@@ -88,3 +88,13 @@ def test_gated_mlp_one_row_in_front_of_an_odd_width():
     with torch.no_grad():
         want, size = oracle.mlp(x, w_in, w_out, None, None, "gelu", None, d[:, :40])
     oracle.within(grad, want["x"], BF, (1.01 * 2.0 ** -8 + 1e-4) * size["x"] + 1e-6)
+
+
+def test_gated_mlp_refuses_weights_on_the_host():
+    gen = _gen("host")
+    x, w_in, w_out = _randn(gen, 4, 8, dtype=BF), _randn(gen, 32, 8, dtype=BF), _randn(gen, 8, 16, dtype=BF)
+    for args in ((x, w_in.cpu(), w_out), (x, w_in, w_out.cpu())):
+        with pytest.raises(ValueError, match="one device"):
+            ops.gated_mlp(*args)
+    with pytest.raises(ValueError, match="one device"):
+        ops.linear(x, w_in.cpu())
