@@ -64,6 +64,7 @@ def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
     res2 = None if residual is None else _flat(residual)
     lib = nv.lib(x2)
     h = x2.new_empty((rows, wide))
+    tuned = False                          # the second product was made, and counted, by `gemm`
     if not keep and rows <= FEW_ROWS:
         y, vg = x2.new_empty((rows, dim)), None
         nv.check(lib.fbam_gated_few_rows(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide, nv.addr(b_out),
@@ -79,7 +80,7 @@ def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
                                           depth, dim, act, nv.status_word(x2.device).data_ptr(), nv.stream()), "fbam_gated_block_fwd")
         if tuned:
             y = gemm(h, w2, bias=b_out, residual=res2)
-    flops.add(2.0 * rows * inner * (2 * x.shape[-1] + dim))
+    flops.add(2.0 * rows * inner * (2 * x.shape[-1] + (0 if tuned else dim)))
     return y if x.dim() == 2 else y.view(*x.shape[:-1], dim), x2, w1, w2, vg, h
 
 

@@ -98,3 +98,40 @@ def test_gated_mlp_refuses_weights_on_the_host():
             ops.gated_mlp(*args)
     with pytest.raises(ValueError, match="one device"):
         ops.linear(x, w_in.cpu())
+
+
+def _block(rows, width, inner, out, needs=("x", "w_in", "w_out")):
+    gen = _gen("block", rows, width)
+    named = {"x": _randn(gen, rows, width, dtype=BF), "w_in": _randn(gen, 2 * inner, width, dtype=BF, scale=width ** -0.5),
+             "w_out": _randn(gen, out, inner, dtype=BF, scale=inner ** -0.5)}
+    for k in needs:
+        named[k].requires_grad_()
+    dy = _randn(gen, rows, out, dtype=BF)
+
+    def step():
+        y = ops.gated_mlp(**named)
+        return y, torch.autograd.grad((y,), [named[k] for k in needs], (dy,))
+    return step
+
+
+@pytest.mark.parametrize("needs", [("x", "w_in", "w_out"), ("x",), ("w_in",), ("w_out",)])
+def test_gated_mlp_counts_its_operations_once(needs):
+    """2 rows inner (2 width + out) forward; of the backward what is wanted.  The same with a table of tuned tiles."""
+    from fbamtrain_b200.ops import tuning
+    from fbamtrain_b200.utils import flops
+    rows, width, inner, out = 100, 48, 80, 24
+    step = _block(rows, width, inner, out, needs)
+    counted = []
+    for table in (None, {}):
+        tuning.set_table(table)
+        try:
+            flops.reset()
+            step()
+            counted.append(flops.snapshot()[0])
+        finally:
+            tuning.set_table(None)
+    unit = 2.0 * rows * inner
+    gating, dx, dw_in, dw_out = unit * out, unit * 2 * width, unit * 2 * width, unit * out
+    want = unit * (2 * width + out) + ("x" in needs or "w_in" in needs) * gating + ("x" in needs) * dx + ("w_in" in needs) * dw_in + \
+        ("w_out" in needs) * dw_out
+    assert counted == [want, want]
