@@ -138,8 +138,8 @@ class _GatedMlp(torch.autograd.Function):
         flops.add(2.0 * rows * inner * (dim * ((d_vg is not None) + (dw_out is not None)) + 2 * width * ((dx is not None) + (dw_in is not None))))
         if tuned:
             dx = gemm(d_vg, w1, b_mn=True) if need_x else None
-            dw_in = gemm(d_vg, x2, a_mn=True, b_mn=True) if need_in else None
-            dw_out = gemm(dy2[:, :dim], h, a_mn=True, b_mn=True) if need_out else None
+            dw_in = gemm(d_vg, x2, a_mn=True, b_mn=True, splits=weight_grad_splits(2 * wide, depth, rows)) if need_in else None
+            dw_out = gemm(dy2[:, :dim], h, a_mn=True, b_mn=True, splits=weight_grad_splits(dim, wide, rows)) if need_out else None
         if depth != width and dx is not None:
             dx = _refit(dx, 1, rows, width)
         if (wide != inner or depth != width) and dw_in is not None:

@@ -135,3 +135,15 @@ def test_gated_mlp_counts_its_operations_once(needs):
     want = unit * (2 * width + out) + ("x" in needs or "w_in" in needs) * gating + ("x" in needs) * dx + ("w_in" in needs) * dw_in + \
         ("w_out" in needs) * dw_out
     assert counted == [want, want]
+
+
+def test_gated_mlp_splits_its_weight_gradients_with_a_tile_table_too():
+    """What is split along the rows is not looked up in a table, as for linear layers."""
+    from fbamtrain_b200.ops import tuning
+    step = _block(4104, 64, 72, 56)
+    y, plain = step()
+    with tuning.recording() as noted:
+        _, tuned = step()
+    assert sorted(noted) == [tuning.gemm_key(4104, 56, 72, False, False), tuning.gemm_key(4104, 64, 144, False, True)]
+    for a, b in zip(plain, tuned):
+        oracle.within(a, b.double(), BF, 2.0 ** -8 * b.double().abs() + 1e-3)
