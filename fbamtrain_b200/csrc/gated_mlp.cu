@@ -604,10 +604,10 @@ long long tiles_of(int rows, int tile_rows, int cols, int tile_cols) {
 // Accumulator width and pairing: 0: single CTAs with 64 columns, 1: with 128, 2: pairs with 256.  Pairs where their tiles reach
 // every SM; below that the wider tile that still does.  us of the whole block's forward, 64 | 128 | pairs: 8192 x 1024 x 4096
 // 261 | 179 | 146, 2048 x 1024 x 4096 83 | 63 | 58, 1001 x 1000 x 2736 54 | 48 | 44, 300 x 1024 x 4096 38 | 36 | 36, 64 x 1024 x
-// 4096 30 | 32 | 34.
-int pick(int rows, int inner, bool back) {
+// 4096 30 | 32 | 34.  `pairs` below 0: by this rule, 0: never, 1: always.
+int pick(int rows, int inner, bool back, int pairs) {
   const int h = back ? 2 : 1;
-  if (tiles_of(rows, 256, inner, 128 * h) >= 74) return 2;
+  if (pairs < 0 ? tiles_of(rows, 256, inner, 128 * h) >= 74 : pairs > 0) return 2;
   return tiles_of(rows, 128, inner, 64 * h) >= 148 ? 1 : 0;
 }
 
@@ -626,10 +626,10 @@ int run(int which, int rows, int inner, const CUtensorMap (&m)[6], const Params&
 // x (rows, depth) pitch ldx, w_in (2 inner, depth) pitch ldw, bias (2 inner) elements or null -> h (rows, inner) dense and, where v
 // is not null, v and g (rows, inner) dense fp32.  inner is a multiple of 8, all rows start on 16-byte boundaries.
 extern "C" int fbam_gated_fwd(const void* x, long long ldx, const void* w_in, long long ldw, const void* bias, void* h, float* v,
-                              float* g, int rows, int inner, int depth, int act, int* status, void* stream) {
+                              float* g, int rows, int inner, int depth, int act, int pairs, int* status, void* stream) {
   if (rows <= 0 || inner <= 0 || depth <= 0 || inner % 8 != 0 || inner > 0x3fffffff || act < 0 || act > 1 || (v == nullptr) != (g == nullptr))
     return GEMM_ERR_SHAPE;
-  const int which = pick(rows, inner, false), box = which == 2 ? 128 : which == 1 ? 64 : 32;
+  const int which = pick(rows, inner, false, pairs), box = which == 2 ? 128 : which == 1 ? 64 : 32;
   CUtensorMap m[6];
   int e = encode(&m[0], x, rows, depth, ldx, BM, BK, false);
   if (!e) e = encode(&m[1], w_in, 2ll * inner, depth, ldw, box, BK, false);
@@ -647,7 +647,7 @@ extern "C" int fbam_gated_fwd(const void* x, long long ldx, const void* w_in, lo
 // dy (rows, depth) pitch ldy, w_out (depth, inner) pitch ldw, v and g as the forward left them -> d_vg (rows, 2 inner) dense, and
 // where col_sums is not null its column sums in db (2 inner) elements; col_sums is the workspace, 2 inner fp32 values for every 32 rows.
 extern "C" int fbam_gated_bwd(const void* dy, long long ldy, const void* w_out, long long ldw, const float* v, const float* g, void* d_vg,
-                              float* col_sums, void* db, int rows, int inner, int depth, int act, int* status, void* stream) {
+                              float* col_sums, void* db, int rows, int inner, int depth, int act, int pairs, int* status, void* stream) {
   if (rows <= 0 || inner <= 0 || depth <= 0 || inner % 8 != 0 || inner > 0x3fffffff || act < 0 || act > 1 ||
       (col_sums == nullptr) != (db == nullptr))
     return GEMM_ERR_SHAPE;
@@ -661,7 +661,7 @@ extern "C" int fbam_gated_bwd(const void* dy, long long ldy, const void* w_out, 
   if (e) return e;
   const Params p{nullptr, col_sums, status, rows, inner, depth, act};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  e = run<BACKWARD>(pick(rows, inner, true), rows, inner, m, p, s);
+  e = run<BACKWARD>(pick(rows, inner, true, pairs), rows, inner, m, p, s);
   if (e || db == nullptr) return e;
   add_sums_kernel<<<(2 * inner + 31) / 32, 256, 0, s>>>(col_sums, (elem_t*)db, (rows + 31) / 32, 2 * inner);
   return cudaGetLastError() == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
@@ -691,11 +691,12 @@ extern "C" int fbam_product(const void* A, long long lda, int a_mn_major, const 
 extern "C" int fbam_colsum_to(const void* x, const void* z, void* dz, void* out, int out_elem, float* work, long long rows, int cols,
                               void* stream);                                                         // kernels_simt.cu
 
-// The block's forward: fbam_gated_fwd, and where y is not null y (rows, out_dim) = h W_outᵀ + b_out + residual, dense.
+// The block's forward: fbam_gated_fwd, and where y is not null y (rows, out_dim) = h W_outᵀ + b_out + residual, dense.  `pairs`, here and
+// in the backward: whether the fused product runs on pairs of CTAs, below 0 by its size, 0 never, 1 always.
 extern "C" int fbam_gated_block_fwd(const void* x, long long ldx, const void* w_in, long long ld_in, const void* b_in, const void* w_out,
                                     long long ld_out, const void* b_out, const void* residual, void* h, float* v, float* g, void* y,
-                                    int rows, int inner, int depth, int out_dim, int act, int* status, void* stream) {
-  const int e = fbam_gated_fwd(x, ldx, w_in, ld_in, b_in, h, v, g, rows, inner, depth, act, status, stream);
+                                    int rows, int inner, int depth, int out_dim, int act, int pairs, int* status, void* stream) {
+  const int e = fbam_gated_fwd(x, ldx, w_in, ld_in, b_in, h, v, g, rows, inner, depth, act, pairs, status, stream);
   if (e || y == nullptr) return e;
   return fbam_product(h, inner, 0, w_out, ld_out, 0, rows, out_dim, inner, y, out_dim, b_out, residual, out_dim, nullptr, 0, status, stream);
 }
@@ -706,10 +707,10 @@ extern "C" int fbam_gated_block_bwd(const void* dy, long long ldy, const void* x
                                     const void* w_out, long long ld_out, const float* v, const float* g, const void* h, void* d_vg,
                                     float* col_sums, void* d_b_in, void* dx, void* d_w_in, void* d_w_out, void* d_b_out, float* col_work,
                                     float* slabs_in, int splits_in, float* slabs_out, int splits_out, int rows, int inner, int depth,
-                                    int out_dim, int act, int* status, void* stream) {
+                                    int out_dim, int act, int pairs, int* status, void* stream) {
   int e = 0;
   if (d_vg != nullptr)
-    e = fbam_gated_bwd(dy, ldy, w_out, ld_out, v, g, d_vg, col_sums, d_b_in, rows, inner, out_dim, act, status, stream);
+    e = fbam_gated_bwd(dy, ldy, w_out, ld_out, v, g, d_vg, col_sums, d_b_in, rows, inner, out_dim, act, pairs, status, stream);
   if (!e && dx != nullptr)
     e = fbam_product(d_vg, 2ll * inner, 0, w_in, ld_in, 1, rows, depth, 2 * inner, dx, depth, nullptr, nullptr, 0, nullptr, 0, status, stream);
   if (!e && d_w_in != nullptr)

@@ -36,7 +36,7 @@ struct ConvClass {
   int k_block_base;
 };
 
-#define FBAM_INTERFACE_REVISION 7  // see fbam_interface_revision; INTERFACE_REVISION in ops/native.py
+#define FBAM_INTERFACE_REVISION 8  // see fbam_interface_revision; INTERFACE_REVISION in ops/native.py
 
 struct GemmParams {
   void* D;                          // output, bf16 or fp32, row pitch ldd elements

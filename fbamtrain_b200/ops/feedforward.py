@@ -9,10 +9,10 @@ from __future__ import annotations
 
 import torch
 
-from ..utils import flops
+from ..utils import debug, flops
 from . import native as nv
-from . import tuning
-from .native_ops import _need_elem, _sum_partials, gemm, weight_grad_splits
+from . import native_ops, tuning
+from .native_ops import _need_elem, _sum_partials, gemm, gemm_nn, gemm_tn, weight_grad_splits
 
 GATES = {"gelu": 0, "silu": 1}
 F32 = torch.float32
@@ -20,6 +20,33 @@ F32 = torch.float32
 # Rows up to which the weights are streamed past the rows instead of tiled.  us, streamed | tiled: 8 x 1024 x 4096 17 | 36, 32 x
 # 1024 x 4096 24 | 34, 8 x 2048 x 8192 34 | 71, 32 x 2048 x 8192 54 | 60.
 FEW_ROWS = 32
+
+
+# What the launchers make of native_ops.TWO_CTA: pairs of CTAs by size, never, always.
+PAIRS = {"auto": -1, False: 0, True: 1}
+
+
+def _apart() -> bool:
+    """Whether the plain products are made one by one through ``gemm``: with a table of tuned tiles, and where a switch that it
+    honours is not as usual."""
+    return (tuning.active() or native_ops.TWO_CTA != "auto" or not native_ops.USE_MN_MAJOR or debug.PROFILE_LABELS or debug.SYNC_EVERY_OP
+            or debug.POISON_ALLOC or debug.DEBUG_KERNEL_LAUNCH)
+
+
+def _launch(apart: bool, entry: str, like: torch.Tensor, *args) -> None:
+    if not apart:
+        nv.check(getattr(nv.lib(like), entry)(*args), entry)
+        return
+    with debug.label(lambda: f"{entry[5:]} of {tuple(like.shape)}"):
+        code = getattr(nv.lib(like), entry)(*args)
+    nv.check(code, entry)
+    debug.after_launch(entry[5:], like)
+
+
+def _fresh(like: torch.Tensor, *shape: int, dtype=None) -> torch.Tensor:
+    if debug.POISON_ALLOC:
+        return debug.fresh(shape, dtype or like.dtype, like.device)
+    return like.new_empty(shape, dtype=dtype or like.dtype)
 
 
 def _up8(n: int) -> int:
@@ -62,25 +89,24 @@ def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
     b_in = None if b_in is None else _dense(b_in)
     b_out = None if b_out is None else _dense(b_out)
     res2 = None if residual is None else _flat(residual)
-    lib = nv.lib(x2)
-    h = x2.new_empty((rows, wide))
-    tuned = False                          # the second product was made, and counted, by `gemm`
+    h = _fresh(x2, rows, wide)
+    apart = _apart()
+    product = False                        # the second product was made, and counted, by `gemm`
     if not keep and rows <= FEW_ROWS:
-        y, vg = x2.new_empty((rows, dim)), None
-        nv.check(lib.fbam_gated_few_rows(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide, nv.addr(b_out),
-                                         nv.addr(res2), dim, h.data_ptr(), y.data_ptr(), rows, depth, wide, dim, act, nv.stream()),
-                 "fbam_gated_few_rows")
+        y, vg = _fresh(x2, rows, dim), None
+        _launch(apart, "fbam_gated_few_rows", x2, x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide,
+                nv.addr(b_out), nv.addr(res2), dim, h.data_ptr(), y.data_ptr(), rows, depth, wide, dim, act, nv.stream())
     else:
-        vg = x2.new_empty((2, rows, wide), dtype=F32) if keep else None
+        vg = _fresh(x2, 2, rows, wide, dtype=F32) if keep else None
         v = vg.data_ptr() if keep else 0
-        tuned = tuning.active()
-        y = None if tuned else x2.new_empty((rows, dim))
-        nv.check(lib.fbam_gated_block_fwd(x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide, nv.addr(b_out),
-                                          nv.addr(res2), h.data_ptr(), v, v + 4 * rows * wide if keep else 0, nv.addr(y), rows, wide,
-                                          depth, dim, act, nv.status_word(x2.device).data_ptr(), nv.stream()), "fbam_gated_block_fwd")
-        if tuned:
+        product = apart
+        y = None if apart else x2.new_empty((rows, dim))
+        _launch(apart, "fbam_gated_block_fwd", x2, x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide,
+                nv.addr(b_out), nv.addr(res2), h.data_ptr(), v, v + 4 * rows * wide if keep else 0, nv.addr(y), rows, wide, depth, dim, act,
+                PAIRS[native_ops.TWO_CTA], nv.status_word(x2.device).data_ptr(), nv.stream())
+        if apart:
             y = gemm(h, w2, bias=b_out, residual=res2)
-    flops.add(2.0 * rows * inner * (2 * x.shape[-1] + (0 if tuned else dim)))
+    flops.add(2.0 * rows * inner * (2 * x.shape[-1] + (0 if product else dim)))
     return y if x.dim() == 2 else y.view(*x.shape[:-1], dim), x2, w1, w2, vg, h
 
 
@@ -109,18 +135,18 @@ class _GatedMlp(torch.autograd.Function):
             dy2 = _refit(dy2, 1, rows, _up8(dim))
         dx = dw_in = dw_out = db_in = db_out = d_vg = sums = work = slabs_in = slabs_out = None
         splits_in = splits_out = 0
-        tuned = tuning.active()
+        apart = _apart()
         if need_x or need_in or need_bin:
-            d_vg = h.new_empty((rows, 2 * wide))
+            d_vg = _fresh(h, rows, 2 * wide)
             if need_bin:
                 db_in, sums = h.new_empty(2 * wide), vg.new_empty(((rows + 31) // 32, 2 * wide))
             if need_x:
-                dx = None if tuned else h.new_empty((rows, depth))
-            if need_in and not tuned:
+                dx = None if apart else h.new_empty((rows, depth))
+            if need_in and not apart:
                 dw_in = h.new_empty((2 * wide, depth))
                 splits_in = weight_grad_splits(2 * wide, depth, rows)
                 slabs_in = _slabs(h, splits_in, 2 * wide, depth)
-        if need_out and not tuned:
+        if need_out and not apart:
             dw_out = h.new_empty((dim, wide))
             splits_out = weight_grad_splits(dim, wide, rows)
             slabs_out = _slabs(h, splits_out, dim, wide)
@@ -129,17 +155,17 @@ class _GatedMlp(torch.autograd.Function):
             parts = _sum_partials("fbam_colsum_partials", rows, _up8(dim), 0)
             work = vg.new_empty(parts * _up8(dim)) if parts else None
         v = vg.data_ptr()
-        nv.check(nv.lib(h).fbam_gated_block_bwd(
-            dy2.data_ptr(), dy2.shape[1], x2.data_ptr(), depth, w1.data_ptr(), depth, w2.data_ptr(), wide, v,
-            v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
-            nv.addr(dw_out), nv.addr(db_out), nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0,
-            nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, depth, dim, act,
-            nv.status_word(h.device).data_ptr(), nv.stream()), "fbam_gated_block_bwd")
+        _launch(apart, "fbam_gated_block_bwd", h, dy2.data_ptr(), dy2.shape[1], x2.data_ptr(), depth, w1.data_ptr(), depth, w2.data_ptr(), wide,
+                v, v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
+                nv.addr(dw_out), nv.addr(db_out), nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0,
+                nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, depth, dim, act,
+                PAIRS[native_ops.TWO_CTA], nv.status_word(h.device).data_ptr(), nv.stream())
         flops.add(2.0 * rows * inner * (dim * ((d_vg is not None) + (dw_out is not None)) + 2 * width * ((dx is not None) + (dw_in is not None))))
-        if tuned:
-            dx = gemm(d_vg, w1, b_mn=True) if need_x else None
-            dw_in = gemm(d_vg, x2, a_mn=True, b_mn=True, splits=weight_grad_splits(2 * wide, depth, rows)) if need_in else None
-            dw_out = gemm(dy2[:, :dim], h, a_mn=True, b_mn=True, splits=weight_grad_splits(dim, wide, rows)) if need_out else None
+        if apart:
+            splits = weight_grad_splits if native_ops.USE_MN_MAJOR else (lambda *sizes: 0)
+            dx = gemm_nn(d_vg, w1) if need_x else None
+            dw_in = gemm_tn(d_vg, x2, splits=splits(2 * wide, depth, rows)) if need_in else None
+            dw_out = gemm_tn(dy2[:, :dim], h, splits=splits(dim, wide, rows)) if need_out else None
         if depth != width and dx is not None:
             dx = _refit(dx, 1, rows, width)
         if (wide != inner or depth != width) and dw_in is not None:

@@ -78,7 +78,7 @@ def available(dtype: torch.dtype = torch.bfloat16) -> bool:
     return os.path.exists(LIB_PATH_FP16 if dtype == torch.float16 else LIB_PATH)
 
 
-INTERFACE_REVISION = 7        # FBAM_INTERFACE_REVISION of csrc/gemm_tcgen05.h
+INTERFACE_REVISION = 8        # FBAM_INTERFACE_REVISION of csrc/gemm_tcgen05.h
 
 
 def _check_struct_layout(library: C.CDLL, path: str) -> None:
@@ -108,9 +108,9 @@ _ARGTYPES = {
     "fbam_embed_bwd_workspace": (_L, _I, _P, _P),
     "fbam_recurrence_fwd": (_P, _L, _L, _L, _P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _P, _P),
     "fbam_recurrence_bwd": (_P, _L, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _P, _I, _I, _I, _P, _P),
-    "fbam_gated_block_fwd": (_P, _L, _P, _L, _P, _P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P),
+    "fbam_gated_block_fwd": (_P, _L, _P, _L, _P, _P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P),
     "fbam_gated_block_bwd": (_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I,
-                             _P, _P),
+                             _I, _P, _P),
     "fbam_refit": (_P, _L, _P, _I, _I, _I, _I, _I, _P),
     "fbam_gated_few_rows": (_P, _L, _P, _L, _P, _P, _L, _P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _P),
     "fbam_logprobs_fwd": (_P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _I, _I, _F, _P),

@@ -147,3 +147,53 @@ def test_gated_mlp_splits_its_weight_gradients_with_a_tile_table_too():
     assert sorted(noted) == [tuning.gemm_key(4104, 56, 72, False, False), tuning.gemm_key(4104, 64, 144, False, True)]
     for a, b in zip(plain, tuned):
         oracle.within(a, b.double(), BF, 2.0 ** -8 * b.double().abs() + 1e-3)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 15, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize("width,inner,out", [(8, 8, 3), (24, 40, 17), (40, 264, 12), (100, 130, 61), (1000, 2056, 1000)])
+@pytest.mark.parametrize("act,extras", [("gelu", True), ("silu", False), ("silu", True)])
+def test_gated_mlp_answers_of_a_few_rows(rows, width, inner, out, act, extras):
+    """Up to 32 rows the weights are streamed past the rows: both halves of 16 rows, parts of K that end inside a warp's run, columns
+    behind the last eight."""
+    _mlp_answer(rows, width, inner, out, BF, act, extras)
+    _mlp_answer(rows, width, inner, out, HALF, act, extras)
+
+
+# tiles of 64, of 128 and of pairs of CTAs with 256 columns of the accumulator, with whole and partial last ones of both sides
+@pytest.mark.parametrize("rows,width,inner,out", [(64, 136, 1000, 72), (1100, 64, 1032, 40), (1300, 72, 1992, 64), (2561, 320, 2072, 136),
+                                                  (4096, 128, 1288, 64)])
+@pytest.mark.parametrize("act,extras", [("gelu", True), ("silu", False)])
+def test_gated_mlp_answers_of_many_rows(rows, width, inner, out, act, extras):
+    _mlp_answer(rows, width, inner, out, BF, act, extras)
+    _mlp_answer(rows, width, inner, out, HALF, act, extras)
+
+
+def _mlp_answer(rows, width, inner, out, dtype, act, extras):
+    """y without gradients, with the bound of test_gated_mlp."""
+    gen = _gen("mlp answer", rows, width, inner, out, act)
+    x, residual = _randn(gen, rows, width, dtype=dtype), _randn(gen, rows, out, dtype=dtype) if extras else None
+    w_in, w_out = _randn(gen, 2 * inner, width, dtype=dtype, scale=width ** -0.5), _randn(gen, out, inner, dtype=dtype, scale=inner ** -0.5)
+    b_in, b_out = (_randn(gen, 2 * inner, dtype=dtype, scale=0.1), _randn(gen, out, dtype=dtype, scale=0.1)) if extras else (None, None)
+    with torch.no_grad():
+        y = ops.gated_mlp(x, w_in, w_out, b_in, b_out, act, residual)
+    want, size = oracle.mlp(x, w_in, w_out, b_in, b_out, act, residual, torch.zeros(rows, out, device="cuda"))
+    relative = 1.01 * oracle.UNIT[dtype] + 8 * (width + inner + 64) * 2.0 ** -24
+    oracle.within(y, want["y"], dtype, relative * size["y"] + 1e-6)
+
+
+@pytest.mark.parametrize("switch", [("TWO_CTA", False), ("TWO_CTA", True), ("USE_MN_MAJOR", False), ("DEBUG_KERNEL_LAUNCH", True),
+                                    ("SYNC_EVERY_OP", True), ("PROFILE_LABELS", True), ("POISON_ALLOC", True)])
+@pytest.mark.parametrize("rows,width,inner,out", [(20, 72, 90, 66), (2600, 256, 2048, 256)])
+def test_gated_mlp_with_the_switches_of_the_other_products(switch, rows, width, inner, out, monkeypatch, capsys):
+    from fbamtrain_b200.ops import native_ops
+    from fbamtrain_b200.utils import debug
+    name, value = switch
+    monkeypatch.setattr(native_ops if hasattr(native_ops, name) else debug, name, value)
+    if value is True and name == "TWO_CTA" and rows < 256:
+        pytest.skip("pairs want tiles of 256 columns")
+    _mlp_check(rows, width, inner, out, BF, "gelu", True)
+    _mlp_answer(rows, width, inner, out, BF, "gelu", True)
+    lines = [line.split("(")[0] for line in capsys.readouterr().out.splitlines() if line.startswith("[launch]")]
+    if name == "DEBUG_KERNEL_LAUNCH":
+        block = ["[launch] gated_few_rows"] if rows <= 32 else ["[launch] gated_block_fwd", "[launch] gemm"]
+        assert lines == ["[launch] gated_block_fwd", "[launch] gemm", "[launch] gated_block_bwd"] + 3 * ["[launch] gemm"] + block
