@@ -10,6 +10,7 @@ import ctypes as C
 import torch
 
 from . import native as nv
+from .derivatives import first_only, tracked
 
 F32 = torch.float32
 
@@ -33,6 +34,7 @@ class _EmbedTokens(torch.autograd.Function):
         return _forward(ids, flat, table, scale, out_dtype, elem)
 
     @staticmethod
+    @first_only("embed_tokens")
     def backward(ctx, d_out):
         (flat,) = ctx.saved_tensors
         vocab, dim, dtype, elem, scale = ctx.meta
@@ -61,5 +63,5 @@ def embed_tokens(ids, table, scale, out_dtype):
     if table.stride(1) != 1:
         table = table.contiguous()
     elem = table.dtype if table.dtype != F32 else out_dtype
-    run = _EmbedTokens.apply if table.requires_grad and torch.is_grad_enabled() else _forward
+    run = _EmbedTokens.apply if tracked(table) else _forward
     return run(ids, flat, table, float(scale), out_dtype, elem)

@@ -12,6 +12,7 @@ import torch
 from ..utils import debug, flops
 from . import native as nv
 from . import native_ops, tuning
+from .derivatives import first_only, tracked
 from .native_ops import _need_elem, _sum_partials, gemm, gemm_nn, gemm_tn, weight_grad_splits
 
 GATES = {"gelu": 0, "silu": 1}
@@ -119,13 +120,15 @@ class _GatedMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, act, residual):
         y, x2, w1, w2, vg, h = _forward(x, w_in, w_out, b_in, b_out, act, residual, True)
-        ctx.save_for_backward(x2, w1, w2, vg, h)
+        # the inputs themselves are what a derivative of the gradients would be of: no memory where their rows are taken as they are
+        ctx.save_for_backward(x2, w1, w2, vg, h, x, w_in, w_out, b_in)
         ctx.meta = (x.shape, w_out.shape[1], act)
         return y
 
     @staticmethod
+    @first_only("gated_mlp")
     def backward(ctx, dy):
-        x2, w1, w2, vg, h = ctx.saved_tensors
+        x2, w1, w2, vg, h = ctx.saved_tensors[:5]
         shape, inner, act = ctx.meta
         need_x, need_in, need_out, need_bin, need_bout, _, need_res = ctx.needs_input_grad
         rows, wide = h.shape
@@ -182,7 +185,6 @@ class _GatedMlp(torch.autograd.Function):
 
 def gated_mlp(x, w_in, w_out, b_in, b_out, act, residual):
     _need_elem(x, w_in, w_out, b_in, b_out, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad or
-                                    any(t is not None and t.requires_grad for t in (b_in, b_out, residual))):
+    if tracked(x, w_in, w_out, b_in, b_out, residual):
         return _GatedMlp.apply(x, w_in, w_out, b_in, b_out, GATES[act], residual)
     return _forward(x, w_in, w_out, b_in, b_out, GATES[act], residual, False)[0]

@@ -5,6 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import native as nv
+from .derivatives import first_only, tracked
 
 F32 = torch.float32
 
@@ -39,6 +40,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return logprob, entropy, top_lp, top_ids
 
     @staticmethod
+    @first_only("token_logprobs")
     def backward(ctx, d_logprob, d_entropy, _lp, _ids):
         logits, targets, stats, entropy = ctx.saved_tensors
         rows, vocab = logits.shape
@@ -65,7 +67,7 @@ def token_logprobs(logits, targets, top, temperature):
         flat = flat.contiguous()
     if targets is not None and not (targets.dim() == 1 and targets.dtype == torch.int64 and targets.is_contiguous()):
         targets = targets.reshape(-1).long().contiguous()
-    if flat.requires_grad and torch.is_grad_enabled():
+    if tracked(flat):
         out = _TokenLogprobs.apply(flat, targets, top, 1.0 / temperature)
     else:
         out = _forward(flat, targets, top, 1.0 / temperature, False)[:4]

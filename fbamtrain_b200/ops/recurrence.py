@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import native as nv
+from .derivatives import first_only, tracked
 
 F32 = torch.float32
 
@@ -47,12 +48,13 @@ class _GatedRecurrence(torch.autograd.Function):
     def forward(ctx, zgo, state, resets):
         ctx.set_materialize_grads(False)
         y, out, saved = _forward(zgo, state, resets, True)
-        ctx.save_for_backward(zgo, resets, saved)
+        ctx.save_for_backward(zgo, resets, saved, state)
         return y, out
 
     @staticmethod
+    @first_only("gated_recurrence")
     def backward(ctx, dy, d_out):
-        zgo, resets, saved = ctx.saved_tensors
+        zgo, resets, saved, _ = ctx.saved_tensors
         b, t, _, d = zgo.shape
         dev = zgo.device
         if dy is None:
@@ -82,6 +84,6 @@ def gated_recurrence(zgo, state, resets):
         zgo = zgo.contiguous()
     if state is not None:
         state = state.contiguous()
-    if torch.is_grad_enabled() and (zgo.requires_grad or (state is not None and state.requires_grad)):
+    if tracked(zgo, state):
         return _GatedRecurrence.apply(zgo, state, resets)
     return _forward(zgo, state, resets, False)[:2]

@@ -197,3 +197,49 @@ def test_gated_mlp_with_the_switches_of_the_other_products(switch, rows, width, 
     if name == "DEBUG_KERNEL_LAUNCH":
         block = ["[launch] gated_few_rows"] if rows <= 32 else ["[launch] gated_block_fwd", "[launch] gemm"]
         assert lines == ["[launch] gated_block_fwd", "[launch] gemm", "[launch] gated_block_bwd"] + 3 * ["[launch] gemm"] + block
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# all
+# ------------------------------------------------------------------------------------------------------------------
+def _calls():
+    """Every operator as a function of one input, and that input."""
+    gen = _gen("calls")
+    ids = torch.randint(0, 20, (30,), generator=gen, device="cuda")
+    w_in, w_out = _randn(gen, 96, 32, dtype=BF), _randn(gen, 24, 48, dtype=BF)
+    return {"embed_tokens": (lambda t: ops.embed_tokens(ids, t), _randn(gen, 20, 16, dtype=BF)),
+            "gated_recurrence": (lambda z: ops.gated_recurrence(z)[0], _randn(gen, 2, 30, 3, 16, dtype=BF)),
+            "gated_mlp": (lambda x: ops.gated_mlp(x, w_in, w_out), _randn(gen, 40, 32, dtype=BF)),
+            "token_logprobs": (lambda x: ops.token_logprobs(x, ids, 2).logprob, _randn(gen, 30, 64, dtype=BF))}
+
+
+@pytest.mark.parametrize("name", ["embed_tokens", "gated_recurrence", "gated_mlp", "token_logprobs"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_tangent_is_refused(name, grad):
+    """Forward-mode differentiation has no formula here, and an answer without its tangent would be a wrong one."""
+    call, x = _calls()[name]
+    with torch.set_grad_enabled(grad):
+        plain = call(x)
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+            inside = call(x)
+        oracle.within(inside, plain.double(), BF if plain.dtype == BF else F32, 2.0 ** -8 * plain.double().abs())
+        assert torch.equal(call(x), plain)
+
+
+@pytest.mark.parametrize("name", ["embed_tokens", "gated_recurrence", "gated_mlp", "token_logprobs"])
+def test_a_second_derivative_is_refused(name):
+    """Of the gradient by what it depends on: the input (but for the embedding, whose gradient does not) and the gradient that
+    comes in; alone and in a sum with what has a derivative."""
+    call, x = _calls()[name]
+    x.requires_grad_()
+    y = call(x)
+    up = torch.ones_like(y).requires_grad_()
+    first, = torch.autograd.grad((y,), (x,), (up.detach(),), retain_graph=True)
+    again, = torch.autograd.grad((y,), (x,), (up,), create_graph=True)
+    assert torch.equal(first, again) and again.requires_grad
+    for of in (up,) if name == "embed_tokens" else (up, x):
+        for value in (again.float().square().sum(), again.float().sum() + of.float().sum()):
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad((value,), (of,), retain_graph=True)
