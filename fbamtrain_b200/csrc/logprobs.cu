@@ -192,7 +192,8 @@ constexpr uint32_t kNothing = 0x007fffffu;    // order_key(-inf)
 // One row per cluster of CTAs (mostly of one), WARPS warps each.  Vector v of a row belongs to thread v mod (threads of the
 // cluster).
 //
-// Alternatives: a thread keeps the key of the best logit of each of its batches.  The k-th best of the CTA's threads' best keys
+// Alternatives: a thread keeps the key of the best logit of each of its batches (of 2^fold of them, where shared memory has no room
+// for all).  The k-th best of the CTA's threads' best keys
 // bounds the k-th best of its logits from below, so only batches whose best reaches that bound are looked at again; what
 // reaches it goes on a list, and a place on the list is the count of those that come before by (value falling, id rising).
 // Where the list overflows, equal logits are taken in order, or each alternative is looked for in a pass of its own.
@@ -206,9 +207,10 @@ template <typename T, int VEC, int WARPS, int ROWS>
 __global__ void __launch_bounds__(WARPS * ROWS * 32, 1024 / (WARPS * ROWS * 32))
 logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ targets, float* __restrict__ logprob,
                     float* __restrict__ entropy, float* __restrict__ stats, float* __restrict__ top_logprobs,
-                    long long* __restrict__ top_ids, long long rows, int vocab, int top, float inv_t, int batches, int candidates) {
+                    long long* __restrict__ top_ids, long long rows, int vocab, int top, float inv_t, int batches, int folded, int candidates) {
   static_assert(WARPS == 1 || ROWS == 1, "rows of a CTA do not wait for one another");
   constexpr int kThreads = WARPS * 32, kBatch = kBatchOf<VEC>;
+  const int fold = WARPS == 1 ? 0 : folded;                   // a warp alone has 32 batches at most (launch_fwd)
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ Stats parts[WARPS];
   __shared__ float whole[3];
@@ -222,7 +224,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
   unsigned long long* sorted = reinterpret_cast<unsigned long long*>(smem_raw) + sub * (kMaxTop + candidates);
   unsigned long long* list = sorted + kMaxTop;                // [candidates]
   uint32_t* best_of = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned long long*>(smem_raw) + ROWS * (kMaxTop + candidates)) +
-                      sub * batches * kThreads;               // [batches][kThreads]
+                      sub * (((batches - 1) >> fold) + 1) * kThreads;       // [batches >> fold, upwards][kThreads]
   int& list_length = list_lengths[sub];
   const Row<T, VEC> row(logits + r * ld, vocab);
   const float c = inv_t * kLog2e;
@@ -251,7 +253,8 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
     const float top_x = highest.top();
     if (top > 0) {
       const uint32_t key = j < vocab ? order_key(top_x) : 0;
-      best_of[i * kThreads + tid] = key;
+      uint32_t& of = best_of[(i >> fold) * kThreads + tid];
+      of = i & ((1 << fold) - 1) ? max(of, key) : key;
       best = max(best, key);
     }
     if (top_x > st.m) st.move_to(top_x, c);
@@ -342,7 +345,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
   auto entry = [](float x, long long j) { return (unsigned long long)order_key(x) << 32 | (uint32_t)(0xffffffffu - (uint32_t)j); };
   const float least = key_value(bound);                       // no logit that reaches the bound is below it
   for (int i = 0; i < batches; ++i) {
-    if (best_of[i * kThreads + tid] < max(bound, 1u)) continue;
+    if (best_of[(i >> fold) * kThreads + tid] < max(bound, 1u)) continue;
     if (*reinterpret_cast<volatile int*>(&list_length) > candidates) break;    // too many anyway
     const long long j0 = first + (long long)i * kBatch * hop;
     Raw<T, VEC> raw[kBatch];
@@ -390,7 +393,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, long long ld, const long long*
     if (tid == 0) list_length = 0;
     sync();
     for (int i = 0; i < batches; ++i) {
-      if (best_of[i * kThreads + tid] <= bound) continue;
+      if (best_of[(i >> fold) * kThreads + tid] <= bound) continue;
       for (int b = 0; b < kBatch; ++b) {
         const long long j = first + (long long)(i * kBatch + b) * hop;
         float x[VEC];
@@ -577,7 +580,10 @@ template <typename T, int VEC, int WARPS, int ROWS>
 int launch_fwd_w(const FwdArgs& a, int ctas, cudaStream_t s) {
   const long long step = (long long)ctas * WARPS * 32 * VEC * kBatchOf<VEC>, batches = (a.vocab + most_lead<T>(a.logits, a.ld) + step - 1) / step;
   const long long candidates = ROWS > 1 ? 256 : 1024, blocks = ROWS > 1 ? (a.rows + ROWS - 1) / ROWS : a.rows * ctas;
-  const long long smem = a.top > 0 ? ROWS * ((candidates + kMaxTop) * 8 + batches * WARPS * 32 * 4) : 0;
+  int fold = 0;
+  auto smem_of = [&]() { return a.top > 0 ? ROWS * ((candidates + kMaxTop) * 8 + (((batches - 1) >> fold) + 1) * WARPS * 32 * 4) : 0; };
+  while (WARPS > 1 && smem_of() > 220 * 1024) ++fold;
+  const long long smem = smem_of();
   if (blocks > 0x7fffffffll || smem > 220 * 1024) return GEMM_ERR_SHAPE;
   auto kernel = logprobs_fwd_kernel<T, VEC, WARPS, ROWS>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
@@ -593,7 +599,7 @@ int launch_fwd_w(const FwdArgs& a, int ctas, cudaStream_t s) {
   cfg.attrs = &attr;
   cfg.numAttrs = ctas > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, (const T*)a.logits, a.ld, a.targets, a.logprob, a.entropy, a.stats, a.top_logprobs, a.top_ids,
-                            a.rows, a.vocab, a.top, a.inv_t, (int)batches, (int)candidates) == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
+                            a.rows, a.vocab, a.top, a.inv_t, (int)batches, fold, (int)candidates) == cudaSuccess ? 0 : GEMM_ERR_LAUNCH;
 }
 
 // Warps of a row: one where the rows alone fill half the machine's warp slots, more for fewer rows and for long ones, whose

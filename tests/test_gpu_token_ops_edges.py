@@ -243,3 +243,22 @@ def test_a_second_derivative_is_refused(name):
         for value in (again.float().square().sum(), again.float().sum() + of.float().sum()):
             with pytest.raises(RuntimeError, match="second derivative"):
                 torch.autograd.grad((value,), (of,), retain_graph=True)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# log probabilities
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,vocab,dtype", [(400, 2_000_003, BF), (2, 15_000_001, BF), (1, 30_000_000, F32), (200, 3_600_007, F32)])
+def test_logprobs_alternatives_of_any_vocabulary(rows, vocab, dtype):
+    """A vocabulary of more batches than shared memory has room for the best of.  A sum in fp32 takes some 260 additions one after
+    the other: that many units of 2^-24, of the logarithm and of differences of up to 6."""
+    gen = _gen("vocabulary", rows, vocab)
+    logits = torch.empty(rows, vocab, dtype=dtype, device="cuda").normal_(generator=gen)
+    logits[0, vocab // 3::7] = 6.0                           # more equal values than candidates
+    r = ops.token_logprobs(logits, None, 32)
+    for i in {0, rows // 2, rows - 1}:
+        ids = oracle.alternatives(logits[i:i + 1], 32)
+        assert torch.equal(r.top_ids[i:i + 1], ids)
+        _, entropy, logp, _ = oracle.logprobs(logits[i:i + 1], torch.zeros(1, dtype=torch.int64, device="cuda"), 1.0)
+        oracle.within(r.entropy[i:i + 1], entropy, F32, 3e-4)
+        oracle.within(r.top_logprobs[i:i + 1], logp.gather(1, ids), F32, 3e-4)
