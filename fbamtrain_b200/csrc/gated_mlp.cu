@@ -756,15 +756,28 @@ refit_kernel(const elem_t* __restrict__ src, uint32_t ld, elem_t* __restrict__ d
 // 6.4 us, 1000 of 2730 to 2736 in 6.5 (element by element, with a division of 64 bits for each, 24 and 14).
 extern "C" int fbam_refit(const void* src, long long ld, void* dst, int blocks, int src_rows, int src_cols, int dst_rows, int dst_cols,
                           void* stream) {
-  const long long total = (long long)blocks * dst_rows * dst_cols;
-  if (blocks <= 0 || src_rows < 0 || src_cols < 0 || dst_rows <= 0 || dst_cols <= 0 || ld < 0 || ld > 0x7fffffff || total > 0x7fffffff ||
+  if (blocks <= 0 || src_rows < 0 || src_cols < 0 || dst_rows <= 0 || dst_cols <= 0 || ld < 0 || ld > 0x7fffffff ||
       (long long)blocks * src_rows > 0x7fffffff)
     return GEMM_ERR_SHAPE;
   const uintptr_t odd = reinterpret_cast<uintptr_t>(src) / 2 | reinterpret_cast<uintptr_t>(dst) / 2 | (uintptr_t)ld | src_cols | dst_cols;
-  auto go = [&](auto kernel, int u) {
-    const long long units = total / u, need = (units + 1023) / 1024;
+  auto part = [&](auto kernel, int u, const elem_t* from, elem_t* to, long long count, int from_rows, int to_rows) {
+    const long long units = count * to_rows * dst_cols / u, need = (units + 1023) / 1024;
     kernel<<<(unsigned)(need < 148 * 8 ? need : 148 * 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-        (const elem_t*)src, (uint32_t)ld, (elem_t*)dst, src_rows, src_cols, dst_rows, dst_cols, (uint32_t)units);
+        from, (uint32_t)ld, to, from_rows, src_cols, to_rows, dst_cols, (uint32_t)units);
+  };
+  // The kernel counts in 32 bits: blocks one by one, and a block in runs of rows, where there are more values than that.
+  constexpr long long kMost = 1ll << 31;
+  auto go = [&](auto kernel, int u) {
+    const elem_t* from = (const elem_t*)src;
+    elem_t* to = (elem_t*)dst;
+    if ((long long)blocks * dst_rows * dst_cols <= kMost) return part(kernel, u, from, to, blocks, src_rows, dst_rows);
+    const int run = (int)(kMost / dst_cols);
+    for (int b = 0; b < blocks; ++b)
+      for (long long r = 0; r < dst_rows; r += run) {
+        const long long left = src_rows - r, rows = dst_rows - r < run ? dst_rows - r : run;
+        part(kernel, u, from + (b * (long long)src_rows + r) * ld, to + (b * (long long)dst_rows + r) * dst_cols, 1,
+             (int)(left < 0 ? 0 : left < rows ? left : rows), (int)rows);
+      }
   };
   if (odd % 8 == 0) go(refit_kernel<8>, 8);
   else if (odd % 4 == 0) go(refit_kernel<4>, 4);

@@ -262,3 +262,31 @@ def test_logprobs_alternatives_of_any_vocabulary(rows, vocab, dtype):
         _, entropy, logp, _ = oracle.logprobs(logits[i:i + 1], torch.zeros(1, dtype=torch.int64, device="cuda"), 1.0)
         oracle.within(r.entropy[i:i + 1], entropy, F32, 3e-4)
         oracle.within(r.top_logprobs[i:i + 1], logp.gather(1, ids), F32, 3e-4)
+
+
+@pytest.mark.parametrize("width,out", [(1001, 8), (8, 1001)])
+def test_gated_mlp_beyond_32_bit_counts(width, out):
+    """More than 2^31 values of rows of an odd width, padded on the way in and cut on the way out."""
+    rows, some = 2_200_000, slice(-100, None)
+    gen = _gen("many rows", width)
+
+    def at_the_end(n, scale):
+        t = torch.zeros(rows, n, dtype=BF, device="cuda")
+        t[some] = _randn(gen, 100, n, dtype=BF, scale=scale)
+        return t
+
+    named = {"x": at_the_end(width, 1.0), "w_in": _randn(gen, 16, width, dtype=BF, scale=width ** -0.5),
+             "w_out": _randn(gen, out, 8, dtype=BF, scale=0.3), "b_in": _randn(gen, 16, dtype=BF), "b_out": _randn(gen, out, dtype=BF)}
+    dy = at_the_end(out, 0.5)
+    for v in named.values():
+        v.requires_grad_()
+    y = ops.gated_mlp(**named)
+    grads = dict(zip(named, torch.autograd.grad((y,), list(named.values()), (dy,))))
+    with torch.no_grad():
+        want, size = oracle.mlp(named["x"][some], *(named[k] for k in ("w_in", "w_out", "b_in", "b_out")), "gelu", None, dy[some])
+        relative = 1.01 * 2.0 ** -8 + 8 * (100 + width + 72) * 2.0 ** -24
+        oracle.within(y[some], want["y"], BF, relative * size["y"] + 1e-6)
+        oracle.within(grads["x"][some], want["x"], BF, relative * size["x"] + 1e-6)
+        for name in ("w_in", "w_out", "b_in", "b_out"):
+            oracle.within(grads[name], want[name], BF, relative * size[name] + 1e-6)
+        assert not grads["x"][:-100].any()
