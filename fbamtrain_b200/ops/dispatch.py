@@ -279,7 +279,7 @@ def gated_mlp(x, w_in, w_out, b_in=None, b_out=None, act: str = "gelu", residual
             raise ValueError(f"{name} is ({n},), got {tuple(bias.shape)}")
     if residual is not None and residual.shape != (*x.shape[:-1], w_out.shape[0]):
         raise ValueError(f"the residual is {(*x.shape[:-1], w_out.shape[0])}, got {tuple(residual.shape)}")
-    if x.numel() and _native(x, family="gemm"):
+    if x.numel() and w_out.shape[0] and _native(x, family="gemm"):
         from .feedforward import gated_mlp as f
         return f(x, w_in, w_out, b_in, b_out, act, residual)
     return ref.gated_mlp(x, w_in, w_out, b_in, b_out, act, residual)

@@ -290,3 +290,13 @@ def test_gated_mlp_beyond_32_bit_counts(width, out):
         for name in ("w_in", "w_out", "b_in", "b_out"):
             oracle.within(grads[name], want[name], BF, relative * size[name] + 1e-6)
         assert not grads["x"][:-100].any()
+
+
+def test_gated_mlp_without_outputs():
+    """No output columns: an empty result and gradients of zeros, as on the CPU."""
+    for device in ("cpu", "cuda"):
+        x, w_in, w_out = (torch.ones(*s, dtype=BF, device=device).requires_grad_() for s in ((3, 8), (12, 8), (0, 6)))
+        y = ops.gated_mlp(x, w_in, w_out)
+        assert y.shape == (3, 0) and y.dtype == BF
+        for g, of in zip(torch.autograd.grad((y,), (x, w_in, w_out), (torch.zeros_like(y),)), (x, w_in, w_out)):
+            assert g.shape == of.shape and not g.any()
