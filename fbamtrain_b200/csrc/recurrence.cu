@@ -11,8 +11,8 @@
 //
 // Bound: 8 bytes a value of h forward, 14 backward (16 bytes more for every 32 of them: the saved states).  The arithmetic is
 // close behind, four operations of the special-function units a value in either direction, so the two gates' exponentials and
-// reciprocals are formed once and everything else is packed.  Measured, bf16: 1 x 30011 x 2048 120 us forward (67 % of the
-// copy rate) and 194 us backward (70 %); 8 x 1024 x 1024 24 and 33 us.
+// reciprocals are formed once and everything else is packed.  Measured, bf16: 1 x 30011 x 2048 123 us forward (65 % of the
+// copy rate) and 198 us backward (68 %); 8 x 1024 x 1024 25 and 34 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -76,6 +76,18 @@ __device__ __forceinline__ Vec<1> rcp(Vec<1> a) { return {rcp(a.v)}; }
 __device__ __forceinline__ Vec<2> rcp(Vec<2> a) { return {make_float2(rcp(a.v.x), rcp(a.v.y))}; }
 __device__ __forceinline__ Vec<1> pick(bool c, Vec<1> a, Vec<1> b) { return {c ? a.v : b.v}; }
 __device__ __forceinline__ Vec<2> pick(bool c, Vec<2> a, Vec<2> b) { return {make_float2(c ? a.v.x : b.v.x, c ? a.v.y : b.v.y)}; }
+template <typename F>
+__device__ __forceinline__ Vec<1> map(F f, Vec<1> a, Vec<1> b) { return {f(a.v, b.v)}; }
+template <typename F>
+__device__ __forceinline__ Vec<2> map(F f, Vec<2> a, Vec<2> b) { return {make_float2(f(a.v.x, b.v.x), f(a.v.y, b.v.y))}; }
+template <typename F>
+__device__ __forceinline__ Vec<1> map(F f, Vec<1> a, Vec<1> b, Vec<1> c) { return {f(a.v, b.v, c.v)}; }
+template <typename F>
+__device__ __forceinline__ Vec<2> map(F f, Vec<2> a, Vec<2> b, Vec<2> c) {
+  return {make_float2(f(a.v.x, b.v.x, c.v.x), f(a.v.y, b.v.y, c.v.y))};
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> magnitude(Vec<VEC> a) { return map([](float x, float) { return fabsf(x); }, a, a); }
 
 // sigmoid(x) to full relative accuracy at both ends
 template <int VEC>
@@ -108,6 +120,35 @@ __device__ __forceinline__ void both_sigmoids(Vec<VEC> x, Vec<VEC>& s, Vec<VEC>&
   const Vec<VEC> e = ex2(below(x * Vec<VEC>::all(-kLog2e), 126.0f));
   s = rcp(e + Vec<VEC>::all(1.0f));
   s1 = e * s;
+}
+
+// What moves a state, to full relative accuracy whichever way the gate stands: -(1 - f), from h on, where f >= 1/2, and f, from z on,
+// where f < 1/2.  The fast walks have -(1 - f) throughout, which is a weight in this sense too.
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> weight(Vec<VEC> x) {
+  const auto of = [](float a, float m) { return __uint_as_float(__float_as_uint(m) | (~__float_as_uint(a) & 0x80000000u)); };
+  const Vec<VEC> e = ex2(magnitude(x) * Vec<VEC>::all(-kLog2e));
+  return map(of, x, e * rcp(e + Vec<VEC>::all(1.0f)));               // min(f, 1 - f) with the sign of -x
+}
+// a where the weight counts from h, else b
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> side(Vec<VEC> w, Vec<VEC> a, Vec<VEC> b) {
+  return map([](float w, float a, float b) { return __float_as_int(w) < 0 ? a : b; }, w, a, b);
+}
+// f h + (1 - f) z, with d = h - z
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> moved(Vec<VEC> w, Vec<VEC> d, Vec<VEC> h, Vec<VEC> z) { return fma(w, d, side(w, h, z)); }
+// f x
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> kept(Vec<VEC> w, Vec<VEC> x) { return fma(w, x, side(w, x, Vec<VEC>::all(0.0f))); }
+// -(1 - f) x
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> minus_taken(Vec<VEC> w, Vec<VEC> x) { return fma(w, x, side(w, Vec<VEC>::all(0.0f), minus(x))); }
+// f (1 - f) x
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> both(Vec<VEC> w, Vec<VEC> x) {
+  const Vec<VEC> m = magnitude(w);
+  return fma(minus(m), m, m) * x;
 }
 
 // VEC elements as they lie in memory
@@ -219,77 +260,90 @@ struct __align__(16) Exchange {
 // by (place of the CTA, place of the warp); round: of this launch, from 0.
 template <int VEC, int WARPS>
 struct Passing {
-  Link<VEC> own, before;            // of this warp, and of the warps of the CTA before it
+  Link<VEC> before;                 // of the warps of the CTA before this one
 
   __device__ __forceinline__ void send(Exchange<VEC, WARPS>& ex, int round, const Link<VEC>& mine, int place, bool backwards) {
-    own = mine;
-    if constexpr (WARPS > 1) {
-      const int lane = threadIdx.x % 32, turn = round & 1;
-      const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-      ex.warps[turn][place][lane] = mine;
-      __syncthreads();
-      before = Link<VEC>{Vec<VEC>::all(1.0f), Vec<VEC>::all(0.0f)};
-      if (ctas > 1) {
+    const int lane = threadIdx.x % 32, turn = round & 1;
+    const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+    ex.warps[turn][place][lane] = mine;
+    __syncthreads();
+    before = Link<VEC>{Vec<VEC>::all(1.0f), Vec<VEC>::all(0.0f)};
+    if (ctas > 1) {
 #pragma unroll
-        for (int w = 0; w < WARPS - 1; ++w)
-          if (w < place) before = before.then(ex.warps[turn][w][lane]);
-        if (place == WARPS - 1) {                                     // of the CTA as a whole
-          const Link<VEC> all = before.then(mine);
-          if (lane == 0) mbar_expect_tx(&ex.arrived[turn], ctas * 32 * (uint32_t)sizeof(Link<VEC>));
-          const int here = backwards ? ctas - 1 - rank : rank;
-          for (int c = 0; c < ctas; ++c) push(ex.cta(turn, here), &ex.arrived[turn], c, all);
-        }
+      for (int w = 0; w < WARPS - 1; ++w)
+        if (w < place) before = before.then(ex.warps[turn][w][lane]);
+      if (place == WARPS - 1) {                                       // of the CTA as a whole
+        const Link<VEC> all = before.then(mine);
+        if (lane == 0) mbar_expect_tx(&ex.arrived[turn], ctas * 32 * (uint32_t)sizeof(Link<VEC>));
+        const int here = backwards ? ctas - 1 - rank : rank;
+        for (int c = 0; c < ctas; ++c) push(ex.cta(turn, here), &ex.arrived[turn], c, all);
       }
     }
   }
 
   // What comes in to this warp's chunk; `carry` is what comes in to the cluster's first chunk, and becomes what its last hands on.
   __device__ __forceinline__ Vec<VEC> take(Exchange<VEC, WARPS>& ex, int round, int place, bool backwards, Vec<VEC>& carry, int* status) {
+    const int lane = threadIdx.x % 32, turn = round & 1;
+    const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
     Vec<VEC> in = carry;
-    if constexpr (WARPS == 1) {
-      carry = own(carry);
-    } else {
-      const int lane = threadIdx.x % 32, turn = round & 1;
-      const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
-      if (ctas == 1) {
+    if (ctas == 1) {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          if (w == place) in = carry;
-          carry = ex.warps[turn][w][lane](carry);
-        }
-      } else {
-        if (!mbar_wait(&ex.arrived[turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_EPILOGUE_TIMEOUT);
-        const int here = backwards ? ctas - 1 - rank : rank;
-#pragma unroll
-        for (int c = 0; c < kMaxCtas; ++c) {
-          if (c >= ctas) break;
-          if (c == here) in = carry;
-          carry = (*ex.cta(turn, c))(carry);
-        }
-        in = before(in);
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == place) in = carry;
+        carry = ex.warps[turn][w][lane](carry);
       }
+    } else {
+      if (!mbar_wait(&ex.arrived[turn], (round >> 1) & 1) && lane == 0) atomicExch(status, GEMM_ERR_EPILOGUE_TIMEOUT);
+      const int here = backwards ? ctas - 1 - rank : rank;
+#pragma unroll
+      for (int c = 0; c < kMaxCtas; ++c) {
+        if (c >= ctas) break;
+        if (c == here) in = carry;
+        carry = (*ex.cta(turn, c))(carry);
+      }
+      in = before(in);
     }
     return in;
   }
 };
 
-// The walks over a chunk of STEPS steps.  FAST: all of them are there and none is a reset.  z, g, o, d: functions of the step
-// that give the inputs (0 behind the end), put: one that takes an output.  nf1: -(1 - f).
-template <bool FAST, int STEPS, int VEC, typename Z, typename G>
-__device__ __forceinline__ void forward_in(Vec<VEC> (&nf1)[STEPS], Link<VEC>& link, int n, uint32_t bits, Z z, G g) {
+// The walks over a chunk of STEPS steps.  z, g, o, d: functions of the step that give the inputs (0 behind the end), put: one that
+// takes an output.
+// MASKED: steps may be missing at the end, or start a new sequence.
+// EXACT: gates may be closed.  The fast walks move by -(1 - f) only: 1 - f is known to its last bits where f is near 1, but f h is
+// off by a unit of h, which is much of it where f is small.  A chunk with a gate below kClosed (f = 1 / 150) is walked again by
+// `weight`, two selections more a step and channel; its warp begins the next chunks that way, until one has no gate below
+// kClosed + 1.  us with gates around 3 | 0 | -2 (spread 1), 1 x 30011 x 2048 bf16: forward 123 | 123 | 152, backward 198 | 198 | 239 (by the fast walks alone 120 and 195).
+constexpr float kClosed = -5.0f;
+__device__ __forceinline__ bool all_above(float least, float bound) { return __all_sync(0xffffffffu, least >= bound); }
+template <int VEC>
+__device__ __forceinline__ float lower(float least, Vec<VEC> g) { return fminf(fminf(least, g.get(0)), g.get(VEC - 1)); }
+
+// Returns the lowest gate.
+template <bool MASKED, bool EXACT, int STEPS, int VEC, typename Z, typename G>
+__device__ __forceinline__ float forward_in(Vec<VEC> (&w)[STEPS], Link<VEC>& link, int n, uint32_t bits, Z z, G g) {
   using V = Vec<VEC>;
+  float least = 0.0f;
   link.gain = V::all(1.0f);
   link.from0 = V::all(0.0f);
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
-    nf1[t] = minus_sigmoid_minus<VEC>(g(t));
-    if (!FAST && t >= n) nf1[t] = V::all(0.0f);             // behind the end nothing changes
-    if (!FAST && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
-    // h - (1 - f) (h - z): 1 - f is known to its last bits where f is near 1
-    link.from0 = fma(nf1[t], link.from0 - z(t), link.from0);
-    link.gain = fma(nf1[t], link.gain, link.gain);
+    if (MASKED && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
+    const V gate = g(t);
+    least = lower(least, gate);
+    w[t] = EXACT ? weight<VEC>(gate) : minus_sigmoid_minus<VEC>(gate);
+    if (MASKED && t >= n) w[t] = V::all(-0.0f);             // behind the end nothing changes
+    const V d = link.from0 - z(t);
+    if constexpr (EXACT) {
+      link.from0 = moved(w[t], d, link.from0, z(t));
+      link.gain = kept(w[t], link.gain);
+    } else {
+      link.from0 = fma(w[t], d, link.from0);
+      link.gain = fma(w[t], link.gain, link.gain);
+    }
   }
-  if (!FAST && bits) link.gain = V::all(-1.0f);
+  if (MASKED && bits) link.gain = V::all(-1.0f);
+  return least;
 }
 
 // Output gates are formed while links are on their way, but only the first kAhead of a chunk: they lie in registers until h is
@@ -302,70 +356,92 @@ __device__ __forceinline__ void forward_ahead(Vec<VEC> (&so)[kAhead], O o) {
   for (int t = 0; t < kAhead; ++t) so[t] = sigmoid<VEC>(o(t));
 }
 
-template <bool FAST, int STEPS, int VEC, typename Z, typename O, typename P>
-__device__ __forceinline__ void forward_out(const Vec<VEC> (&nf1)[STEPS], const Vec<VEC> (&so)[kAhead], Vec<VEC>& h, float* saved, int dim,
+template <bool MASKED, bool EXACT, int STEPS, int VEC, typename Z, typename O, typename P>
+__device__ __forceinline__ void forward_out(const Vec<VEC> (&w)[STEPS], const Vec<VEC> (&so)[kAhead], Vec<VEC>& h, float* saved, int dim,
                                             int n, uint32_t bits, Z z, O o, P put) {
   using V = Vec<VEC>;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
-    if (t % kSaved == 0 && saved != nullptr && (FAST || t < n)) store(saved + t / kSaved * dim, h);
-    if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
-    h = fma(nf1[t], h - z(t), h);
+    if (t % kSaved == 0 && saved != nullptr && (!MASKED || t < n)) store(saved + t / kSaved * dim, h);
+    if (MASKED && ((bits >> t) & 1)) h = V::all(0.0f);
+    const V d = h - z(t);
+    if constexpr (EXACT) h = moved(w[t], d, h, z(t));
+    else h = fma(w[t], d, h);
     put(t, (t < kAhead ? so[t] : sigmoid<VEC>(o(t))) * h);
   }
 }
 
-// What a link needs: nf1, nf, so1 = 1 - sigmoid(o), and dh0, the part of dh that a step's own y gives.
-template <bool FAST, int STEPS, int VEC, typename G, typename O, typename D>
-__device__ __forceinline__ void backward_in(Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&nf)[STEPS], Vec<VEC> (&so1)[STEPS], Vec<VEC> (&dh0)[STEPS],
-                                            Link<VEC>& link, int n, uint32_t bits, G g, O o, D d) {
+// What a link needs: w, nf = -f (not where EXACT), so1 = 1 - sigmoid(o), and dh0, the part of dh that a step's own y gives.
+template <bool MASKED, bool EXACT, int STEPS, int VEC, typename G, typename O, typename D>
+__device__ __forceinline__ float backward_in(Vec<VEC> (&w)[STEPS], Vec<VEC> (&nf)[STEPS], Vec<VEC> (&so1)[STEPS], Vec<VEC> (&dh0)[STEPS],
+                                             Link<VEC>& link, int n, uint32_t bits, G g, O o, D d) {
   using V = Vec<VEC>;
+  float least = 0.0f;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
     V so;
-    gates<VEC>(g(t), nf[t], nf1[t]);
+    const V gate = g(t);
+    least = lower(least, gate);
+    if constexpr (EXACT) w[t] = weight<VEC>(gate);
+    else gates<VEC>(gate, nf[t], w[t]);
     both_sigmoids<VEC>(o(t), so, so1[t]);
     dh0[t] = d(t) * so;
-    if (!FAST && t >= n) nf1[t] = dh0[t] = V::all(0.0f);    // behind the end e passes unchanged
+    if (MASKED && t >= n) w[t] = V::all(-0.0f), dh0[t] = V::all(0.0f);      // behind the end e passes unchanged
   }
   link.gain = V::all(1.0f);
   link.from0 = V::all(0.0f);
 #pragma unroll
   for (int t = STEPS - 1; t >= 0; --t) {
     const V dh = link.from0 + dh0[t];
-    link.from0 = fma(nf1[t], dh, dh);
-    if (!FAST && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
-    link.gain = fma(nf1[t], link.gain, link.gain);
+    if constexpr (EXACT) {
+      link.from0 = kept(w[t], dh);
+      link.gain = kept(w[t], link.gain);
+    } else {
+      link.from0 = fma(w[t], dh, dh);
+      link.gain = fma(w[t], link.gain, link.gain);
+    }
+    if (MASKED && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
   }
-  if (!FAST && bits) link.gain = V::all(-1.0f);
+  if (MASKED && bits) link.gain = V::all(-1.0f);
+  return least;
 }
 
 // Forwards over the chunk from the state h in front of it: the gradient of the output gates, and u, the factor of dg, over nf.
-template <bool FAST, int STEPS, int VEC, typename Z, typename P>
-__device__ __forceinline__ void backward_states(const Vec<VEC> (&nf1)[STEPS], Vec<VEC> (&nf)[STEPS], const Vec<VEC> (&so1)[STEPS],
+template <bool MASKED, bool EXACT, int STEPS, int VEC, typename Z, typename P>
+__device__ __forceinline__ void backward_states(const Vec<VEC> (&w)[STEPS], Vec<VEC> (&nf)[STEPS], const Vec<VEC> (&so1)[STEPS],
                                                 const Vec<VEC> (&dh0)[STEPS], Vec<VEC> h, uint32_t bits, Z z, P put) {
   using V = Vec<VEC>;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
-    if (!FAST && ((bits >> t) & 1)) h = V::all(0.0f);
+    if (MASKED && ((bits >> t) & 1)) h = V::all(0.0f);
     const V step = h - z(t);
-    h = fma(nf1[t], step, h);
-    nf[t] = (step * nf[t]) * nf1[t];
+    if constexpr (EXACT) {
+      h = moved(w[t], step, h, z(t));
+      nf[t] = both(w[t], step);
+    } else {
+      h = fma(w[t], step, h);
+      nf[t] = (step * nf[t]) * w[t];
+    }
     put(t, (dh0[t] * h) * so1[t]);
   }
 }
 
-template <bool FAST, int STEPS, int VEC, typename P, typename Q>
-__device__ __forceinline__ void backward_out(const Vec<VEC> (&nf1)[STEPS], const Vec<VEC> (&u)[STEPS], const Vec<VEC> (&dh0)[STEPS],
-                                             Vec<VEC> e, uint32_t bits, P put_z, Q put_g) {
+template <bool MASKED, bool EXACT, int STEPS, int VEC, typename P, typename Q>
+__device__ __forceinline__ void backward_out(const Vec<VEC> (&w)[STEPS], const Vec<VEC> (&u)[STEPS], const Vec<VEC> (&dh0)[STEPS],
+                                             Vec<VEC>& e, uint32_t bits, P put_z, Q put_g) {
   using V = Vec<VEC>;
 #pragma unroll
   for (int t = STEPS - 1; t >= 0; --t) {
     const V dh = e + dh0[t];
-    put_z(t, minus(nf1[t] * dh));
     put_g(t, u[t] * dh);
-    e = fma(nf1[t], dh, dh);
-    if (!FAST && ((bits >> t) & 1)) e = V::all(0.0f);
+    if constexpr (EXACT) {
+      put_z(t, minus(minus_taken(w[t], dh)));
+      e = kept(w[t], dh);
+    } else {
+      put_z(t, minus(w[t] * dh));
+      e = fma(w[t], dh, dh);
+    }
+    if (MASKED && ((bits >> t) & 1)) e = V::all(0.0f);
   }
 }
 
@@ -414,6 +490,7 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
   const Channels<VEC> c(unit % slabs, s.dim);
   Vec<VEC> carry = state_in != nullptr ? c.load(state_in + (long long)b * s.dim) : Vec<VEC>::all(0.0f);
   int round = 0;
+  bool closed = false;              // gates of the last chunk
   for (int c0 = 0; c0 < s.states; c0 += ctas * WARPS, ++round) {
     const int chunk = c0 + rank * WARPS + warp, t0 = chunk * STEPS;
     const int n = min(STEPS, s.steps - t0);                 // may be below 0
@@ -423,18 +500,30 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
     c.fetch(g, src + s.zk, s.zt, n);
     c.fetch(z, src, s.zt, n);
     c.fetch(o, src + 2 * s.zk, s.zt, n);
-    Vec<VEC> nf1[STEPS];
+    const auto get_z = [&](int t) { return z[t].get(); };
+    const auto get_g = [&](int t) { return g[t].get(); };
+    const auto get_o = [&](int t) { return o[t].get(); };
+    Vec<VEC> w[STEPS], so[kAhead];
     Link<VEC> link;
-    forward_in<false>(nf1, link, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return g[t].get(); });
-    Passing<VEC, WARPS> passing;
-    passing.send(ex, round, link, warp, false);
-    Vec<VEC> so[kAhead];
-    forward_ahead(so, [&](int t) { return o[t].get(); });
-    Vec<VEC> h = passing.take(ex, round, warp, false, carry, status);
+    Vec<VEC> h;
+    bool exact = WARPS == 1 || closed;
+    if (!exact) exact = !all_above(forward_in<true, false>(w, link, n, bits, get_z, get_g), kClosed);
+    if (exact) closed = !all_above(forward_in<true, true>(w, link, n, bits, get_z, get_g), kClosed + 1.0f);
+    if constexpr (WARPS == 1) {                             // needs no link
+      forward_ahead(so, get_o);
+      h = carry;
+    } else {
+      Passing<VEC, WARPS> passing;
+      passing.send(ex, round, link, warp, false);
+      forward_ahead(so, get_o);
+      h = passing.take(ex, round, warp, false, carry, status);
+    }
     elem_t* out = y + b * s.yb + t0 * s.yt;
     float* at = saved != nullptr && c.in ? saved + ((long long)b * s.states + chunk) * s.dim + c.ch : nullptr;
-    forward_out<false>(nf1, so, h, at, s.dim, n, bits, [&](int t) { return z[t].get(); }, [&](int t) { return o[t].get(); },
-                       [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * s.yt, v); });
+    const auto put = [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * s.yt, v); };
+    if (exact) forward_out<true, true>(w, so, h, at, s.dim, n, bits, get_z, get_o, put);
+    else forward_out<true, false>(w, so, h, at, s.dim, n, bits, get_z, get_o, put);
+    if constexpr (WARPS == 1) carry = h;
     if (t0 + STEPS >= s.steps && n > 0) c.put(state_out + (long long)b * s.dim, h);
   }
   if (ctas > 1) cluster_sync();     // no CTA leaves while another may still read its links
@@ -455,6 +544,7 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
   const Channels<VEC> c(unit % slabs, s.dim);
   Vec<VEC> carry = d_state_out != nullptr ? c.load(d_state_out + (long long)b * s.dim) : Vec<VEC>::all(0.0f);
   const int per_step = ctas * WARPS, rounds = (s.states + per_step - 1) / per_step;
+  bool closed = false;
   for (int round = 0; round < rounds; ++round) {
     const int chunk = (rounds - 1 - round) * per_step + rank * WARPS + warp, t0 = chunk * STEPS;
     const int n = min(STEPS, s.steps - t0);
@@ -467,17 +557,27 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
     c.fetch(o, src + 2 * s.zk, s.zt, n);
     c.fetch(d, dy + b * s.yb + t0 * s.yt, s.yt, n);
     const Vec<VEC> h = n > 0 ? c.load(saved + ((long long)b * s.states + chunk) * s.dim) : Vec<VEC>::all(0.0f);
-    Vec<VEC> nf1[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
+    const auto get_z = [&](int t) { return z[t].get(); };
+    const auto get_g = [&](int t) { return g[t].get(); };
+    const auto get_o = [&](int t) { return o[t].get(); };
+    const auto get_d = [&](int t) { return d[t].get(); };
+    const auto put_z = [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt, v); };
+    const auto put_g = [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt + s.dim, v); };
+    const auto put_o = [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt + 2 * s.dim, v); };
+    Vec<VEC> w[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
     Link<VEC> link;
-    backward_in<false>(nf1, u, so1, dh0, link, n, bits, [&](int t) { return g[t].get(); }, [&](int t) { return o[t].get(); },
-                       [&](int t) { return d[t].get(); });
+    bool exact = WARPS == 1 || closed;
+    if (!exact) exact = !all_above(backward_in<true, false>(w, u, so1, dh0, link, n, bits, get_g, get_o, get_d), kClosed);
+    if (exact) closed = !all_above(backward_in<true, true>(w, u, so1, dh0, link, n, bits, get_g, get_o, get_d), kClosed + 1.0f);
     Passing<VEC, WARPS> passing;
-    passing.send(ex, round, link, WARPS - 1 - warp, true);
-    backward_states<false>(nf1, u, so1, dh0, h, bits, [&](int t) { return z[t].get(); },
-                           [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt + 2 * s.dim, v); });
-    const Vec<VEC> e = passing.take(ex, round, WARPS - 1 - warp, true, carry, status);
-    backward_out<false>(nf1, u, dh0, e, bits, [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt, v); },
-                        [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * dt + s.dim, v); });
+    if constexpr (WARPS > 1) passing.send(ex, round, link, WARPS - 1 - warp, true);
+    if (exact) backward_states<true, true>(w, u, so1, dh0, h, bits, get_z, put_o);
+    else backward_states<true, false>(w, u, so1, dh0, h, bits, get_z, put_o);
+    Vec<VEC> e = carry;
+    if constexpr (WARPS > 1) e = passing.take(ex, round, WARPS - 1 - warp, true, carry, status);
+    if (exact) backward_out<true, true>(w, u, dh0, e, bits, put_z, put_g);
+    else backward_out<true, false>(w, u, dh0, e, bits, put_z, put_g);
+    if constexpr (WARPS == 1) carry = e;
   }
   if (rank == 0 && warp == 0 && d_state_in != nullptr) c.put(d_state_in + (long long)b * s.dim, carry);
   if (ctas > 1) cluster_sync();
@@ -538,11 +638,12 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     issue_o(t0, 0);
   }
   uint32_t next_bits = reset_bits(resets, s, b, t0, min(STEPS, s.steps - t0));
+  bool closed = false;              // gates of the last chunk
   for (int base = 0, round = 0; base < s.steps; base += per_step, t0 += per_step, ++round) {
     const int turn = round & 1;
     const int n = min(STEPS, s.steps - t0);                 // may be below 0
     const uint32_t bits = next_bits;
-    const bool fast = n == STEPS && bits == 0;
+    const bool whole = n == STEPS && bits == 0;
     const elem_t *zs = &sm.tiles[warp][turn][0][0][2 * lane], *gs = &sm.tiles[warp][turn][1][0][2 * lane];
     elem_t* oy = &sm.tiles[warp][turn][2][0][2 * lane];
     const bool more = t0 + per_step < s.steps;
@@ -553,10 +654,11 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     auto g = [&](int t) { return get(gs + t * kSlab); };
     auto o = [&](int t) { return get(oy + t * kSlab); };
     auto put = [&](int t, Vec<2> v) { store(oy + t * kSlab, v); };
-    Vec<2> nf1[STEPS], so[kAhead];
+    Vec<2> w[STEPS], so[kAhead];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
-    if (fast) forward_in<true>(nf1, link, n, bits, z, g);
-    else if (n > 0) forward_in<false>(nf1, link, n, bits, z, g);
+    bool exact = closed || !whole;
+    if (!exact) exact = !all_above(forward_in<false, false>(w, link, n, bits, z, g), kClosed);
+    if (exact && n > 0) closed = !all_above(forward_in<true, true>(w, link, n, bits, z, g), kClosed + 1.0f);
     Passing<2, kWarps> passing;
     passing.send(sm.ex, round, link, warp, false);
     // Results go over the output gates that they come from.  The ones of the step before take a while to leave the other buffer,
@@ -573,8 +675,8 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     Vec<2> h = passing.take(sm.ex, round, warp, false, carry, status);
     if (n <= 0) continue;
     float* at = saved != nullptr && in ? saved + ((long long)b * s.states + t0 / kSaved) * s.dim + ch : nullptr;
-    if (fast) forward_out<true>(nf1, so, h, at, s.dim, n, bits, z, o, put);
-    else forward_out<false>(nf1, so, h, at, s.dim, n, bits, z, o, put);
+    if (exact) forward_out<true, true>(w, so, h, at, s.dim, n, bits, z, o, put);
+    else forward_out<false, false>(w, so, h, at, s.dim, n, bits, z, o, put);
     if (in && t0 + STEPS >= s.steps) store(state_out + (long long)b * s.dim + ch, h);
     fence_proxy_async_smem();
     __syncwarp();
@@ -633,10 +735,11 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
   if (lane == 0 && t0 < s.steps) issue(t0, 0);
   uint32_t next_bits = reset_bits(resets, s, b, t0, min(STEPS, s.steps - t0));
   uint32_t phases = 0;
+  bool closed = false;
   for (int round = 0, stage = 0; round < rounds; ++round, t0 -= per_step, stage ^= 1) {
     const int n = min(STEPS, s.steps - t0);
     const uint32_t bits = next_bits;
-    const bool fast = n == STEPS && bits == 0;
+    const bool whole = n == STEPS && bits == 0;
     const elem_t *zgo = &sm.zgo[warp][stage][0][0][2 * lane], *dy = &sm.dy[warp][stage][0][2 * lane];
     elem_t* result = &sm.results[warp][0][0][2 * lane];
     if (n > 0) {
@@ -655,23 +758,24 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     auto put_z = [&](int t, Vec<2> v) { store(result + 3 * t * kSlab, v); };
     auto put_g = [&](int t, Vec<2> v) { store(result + (3 * t + 1) * kSlab, v); };
     auto put_o = [&](int t, Vec<2> v) { dout[t] = ff2e2(v.v.x, v.v.y); };
-    Vec<2> nf1[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
+    Vec<2> w[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
-    if (fast) backward_in<true>(nf1, u, so1, dh0, link, n, bits, g, o, d);
-    else if (n > 0) backward_in<false>(nf1, u, so1, dh0, link, n, bits, g, o, d);
+    bool exact = closed || !whole;
+    if (!exact) exact = !all_above(backward_in<false, false>(w, u, so1, dh0, link, n, bits, g, o, d), kClosed);
+    if (exact && n > 0) closed = !all_above(backward_in<true, true>(w, u, so1, dh0, link, n, bits, g, o, d), kClosed + 1.0f);
     Passing<2, kWarps> passing;
     passing.send(sm.ex, round, link, kWarps - 1 - warp, true);
     const Vec<2> h = load<2>(&sm.states[warp][stage][2 * lane]);
-    if (fast) backward_states<true>(nf1, u, so1, dh0, h, bits, z, put_o);
-    else if (n > 0) backward_states<false>(nf1, u, so1, dh0, h, bits, z, put_o);
-    const Vec<2> e = passing.take(sm.ex, round, kWarps - 1 - warp, true, carry, status);
+    if (!exact) backward_states<false, false>(w, u, so1, dh0, h, bits, z, put_o);
+    else if (n > 0) backward_states<true, true>(w, u, so1, dh0, h, bits, z, put_o);
+    Vec<2> e = passing.take(sm.ex, round, kWarps - 1 - warp, true, carry, status);
     if (n <= 0) continue;
     if (lane == 0) bulk_wait_group_read<0>();               // the results of the step before have left
     __syncwarp();
 #pragma unroll
     for (int t = 0; t < STEPS; ++t) *reinterpret_cast<elem2_t*>(result + (3 * t + 2) * kSlab) = dout[t];
-    if (fast) backward_out<true>(nf1, u, dh0, e, bits, put_z, put_g);
-    else backward_out<false>(nf1, u, dh0, e, bits, put_z, put_g);
+    if (exact) backward_out<true, true>(w, u, dh0, e, bits, put_z, put_g);
+    else backward_out<false, false>(w, u, dh0, e, bits, put_z, put_g);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {

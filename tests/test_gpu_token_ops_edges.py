@@ -300,3 +300,123 @@ def test_gated_mlp_without_outputs():
         assert y.shape == (3, 0) and y.dtype == BF
         for g, of in zip(torch.autograd.grad((y,), (x, w_in, w_out), (torch.zeros_like(y),)), (x, w_in, w_out)):
             assert g.shape == of.shape and not g.any()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# gated recurrence
+# ------------------------------------------------------------------------------------------------------------------
+UNIT = 2.0 ** -24
+
+
+def _scan_bounds(zgo, state, resets, dy, d_state, drop=None):
+    """In 64 bits, time first: y, the last state, d_zgo and d_state, and for each a bound of the absolute error of its fp32 value.
+
+    Every quantity goes through the scan three times: its value, the sum A of its terms' absolute values and its error E.  An
+    exponential's argument is rounded once and its value is off by 2 units, the reciprocal by one: (|g| + 8) units of min(f, 1 - f),
+    which is what moves the state; where f is small, but not far out (g >= -5), 1 - f may do.  So a step adds (|g| + 8) units of
+    q A with q = 1 - f where g >= -5 and f below, and 4 units of A for its sums and the product of gates that carries the same
+    value through a link; folding links adds 32 units of A at the end.
+    `drop`: a step in front of which what the steps behind it hand on is lost (a mistake, for the test of the bounds)."""
+    z, g, o = (x.transpose(0, 1) for x in zgo.detach().double().unbind(2))
+    f, f1, s, s1 = torch.sigmoid(g), torch.sigmoid(-g), torch.sigmoid(o), torch.sigmoid(-o)
+    q = torch.where(g >= -5, f1, f)
+    off_g, off_o = UNIT * (g.abs() + 8), UNIT * (o.abs() + 8)
+    steps = z.shape[0]
+    h = torch.zeros_like(z[0]) if state is None else state.detach().double()
+    size, err = h.abs(), torch.zeros_like(h)
+    before, after, e_before, e_after, a_after = [], [], [], [], []
+    for t in range(steps):
+        if resets is not None:
+            gone = resets[:, t].unsqueeze(1)
+            h, size, err = (torch.where(gone, torch.zeros_like(v), v) for v in (h, size, err))
+        before.append(h)
+        e_before.append(err + 32 * UNIT * size)
+        h = f[t] * h + f1[t] * z[t]
+        add = off_g[t] * q[t] * (size + z[t].abs())
+        size = f[t] * size + f1[t] * z[t].abs()
+        err = f[t] * err + add + 4 * UNIT * size
+        after.append(h)
+        e_after.append(err + 32 * UNIT * size)
+        a_after.append(size)
+    before, after, e_before, e_after, a_after = (torch.stack(v) for v in (before, after, e_before, e_after, a_after))
+    out = {"y": (s * after).transpose(0, 1), "last": h}
+    bound = {"y": (s * e_after + 2 * off_o * s * a_after).transpose(0, 1), "last": e_after[-1]}
+    d = dy.detach().double().transpose(0, 1)
+    e = torch.zeros_like(z[0]) if d_state is None else d_state.detach().double()
+    size, err = e.abs(), torch.zeros_like(e)
+    grads, bounds = [], []
+    for t in range(steps - 1, -1, -1):
+        if t + 1 == drop:
+            e = torch.zeros_like(e)
+        dh = d[t] * s[t] + e
+        a = d[t].abs() * s[t] + size
+        eh = err + 32 * UNIT * size + 2 * off_o[t] * d[t].abs() * s[t] + UNIT * a
+        step = before[t] - z[t]
+        e_step = e_before[t] + UNIT * (before[t].abs() + z[t].abs())
+        grads.append(torch.stack([dh * f1[t], dh * step * f[t] * f1[t], d[t] * after[t] * s[t] * s1[t]], 1))
+        bounds.append(torch.stack([f1[t] * (eh + 2 * off_g[t] * a),
+                                   f[t] * f1[t] * (step.abs() * eh + a * e_step + 4 * off_g[t] * a * (step.abs() + e_step)),
+                                   d[t].abs() * s[t] * s1[t] * (e_after[t] + 4 * off_o[t] * a_after[t])], 1))
+        add = off_g[t] * q[t] * a + 4 * UNIT * f[t] * a
+        e, size, err = f[t] * dh, f[t] * a, f[t] * (err + 2 * off_o[t] * d[t].abs() * s[t] + UNIT * a) + add
+        if resets is not None:
+            gone = resets[:, t].unsqueeze(1)
+            e, size, err = (torch.where(gone, torch.zeros_like(v), v) for v in (e, size, err))
+    out.update(d_zgo=torch.stack(grads[::-1], 1), d_state=e)
+    bound.update(d_zgo=torch.stack(bounds[::-1], 1), d_state=err + 32 * UNIT * size)
+    return out, bound
+
+
+def _recurrence_case(b, t, d, dtype, kind, extras, time_major):
+    gen = _gen("recurrence", b, t, d, kind, extras)
+    zgo = _randn(gen, t, b, 3, d, dtype=dtype).transpose(0, 1) if time_major else _randn(gen, b, t, 3, d, dtype=dtype)
+    if kind == "long":                      # memories of some twenty steps
+        zgo[:, :, 1] += 3.0
+    elif kind == "short":                   # of one or two
+        pass
+    elif kind == "closed":                  # most gates far out on either side, and values of very different sizes
+        zgo[:, :, 1] = (torch.rand(b, t, d, generator=gen, device="cuda") * 60 - 30).to(dtype)
+        zgo[:, :, 0] *= torch.tensor([1.0, 1000.0, 0.01, 30.0], device="cuda").to(dtype).repeat(d // 4 + 1)[:d]
+    state = _randn(gen, b, d, scale=1e4 if kind == "closed" else 1.0) if "state" in extras else None
+    resets = torch.rand(b, t, generator=gen, device="cuda") < 0.01 if "resets" in extras else None
+    return zgo, state, resets, _randn(gen, b, t, d, dtype=dtype), _randn(gen, b, d)
+
+
+def _recurrence_run(zgo, state, resets, dy, d_state):
+    zgo = zgo.detach().requires_grad_()
+    state = None if state is None else state.detach().requires_grad_()
+    y, last = ops.gated_recurrence(zgo, state, resets)
+    grads = torch.autograd.grad((y, last), (zgo,) if state is None else (zgo, state), (dy, d_state))
+    return {"y": y, "last": last, "d_zgo": grads[0], "d_state": grads[1] if state is not None else None}
+
+
+# whole chunks and parts, one round and several of one CTA and of clusters, tiled and plain
+RECURRENCE = [(2, 1, 64), (3, 5, 40), (2, 8, 33), (2, 128, 64), (1, 129, 130), (2, 257, 96), (1, 1025, 72), (1, 4100, 64), (1, 2100, 1300),
+              (3, 700, 1024), (2, 900, 1416), (1, 2500, 65), (93, 200, 64)]
+
+
+@pytest.mark.parametrize("b,t,d", RECURRENCE)
+@pytest.mark.parametrize("kind", ["long", "short", "closed"])
+@pytest.mark.parametrize("extras", ["", "state", "state resets"])
+def test_recurrence_values_and_gradients(b, t, d, kind, extras):
+    """Each value against its own bound."""
+    dtype = HALF if extras == "state" else BF
+    case = _recurrence_case(b, t, d, dtype, kind, extras, time_major=extras == "state")
+    want, bound = _scan_bounds(*case)
+    for name, got in _recurrence_run(*case).items():
+        if got is not None:
+            oracle.within(got, want[name], F32 if name in ("last", "d_state") else dtype, bound[name])
+
+
+@pytest.mark.parametrize("b,t,d", [(2, 128, 64), (1, 1025, 72), (1, 4100, 64), (3, 700, 1024)])
+def test_recurrence_bounds_see_what_is_missing(b, t, d):
+    """A gradient of zeros is outside the bounds nearly everywhere, and one that lost what is handed on in front of any chunk is
+    outside in the steps before."""
+    case = _recurrence_case(b, t, d, BF, "long", "state", False)
+    want, bound = _scan_bounds(*case)
+    allowed = bound["d_zgo"] + 2.0 ** -8 * want["d_zgo"].abs() + 2.0 ** -25
+    assert float((allowed < want["d_zgo"].abs()).double().mean()) > 0.99
+    for drop in (8, t // 2 // 8 * 8, (t - 1) // 8 * 8):
+        wrong, _ = _scan_bounds(*case, drop=drop)
+        over = (wrong["d_zgo"] - want["d_zgo"]).abs() > allowed
+        assert bool(over[:, drop - 1, 0].any())
