@@ -11,8 +11,8 @@
 //
 // Bound: 8 bytes a value of h forward, 14 backward (16 bytes more for every 32 of them: the saved states).  The arithmetic is
 // close behind, four operations of the special-function units a value in either direction, so the two gates' exponentials and
-// reciprocals are formed once and everything else is packed.  Measured, bf16: 1 x 30011 x 2048 123 us forward (65 % of the
-// copy rate) and 198 us backward (68 %); 8 x 1024 x 1024 25 and 34 us.
+// reciprocals are formed once and everything else is packed.  Measured, bf16: 1 x 30011 x 2048 121 us forward (66 % of the
+// copy rate) and 203 us backward (67 %); 8 x 1024 x 1024 25 and 34 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -151,6 +151,42 @@ __device__ __forceinline__ Vec<VEC> both(Vec<VEC> w, Vec<VEC> x) {
   return fma(minus(m), m, m) * x;
 }
 
+// The same where values may be infinite, or their difference.  A gate's share is above 0 however small it is in fp32.
+__device__ __forceinline__ float share(float a) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(1.17549435e-38f));
+  return r;
+}
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
+__device__ __forceinline__ float f_of(float w) { return __float_as_int(w) < 0 ? 1.0f + w : w; }
+__device__ __forceinline__ float f1_of(float w) { return __float_as_int(w) < 0 ? -w : 1.0f - w; }
+__device__ __forceinline__ float share_of(float a, float x) { return (is_finite(x) ? a : share(a)) * x; }
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> share_of(Vec<VEC> a, Vec<VEC> x) {
+  return map([](float a, float x) { return share_of(a, x); }, a, x);
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> any_moved(Vec<VEC> w, Vec<VEC> h, Vec<VEC> z) {
+  return map([](float w, float h, float z) {
+    const float d = h - z;
+    return is_finite(d) ? fmaf(w, d, __float_as_int(w) < 0 ? h : z) : fmaf(share(f_of(w)), h, share(f1_of(w)) * z);
+  }, w, h, z);
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> any_kept(Vec<VEC> w, Vec<VEC> x) {
+  return map([](float w, float x) { return is_finite(x) ? fmaf(w, x, __float_as_int(w) < 0 ? x : 0.0f) : share(f_of(w)) * x; }, w, x);
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> any_taken(Vec<VEC> w, Vec<VEC> x) {
+  return map([](float w, float x) {
+    return is_finite(x) ? -fmaf(w, x, __float_as_int(w) < 0 ? 0.0f : -x) : share(f1_of(w)) * x;
+  }, w, x);
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> any_both(Vec<VEC> w, Vec<VEC> x) {
+  return map([](float w, float x) { return share_of(fmaf(-fabsf(w), fabsf(w), fabsf(w)), x); }, w, x);
+}
+
 // VEC elements as they lie in memory
 template <int VEC>
 struct Raw {
@@ -178,7 +214,13 @@ __device__ __forceinline__ Vec<VEC> load(const float* p) {
 }
 
 // What a chunk makes of a value that comes in.  A gain below 0 marks a chunk with a reset: nothing of what comes in goes on,
-// not even as a product of 0 with an infinity or a NaN of the sequence before.
+// not even as a product of 0 with an infinity or a NaN of the sequence before.  A gain is never 0, for the same reason: of an
+// infinite value that comes in, however small a share is infinite.
+constexpr float kLeastGain = 0x1p-149f;
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> above_zero(Vec<VEC> gain) {      // a NaN, which is in from0 too, is not kept
+  return map([](float a, float b) { return fmaxf(a, b); }, gain, Vec<VEC>::all(kLeastGain));
+}
 template <int VEC>
 struct Link {
   Vec<VEC> gain, from0;
@@ -189,6 +231,7 @@ struct Link {
   __device__ __forceinline__ Link then(const Link& next) const {
     return {pick(gain.get(0) < 0.0f || next.gain.get(0) < 0.0f, Vec<VEC>::all(-1.0f), gain * next.gain), next(from0)};
   }
+  __device__ __forceinline__ Link above0() const { return {pick(gain.get(0) < 0.0f, gain, above_zero(gain)), from0}; }
 };
 
 struct Shape {
@@ -272,8 +315,9 @@ struct Passing {
 #pragma unroll
       for (int w = 0; w < WARPS - 1; ++w)
         if (w < place) before = before.then(ex.warps[turn][w][lane]);
+      before = before.above0();
       if (place == WARPS - 1) {                                       // of the CTA as a whole
-        const Link<VEC> all = before.then(mine);
+        const Link<VEC> all = before.then(mine).above0();
         if (lane == 0) mbar_expect_tx(&ex.arrived[turn], ctas * 32 * (uint32_t)sizeof(Link<VEC>));
         const int here = backwards ? ctas - 1 - rank : rank;
         for (int c = 0; c < ctas; ++c) push(ex.cta(turn, here), &ex.arrived[turn], c, all);
@@ -313,24 +357,41 @@ struct Passing {
 // EXACT: gates may be closed.  The fast walks move by -(1 - f) only: 1 - f is known to its last bits where f is near 1, but f h is
 // off by a unit of h, which is much of it where f is small.  A chunk with a gate below kClosed (f = 1 / 150) is walked again by
 // `weight`, two selections more a step and channel; its warp begins the next chunks that way, until one has no gate below
-// kClosed + 1.  us with gates around 3 | 0 | -2 (spread 1), 1 x 30011 x 2048 bf16: forward 123 | 123 | 152, backward 198 | 198 | 239 (by the fast walks alone 120 and 195).
+// kClosed + 1.  us with gates around 3 | 0 | -2 (spread 1), 1 x 30011 x 2048 bf16: forward 121 | 121 | 152, backward 203 | 203 | 239 (by the
+// fast walks alone 119 and 193).
 constexpr float kClosed = -5.0f;
-__device__ __forceinline__ bool all_above(float least, float bound) { return __all_sync(0xffffffffu, least >= bound); }
+// What the walks find out for the whole warp: the lowest gate, and whether every value that they passed was finite and no
+// difference of two beyond the largest number (`probe` stays 0, else it becomes NaN; looked at in front of a reset and at the end,
+// since what is not finite stays so).  Where one was not, `any_forward` and `any_backward` do the chunk again.
 template <int VEC>
-__device__ __forceinline__ float lower(float least, Vec<VEC> g) { return fminf(fminf(least, g.get(0)), g.get(VEC - 1)); }
-
-// Returns the lowest gate.
-template <bool MASKED, bool EXACT, int STEPS, int VEC, typename Z, typename G>
-__device__ __forceinline__ float forward_in(Vec<VEC> (&w)[STEPS], Link<VEC>& link, int n, uint32_t bits, Z z, G g) {
-  using V = Vec<VEC>;
+struct Found {
   float least = 0.0f;
+  Vec<VEC> probe = Vec<VEC>::all(0.0f);
+  __device__ __forceinline__ void gate(Vec<VEC> g) { least = fminf(fminf(least, g.get(0)), g.get(VEC - 1)); }
+  __device__ __forceinline__ void value(Vec<VEC> x) { probe = fma(x, Vec<VEC>::all(0.0f), probe); }
+  __device__ __forceinline__ bool clean() const { return probe.get(0) == 0.0f && probe.get(VEC - 1) == 0.0f; }
+  __device__ __forceinline__ bool all_clean() const { return __all_sync(0xffffffffu, clean()); }
+  __device__ __forceinline__ bool all_open(float bound) const { return __all_sync(0xffffffffu, least >= bound); }
+  __device__ __forceinline__ bool all_fast() const { return __all_sync(0xffffffffu, least >= kClosed && clean()); }
+};
+// A value that comes in to a chunk of finite ones: so far below the largest number that it moves no difference beyond it
+template <int VEC>
+__device__ __forceinline__ bool moderate(Vec<VEC> x) { return fabsf(x.get(0)) < 0x1p60f && fabsf(x.get(VEC - 1)) < 0x1p60f; }
+
+template <bool MASKED, bool EXACT, int STEPS, int VEC, typename Z, typename G>
+__device__ __forceinline__ Found<VEC> forward_in(Vec<VEC> (&w)[STEPS], Link<VEC>& link, int n, uint32_t bits, Z z, G g) {
+  using V = Vec<VEC>;
+  Found<VEC> found;
   link.gain = V::all(1.0f);
   link.from0 = V::all(0.0f);
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
-    if (MASKED && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
+    if (MASKED && ((bits >> t) & 1)) {
+      found.value(link.from0);
+      link.from0 = V::all(0.0f);
+    }
     const V gate = g(t);
-    least = lower(least, gate);
+    found.gate(gate);
     w[t] = EXACT ? weight<VEC>(gate) : minus_sigmoid_minus<VEC>(gate);
     if (MASKED && t >= n) w[t] = V::all(-0.0f);             // behind the end nothing changes
     const V d = link.from0 - z(t);
@@ -342,8 +403,10 @@ __device__ __forceinline__ float forward_in(Vec<VEC> (&w)[STEPS], Link<VEC>& lin
       link.gain = fma(w[t], link.gain, link.gain);
     }
   }
+  if (EXACT) link.gain = above_zero(link.gain);
   if (MASKED && bits) link.gain = V::all(-1.0f);
-  return least;
+  found.value(link.from0);
+  return found;
 }
 
 // Output gates are formed while links are on their way, but only the first kAhead of a chunk: they lie in registers until h is
@@ -357,31 +420,65 @@ __device__ __forceinline__ void forward_ahead(Vec<VEC> (&so)[kAhead], O o) {
 }
 
 template <bool MASKED, bool EXACT, int STEPS, int VEC, typename Z, typename O, typename P>
-__device__ __forceinline__ void forward_out(const Vec<VEC> (&w)[STEPS], const Vec<VEC> (&so)[kAhead], Vec<VEC>& h, float* saved, int dim,
-                                            int n, uint32_t bits, Z z, O o, P put) {
+__device__ __forceinline__ Found<VEC> forward_out(const Vec<VEC> (&w)[STEPS], const Vec<VEC> (&so)[kAhead], Vec<VEC>& h, float* saved, int dim,
+                                                  int n, uint32_t bits, Z z, O o, P put) {
   using V = Vec<VEC>;
+  Found<VEC> found;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
     if (t % kSaved == 0 && saved != nullptr && (!MASKED || t < n)) store(saved + t / kSaved * dim, h);
-    if (MASKED && ((bits >> t) & 1)) h = V::all(0.0f);
+    if (MASKED && ((bits >> t) & 1)) {
+      found.value(h);
+      h = V::all(0.0f);
+    }
     const V d = h - z(t);
     if constexpr (EXACT) h = moved(w[t], d, h, z(t));
     else h = fma(w[t], d, h);
     put(t, (t < kAhead ? so[t] : sigmoid<VEC>(o(t))) * h);
   }
+  found.value(h);
+  return found;
+}
+
+// The link and the outputs of a chunk whose values may be infinite, in loops of few instructions.  What is finite of it has the bits
+// of the walk that it stands for.
+template <int VEC, typename Z, typename G>
+__device__ __forceinline__ void any_forward_in(bool exact, Link<VEC>& link, int n, uint32_t bits, Z z, G g) {
+  using V = Vec<VEC>;
+  link.gain = V::all(1.0f);
+  link.from0 = V::all(0.0f);
+#pragma unroll 1
+  for (int t = 0; t < n; ++t) {
+    const V w = exact ? weight<VEC>(g(t)) : minus_sigmoid_minus<VEC>(g(t));
+    if ((bits >> t) & 1) link.from0 = V::all(0.0f);
+    link.from0 = any_moved<VEC>(w, link.from0, z(t));
+    link.gain = kept(w, link.gain);
+  }
+  link.gain = bits ? V::all(-1.0f) : above_zero(link.gain);
+}
+template <int VEC, typename Z, typename G, typename O, typename P>
+__device__ __forceinline__ void any_forward_out(bool exact, Vec<VEC>& h, float* saved, int dim, int n, uint32_t bits, Z z, G g, O o, P put) {
+  using V = Vec<VEC>;
+#pragma unroll 1
+  for (int t = 0; t < n; ++t) {
+    if (t % kSaved == 0 && saved != nullptr) store(saved + t / kSaved * dim, h);
+    if ((bits >> t) & 1) h = V::all(0.0f);
+    h = any_moved<VEC>(exact ? weight<VEC>(g(t)) : minus_sigmoid_minus<VEC>(g(t)), h, z(t));
+    put(t, share_of(sigmoid<VEC>(o(t)), h));
+  }
 }
 
 // What a link needs: w, nf = -f (not where EXACT), so1 = 1 - sigmoid(o), and dh0, the part of dh that a step's own y gives.
 template <bool MASKED, bool EXACT, int STEPS, int VEC, typename G, typename O, typename D>
-__device__ __forceinline__ float backward_in(Vec<VEC> (&w)[STEPS], Vec<VEC> (&nf)[STEPS], Vec<VEC> (&so1)[STEPS], Vec<VEC> (&dh0)[STEPS],
-                                             Link<VEC>& link, int n, uint32_t bits, G g, O o, D d) {
+__device__ __forceinline__ Found<VEC> backward_in(Vec<VEC> (&w)[STEPS], Vec<VEC> (&nf)[STEPS], Vec<VEC> (&so1)[STEPS],
+                                                  Vec<VEC> (&dh0)[STEPS], Link<VEC>& link, int n, uint32_t bits, G g, O o, D d) {
   using V = Vec<VEC>;
-  float least = 0.0f;
+  Found<VEC> found;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
     V so;
     const V gate = g(t);
-    least = lower(least, gate);
+    found.gate(gate);
     if constexpr (EXACT) w[t] = weight<VEC>(gate);
     else gates<VEC>(gate, nf[t], w[t]);
     both_sigmoids<VEC>(o(t), so, so1[t]);
@@ -400,20 +497,29 @@ __device__ __forceinline__ float backward_in(Vec<VEC> (&w)[STEPS], Vec<VEC> (&nf
       link.from0 = fma(w[t], dh, dh);
       link.gain = fma(w[t], link.gain, link.gain);
     }
-    if (MASKED && ((bits >> t) & 1)) link.from0 = V::all(0.0f);
+    if (MASKED && ((bits >> t) & 1)) {
+      found.value(link.from0);
+      link.from0 = V::all(0.0f);
+    }
   }
+  if (EXACT) link.gain = above_zero(link.gain);
   if (MASKED && bits) link.gain = V::all(-1.0f);
-  return least;
+  found.value(link.from0);
+  return found;
 }
 
 // Forwards over the chunk from the state h in front of it: the gradient of the output gates, and u, the factor of dg, over nf.
 template <bool MASKED, bool EXACT, int STEPS, int VEC, typename Z, typename P>
-__device__ __forceinline__ void backward_states(const Vec<VEC> (&w)[STEPS], Vec<VEC> (&nf)[STEPS], const Vec<VEC> (&so1)[STEPS],
-                                                const Vec<VEC> (&dh0)[STEPS], Vec<VEC> h, uint32_t bits, Z z, P put) {
+__device__ __forceinline__ Found<VEC> backward_states(const Vec<VEC> (&w)[STEPS], Vec<VEC> (&nf)[STEPS], const Vec<VEC> (&so1)[STEPS],
+                                                      const Vec<VEC> (&dh0)[STEPS], Vec<VEC> h, uint32_t bits, Z z, P put) {
   using V = Vec<VEC>;
+  Found<VEC> found;
 #pragma unroll
   for (int t = 0; t < STEPS; ++t) {
-    if (MASKED && ((bits >> t) & 1)) h = V::all(0.0f);
+    if (MASKED && ((bits >> t) & 1)) {
+      found.value(h);
+      h = V::all(0.0f);
+    }
     const V step = h - z(t);
     if constexpr (EXACT) {
       h = moved(w[t], step, h, z(t));
@@ -424,12 +530,15 @@ __device__ __forceinline__ void backward_states(const Vec<VEC> (&w)[STEPS], Vec<
     }
     put(t, (dh0[t] * h) * so1[t]);
   }
+  found.value(h);
+  return found;
 }
 
 template <bool MASKED, bool EXACT, int STEPS, int VEC, typename P, typename Q>
-__device__ __forceinline__ void backward_out(const Vec<VEC> (&w)[STEPS], const Vec<VEC> (&u)[STEPS], const Vec<VEC> (&dh0)[STEPS],
-                                             Vec<VEC>& e, uint32_t bits, P put_z, Q put_g) {
+__device__ __forceinline__ Found<VEC> backward_out(const Vec<VEC> (&w)[STEPS], const Vec<VEC> (&u)[STEPS], const Vec<VEC> (&dh0)[STEPS],
+                                                   Vec<VEC>& e, uint32_t bits, P put_z, Q put_g) {
   using V = Vec<VEC>;
+  Found<VEC> found;
 #pragma unroll
   for (int t = STEPS - 1; t >= 0; --t) {
     const V dh = e + dh0[t];
@@ -441,7 +550,57 @@ __device__ __forceinline__ void backward_out(const Vec<VEC> (&w)[STEPS], const V
       put_z(t, minus(w[t] * dh));
       e = fma(w[t], dh, dh);
     }
-    if (MASKED && ((bits >> t) & 1)) e = V::all(0.0f);
+    if (MASKED && ((bits >> t) & 1)) {
+      found.value(e);
+      e = V::all(0.0f);
+    }
+  }
+  found.value(e);
+  return found;
+}
+
+// The same for a chunk whose values may be infinite: its link, and all of its gradients.
+template <int VEC, typename G, typename O, typename D>
+__device__ __forceinline__ void any_backward_in(bool exact, Link<VEC>& link, int n, uint32_t bits, G g, O o, D d) {
+  using V = Vec<VEC>;
+  link.gain = V::all(1.0f);
+  link.from0 = V::all(0.0f);
+#pragma unroll 1
+  for (int t = n - 1; t >= 0; --t) {
+    V w, nf, so, so1;
+    gates<VEC>(g(t), nf, w);
+    if (exact) w = weight<VEC>(g(t));
+    both_sigmoids<VEC>(o(t), so, so1);
+    link.from0 = any_kept<VEC>(w, link.from0 + share_of(so, d(t)));
+    if ((bits >> t) & 1) link.from0 = V::all(0.0f);
+    link.gain = kept(w, link.gain);
+  }
+  link.gain = bits ? V::all(-1.0f) : above_zero(link.gain);
+}
+// h: in front of the chunk.  The state in front of a step is walked to anew for each.
+template <int VEC, typename Z, typename G, typename O, typename D, typename P, typename Q, typename R>
+__device__ __forceinline__ void any_backward(bool exact, const Vec<VEC> h, Vec<VEC>& e, int n, uint32_t bits, Z z, G g, O o, D d, P put_z,
+                                             Q put_g, R put_o) {
+  using V = Vec<VEC>;
+#pragma unroll 1
+  for (int t = n - 1; t >= 0; --t) {
+    V at = h, before = h, w, nf;
+#pragma unroll 1
+    for (int q = 0; q <= t; ++q) {
+      gates<VEC>(g(q), nf, w);
+      if (exact) w = weight<VEC>(g(q));
+      before = (bits >> q) & 1 ? V::all(0.0f) : at;
+      at = any_moved<VEC>(w, before, z(q));
+    }
+    V so, so1;
+    both_sigmoids<VEC>(o(t), so, so1);
+    const V step = before - z(t), dh0 = share_of(so, d(t)), dh = e + dh0;
+    const V fast = share_of(minus(w), share_of(minus(nf), step));
+    put_o(t, share_of(so1, dh0 * at));
+    put_g(t, (exact ? any_both<VEC>(w, step) : fast) * dh);
+    put_z(t, any_taken<VEC>(w, dh));
+    e = any_kept<VEC>(w, dh);
+    if ((bits >> t) & 1) e = V::all(0.0f);
   }
 }
 
@@ -465,6 +624,11 @@ struct Channels {
       r[t].u = 0;
       if (t < n) r[t].load(row + t * step + ch);
     }
+  }
+  __device__ __forceinline__ Vec<VEC> read(const elem_t* row) const {
+    Raw<VEC> r;
+    r.load(row + ch);
+    return r.get();
   }
   __device__ __forceinline__ Vec<VEC> load(const float* row) const {
     if constexpr (VEC == 1) return {row[ch]};
@@ -507,22 +671,43 @@ recurrence_fwd_kernel(const elem_t* __restrict__ zgo, const float* __restrict__ 
     Link<VEC> link;
     Vec<VEC> h;
     bool exact = WARPS == 1 || closed;
-    if (!exact) exact = !all_above(forward_in<true, false>(w, link, n, bits, get_z, get_g), kClosed);
-    if (exact) closed = !all_above(forward_in<true, true>(w, link, n, bits, get_z, get_g), kClosed + 1.0f);
+    bool any = false;
+    if (!exact) {
+      const Found<VEC> found = forward_in<true, false>(w, link, n, bits, get_z, get_g);
+      if (__builtin_expect(!found.all_fast(), 0)) {
+        exact = !found.all_open(kClosed);
+        any = !exact;
+      }
+    }
+    if (exact) {
+      const Found<VEC> found = forward_in<true, true>(w, link, n, bits, get_z, get_g);
+      if constexpr (WARPS > 1) {
+        closed = !found.all_open(kClosed + 1.0f);
+        any = !found.all_clean();
+      }
+    }
+    const auto mem_z = [&](int t) { return c.read(src + t * s.zt); };
+    const auto mem_g = [&](int t) { return c.read(src + t * s.zt + s.zk); };
+    const auto mem_o = [&](int t) { return c.read(src + t * s.zt + 2 * s.zk); };
     if constexpr (WARPS == 1) {                             // needs no link
       forward_ahead(so, get_o);
       h = carry;
     } else {
+      if (__builtin_expect(any, 0)) any_forward_in<VEC>(exact, link, n, bits, mem_z, mem_g);
       Passing<VEC, WARPS> passing;
       passing.send(ex, round, link, warp, false);
       forward_ahead(so, get_o);
       h = passing.take(ex, round, warp, false, carry, status);
+      any = any || !__all_sync(0xffffffffu, moderate(h));
     }
     elem_t* out = y + b * s.yb + t0 * s.yt;
     float* at = saved != nullptr && c.in ? saved + ((long long)b * s.states + chunk) * s.dim + c.ch : nullptr;
     const auto put = [&](int t, Vec<VEC> v) { if (t < n) c.put(out + t * s.yt, v); };
-    if (exact) forward_out<true, true>(w, so, h, at, s.dim, n, bits, get_z, get_o, put);
-    else forward_out<true, false>(w, so, h, at, s.dim, n, bits, get_z, get_o, put);
+    if (!any) {
+      if (!exact) forward_out<true, false>(w, so, h, at, s.dim, n, bits, get_z, get_o, put);
+      else if (!forward_out<true, true>(w, so, h, at, s.dim, n, bits, get_z, get_o, put).all_clean() && WARPS == 1) any = true, h = carry;
+    }
+    if (__builtin_expect(any, 0)) any_forward_out<VEC>(exact, h, at, s.dim, n, bits, mem_z, mem_g, mem_o, put);
     if constexpr (WARPS == 1) carry = h;
     if (t0 + STEPS >= s.steps && n > 0) c.put(state_out + (long long)b * s.dim, h);
   }
@@ -567,16 +752,46 @@ recurrence_bwd_kernel(const elem_t* __restrict__ zgo, const uint8_t* __restrict_
     Vec<VEC> w[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
     Link<VEC> link;
     bool exact = WARPS == 1 || closed;
-    if (!exact) exact = !all_above(backward_in<true, false>(w, u, so1, dh0, link, n, bits, get_g, get_o, get_d), kClosed);
-    if (exact) closed = !all_above(backward_in<true, true>(w, u, so1, dh0, link, n, bits, get_g, get_o, get_d), kClosed + 1.0f);
+    bool any = false;
+    if (!exact) {
+      const Found<VEC> found = backward_in<true, false>(w, u, so1, dh0, link, n, bits, get_g, get_o, get_d);
+      if (__builtin_expect(!found.all_fast(), 0)) {
+        exact = !found.all_open(kClosed);
+        any = !exact;
+      }
+    }
+    if (exact) {
+      const Found<VEC> found = backward_in<true, true>(w, u, so1, dh0, link, n, bits, get_g, get_o, get_d);
+      if constexpr (WARPS > 1) {
+        closed = !found.all_open(kClosed + 1.0f);
+        any = !found.all_clean();
+      }
+    }
+    const auto mem_z = [&](int t) { return c.read(src + t * s.zt); };
+    const auto mem_g = [&](int t) { return c.read(src + t * s.zt + s.zk); };
+    const auto mem_o = [&](int t) { return c.read(src + t * s.zt + 2 * s.zk); };
+    const auto mem_d = [&](int t) { return c.read(dy + b * s.yb + (t0 + t) * s.yt); };
     Passing<VEC, WARPS> passing;
-    if constexpr (WARPS > 1) passing.send(ex, round, link, WARPS - 1 - warp, true);
-    if (exact) backward_states<true, true>(w, u, so1, dh0, h, bits, get_z, put_o);
-    else backward_states<true, false>(w, u, so1, dh0, h, bits, get_z, put_o);
+    if constexpr (WARPS > 1) {
+      if (__builtin_expect(any, 0)) any_backward_in<VEC>(exact, link, n, bits, mem_g, mem_o, mem_d);
+      passing.send(ex, round, link, WARPS - 1 - warp, true);
+    }
+    Found<VEC> found = exact ? backward_states<true, true>(w, u, so1, dh0, h, bits, get_z, put_o)
+                             : backward_states<true, false>(w, u, so1, dh0, h, bits, get_z, put_o);
     Vec<VEC> e = carry;
-    if constexpr (WARPS > 1) e = passing.take(ex, round, WARPS - 1 - warp, true, carry, status);
-    if (exact) backward_out<true, true>(w, u, dh0, e, bits, put_z, put_g);
-    else backward_out<true, false>(w, u, dh0, e, bits, put_z, put_g);
+    if constexpr (WARPS > 1) {
+      e = passing.take(ex, round, WARPS - 1 - warp, true, carry, status);
+      any = any || !__all_sync(0xffffffffu, found.clean() && moderate(h) && moderate(e));
+    }
+    if (!any) {
+      if (!exact) {
+        backward_out<true, false>(w, u, dh0, e, bits, put_z, put_g);
+      } else {
+        const Found<VEC> last = backward_out<true, true>(w, u, dh0, e, bits, put_z, put_g);
+        if (WARPS == 1 && !__all_sync(0xffffffffu, found.clean() && last.clean())) any = true, e = carry;
+      }
+    }
+    if (__builtin_expect(any, 0)) any_backward<VEC>(exact, h, e, n, bits, mem_z, mem_g, mem_o, mem_d, put_z, put_g, put_o);
     if constexpr (WARPS == 1) carry = e;
   }
   if (rank == 0 && warp == 0 && d_state_in != nullptr) c.put(d_state_in + (long long)b * s.dim, carry);
@@ -657,8 +872,20 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     Vec<2> w[STEPS], so[kAhead];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
     bool exact = closed || !whole;
-    if (!exact) exact = !all_above(forward_in<false, false>(w, link, n, bits, z, g), kClosed);
-    if (exact && n > 0) closed = !all_above(forward_in<true, true>(w, link, n, bits, z, g), kClosed + 1.0f);
+    bool any = false;
+    if (!exact) {
+      const Found<2> found = forward_in<false, false>(w, link, n, bits, z, g);
+      if (__builtin_expect(!found.all_fast(), 0)) {
+        exact = !found.all_open(kClosed);
+        any = !exact;
+      }
+    }
+    if (__builtin_expect(exact && n > 0, 0)) {
+      const Found<2> found = forward_in<true, true>(w, link, n, bits, z, g);
+      closed = !found.all_open(kClosed + 1.0f);
+      any = !found.all_clean();
+    }
+    if (__builtin_expect(any, 0)) any_forward_in<2>(exact, link, n, bits, z, g);
     Passing<2, kWarps> passing;
     passing.send(sm.ex, round, link, warp, false);
     // Results go over the output gates that they come from.  The ones of the step before take a while to leave the other buffer,
@@ -675,7 +902,8 @@ recurrence_fwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     Vec<2> h = passing.take(sm.ex, round, warp, false, carry, status);
     if (n <= 0) continue;
     float* at = saved != nullptr && in ? saved + ((long long)b * s.states + t0 / kSaved) * s.dim + ch : nullptr;
-    if (exact) forward_out<true, true>(w, so, h, at, s.dim, n, bits, z, o, put);
+    if (any || !__all_sync(0xffffffffu, moderate(h))) any_forward_out<2>(exact, h, at, s.dim, n, bits, z, g, o, put);
+    else if (exact) forward_out<true, true>(w, so, h, at, s.dim, n, bits, z, o, put);
     else forward_out<false, false>(w, so, h, at, s.dim, n, bits, z, o, put);
     if (in && t0 + STEPS >= s.steps) store(state_out + (long long)b * s.dim + ch, h);
     fence_proxy_async_smem();
@@ -761,21 +989,40 @@ recurrence_bwd_tma_kernel(const __grid_constant__ CUtensorMap map_in, const __gr
     Vec<2> w[STEPS], u[STEPS], so1[STEPS], dh0[STEPS];
     Link<2> link{Vec<2>::all(1.0f), Vec<2>::all(0.0f)};
     bool exact = closed || !whole;
-    if (!exact) exact = !all_above(backward_in<false, false>(w, u, so1, dh0, link, n, bits, g, o, d), kClosed);
-    if (exact && n > 0) closed = !all_above(backward_in<true, true>(w, u, so1, dh0, link, n, bits, g, o, d), kClosed + 1.0f);
+    bool any = false;
+    if (!exact) {
+      const Found<2> found = backward_in<false, false>(w, u, so1, dh0, link, n, bits, g, o, d);
+      if (__builtin_expect(!found.all_fast(), 0)) {
+        exact = !found.all_open(kClosed);
+        any = !exact;
+      }
+    }
+    if (__builtin_expect(exact && n > 0, 0)) {
+      const Found<2> found = backward_in<true, true>(w, u, so1, dh0, link, n, bits, g, o, d);
+      closed = !found.all_open(kClosed + 1.0f);
+      any = !found.all_clean();
+    }
+    if (__builtin_expect(any, 0)) any_backward_in<2>(exact, link, n, bits, g, o, d);
     Passing<2, kWarps> passing;
     passing.send(sm.ex, round, link, kWarps - 1 - warp, true);
     const Vec<2> h = load<2>(&sm.states[warp][stage][2 * lane]);
-    if (!exact) backward_states<false, false>(w, u, so1, dh0, h, bits, z, put_o);
-    else if (n > 0) backward_states<true, true>(w, u, so1, dh0, h, bits, z, put_o);
+    Found<2> found;
+    if (!exact) found = backward_states<false, false>(w, u, so1, dh0, h, bits, z, put_o);
+    else if (n > 0) found = backward_states<true, true>(w, u, so1, dh0, h, bits, z, put_o);
+    const bool ok = found.clean() && moderate(h);
     Vec<2> e = passing.take(sm.ex, round, kWarps - 1 - warp, true, carry, status);
     if (n <= 0) continue;
     if (lane == 0) bulk_wait_group_read<0>();               // the results of the step before have left
     __syncwarp();
+    any = any || !__all_sync(0xffffffffu, !in || (ok && moderate(e)));
+    if (any) {
+      any_backward<2>(exact, h, e, n, bits, z, g, o, d, put_z, put_g, [&](int t, Vec<2> v) { store(result + (3 * t + 2) * kSlab, v); });
+    } else {
 #pragma unroll
-    for (int t = 0; t < STEPS; ++t) *reinterpret_cast<elem2_t*>(result + (3 * t + 2) * kSlab) = dout[t];
-    if (exact) backward_out<true, true>(w, u, dh0, e, bits, put_z, put_g);
-    else backward_out<false, false>(w, u, dh0, e, bits, put_z, put_g);
+      for (int t = 0; t < STEPS; ++t) *reinterpret_cast<elem2_t*>(result + (3 * t + 2) * kSlab) = dout[t];
+      if (exact) backward_out<true, true>(w, u, dh0, e, bits, put_z, put_g);
+      else backward_out<false, false>(w, u, dh0, e, bits, put_z, put_g);
+    }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {

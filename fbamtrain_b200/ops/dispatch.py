@@ -252,7 +252,10 @@ def gated_recurrence(zgo, state=None, resets=None):
     """``zgo`` ``(B, T, 3, D)``: candidates ``z``, gates ``g`` and output gates ``o`` of whole sequences (or of one step).
     ``h_t = σ(g) h_{t-1} + (1 - σ(g)) z``, ``y = σ(o) h``.  ``state`` ``(B, D)`` fp32 is the ``h`` before the first step
     (zeros by default); where ``resets`` ``(B, T)`` bool is set, a step starts a new sequence and drops ``h_{t-1}``.
-    Returns ``(y (B, T, D), state (B, D) fp32)``; sequences may be time-major views, which ``y`` then is too."""
+    Returns ``(y (B, T, D), state (B, D) fp32)``; sequences may be time-major views, which ``y`` then is too.
+
+    An infinite candidate or state makes the state infinite until a reset, however small a share of it a finite gate keeps;
+    infinities of both signs, and NaN, make it NaN until then.  The same holds backwards for gradients."""
     if zgo.dim() != 4 or zgo.shape[2] != 3 or zgo.shape[3] == 0:
         raise ValueError(f"the projections are (batch, steps, 3, width), got {tuple(zgo.shape)}")
     b, t, _, d = zgo.shape

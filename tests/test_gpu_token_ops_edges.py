@@ -395,9 +395,10 @@ RECURRENCE = [(2, 1, 64), (3, 5, 40), (2, 8, 33), (2, 128, 64), (1, 129, 130), (
               (3, 700, 1024), (2, 900, 1416), (1, 2500, 65), (93, 200, 64)]
 
 
-@pytest.mark.parametrize("b,t,d", RECURRENCE)
+# (the oracle of a long one takes seconds: one of the extras each)
+@pytest.mark.parametrize("b,t,d,extras", [(*s, e) for i, s in enumerate(RECURRENCE) for j, e in enumerate(["", "state", "state resets"])
+                                          if s[1] < 500 or (i + j) % 3 == 0])
 @pytest.mark.parametrize("kind", ["long", "short", "closed"])
-@pytest.mark.parametrize("extras", ["", "state", "state resets"])
 def test_recurrence_values_and_gradients(b, t, d, kind, extras):
     """Each value against its own bound."""
     dtype = HALF if extras == "state" else BF
@@ -408,7 +409,7 @@ def test_recurrence_values_and_gradients(b, t, d, kind, extras):
             oracle.within(got, want[name], F32 if name in ("last", "d_state") else dtype, bound[name])
 
 
-@pytest.mark.parametrize("b,t,d", [(2, 128, 64), (1, 1025, 72), (1, 4100, 64), (3, 700, 1024)])
+@pytest.mark.parametrize("b,t,d", [(2, 128, 64), (1, 1025, 72), (3, 700, 1024)])
 def test_recurrence_bounds_see_what_is_missing(b, t, d):
     """A gradient of zeros is outside the bounds nearly everywhere, and one that lost what is handed on in front of any chunk is
     outside in the steps before."""
@@ -420,3 +421,47 @@ def test_recurrence_bounds_see_what_is_missing(b, t, d):
         wrong, _ = _scan_bounds(*case, drop=drop)
         over = (wrong["d_zgo"] - want["d_zgo"]).abs() > allowed
         assert bool(over[:, drop - 1, 0].any())
+
+
+def _oracle_equal(got, want, dtype, finite_slack):
+    """Infinities and NaN in the same places, what is finite within the type's rounding and a share of its row's size."""
+    oracle.within(got, want, dtype, finite_slack * want.abs().nan_to_num(0.0, 0.0, 0.0) + finite_slack)
+
+
+@pytest.mark.parametrize("b,t,d", [(2, 1, 64), (3, 7, 33), (2, 40, 64), (2, 300, 65), (1, 1500, 72), (1, 700, 1030), (1, 3000, 64)])
+@pytest.mark.parametrize("where", ["z", "state", "z and state", "dy", "d_state", "all"])
+@pytest.mark.parametrize("resets", [False, True])
+def test_recurrence_infinities(b, t, d, where, resets):
+    """An infinite candidate or state is what the definition makes of it: f inf + (1 - f) z is infinite until a reset, and of
+    both signs together NaN; the same for gradients."""
+    gen = _gen("infinities", b, t, d, where, resets)
+    zgo = _randn(gen, b, t, 3, d, dtype=BF)
+    zgo[:, :, 1] = zgo[:, :, 1] * 2 - 1                      # closed often: products of gates fall below the smallest number
+    zgo[:, :, 1, : d // 2] += 4
+    state, dy, d_state = _randn(gen, b, d), _randn(gen, b, t, d, dtype=BF), _randn(gen, b, d)
+    marks = torch.rand(b, t, generator=gen, device="cuda") < 0.01 if resets else None
+
+    def some(shape, share):
+        sign = torch.where(torch.rand(shape, generator=gen, device="cuda") < 0.5, -INF, INF)
+        return torch.rand(shape, generator=gen, device="cuda") < share, sign
+
+    if "z" in where or where == "all":
+        at, sign = some((b, t, d), 0.6 / t)
+        zgo[:, :, 0] = torch.where(at, sign.to(BF), zgo[:, :, 0])
+    if where in ("state", "z and state", "all"):
+        at, sign = some((b, d), 0.3)
+        state = torch.where(at, sign, state)
+    if where in ("dy", "all"):
+        at, sign = some((b, t, d), 0.6 / t)
+        dy = torch.where(at, sign.to(BF), dy)
+    if where in ("d_state", "all"):
+        at, sign = some((b, d), 0.3)
+        d_state = torch.where(at, sign, d_state)
+    got = _recurrence_run(zgo, state, marks, dy, d_state)
+    want_y, want_last, _, _ = oracle.recurrence(zgo, state, marks)
+    want_zgo, want_state = oracle.recurrence_grad(zgo, state, marks, dy, d_state)
+    # what is finite: 64 units of the largest value of each, over memories of up to some hundred steps
+    _oracle_equal(got["y"], want_y, BF, 1e-3)
+    _oracle_equal(got["last"], want_last, F32, 1e-3)
+    _oracle_equal(got["d_zgo"], want_zgo, BF, 1e-2)
+    _oracle_equal(got["d_state"], want_state, F32, 1e-2)
