@@ -59,12 +59,14 @@ __device__ __forceinline__ void act_and_grad2(float2 g, int act, float2& a, floa
     a = __fmul2_rn(g, cdf);
     da = __ffma2_rn(__fmul2_rn(g, gelu_math::f2(0.3989422804014327f)), e, cdf);
   } else {
+    // 1 - s = e s, to its last bits however large g is; e stays finite for its product with 0
     const float2 x = __fmul2_rn(g, gelu_math::f2(-1.4426950408889634f));
-    const float2 d = __fadd2_rn(make_float2(gelu_math::ex2_approx(x.x), gelu_math::ex2_approx(x.y)), gelu_math::f2(1.0f));
+    const float2 e = make_float2(gelu_math::ex2_approx(fminf(x.x, 126.0f)), gelu_math::ex2_approx(fminf(x.y, 126.0f)));
+    const float2 d = __fadd2_rn(e, gelu_math::f2(1.0f));
     const float2 s = make_float2(gelu_math::rcp_approx(d.x), gelu_math::rcp_approx(d.y));
     a = __fmul2_rn(g, s);
     // s + a (1 - s)
-    da = __ffma2_rn(__fmul2_rn(a, gelu_math::f2(-1.0f)), s, __fadd2_rn(s, a));
+    da = __ffma2_rn(a, __fmul2_rn(e, s), s);
   }
 }
 

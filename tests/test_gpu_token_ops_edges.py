@@ -465,3 +465,27 @@ def test_recurrence_infinities(b, t, d, where, resets):
     _oracle_equal(got["last"], want_last, F32, 1e-3)
     _oracle_equal(got["d_zgo"], want_zgo, BF, 1e-2)
     _oracle_equal(got["d_state"], want_state, F32, 1e-2)
+
+
+@pytest.mark.parametrize("dtype", [BF, HALF])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_gated_mlp_gradients_of_large_gates(act, dtype):
+    """Far out the activation's derivative is 1 or 0.  Gates from rows of the identity, values of 1: no sum has a second term, so
+    each gradient is a product of a few factors of 8 units each, and roundings of the type."""
+    far = [300.0, 3e3, 3e4, 6e4] + ([1e8, 3e30] if dtype == BF else [5e4, 100.0]) + [20.0, 8.0]
+    gates = torch.tensor(far + [-g for g in far] + [0.0, -0.0] + [3.0, -3.0] * 7, device="cuda").repeat(2)
+    x = torch.eye(64, device="cuda").to(dtype)
+    w_in = torch.zeros(128, 64, device="cuda")
+    w_in[:64].fill_diagonal_(1.0)
+    w_in[64:] = torch.diag(gates)
+    w_in, w_out, dy = w_in.to(dtype).requires_grad_(), torch.eye(64, device="cuda").to(dtype), torch.eye(64, device="cuda").to(dtype)
+    b_in = torch.zeros(128, dtype=dtype, device="cuda").requires_grad_()
+    y = ops.gated_mlp(x, w_in, w_out, b_in, None, act)
+    d_w, d_b = torch.autograd.grad((y,), (w_in, b_in), (dy,))
+    with torch.no_grad():
+        want, size = oracle.mlp(x, w_in, w_out, b_in, None, act, None, dy)
+    unit = oracle.UNIT[dtype]
+    # erf is approximated to 1.5e-7; the gates at which that shows are some units of 1
+    slack = 1e-6
+    oracle.within(d_w, want["w_in"], dtype, (1.01 * unit + 64 * 2.0 ** -24) * size["w_in"] + slack)
+    oracle.within(d_b, want["b_in"], dtype, (1.01 * unit + 64 * 2.0 ** -24) * size["b_in"] + slack)
