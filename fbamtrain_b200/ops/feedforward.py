@@ -119,7 +119,8 @@ def _slabs(like, splits, m, n):
 class _GatedMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, act, residual):
-        y, x2, w1, w2, vg, h = _forward(x, w_in, w_out, b_in, b_out, act, residual, True)
+        need_x, need_in, _, need_bin = ctx.needs_input_grad[:4]
+        y, x2, w1, w2, vg, h = _forward(x, w_in, w_out, b_in, b_out, act, residual, need_x or need_in or need_bin)
         # the inputs themselves are what a derivative of the gradients would be of: no memory where their rows are taken as they are
         ctx.save_for_backward(x2, w1, w2, vg, h, x, w_in, w_out, b_in)
         ctx.meta = (x.shape, w_out.shape[1], act)
@@ -156,10 +157,10 @@ class _GatedMlp(torch.autograd.Function):
         if need_bout:
             db_out = h.new_empty(_up8(dim))
             parts = _sum_partials("fbam_colsum_partials", rows, _up8(dim), 0)
-            work = vg.new_empty(parts * _up8(dim)) if parts else None
-        v = vg.data_ptr()
+            work = h.new_empty(parts * _up8(dim), dtype=F32) if parts else None
+        v = nv.addr(vg)
         _launch(apart, "fbam_gated_block_bwd", h, dy2.data_ptr(), dy2.shape[1], x2.data_ptr(), depth, w1.data_ptr(), depth, w2.data_ptr(), wide,
-                v, v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
+                v, v and v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
                 nv.addr(dw_out), nv.addr(db_out), nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0,
                 nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, depth, dim, act,
                 PAIRS[native_ops.TWO_CTA], nv.status_word(h.device).data_ptr(), nv.stream())

@@ -489,3 +489,21 @@ def test_gated_mlp_gradients_of_large_gates(act, dtype):
     slack = 1e-6
     oracle.within(d_w, want["w_in"], dtype, (1.01 * unit + 64 * 2.0 ** -24) * size["w_in"] + slack)
     oracle.within(d_b, want["b_in"], dtype, (1.01 * unit + 64 * 2.0 ** -24) * size["b_in"] + slack)
+
+
+@pytest.mark.parametrize("needs,kept", [(("w_out", "b_out", "residual"), False), (("x",), True), (("w_in",), True), (("b_in",), True)])
+@pytest.mark.parametrize("rows", [20, 300])
+def test_gated_mlp_keeps_its_factors_where_they_are_needed(needs, kept, rows):
+    """The fp32 factors, 8 bytes a hidden value, are for the gradients in front of the gating only."""
+    gen = _gen("kept")
+    named = {"x": _randn(gen, rows, 44, dtype=BF), "w_in": _randn(gen, 2 * 30, 44, dtype=BF, scale=0.1),
+             "w_out": _randn(gen, 20, 30, dtype=BF, scale=0.1), "b_in": _randn(gen, 60, dtype=BF), "b_out": _randn(gen, 20, dtype=BF),
+             "residual": _randn(gen, rows, 20, dtype=BF)}
+    dy = _randn(gen, rows, 20, dtype=BF)
+    want, size = oracle.mlp(*(named[k] for k in ("x", "w_in", "w_out", "b_in", "b_out")), "gelu", named["residual"], dy)
+    for k in needs:
+        named[k].requires_grad_()
+    y = ops.gated_mlp(**named)
+    assert any(t is not None and t.dtype == F32 for t in y.grad_fn.saved_tensors) == kept
+    for k, g in zip(needs, torch.autograd.grad((y,), [named[k] for k in needs], (dy,))):
+        oracle.within(g, want[k], BF, (1.01 * 2.0 ** -8 + 1e-4) * size[k] + 1e-6)
