@@ -1086,7 +1086,7 @@ int launch(size_t smem, const Shape& s, cudaStream_t stream, Args... args) {
   constexpr size_t cta_links = 2 * 32 * sizeof(Link<VEC>);
   static std::atomic<int> held[kMaxCtas + 1];               // clusters of each size that the machine holds at once
   const long long units = (long long)((s.dim + 32 * VEC - 1) / (32 * VEC)) * s.batch;
-  if (units * kMaxCtas > 0x7fffffffll) return GEMM_ERR_SHAPE;
+  if (units * (WARPS > 1 ? kMaxCtas : 1) > 0x7fffffffll) return GEMM_ERR_SHAPE;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   cudaLaunchConfig_t cfg = {};

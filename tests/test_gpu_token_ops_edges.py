@@ -507,3 +507,16 @@ def test_gated_mlp_keeps_its_factors_where_they_are_needed(needs, kept, rows):
     assert any(t is not None and t.dtype == F32 for t in y.grad_fn.saved_tensors) == kept
     for k, g in zip(needs, torch.autograd.grad((y,), [named[k] for k in needs], (dy,))):
         oracle.within(g, want[k], BF, (1.01 * 2.0 ** -8 + 1e-4) * size[k] + 1e-6)
+
+
+def test_recurrence_of_more_sequences_than_clusters_of_sixteen_could_have():
+    b = 140_000_000
+    gen = _gen("very many")
+    zgo = torch.zeros(b, 1, 3, 1, dtype=BF, device="cuda")
+    tail = _randn(gen, 100, 1, 3, 1, dtype=BF)
+    zgo[-100:] = tail
+    y, last = ops.gated_recurrence(zgo)
+    want_y, want_last, _, _ = oracle.recurrence(tail, None, None)
+    oracle.within(y[-100:], want_y, BF, 1e-5)
+    oracle.within(last[-100:], want_last, F32, 1e-5)
+    assert not y[:-100].any()
