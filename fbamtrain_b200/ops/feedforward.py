@@ -27,27 +27,30 @@ FEW_ROWS = 32
 PAIRS = {"auto": -1, False: 0, True: 1}
 
 
-def _apart() -> bool:
+def _watched() -> bool:
+    """Whether a switch is on that looks at launches or at fresh memory."""
+    return debug.PROFILE_LABELS or debug.SYNC_EVERY_OP or debug.POISON_ALLOC or debug.DEBUG_KERNEL_LAUNCH
+
+
+def _apart(watched: bool) -> bool:
     """Whether the plain products are made one by one through ``gemm``: with a table of tuned tiles, and where a switch that it
     honours is not as usual."""
-    return (tuning.active() or native_ops.TWO_CTA != "auto" or not native_ops.USE_MN_MAJOR or debug.PROFILE_LABELS or debug.SYNC_EVERY_OP
-            or debug.POISON_ALLOC or debug.DEBUG_KERNEL_LAUNCH)
+    return watched or native_ops.TWO_CTA != "auto" or not native_ops.USE_MN_MAJOR or tuning.active()
 
 
-def _launch(apart: bool, entry: str, like: torch.Tensor, *args) -> None:
-    if not apart:
+def _launch(watched: bool, entry: str, like: torch.Tensor, args: tuple) -> None:
+    if watched:
+        with debug.label(lambda: f"{entry[5:]} of {tuple(like.shape)}"):
+            code = getattr(nv.lib(like), entry)(*args)
+        nv.check(code, entry)
+        debug.after_launch(entry[5:], like)
+    else:
         nv.check(getattr(nv.lib(like), entry)(*args), entry)
-        return
-    with debug.label(lambda: f"{entry[5:]} of {tuple(like.shape)}"):
-        code = getattr(nv.lib(like), entry)(*args)
-    nv.check(code, entry)
-    debug.after_launch(entry[5:], like)
 
 
-def _fresh(like: torch.Tensor, *shape: int, dtype=None) -> torch.Tensor:
-    if debug.POISON_ALLOC:
-        return debug.fresh(shape, dtype or like.dtype, like.device)
-    return like.new_empty(shape, dtype=dtype or like.dtype)
+def _fresh(like: torch.Tensor, shape: tuple, dtype=None) -> torch.Tensor:
+    """``new_empty`` that honours the poison switch."""
+    return debug.fresh(shape, dtype or like.dtype, like.device)
 
 
 def _up8(n: int) -> int:
@@ -90,21 +93,24 @@ def _forward(x, w_in, w_out, b_in, b_out, act, residual, keep):
     b_in = None if b_in is None else _dense(b_in)
     b_out = None if b_out is None else _dense(b_out)
     res2 = None if residual is None else _flat(residual)
-    h = _fresh(x2, rows, wide)
-    apart = _apart()
+    watched = _watched()
+    h = _fresh(x2, (rows, wide)) if watched else x2.new_empty((rows, wide))
     product = False                        # the second product was made, and counted, by `gemm`
     if not keep and rows <= FEW_ROWS:
-        y, vg = _fresh(x2, rows, dim), None
-        _launch(apart, "fbam_gated_few_rows", x2, x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide,
-                nv.addr(b_out), nv.addr(res2), dim, h.data_ptr(), y.data_ptr(), rows, depth, wide, dim, act, nv.stream())
+        y, vg = _fresh(x2, (rows, dim)) if watched else x2.new_empty((rows, dim)), None
+        _launch(watched, "fbam_gated_few_rows", x2,
+                (x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide, nv.addr(b_out), nv.addr(res2), dim,
+                 h.data_ptr(), y.data_ptr(), rows, depth, wide, dim, act, nv.stream()))
     else:
-        vg = _fresh(x2, 2, rows, wide, dtype=F32) if keep else None
+        apart = _apart(watched)
+        vg = (_fresh(x2, (2, rows, wide), F32) if watched else x2.new_empty((2, rows, wide), dtype=F32)) if keep else None
         v = vg.data_ptr() if keep else 0
         product = apart
         y = None if apart else x2.new_empty((rows, dim))
-        _launch(apart, "fbam_gated_block_fwd", x2, x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide,
-                nv.addr(b_out), nv.addr(res2), h.data_ptr(), v, v + 4 * rows * wide if keep else 0, nv.addr(y), rows, wide, depth, dim, act,
-                PAIRS[native_ops.TWO_CTA], nv.status_word(x2.device).data_ptr(), nv.stream())
+        _launch(watched, "fbam_gated_block_fwd", x2,
+                (x2.data_ptr(), depth, w1.data_ptr(), depth, nv.addr(b_in), w2.data_ptr(), wide, nv.addr(b_out), nv.addr(res2),
+                 h.data_ptr(), v, v + 4 * rows * wide if keep else 0, nv.addr(y), rows, wide, depth, dim, act, PAIRS[native_ops.TWO_CTA],
+                 nv.status_word(x2.device).data_ptr(), nv.stream()))
         if apart:
             y = gemm(h, w2, bias=b_out, residual=res2)
     flops.add(2.0 * rows * inner * (2 * x.shape[-1] + (0 if product else dim)))
@@ -121,8 +127,11 @@ class _GatedMlp(torch.autograd.Function):
     def forward(ctx, x, w_in, w_out, b_in, b_out, act, residual):
         need_x, need_in, _, need_bin = ctx.needs_input_grad[:4]
         y, x2, w1, w2, vg, h = _forward(x, w_in, w_out, b_in, b_out, act, residual, need_x or need_in or need_bin)
-        # the inputs themselves are what a derivative of the gradients would be of: no memory where their rows are taken as they are
-        ctx.save_for_backward(x2, w1, w2, vg, h, x, w_in, w_out, b_in)
+        # what else the gradients depend on in the graph, for `first_only`: inputs whose rows were not taken as they are
+        others = [t for t, rows in ((x, x2), (w_in, w1), (w_out, w2)) if t is not rows]
+        if b_in is not None:
+            others.append(b_in)
+        ctx.save_for_backward(x2, w1, w2, vg, h, *others)
         ctx.meta = (x.shape, w_out.shape[1], act)
         return y
 
@@ -139,9 +148,10 @@ class _GatedMlp(torch.autograd.Function):
             dy2 = _refit(dy2, 1, rows, _up8(dim))
         dx = dw_in = dw_out = db_in = db_out = d_vg = sums = work = slabs_in = slabs_out = None
         splits_in = splits_out = 0
-        apart = _apart()
+        watched = _watched()
+        apart = _apart(watched)
         if need_x or need_in or need_bin:
-            d_vg = _fresh(h, rows, 2 * wide)
+            d_vg = _fresh(h, (rows, 2 * wide)) if watched else h.new_empty((rows, 2 * wide))
             if need_bin:
                 db_in, sums = h.new_empty(2 * wide), vg.new_empty(((rows + 31) // 32, 2 * wide))
             if need_x:
@@ -159,11 +169,12 @@ class _GatedMlp(torch.autograd.Function):
             parts = _sum_partials("fbam_colsum_partials", rows, _up8(dim), 0)
             work = h.new_empty(parts * _up8(dim), dtype=F32) if parts else None
         v = nv.addr(vg)
-        _launch(apart, "fbam_gated_block_bwd", h, dy2.data_ptr(), dy2.shape[1], x2.data_ptr(), depth, w1.data_ptr(), depth, w2.data_ptr(), wide,
-                v, v and v + 4 * rows * wide, h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in),
-                nv.addr(dw_out), nv.addr(db_out), nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0,
-                nv.addr(slabs_out), splits_out if slabs_out is not None else 0, rows, wide, depth, dim, act,
-                PAIRS[native_ops.TWO_CTA], nv.status_word(h.device).data_ptr(), nv.stream())
+        _launch(watched, "fbam_gated_block_bwd", h,
+                (dy2.data_ptr(), dy2.shape[1], x2.data_ptr(), depth, w1.data_ptr(), depth, w2.data_ptr(), wide, v, v and v + 4 * rows * wide,
+                 h.data_ptr(), nv.addr(d_vg), nv.addr(sums), nv.addr(db_in), nv.addr(dx), nv.addr(dw_in), nv.addr(dw_out), nv.addr(db_out),
+                 nv.addr(work), nv.addr(slabs_in), splits_in if slabs_in is not None else 0, nv.addr(slabs_out),
+                 splits_out if slabs_out is not None else 0, rows, wide, depth, dim, act, PAIRS[native_ops.TWO_CTA],
+                 nv.status_word(h.device).data_ptr(), nv.stream()))
         flops.add(2.0 * rows * inner * (dim * ((d_vg is not None) + (dw_out is not None)) + 2 * width * ((dx is not None) + (dw_in is not None))))
         if apart:
             splits = weight_grad_splits if native_ops.USE_MN_MAJOR else (lambda *sizes: 0)

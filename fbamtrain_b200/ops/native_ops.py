@@ -36,7 +36,7 @@ def _need_elem(*ts) -> torch.dtype:
     """All given tensors must share one 16-bit element type (bf16 or half) and one device; returns the type."""
     dtype = device = None
     for t in ts:
-        if t is None:
+        if t is None or (t.dtype == dtype and t.device == device):
             continue
         if t.dtype not in nv.ELEM_DTYPES:
             raise TypeError(f"native kernels take bf16 or fp16 tensors, got {t.dtype}")
