@@ -32,8 +32,9 @@ class _First(torch.autograd.Function):
 
 
 def first_only(name: str):
-    """For a ``backward`` whose gradients depend on the saved tensors and the gradients that come in: with ``create_graph`` they
-    depend on those in the graph too, and a derivative of them raises."""
+    """For a ``backward`` whose gradients depend on the saved tensors, on ``ctx.linked`` (inputs that it does not read itself, so
+    that they may be overwritten) and the gradients that come in: with ``create_graph`` they depend on those in the graph too,
+    and a derivative of them raises."""
     def decorate(backward):
         @functools.wraps(backward)
         def run(ctx, *grads):
@@ -41,7 +42,7 @@ def first_only(name: str):
                 return backward(ctx, *grads)
             with torch.no_grad():
                 out = backward(ctx, *grads)
-            of = [t for t in (*ctx.saved_tensors, *grads) if t is not None]
+            of = [t for t in (*ctx.saved_tensors, *ctx.linked, *grads) if t is not None]
             return tuple(None if g is None else _First.apply(name, g, *of) for g in out)
         return run
     return decorate

@@ -30,6 +30,7 @@ class _EmbedTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, flat, table, scale, out_dtype, elem):
         ctx.save_for_backward(flat)
+        ctx.linked = ()
         ctx.meta = (*table.shape, table.dtype, elem, scale)
         return _forward(ids, flat, table, scale, out_dtype, elem)
 

@@ -127,18 +127,15 @@ class _GatedMlp(torch.autograd.Function):
     def forward(ctx, x, w_in, w_out, b_in, b_out, act, residual):
         need_x, need_in, _, need_bin = ctx.needs_input_grad[:4]
         y, x2, w1, w2, vg, h = _forward(x, w_in, w_out, b_in, b_out, act, residual, need_x or need_in or need_bin)
-        # what else the gradients depend on in the graph, for `first_only`: inputs whose rows were not taken as they are
-        others = [t for t, rows in ((x, x2), (w_in, w1), (w_out, w2)) if t is not rows]
-        if b_in is not None:
-            others.append(b_in)
-        ctx.save_for_backward(x2, w1, w2, vg, h, *others)
+        ctx.save_for_backward(x2, w1, w2, vg, h)
+        ctx.linked = [t for t, rows in ((x, x2), (w_in, w1), (w_out, w2), (b_in, None)) if t is not rows and t.requires_grad]
         ctx.meta = (x.shape, w_out.shape[1], act)
         return y
 
     @staticmethod
     @first_only("gated_mlp")
     def backward(ctx, dy):
-        x2, w1, w2, vg, h = ctx.saved_tensors[:5]
+        x2, w1, w2, vg, h = ctx.saved_tensors
         shape, inner, act = ctx.meta
         need_x, need_in, need_out, need_bin, need_bout, _, need_res = ctx.needs_input_grad
         rows, wide = h.shape

@@ -36,6 +36,7 @@ class _TokenLogprobs(torch.autograd.Function):
         if top:
             ctx.mark_non_differentiable(top_lp, top_ids)
         ctx.save_for_backward(logits, targets, stats, entropy)
+        ctx.linked = ()
         ctx.inv_t = inv_t
         return logprob, entropy, top_lp, top_ids
 

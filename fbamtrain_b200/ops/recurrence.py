@@ -48,13 +48,14 @@ class _GatedRecurrence(torch.autograd.Function):
     def forward(ctx, zgo, state, resets):
         ctx.set_materialize_grads(False)
         y, out, saved = _forward(zgo, state, resets, True)
-        ctx.save_for_backward(zgo, resets, saved, state)
+        ctx.save_for_backward(zgo, resets, saved)
+        ctx.linked = (state,)
         return y, out
 
     @staticmethod
     @first_only("gated_recurrence")
     def backward(ctx, dy, d_out):
-        zgo, resets, saved, _ = ctx.saved_tensors
+        zgo, resets, saved = ctx.saved_tensors
         b, t, _, d = zgo.shape
         dev = zgo.device
         if dy is None:

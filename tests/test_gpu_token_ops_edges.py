@@ -228,6 +228,21 @@ def test_a_tangent_is_refused(name, grad):
         assert torch.equal(call(x), plain)
 
 
+@pytest.mark.parametrize("shape", [(40, 32, 48, 24), (40, 30, 50, 21)])
+@pytest.mark.parametrize("name", ["x", "w_in", "w_out", "b_in"])
+def test_a_second_derivative_of_the_block_is_refused(name, shape):
+    gen = _gen("second", shape)
+    rows, width, inner, out = shape
+    named = {"x": _randn(gen, 5, rows // 5, width, dtype=BF), "w_in": _randn(gen, 2 * inner, width, dtype=BF),
+             "w_out": _randn(gen, out, inner, dtype=BF), "b_in": _randn(gen, 2 * inner, dtype=BF)}
+    for v in named.values():
+        v.requires_grad_()
+    y = ops.gated_mlp(**named)
+    first, = torch.autograd.grad((y,), (named["w_in"],), (torch.ones_like(y),), create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad((first.float().sum() + named[name].float().sum(),), (named[name],))
+
+
 @pytest.mark.parametrize("name", ["embed_tokens", "gated_recurrence", "gated_mlp", "token_logprobs"])
 def test_a_second_derivative_is_refused(name):
     """Of the gradient by what it depends on: the input (but for the embedding, whose gradient does not) and the gradient that
@@ -520,3 +535,23 @@ def test_recurrence_of_more_sequences_than_clusters_of_sixteen_could_have():
     oracle.within(y[-100:], want_y, BF, 1e-5)
     oracle.within(last[-100:], want_last, F32, 1e-5)
     assert not y[:-100].any()
+
+
+def test_inputs_that_the_gradients_do_not_read_may_be_overwritten():
+    """A carried state in its place, and a bias, between the forward and the backward."""
+    gen = _gen("overwritten")
+    zgo, buffer, dy = _randn(gen, 2, 9, 3, 16, dtype=BF).requires_grad_(), _randn(gen, 2, 16), _randn(gen, 2, 9, 16, dtype=BF)
+    want, = torch.autograd.grad(ops.gated_recurrence(zgo, buffer.clone())[:1], (zgo,), (dy,))
+    y, last = ops.gated_recurrence(zgo, buffer)
+    buffer.copy_(last.detach())
+    assert torch.equal(torch.autograd.grad((y,), (zgo,), (dy,))[0], want)
+    x, w_in, w_out, b_in = _randn(gen, 40, 30, dtype=BF), _randn(gen, 20, 30, dtype=BF), _randn(gen, 24, 10, dtype=BF), _randn(gen, 20, dtype=BF)
+    w_in.requires_grad_()
+    b_in.requires_grad_()
+    dy = _randn(gen, 40, 24, dtype=BF)
+    want = torch.autograd.grad((ops.gated_mlp(x, w_in, w_out, b_in),), (w_in, b_in), (dy,))
+    y = ops.gated_mlp(x, w_in, w_out, b_in)
+    with torch.no_grad():
+        b_in.zero_()
+    for a, b in zip(torch.autograd.grad((y,), (w_in, b_in), (dy,)), want):
+        assert torch.equal(a, b)
