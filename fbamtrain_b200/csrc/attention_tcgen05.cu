@@ -23,11 +23,12 @@
 // kernel_gen/kernel_gen/kernels/flash_attention_codegen/compile.py:280-330, kernels/flash_attention_fwd.py:36-266,
 // kernels/flash_attention_bwd.py:6-313; selected in src/passes/mha_attention_pass.cpp).  The reference supports
 // head dimension 128 only; 64 is added here.
-#include "tc05.cuh"
+#include "attention_tile.cuh"
 
 namespace {
 
 using namespace tc05;
+using namespace attn;
 
 constexpr int BQ = 128;   // queries per tile (TMEM lanes)
 constexpr int BKV = 128;  // keys per block
@@ -49,21 +50,6 @@ __device__ __forceinline__ void tma_load_attn(void* dst, const CUtensorMap* map,
 }
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Arrival of a whole warp (one per warp: 32 arrivals on one barrier would be served one after the other): every lane
-// has fenced its own accesses before.
-__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-
-// Address of element (row, col8 = 8-element group index) in a [rows x 64]-bf16 panel with 128-byte swizzle.
-__device__ __forceinline__ uint32_t swz(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
 // -------------------------------------------------------------------------------------------------
 // forward
@@ -1005,14 +991,7 @@ int encode_bthd(CUtensorMap* map, const void* base, int B, int T, int H, int D, 
                 long long sh) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return 4;
-  {  // the driver entry point needs a context current on this thread (see gemm_tcgen05.h)
-    static thread_local int bound = -1;
-    int dev = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess && dev != bound) {
-      cudaSetDevice(dev);
-      bound = dev;
-    }
-  }
+  bind_context();
   if ((reinterpret_cast<uintptr_t>(base) & 15) || (sb * 2) % 16 || (st * 2) % 16 || (sh * 2) % 16) return 2;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2, (cuuint64_t)sb * 2};
@@ -1022,11 +1001,6 @@ int encode_bthd(CUtensorMap* map, const void* base, int B, int T, int H, int D, 
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : 3;
-}
-
-template <typename K>
-int set_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess ? 0 : 5;
 }
 
 }  // namespace

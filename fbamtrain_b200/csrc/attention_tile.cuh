@@ -1,0 +1,58 @@
+// What the attention kernels share: exponentials, the swizzled operand layout, arrivals of whole warps, a current context for the
+// tensor-map encoder.
+#pragma once
+#include "tc05.cuh"
+#include "tensor_map.h"
+
+namespace attn {
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Arrival of a whole warp (one per warp: 32 arrivals on one barrier would be served one after the other): every lane
+// has fenced its own accesses before.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) tc05::mbar_arrive(bar);
+}
+
+// Address of element (row, col8 = 8-element group index) in a [rows x 64]-bf16 panel with 128-byte swizzle.
+__device__ __forceinline__ uint32_t swz(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// The driver entry point needs a context current on this thread (see gemm_tcgen05.h).
+inline void bind_context() {
+  static thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != bound) {
+    cudaSetDevice(dev);
+    bound = dev;
+  }
+}
+
+// Map of an (outer, rows, heads, D) view with element strides and inner stride 1: boxes of 64 channels x `box_heads` x `box_rows`.
+inline int encode_heads(CUtensorMap* map, const void* base, int D, int heads, int rows, int outer, long long sh, long long sr, long long so,
+                        int box_heads, int box_rows) {
+  FbamEncodeTiledFn enc = fbam_encode_tiled();
+  if (!enc) return 4;
+  bind_context();
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || sh % 8 || sr % 8 || so % 8) return 2;
+  // a dimension of one entry is never stepped over, whatever stride the tensor names; the encoder wants some
+  const cuuint64_t step = (cuuint64_t)D * 2;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)outer};
+  cuuint64_t strides[3] = {heads > 1 ? (cuuint64_t)sh * 2 : step, rows > 1 ? (cuuint64_t)sr * 2 : step, outer > 1 ? (cuuint64_t)so * 2 : step};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, ELEM_TMAP, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 3;
+}
+
+template <typename K>
+int set_smem(K kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess ? 0 : 5;
+}
+
+}  // namespace attn
