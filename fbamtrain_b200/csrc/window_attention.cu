@@ -1,0 +1,623 @@
+// Causal attention that sees a sliding window and the first few tokens, over whole sequences (with its backward pass in
+// window_attention_bwd.cu) and for new tokens over a paged cache; query heads may share key heads.
+//
+// A query at position i sees key j iff j <= i and (i - j < window or j < sinks), j within the sequence.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = 2^(s_ij scale log2(e) - m_i) / l_i,  s = q k^T,  m the running maximum, l the running sum
+//
+// One thread block takes two tiles of queries of one key head.  A tile's 128 rows are TOKENS x the query heads that share the
+// key head, so a key block is read once for all of them and one token of a shared head fills as many rows as there are heads.
+// Key blocks of 128 pass through a ring in shared memory, K and V in turn; only blocks that some row of the tiles sees are
+// visited (those of the first tokens, then those of the window).  Per block and tile: S = Q K^T into tensor memory
+// (tcgen05.mma); four softmax warps, one row a thread, read S, form the exponentials and write P over S as 16-bit values; the
+// second product takes P from tensor memory and adds P V to the tile's output there, which is rescaled only when a row's
+// maximum has grown by more than 2^8.  The two tiles take turns on the tensor cores.
+//
+// Over a cache the ring is filled page by page: the lanes of the loading warp each look up one page (or part of one of 128 slots
+// or more) and issue its copy.  Entries that are no page, slots behind the sequence and pages that nothing sees are filled with
+// zeros by the copy engine (a coordinate behind the last page).  With few rows the keys are split over several thread blocks,
+// whose partial sums a second kernel joins.
+//
+// Rows of V that no query of the block sees may hold anything (slots never written): they are zeroed in shared memory, since
+// 0 x NaN is NaN in a product.
+#include "attention_tile.cuh"
+
+namespace {
+
+using namespace tc05;
+using namespace attn;
+
+constexpr int kRows = 128;       // rows of a tile (TMEM lanes)
+constexpr int kKeys = 128;       // keys of a block
+constexpr int kNoWindow = 0x3fffffff;
+enum { ATT_ERR_TIMEOUT = 501 };
+
+struct FwdParams {
+  int T;                  // dense: tokens of a sequence; paged: rows of q
+  int B, kv_heads, group, tile_tokens;
+  int window, sinks;
+  const int* lengths;     // (B); null: T everywhere
+  // paged
+  const int* offsets;     // (B + 1); null: one new token each
+  const int* tables;      // (B, max_pages)
+  long long t_sb;
+  int max_pages, page, pages, piece;
+  int splits;
+  float scale_log2;
+  elem_t* out;            // (B, T, heads, D) or (rows, heads, D), contiguous
+  float* lse;             // (B, kv_heads, T, group): log2 of the sum of 2^(s scale log2(e)); null where no gradient is wanted
+  float* part_o;          // (splits, rows, heads, D) and (splits, rows, heads): sums of a split and (reference, total)
+  float2* part_ml;
+  int* status;
+};
+
+template <int D>
+constexpr int kSlots = D == 64 ? 8 : 5;
+template <int D>
+constexpr int fwd_smem_bytes() { return 2 * kRows * D * 2 + kSlots<D> * kKeys * D * 2 + 256 + 1024; }
+
+constexpr int kFwdThreads = 320;   // MMA issue, eight softmax warps, loads
+
+// D[tmem] (+)= A[tmem] * B[smem desc]; single-thread issue.  A: 128 rows, 16-bit elements two to a column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Queries of one tile, or of both, as the kernel needs them: token numbers within the sequence's new tokens.
+struct Span {
+  int p0, p1;      // positions of the first and the last valid query; p1 < p0: none
+  int lo, hi;      // key blocks of the window (first tokens apart)
+};
+
+__device__ __forceinline__ Span make_span(int i0, int i1, int base, int key_end, int window) {
+  Span s;
+  s.p0 = max(0, base + i0);
+  s.p1 = base + i1 - 1;
+  const int end = min(s.p1 + 1, key_end);
+  if (i1 <= i0 || end <= 0) { s.p1 = s.p0 - 1; s.lo = 0; s.hi = -1; return s; }
+  s.lo = max(0, s.p0 - window + 1) / kKeys;
+  s.hi = (end - 1) / kKeys;
+  return s;
+}
+
+template <int D, bool PAGED>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
+  constexpr int DP = D / 64;                 // 64-wide panels per row
+  constexpr int kQBytes = kRows * D * 2;     // one tile
+  constexpr int kKVBytes = kKeys * D * 2;
+  constexpr int NS = kSlots<D>;
+  constexpr uint32_t kTmemCols = 512;        // S/P_A [0,128) S/P_B [128,256) O_A [256,256+D) O_B [256+D,256+2D)
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                        // two tiles
+  uint8_t* sKV = sQ + 2 * kQBytes;           // NS slots: K and V of the blocks in turn
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + NS * kKVBytes);
+  uint64_t* q_full = bars;
+  uint64_t* full = bars + 1;                 // [NS]
+  uint64_t* empty = full + NS;               // [NS]
+  uint64_t* s_full = empty + NS;             // [2]
+  uint64_t* p_ready = s_full + 2;            // [2]
+  uint64_t* pv_full = p_ready + 2;           // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_full + 2);
+  int* found = reinterpret_cast<int*>(tmem_slot + 1);   // sequence, pair
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = p.kv_heads * p.group;
+  int b, pair, kvh, split = 0;
+  if constexpr (PAGED) {
+    kvh = blockIdx.y;
+    split = blockIdx.z;
+    if (p.offsets == nullptr) {
+      b = blockIdx.x;
+      pair = 0;
+    } else {
+      // which sequence this block's pair of tiles belongs to; the rows behind the last sequence count as one more, without keys
+      if (warp == 0) {
+        int before = 0, at = -1, which = 0;
+        for (int b0 = 0; b0 <= p.B && at < 0; b0 += 32) {
+          const int i = b0 + lane;
+          int pairs = 0;
+          if (i <= p.B) {
+            const int r0 = min(max(p.offsets[i], 0), p.T), r1 = i < p.B ? min(max(p.offsets[i + 1], r0), p.T) : p.T;
+            pairs = (r1 - r0 + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+          }
+          int sum = pairs;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+          }
+          const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + sum);
+          if (hit) {
+            const int first = __ffs(hit) - 1;
+            at = b0 + first;
+            which = (int)blockIdx.x - (before + __shfl_sync(0xffffffffu, sum - pairs, first));
+          }
+          before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) { found[0] = at; found[1] = which; }
+      }
+      __syncthreads();
+      b = found[0];
+      pair = found[1];
+      if (b < 0) return;
+    }
+  } else {
+    // the last tokens of all sequences first: without a window they see the most keys
+    const int bh = blockIdx.x % (p.B * p.kv_heads);
+    b = bh / p.kv_heads;
+    kvh = bh % p.kv_heads;
+    pair = (p.T + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) - 1 - blockIdx.x / (p.B * p.kv_heads);
+  }
+  // this sequence: its rows, where its queries stand, where its keys end
+  int row0 = 0, n_rows = p.T, n_valid = p.T, base = 0, key_end;
+  if constexpr (PAGED) {
+    if (p.offsets == nullptr) {
+      row0 = b;
+      n_rows = 1;
+    } else {
+      row0 = min(max(p.offsets[b], 0), p.T);
+      n_rows = (b < p.B ? min(max(p.offsets[b + 1], row0), p.T) : p.T) - row0;
+    }
+    n_valid = n_rows;
+    const int length = b < p.B ? max(p.lengths[b], 0) : 0;
+    base = length - n_rows;
+    key_end = (int)min((long long)length, (long long)p.max_pages * p.page);
+  } else {
+    if (p.lengths != nullptr) n_valid = min(max(p.lengths[b], 0), p.T);
+    key_end = n_valid;
+  }
+  const int tok0 = pair * 2 * p.tile_tokens;
+  Span span[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    span[g] = make_span(tok0 + g * p.tile_tokens, min(tok0 + (g + 1) * p.tile_tokens, n_valid), base, key_end, p.window);
+  const Span both = make_span(tok0, min(tok0 + 2 * p.tile_tokens, n_valid), base, key_end, p.window);
+  const int near = max(0, both.p0 - p.window + 1), end = min(both.p1 + 1, key_end);       // what both tiles see together:
+  const int sink_end = min(p.sinks, end);                                                  // [0, sink_end) and [near, end)
+  const int ns = both.hi < 0 ? 0 : min((p.sinks + kKeys - 1) / kKeys, both.hi + 1);        // blocks with first tokens
+  const int range0 = max(both.lo, ns);
+  const int listed = ns + max(0, both.hi - range0 + 1);                                    // a table may end in front of the window
+  int c0 = 0, c1 = listed;
+  if (PAGED && p.splits > 1) {
+    c0 = (int)((long long)listed * split / p.splits);
+    c1 = (int)((long long)listed * (split + 1) / p.splits);
+  }
+  auto block_of = [&](int c) { return c < ns ? c : c - ns + range0; };
+  auto needed = [&](int g, int kb) { return kb <= span[g].hi && (kb < ns || kb >= span[g].lo); };
+
+  const bool partial = PAGED && p.splits > 1;
+  if (c0 >= c1) {                              // no keys: zeros, or a part that adds nothing
+    const int i1 = min(tok0 + 2 * p.tile_tokens, n_rows);
+    const int per = p.group * (D / 8);
+    for (int i = threadIdx.x; i < (i1 - tok0) * per; i += kFwdThreads) {
+      const int t = tok0 + i / per, r = i % per;
+      const long long row = (PAGED ? (long long)row0 : (long long)b * p.T) + t;
+      const long long at = row * heads + kvh * p.group + r / (D / 8);
+      if (partial) {
+        if (r % (D / 8) == 0) p.part_ml[(long long)split * p.T * heads + at] = make_float2(-INFINITY, 0.0f);
+      } else {
+        *reinterpret_cast<uint4*>(p.out + at * D + r % (D / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+    mbar_init(q_full, 1);
+    for (int s = 0; s < NS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_ready[g], 4);
+      mbar_init(&pv_full[g], 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 0) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 9) {
+    // ---------------------------------------------------------------- loads
+    bool ok = true;
+    if (lane == 0) {
+      const int tiles = span[1].hi >= 0 ? 2 : 1;
+      mbar_expect_tx(q_full, tiles * p.tile_tokens * p.group * D * 2);
+      for (int g = 0; g < tiles; ++g)
+#pragma unroll
+        for (int j = 0; j < DP; ++j)           // rows beyond the tensor are filled with zeros
+          tma_load_4d(sQ + g * kQBytes + j * kRows * 128, &map_q, q_full, j * 64, kvh * p.group, row0 + tok0 + g * p.tile_tokens,
+                      PAGED ? 0 : b);
+    }
+    // the page (or part of it) that this lane fetches of a block; the number of pages where there is nothing to fetch
+    auto look_up = [&](int kb) {
+      const int key = kb * kKeys + lane * p.piece;
+      int id = -1;
+      if (lane * p.piece < kKeys && key < end && (key < sink_end || key + p.piece > near)) {
+        const int at = key / p.page;
+        if (at < p.max_pages) id = p.tables[b * p.t_sb + at];
+      }
+      return id < 0 || id >= p.pages ? p.pages : id;
+    };
+    int next = 0;
+    if (PAGED) next = look_up(block_of(c0));
+    for (int c = c0; c < c1 && ok; ++c) {
+      const int kb = block_of(c), id = next;
+      if (PAGED && c + 1 < c1) next = look_up(block_of(c + 1));
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int f = 2 * (c - c0) + kv, s = f % NS;
+        if (f >= NS && !mbar_wait(&empty[s], (f / NS - 1) & 1)) { ok = false; break; }
+        const CUtensorMap* map = kv ? &map_v : &map_k;
+        if (lane == 0) mbar_expect_tx(&full[s], kKVBytes);
+        __syncwarp();
+        if constexpr (PAGED) {
+          if (lane * p.piece < kKeys) {
+            const int slot = (kb * kKeys + lane * p.piece) % p.page;
+#pragma unroll
+            for (int j = 0; j < DP; ++j)
+              tma_load_4d(sKV + s * kKVBytes + j * kKeys * 128 + lane * p.piece * 128, map, &full[s], j * 64, kvh, slot, id);
+          }
+        } else if (lane == 0) {
+#pragma unroll
+          for (int j = 0; j < DP; ++j) tma_load_4d(sKV + s * kKVBytes + j * kKeys * 128, map, &full[s], j * 64, kvh, kb * kKeys, b);
+        }
+      }
+    }
+    if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
+  } else if (warp == 0) {
+    // ---------------------------------------------------------------- products
+    if (elect_one()) {
+      const uint32_t idesc_s = make_idesc_f16kind(128, kKeys, false, false);
+      const uint32_t idesc_pv = make_idesc_f16kind(128, D, false, true);   // B = V is MN-major
+      auto slot_addr = [&](int f) { return smem_u32(sKV + f % NS * kKVBytes); };
+      auto wait_full = [&](int f) { return mbar_wait(&full[f % NS], (f / NS) & 1); };
+      auto issue_s = [&](int g, int f) {       // S_g = Q_g K^T
+        const uint32_t q_addr = smem_u32(sQ + g * kQBytes), k_addr = slot_addr(f);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t da = make_smem_desc_sw128(q_addr + (k / 4) * kRows * 128 + (k % 4) * 32, 16, 1024);
+          const uint64_t db = make_smem_desc_sw128(k_addr + (k / 4) * kKeys * 128 + (k % 4) * 32, 16, 1024);
+          mma_f16_ss(tmem + g * 128, da, db, idesc_s, k != 0);
+        }
+        mma_commit(&s_full[g]);
+      };
+      auto issue_pv = [&](int g, int f, bool first) {     // O_g (+)= P_g V
+        const uint32_t v_addr = slot_addr(f);
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, make_smem_desc_sw128(v_addr + k * 16 * 128, kKeys * 128, 1024), idesc_pv,
+                     !first || k != 0);
+        mma_commit(&pv_full[g]);
+      };
+      int done[2] = {0, 0};                    // blocks of each tile whose P V has been issued
+      bool ok = mbar_wait(q_full, 0) && wait_full(0);
+      if (ok) {
+        fence_after_sync();
+        const int kb = block_of(c0);
+        if (needed(0, kb)) issue_s(0, 0);
+        if (needed(1, kb)) issue_s(1, 0);
+        mma_commit(&empty[0]);
+      }
+      for (int c = c0; c < c1 && ok; ++c) {
+        const int f = 2 * (c - c0), kb = block_of(c);
+        const bool more = c + 1 < c1;
+        const int kb1 = more ? block_of(c + 1) : -1;
+        if (!wait_full(f + 1)) { ok = false; break; }
+        auto step_pv = [&](int g) {
+          if (!needed(g, kb)) return;
+          if (!mbar_wait(&p_ready[g], done[g] & 1)) { ok = false; return; }
+          fence_after_sync();
+          issue_pv(g, f + 1, done[g] == 0);
+          ++done[g];
+        };
+        step_pv(0);
+        if (!ok) break;
+        if (more) {
+          if (!wait_full(f + 2)) { ok = false; break; }
+          fence_after_sync();
+          if (needed(0, kb1)) issue_s(0, f + 2);   // S_0 of this block was read before p_ready[0] arrived
+        }
+        step_pv(1);
+        if (!ok) break;
+        mma_commit(&empty[(f + 1) % NS]);
+        if (more) {
+          if (needed(1, kb1)) issue_s(1, f + 2);
+          mma_commit(&empty[(f + 2) % NS]);
+        }
+      }
+      if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax / output threads of one tile
+    const int g = (warp - 1) >> 2;                   // tile of this warp group
+    const int lane_group = warp & 3;                 // TMEM lane quarter this warp may access
+    const int row = lane_group * 32 + lane;
+    const int token = row / p.group;
+    const int i = tok0 + g * p.tile_tokens + token;  // the row's token among the sequence's new ones
+    const int pos = base + i;
+    const bool stored = token < p.tile_tokens && i < n_rows;
+    const bool valid = stored && i < n_valid && pos >= 0;
+    const uint32_t lane_addr = uint32_t(lane_group * 32) << 16;
+    const uint32_t tmem_s = tmem + g * 128, tmem_pv = tmem + 256 + g * D;
+    const Span mine = g == 0 ? span[0] : span[1];
+    // m is the reference of the exponentials accumulated so far: p = 2^((s - m) scale).  It follows the running row maximum only
+    // when that has moved by more than 2^8 past it, so that the output accumulator is rescaled on a few blocks only (values of p
+    // stay below 2^8, far inside the 16-bit range; the final division by the row sum uses the same reference).
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    int it = 0;
+    for (int c = c0; c < c1; ++c) {
+      const int kb = block_of(c);
+      if (!needed(g, kb)) continue;
+      const int k0 = kb * kKeys;
+      if (k0 + kKeys > end || (k0 < near && k0 + kKeys > sink_end)) {
+        // rows of V that no query of this block sees
+        const int f = 2 * (c - c0) + 1;
+        if (!mbar_wait(&full[f % NS], (f / NS) & 1)) { ok = false; break; }
+        const int key = k0 + row;
+        if (key >= end || (key < near && key >= sink_end)) {
+          uint8_t* at = sKV + f % NS * kKVBytes + row * 128;
+#pragma unroll
+          for (int j = 0; j < DP * 8; ++j) *reinterpret_cast<uint4*>(at + (j / 8) * kKeys * 128 + (j % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      if (!mbar_wait(&s_full[g], it & 1)) { ok = false; break; }
+      fence_after_sync();
+      uint32_t r[kKeys];
+#pragma unroll
+      for (int j = 0; j < kKeys; j += 32) tmem_ld_32x32(tmem_s + lane_addr + j, *reinterpret_cast<uint32_t(*)[32]>(r + j));
+      tmem_ld_wait();
+      // Masking is a pass of its own that only blocks on an edge take.
+      if (k0 + kKeys > min(mine.p0 + 1, key_end) || (k0 <= mine.p1 - p.window && k0 + kKeys > p.sinks)) {
+        const int hi = min(pos + 1, key_end) - k0, lo = pos - p.window + 1 - k0, first = p.sinks - k0;
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+          if (j >= hi || (j < lo && j >= first)) r[j] = 0xff800000u;      // -inf
+      }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kKeys; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(r[j]));
+      const float m_blk = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      const bool grow = (m_blk - m) * p.scale_log2 > 8.0f;      // true on the first block of any visible key
+      float alpha = 1.0f;
+      if (grow) {
+        alpha = (m == -INFINITY) ? 0.0f : fast_exp2((m - m_blk) * p.scale_log2);
+        m = m_blk;
+      }
+      const float m_use = (m == -INFINITY) ? 0.0f : m;
+      if (it > 0 && __any_sync(0xffffffffu, grow)) {
+        // some row of this warp moved its reference: scale the accumulated output rows.  The product that adds the block before
+        // has completed (S of this block was issued after it); the wait makes that explicit and returns at once.
+        if (!mbar_wait(&pv_full[g], (it - 1) & 1)) { ok = false; break; }
+        fence_after_sync();
+        const float2 a2 = make_float2(alpha, alpha);
+#pragma unroll 1
+        for (int d0 = 0; d0 < D; d0 += 32) {
+          uint32_t ro[32];
+          tmem_ld_32x32(tmem_pv + lane_addr + d0, ro);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 v = __fmul2_rn(make_float2(__uint_as_float(ro[j]), __uint_as_float(ro[j + 1])), a2);
+            ro[j] = __float_as_uint(v.x);
+            ro[j + 1] = __float_as_uint(v.y);
+          }
+          tmem_st_32x32(tmem_pv + lane_addr + d0, ro);
+        }
+      }
+      // p = 2^(s scale - m scale): one packed multiply-add per pair, then the exponential; the row sum is taken over the fp32
+      // values.  P is rounded to 16 bits as an operand of the second product (half a step of its type, relative to values whose
+      // largest is near 1).
+      const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+      const float nm = -m_use * p.scale_log2;
+      const float2 nm2 = make_float2(nm, nm);
+      float2 rs2 = make_float2(0.0f, 0.0f), rs2b = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int at = half * 64 + 2 * j;
+          const float2 e = __ffma2_rn(make_float2(__uint_as_float(r[at]), __uint_as_float(r[at + 1])), sc2, nm2);
+          const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+          if (j & 1) rs2b = __fadd2_rn(rs2b, pe); else rs2 = __fadd2_rn(rs2, pe);
+          elem2_t h = f22e2(pe);
+          packed[j] = *reinterpret_cast<uint32_t*>(&h);
+        }
+        tmem_st_32x32(tmem_s + lane_addr + half * 32, packed);
+      }
+      l = l * alpha + ((rs2.x + rs2.y) + (rs2b.x + rs2b.y));
+      tmem_st_wait();
+      fence_before_sync();
+      warp_arrive(&p_ready[g]);
+      ++it;
+    }
+    if (ok) {
+      // the last product completes the output rows in tensor memory: divide by the row sum and store
+      if (it > 0 && !mbar_wait(&pv_full[g], (it - 1) & 1)) ok = false;
+      fence_after_sync();
+    }
+    if (ok) {
+      const long long at_row = (PAGED ? (long long)row0 : (long long)b * p.T) + i;
+      const long long at = at_row * heads + kvh * p.group + (row - token * p.group);
+      if (!valid) l = 0.0f;
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float2 inv2 = make_float2(inv, inv);
+#pragma unroll 1
+      for (int d0 = 0; d0 < D; d0 += 32) {
+        uint32_t r[32];
+        if (it > 0) {
+          tmem_ld_32x32(tmem_pv + lane_addr + d0, r);
+          tmem_ld_wait();
+        }
+        if (it == 0 || !(l > 0.0f)) {          // nothing seen
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0u;
+        }
+        if (stored) {
+          if (partial) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + ((long long)split * p.T * heads + at) * D + d0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                                   __uint_as_float(r[4 * j + 3]));
+          } else {
+#pragma unroll
+            for (int d = 0; d < 32; d += 8) {
+              __align__(16) elem2_t hh[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                hh[q] = f22e2(__fmul2_rn(make_float2(__uint_as_float(r[d + 2 * q]), __uint_as_float(r[d + 2 * q + 1])), inv2));
+              *reinterpret_cast<uint4*>(p.out + at * D + d0 + d) = *reinterpret_cast<uint4*>(hh);
+            }
+          }
+        }
+      }
+      if (stored) {
+        if (partial) {
+          p.part_ml[(long long)split * p.T * heads + at] = make_float2(l > 0.0f ? m * p.scale_log2 : -INFINITY, l);
+        } else if (!PAGED && p.lse != nullptr) {
+          p.lse[(((long long)b * p.kv_heads + kvh) * p.T + i) * p.group + (row - token * p.group)] =
+              l > 0.0f ? m * p.scale_log2 + log2f(l) : 0.0f;
+        }
+      }
+    }
+    fence_before_sync();
+    if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 0) { fence_after_sync(); tmem_dealloc(tmem, kTmemCols); }
+}
+
+// Partial sums of a row's splits to its output: a warp a row.  With each split's reference m_s and total l_s,
+// o = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M).  The order of the sums is that of the splits.
+template <int D>
+__global__ void __launch_bounds__(256) window_join_kernel(const float* part_o, const float2* part_ml, elem_t* out, long long rows, int splits) {
+  constexpr int V = D / 32;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml[s * rows + row].x);
+  float total = 0.0f, o[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    const float2 ml = part_ml[s * rows + row];
+    if (!(ml.y > 0.0f)) continue;              // also: sums that were not written
+    const float w = exp2f(ml.x - top);
+    total += ml.y * w;
+    const float* src = part_o + (s * rows + row) * D + lane * V;
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] += src[v] * w;
+  }
+  const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+  elem_t* dst = out + row * D + lane * V;
+#pragma unroll
+  for (int v = 0; v < V; v += 2) *reinterpret_cast<elem2_t*>(dst + v) = ff2e2(o[v] * inv, o[v + 1] * inv);
+}
+
+}  // namespace
+
+extern "C" {
+
+// q (B, T, heads, D), k and v (B, T, kv_heads, D) with element strides each; out contiguous; lse fp32 (B, kv_heads, T, group) or
+// null; lengths (B) or null.
+int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_sh, const void* k, const void* v, long long k_sb,
+                    long long k_st, long long k_sh, long long v_sb, long long v_st, long long v_sh, void* out, float* lse,
+                    const int* lengths, int B, int T, int kv_heads, int group, int D, int window, int sinks, float scale, int* status,
+                    void* stream) {
+  if ((D != 64 && D != 128) || B < 1 || T < 1 || kv_heads < 1 || group < 1 || group > kRows || sinks < 0) return 1;
+  FwdParams p = {};
+  p.T = T; p.B = B; p.kv_heads = kv_heads; p.group = group;
+  p.tile_tokens = kRows / group;
+  p.window = window < 1 || window > kNoWindow ? kNoWindow : window;   // 0: none
+  p.sinks = p.window == kNoWindow ? 0 : sinks < kNoWindow ? sinks : kNoWindow;
+  p.lengths = lengths;
+  p.splits = 1;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.out = (elem_t*)out;
+  p.lse = lse;
+  p.status = status;
+  const long long pairs = (T + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens), blocks = pairs * B * kv_heads;
+  if (blocks > 0x7fffffffll || (uintptr_t)out & 15) return (uintptr_t)out & 15 ? 2 : 1;
+  CUtensorMap mq, mk, mv;
+  int e;
+  if ((e = encode_heads(&mq, q, D, kv_heads * group, T, B, q_sh, q_st, q_sb, group, p.tile_tokens))) return e;
+  if ((e = encode_heads(&mk, k, D, kv_heads, T, B, k_sh, k_st, k_sb, 1, kKeys))) return e;
+  if ((e = encode_heads(&mv, v, D, kv_heads, T, B, v_sh, v_st, v_sb, 1, kKeys))) return e;
+  const int smem = D == 64 ? fwd_smem_bytes<64>() : fwd_smem_bytes<128>();
+  auto kernel = D == 64 ? window_fwd_kernel<64, false> : window_fwd_kernel<128, false>;
+  if (set_smem(kernel, smem)) return 5;
+  kernel<<<(unsigned)blocks, kFwdThreads, smem, (cudaStream_t)stream>>>(mq, mk, mv, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : 5;
+}
+
+// q (rows, heads, D) with strides; pages (pages, page, kv_heads, D) with strides; tables (B, max_pages) with stride t_sb; lengths
+// (B); offsets (B + 1) or null (rows == B); out contiguous.  With splits > 1 part_o (splits, rows, heads, D) and part_ml (splits,
+// rows, heads, 2) fp32.
+int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const void* k_pages, long long k_sp, long long k_ss, long long k_sh,
+                         const void* v_pages, long long v_sp, long long v_ss, long long v_sh, const int* tables, long long t_sb,
+                         const int* lengths, const int* offsets, void* out, float* part_o, void* part_ml, int splits, int rows, int B,
+                         int max_pages, int page, int pages, int kv_heads, int group, int D, int window, int sinks, float scale,
+                         int* status, void* stream) {
+  if ((D != 64 && D != 128) || B < 1 || rows < 1 || kv_heads < 1 || group < 1 || group > kRows || sinks < 0 || splits < 1 || pages < 1 ||
+      page < 8 || page % 8 || max_pages < 0 || splits > 65535 || kv_heads > 65535)
+    return 1;
+  FwdParams p = {};
+  p.T = rows; p.B = B; p.kv_heads = kv_heads; p.group = group;
+  p.tile_tokens = kRows / group;
+  p.window = window < 1 || window > kNoWindow ? kNoWindow : window;   // 0: none
+  p.sinks = p.window == kNoWindow ? 0 : sinks < kNoWindow ? sinks : kNoWindow;
+  p.lengths = lengths; p.offsets = offsets; p.tables = tables; p.t_sb = t_sb;
+  p.max_pages = max_pages; p.page = page; p.pages = pages;
+  p.piece = page;                            // slots of one copy: the largest power of two in a page, 128 at most
+  for (int r = 128; r >= 8; r >>= 1)
+    if (page % r == 0) { p.piece = r; break; }
+  p.splits = splits;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.out = (elem_t*)out;
+  p.part_o = part_o;
+  p.part_ml = (float2*)part_ml;
+  p.status = status;
+  if (((uintptr_t)out | (uintptr_t)part_o | (uintptr_t)part_ml) & 15) return 2;
+  CUtensorMap mq, mk, mv;
+  int e;
+  if ((e = encode_heads(&mq, q, D, kv_heads * group, rows, 1, q_sh, q_st, (long long)rows * q_st, group, p.tile_tokens))) return e;
+  if ((e = encode_heads(&mk, k_pages, D, kv_heads, page, pages, k_sh, k_ss, k_sp, 1, p.piece))) return e;
+  if ((e = encode_heads(&mv, v_pages, D, kv_heads, page, pages, v_sh, v_ss, v_sp, 1, p.piece))) return e;
+  cudaStream_t s = (cudaStream_t)stream;
+  // pairs of tiles: one a sequence without offsets; with them, at most one that is not full of each sequence
+  const int per = 2 * p.tile_tokens;
+  const long long pairs = offsets == nullptr ? B : rows / per + (rows < B ? rows : B) + 1;
+  const int smem = D == 64 ? fwd_smem_bytes<64>() : fwd_smem_bytes<128>();
+  auto kernel = D == 64 ? window_fwd_kernel<64, true> : window_fwd_kernel<128, true>;
+  if (set_smem(kernel, smem)) return 5;
+  kernel<<<dim3((unsigned)pairs, kv_heads, splits), kFwdThreads, smem, s>>>(mq, mk, mv, p);
+  if (splits > 1) {
+    const long long all = (long long)rows * kv_heads * group;
+    const unsigned blocks = (unsigned)((all + 7) / 8);
+    if (D == 64)
+      window_join_kernel<64><<<blocks, 256, 0, s>>>(part_o, p.part_ml, p.out, all, splits);
+    else
+      window_join_kernel<128><<<blocks, 256, 0, s>>>(part_o, p.part_ml, p.out, all, splits);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : 5;
+}
+
+}  // extern "C"

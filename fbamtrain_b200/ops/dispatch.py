@@ -318,3 +318,191 @@ def token_logprobs(logits, targets=None, top: int = 0, temperature: float = 1.0)
         from .logprobs import token_logprobs as f
         return TokenLogprobs(*f(logits, targets, top, temperature))
     return TokenLogprobs(*ref.token_logprobs(logits, targets, top, temperature))
+
+
+def rotary_frequencies(dims: int, base: float = 10000.0, factor: float = 1.0, context: Optional[int] = None, few: float = 1.0,
+                       many: float = 32.0):
+    """The frequencies of :func:`rotary`, made once by a model: pair ``i`` of ``dims / 2`` turns by ``base^(-2 i / dims)`` a
+    position.
+
+    ``factor`` scales positions for contexts that many times as long: all frequencies are divided by it, or, with the ``context``
+    that the model was trained on, those that turn around fewer than ``few`` times within it; those that do more than ``many`` times
+    stay, the ones between go over linearly, and what is turned is multiplied by ``1 + 0.1 ln(factor)``."""
+    if not 0 <= dims <= 256 or dims % 2:
+        raise ValueError(f"between 0 and 256 channels turn, in pairs, got {dims}")
+    if not 0.0 < base < float("inf"):
+        raise ValueError(f"the base is above 0 and finite, got {base}")
+    if not 1.0 <= factor < float("inf"):
+        raise ValueError(f"the factor is 1 or more and finite, got {factor}")
+    if context is not None and (context < 1 or not 0.0 <= few < many < float("inf")):
+        raise ValueError(f"a context of one token or more and 0 <= few < many, got {context}, {few} and {many}")
+    from .positions import rotary_frequencies as f
+    return f(dims, base, factor, context, few, many)
+
+
+def rotary(x, positions, freqs, heads: Optional[int] = None, interleaved: bool = False):
+    """``x`` ``(B, T, H, D)`` with the first ``heads`` heads (all by default) turned by their positions: of their first
+    ``freqs.dims`` channels the pairs ``(i, i + dims / 2)``, or ``(2 i, 2 i + 1)`` where ``interleaved``.  Everything else is copied,
+    so a fused projection goes through whole (``heads``: its query and key heads).  ``positions`` ``(B, T)``, ``(1, T)`` or
+    ``(T,)`` int32 or int64, of any size: angles are exact to 2^-32 of a turn.  Differentiable in ``x``."""
+    if x.dim() != 4:
+        raise ValueError(f"heads are (batch, steps, heads, width), got {tuple(x.shape)}")
+    b, t, h, d = x.shape
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"positions are int32 or int64, got {positions.dtype}")
+    if positions.shape not in ((b, t), (1, t), (t,)):
+        raise ValueError(f"positions are {(b, t)}, {(1, t)} or {(t,)}, got {tuple(positions.shape)}")
+    heads = h if heads is None else heads
+    if not 0 <= heads <= h:
+        raise ValueError(f"between 0 and {h} heads turn, got {heads}")
+    if freqs.dims > d:
+        raise ValueError(f"frequencies of {freqs.dims} channels do not fit heads of {d}")
+    if x.numel() and _native(x, family="mha"):
+        from .positions import rotary as f
+        return f(x, positions, freqs, heads, interleaved)
+    return ref.rotary(x, positions, freqs, heads, interleaved)
+
+
+def _check_window(heads: int, kv_heads: int, window, sinks) -> None:
+    if kv_heads < 1 or heads < 1 or heads % kv_heads or heads // kv_heads > 128:
+        raise ValueError(f"{heads} query heads do not share {kv_heads} key heads")
+    if window is not None and window < 1:
+        raise ValueError(f"a window is one token or more (None for no limit), got {window}")
+    if sinks < 0:
+        raise ValueError(f"the number of first tokens is 0 or more, got {sinks}")
+
+
+def _check_lengths(lengths, b) -> None:
+    if lengths is not None and (lengths.shape != (b,) or lengths.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"lengths are int32 or int64 ({b},), got {lengths.dtype} {tuple(lengths.shape)}")
+
+
+def _kernel_width(d: int) -> Optional[int]:
+    """The head dimension of the kernels that one of ``d`` runs as, or None."""
+    return 64 if d <= 64 else 128 if d <= 128 else None
+
+
+def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, lengths=None):
+    """Causal attention over the last ``window`` tokens (None: all) and the first ``sinks``: ``q`` ``(B, T, H, D)``, ``k`` and ``v``
+    ``(B, T, Hkv, D)`` with ``H`` a multiple of ``Hkv`` (head ``h`` reads key head ``h Hkv // H``) → ``(B, T, H, D)``.  Query ``i``
+    sees key ``j`` where ``j <= i`` and ``i - j < window`` or ``j < sinks``; scores are scaled by ``D ** -0.5``.
+
+    ``lengths`` ``(B,)``: tokens of each sequence of a padded batch.  What lies behind them may hold anything, gives zeros and has
+    zero gradients.  Values within the sequences are finite.  Results and gradients do not vary from run to run.  Heads of up to
+    128 channels run on the kernels (as 64 or 128); wider ones take the PyTorch definition."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.shape[3] == 0:
+        raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not go together")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"queries, keys and values are of one type, got {q.dtype}, {k.dtype} and {v.dtype}")
+    _check_window(q.shape[2], k.shape[2], window, sinks)
+    _check_lengths(lengths, q.shape[0])
+    d, wide = q.shape[3], _kernel_width(q.shape[3])
+    if q.numel() and wide and _native(q, family="mha"):
+        from .window import window_attention as f
+        if d == wide:
+            return f(q, k, v, window, sinks, lengths, d ** -0.5)
+        pad = (0, wide - d)
+        return f(*(torch.nn.functional.pad(x, pad) for x in (q, k, v)), window, sinks, lengths, d ** -0.5)[..., :d]
+    return ref.window_attention(q, k, v, window, sinks, lengths)
+
+
+def window_attention_qkv(qkv, kv_heads: int, window: Optional[int] = None, sinks: int = 0, lengths=None):
+    """:func:`window_attention` on a fused projection ``(B, T, H + 2 Hkv, D)``: query heads, key heads, value heads.  Its gradient is
+    one tensor."""
+    if qkv.dim() != 4 or qkv.shape[3] == 0:
+        raise ValueError(f"the projection is (batch, steps, heads, width), got {tuple(qkv.shape)}")
+    heads = qkv.shape[2] - 2 * kv_heads
+    _check_window(heads, kv_heads, window, sinks)
+    _check_lengths(lengths, qkv.shape[0])
+    d, wide = qkv.shape[3], _kernel_width(qkv.shape[3])
+    if qkv.numel() and wide and _native(qkv, family="mha"):
+        from .window import window_attention_qkv as f
+        if d == wide:
+            return f(qkv, kv_heads, window, sinks, lengths, d ** -0.5)
+        return f(torch.nn.functional.pad(qkv, (0, wide - d)), kv_heads, window, sinks, lengths, d ** -0.5)[..., :d]
+    return ref.window_attention(*qkv.split((heads, kv_heads, kv_heads), 2), window, sinks, lengths)
+
+
+def _check_cache(n, kv_heads, d, dtype, device, k_pages, v_pages, tables, lengths, offsets) -> None:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[2:] != (kv_heads, d) or 0 in k_pages.shape[:2]:
+        raise ValueError(f"pages are (pages, slots, {kv_heads}, {d}), got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    if not k_pages.dtype == v_pages.dtype == dtype:
+        raise TypeError(f"the tokens are {dtype}, the pages {k_pages.dtype} and {v_pages.dtype}")
+    if tables.dim() != 2 or tables.dtype != torch.int32 or (tables.shape[1] > 1 and tables.stride(1) != 1):
+        raise ValueError(f"page tables are int32 (sequences, pages) with dense rows, got {tables.dtype} {tuple(tables.shape)}")
+    b = tables.shape[0]
+    if lengths.shape != (b,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        raise ValueError(f"lengths are int32 ({b},), got {lengths.dtype} {tuple(lengths.shape)}")
+    if offsets is None and n != b:
+        raise ValueError(f"without offsets there is one new token for each of {b} sequences, got {n}")
+    if offsets is not None and (offsets.shape != (b + 1,) or offsets.dtype != torch.int32 or not offsets.is_contiguous()):
+        raise ValueError(f"offsets are int32 ({b + 1},), got {offsets.dtype} {tuple(offsets.shape)}")
+    for name, x in (("key pages", k_pages), ("value pages", v_pages), ("page tables", tables), ("lengths", lengths), ("offsets", offsets)):
+        if x is not None and x.device != device:
+            raise ValueError(f"{name} are on {x.device}, the tokens on {device}")
+
+
+def _check_cache_native(d, k_pages, v_pages) -> None:
+    """What the kernels want of a cache beyond what the definition does: a call cannot lay pages out anew."""
+    if d not in (64, 128):
+        raise ValueError(f"the kernels keep heads of 64 or 128 channels in a cache, got {d}")
+    if k_pages.shape[1] % 8:
+        raise ValueError(f"pages have a multiple of 8 slots, got {k_pages.shape[1]}")
+    for x in (k_pages, v_pages):
+        sp, ss, sh, sd = x.stride()
+        if sd != 1 or sp % 8 or ss % 8 or sh % 8 or x.data_ptr() % 16:
+            raise ValueError("pages start at 16-byte boundaries, with 16-byte strides and channels side by side")
+
+
+def _no_gradient(name, *tensors) -> None:
+    from .derivatives import tracked
+    if tracked(*tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train with window_attention")
+
+
+def cache_append(qkv, k_pages, v_pages, tables, lengths, offsets=None, freqs=None, interleaved: bool = False):
+    """New tokens into a paged cache.  ``qkv`` ``(N, H + 2 Hkv, D)``: query, key and value heads; ``k_pages`` and ``v_pages``
+    ``(pages, slots, Hkv, D)``; ``tables`` ``(B, M)`` int32: the pages of each sequence in order, -1 where it has none; ``lengths``
+    ``(B,)`` int32: tokens of each sequence WITH the new ones; ``offsets`` ``(B + 1,)`` int32 from 0: the rows of each sequence's new
+    tokens, one each by default.
+
+    The new tokens are the last ones of their sequences.  Queries and keys are turned by their positions (``freqs``, ``interleaved`` as in
+    :func:`rotary`; None: as they are), keys and values are written to their slots, and the queries are returned ``(N, H, D)``.  Rows
+    behind the last offset, and tokens that would lie in front of their sequence's start, give zeros and are not written; nor is a token
+    whose entry in the table is no page.  Sequences may share pages, but no two tokens of a call a slot."""
+    if qkv.dim() != 3 or k_pages.dim() != 4:
+        raise ValueError(f"new tokens are (tokens, heads, width) and pages (pages, slots, heads, width), got {tuple(qkv.shape)} and {tuple(k_pages.shape)}")
+    n, all_heads, d = qkv.shape
+    kv = k_pages.shape[2]
+    heads = all_heads - 2 * kv
+    _check_window(heads, kv, None, 0)
+    _check_cache(n, kv, d, qkv.dtype, qkv.device, k_pages, v_pages, tables, lengths, offsets)
+    if freqs is not None and freqs.dims > d:
+        raise ValueError(f"frequencies of {freqs.dims} channels do not fit heads of {d}")
+    _no_gradient("cache_append", qkv, k_pages, v_pages)
+    if n and tables.shape[0] and _native(qkv, family="mha"):
+        _check_cache_native(d, k_pages, v_pages)
+        if freqs is not None and freqs.dims % (8 if interleaved else 16):
+            raise ValueError(f"the kernels turn a multiple of {8 if interleaved else 16} channels in a cache, got {freqs.dims}")
+        from .positions import cache_append as f
+        return f(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interleaved, heads, kv)
+    return ref.cache_append(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interleaved, heads, kv)
+
+
+def cache_attention(q, k_pages, v_pages, tables, lengths, offsets=None, window: Optional[int] = None, sinks: int = 0):
+    """Attention of new tokens ``q`` ``(N, H, D)`` over a paged cache that holds them already (arguments as in
+    :func:`cache_append`, mask as in :func:`window_attention`) → ``(N, H, D)``.  Slots that no query of a sequence sees may hold
+    anything and their pages may be gone from the table (-1) or belong to others; an entry that is no page where a query does see it
+    counts as keys and values of zero.  Rows of no sequence, or in front of one's start, give zeros.  Keys behind the table's width do
+    not exist."""
+    if q.dim() != 3 or k_pages.dim() != 4:
+        raise ValueError(f"new tokens are (tokens, heads, width) and pages (pages, slots, heads, width), got {tuple(q.shape)} and {tuple(k_pages.shape)}")
+    n, heads, d = q.shape
+    _check_window(heads, k_pages.shape[2], window, sinks)
+    _check_cache(n, k_pages.shape[2], d, q.dtype, q.device, k_pages, v_pages, tables, lengths, offsets)
+    _no_gradient("cache_attention", q, k_pages, v_pages)
+    if n and tables.shape[0] and _native(q, family="mha"):
+        _check_cache_native(d, k_pages, v_pages)
+        from .window import cache_attention as f
+        return f(q, k_pages, v_pages, tables, lengths, offsets, window, sinks)
+    return ref.cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks)

@@ -30,7 +30,7 @@ GEMM_ACC_NONE, GEMM_ACC_RMW, GEMM_ACC_ATOMIC = 0, 1, 2
 _ERRORS = {1: "unsupported shape", 2: "operand not 16-byte aligned", 3: "tensor-map encode failed",
            4: "driver entry point unavailable", 5: "kernel launch failed",
            101: "TMA producer wait timed out", 102: "MMA wait timed out", 103: "epilogue wait timed out",
-           201: "LSTM step exchange timed out"}
+           201: "LSTM step exchange timed out", 501: "attention wait timed out"}
 
 
 class ConvGeom(C.Structure):
@@ -78,7 +78,7 @@ def available(dtype: torch.dtype = torch.bfloat16) -> bool:
     return os.path.exists(LIB_PATH_FP16 if dtype == torch.float16 else LIB_PATH)
 
 
-INTERFACE_REVISION = 8        # FBAM_INTERFACE_REVISION of csrc/gemm_tcgen05.h
+INTERFACE_REVISION = 9        # FBAM_INTERFACE_REVISION of csrc/gemm_tcgen05.h
 
 
 def _check_struct_layout(library: C.CDLL, path: str) -> None:
@@ -115,6 +115,14 @@ _ARGTYPES = {
     "fbam_gated_few_rows": (_P, _L, _P, _L, _P, _P, _L, _P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _P),
     "fbam_logprobs_fwd": (_P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _I, _I, _F, _P),
     "fbam_logprobs_bwd": (_P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _L, _I, _F, _P),
+    "fbam_rotary": (_P, _L, _L, _L, _P, _P, _I, _L, _L, _P, _I, _F, _I, _I, _L, _L, _I, _I, _I, _P),
+    "fbam_cache_append": (_P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _P, _P, _P, _I, _F, _I, _L, _I, _I, _I, _I, _I, _I, _I, _P),
+    "fbam_window_fwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P),
+    "fbam_window_bwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _P, _L, _P, _L, _L, _L, _P, _L, _L, _L,
+                        _P, _L, _L, _L, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P),
+    "fbam_window_bwd_workspace": (_I, _I, _I, _I, _I),
+    "fbam_cache_attention": (_P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
+                             _F, _P, _P),
 }
 
 
@@ -128,6 +136,7 @@ def _load(path: str) -> C.CDLL:
         getattr(library, name).restype = C.c_int
     for name, types in _ARGTYPES.items():
         getattr(library, name).argtypes = types
+    library.fbam_window_bwd_workspace.restype = C.c_longlong
     return library
 
 

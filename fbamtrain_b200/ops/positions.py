@@ -1,0 +1,91 @@
+"""Rotary positions and the append of new tokens to a paged cache (``csrc/rotary.cu``)."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import native as nv
+from .derivatives import first_only, tracked
+
+MAX_PAIRS = 128
+
+
+class RotaryFrequencies(NamedTuple):
+    """How far each pair of channels turns a position: fractions of a turn, times 2^64, and the factor on what is turned."""
+    turns: Tuple[int, ...]
+    magnitude: float
+    table: C.Array                                      # ``turns`` as the kernels take them
+
+    @property
+    def dims(self) -> int:
+        return 2 * len(self.turns)
+
+
+def rotary_frequencies(dims: int, base: float, factor: float, context: Optional[int], few: float, many: float) -> RotaryFrequencies:
+    turns, magnitude = [], 1.0
+    for i in range(dims // 2):
+        theta = base ** (-2.0 * i / dims)
+        if factor != 1.0:
+            kept = 0.0
+            if context is not None:
+                around = context * theta / (2.0 * math.pi)
+                kept = min(1.0, max(0.0, (around - few) / (many - few)))
+            theta *= kept + (1.0 - kept) / factor
+        turns.append(round(math.ldexp(theta / (2.0 * math.pi), 64)) % 2 ** 64)
+    if factor > 1.0 and context is not None:
+        magnitude = 1.0 + 0.1 * math.log(factor)
+    return RotaryFrequencies(tuple(turns), magnitude, (C.c_ulonglong * max(1, len(turns)))(*turns))
+
+
+def _turned(x, positions, freqs, heads, interleaved, inverse):
+    b, t, h, d = x.shape
+    if x.stride(3) != 1:
+        x = x.contiguous()
+    y = x.new_empty((b, t, h, d))
+    sb, st, sh, _ = x.stride()
+    pb, pt = positions.stride()
+    nv.check(nv.lib(x).fbam_rotary(x.data_ptr(), sb, st, sh, y.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, pb, pt,
+                                   freqs.table, len(freqs.turns), freqs.magnitude, interleaved, inverse, b, t, h, d, heads, nv.stream()),
+             "fbam_rotary")
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, freqs, heads, interleaved):
+        ctx.save_for_backward(positions)
+        ctx.linked = ()
+        ctx.how = (freqs, heads, interleaved)
+        return _turned(x, positions, freqs, heads, interleaved, False)
+
+    @staticmethod
+    @first_only("rotary")
+    def backward(ctx, dy):
+        positions, = ctx.saved_tensors
+        return _turned(dy, positions, *ctx.how, True), None, None, None, None
+
+
+def rotary(x, positions, freqs, heads, interleaved):
+    if positions.device != x.device:
+        raise ValueError(f"positions are on {positions.device}, the heads on {x.device}")
+    positions = positions.expand(x.shape[:2])
+    if tracked(x):
+        return _Rotary.apply(x, positions, freqs, heads, interleaved)
+    return _turned(x, positions, freqs, heads, interleaved, False)
+
+
+def cache_append(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interleaved, q_heads, kv_heads):
+    n, _, d = qkv.shape
+    if qkv.stride(2) != 1 or qkv.stride(0) % 8 or qkv.stride(1) % 8 or qkv.data_ptr() % 16:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    q = qkv.new_empty((n, q_heads, d))
+    turns, pairs, magnitude = (None, 0, 1.0) if freqs is None else (freqs.table, len(freqs.turns), freqs.magnitude)
+    nv.check(nv.lib(qkv).fbam_cache_append(
+        qkv.data_ptr(), qkv.stride(0), qkv.stride(1), q.data_ptr(), k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(),
+        *v_pages.stride()[:3], tables.data_ptr(), tables.stride(0), lengths.data_ptr(), nv.addr(offsets), turns, pairs, magnitude,
+        interleaved, n, tables.shape[0], tables.shape[1], k_pages.shape[1], k_pages.shape[0], q_heads, kv_heads, d, nv.stream()),
+        "fbam_cache_append")
+    return q

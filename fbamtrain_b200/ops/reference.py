@@ -193,3 +193,102 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], top: i
         order = torch.where(order.isnan(), float("-inf"), order)
         ids = order.sort(dim=-1, descending=True, stable=True)[1][..., :top]
         return logprob, entropy, logp.gather(-1, ids), ids
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freqs, heads: int, interleaved: bool) -> torch.Tensor:
+    """``x`` ``(B, T, H, D)``: the pairs of the first ``2 len(freqs.turns)`` channels of the first ``heads`` heads turned by
+    ``positions`` (broadcast to ``(B, T)``) times the frequencies; the angles in 64 bits."""
+    n = 2 * len(freqs.turns)
+    theta = torch.tensor([t * (2 * math.pi / 2 ** 64) for t in freqs.turns], dtype=torch.float64, device=x.device)
+    angle = (positions.expand(x.shape[:2]).double().unsqueeze(-1) * theta).unsqueeze(2)
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    cos, sin = (freqs.magnitude * angle.cos()).to(wide), (freqs.magnitude * angle.sin()).to(wide)
+    r = x[:, :, :heads, :n].to(wide)
+    if interleaved:
+        a, b = r[..., 0::2], r[..., 1::2]
+        r = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+    else:
+        a, b = r[..., :n // 2], r[..., n // 2:]
+        r = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    turned = torch.cat([r.to(x.dtype), x[:, :, :heads, n:]], -1)
+    return torch.cat([turned, x[:, :, heads:]], 2)
+
+
+def _attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, at: torch.Tensor, end, window: Optional[int], sinks: int) -> torch.Tensor:
+    """One sequence: ``q`` ``(n, H, D)`` at positions ``at``, ``k`` and ``v`` ``(m, Hkv, D)`` from position 0 on, of which the
+    first ``end`` are there; queries that see nothing give zeros."""
+    n, h, d = q.shape
+    kv, like = k.shape[1], q
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    j = torch.arange(k.shape[0], device=q.device)
+    there = (j < end).view(-1, 1, 1)
+    # what lies behind the end can hold anything
+    q = torch.where((at < end).view(-1, 1, 1), q.to(wide), 0.0)
+    k, v = torch.where(there, k.to(wide), 0.0), torch.where(there, v.to(wide), 0.0)
+    seen = (j <= at.unsqueeze(1)) & (j < end) & (at.unsqueeze(1) < end)
+    if window is not None:
+        seen = seen & ((at.unsqueeze(1) - j < window) | (j < sinks))
+    s = torch.einsum("ngrd,mgd->grnm", q.reshape(n, kv, h // kv, d), k) * d ** -0.5
+    nothing = ~seen.any(1)
+    s = s.masked_fill(~seen & ~nothing.unsqueeze(1), float("-inf"))
+    p = torch.softmax(s, dim=-1).masked_fill(nothing.unsqueeze(1), 0.0)
+    o = torch.einsum("grnm,mgd->ngrd", p, v).reshape(n, h, d)
+    return o.masked_fill(nothing.view(-1, 1, 1), 0.0).to(like.dtype)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int], sinks: int,
+                     lengths: Optional[torch.Tensor]) -> torch.Tensor:
+    """``q`` ``(B, T, H, D)``, ``k`` and ``v`` ``(B, T, Hkv, D)``: query ``i`` sees key ``j`` where ``j <= i`` and ``i - j <
+    window`` or ``j < sinks``, both within the sequence's length; other queries give zeros."""
+    b, t = q.shape[:2]
+    at = torch.arange(t, device=q.device)
+    rows = [_attend(q[i], k[i], v[i], at, t if lengths is None else lengths[i], window, sinks) for i in range(b)]
+    return torch.stack(rows) if rows else torch.empty_like(q)
+
+
+def _new_tokens(n: int, tables: torch.Tensor, lengths: torch.Tensor, offsets: Optional[torch.Tensor]):
+    """Of each sequence: its number, the rows of its new tokens and its length."""
+    starts = list(range(tables.shape[0] + 1)) if offsets is None else offsets.tolist()
+    return [(b, starts[b], min(starts[b + 1], n), max(length, 0)) for b, length in enumerate(lengths.tolist())]
+
+
+def cache_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
+                 offsets: Optional[torch.Tensor], freqs, interleaved: bool, q_heads: int, kv_heads: int) -> torch.Tensor:
+    """Turns the queries and keys of new tokens by their positions, writes keys and values into the pages and returns the
+    queries; rows of no sequence, or in front of one's start, give zeros, and tokens without a page are not written."""
+    pages, page = k_pages.shape[:2]
+    q = qkv.new_zeros((qkv.shape[0], q_heads, qkv.shape[2]))
+    for b, lo, hi, length in _new_tokens(qkv.shape[0], tables, lengths, offsets):
+        for n in range(lo, hi):
+            at = length - (hi - n)
+            if at < 0:
+                continue
+            row = qkv[n:n + 1].unsqueeze(0)
+            if freqs is not None:
+                row = rotary(row, torch.tensor([[at]], device=qkv.device), freqs, q_heads + kv_heads, interleaved)
+            q[n] = row[0, 0, :q_heads]
+            where = int(tables[b, at // page]) if at // page < tables.shape[1] else -1
+            if 0 <= where < pages:
+                k_pages[where, at % page] = row[0, 0, q_heads:q_heads + kv_heads]
+                v_pages[where, at % page] = row[0, 0, q_heads + kv_heads:]
+    return q
+
+
+def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
+                    offsets: Optional[torch.Tensor], window: Optional[int], sinks: int) -> torch.Tensor:
+    """New tokens ``(N, H, D)``, the last ones of their sequences, over the keys and values that the sequences have in the pages
+    (zeros where an entry of the table is no page); rows of no sequence, or in front of one's start, give zeros."""
+    pages, page = k_pages.shape[:2]
+    out = torch.zeros_like(q)
+    for b, lo, hi, length in _new_tokens(q.shape[0], tables, lengths, offsets):
+        first = length - (hi - lo)
+        skip = max(0, -first)
+        if lo + skip >= hi:
+            continue
+        ids = tables[b].long()
+        there = ((ids >= 0) & (ids < pages)).view(-1, 1, 1, 1)
+        k, v = (torch.where(there, x[ids.clamp(0, pages - 1)], 0.0).flatten(0, 1) for x in (k_pages, v_pages))
+        at = torch.arange(first + skip, length, device=q.device)
+        # queries behind the end of the table see what is in front of it
+        out[lo + skip:hi] = _attend(q[lo + skip:hi], k[:length], v[:length], at, length, window, sinks)
+    return out

@@ -1,0 +1,160 @@
+"""Attention over a sliding window and the first few tokens (``csrc/window_attention.cu``, ``csrc/window_attention_bwd.cu``).
+
+Query heads may share key heads.  Heads come as views: of three tensors, or of one fused projection ``(B, T, heads + 2 kv_heads,
+D)``, whose gradient is one tensor then (gradients of three selections would each be a zero-filled tensor of the full size).  The
+forward keeps its output and one fp32 value per query row for the backward.
+"""
+from __future__ import annotations
+
+import torch
+
+from ..utils import flops
+from . import native as nv
+from .derivatives import first_only, tracked
+
+F32 = torch.float32
+
+
+def _usable(x: torch.Tensor) -> bool:
+    """Whether the copy engine can fetch ``x`` ``(B, T, H, D)`` where it lies: 16-byte strides and start."""
+    sb, st, sh, sd = x.stride()
+    return sd == 1 and not (sb % 8 or st % 8 or sh % 8) and x.data_ptr() % 16 == 0
+
+
+def _pairs(b, t, window):
+    """Pairs of a query and a key in ``b`` sequences of ``t`` tokens, the first tokens apart."""
+    w = t if window is None else min(window, t)
+    return b * (w * (w + 1) // 2 + (t - w) * w)
+
+
+def _forward(q, k, v, window, sinks, lengths, scale, keep):
+    """``(out, lse)``; ``lse`` with ``keep``: what the backward needs."""
+    b, t, h, d = q.shape
+    kv = k.shape[2]
+    out = q.new_empty((b, t, h, d))
+    lse = q.new_empty((b, kv, t, h // kv), dtype=F32) if keep else None
+    nv.check(nv.lib(q).fbam_window_fwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+                                       out.data_ptr(), nv.addr(lse), nv.addr(lengths), b, t, kv, h // kv, d, window or 0, sinks, scale,
+                                       nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_fwd")
+    flops.add(4.0 * h * d * _pairs(b, t, window))
+    return out, lse
+
+
+def _backward(saved, d_out, into, window, sinks, scale):
+    """Fills ``into``: views for the gradients of the heads."""
+    q, k, v, out, lse, lengths = saved
+    b, t, h, d = q.shape
+    kv = k.shape[2]
+    if not _usable(d_out):
+        d_out = d_out.clone(memory_format=torch.contiguous_format)
+    lib = nv.lib(q)
+    floats = lib.fbam_window_bwd_workspace(b, t, kv, h // kv, d)
+    work = lse.new_empty(floats)
+    dq, dk, dv = into
+    nv.check(lib.fbam_window_bwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+                                 out.data_ptr(), d_out.data_ptr(), *d_out.stride()[:3], lse.data_ptr(), nv.addr(lengths),
+                                 work.data_ptr(), floats, dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(),
+                                 *dv.stride()[:3], b, t, kv, h // kv, d, window or 0, sinks, scale,
+                                 nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_bwd")
+    flops.add(10.0 * h * d * _pairs(b, t, window))
+
+
+class _Window(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, lengths, scale):
+        out, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        ctx.linked = ()
+        ctx.how = (window, sinks, scale)
+        return out
+
+    @staticmethod
+    @first_only("window_attention")
+    def backward(ctx, d_out):
+        saved = ctx.saved_tensors
+        into = [x.new_empty(x.shape) for x in saved[:3]]
+        _backward(saved, d_out, into, *ctx.how)
+        return (*into, None, None, None, None)
+
+
+class _WindowQkv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, kv, window, sinks, lengths, scale):
+        q, k, v = _heads(qkv, kv)
+        out, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
+        ctx.save_for_backward(qkv, out, lse, lengths)
+        ctx.linked = ()
+        ctx.how = (window, sinks, scale)
+        ctx.kv = kv
+        return out
+
+    @staticmethod
+    @first_only("window_attention_qkv")
+    def backward(ctx, d_out):
+        qkv, out, lse, lengths = ctx.saved_tensors
+        grad = qkv.new_empty(qkv.shape)
+        _backward((*_heads(qkv, ctx.kv), out, lse, lengths), d_out, _heads(grad, ctx.kv), *ctx.how)
+        return grad, None, None, None, None, None
+
+
+def _heads(qkv, kv):
+    return qkv.split((qkv.shape[2] - 2 * kv, kv, kv), 2)
+
+
+def _lengths(lengths, like):
+    if lengths is None:
+        return None
+    if lengths.device != like.device:
+        raise ValueError(f"lengths are on {lengths.device}, the heads on {like.device}")
+    return lengths.to(torch.int32).contiguous()
+
+
+def window_attention(q, k, v, window, sinks, lengths, scale):
+    lengths = _lengths(lengths, q)
+    for name, x in (("keys", k), ("values", v)):
+        if x.device != q.device:
+            raise ValueError(f"{name} are on {x.device}, the queries on {q.device}")
+    q, k, v = (x if _usable(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
+    if tracked(q, k, v):
+        return _Window.apply(q, k, v, window, sinks, lengths, scale)
+    return _forward(q, k, v, window, sinks, lengths, scale, False)[0]
+
+
+def window_attention_qkv(qkv, kv, window, sinks, lengths, scale):
+    lengths = _lengths(lengths, qkv)
+    if not _usable(qkv):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    if tracked(qkv):
+        return _WindowQkv.apply(qkv, kv, window, sinks, lengths, scale)
+    return _forward(*_heads(qkv, kv), window, sinks, lengths, scale, False)[0]
+
+
+def _splits(units: int, blocks: int) -> int:
+    """How many thread blocks share the keys of one pair of query tiles."""
+    if units >= 148:
+        return 1
+    return max(1, min(148 // units, blocks // 2, 64))
+
+
+def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks):
+    n, h, d = q.shape
+    b, most = tables.shape
+    pages, page, kv, _ = k_pages.shape
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = q.new_empty((n, h, d))
+    lib = nv.lib(q)
+    per = 2 * (128 // (h // kv))
+    units = kv * (b if offsets is None else n // per + min(n, b))
+    keys = most * page if window is None else min(most * page, window + per + sinks + 256)
+    splits = _splits(units, (keys + 127) // 128)
+    part_o = part_ml = None
+    if splits > 1:
+        part_o = q.new_empty((splits, n, h, d), dtype=F32)
+        part_ml = part_o.new_empty((splits, n, h, 2))
+    nv.check(lib.fbam_cache_attention(
+        q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
+        tables.data_ptr(), tables.stride(0), lengths.data_ptr(), nv.addr(offsets), out.data_ptr(), nv.addr(part_o), nv.addr(part_ml),
+        splits, n, b, most, page, pages, kv, h // kv, d, window or 0, sinks, d ** -0.5, nv.status_word(q.device).data_ptr(), nv.stream()),
+        "fbam_cache_attention")
+    return out
