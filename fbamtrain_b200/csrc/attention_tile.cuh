@@ -19,8 +19,26 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) tc05::mbar_arrive(bar);
 }
 
+// Descriptors of a [128 x D] operand in 64-wide panels, whose rows are contiguous along K (K-major) or along M or N (MN-major), and the
+// steps of 16 along K from their start.  A product is issued by one thread: with a descriptor formed for every instruction, eight
+// instructions took that thread as long as the tensor core (520 cycles at 128 x 128 x 128).
+__device__ __forceinline__ uint64_t k_major(uint32_t smem_addr) { return tc05::make_smem_desc_sw128(smem_addr, 16, 1024); }
+__device__ __forceinline__ uint64_t mn_major(uint32_t smem_addr) { return tc05::make_smem_desc_sw128(smem_addr, 128 * 128, 1024); }
+__device__ __forceinline__ constexpr uint64_t k_step(int k) { return uint64_t((k / 4) * 128 * 128 + (k % 4) * 32) >> 4; }
+__device__ __forceinline__ constexpr uint64_t mn_step(int k) { return uint64_t(k * 16 * 128) >> 4; }
+
 // Address of element (row, col8 = 8-element group index) in a [rows x 64]-bf16 panel with 128-byte swizzle.
 __device__ __forceinline__ uint32_t swz(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// D[tmem] (+)= A[tmem] * B[smem desc]; single-thread issue.  A: 128 rows, 16-bit elements two to a column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 
 // The driver entry point needs a context current on this thread (see gemm_tcgen05.h).
 inline void bind_context() {

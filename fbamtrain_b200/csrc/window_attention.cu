@@ -45,7 +45,8 @@ struct FwdParams {
   int splits;
   float scale_log2;
   elem_t* out;            // (B, T, heads, D) or (rows, heads, D), contiguous
-  float* lse;             // (B, kv_heads, T, group): log2 of the sum of 2^(s scale log2(e)); null where no gradient is wanted
+  float* lse;             // (B, kv_heads, tiles, 128): minus log2 of the sum of 2^(s scale log2(e)); null where no gradient is wanted
+  int tiles;              // of a sequence
   float* part_o;          // (splits, rows, heads, D) and (splits, rows, heads): sums of a split and (reference, total)
   float2* part_ml;
   int* status;
@@ -57,16 +58,6 @@ template <int D>
 constexpr int fwd_smem_bytes() { return 2 * kRows * D * 2 + kSlots<D> * kKeys * D * 2 + 256 + 1024; }
 
 constexpr int kFwdThreads = 320;   // MMA issue, eight softmax warps, loads
-
-// D[tmem] (+)= A[tmem] * B[smem desc]; single-thread issue.  A: 128 rows, 16-bit elements two to a column.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 
 // Queries of one tile, or of both, as the kernel needs them: token numbers within the sequence's new tokens.
 struct Span {
@@ -282,24 +273,19 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (elect_one()) {
       const uint32_t idesc_s = make_idesc_f16kind(128, kKeys, false, false);
       const uint32_t idesc_pv = make_idesc_f16kind(128, D, false, true);   // B = V is MN-major
-      auto slot_addr = [&](int f) { return smem_u32(sKV + f % NS * kKVBytes); };
       auto wait_full = [&](int f) { return mbar_wait(&full[f % NS], (f / NS) & 1); };
+      const uint64_t kQ = k_major(smem_u32(sQ)), kKV = k_major(smem_u32(sKV)), mKV = mn_major(smem_u32(sKV));
       auto issue_s = [&](int g, int f) {       // S_g = Q_g K^T
-        const uint32_t q_addr = smem_u32(sQ + g * kQBytes), k_addr = slot_addr(f);
+        const uint64_t a = kQ + g * (kQBytes >> 4), bk = kKV + f % NS * (kKVBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t da = make_smem_desc_sw128(q_addr + (k / 4) * kRows * 128 + (k % 4) * 32, 16, 1024);
-          const uint64_t db = make_smem_desc_sw128(k_addr + (k / 4) * kKeys * 128 + (k % 4) * 32, 16, 1024);
-          mma_f16_ss(tmem + g * 128, da, db, idesc_s, k != 0);
-        }
+        for (int k = 0; k < D / 16; ++k) mma_f16_ss(tmem + g * 128, a + k_step(k), bk + k_step(k), idesc_s, k != 0);
         mma_commit(&s_full[g]);
       };
       auto issue_pv = [&](int g, int f, bool first) {     // O_g (+)= P_g V
-        const uint32_t v_addr = slot_addr(f);
+        const uint64_t bv = mKV + f % NS * (kKVBytes >> 4);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
-          mma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, make_smem_desc_sw128(v_addr + k * 16 * 128, kKeys * 128, 1024), idesc_pv,
-                     !first || k != 0);
+          mma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, bv + mn_step(k), idesc_pv, !first || k != 0);
         mma_commit(&pv_full[g]);
       };
       int done[2] = {0, 0};                    // blocks of each tile whose P V has been issued
@@ -491,8 +477,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (partial) {
           p.part_ml[(long long)split * p.T * heads + at] = make_float2(l > 0.0f ? m * p.scale_log2 : -INFINITY, l);
         } else if (!PAGED && p.lse != nullptr) {
-          p.lse[(((long long)b * p.kv_heads + kvh) * p.T + i) * p.group + (row - token * p.group)] =
-              l > 0.0f ? m * p.scale_log2 + log2f(l) : 0.0f;
+          p.lse[(((long long)b * p.kv_heads + kvh) * p.tiles + pair * 2 + g) * kRows + row] = l > 0.0f ? -(m * p.scale_log2 + log2f(l)) : 0.0f;
         }
       }
     }
@@ -536,8 +521,8 @@ __global__ void __launch_bounds__(256) window_join_kernel(const float* part_o, c
 
 extern "C" {
 
-// q (B, T, heads, D), k and v (B, T, kv_heads, D) with element strides each; out contiguous; lse fp32 (B, kv_heads, T, group) or
-// null; lengths (B) or null.
+// q (B, T, heads, D), k and v (B, T, kv_heads, D) with element strides each; out contiguous; lse fp32 (B, kv_heads, tiles, 128) or
+// null, where a tile has 128 / group tokens; lengths (B) or null.
 int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_sh, const void* k, const void* v, long long k_sb,
                     long long k_st, long long k_sh, long long v_sb, long long v_st, long long v_sh, void* out, float* lse,
                     const int* lengths, int B, int T, int kv_heads, int group, int D, int window, int sinks, float scale, int* status,
@@ -553,6 +538,7 @@ int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_s
   p.scale_log2 = scale * 1.4426950408889634f;
   p.out = (elem_t*)out;
   p.lse = lse;
+  p.tiles = (T + p.tile_tokens - 1) / p.tile_tokens;
   p.status = status;
   const long long pairs = (T + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens), blocks = pairs * B * kv_heads;
   if (blocks > 0x7fffffffll || (uintptr_t)out & 15) return (uintptr_t)out & 15 ? 2 : 1;

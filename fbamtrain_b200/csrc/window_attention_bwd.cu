@@ -4,21 +4,31 @@
 //   delta = rowsum(dO O)
 //
 // One thread block owns 128 keys of a key head and walks the tiles of queries that see any of them; a tile's 128 rows are tokens x
-// the query heads that share the key head, so dK and dV, which sum over those heads, are summed in tensor memory.  Five tcgen05
-// products a tile; roles and barriers as in the backward of the plain causal kernel:
-//   warp 21     TMA: K, V once; Q two tiles deep; dO two deep (D = 64) or one (D = 128: shared memory is full)
-//   warp 20     MMA issue: S(i+1), dV(i) once P(i) is stored, then dP(i+1), dQ(i), dK(i) (D = 64) or dQ(i), dK(i), dP(i+1)
-//               (D = 128, where dQ borrows dP's columns) once dS(i) is stored
-//   warps 4-19  point-wise: four threads per row, 32 keys each
-//   warps 0-3   add dQ to its tile's sum
+// the query heads that share the key head, so dK and dV, which sum over those heads, are summed in tensor memory.  All scores are
+// TRANSPOSED, a key a row: S^T = K Q^T and dP^T = V dO^T.  Then P^T is the first operand of dV as it stands and goes over S^T in tensor
+// memory; dS^T goes to shared memory once, where dK reads it as it lies and dQ transposed (an MN-major operand).  Roles:
+//   warp 13     TMA: K, V once; Q with lse two tiles deep; dO with delta two deep (D = 64) or one (D = 128: shared memory is full)
+//   warp 12     MMA issue: dV(i), S(i+1) once P(i) is stored; dQ(i), dK(i) once dS(i) is; dP in front of dQ(i-1) (D = 64), or, where
+//               dQ borrows its columns (D = 128), behind dV(i) once dQ(i-1) is read
+//   warps 4-11  point-wise: 32 keys and 64 queries each
+//   warps 0-3   take dQ out of tensor memory and pass it through shared memory, 16 columns at a time
+//   warps 14-15 have the copy engine add those to the tile's sum, in turns: a tile's are complete long after the next one's begin
+// Sixteen warps leave 128 registers a thread: with four threads a key (80 registers) a hundred bytes a thread were spilled, more than
+// the L1 that shared memory leaves holds, and each step waited for L2 (T 30011, 16 over 4 heads of 128, window 2048: 3 037 us).
+// Every barrier that a role waits on can complete its next phase only after that role has gone on, so a wait by phase parity cannot
+// miss a phase.
 //
-// dQ of a tile is a sum over the key blocks that it sees.  They add to it in one fixed order, so that the result does not depend on
-// which block runs when: the blocks of the first tokens, then the others from the last one down.  The first one stores, those between
-// add, the last one adds and writes the rounded gradient, so there is neither a zero fill nor a pass behind the kernel.  Each tile
-// has a counter per draining warp; a warp waits until the contributions before its own are in.  Blocks start in an order (a ticket)
-// in which every contribution waits for earlier tickets only, so a wait always ends; and each walks its tiles so that it meets a
-// tile one step after the block in front of it did: the blocks of the first tokens from the last tile back, the others from their
-// first tile on.
+// dQ of a tile is a sum over the key blocks that it sees.  They add to it in one fixed order, the last key block first, so that the
+// result does not depend on which block runs when.  The first one stores, those between add, the last one adds and writes the rounded
+// gradient, so there is neither a zero fill nor a pass behind the kernel.  Each tile has a counter of the contributions that are in.  Thread blocks take their work by a ticket, the last keys first, in which every
+// contribution waits for earlier tickets only, so a wait always ends; and all walk their tiles forward, so that a thread block meets a
+// tile one step after the one with the keys behind its own did.
+//
+// The first tokens are seen by all tiles behind them, a window's keys by those of a window only: a walk over all tiles by one thread
+// block would last as long as everything else together (3 817 against 3 216 us at T 30011, 16 over 4 heads of 128, window 2048).  It is
+// divided into parts, behind all others: run ahead of them instead, they held up the walks behind (1 947 against 2 117 us).  Long walks
+// over a window are divided as well, into halves of what a multiprocessor has to do.  The parts of a walk write their dK and dV in
+// fp32, and a last kernel adds them up in their order.
 #include "attention_tile.cuh"
 
 namespace {
@@ -34,11 +44,14 @@ struct BwdParams {
   int window, sinks;
   const int* lengths;    // (B) or null
   float scale_log2, scale;
-  const float* lse;      // (B, kv_heads, T, group), log2
-  const float* delta;    // the same
-  float4* sums;          // (B, kv_heads, tile, D / 4, 128) fp32: written before it is read
-  int* counters;         // (B, kv_heads, tile, 4): contributions that are in; zeroed
+  const float* lse;      // (B, kv_heads, tile, 128): minus log2 of the sum of 2^(s scale log2(e))
+  const float* delta;    // the same: minus delta
+  float* sums;           // (B, kv_heads, tile, D / 4, 128, 4) fp32: written before it is read
+  int* counters;         // (B, kv_heads, tile): contributions that are in; zeroed
   int* ticket;           // zeroed
+  float4* kv_parts;      // (part of a divided walk, dV | dK, D / 4, 128) fp32
+  int blocks, firsts;    // key blocks, and those of them with first tokens
+  int parts, part_tiles, first_parts, first_part_tiles;   // parts of a walk and their tiles; the same of the first tokens' blocks
   elem_t* dq;
   elem_t* dk;
   elem_t* dv;
@@ -81,17 +94,66 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restr
   }
 #pragma unroll
   for (int off = kLanes / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  if (there && part == 0) delta[(((long long)b * p.kv_heads + h / p.group) * p.T + t) * p.group + h % p.group] = s;
+  if (there && part == 0)
+    delta[(((long long)b * p.kv_heads + h / p.group) * p.tiles + t / p.tile_tokens) * kRows + t % p.tile_tokens * p.group + h % p.group] = -s;
 }
 
-constexpr int kBwdWarps = 22, kBwdThreads = kBwdWarps * 32;
+constexpr int kBwdWarps = 16, kBwdThreads = kBwdWarps * 32;
 template <int D>
 constexpr int kDoStages = D == 64 ? 2 : 1;
+constexpr int kStage = 128 * 16 * 4, kStages = 4;   // 16 columns of dQ on their way to the sum
 template <int D>
-constexpr int kPBuffers = D == 64 ? 2 : 1;
-template <int D>
-constexpr int bwd_smem_bytes() { return (4 + kDoStages<D>) * 128 * D * 2 + (1 + kPBuffers<D>) * 128 * 128 * 2 + 256 + 1024; }
+constexpr int bwd_smem_bytes() {
+  return (4 + kDoStages<D>) * 128 * D * 2 + 128 * 128 * 2 + kStages * kStage + (2 + kDoStages<D>) * 512 + 256 + 1024;
+}
 
+// Thread i of the warp receives 16 consecutive columns of row (lane_base + i).
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 rows x 64 columns of fp32 in the layout of matrix fragments: thread t receives, for each 8 columns j, columns 8 j + 2 (t % 4) and
+// the one behind it of row t / 4 (x[4 j], x[4 j + 1]) and of row t / 4 + 8 (x[4 j + 2], x[4 j + 3]).
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&x)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 rows x 32 columns of pairs of 16-bit values: thread t gives, for each 4 columns j, column 4 j + t % 4 of row t / 4 (x[2 j]) and of
+// row t / 4 + 8 (x[2 j + 1]): the pairs that tmem_ld_16x64 gave it.
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t (&x)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
+      : "memory");
+}
+// Four 8 x 8 matrices of 16-bit values in the same layout to shared memory; lane l names row l % 8 of matrix l / 8.
+__device__ __forceinline__ void store_matrices(const void* row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint32_t pack(uint32_t a, uint32_t b) {
+  const elem2_t h = ff2e2(__uint_as_float(a), __uint_as_float(b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// `bytes` of shared memory to global memory, or added to fp32 values there; both addresses on 16-byte boundaries.
+__device__ __forceinline__ void bulk_store(float* dst, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(__cvta_generic_to_global(dst)), "r"(smem_u32(smem_src)),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_add(float* dst, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.reduce.async.bulk.global.shared::cta.bulk_group.add.f32 [%0], [%1], %2;" ::"l"(__cvta_generic_to_global(dst)),
+               "r"(smem_u32(smem_src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ int load_acquire(const int* at) {
   int v;
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
@@ -101,6 +163,62 @@ __device__ __forceinline__ void store_release(int* at, int v) {
   asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(at), "r"(v) : "memory");
 }
 
+// Sums of several thread blocks in a fixed order, by whole warps: wait until `rank` contributions are in, add, hand on to the next.
+__device__ __forceinline__ bool reached(const int* counter, int rank) {
+  for (uint32_t spin = 0; spin < kSpinLimit; ++spin)
+    if (load_acquire(counter) >= rank) return true;
+  return false;
+}
+__device__ __forceinline__ bool wait_for(const int* counter, int rank) { return __all_sync(0xffffffffu, reached(counter, rank)); }
+// N columns of a row; a thread's 16-byte pieces lie PITCH pieces apart, so that a warp's are side by side.
+template <int PITCH, int N>
+__device__ __forceinline__ void store_part(float4* sum, const uint32_t (&r)[N]) {
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j)
+    __stcg(sum + j * PITCH, make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                                        __uint_as_float(r[4 * j + 3])));
+}
+template <int PITCH, int N>
+__device__ __forceinline__ void add_from(uint32_t (&r)[N], const float4* sum) {
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    const float4 v = __ldcg(sum + j * PITCH);
+    r[4 * j] = __float_as_uint(v.x + __uint_as_float(r[4 * j]));
+    r[4 * j + 1] = __float_as_uint(v.y + __uint_as_float(r[4 * j + 1]));
+    r[4 * j + 2] = __float_as_uint(v.z + __uint_as_float(r[4 * j + 2]));
+    r[4 * j + 3] = __float_as_uint(v.w + __uint_as_float(r[4 * j + 3]));
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_row(elem_t* dst, const uint32_t (&r)[N], float scale) {
+#pragma unroll
+  for (int j = 0; j < N; j += 8) {
+    __align__(16) elem2_t hh[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j + 2 * q]) * scale, __uint_as_float(r[j + 2 * q + 1]) * scale);
+    *reinterpret_cast<uint4*>(dst + j) = *reinterpret_cast<uint4*>(hh);
+  }
+}
+
+// The tiles that see a key block, and of which of them the parts of its walk consist.
+struct Walk {
+  int first, tiles, last_part;
+};
+__device__ __forceinline__ Walk walk_of(const BwdParams& p, int kb, int len) {
+  const int k0 = kb * kKeys, end = kb < p.firsts ? len : min(len, k0 + kKeys - 1 + p.window);
+  Walk w;
+  w.first = k0 / p.tile_tokens;
+  w.tiles = k0 < len ? (end + p.tile_tokens - 1) / p.tile_tokens - w.first : 0;
+  const int part = kb < p.firsts ? p.first_part_tiles : p.part_tiles;
+  w.last_part = w.tiles > 0 ? (w.tiles + part - 1) / part - 1 : 0;
+  return w;
+}
+__device__ __forceinline__ long long slot_of(const BwdParams& p, int bh, int kb, int part) {
+  if (kb < p.firsts) return ((long long)bh * p.firsts + kb) * p.first_parts + part;
+  const long long behind = p.first_parts > 1 ? (long long)p.B * p.kv_heads * p.firsts * p.first_parts : 0;
+  return behind + ((long long)bh * (p.blocks - p.firsts) + kb - p.firsts) * p.parts + part;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -108,8 +226,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                   const __grid_constant__ BwdParams p) {
   constexpr int DP = D / 64;
   constexpr int kTile = 128 * D * 2;           // a 128-row x D operand tile
-  constexpr int kSq = 128 * 128 * 2;           // P / dS tiles
-  constexpr int DOS = kDoStages<D>, PB = kPBuffers<D>;
+  constexpr int kSq = 128 * 128 * 2;           // dS tile
+  constexpr int DOS = kDoStages<D>;
   constexpr bool kOwnDq = D == 64;             // dQ has tensor-memory columns of its own
   constexpr uint32_t kTmemCols = 512;
   extern __shared__ uint8_t smem_raw[];
@@ -118,48 +236,52 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint8_t* sV = sK + kTile;
   uint8_t* sQ = sV + kTile;                    // two stages
   uint8_t* sDO = sQ + 2 * kTile;               // DOS stages
-  uint8_t* sP = sDO + DOS * kTile;
-  uint8_t* sDS = sP + PB * kSq;                // P: PB buffers
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sDS + kSq);
+  uint8_t* sDS = sDO + DOS * kTile;
+  uint8_t* sStage = sDS + kSq;                 // kStages
+  float* sL = reinterpret_cast<float*>(sStage + kStages * kStage);   // two stages of 128: minus lse
+  float* sD = sL + 2 * 128;                    // DOS stages: minus delta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + DOS * 128);
   uint64_t* kv_full = bars;
   uint64_t* q_full = bars + 1;      // [2]
   uint64_t* do_full = bars + 3;     // [2]
   uint64_t* q_free = bars + 5;      // [2] dK(i) has read the stage
-  uint64_t* do_free = bars + 7;     // [2] dV(i) has read the stage
+  uint64_t* do_free = bars + 7;     // [2] dP(i) and dV(i) have read the stage, and the point-wise warps delta (9)
   uint64_t* s_full = bars + 9;      // S(i) in tensor memory
   uint64_t* dp_full = bars + 10;    // dP(i) in tensor memory
-  uint64_t* p_ready = bars + 11;    // P(i) stored, S(i) read (16 warps)
-  uint64_t* ds_ready = bars + 12;   // dS(i) stored, dP(i) read (16 warps)
-  uint64_t* dv_done = bars + 13;    // [2] dV(i) has read the P buffer
-  uint64_t* dq_full = bars + 15;    // dQ(i) in tensor memory
-  uint64_t* dq_read = bars + 16;    // dQ(i) drained (4 warps)
-  uint64_t* dk_done = bars + 17;    // dQ(i) and dK(i) have read dS; all products so far are complete
-  uint64_t* kv_clean = bars + 18;   // K and V rows behind the sequence's end are zeros (16 warps)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* p_ready = bars + 11;    // P(i) stored over S(i) (8 warps)
+  uint64_t* ds_ready = bars + 12;   // dS(i) stored, dP(i) read (8 warps)
+  uint64_t* dq_full = bars + 13;    // dQ(i) in tensor memory
+  uint64_t* dq_read = bars + 14;    // dQ(i) taken out (4 warps)
+  uint64_t* dk_done = bars + 15;    // dQ(i) and dK(i) have read dS; all products so far are complete
+  uint64_t* kv_clean = bars + 16;   // K and V rows behind the sequence's end are zeros (8 warps)
+  uint64_t* staged = bars + 17;     // [tile's turn][kStages] a stage is full (4 warps)
+  uint64_t* stage_free = staged + 2 * kStages;   // [kStages] the copy engine has read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stage_free + kStages);
   int* my_ticket = reinterpret_cast<int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     *my_ticket = atomicAdd(p.ticket, 1);
     prefetch_tensormap(&map_q); prefetch_tensormap(&map_k); prefetch_tensormap(&map_v); prefetch_tensormap(&map_do);
-    for (int i = 0; i < 19; ++i) mbar_init(&bars[i], i == 11 || i == 12 || i == 18 ? 16 : i == 16 ? 4 : 1);
+    for (int i = 0; i < 17 + 3 * kStages; ++i)
+      mbar_init(&bars[i], i == 7 || i == 8 ? 9 : i == 11 || i == 12 || i == 16 ? 8 : i == 14 || (i >= 17 && i < 17 + 2 * kStages) ? 4 : 1);
     mbar_fence_init();
   }
   __syncthreads();
-  const int ticket = *my_ticket;
-  const int bhs = p.B * p.kv_heads, nkb = (p.T + kKeys - 1) / kKeys;
-  const int ns = min((p.sinks + kKeys - 1) / kKeys, nkb);          // blocks of first tokens
-  const int nth = ticket / bhs, bh = ticket % bhs;
-  const int kb = nth < ns ? nth : nkb - 1 - (nth - ns);
+  const int ticket = __shfl_sync(0xffffffffu, *my_ticket, 0);      // the same in all lanes: what follows from it takes uniform registers
+  const int bhs = p.B * p.kv_heads, ns = p.firsts;
+  const int bh = ticket % bhs, behind = ticket / bhs - (p.blocks - ns) * p.parts;   // 0 or more: a block of first tokens
+  const int kb = behind < 0 ? p.blocks - 1 - ticket / bhs / p.parts : ns - 1 - behind / p.first_parts;
+  const int part_at = behind < 0 ? ticket / bhs % p.parts : behind % p.first_parts;
+  const int part_tiles = behind < 0 ? p.part_tiles : p.first_part_tiles;
   const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
   const int k0 = kb * kKeys;
   const int len = p.lengths == nullptr ? p.T : min(max(p.lengths[b], 0), p.T);
-  const bool first_block = kb < ns;
-  const int m_lo = k0 / p.tile_tokens, tok_end = first_block ? len : min(len, k0 + kKeys - 1 + p.window);
-  const int m_hi = (tok_end + p.tile_tokens - 1) / p.tile_tokens;
-  const int n = k0 < len ? m_hi - m_lo : 0;                        // tiles that see the block
-  auto tile_of = [&](int i) { return first_block ? m_hi - 1 - i : m_lo + i; };
-  if (n <= 0) {                                                    // keys behind the sequence's end
+  const Walk walk = walk_of(p, kb, len);
+  const int last_part = walk.last_part;
+  if (part_at > last_part) return;
+  const int m0 = walk.first + part_at * part_tiles, n = min(part_tiles, walk.tiles - part_at * part_tiles);   // the tiles of this part
+  if (walk.tiles <= 0) {                                           // keys behind the sequence's end
     for (int i = threadIdx.x; i < kKeys * (D / 8) * 2; i += kBwdThreads) {
       const int which = i & 1, r = (i >> 1) / (D / 8), d = (i >> 1) % (D / 8) * 8;
       if (k0 + r < p.T) {
@@ -180,7 +302,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
     fence_proxy_async_smem();
   }
-  if (warp == 20) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
+  if (warp == 12) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -188,7 +310,18 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const uint32_t tm_s = tmem, tm_dp = tmem + 128, tm_dv = tmem + 256, tm_dk = tmem + 256 + D;
   const uint32_t tm_dq = kOwnDq ? tmem + 256 + 2 * D : tm_dp;
 
-  if (warp == 21) {
+  // the key blocks that add to a tile: hi down to lo, then those of the first tokens; ours is number `rank` of 0 to `last`
+  auto order = [&](int m, int& rank, int& last) {
+    const int t0 = m * p.tile_tokens, t1 = min(t0 + p.tile_tokens, len) - 1;
+    const int hi = t1 / kKeys, firsts = min(ns, hi + 1), near = hi + 1 - max(max(0, t0 - p.window + 1) / kKeys, firsts);
+    rank = kb >= ns ? hi - kb : near + firsts - 1 - kb;
+    last = near + firsts - 1;
+  };
+
+  // Registers go where the scores are: four warps of 96, four of 144 and eight of 136 of the 128 a thread that the block was launched with.
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+  if (warp == 13) {
     if (elect_one()) {
       bool ok = true;
       auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int t) {
@@ -197,14 +330,16 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       };
       auto load_q = [&](int i) {
         if (i >= 2 && !mbar_wait(&q_free[i & 1], ((i >> 1) - 1) & 1)) { ok = false; return; }
-        mbar_expect_tx(&q_full[i & 1], used * D * 2);
-        load(sQ + (i & 1) * kTile, &map_q, &q_full[i & 1], kvh * p.group, tile_of(i) * p.tile_tokens);
+        mbar_expect_tx(&q_full[i & 1], used * D * 2 + 512);
+        bulk_load(sL + (i & 1) * 128, p.lse + ((long long)bh * p.tiles + m0 + i) * kRows, 512, &q_full[i & 1]);
+        load(sQ + (i & 1) * kTile, &map_q, &q_full[i & 1], kvh * p.group, (m0 + i) * p.tile_tokens);
       };
       auto load_do = [&](int i) {
         const int s = i % DOS;
         if (i >= DOS && !mbar_wait(&do_free[s], (i / DOS - 1) & 1)) { ok = false; return; }
-        mbar_expect_tx(&do_full[s], used * D * 2);
-        load(sDO + s * kTile, &map_do, &do_full[s], kvh * p.group, tile_of(i) * p.tile_tokens);
+        mbar_expect_tx(&do_full[s], used * D * 2 + 512);
+        bulk_load(sD + s * 128, p.delta + ((long long)bh * p.tiles + m0 + i) * kRows, 512, &do_full[s]);
+        load(sDO + s * kTile, &map_do, &do_full[s], kvh * p.group, (m0 + i) * p.tile_tokens);
       };
       mbar_expect_tx(kv_full, 2 * kTile);
       load(sK, &map_k, kv_full, kvh, k0);
@@ -218,51 +353,45 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
     }
-  } else if (warp == 20) {
+  } else if (warp == 12) {
     if (elect_one()) {
       bool ok = true;
-      const uint32_t id_s = make_idesc_f16kind(128, 128, false, false);   // S = Q K^T, dP = dO V^T
-      const uint32_t id_t = make_idesc_f16kind(128, D, true, true);       // dV = P^T dO, dK = dS^T Q (A, B MN-major)
-      const uint32_t id_q = make_idesc_f16kind(128, D, false, true);      // dQ = dS K (B MN-major)
-      const uint32_t aK = smem_u32(sK), aV = smem_u32(sV), aP = smem_u32(sP), aDS = smem_u32(sDS);
-      auto scores = [&](uint32_t d, uint32_t a, uint32_t bb) {            // both operands K-major over D
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * 128 * 128 + (k % 4) * 32;
-          mma_f16_ss(d, make_smem_desc_sw128(a + off, 16, 1024), make_smem_desc_sw128(bb + off, 16, 1024), id_s, k != 0);
-        }
-      };
-      auto transposed = [&](uint32_t d, uint32_t a, uint32_t bb, bool first) {
-        // K dimension = queries, 16 rows per step.  A (P or dS) is [query rows][keys]: as an MN-major operand its M = keys
-#pragma unroll
-        for (int k = 0; k < 128 / 16; ++k)
-          mma_f16_ss(d, make_smem_desc_sw128(a + k * 16 * 128, 128 * 128, 1024),
-                     make_smem_desc_sw128(bb + k * 16 * 128, 128 * 128, 1024), id_t, !first || k != 0);
-      };
+      const uint32_t id_s = make_idesc_f16kind(128, 128, false, false);   // S^T = K Q^T, dP^T = V dO^T
+      const uint32_t id_t = make_idesc_f16kind(128, D, false, true);      // dV = P^T dO, dK = dS^T Q (B MN-major)
+      const uint32_t id_q = make_idesc_f16kind(128, D, true, true);       // dQ = dS K (A, B MN-major)
+      const uint64_t kK = k_major(smem_u32(sK)), kV = k_major(smem_u32(sV)), kQ = k_major(smem_u32(sQ)), kDO = k_major(smem_u32(sDO));
+      const uint64_t mK = mn_major(smem_u32(sK)), mQ = mn_major(smem_u32(sQ)), mDO = mn_major(smem_u32(sDO));
+      const uint64_t kDS = k_major(smem_u32(sDS)), mDS = mn_major(smem_u32(sDS));
+      constexpr uint64_t kNext = kTile >> 4;                              // to the next stage
       auto issue_s = [&](int i) {
         if (!mbar_wait(&q_full[i & 1], (i >> 1) & 1)) { ok = false; return; }
         fence_after_sync();
-        scores(tm_s, smem_u32(sQ + (i & 1) * kTile), aK);
+        const uint64_t b = kQ + (i & 1) * kNext;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) mma_f16_ss(tm_s, kK + k_step(k), b + k_step(k), id_s, k != 0);
         mma_commit(s_full);
       };
       auto issue_dp = [&](int i) {
         if (!mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; return; }
         fence_after_sync();
-        scores(tm_dp, smem_u32(sDO + (i % DOS) * kTile), aV);
+        const uint64_t b = kDO + (i % DOS) * kNext;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) mma_f16_ss(tm_dp, kV + k_step(k), b + k_step(k), id_s, k != 0);
         mma_commit(dp_full);
       };
       ok = mbar_wait(kv_full, 0) && mbar_wait(kv_clean, 0);
       if (ok) issue_s(0);
       if (ok) issue_dp(0);
       for (int i = 0; i < n && ok; ++i) {
-        if (!mbar_wait(p_ready, i & 1)) { ok = false; break; }
+        if (!mbar_wait(p_ready, i & 1) || !mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; break; }
         fence_after_sync();
-        if (i + 1 < n) issue_s(i + 1);
-        if (!ok) break;
-        transposed(tm_dv, aP + (i % PB) * kSq, smem_u32(sDO + (i % DOS) * kTile), i == 0);
-        mma_commit(&dv_done[i % PB]);
+        const uint64_t bDO = mDO + (i % DOS) * kNext, bQ = mQ + (i & 1) * kNext;
+#pragma unroll
+        for (int k = 0; k < 128 / 16; ++k)     // the 16-bit values of 64 queries lie in the first 32 columns of their scores
+          mma_f16_ts(tm_dv, tm_s + (k / 4) * 64 + (k % 4) * 8, bDO + mn_step(k), id_t, i != 0 || k != 0);
         mma_commit(&do_free[i % DOS]);
-        if (!mbar_wait(ds_ready, i & 1)) { ok = false; break; }
+        if (ok && i + 1 < n) issue_s(i + 1);
+        if (!ok || !mbar_wait(ds_ready, i & 1)) { ok = false; break; }
         fence_after_sync();
         if (kOwnDq) {
           if (i + 1 < n) issue_dp(i + 1);
@@ -270,41 +399,78 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           fence_after_sync();
         }
 #pragma unroll
-        for (int k = 0; k < 128 / 16; ++k) {   // dQ = dS (K-major over keys) · K (MN-major: key rows, D contiguous)
-          const uint64_t a_ds = make_smem_desc_sw128(aDS + (k / 4) * 128 * 128 + (k % 4) * 32, 16, 1024);
-          const uint64_t b_k = make_smem_desc_sw128(aK + k * 16 * 128, 128 * 128, 1024);
-          mma_f16_ss(tm_dq, a_ds, b_k, id_q, k != 0);
-        }
+        for (int k = 0; k < 128 / 16; ++k)     // K dimension = keys; M = queries, two panels of 64
+          mma_f16_ss(tm_dq, mDS + mn_step(k), mK + mn_step(k), id_q, k != 0);
         mma_commit(dq_full);
-        transposed(tm_dk, aDS, smem_u32(sQ + (i & 1) * kTile), i == 0);
+#pragma unroll
+        for (int k = 0; k < 128 / 16; ++k)     // K dimension = queries
+          mma_f16_ss(tm_dk, kDS + k_step(k), bQ + mn_step(k), id_t, i != 0 || k != 0);
         mma_commit(dk_done);
         mma_commit(&q_free[i & 1]);
         if (!kOwnDq && i + 1 < n) {
           if (!mbar_wait(dq_read, i & 1)) { ok = false; break; }
-          fence_after_sync();
           issue_dp(i + 1);
         }
       }
       if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
     }
+  } else if (warp >= 14) {
+    // ---------------------------------------------------------------- dQ to its tile's sum: every other tile that is not finished here
+    bool ok = true;
+    if (elect_one()) {
+      const int turn = warp - 14;
+      int nth = 0;                               // tiles of both turns so far
+      for (int i = 0; i < n && ok; ++i) {
+        int rank, last;
+        order(m0 + i, rank, last);
+        if (rank == last || (nth++ & 1) != turn) continue;
+        const long long tile = (long long)bh * p.tiles + m0 + i;
+        if (rank > 0) {
+          if (!reached(p.counters + tile, rank)) { ok = false; break; }
+          fence_proxy_async_all();
+        }
+        for (int c = 0; c < D / 16; ++c) {
+          if (!mbar_wait(&staged[turn * kStages + c % kStages], ((nth - 1 >> 1) * (D / 64) + c / kStages) & 1)) { ok = false; break; }
+          float* dst = p.sums + (tile * (D / 16) + c) * (kStage / 4);
+          const uint8_t* src = sStage + c % kStages * kStage;
+          if (rank == 0) bulk_store(dst, src, kStage); else bulk_add(dst, src, kStage);
+          bulk_commit_group();
+          if (c > 1) {                           // all copies but the last two have read their stages
+            bulk_wait_group_read<2>();
+            mbar_arrive(&stage_free[(c - 2) % kStages]);
+          }
+        }
+        if (!ok) break;
+        bulk_wait_group_read<1>();
+        mbar_arrive(&stage_free[kStages - 2]);
+        bulk_wait_group_read<0>();
+        mbar_arrive(&stage_free[kStages - 1]);
+        bulk_wait_group_all();
+        fence_proxy_async_all();
+        __threadfence();
+        store_release(p.counters + tile, rank + 1);
+      }
+      if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
+    }
+  }
   } else if (warp >= 4) {
-    // ---------------------------------------------------------------- point-wise: one row, 32 keys per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    // ---------------------------------------------------------------- point-wise: 32 keys and 64 queries per warp
+    // In the fragment layout a thread has 16 of the 64 queries (of four keys), so it fetches 16 values of lse and of delta.  With a key a
+    // thread it needed all 64, the same in all lanes: 1 024 cycles of shared memory a tile, which the products keep busy.
     const int lane_group = warp & 3, part = (warp - 4) >> 2;
-    const int row = lane_group * 32 + lane;
-    const int token = row / p.group;                 // tile_tokens or more: no row
+    const int row = lane_group * 32 + lane, key = k0 + row;
     const uint32_t lane_addr = uint32_t(lane_group * 32) << 16;
-    const long long stat0 = (long long)bh * p.T * p.group;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-    uint8_t* pRow = sP + (part >> 1) * 128 * 128;      // the 64-key panel
-    uint8_t* dsRow = sDS + (part >> 1) * 128 * 128;
-    const int chunk0 = (part & 1) * 4;                 // first 16-byte piece of the panel row
+    uint8_t* dsPanel = sDS + part * 128 * 128;         // 64 queries
+    const int my_row = lane_group * 32 + (lane >> 3 & 1) * 8 + (lane & 7), my_chunk = lane >> 4;   // as an address of store_matrices
     bool ok = true;
     if (k0 + kKeys > len && len < p.T) {
       // K and V behind the sequence's end may hold anything: 0 x NaN is NaN in the products over keys
       ok = mbar_wait(kv_full, 0);
       if (ok && k0 + row >= len) {
 #pragma unroll
-        for (int j = part; j < DP * 8; j += 4) {
+        for (int j = part; j < DP * 8; j += 2) {
           const int at = (j / 8) * 128 * 128 + row * 128 + (j % 8) * 16;
           *reinterpret_cast<uint4*>(sK + at) = make_uint4(0u, 0u, 0u, 0u);
           *reinterpret_cast<uint4*>(sV + at) = make_uint4(0u, 0u, 0u, 0u);
@@ -313,218 +479,264 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       fence_proxy_async_smem();
     }
     warp_arrive(kv_clean);
-    float lse_next = 0.0f, dl_next = 0.0f;             // statistics of the next tile: fetched one tile ahead
-    auto fetch = [&](int i) {
-      const int t = tile_of(i) * p.tile_tokens + token;
-      if (i < n && token < p.tile_tokens && t < len) {
-        const long long at = stat0 + (long long)t * p.group + (row - token * p.group);
-        lse_next = p.lse[at];
-        dl_next = p.delta[at];
-      } else {
-        lse_next = dl_next = 0.0f;
-      }
+    // lse is fetched a tile ahead, and delta before P is handed to the products.
+    float2 ahead[8];
+    auto fetch = [&](const float* from) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ahead[j] = *reinterpret_cast<const float2*>(from + part * 64 + j * 8 + (lane & 3) * 2);
     };
-    fetch(0);
+    if (ok) ok = mbar_wait(&q_full[0], 0);               // lse comes with Q
+    if (ok) fetch(sL);
     for (int i = 0; i < n && ok; ++i) {
-      const int t0 = tile_of(i) * p.tile_tokens, t_q = t0 + token;
-      const bool row_ok = token < p.tile_tokens && t_q < len;
-      const float nl = -lse_next, dl = dl_next;
-      fetch(i + 1);
-      const float2 nl2 = make_float2(nl, nl);
-      // which of its 32 keys the row sees
-      uint32_t seen = 0xffffffffu;
-      if (k0 + kKeys - 1 > t0 || (k0 <= t0 + p.tile_tokens - 1 - p.window && k0 + kKeys > p.sinks) || t0 + p.tile_tokens > len ||
-          used < kRows) {
-        const int kk = k0 + part * 32;
-        auto below = [](int c) { return c <= 0 ? 0u : c >= 32 ? 0xffffffffu : (1u << c) - 1u; };
-        seen = row_ok ? below(t_q + 1 - kk) & (~below(t_q - p.window + 1 - kk) | below(p.sinks - kk)) : 0u;
-      }
+      const int t0 = (m0 + i) * p.tile_tokens;
+      const int rows = min(p.tile_tokens, len - t0) * p.group;     // rows of the tile that are queries
+      const bool edge = k0 + kKeys - 1 > t0 || (k0 <= t0 + p.tile_tokens - 1 - p.window && k0 + kKeys > p.sinks) || rows < kRows;
       if (!mbar_wait(s_full, i & 1)) { ok = false; break; }
       fence_after_sync();
       if (t0 + p.tile_tokens > len && len < p.T) {
         // Q and dO behind the sequence's end, operands of the products over queries.  S(i) has read Q; dP(i) may be reading dO, but
         // only rows whose dS is set to zero below.
         if (!mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; break; }
-        if (!row_ok) {
+        if (row >= rows) {
 #pragma unroll
-          for (int j = part; j < DP * 8; j += 4) {
+          for (int j = part; j < DP * 8; j += 2) {
             const int at = (j / 8) * 128 * 128 + row * 128 + (j % 8) * 16;
             *reinterpret_cast<uint4*>(sQ + (i & 1) * kTile + at) = make_uint4(0u, 0u, 0u, 0u);
             *reinterpret_cast<uint4*>(sDO + (i % DOS) * kTile + at) = make_uint4(0u, 0u, 0u, 0u);
           }
+          fence_proxy_async_smem();
         }
       }
-      uint32_t r[32];
-      float pr[32];
-      tmem_ld_32x32(tm_s + lane_addr + part * 32, r);
+      // sets what a query does not see to zero: of the thread's 64 values those of key k and query c that are not in [from, to)
+      auto mask = [&](uint32_t (&x)[2][32]) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int k = k0 + lane_group * 32 + r4 * 8 + (lane >> 2), c0 = part * 64 + (lane & 3) * 2;
+          const int from = max(0, k - t0) * p.group;                                     // t >= k
+          const int to = k < p.sinks ? rows : min(rows, max(0, min(k - t0 + p.window, p.tile_tokens)) * p.group);   // t < k + window
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = c0 + j * 8 + e;
+              if (c < from || c >= to) x[r4 >> 1][j * 4 + (r4 & 1) * 2 + e] = 0u;
+            }
+        }
+      };
+      uint32_t pr[2][32];                                // scores, then P, then dS, as fp32 bits: 16 keys each
+#pragma unroll
+      for (int h = 0; h < 2; ++h) tmem_ld_16x64(tm_s + lane_addr + (uint32_t(h * 16) << 16) + part * 64, pr[h]);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        const float2 e = __ffma2_rn(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), sc2, nl2);
-        pr[j] = fast_exp2(e.x);
-        pr[j + 1] = fast_exp2(e.y);
-      }
-      if (seen != 0xffffffffu) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (!(seen >> j & 1u)) pr[j] = 0.0f;
-      }
-      // dV(i - PB) has read the buffer
-      if (i >= PB && !mbar_wait(&dv_done[i % PB], (i / PB - 1) & 1)) { ok = false; break; }
+        for (int j = 0; j < 32; j += 2) {
+          const float2 e = __ffma2_rn(make_float2(__uint_as_float(pr[h][j]), __uint_as_float(pr[h][j + 1])), sc2, ahead[j / 4]);
+          pr[h][j] = __float_as_uint(fast_exp2(e.x));
+          pr[h][j + 1] = __float_as_uint(fast_exp2(e.y));
+        }
+      if (edge) mask(pr);
       // P and dS are rounded to 16 bits as operands of the products
 #pragma unroll
-      for (int j8 = 0; j8 < 4; ++j8) {
-        __align__(16) elem2_t hp[4];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t packed[16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) hp[q] = ff2e2(pr[j8 * 8 + 2 * q], pr[j8 * 8 + 2 * q + 1]);
-        *reinterpret_cast<uint4*>(pRow + (i % PB) * kSq + swz(row, chunk0 + j8)) = *reinterpret_cast<uint4*>(hp);
+        for (int j = 0; j < 16; ++j) packed[j] = pack(pr[h][2 * j], pr[h][2 * j + 1]);
+        tmem_st_16x32(tm_s + lane_addr + (uint32_t(h * 16) << 16) + part * 64, packed);
       }
-      fence_proxy_async_smem();
+      tmem_st_wait();
+      if (!mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; break; }   // delta comes with dO
+      fetch(sD + (i % DOS) * 128);
       fence_before_sync();
       warp_arrive(p_ready);
+      warp_arrive(&do_free[i % DOS]);
       if (!mbar_wait(dp_full, i & 1)) { ok = false; break; }
       fence_after_sync();
-      tmem_ld_32x32(tm_dp + lane_addr + part * 32, r);
-      tmem_ld_wait();
+      if (i > 0 && !mbar_wait(dk_done, (i - 1) & 1)) { ok = false; break; }      // dQ(i-1), dK(i-1) have read dS
+      {
+        uint32_t dp[2][32];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) pr[j] = pr[j] * (__uint_as_float(r[j]) - dl) * p.scale;
-      if (seen != 0xffffffffu) {
+        for (int h = 0; h < 2; ++h) tmem_ld_16x64(tm_dp + lane_addr + (uint32_t(h * 16) << 16) + part * 64, dp[h]);
+        tmem_ld_wait();
+        // dS without the scale: dQ and dK are scaled once, at their ends
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (!(seen >> j & 1u)) pr[j] = 0.0f;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 d = __fmul2_rn(make_float2(__uint_as_float(pr[h][j]), __uint_as_float(pr[h][j + 1])),
+                                        __fadd2_rn(make_float2(__uint_as_float(dp[h][j]), __uint_as_float(dp[h][j + 1])), ahead[j / 4]));
+            pr[h][j] = __float_as_uint(d.x);
+            pr[h][j + 1] = __float_as_uint(d.y);
+          }
       }
-      if (i > 0 && !mbar_wait(dk_done, (i - 1) & 1)) { ok = false; break; }   // dQ(i-1), dK(i-1) have read dS
+      if (rows < kRows) mask(pr);                        // behind the last query dO and delta may be anything
 #pragma unroll
-      for (int j8 = 0; j8 < 4; ++j8) {
-        __align__(16) elem2_t hd[4];
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) hd[q] = ff2e2(pr[j8 * 8 + 2 * q], pr[j8 * 8 + 2 * q + 1]);
-        *reinterpret_cast<uint4*>(dsRow + swz(row, chunk0 + j8)) = *reinterpret_cast<uint4*>(hd);
-      }
+        for (int j = 0; j < 8; j += 2)                   // 8 queries j and the next 8
+          store_matrices(dsPanel + swz(my_row + h * 16, j + my_chunk), pack(pr[h][4 * j], pr[h][4 * j + 1]), pack(pr[h][4 * j + 2], pr[h][4 * j + 3]),
+                         pack(pr[h][4 * j + 4], pr[h][4 * j + 5]), pack(pr[h][4 * j + 6], pr[h][4 * j + 7]));
       fence_proxy_async_smem();
       fence_before_sync();
       warp_arrive(ds_ready);
+      if (i + 1 < n) {
+        if (!mbar_wait(&q_full[(i + 1) & 1], ((i + 1) >> 1) & 1)) { ok = false; break; }
+        fetch(sL + ((i + 1) & 1) * 128);
+      }
     }
-    // dV (parts 0, 1) and dK (parts 2, 3) of this key block, half of the columns each
+    // dV (part 0) and dK (part 1) of this key block
     if (ok && mbar_wait(dk_done, (n - 1) & 1)) {
       fence_after_sync();
-      const int t_k = k0 + row;
-      elem_t* dst = part < 2 ? p.dv + b * p.v_sb + t_k * p.v_st + kvh * p.v_sh : p.dk + b * p.k_sb + t_k * p.k_st + kvh * p.k_sh;
-      const uint32_t src = part < 2 ? tm_dv : tm_dk;
+      const int t_k = key;
+      elem_t* dst = part == 0 ? p.dv + b * p.v_sb + t_k * p.v_st + kvh * p.v_sh : p.dk + b * p.k_sb + t_k * p.k_st + kvh * p.k_sh;
+      const uint32_t src = part == 0 ? tm_dv : tm_dk;
+      float4* to = p.kv_parts + (slot_of(p, bh, kb, part_at) * 2 + part) * (D / 4) * kKeys + row;
 #pragma unroll 1
-      for (int c0 = (part & 1) * (D / 2); c0 < ((part & 1) + 1) * (D / 2); c0 += 32) {
+      for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t r[32];
         tmem_ld_32x32(src + lane_addr + c0, r);
         tmem_ld_wait();
-        if (t_k < p.T) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            __align__(16) elem2_t hh[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j + 2 * q]), __uint_as_float(r[j + 2 * q + 1]));
-            *reinterpret_cast<uint4*>(dst + c0 + j) = *reinterpret_cast<uint4*>(hh);
-          }
-        }
+        if (last_part > 0)
+          store_part<kKeys>(to + c0 / 4 * kKeys, r);
+        else if (t_k < p.T)
+          store_row(dst + c0, r, part == 0 ? 1.0f : p.scale);
       }
     } else {
       ok = false;
     }
     if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // ---------------------------------------------------------------- dQ: one row per thread
     const int row = warp * 32 + lane, token = row / p.group;
     const uint32_t lane_addr = uint32_t(warp * 32) << 16;
     const int h = kvh * p.group + (row - token * p.group);
     bool ok = true;
+    int f = 0;                                           // tiles that went through the stages so far: the finishing warps take turns
     for (int i = 0; i < n && ok; ++i) {
-      const int m = tile_of(i), t0 = m * p.tile_tokens, t1 = min(t0 + p.tile_tokens, len) - 1, t_q = t0 + token;
-      const bool row_ok = token < p.tile_tokens && t_q < len;
-      // the key blocks that add to this tile: [0, firsts), then hi down to lo
-      const int hi = t1 / kKeys, firsts = min(ns, hi + 1), lo = max(max(0, t0 - p.window + 1) / kKeys, firsts);
-      const int rank = first_block ? kb : firsts + hi - kb, last = firsts + (hi - lo + 1) - 1;
-      int* counter = p.counters + ((long long)bh * p.tiles + m) * 4 + warp;
-      float4* sum = p.sums + ((long long)bh * p.tiles + m) * (D / 4) * kRows + row;
-      elem_t* dst = p.dq + b * p.q_sb + t_q * p.q_st + h * p.q_sh;
-      if (!mbar_wait(dq_full, i & 1)) { ok = false; break; }
-      fence_after_sync();
-      if (rank > 0) {
-        bool in = false;
-        for (uint32_t spin = 0; spin < kSpinLimit && !in; ++spin) in = load_acquire(counter) >= rank;
-        if (!__all_sync(0xffffffffu, in)) { ok = false; break; }
-      }
-#pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32(tm_dq + lane_addr + c0, r);
+      const int t_q = (m0 + i) * p.tile_tokens + token;
+      int rank, last;
+      order(m0 + i, rank, last);
+      if (rank < last) {
+        if (!mbar_wait(dq_full, i & 1)) { ok = false; break; }
+        fence_after_sync();
+        // all columns go into registers, so that they are free again before anything has left
+        uint32_t r[D / 32][32];
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) tmem_ld_32x32(tm_dq + lane_addr + c * 32, r[c]);
         tmem_ld_wait();
-        if (c0 + 32 == D) {      // all of dQ(i) has been read: the columns may be written again
-          fence_before_sync();
-          warp_arrive(dq_read);
+        fence_before_sync();
+        warp_arrive(dq_read);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          const int fill = f * (D / 64) + c / kStages;
+          if (fill > 0 && !mbar_wait(&stage_free[c % kStages], (fill - 1) & 1)) { ok = false; break; }
+          uint8_t* at = sStage + c % kStages * kStage + row * 16;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t* x = r[c / 2] + c % 2 * 16 + 4 * j;
+            *reinterpret_cast<uint4*>(at + j * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+          fence_proxy_async_smem();
+          warp_arrive(&staged[(f & 1) * kStages + c % kStages]);
         }
-        float4* at = sum + c0 / 4 * kRows;
-        if (rank == last) {
-          if (rank > 0) {
+        ++f;
+      } else {
+        const long long tile = (long long)bh * p.tiles + m0 + i;
+        const float4* sum = reinterpret_cast<const float4*>(p.sums) + tile * (D / 4) * kRows + row;
+        if (!mbar_wait(dq_full, i & 1)) { ok = false; break; }
+        fence_after_sync();
+        elem_t* dst = p.dq + b * p.q_sb + t_q * p.q_st + h * p.q_sh;
+        uint32_t r[D / 16][16];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 v = __ldcg(at + j * kRows);
-              r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) + v.x);
-              r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) + v.y);
-              r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) + v.z);
-              r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) + v.w);
-            }
-          }
-          if (row_ok) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              __align__(16) elem2_t hh[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j + 2 * q]), __uint_as_float(r[j + 2 * q + 1]));
-              *reinterpret_cast<uint4*>(dst + c0 + j) = *reinterpret_cast<uint4*>(hh);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 v = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
-                                         __uint_as_float(r[4 * j + 3]));
-            if (rank == 0) __stcg(at + j * kRows, v); else atomicAdd(at + j * kRows, v);
-          }
+        for (int c = 0; c < D / 16; ++c) tmem_ld_32x16(tm_dq + lane_addr + c * 16, r[c]);
+        tmem_ld_wait();
+        fence_before_sync();
+        warp_arrive(dq_read);
+        if (rank > 0) {
+          if (!wait_for(p.counters + tile, rank)) { ok = false; break; }
+          fence_proxy_async_all();
         }
-      }
-      if (rank != last) {
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) store_release(counter, rank + 1);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          if (rank > 0) add_from<kRows>(r[c], sum + c * 4 * kRows);
+          if (token < p.tile_tokens && t_q < len) store_row(dst + c * 16, r[c], p.scale);
+        }
       }
     }
     if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 20) { fence_after_sync(); tmem_dealloc(tmem, kTmemCols); }
+  if (warp == 12) { fence_after_sync(); tmem_dealloc(tmem, kTmemCols); }
 }
 
-// Floats of the parts of the workspace: sums of dQ (none where no tile has two key blocks), counters and the ticket, delta.
-struct Workspace {
-  long long sums, counters, delta;
-};
-Workspace workspace(long long B, long long T, long long kv_heads, long long group, int D) {
-  const long long tile_tokens = kRows / group, tiles = (T + tile_tokens - 1) / tile_tokens;
-  Workspace w;
-  w.sums = T <= kKeys ? 0 : B * kv_heads * tiles * kRows * D;
-  w.counters = (B * kv_heads * tiles * 4 + 1 + 3) / 4 * 4;
-  w.delta = B * kv_heads * T * group;
-  return w;
+// dK and dV of the key blocks whose walks were divided: the parts' sums in their order.  A thread a row's four columns.
+template <int D>
+__global__ void __launch_bounds__(256) window_parts_kernel(const __grid_constant__ BwdParams p, int kb0, int count) {
+  const int kb = kb0 + blockIdx.x % count, bh = blockIdx.x / count, which = blockIdx.y;      // which: dV, dK
+  const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
+  const int len = p.lengths == nullptr ? p.T : min(max(p.lengths[b], 0), p.T);
+  const Walk walk = walk_of(p, kb, len);
+  if (walk.last_part == 0) return;                   // one part, or none: written by the main kernel
+  const int i = blockIdx.z * 256 + threadIdx.x, row = i % kKeys, piece = i / kKeys, key = kb * kKeys + row;
+  const float4* at = p.kv_parts + slot_of(p, bh, kb, 0) * 2 * (D / 4) * kKeys + which * (D / 4) * kKeys + i;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int part = 0; part <= walk.last_part; ++part) {
+    const float4 v = __ldcg(at + (long long)part * 2 * (D / 4) * kKeys);
+    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+  }
+  if (key >= p.T) return;
+  const float scale = which ? p.scale : 1.0f;
+  elem_t* dst = which ? p.dk + b * p.k_sb + key * p.k_st + kvh * p.k_sh : p.dv + b * p.v_sb + key * p.v_st + kvh * p.v_sh;
+  __align__(8) elem2_t out[2] = {ff2e2(sum.x * scale, sum.y * scale), ff2e2(sum.z * scale, sum.w * scale)};
+  *reinterpret_cast<uint2*>(dst + piece * 4) = *reinterpret_cast<uint2*>(out);
 }
+
+// How the walks are divided, and the workspace in units of four bytes: sums of dQ (none where no tile has two key blocks), dK and dV
+// of the parts of divided walks, counters with the ticket, delta.
+struct Plan {
+  int tile_tokens, tiles, window, sinks, blocks, firsts, parts, part_tiles, first_parts, first_part_tiles;
+  long long sums, kv_parts, counters, delta, thread_blocks;
+};
+Plan make_plan(long long B, long long T, long long kv_heads, int group, int D, int window, int sinks) {
+  Plan a;
+  a.tile_tokens = kRows / group;
+  a.tiles = (int)((T + a.tile_tokens - 1) / a.tile_tokens);
+  a.window = window < 1 || window > kNoWindow ? kNoWindow : window;   // 0: none
+  a.sinks = a.window == kNoWindow ? 0 : sinks < kNoWindow ? sinks : kNoWindow;
+  a.blocks = (int)((T + kKeys - 1) / kKeys);
+  const long long first_blocks = ((long long)a.sinks + kKeys - 1) / kKeys;
+  a.firsts = (int)(first_blocks < a.blocks ? first_blocks : a.blocks);
+  // tiles of the longest walks, and how many of them the machine's 148 multiprocessors take each
+  const long long reach = ((long long)kKeys - 1 + a.window) / a.tile_tokens + 2;
+  const long long walk = a.tiles < reach ? a.tiles : reach;
+  const long long steps = (((long long)a.blocks - a.firsts) * walk + (long long)a.firsts * a.tiles) * B * kv_heads / 148;
+  auto divide = [](long long longest, long long share, int& parts, int& tiles) {
+    tiles = (int)(share < 8 ? 8 : share);
+    parts = (int)((longest + tiles - 1) / tiles);
+  };
+  divide(walk, steps / 2, a.parts, a.part_tiles);
+  divide(a.tiles, (long long)a.firsts * a.tiles * B * kv_heads / 296, a.first_parts, a.first_part_tiles);     // two a multiprocessor
+  const long long bh = B * kv_heads;
+  a.sums = a.blocks < 2 ? 0 : bh * a.tiles * kRows * D;
+  a.kv_parts = ((a.first_parts > 1 ? (long long)a.firsts * a.first_parts : 0) + (a.parts > 1 ? (long long)(a.blocks - a.firsts) * a.parts : 0)) *
+               bh * 2 * kKeys * D;
+  a.counters = bh * a.tiles;
+  a.delta = bh * a.tiles * kRows;
+  a.thread_blocks = bh * ((long long)(a.blocks - a.firsts) * a.parts + (long long)a.firsts * a.first_parts);
+  return a;
+}
+long long zeroed(const Plan& a) { return (a.counters + 1 + 3) / 4 * 4; }     // counters and the ticket
 
 }  // namespace
 
 extern "C" {
 
-long long fbam_window_bwd_workspace(int B, int T, int kv_heads, int group, int D) {
-  if (group < 1 || group > kRows) return 0;
-  const Workspace w = workspace(B, T, kv_heads, group, D);
-  return w.sums + w.counters + w.delta;
+long long fbam_window_bwd_workspace(int B, int T, int kv_heads, int group, int D, int window, int sinks) {
+  if (group < 1 || group > kRows || B < 1 || T < 1 || kv_heads < 1 || sinks < 0) return 0;
+  const Plan a = make_plan(B, T, kv_heads, group, D, window, sinks);
+  return a.sums + a.kv_parts + zeroed(a) + a.delta;
 }
 
 // Operands as in fbam_window_fwd; out contiguous, as the forward wrote it; d_o (B, T, heads, D) with strides; the gradients with
@@ -536,36 +748,36 @@ int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_s
                     long long dk_st, long long dk_sh, void* dv, long long dv_sb, long long dv_st, long long dv_sh, int B, int T,
                     int kv_heads, int group, int D, int window, int sinks, float scale, int* status, void* stream) {
   if ((D != 64 && D != 128) || B < 1 || T < 1 || kv_heads < 1 || group < 1 || group > kRows || sinks < 0) return 1;
-  const Workspace w = workspace(B, T, kv_heads, group, D);
-  if (work_floats < w.sums + w.counters + w.delta) return 1;
+  const Plan a = make_plan(B, T, kv_heads, group, D, window, sinks);
+  if (work_floats < a.sums + a.kv_parts + zeroed(a) + a.delta) return 1;
   const uintptr_t outs = (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)out | (uintptr_t)work;
   if ((outs & 15) || dq_sb % 8 || dq_st % 8 || dq_sh % 8 || dk_sb % 8 || dk_st % 8 || dk_sh % 8 || dv_sb % 8 || dv_st % 8 || dv_sh % 8)
     return 2;
   BwdParams p = {};
   p.T = T; p.B = B; p.kv_heads = kv_heads; p.group = group;
-  p.tile_tokens = kRows / group;
-  p.tiles = (T + p.tile_tokens - 1) / p.tile_tokens;
-  p.window = window < 1 || window > kNoWindow ? kNoWindow : window;   // 0: none
-  p.sinks = p.window == kNoWindow ? 0 : sinks < kNoWindow ? sinks : kNoWindow;
+  p.tile_tokens = a.tile_tokens; p.tiles = a.tiles;
+  p.window = a.window; p.sinks = a.sinks;
+  p.blocks = a.blocks; p.firsts = a.firsts;
+  p.parts = a.parts; p.part_tiles = a.part_tiles; p.first_parts = a.first_parts; p.first_part_tiles = a.first_part_tiles;
   p.lengths = lengths;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.scale = scale;
-  p.sums = (float4*)work;
-  p.counters = (int*)(work + w.sums);
-  p.ticket = p.counters + w.counters - 1;
+  p.sums = work;
+  p.kv_parts = (float4*)(work + a.sums);
+  p.counters = (int*)(work + a.sums + a.kv_parts);
+  p.ticket = p.counters + a.counters;
   p.lse = lse;
-  float* delta = work + w.sums + w.counters;
+  float* delta = work + a.sums + a.kv_parts + zeroed(a);
   p.delta = delta;
   p.dq = (elem_t*)dq; p.dk = (elem_t*)dk; p.dv = (elem_t*)dv;
   p.q_sb = dq_sb; p.q_st = dq_st; p.q_sh = dq_sh;
   p.k_sb = dk_sb; p.k_st = dk_st; p.k_sh = dk_sh;
   p.v_sb = dv_sb; p.v_st = dv_st; p.v_sh = dv_sh;
   p.status = status;
-  const long long nkb = (T + kKeys - 1) / kKeys, blocks = nkb * B * kv_heads;
   const long long rows = (long long)B * T * kv_heads * group;
   long long threads = rows * (D / 8);
-  if (threads < w.counters) threads = w.counters;
-  if (blocks > 0x7fffffffll || w.counters > 0x7fffffffll || (threads + 255) / 256 > 0x7fffffffll) return 1;
+  if (threads < zeroed(a)) threads = zeroed(a);
+  if (a.thread_blocks > 0x7fffffffll || zeroed(a) > 0x7fffffffll || (threads + 255) / 256 > 0x7fffffffll) return 1;
   CUtensorMap mq, mk, mv, mdo;
   int e;
   if ((e = encode_heads(&mq, q, D, kv_heads * group, T, B, q_sh, q_st, q_sb, group, p.tile_tokens))) return e;
@@ -575,13 +787,16 @@ int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_s
   cudaStream_t s = (cudaStream_t)stream;
   const unsigned pre = (unsigned)((threads + 255) / 256);
   if (D == 64)
-    window_delta_kernel<64><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)w.counters, p);
+    window_delta_kernel<64><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)zeroed(a), p);
   else
-    window_delta_kernel<128><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)w.counters, p);
+    window_delta_kernel<128><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)zeroed(a), p);
   auto kernel = D == 64 ? window_bwd_kernel<64> : window_bwd_kernel<128>;
   const int smem = D == 64 ? bwd_smem_bytes<64>() : bwd_smem_bytes<128>();
   if (set_smem(kernel, smem)) return 5;
-  kernel<<<(unsigned)blocks, kBwdThreads, smem, s>>>(mq, mk, mv, mdo, p);
+  kernel<<<(unsigned)a.thread_blocks, kBwdThreads, smem, s>>>(mq, mk, mv, mdo, p);
+  auto parts = D == 64 ? window_parts_kernel<64> : window_parts_kernel<128>;
+  const int kb0 = a.first_parts > 1 ? 0 : a.firsts, kb1 = a.parts > 1 ? a.blocks : a.firsts;      // the blocks whose walks are divided
+  if (kb1 > kb0) parts<<<dim3((unsigned)(B * kv_heads * (kb1 - kb0)), 2, D / 4 * kKeys / 256), 256, 0, s>>>(p, kb0, kb1 - kb0);
   return cudaGetLastError() == cudaSuccess ? 0 : 5;
 }
 

@@ -120,7 +120,7 @@ _ARGTYPES = {
     "fbam_window_fwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P),
     "fbam_window_bwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _P, _L, _P, _L, _L, _L, _P, _L, _L, _L,
                         _P, _L, _L, _L, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P),
-    "fbam_window_bwd_workspace": (_I, _I, _I, _I, _I),
+    "fbam_window_bwd_workspace": (_I, _I, _I, _I, _I, _I, _I),
     "fbam_cache_attention": (_P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
                              _F, _P, _P),
 }

@@ -32,7 +32,8 @@ def _forward(q, k, v, window, sinks, lengths, scale, keep):
     b, t, h, d = q.shape
     kv = k.shape[2]
     out = q.new_empty((b, t, h, d))
-    lse = q.new_empty((b, kv, t, h // kv), dtype=F32) if keep else None
+    tokens = 128 // (h // kv)                            # of a tile of 128 rows
+    lse = q.new_empty((b, kv, (t + tokens - 1) // tokens, 128), dtype=F32) if keep else None
     nv.check(nv.lib(q).fbam_window_fwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
                                        out.data_ptr(), nv.addr(lse), nv.addr(lengths), b, t, kv, h // kv, d, window or 0, sinks, scale,
                                        nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_fwd")
@@ -48,7 +49,7 @@ def _backward(saved, d_out, into, window, sinks, scale):
     if not _usable(d_out):
         d_out = d_out.clone(memory_format=torch.contiguous_format)
     lib = nv.lib(q)
-    floats = lib.fbam_window_bwd_workspace(b, t, kv, h // kv, d)
+    floats = lib.fbam_window_bwd_workspace(b, t, kv, h // kv, d, window or 0, sinks)
     work = lse.new_empty(floats)
     dq, dk, dv = into
     nv.check(lib.fbam_window_bwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
