@@ -52,12 +52,17 @@ struct FwdParams {
   int* status;
 };
 
-template <int D>
-constexpr int kSlots = D == 64 ? 8 : 5;
-template <int D>
-constexpr int fwd_smem_bytes() { return 2 * kRows * D * 2 + kSlots<D> * kKeys * D * 2 + 256 + 1024; }
-
-constexpr int kFwdThreads = 320;   // MMA issue, eight softmax warps, loads
+// TILES = 2: two tiles a thread block, one thread block a multiprocessor.  TILES = 1: one tile of one token with up to 16 heads, two
+// thread blocks a multiprocessor: such a tile has little to do for each key block that arrives, and two of them hide each other's waits.
+// Its Q keeps 16 rows a panel; what the product reads behind them are other buffers, in rows that nobody looks at.
+template <int D, int TILES>
+constexpr int kSlots = TILES == 2 ? (D == 64 ? 8 : 5) : (D == 64 ? 6 : 3);
+template <int TILES>
+constexpr int kQPanel = TILES == 2 ? kRows * 128 : 16 * 128;       // bytes of 64 channels of a tile
+template <int D, int TILES>
+constexpr int fwd_smem_bytes() { return TILES * (D / 64) * kQPanel<TILES> + kSlots<D, TILES> * kKeys * D * 2 + 256 + 1024; }
+template <int TILES>
+constexpr int kFwdThreads = TILES * 128 + 128;                     // MMA issue, loads, two idle warps; four softmax warps a tile
 
 // Queries of one tile, or of both, as the kernel needs them: token numbers within the sequence's new tokens.
 struct Span {
@@ -76,19 +81,19 @@ __device__ __forceinline__ Span make_span(int i0, int i1, int base, int key_end,
   return s;
 }
 
-template <int D, bool PAGED>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+template <int D, bool PAGED, int TILES>
+__global__ void __launch_bounds__(kFwdThreads<TILES>, TILES == 2 ? 1 : 2)
 window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
   constexpr int DP = D / 64;                 // 64-wide panels per row
-  constexpr int kQBytes = kRows * D * 2;     // one tile
+  constexpr int kQBytes = DP * kQPanel<TILES>;   // one tile
   constexpr int kKVBytes = kKeys * D * 2;
-  constexpr int NS = kSlots<D>;
-  constexpr uint32_t kTmemCols = 512;        // S/P_A [0,128) S/P_B [128,256) O_A [256,256+D) O_B [256+D,256+2D)
+  constexpr int NS = kSlots<D, TILES>;
+  constexpr uint32_t kTmemO = TILES * 128, kTmemCols = TILES * 256;   // S/P of each tile, 128 columns; then O of each, D
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                        // two tiles
-  uint8_t* sKV = sQ + 2 * kQBytes;           // NS slots: K and V of the blocks in turn
+  uint8_t* sQ = smem;                        // TILES tiles
+  uint8_t* sKV = sQ + TILES * kQBytes;           // NS slots: K and V of the blocks in turn
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + NS * kKVBytes);
   uint64_t* q_full = bars;
   uint64_t* full = bars + 1;                 // [NS]
@@ -117,7 +122,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           int pairs = 0;
           if (i <= p.B) {
             const int r0 = min(max(p.offsets[i], 0), p.T), r1 = i < p.B ? min(max(p.offsets[i + 1], r0), p.T) : p.T;
-            pairs = (r1 - r0 + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+            pairs = (r1 - r0 + TILES * p.tile_tokens - 1) / (TILES * p.tile_tokens);
           }
           int sum = pairs;
 #pragma unroll
@@ -145,7 +150,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int bh = blockIdx.x % (p.B * p.kv_heads);
     b = bh / p.kv_heads;
     kvh = bh % p.kv_heads;
-    pair = (p.T + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) - 1 - blockIdx.x / (p.B * p.kv_heads);
+    pair = (p.T + TILES * p.tile_tokens - 1) / (TILES * p.tile_tokens) - 1 - blockIdx.x / (p.B * p.kv_heads);
   }
   // this sequence: its rows, where its queries stand, where its keys end
   int row0 = 0, n_rows = p.T, n_valid = p.T, base = 0, key_end;
@@ -165,12 +170,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (p.lengths != nullptr) n_valid = min(max(p.lengths[b], 0), p.T);
     key_end = n_valid;
   }
-  const int tok0 = pair * 2 * p.tile_tokens;
-  Span span[2];
+  const int tok0 = pair * TILES * p.tile_tokens;
+  Span span[TILES];
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
+  for (int g = 0; g < TILES; ++g)
     span[g] = make_span(tok0 + g * p.tile_tokens, min(tok0 + (g + 1) * p.tile_tokens, n_valid), base, key_end, p.window);
-  const Span both = make_span(tok0, min(tok0 + 2 * p.tile_tokens, n_valid), base, key_end, p.window);
+  const Span both = make_span(tok0, min(tok0 + TILES * p.tile_tokens, n_valid), base, key_end, p.window);
   const int near = max(0, both.p0 - p.window + 1), end = min(both.p1 + 1, key_end);       // what both tiles see together:
   const int sink_end = min(p.sinks, end);                                                  // [0, sink_end) and [near, end)
   const int ns = both.hi < 0 ? 0 : min((p.sinks + kKeys - 1) / kKeys, both.hi + 1);        // blocks with first tokens
@@ -182,13 +187,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     c1 = (int)((long long)listed * (split + 1) / p.splits);
   }
   auto block_of = [&](int c) { return c < ns ? c : c - ns + range0; };
-  auto needed = [&](int g, int kb) { return kb <= span[g].hi && (kb < ns || kb >= span[g].lo); };
+  auto needed = [&](const Span& s, int kb) { return kb <= s.hi && (kb < ns || kb >= s.lo); };
 
   const bool partial = PAGED && p.splits > 1;
   if (c0 >= c1) {                              // no keys: zeros, or a part that adds nothing
-    const int i1 = min(tok0 + 2 * p.tile_tokens, n_rows);
+    const int i1 = min(tok0 + TILES * p.tile_tokens, n_rows);
     const int per = p.group * (D / 8);
-    for (int i = threadIdx.x; i < (i1 - tok0) * per; i += kFwdThreads) {
+    for (int i = threadIdx.x; i < (i1 - tok0) * per; i += kFwdThreads<TILES>) {
       const int t = tok0 + i / per, r = i % per;
       const long long row = (PAGED ? (long long)row0 : (long long)b * p.T) + t;
       const long long at = row * heads + kvh * p.group + r / (D / 8);
@@ -207,7 +212,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     prefetch_tensormap(&map_v);
     mbar_init(q_full, 1);
     for (int s = 0; s < NS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < TILES; ++g) {
       mbar_init(&s_full[g], 1);
       mbar_init(&p_ready[g], 4);
       mbar_init(&pv_full[g], 1);
@@ -220,16 +225,23 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 9) {
+  // Registers go where the scores are, four warps at a time: launched with 168 (TILES = 2) or 128 a thread, a softmax thread keeps a row of
+  // 128 scores.  With 168 for it a hundred bytes were spilled.
+  if (warp < 4) {
+    if constexpr (TILES == 2)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  if (warp == 1) {
     // ---------------------------------------------------------------- loads
     bool ok = true;
     if (lane == 0) {
-      const int tiles = span[1].hi >= 0 ? 2 : 1;
+      const int tiles = span[TILES - 1].hi >= 0 ? TILES : 1;
       mbar_expect_tx(q_full, tiles * p.tile_tokens * p.group * D * 2);
       for (int g = 0; g < tiles; ++g)
 #pragma unroll
         for (int j = 0; j < DP; ++j)           // rows beyond the tensor are filled with zeros
-          tma_load_4d(sQ + g * kQBytes + j * kRows * 128, &map_q, q_full, j * 64, kvh * p.group, row0 + tok0 + g * p.tile_tokens,
+          tma_load_4d(sQ + g * kQBytes + j * kQPanel<TILES>, &map_q, q_full, j * 64, kvh * p.group, row0 + tok0 + g * p.tile_tokens,
                       PAGED ? 0 : b);
     }
     // the page (or part of it) that this lane fetches of a block; the number of pages where there is nothing to fetch
@@ -278,23 +290,24 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       auto issue_s = [&](int g, int f) {       // S_g = Q_g K^T
         const uint64_t a = kQ + g * (kQBytes >> 4), bk = kKV + f % NS * (kKVBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) mma_f16_ss(tmem + g * 128, a + k_step(k), bk + k_step(k), idesc_s, k != 0);
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16_ss(tmem + g * 128, a + ((k / 4 * kQPanel<TILES> + k % 4 * 32) >> 4), bk + k_step(k), idesc_s, k != 0);
         mma_commit(&s_full[g]);
       };
       auto issue_pv = [&](int g, int f, bool first) {     // O_g (+)= P_g V
         const uint64_t bv = mKV + f % NS * (kKVBytes >> 4);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
-          mma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, bv + mn_step(k), idesc_pv, !first || k != 0);
+          mma_f16_ts(tmem + kTmemO + g * D, tmem + g * 128 + k * 8, bv + mn_step(k), idesc_pv, !first || k != 0);
         mma_commit(&pv_full[g]);
       };
-      int done[2] = {0, 0};                    // blocks of each tile whose P V has been issued
+      int done[TILES] = {};                    // blocks of each tile whose P V has been issued
       bool ok = mbar_wait(q_full, 0) && wait_full(0);
       if (ok) {
         fence_after_sync();
         const int kb = block_of(c0);
-        if (needed(0, kb)) issue_s(0, 0);
-        if (needed(1, kb)) issue_s(1, 0);
+        if (needed(span[0], kb)) issue_s(0, 0);
+        if (TILES == 2 && needed(span[TILES - 1], kb)) issue_s(TILES - 1, 0);
         mma_commit(&empty[0]);
       }
       for (int c = c0; c < c1 && ok; ++c) {
@@ -303,7 +316,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const int kb1 = more ? block_of(c + 1) : -1;
         if (!wait_full(f + 1)) { ok = false; break; }
         auto step_pv = [&](int g) {
-          if (!needed(g, kb)) return;
+          if (!needed(g == 0 ? span[0] : span[TILES - 1], kb)) return;
           if (!mbar_wait(&p_ready[g], done[g] & 1)) { ok = false; return; }
           fence_after_sync();
           issue_pv(g, f + 1, done[g] == 0);
@@ -314,21 +327,26 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (more) {
           if (!wait_full(f + 2)) { ok = false; break; }
           fence_after_sync();
-          if (needed(0, kb1)) issue_s(0, f + 2);   // S_0 of this block was read before p_ready[0] arrived
+          if (needed(span[0], kb1)) issue_s(0, f + 2);   // S_0 of this block was read before p_ready[0] arrived
         }
-        step_pv(1);
+        if (TILES == 2) step_pv(TILES - 1);
         if (!ok) break;
         mma_commit(&empty[(f + 1) % NS]);
         if (more) {
-          if (needed(1, kb1)) issue_s(1, f + 2);
+          if (TILES == 2 && needed(span[TILES - 1], kb1)) issue_s(TILES - 1, f + 2);
           mma_commit(&empty[(f + 2) % NS]);
         }
       }
       if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
     }
+  }
   } else {
+    if constexpr (TILES == 2)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ---------------------------------------------------------------- softmax / output threads of one tile
-    const int g = (warp - 1) >> 2;                   // tile of this warp group
+    const int g = (warp - 4) >> 2;                   // tile of this warp group
     const int lane_group = warp & 3;                 // TMEM lane quarter this warp may access
     const int row = lane_group * 32 + lane;
     const int token = row / p.group;
@@ -337,8 +355,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const bool stored = token < p.tile_tokens && i < n_rows;
     const bool valid = stored && i < n_valid && pos >= 0;
     const uint32_t lane_addr = uint32_t(lane_group * 32) << 16;
-    const uint32_t tmem_s = tmem + g * 128, tmem_pv = tmem + 256 + g * D;
-    const Span mine = g == 0 ? span[0] : span[1];
+    const uint32_t tmem_s = tmem + g * 128, tmem_pv = tmem + kTmemO + g * D;
+    const Span mine = g == 0 ? span[0] : span[TILES - 1];
+    const bool idle = TILES == 1 && lane_group * 32 >= p.group;   // rows that nobody looks at
     // m is the reference of the exponentials accumulated so far: p = 2^((s - m) scale).  It follows the running row maximum only
     // when that has moved by more than 2^8 past it, so that the output accumulator is rescaled on a few blocks only (values of p
     // stay below 2^8, far inside the 16-bit range; the final division by the row sum uses the same reference).
@@ -347,7 +366,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     int it = 0;
     for (int c = c0; c < c1; ++c) {
       const int kb = block_of(c);
-      if (!needed(g, kb)) continue;
+      if (!needed(mine, kb)) continue;
       const int k0 = kb * kKeys;
       if (k0 + kKeys > end || (k0 < near && k0 + kKeys > sink_end)) {
         // rows of V that no query of this block sees
@@ -363,6 +382,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       if (!mbar_wait(&s_full[g], it & 1)) { ok = false; break; }
       fence_after_sync();
+      if (idle) {
+        warp_arrive(&p_ready[g]);
+        ++it;
+        continue;
+      }
       uint32_t r[kKeys];
 #pragma unroll
       for (int j = 0; j < kKeys; j += 32) tmem_ld_32x32(tmem_s + lane_addr + j, *reinterpret_cast<uint32_t(*)[32]>(r + j));
@@ -370,9 +394,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // Masking is a pass of its own that only blocks on an edge take.
       if (k0 + kKeys > min(mine.p0 + 1, key_end) || (k0 <= mine.p1 - p.window && k0 + kKeys > p.sinks)) {
         const int hi = min(pos + 1, key_end) - k0, lo = pos - p.window + 1 - k0, first = p.sinks - k0;
+        auto below = [](int c) { return c <= 0 ? 0u : c >= 32 ? 0xffffffffu : (1u << c) - 1u; };
 #pragma unroll
-        for (int j = 0; j < kKeys; ++j)
-          if (j >= hi || (j < lo && j >= first)) r[j] = 0xff800000u;      // -inf
+        for (int w = 0; w < kKeys / 32; ++w) {
+          const uint32_t seen = below(hi - w * 32) & (~below(lo - w * 32) | below(first - w * 32));
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[w * 32 + j] = seen & (1u << j) ? r[w * 32 + j] : 0xff800000u;      // -inf
+        }
       }
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -413,18 +441,18 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const float2 nm2 = make_float2(nm, nm);
       float2 rs2 = make_float2(0.0f, 0.0f), rs2b = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t packed[32];
+      for (int part = 0; part < 4; ++part) {
+        uint32_t packed[16];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int at = half * 64 + 2 * j;
+        for (int j = 0; j < 16; ++j) {
+          const int at = part * 32 + 2 * j;
           const float2 e = __ffma2_rn(make_float2(__uint_as_float(r[at]), __uint_as_float(r[at + 1])), sc2, nm2);
           const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
           if (j & 1) rs2b = __fadd2_rn(rs2b, pe); else rs2 = __fadd2_rn(rs2, pe);
           elem2_t h = f22e2(pe);
           packed[j] = *reinterpret_cast<uint32_t*>(&h);
         }
-        tmem_st_32x32(tmem_s + lane_addr + half * 32, packed);
+        tmem_st_32x16(tmem_s + lane_addr + part * 16, packed);
       }
       l = l * alpha + ((rs2.x + rs2.y) + (rs2b.x + rs2b.y));
       tmem_st_wait();
@@ -547,10 +575,10 @@ int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_s
   if ((e = encode_heads(&mq, q, D, kv_heads * group, T, B, q_sh, q_st, q_sb, group, p.tile_tokens))) return e;
   if ((e = encode_heads(&mk, k, D, kv_heads, T, B, k_sh, k_st, k_sb, 1, kKeys))) return e;
   if ((e = encode_heads(&mv, v, D, kv_heads, T, B, v_sh, v_st, v_sb, 1, kKeys))) return e;
-  const int smem = D == 64 ? fwd_smem_bytes<64>() : fwd_smem_bytes<128>();
-  auto kernel = D == 64 ? window_fwd_kernel<64, false> : window_fwd_kernel<128, false>;
+  const int smem = D == 64 ? fwd_smem_bytes<64, 2>() : fwd_smem_bytes<128, 2>();
+  auto kernel = D == 64 ? window_fwd_kernel<64, false, 2> : window_fwd_kernel<128, false, 2>;
   if (set_smem(kernel, smem)) return 5;
-  kernel<<<(unsigned)blocks, kFwdThreads, smem, (cudaStream_t)stream>>>(mq, mk, mv, p);
+  kernel<<<(unsigned)blocks, kFwdThreads<2>, smem, (cudaStream_t)stream>>>(mq, mk, mv, p);
   return cudaGetLastError() == cudaSuccess ? 0 : 5;
 }
 
@@ -582,19 +610,29 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   p.part_ml = (float2*)part_ml;
   p.status = status;
   if (((uintptr_t)out | (uintptr_t)part_o | (uintptr_t)part_ml) & 15) return 2;
-  CUtensorMap mq, mk, mv;
+  // pairs of tiles: one a sequence without offsets; with them, at most one that is not full of each sequence
+  const bool single = offsets == nullptr && group <= 16;
+  if (single) p.tile_tokens = 1;
+  const int per = 2 * p.tile_tokens;
+  const long long pairs = offsets == nullptr ? B : rows / per + (rows < B ? rows : B) + 1;
   int e;
+  CUtensorMap mq, mk, mv;
   if ((e = encode_heads(&mq, q, D, kv_heads * group, rows, 1, q_sh, q_st, (long long)rows * q_st, group, p.tile_tokens))) return e;
   if ((e = encode_heads(&mk, k_pages, D, kv_heads, page, pages, k_sh, k_ss, k_sp, 1, p.piece))) return e;
   if ((e = encode_heads(&mv, v_pages, D, kv_heads, page, pages, v_sh, v_ss, v_sp, 1, p.piece))) return e;
   cudaStream_t s = (cudaStream_t)stream;
-  // pairs of tiles: one a sequence without offsets; with them, at most one that is not full of each sequence
-  const int per = 2 * p.tile_tokens;
-  const long long pairs = offsets == nullptr ? B : rows / per + (rows < B ? rows : B) + 1;
-  const int smem = D == 64 ? fwd_smem_bytes<64>() : fwd_smem_bytes<128>();
-  auto kernel = D == 64 ? window_fwd_kernel<64, true> : window_fwd_kernel<128, true>;
-  if (set_smem(kernel, smem)) return 5;
-  kernel<<<dim3((unsigned)pairs, kv_heads, splits), kFwdThreads, smem, s>>>(mq, mk, mv, p);
+  const dim3 grid((unsigned)pairs, kv_heads, splits);
+  if (single) {
+    const int smem = D == 64 ? fwd_smem_bytes<64, 1>() : fwd_smem_bytes<128, 1>();
+    auto kernel = D == 64 ? window_fwd_kernel<64, true, 1> : window_fwd_kernel<128, true, 1>;
+    if (set_smem(kernel, smem)) return 5;
+    kernel<<<grid, kFwdThreads<1>, smem, s>>>(mq, mk, mv, p);
+  } else {
+    const int smem = D == 64 ? fwd_smem_bytes<64, 2>() : fwd_smem_bytes<128, 2>();
+    auto kernel = D == 64 ? window_fwd_kernel<64, true, 2> : window_fwd_kernel<128, true, 2>;
+    if (set_smem(kernel, smem)) return 5;
+    kernel<<<grid, kFwdThreads<2>, smem, s>>>(mq, mk, mv, p);
+  }
   if (splits > 1) {
     const long long all = (long long)rows * kv_heads * group;
     const unsigned blocks = (unsigned)((all + 7) / 8);

@@ -222,8 +222,8 @@ __device__ __forceinline__ long long slot_of(const BwdParams& p, int bh, int kb,
 template <int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
-                  const __grid_constant__ BwdParams p) {
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_dk,
+                  const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ BwdParams p) {
   constexpr int DP = D / 64;
   constexpr int kTile = 128 * D * 2;           // a 128-row x D operand tile
   constexpr int kSq = 128 * 128 * 2;           // dS tile
@@ -260,14 +260,30 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   int* my_ticket = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int used = p.tile_tokens * p.group;                        // rows of a tile
   if (threadIdx.x == 0) {
     *my_ticket = atomicAdd(p.ticket, 1);
     prefetch_tensormap(&map_q); prefetch_tensormap(&map_k); prefetch_tensormap(&map_v); prefetch_tensormap(&map_do);
+  }
+  if (warp == 12) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
+  if (threadIdx.x == 13 * 32) {
     for (int i = 0; i < 17 + 3 * kStages; ++i)
       mbar_init(&bars[i], i == 7 || i == 8 ? 9 : i == 11 || i == 12 || i == 16 ? 8 : i == 14 || (i >= 17 && i < 17 + 2 * kStages) ? 4 : 1);
     mbar_fence_init();
   }
+  if (used < kRows) {
+    // the copies never write the rows behind them; they are operands of the transposed products
+    const int rows = kRows - used, per = (2 + DOS) * DP * rows * 8;
+    for (int i = threadIdx.x; i < per; i += kBwdThreads) {
+      const int chunk = i & 7, r = used + (i >> 3) % rows, panel = (i >> 3) / rows;    // Q stages and dO stages lie in a row
+      *reinterpret_cast<uint4*>(sQ + panel * 128 * 128 + r * 128 + chunk * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+  }
+  fence_before_sync();
   __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
   const int ticket = __shfl_sync(0xffffffffu, *my_ticket, 0);      // the same in all lanes: what follows from it takes uniform registers
   const int bhs = p.B * p.kv_heads, ns = p.firsts;
   const int bh = ticket % bhs, behind = ticket / bhs - (p.blocks - ns) * p.parts;   // 0 or more: a block of first tokens
@@ -279,7 +295,10 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int len = p.lengths == nullptr ? p.T : min(max(p.lengths[b], 0), p.T);
   const Walk walk = walk_of(p, kb, len);
   const int last_part = walk.last_part;
-  if (part_at > last_part) return;
+  if (part_at > last_part) {
+    if (warp == 12) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
   const int m0 = walk.first + part_at * part_tiles, n = min(part_tiles, walk.tiles - part_at * part_tiles);   // the tiles of this part
   if (walk.tiles <= 0) {                                           // keys behind the sequence's end
     for (int i = threadIdx.x; i < kKeys * (D / 8) * 2; i += kBwdThreads) {
@@ -290,23 +309,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         *reinterpret_cast<uint4*>(at + d) = make_uint4(0u, 0u, 0u, 0u);
       }
     }
+    if (warp == 12) tmem_dealloc(tmem, kTmemCols);
     return;
   }
-  const int used = p.tile_tokens * p.group;                        // rows of a tile
-  if (used < kRows) {
-    // the copies never write the rows behind them; they are operands of the transposed products
-    const int rows = kRows - used, per = (2 + DOS) * DP * rows * 8;
-    for (int i = threadIdx.x; i < per; i += kBwdThreads) {
-      const int chunk = i & 7, r = used + (i >> 3) % rows, panel = (i >> 3) / rows;    // Q stages and dO stages lie in a row
-      *reinterpret_cast<uint4*>(sQ + panel * 128 * 128 + r * 128 + chunk * 16) = make_uint4(0u, 0u, 0u, 0u);
-    }
-    fence_proxy_async_smem();
-  }
-  if (warp == 12) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
   const uint32_t tm_s = tmem, tm_dp = tmem + 128, tm_dv = tmem + 256, tm_dk = tmem + 256 + D;
   const uint32_t tm_dq = kOwnDq ? tmem + 256 + 2 * D : tm_dp;
 
@@ -459,7 +464,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // In the fragment layout a thread has 16 of the 64 queries (of four keys), so it fetches 16 values of lse and of delta.  With a key a
     // thread it needed all 64, the same in all lanes: 1 024 cycles of shared memory a tile, which the products keep busy.
     const int lane_group = warp & 3, part = (warp - 4) >> 2;
-    const int row = lane_group * 32 + lane, key = k0 + row;
+    const int row = lane_group * 32 + lane;
     const uint32_t lane_addr = uint32_t(lane_group * 32) << 16;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     uint8_t* dsPanel = sDS + part * 128 * 128;         // 64 queries
@@ -509,18 +514,23 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       // sets what a query does not see to zero: of the thread's 64 values those of key k and query c that are not in [from, to)
       auto mask = [&](uint32_t (&x)[2][32]) {
+        auto below = [](int c) { return c <= 0 ? 0u : c >= 32 ? 0xffffffffu : (1u << c) - 1u; };
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const int k = k0 + lane_group * 32 + r4 * 8 + (lane >> 2), c0 = part * 64 + (lane & 3) * 2;
+          const int k = k0 + lane_group * 32 + r4 * 8 + (lane >> 2);
           const int from = max(0, k - t0) * p.group;                                     // t >= k
           const int to = k < p.sinks ? rows : min(rows, max(0, min(k - t0 + p.window, p.tile_tokens)) * p.group);   // t < k + window
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int w = 0; w < 2; ++w) {                    // 32 queries
+            const uint32_t seen = (below(to - part * 64 - w * 32) & ~below(from - part * 64 - w * 32)) >> (lane & 3) * 2;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int c = c0 + j * 8 + e;
-              if (c < from || c >= to) x[r4 >> 1][j * 4 + (r4 & 1) * 2 + e] = 0u;
-            }
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t& v = x[r4 >> 1][(w * 4 + j) * 4 + (r4 & 1) * 2 + e];
+                v = seen & (1u << (j * 8 + e)) ? v : 0u;
+              }
+          }
         }
       };
       uint32_t pr[2][32];                                // scores, then P, then dS, as fp32 bits: 16 keys each
@@ -587,19 +597,42 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // dV (part 0) and dK (part 1) of this key block
     if (ok && mbar_wait(dk_done, (n - 1) & 1)) {
       fence_after_sync();
-      const int t_k = key;
-      elem_t* dst = part == 0 ? p.dv + b * p.v_sb + t_k * p.v_st + kvh * p.v_sh : p.dk + b * p.k_sb + t_k * p.k_st + kvh * p.k_sh;
       const uint32_t src = part == 0 ? tm_dv : tm_dk;
-      float4* to = p.kv_parts + (slot_of(p, bh, kb, part_at) * 2 + part) * (D / 4) * kKeys + row;
+      if (last_part > 0) {
+        float4* to = p.kv_parts + (slot_of(p, bh, kb, part_at) * 2 + part) * (D / 4) * kKeys + row;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32(src + lane_addr + c0, r);
-        tmem_ld_wait();
-        if (last_part > 0)
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32(src + lane_addr + c0, r);
+          tmem_ld_wait();
           store_part<kKeys>(to + c0 / 4 * kKeys, r);
-        else if (t_k < p.T)
-          store_row(dst + c0, r, part == 0 ? 1.0f : p.scale);
+        }
+      } else {
+        // through the stages of Q, which nothing reads any more, and out by the copy engine: as rows from registers they took 4 400
+        // (D = 64) to 9 000 cycles of every thread block
+        uint8_t* tile = sQ + part * kTile;
+        const float scale = part == 0 ? 1.0f : p.scale;
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32(src + lane_addr + c0, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            __align__(16) elem2_t hh[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j * 8 + 2 * q]) * scale, __uint_as_float(r[j * 8 + 2 * q + 1]) * scale);
+            *reinterpret_cast<uint4*>(tile + c0 / 64 * 128 * 128 + swz(row, c0 % 64 / 8 + j)) = *reinterpret_cast<uint4*>(hh);
+          }
+        }
+        fence_proxy_async_smem();
+        if (part == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");   // four warps
+        if (lane_group == 0 && elect_one()) {
+#pragma unroll
+          for (int j = 0; j < DP; ++j) tma_store_4d(part == 0 ? &map_dv : &map_dk, tile + j * 128 * 128, j * 64, kvh, k0, b);   // rows behind T are cut
+          bulk_commit_group();
+          bulk_wait_group_read<0>();
+        }
       }
     } else {
       ok = false;
@@ -778,12 +811,14 @@ int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_s
   long long threads = rows * (D / 8);
   if (threads < zeroed(a)) threads = zeroed(a);
   if (a.thread_blocks > 0x7fffffffll || zeroed(a) > 0x7fffffffll || (threads + 255) / 256 > 0x7fffffffll) return 1;
-  CUtensorMap mq, mk, mv, mdo;
+  CUtensorMap mq, mk, mv, mdo, mdk, mdv;
   int e;
   if ((e = encode_heads(&mq, q, D, kv_heads * group, T, B, q_sh, q_st, q_sb, group, p.tile_tokens))) return e;
   if ((e = encode_heads(&mk, k, D, kv_heads, T, B, k_sh, k_st, k_sb, 1, kKeys))) return e;
   if ((e = encode_heads(&mv, v, D, kv_heads, T, B, v_sh, v_st, v_sb, 1, kKeys))) return e;
   if ((e = encode_heads(&mdo, d_o, D, kv_heads * group, T, B, do_sh, do_st, do_sb, group, p.tile_tokens))) return e;
+  if ((e = encode_heads(&mdk, dk, D, kv_heads, T, B, dk_sh, dk_st, dk_sb, 1, kKeys))) return e;
+  if ((e = encode_heads(&mdv, dv, D, kv_heads, T, B, dv_sh, dv_st, dv_sb, 1, kKeys))) return e;
   cudaStream_t s = (cudaStream_t)stream;
   const unsigned pre = (unsigned)((threads + 255) / 256);
   if (D == 64)
@@ -793,7 +828,7 @@ int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_s
   auto kernel = D == 64 ? window_bwd_kernel<64> : window_bwd_kernel<128>;
   const int smem = D == 64 ? bwd_smem_bytes<64>() : bwd_smem_bytes<128>();
   if (set_smem(kernel, smem)) return 5;
-  kernel<<<(unsigned)a.thread_blocks, kBwdThreads, smem, s>>>(mq, mk, mv, mdo, p);
+  kernel<<<(unsigned)a.thread_blocks, kBwdThreads, smem, s>>>(mq, mk, mv, mdo, mdk, mdv, p);
   auto parts = D == 64 ? window_parts_kernel<64> : window_parts_kernel<128>;
   const int kb0 = a.first_parts > 1 ? 0 : a.firsts, kb1 = a.parts > 1 ? a.blocks : a.firsts;      // the blocks whose walks are divided
   if (kb1 > kb0) parts<<<dim3((unsigned)(B * kv_heads * (kb1 - kb0)), 2, D / 4 * kKeys / 256), 256, 0, s>>>(p, kb0, kb1 - kb0);

@@ -6,6 +6,8 @@ forward keeps its output and one fp32 value per query row for the backward.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ..utils import flops
@@ -130,11 +132,20 @@ def window_attention_qkv(qkv, kv, window, sinks, lengths, scale):
     return _forward(*_heads(qkv, kv), window, sinks, lengths, scale, False)[0]
 
 
-def _splits(units: int, blocks: int) -> int:
-    """How many thread blocks share the keys of one pair of query tiles."""
-    if units >= 148:
+@functools.lru_cache(maxsize=1024)
+def _splits(units: int, blocks: int, slots: int) -> int:
+    """How many thread blocks share the keys of one tile (or pair of tiles) of queries, where ``units`` of them have up to ``blocks``
+    key blocks each and the machine holds ``slots`` thread blocks: what takes the least of (waves) x (key blocks of a share, and three
+    for a thread block's start and end), with eight for joining the shares (another launch, and on the host two more tensors).
+    Where the units alone fill the machine twice, shares would save nothing and their sums are large."""
+    best, splits = None, 1
+    if units >= 2 * slots:
         return 1
-    return max(1, min(148 // units, blocks // 2, 64))
+    for s in range(1, min(64, blocks) + 1):
+        cost = -(-units * s // slots) * (-(-blocks // s) + 3) + (8 if s > 1 else 0)
+        if best is None or cost < best:
+            best, splits = cost, s
+    return splits
 
 
 def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks):
@@ -146,9 +157,10 @@ def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks
     out = q.new_empty((n, h, d))
     lib = nv.lib(q)
     per = 2 * (128 // (h // kv))
+    single = offsets is None and h // kv <= 16              # one token a sequence: two thread blocks a multiprocessor
     units = kv * (b if offsets is None else n // per + min(n, b))
     keys = most * page if window is None else min(most * page, window + per + sinks + 256)
-    splits = _splits(units, (keys + 127) // 128)
+    splits = _splits(units, max(1, (keys + 127) // 128), 296 if single else 148)
     part_o = part_ml = None
     if splits > 1:
         part_o = q.new_empty((splits, n, h, d), dtype=F32)
