@@ -82,4 +82,16 @@ int set_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess ? 0 : 5;
 }
 
+// The same once for a device and thread, for calls of a few microseconds.
+template <auto kernel>
+int set_smem_once(int bytes) {
+  static thread_local int done = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 5;
+  if (dev == done) return 0;
+  if (set_smem(kernel, bytes)) return 5;
+  done = dev;
+  return 0;
+}
+
 }  // namespace attn

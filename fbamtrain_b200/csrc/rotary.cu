@@ -12,15 +12,17 @@
 // The append form is the same pass of a serving step: the heads of new tokens come as (tokens, query + key + value heads, D);
 // turned queries go to a tensor, turned keys and the values into the pages of a cache.
 //
-// Bound by memory: each value is read and written once.  A thread block takes a few tokens (some 2048 16-byte pieces), forms
-// their angles in shared memory and walks the pieces, four loads in flight a thread.
+// Bound by memory: each value is read and written once.  A thread has one piece of a head (in the half layout 8 channels and the 8 that
+// they turn with) and walks the heads of its token, four at a time: it forms its sines and cosines once, in registers, and the heads'
+// loads are on their way together.  A first form kept the angles of a few tokens in shared memory and gave pieces to threads in any
+// order: a block's loads waited for its angles and every piece for two divisions (27 against NEW us at 8192 tokens of 48 heads of 64).
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include "elem16.cuh"
 
 namespace {
 
-constexpr int kMaxPairs = 128, kThreads = 256, kMaxTokens = 32, kUnroll = 4;
+constexpr int kMaxPairs = 128, kThreads = 256, kUnroll = 4;
 
 struct RotaryParams {
   unsigned long long turns[kMaxPairs];  // fraction of a turn a position, times 2^64
@@ -34,7 +36,8 @@ struct RotaryParams {
   int T, H, D, turned, pairs;
   int inverse;
   float magnitude;
-  int per_block;                        // tokens of a thread block
+  int pieces;                           // of a head
+  int heads_each;                       // heads of a thread
   // append
   elem_t* k_pages;
   elem_t* v_pages;                      // (pages, page, kv_heads, D)
@@ -100,110 +103,70 @@ __device__ __forceinline__ void rotate4(uint4& a, const float2* cs, float m) {
 // turn with; everything else, and all of the interleaved layout, is one vector.
 template <bool APPEND, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ float2 cs[];        // (tokens, pairs)
-  __shared__ long long src_at[kMaxTokens];
-  __shared__ long long dst_k[kMaxTokens], dst_v[kMaxTokens];
-  __shared__ long long pos[kMaxTokens];
-  const long long n0 = (long long)blockIdx.x * p.per_block;
-  const int tokens = (int)min((long long)p.per_block, p.tokens - n0);
-  if (threadIdx.x < tokens) {
-    const long long n = n0 + threadIdx.x;
-    if constexpr (APPEND) {
-      int b;
-      const long long at = append_position(p, n, b);
-      pos[threadIdx.x] = at;
-      src_at[threadIdx.x] = n * p.x_st;
-      long long dk = -1, dv = -1;
-      if (at >= 0 && at / p.page < p.max_pages) {
-        const int which = p.tables[b * p.t_sb + at / p.page];
-        if (which >= 0 && which < p.pages) {
-          dk = which * p.k_sp + at % p.page * p.k_ss;
-          dv = which * p.v_sp + at % p.page * p.v_ss;
-        }
+  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, n = i / p.pieces;
+  if (n >= p.tokens) return;
+  const int c = (int)(i - n * p.pieces);
+  const int h0 = blockIdx.y * p.heads_each, h1 = min(p.H, h0 + p.heads_each);
+  const bool turns = INTERLEAVED ? c * 8 < 2 * p.pairs : c * 8 < p.pairs, two = !INTERLEAVED && turns;
+  const int ch = INTERLEAVED || turns ? c * 8 : c * 8 + p.pairs;          // first channel: behind both halves where nothing turns
+  long long pos, src;
+  long long dst_k = -1, dst_v = -1;
+  if constexpr (APPEND) {
+    int b;
+    pos = append_position(p, n, b);
+    src = n * p.x_st;
+    if (pos >= 0 && pos / p.page < p.max_pages) {
+      const int which = p.tables[b * p.t_sb + pos / p.page];
+      if (which >= 0 && which < p.pages) {
+        dst_k = which * p.k_sp + pos % p.page * p.k_ss;
+        dst_v = which * p.v_sp + pos % p.page * p.v_ss;
       }
-      dst_k[threadIdx.x] = dk;
-      dst_v[threadIdx.x] = dv;
-    } else {
-      const long long b = n / p.T, t = n % p.T;
-      src_at[threadIdx.x] = b * p.x_sb + t * p.x_st;
-      const long long at = b * p.p_sb + t * p.p_st;
-      pos[threadIdx.x] = p.positions64 ? ((const long long*)p.positions)[at] : (long long)((const int*)p.positions)[at];
+    }
+  } else {
+    const long long b = n / p.T, t = n - b * p.T, at = b * p.p_sb + t * p.p_st;
+    src = b * p.x_sb + t * p.x_st;
+    pos = p.positions64 ? ((const long long*)p.positions)[at] : (long long)((const int*)p.positions)[at];
+  }
+  const elem_t* x = p.x + src + ch;
+  float2 cs[8];
+  if (turns && h0 < p.turned) {
+#pragma unroll
+    for (int j = 0; j < (INTERLEAVED ? 4 : 8); ++j) {
+      cs[j] = turn(p.turns[c * (INTERLEAVED ? 4 : 8) + j], pos);
+      if (p.inverse) cs[j].y = -cs[j].y;
     }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < tokens * p.pairs; i += kThreads) {
-    const int t = i / p.pairs;
-    float2 v = turn(p.turns[i - t * p.pairs], pos[t]);
-    if (p.inverse) v.y = -v.y;
-    cs[i] = v;
-  }
-  __syncthreads();
-  const int half = p.pairs >> 3;                                             // two-vector pieces (half layout)
-  const int per_turned = INTERLEAVED ? p.D / 8 : p.D / 8 - half, per_plain = p.D / 8;
-  const int in_turned = p.turned * per_turned, per_token = in_turned + (p.H - p.turned) * per_plain;
-  const int all = tokens * per_token;
-  for (int base = threadIdx.x; base < all; base += kThreads * kUnroll) {
+  for (int h = h0; h < h1; h += kUnroll) {
     uint4 a[kUnroll], b[kUnroll];
-    elem_t* dst[kUnroll];
-    const float2* angle[kUnroll];
-    int kind[kUnroll];                  // 0: nothing, 1: copy, 2: interleaved vector, 3: two vectors, 4: zeros
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = base + u * kThreads;
-      kind[u] = 0;
-      if (i < all) {
-        const int t = i / per_token, r = i - t * per_token;
-        int h, c;
-        if (r < in_turned) {
-          h = r / per_turned;
-          c = r - h * per_turned;
-        } else {
-          h = (r - in_turned) / per_plain;
-          c = r - in_turned - h * per_plain;
-          h += p.turned;
-        }
-        const bool turned = h < p.turned;
-        kind[u] = 1;
-        int ch = c * 8;                 // first channel
-        if (turned) {
-          if (INTERLEAVED) {
-            if (ch < 2 * p.pairs) { kind[u] = 2; angle[u] = cs + t * p.pairs + c * 4; }
-          } else if (c < half) {
-            kind[u] = 3;
-            angle[u] = cs + t * p.pairs + c * 8;
-          } else {
-            ch += p.pairs;              // behind both halves
-          }
-        }
-        if constexpr (APPEND) {
-          const bool there = pos[t] >= 0;
-          if (h < p.q_heads) {
-            dst[u] = p.y + ((n0 + t) * p.q_heads + h) * p.D + ch;
-            if (!there) kind[u] = kind[u] == 3 ? 5 : 4;
-          } else if (h < p.q_heads + p.kv_heads) {
-            dst[u] = p.k_pages + dst_k[t] + (h - p.q_heads) * p.k_sh + ch;
-            if (dst_k[t] < 0) kind[u] = 0;
-          } else {
-            dst[u] = p.v_pages + dst_v[t] + (h - p.q_heads - p.kv_heads) * p.v_sh + ch;
-            if (dst_k[t] < 0) kind[u] = 0;
-          }
-        } else {
-          dst[u] = p.y + ((n0 + t) * p.H + h) * p.D + ch;
-        }
-        const elem_t* src = p.x + src_at[t] + h * p.x_sh + ch;
-        if (kind[u] != 0) a[u] = __ldcs(reinterpret_cast<const uint4*>(src));
-        if (kind[u] == 3) b[u] = __ldcs(reinterpret_cast<const uint4*>(src + p.pairs));
+    for (int u = 0; u < kUnroll; ++u)
+      if (h + u < h1) {
+        a[u] = __ldcs(reinterpret_cast<const uint4*>(x + (h + u) * p.x_sh));
+        if (two) b[u] = __ldcs(reinterpret_cast<const uint4*>(x + (h + u) * p.x_sh + p.pairs));
       }
-    }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (kind[u] == 0) continue;
-      if (kind[u] == 2) rotate4(a[u], angle[u], p.magnitude);
-      if (kind[u] == 3) rotate8(a[u], b[u], angle[u], p.magnitude);
-      if (kind[u] >= 4) a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
-      *reinterpret_cast<uint4*>(dst[u]) = a[u];
-      if (kind[u] == 3 || kind[u] == 5) *reinterpret_cast<uint4*>(dst[u] + p.pairs) = b[u];
-    }
+    for (int u = 0; u < kUnroll; ++u)
+      if (h + u < h1) {
+        const int head = h + u;
+        if (turns && head < p.turned) {
+          if constexpr (INTERLEAVED) rotate4(a[u], cs, p.magnitude); else rotate8(a[u], b[u], cs, p.magnitude);
+        }
+        elem_t* dst;
+        if constexpr (APPEND) {
+          if (head < p.q_heads) {
+            dst = p.y + (n * p.q_heads + head) * p.D;
+            if (pos < 0) a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            if (dst_k < 0) continue;
+            dst = head < p.q_heads + p.kv_heads ? p.k_pages + dst_k + (head - p.q_heads) * p.k_sh
+                                                : p.v_pages + dst_v + (head - p.q_heads - p.kv_heads) * p.v_sh;
+          }
+        } else {
+          dst = p.y + (n * p.H + head) * p.D;
+        }
+        *reinterpret_cast<uint4*>(dst + ch) = a[u];
+        if (two) *reinterpret_cast<uint4*>(dst + ch + p.pairs) = b[u];
+      }
   }
 }
 
@@ -238,21 +201,20 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_const
   }
 }
 
-// Pieces of a token and from them the tokens of a block: some 2048 pieces, but no fewer blocks than fill the machine twice.
+// Eight heads a thread, or fewer where there are so few tokens that the machine would not be full.
 template <bool APPEND>
 int launch(RotaryParams& p, bool interleaved, cudaStream_t s) {
-  const long long pieces = (long long)p.H * (p.D / 8);
-  long long per = 2048 / (pieces < 1 ? 1 : pieces);
-  const long long spread = p.tokens / 296;
-  per = per < spread ? per : spread;
-  p.per_block = (int)(per < 1 ? 1 : per > kMaxTokens ? kMaxTokens : per);
-  const long long blocks = (p.tokens + p.per_block - 1) / p.per_block;
-  if (blocks > 0x7fffffffll || pieces * p.per_block > 0x7fffffffll) return 1;
-  const size_t smem = (size_t)p.per_block * (p.pairs < 1 ? 1 : p.pairs) * sizeof(float2);
+  p.pieces = interleaved ? p.D / 8 : (p.D - p.pairs) / 8;
+  const long long threads = p.tokens * p.pieces, blocks = (threads + kThreads - 1) / kThreads;
+  p.heads_each = 8;
+  while (p.heads_each > 1 && threads * ((p.H + p.heads_each - 1) / p.heads_each) < 148 * 1024) p.heads_each >>= 1;
+  const int parts = (p.H + p.heads_each - 1) / p.heads_each;
+  if (blocks > 0x7fffffffll || parts > 65535) return 1;
+  const dim3 grid((unsigned)blocks, parts);
   if (interleaved)
-    rotary_kernel<APPEND, true><<<(unsigned)blocks, kThreads, smem, s>>>(p);
+    rotary_kernel<APPEND, true><<<grid, kThreads, 0, s>>>(p);
   else
-    rotary_kernel<APPEND, false><<<(unsigned)blocks, kThreads, smem, s>>>(p);
+    rotary_kernel<APPEND, false><<<grid, kThreads, 0, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : 5;
 }
 

@@ -84,7 +84,8 @@ __device__ __forceinline__ Span make_span(int i0, int i1, int base, int key_end,
 template <int D, bool PAGED, int TILES>
 __global__ void __launch_bounds__(kFwdThreads<TILES>, TILES == 2 ? 1 : 2)
 window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+                  const __grid_constant__ CUtensorMap map_low, const __grid_constant__ FwdParams p) {
   constexpr int DP = D / 64;                 // 64-wide panels per row
   constexpr int kQBytes = DP * kQPanel<TILES>;   // one tile
   constexpr int kKVBytes = kKeys * D * 2;
@@ -471,33 +472,80 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!valid) l = 0.0f;
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       const float2 inv2 = make_float2(inv, inv);
+      if constexpr (PAGED) {
 #pragma unroll 1
-      for (int d0 = 0; d0 < D; d0 += 32) {
-        uint32_t r[32];
-        if (it > 0) {
-          tmem_ld_32x32(tmem_pv + lane_addr + d0, r);
-          tmem_ld_wait();
-        }
-        if (it == 0 || !(l > 0.0f)) {          // nothing seen
+        for (int d0 = 0; d0 < D; d0 += 32) {
+          uint32_t r[32];
+          if (it > 0) {
+            tmem_ld_32x32(tmem_pv + lane_addr + d0, r);
+            tmem_ld_wait();
+          }
+          if (it == 0 || !(l > 0.0f)) {          // nothing seen
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = 0u;
-        }
-        if (stored) {
-          if (partial) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + ((long long)split * p.T * heads + at) * D + d0);
+            for (int j = 0; j < 32; ++j) r[j] = 0u;
+          }
+          if (stored) {
+            if (partial) {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + ((long long)split * p.T * heads + at) * D + d0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
-                                   __uint_as_float(r[4 * j + 3]));
-          } else {
+              for (int j = 0; j < 8; ++j)
+                dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                                     __uint_as_float(r[4 * j + 3]));
+            } else {
+#pragma unroll
+              for (int d = 0; d < 32; d += 8) {
+                __align__(16) elem2_t hh[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  hh[q] = f22e2(__fmul2_rn(make_float2(__uint_as_float(r[d + 2 * q]), __uint_as_float(r[d + 2 * q + 1])), inv2));
+                *reinterpret_cast<uint4*>(p.out + at * D + d0 + d) = *reinterpret_cast<uint4*>(hh);
+              }
+            }
+          }
+        }
+      } else {
+        // Whole tiles go out by the copy engine, from the tile's Q, which its products have read; rows behind T are cut off.  With a
+        // gradient to come, what the rounding took off goes out as well: delta = sum dO O from the rounded output alone was the largest
+        // error of the gradients where few keys are seen.
+        const int passes = p.lse != nullptr ? 2 : 1;
+        for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll 1
+          for (int d0 = 0; d0 < D; d0 += 32) {
+            uint32_t r[32];
+            if (it > 0) {
+              tmem_ld_32x32(tmem_pv + lane_addr + d0, r);
+              tmem_ld_wait();
+            }
+            if (it == 0 || !(l > 0.0f)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = 0u;
+            }
 #pragma unroll
             for (int d = 0; d < 32; d += 8) {
               __align__(16) elem2_t hh[4];
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                hh[q] = f22e2(__fmul2_rn(make_float2(__uint_as_float(r[d + 2 * q]), __uint_as_float(r[d + 2 * q + 1])), inv2));
-              *reinterpret_cast<uint4*>(p.out + at * D + d0 + d) = *reinterpret_cast<uint4*>(hh);
+              for (int q = 0; q < 4; ++q) {
+                const float2 o = __fmul2_rn(make_float2(__uint_as_float(r[d + 2 * q]), __uint_as_float(r[d + 2 * q + 1])), inv2);
+                hh[q] = f22e2(o);
+                if (pass) {
+                  const float2 rounded = e22ff(hh[q]);
+                  hh[q] = ff2e2(o.x - rounded.x, o.y - rounded.y);
+                }
+              }
+              *reinterpret_cast<uint4*>(sQ + g * kQBytes + d0 / 64 * kQPanel<TILES> + swz(row, d0 % 64 / 8 + d / 8)) = *reinterpret_cast<uint4*>(hh);
             }
+          }
+          fence_proxy_async_smem();
+          if (g == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");   // the tile's warps
+          if (lane_group == 0 && tok0 + g * p.tile_tokens < p.T && elect_one()) {
+#pragma unroll
+            for (int j = 0; j < DP; ++j)
+              tma_store_4d(pass ? &map_low : &map_out, sQ + g * kQBytes + j * kQPanel<TILES>, j * 64, kvh * p.group, tok0 + g * p.tile_tokens, b);
+            bulk_commit_group();
+            bulk_wait_group_read<0>();
+          }
+          if (pass + 1 < passes) {
+            if (g == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
           }
         }
       }
@@ -545,14 +593,23 @@ __global__ void __launch_bounds__(256) window_join_kernel(const float* part_o, c
   for (int v = 0; v < V; v += 2) *reinterpret_cast<elem2_t*>(dst + v) = ff2e2(o[v] * inv, o[v + 1] * inv);
 }
 
+template <int D, bool PAGED, int TILES>
+int launch(dim3 grid, cudaStream_t s, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& out, const CUtensorMap& low,
+           const FwdParams& p) {
+  constexpr int smem = fwd_smem_bytes<D, TILES>();
+  if (set_smem_once<window_fwd_kernel<D, PAGED, TILES>>(smem)) return 5;
+  window_fwd_kernel<D, PAGED, TILES><<<grid, kFwdThreads<TILES>, smem, s>>>(q, k, v, out, low, p);
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
 
 // q (B, T, heads, D), k and v (B, T, kv_heads, D) with element strides each; out contiguous; lse fp32 (B, kv_heads, tiles, 128) or
-// null, where a tile has 128 / group tokens; lengths (B) or null.
+// null, where a tile has 128 / group tokens, and with it low like out: what rounding took off out; lengths (B) or null.
 int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_sh, const void* k, const void* v, long long k_sb,
-                    long long k_st, long long k_sh, long long v_sb, long long v_st, long long v_sh, void* out, float* lse,
+                    long long k_st, long long k_sh, long long v_sb, long long v_st, long long v_sh, void* out, void* low, float* lse,
                     const int* lengths, int B, int T, int kv_heads, int group, int D, int window, int sinks, float scale, int* status,
                     void* stream) {
   if ((D != 64 && D != 128) || B < 1 || T < 1 || kv_heads < 1 || group < 1 || group > kRows || sinks < 0) return 1;
@@ -569,16 +626,20 @@ int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_s
   p.tiles = (T + p.tile_tokens - 1) / p.tile_tokens;
   p.status = status;
   const long long pairs = (T + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens), blocks = pairs * B * kv_heads;
-  if (blocks > 0x7fffffffll || (uintptr_t)out & 15) return (uintptr_t)out & 15 ? 2 : 1;
-  CUtensorMap mq, mk, mv;
+  if (blocks > 0x7fffffffll) return 1;
+  const int heads = kv_heads * group;
+  const long long o_sb = (long long)T * heads * D;
+  CUtensorMap mq, mk, mv, mo, ml;
   int e;
   if ((e = encode_heads(&mq, q, D, kv_heads * group, T, B, q_sh, q_st, q_sb, group, p.tile_tokens))) return e;
   if ((e = encode_heads(&mk, k, D, kv_heads, T, B, k_sh, k_st, k_sb, 1, kKeys))) return e;
   if ((e = encode_heads(&mv, v, D, kv_heads, T, B, v_sh, v_st, v_sb, 1, kKeys))) return e;
-  const int smem = D == 64 ? fwd_smem_bytes<64, 2>() : fwd_smem_bytes<128, 2>();
-  auto kernel = D == 64 ? window_fwd_kernel<64, false, 2> : window_fwd_kernel<128, false, 2>;
-  if (set_smem(kernel, smem)) return 5;
-  kernel<<<(unsigned)blocks, kFwdThreads<2>, smem, (cudaStream_t)stream>>>(mq, mk, mv, p);
+  if ((e = encode_heads(&mo, out, D, heads, T, B, D, heads * D, o_sb, group, p.tile_tokens))) return e;
+  if ((e = encode_heads(&ml, lse != nullptr ? low : out, D, heads, T, B, D, heads * D, o_sb, group, p.tile_tokens))) return e;
+  const unsigned grid = (unsigned)blocks;
+  if (D == 64 ? launch<64, false, 2>(grid, (cudaStream_t)stream, mq, mk, mv, mo, ml, p)
+              : launch<128, false, 2>(grid, (cudaStream_t)stream, mq, mk, mv, mo, ml, p))
+    return 5;
   return cudaGetLastError() == cudaSuccess ? 0 : 5;
 }
 
@@ -622,17 +683,9 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   if ((e = encode_heads(&mv, v_pages, D, kv_heads, page, pages, v_sh, v_ss, v_sp, 1, p.piece))) return e;
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)pairs, kv_heads, splits);
-  if (single) {
-    const int smem = D == 64 ? fwd_smem_bytes<64, 1>() : fwd_smem_bytes<128, 1>();
-    auto kernel = D == 64 ? window_fwd_kernel<64, true, 1> : window_fwd_kernel<128, true, 1>;
-    if (set_smem(kernel, smem)) return 5;
-    kernel<<<grid, kFwdThreads<1>, smem, s>>>(mq, mk, mv, p);
-  } else {
-    const int smem = D == 64 ? fwd_smem_bytes<64, 2>() : fwd_smem_bytes<128, 2>();
-    auto kernel = D == 64 ? window_fwd_kernel<64, true, 2> : window_fwd_kernel<128, true, 2>;
-    if (set_smem(kernel, smem)) return 5;
-    kernel<<<grid, kFwdThreads<2>, smem, s>>>(mq, mk, mv, p);
-  }
+  if (single ? (D == 64 ? launch<64, true, 1>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1>(grid, s, mq, mk, mv, mq, mq, p))
+             : (D == 64 ? launch<64, true, 2>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 2>(grid, s, mq, mk, mv, mq, mq, p)))
+    return 5;
   if (splits > 1) {
     const long long all = (long long)rows * kv_heads * group;
     const unsigned blocks = (unsigned)((all + 7) / 8);

@@ -1,7 +1,7 @@
 // Backward of the attention over a sliding window and the first tokens (forward and definition in window_attention.cu).
 //
 //   P = 2^(S scale log2(e) - lse),  dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta) scale,  dQ = dS K,  dK = dS^T Q,
-//   delta = rowsum(dO O)
+//   delta = rowsum(dO O), from the output and what its rounding took off
 //
 // One thread block owns 128 keys of a key head and walks the tiles of queries that see any of them; a tile's 128 rows are tokens x
 // the query heads that share the key head, so dK and dV, which sum over those heads, are summed in tensor memory.  All scores are
@@ -59,43 +59,68 @@ struct BwdParams {
   int* status;
 };
 
-// delta, and what else has to be there before the main kernel: counters at zero, dQ of the rows behind a sequence's end.
+// delta, and what else has to be there before the main kernel: counters at zero, dQ of the rows behind a sequence's end.  D / 8 threads
+// a row, four rows a thread whose loads are on their way together.
 template <int D>
-__global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restrict__ o, const elem_t* __restrict__ d_o, long long do_sb,
-                                                           long long do_st, long long do_sh, float* __restrict__ delta, int* counters,
+__global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restrict__ o, const elem_t* __restrict__ low, const elem_t* __restrict__ d_o, long long do_sb, long long do_st, long long do_sh, float* __restrict__ delta, int* counters,
                                                            int n_counters, const BwdParams p) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 8, kRowsEach = 4, kStep = 256 / kLanes;
   const long long thread = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (thread < n_counters) counters[thread] = 0;
-  const int heads = p.kv_heads * p.group;
-  const long long idx = thread / kLanes;                     // (b, t, h) row
-  const int part = threadIdx.x % kLanes;
-  const bool on = idx < (long long)p.B * p.T * heads;
-  float s = 0.0f;
-  const int h = (int)(idx % heads);
-  const long long bt = idx / heads;
-  const int t = (int)(bt % p.T), b = (int)(bt / p.T);
-  bool there = on;
-  if (on) {
-    there = p.lengths == nullptr || t < p.lengths[b];
-    if (there) {
-      const uint4 ov = *reinterpret_cast<const uint4*>(o + idx * D + part * 8);
-      const uint4 gv = *reinterpret_cast<const uint4*>(d_o + b * do_sb + t * do_st + h * do_sh + part * 8);
-      const elem2_t* oe = reinterpret_cast<const elem2_t*>(&ov);
-      const elem2_t* ge = reinterpret_cast<const elem2_t*>(&gv);
+  const int heads = p.kv_heads * p.group, part = threadIdx.x % kLanes;
+  const long long all = (long long)p.B * p.T * heads, row0 = (long long)blockIdx.x * kStep * kRowsEach + threadIdx.x / kLanes;   // (b, t, h)
+  uint4 ov[kRowsEach], lv[kRowsEach], gv[kRowsEach];
+  int h[kRowsEach], t[kRowsEach], b[kRowsEach];
+  bool there[kRowsEach];
+  const long long bt = row0 / heads;                 // divided once: the next rows are counted on
+  int h_at = (int)(row0 - bt * heads), b_at = (int)(bt / p.T), t_at = (int)(bt - (long long)b_at * p.T);
+  const int step_t = kStep / heads, step_h = kStep - step_t * heads;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x = e22ff(oe[i]), y = e22ff(ge[i]);
-        s += x.x * y.x + x.y * y.y;
-      }
+  for (int u = 0; u < kRowsEach; ++u) {
+    const long long idx = row0 + u * kStep;
+    h[u] = h_at;
+    t[u] = t_at;
+    b[u] = b_at;
+    h_at += step_h;
+    t_at += step_t;
+    if (h_at >= heads) {
+      h_at -= heads;
+      ++t_at;
+    }
+    while (t_at >= p.T) {
+      t_at -= p.T;
+      ++b_at;
+    }
+    there[u] = idx < all;
+    if (!there[u]) continue;
+    if (p.lengths != nullptr && t[u] >= p.lengths[b[u]]) {
+      there[u] = false;
+      *reinterpret_cast<uint4*>(p.dq + b[u] * p.q_sb + t[u] * p.q_st + h[u] * p.q_sh + part * 8) = make_uint4(0u, 0u, 0u, 0u);
     } else {
-      *reinterpret_cast<uint4*>(p.dq + b * p.q_sb + t * p.q_st + h * p.q_sh + part * 8) = make_uint4(0u, 0u, 0u, 0u);
+      ov[u] = *reinterpret_cast<const uint4*>(o + idx * D + part * 8);
+      lv[u] = *reinterpret_cast<const uint4*>(low + idx * D + part * 8);
+      gv[u] = *reinterpret_cast<const uint4*>(d_o + b[u] * do_sb + t[u] * do_st + h[u] * do_sh + part * 8);
     }
   }
 #pragma unroll
-  for (int off = kLanes / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  if (there && part == 0)
-    delta[(((long long)b * p.kv_heads + h / p.group) * p.tiles + t / p.tile_tokens) * kRows + t % p.tile_tokens * p.group + h % p.group] = -s;
+  for (int u = 0; u < kRowsEach; ++u) {
+    float s = 0.0f;
+    if (there[u]) {
+      const elem2_t* oe = reinterpret_cast<const elem2_t*>(&ov[u]);
+      const elem2_t* le = reinterpret_cast<const elem2_t*>(&lv[u]);
+      const elem2_t* ge = reinterpret_cast<const elem2_t*>(&gv[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = e22ff(oe[i]), z = e22ff(le[i]), y = e22ff(ge[i]);
+        s += (x.x + z.x) * y.x + (x.y + z.y) * y.y;
+      }
+    }
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (there[u] && part == 0)
+      delta[(((long long)b[u] * p.kv_heads + (unsigned)h[u] / p.group) * p.tiles + (unsigned)t[u] / p.tile_tokens) * kRows +
+            (unsigned)t[u] % p.tile_tokens * p.group + (unsigned)h[u] % p.group] = -s;
+  }
 }
 
 constexpr int kBwdWarps = 16, kBwdThreads = kBwdWarps * 32;
@@ -772,10 +797,10 @@ long long fbam_window_bwd_workspace(int B, int T, int kv_heads, int group, int D
   return a.sums + a.kv_parts + zeroed(a) + a.delta;
 }
 
-// Operands as in fbam_window_fwd; out contiguous, as the forward wrote it; d_o (B, T, heads, D) with strides; the gradients with
+// Operands as in fbam_window_fwd; out and low contiguous, as the forward wrote them; d_o (B, T, heads, D) with strides; the gradients with
 // strides each; work: fp32 workspace of fbam_window_bwd_workspace values, 16-byte aligned.
 int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_sh, const void* k, const void* v, long long k_sb,
-                    long long k_st, long long k_sh, long long v_sb, long long v_st, long long v_sh, const void* out, const void* d_o,
+                    long long k_st, long long k_sh, long long v_sb, long long v_st, long long v_sh, const void* out, const void* low, const void* d_o,
                     long long do_sb, long long do_st, long long do_sh, const float* lse, const int* lengths, float* work,
                     long long work_floats, void* dq, long long dq_sb, long long dq_st, long long dq_sh, void* dk, long long dk_sb,
                     long long dk_st, long long dk_sh, void* dv, long long dv_sb, long long dv_st, long long dv_sh, int B, int T,
@@ -783,7 +808,7 @@ int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_s
   if ((D != 64 && D != 128) || B < 1 || T < 1 || kv_heads < 1 || group < 1 || group > kRows || sinks < 0) return 1;
   const Plan a = make_plan(B, T, kv_heads, group, D, window, sinks);
   if (work_floats < a.sums + a.kv_parts + zeroed(a) + a.delta) return 1;
-  const uintptr_t outs = (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)out | (uintptr_t)work;
+  const uintptr_t outs = (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)out | (uintptr_t)low | (uintptr_t)work;
   if ((outs & 15) || dq_sb % 8 || dq_st % 8 || dq_sh % 8 || dk_sb % 8 || dk_st % 8 || dk_sh % 8 || dv_sb % 8 || dv_st % 8 || dv_sh % 8)
     return 2;
   BwdParams p = {};
@@ -808,7 +833,7 @@ int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_s
   p.v_sb = dv_sb; p.v_st = dv_st; p.v_sh = dv_sh;
   p.status = status;
   const long long rows = (long long)B * T * kv_heads * group;
-  long long threads = rows * (D / 8);
+  long long threads = (rows + 3) / 4 * (D / 8);
   if (threads < zeroed(a)) threads = zeroed(a);
   if (a.thread_blocks > 0x7fffffffll || zeroed(a) > 0x7fffffffll || (threads + 255) / 256 > 0x7fffffffll) return 1;
   CUtensorMap mq, mk, mv, mdo, mdk, mdv;
@@ -822,12 +847,12 @@ int fbam_window_bwd(const void* q, long long q_sb, long long q_st, long long q_s
   cudaStream_t s = (cudaStream_t)stream;
   const unsigned pre = (unsigned)((threads + 255) / 256);
   if (D == 64)
-    window_delta_kernel<64><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)zeroed(a), p);
+    window_delta_kernel<64><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)low, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)zeroed(a), p);
   else
-    window_delta_kernel<128><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)zeroed(a), p);
+    window_delta_kernel<128><<<pre, 256, 0, s>>>((const elem_t*)out, (const elem_t*)low, (const elem_t*)d_o, do_sb, do_st, do_sh, delta, p.counters, (int)zeroed(a), p);
   auto kernel = D == 64 ? window_bwd_kernel<64> : window_bwd_kernel<128>;
   const int smem = D == 64 ? bwd_smem_bytes<64>() : bwd_smem_bytes<128>();
-  if (set_smem(kernel, smem)) return 5;
+  if (D == 64 ? set_smem_once<window_bwd_kernel<64>>(smem) : set_smem_once<window_bwd_kernel<128>>(smem)) return 5;
   kernel<<<(unsigned)a.thread_blocks, kBwdThreads, smem, s>>>(mq, mk, mv, mdo, mdk, mdv, p);
   auto parts = D == 64 ? window_parts_kernel<64> : window_parts_kernel<128>;
   const int kb0 = a.first_parts > 1 ? 0 : a.firsts, kb1 = a.parts > 1 ? a.blocks : a.firsts;      // the blocks whose walks are divided

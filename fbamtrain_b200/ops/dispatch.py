@@ -6,6 +6,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import reference as ref
+from .derivatives import tracked
 
 import os
 
@@ -455,7 +456,6 @@ def _check_cache_native(d, k_pages, v_pages) -> None:
 
 
 def _no_gradient(name, *tensors) -> None:
-    from .derivatives import tracked
     if tracked(*tensors):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train with window_attention")
 

@@ -117,8 +117,8 @@ _ARGTYPES = {
     "fbam_logprobs_bwd": (_P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _L, _I, _F, _P),
     "fbam_rotary": (_P, _L, _L, _L, _P, _P, _I, _L, _L, _P, _I, _F, _I, _I, _L, _L, _I, _I, _I, _P),
     "fbam_cache_append": (_P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _P, _P, _P, _I, _F, _I, _L, _I, _I, _I, _I, _I, _I, _I, _P),
-    "fbam_window_fwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P),
-    "fbam_window_bwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _P, _L, _P, _L, _L, _L, _P, _L, _L, _L,
+    "fbam_window_fwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P),
+    "fbam_window_bwd": (_P, _L, _L, _L, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P, _L, _L, _L, _P, _P, _P, _L, _P, _L, _L, _L, _P, _L, _L, _L,
                         _P, _L, _L, _L, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P),
     "fbam_window_bwd_workspace": (_I, _I, _I, _I, _I, _I, _I),
     "fbam_cache_attention": (_P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,

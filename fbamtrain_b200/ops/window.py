@@ -2,7 +2,7 @@
 
 Query heads may share key heads.  Heads come as views: of three tensors, or of one fused projection ``(B, T, heads + 2 kv_heads,
 D)``, whose gradient is one tensor then (gradients of three selections would each be a zero-filled tensor of the full size).  The
-forward keeps its output and one fp32 value per query row for the backward.
+forward keeps its output, what rounding took off it and one fp32 value per query row for the backward.
 """
 from __future__ import annotations
 
@@ -30,22 +30,25 @@ def _pairs(b, t, window):
 
 
 def _forward(q, k, v, window, sinks, lengths, scale, keep):
-    """``(out, lse)``; ``lse`` with ``keep``: what the backward needs."""
+    """``(out, low, lse)``; the last two with ``keep``: what the backward needs, ``low`` being what rounding took off ``out``."""
     b, t, h, d = q.shape
     kv = k.shape[2]
     out = q.new_empty((b, t, h, d))
     tokens = 128 // (h // kv)                            # of a tile of 128 rows
-    lse = q.new_empty((b, kv, (t + tokens - 1) // tokens, 128), dtype=F32) if keep else None
+    low = lse = None
+    if keep:
+        low = torch.empty_like(out)
+        lse = q.new_empty((b, kv, (t + tokens - 1) // tokens, 128), dtype=F32)
     nv.check(nv.lib(q).fbam_window_fwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-                                       out.data_ptr(), nv.addr(lse), nv.addr(lengths), b, t, kv, h // kv, d, window or 0, sinks, scale,
+                                       out.data_ptr(), nv.addr(low), nv.addr(lse), nv.addr(lengths), b, t, kv, h // kv, d, window or 0, sinks, scale,
                                        nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_fwd")
     flops.add(4.0 * h * d * _pairs(b, t, window))
-    return out, lse
+    return out, low, lse
 
 
 def _backward(saved, d_out, into, window, sinks, scale):
     """Fills ``into``: views for the gradients of the heads."""
-    q, k, v, out, lse, lengths = saved
+    q, k, v, out, low, lse, lengths = saved
     b, t, h, d = q.shape
     kv = k.shape[2]
     if not _usable(d_out):
@@ -55,7 +58,7 @@ def _backward(saved, d_out, into, window, sinks, scale):
     work = lse.new_empty(floats)
     dq, dk, dv = into
     nv.check(lib.fbam_window_bwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-                                 out.data_ptr(), d_out.data_ptr(), *d_out.stride()[:3], lse.data_ptr(), nv.addr(lengths),
+                                 out.data_ptr(), low.data_ptr(), d_out.data_ptr(), *d_out.stride()[:3], lse.data_ptr(), nv.addr(lengths),
                                  work.data_ptr(), floats, dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(),
                                  *dv.stride()[:3], b, t, kv, h // kv, d, window or 0, sinks, scale,
                                  nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_bwd")
@@ -65,8 +68,8 @@ def _backward(saved, d_out, into, window, sinks, scale):
 class _Window(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, lengths, scale):
-        out, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        out, low, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, lengths)
         ctx.linked = ()
         ctx.how = (window, sinks, scale)
         return out
@@ -84,8 +87,8 @@ class _WindowQkv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, kv, window, sinks, lengths, scale):
         q, k, v = _heads(qkv, kv)
-        out, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
-        ctx.save_for_backward(qkv, out, lse, lengths)
+        out, low, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
+        ctx.save_for_backward(qkv, out, low, lse, lengths)
         ctx.linked = ()
         ctx.how = (window, sinks, scale)
         ctx.kv = kv
@@ -94,9 +97,9 @@ class _WindowQkv(torch.autograd.Function):
     @staticmethod
     @first_only("window_attention_qkv")
     def backward(ctx, d_out):
-        qkv, out, lse, lengths = ctx.saved_tensors
+        qkv, out, low, lse, lengths = ctx.saved_tensors
         grad = qkv.new_empty(qkv.shape)
-        _backward((*_heads(qkv, ctx.kv), out, lse, lengths), d_out, _heads(grad, ctx.kv), *ctx.how)
+        _backward((*_heads(qkv, ctx.kv), out, low, lse, lengths), d_out, _heads(grad, ctx.kv), *ctx.how)
         return grad, None, None, None, None, None
 
 
