@@ -132,15 +132,6 @@ constexpr int bwd_smem_bytes() {
   return (4 + kDoStages<D>) * 128 * D * 2 + 128 * 128 * 2 + kStages * kStage + (2 + kDoStages<D>) * 512 + 256 + 1024;
 }
 
-// Thread i of the warp receives 16 consecutive columns of row (lane_base + i).
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
 // 16 rows x 64 columns of fp32 in the layout of matrix fragments: thread t receives, for each 8 columns j, columns 8 j + 2 (t % 4) and
 // the one behind it of row t / 4 (x[4 j], x[4 j + 1]) and of row t / 4 + 8 (x[4 j + 2], x[4 j + 3]).
 __device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&x)[32]) {
@@ -202,17 +193,6 @@ __device__ __forceinline__ void store_part(float4* sum, const uint32_t (&r)[N]) 
   for (int j = 0; j < N / 4; ++j)
     __stcg(sum + j * PITCH, make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
                                         __uint_as_float(r[4 * j + 3])));
-}
-template <int PITCH, int N>
-__device__ __forceinline__ void add_from(uint32_t (&r)[N], const float4* sum) {
-#pragma unroll
-  for (int j = 0; j < N / 4; ++j) {
-    const float4 v = __ldcg(sum + j * PITCH);
-    r[4 * j] = __float_as_uint(v.x + __uint_as_float(r[4 * j]));
-    r[4 * j + 1] = __float_as_uint(v.y + __uint_as_float(r[4 * j + 1]));
-    r[4 * j + 2] = __float_as_uint(v.z + __uint_as_float(r[4 * j + 2]));
-    r[4 * j + 3] = __float_as_uint(v.w + __uint_as_float(r[4 * j + 3]));
-  }
 }
 template <int N>
 __device__ __forceinline__ void store_row(elem_t* dst, const uint32_t (&r)[N], float scale) {
@@ -700,25 +680,45 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         ++f;
       } else {
+        // the last one: the sum so far is fetched, 64 columns at a time, while its own part is on its way
         const long long tile = (long long)bh * p.tiles + m0 + i;
         const float4* sum = reinterpret_cast<const float4*>(p.sums) + tile * (D / 4) * kRows + row;
-        if (!mbar_wait(dq_full, i & 1)) { ok = false; break; }
-        fence_after_sync();
         elem_t* dst = p.dq + b * p.q_sb + t_q * p.q_st + h * p.q_sh;
-        uint32_t r[D / 16][16];
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) tmem_ld_32x16(tm_dq + lane_addr + c * 16, r[c]);
-        tmem_ld_wait();
-        fence_before_sync();
-        warp_arrive(dq_read);
         if (rank > 0) {
           if (!wait_for(p.counters + tile, rank)) { ok = false; break; }
           fence_proxy_async_all();
         }
+        float4 v[16];
+        auto fetch = [&](int half) {
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          if (rank > 0) add_from<kRows>(r[c], sum + c * 4 * kRows);
-          if (token < p.tile_tokens && t_q < len) store_row(dst + c * 16, r[c], p.scale);
+          for (int j = 0; j < 16; ++j) v[j] = rank > 0 ? __ldcg(sum + (half * 16 + j) * kRows) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        };
+        fetch(0);
+        if (!mbar_wait(dq_full, i & 1)) { ok = false; break; }
+        fence_after_sync();
+#pragma unroll
+        for (int half = 0; half < D / 64; ++half) {
+          uint32_t r[2][32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) tmem_ld_32x32(tm_dq + lane_addr + half * 64 + c * 32, r[c]);
+          tmem_ld_wait();
+          if (half + 1 == D / 64) {
+            fence_before_sync();
+            warp_arrive(dq_read);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            uint32_t* x = r[j / 8] + j % 8 * 4;
+            x[0] = __float_as_uint(v[j].x + __uint_as_float(x[0]));
+            x[1] = __float_as_uint(v[j].y + __uint_as_float(x[1]));
+            x[2] = __float_as_uint(v[j].z + __uint_as_float(x[2]));
+            x[3] = __float_as_uint(v[j].w + __uint_as_float(x[3]));
+          }
+          if (half + 1 < D / 64) fetch(half + 1);
+          if (token < p.tile_tokens && t_q < len) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) store_row(dst + half * 64 + c * 32, r[c], p.scale);
+          }
         }
       }
     }
