@@ -5,6 +5,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
+from . import native as nv
 from . import reference as ref
 from .derivatives import tracked
 
@@ -360,7 +361,8 @@ def rotary(x, positions, freqs, heads: Optional[int] = None, interleaved: bool =
         raise ValueError(f"frequencies of {freqs.dims} channels do not fit heads of {d}")
     if x.numel() and _native(x, family="mha"):
         from .positions import rotary as f
-        return f(x, positions, freqs, heads, interleaved)
+        with nv.at(x.device):
+            return f(x, positions, freqs, heads, interleaved)
     return ref.rotary(x, positions, freqs, heads, interleaved)
 
 
@@ -400,10 +402,11 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, leng
     d, wide = q.shape[3], _kernel_width(q.shape[3])
     if q.numel() and wide and _native(q, family="mha"):
         from .window import window_attention as f
-        if d == wide:
-            return f(q, k, v, window, sinks, lengths, d ** -0.5)
-        pad = (0, wide - d)
-        return f(*(torch.nn.functional.pad(x, pad) for x in (q, k, v)), window, sinks, lengths, d ** -0.5)[..., :d]
+        with nv.at(q.device):
+            if d == wide:
+                return f(q, k, v, window, sinks, lengths, d ** -0.5)
+            pad = (0, wide - d)
+            return f(*(torch.nn.functional.pad(x, pad) for x in (q, k, v)), window, sinks, lengths, d ** -0.5)[..., :d]
     return ref.window_attention(q, k, v, window, sinks, lengths)
 
 
@@ -418,9 +421,10 @@ def window_attention_qkv(qkv, kv_heads: int, window: Optional[int] = None, sinks
     d, wide = qkv.shape[3], _kernel_width(qkv.shape[3])
     if qkv.numel() and wide and _native(qkv, family="mha"):
         from .window import window_attention_qkv as f
-        if d == wide:
-            return f(qkv, kv_heads, window, sinks, lengths, d ** -0.5)
-        return f(torch.nn.functional.pad(qkv, (0, wide - d)), kv_heads, window, sinks, lengths, d ** -0.5)[..., :d]
+        with nv.at(qkv.device):
+            if d == wide:
+                return f(qkv, kv_heads, window, sinks, lengths, d ** -0.5)
+            return f(torch.nn.functional.pad(qkv, (0, wide - d)), kv_heads, window, sinks, lengths, d ** -0.5)[..., :d]
     return ref.window_attention(*qkv.split((heads, kv_heads, kv_heads), 2), window, sinks, lengths)
 
 
@@ -450,8 +454,8 @@ def _check_cache_native(d, k_pages, v_pages) -> None:
     if k_pages.shape[1] % 8:
         raise ValueError(f"pages have a multiple of 8 slots, got {k_pages.shape[1]}")
     for x in (k_pages, v_pages):
-        sp, ss, sh, sd = x.stride()
-        if sd != 1 or sp % 8 or ss % 8 or sh % 8 or x.data_ptr() % 16:
+        *outer, inner = x.stride()
+        if inner != 1 or x.data_ptr() % 16 or any(s % 8 or (s == 0 and n > 1) for s, n in zip(outer, x.shape)):
             raise ValueError("pages start at 16-byte boundaries, with 16-byte strides and channels side by side")
 
 
@@ -485,7 +489,8 @@ def cache_append(qkv, k_pages, v_pages, tables, lengths, offsets=None, freqs=Non
         if freqs is not None and freqs.dims % (8 if interleaved else 16):
             raise ValueError(f"the kernels turn a multiple of {8 if interleaved else 16} channels in a cache, got {freqs.dims}")
         from .positions import cache_append as f
-        return f(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interleaved, heads, kv)
+        with nv.at(qkv.device):
+            return f(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interleaved, heads, kv)
     return ref.cache_append(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interleaved, heads, kv)
 
 
@@ -504,5 +509,6 @@ def cache_attention(q, k_pages, v_pages, tables, lengths, offsets=None, window: 
     if n and tables.shape[0] and _native(q, family="mha"):
         _check_cache_native(d, k_pages, v_pages)
         from .window import cache_attention as f
-        return f(q, k_pages, v_pages, tables, lengths, offsets, window, sinks)
+        with nv.at(q.device):
+            return f(q, k_pages, v_pages, tables, lengths, offsets, window, sinks)
     return ref.cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks)

@@ -9,6 +9,7 @@ silently.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from typing import Optional
@@ -189,6 +190,14 @@ def check(code: int, what: str) -> None:
     recording = _plan.active()
     if recording is not None:
         recording.on_launch(what)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def at(device: torch.device):
+    """A context in which ``device`` is the current one: launches and allocations of a call go where its operands are."""
+    return _HERE_ALREADY if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def stream_ptr() -> C.c_void_p:

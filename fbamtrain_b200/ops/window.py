@@ -18,9 +18,14 @@ F32 = torch.float32
 
 
 def _usable(x: torch.Tensor) -> bool:
-    """Whether the copy engine can fetch ``x`` ``(B, T, H, D)`` where it lies: 16-byte strides and start."""
-    sb, st, sh, sd = x.stride()
-    return sd == 1 and not (sb % 8 or st % 8 or sh % 8) and x.data_ptr() % 16 == 0
+    """Whether the copy engine can fetch ``x`` ``(..., heads, channels)`` where it lies: channels side by side, a start and strides of 16
+    bytes, nothing expanded."""
+    *outer, inner = x.stride()
+    return inner == 1 and x.data_ptr() % 16 == 0 and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in zip(outer, x.shape))
+
+
+def _fetchable(x: torch.Tensor) -> torch.Tensor:
+    return x if _usable(x) else x.clone(memory_format=torch.contiguous_format)
 
 
 def _pairs(b, t, window):
@@ -51,8 +56,7 @@ def _backward(saved, d_out, into, window, sinks, scale):
     q, k, v, out, low, lse, lengths = saved
     b, t, h, d = q.shape
     kv = k.shape[2]
-    if not _usable(d_out):
-        d_out = d_out.clone(memory_format=torch.contiguous_format)
+    d_out = _fetchable(d_out)
     lib = nv.lib(q)
     floats = lib.fbam_window_bwd_workspace(b, t, kv, h // kv, d, window or 0, sinks)
     work = lse.new_empty(floats)
@@ -120,7 +124,7 @@ def window_attention(q, k, v, window, sinks, lengths, scale):
     for name, x in (("keys", k), ("values", v)):
         if x.device != q.device:
             raise ValueError(f"{name} are on {x.device}, the queries on {q.device}")
-    q, k, v = (x if _usable(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
+    q, k, v = _fetchable(q), _fetchable(k), _fetchable(v)
     if tracked(q, k, v):
         return _Window.apply(q, k, v, window, sinks, lengths, scale)
     return _forward(q, k, v, window, sinks, lengths, scale, False)[0]
@@ -128,8 +132,7 @@ def window_attention(q, k, v, window, sinks, lengths, scale):
 
 def window_attention_qkv(qkv, kv, window, sinks, lengths, scale):
     lengths = _lengths(lengths, qkv)
-    if not _usable(qkv):
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    qkv = _fetchable(qkv)
     if tracked(qkv):
         return _WindowQkv.apply(qkv, kv, window, sinks, lengths, scale)
     return _forward(*_heads(qkv, kv), window, sinks, lengths, scale, False)[0]
@@ -155,8 +158,7 @@ def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks
     n, h, d = q.shape
     b, most = tables.shape
     pages, page, kv, _ = k_pages.shape
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
+    q = _fetchable(q)
     out = q.new_empty((n, h, d))
     lib = nv.lib(q)
     per = 2 * (128 // (h // kv))
