@@ -15,7 +15,7 @@
 // Bound by memory: each value is read and written once.  A thread has one piece of a head (in the half layout 8 channels and the 8 that
 // they turn with) and walks the heads of its token, four at a time: it forms its sines and cosines once, in registers, and the heads'
 // loads are on their way together.  A first form kept the angles of a few tokens in shared memory and gave pieces to threads in any
-// order: a block's loads waited for its angles and every piece for two divisions (27 against NEW us at 8192 tokens of 48 heads of 64).
+// order: a block's loads waited for its angles and every piece for two divisions (27 against 20 us at 8192 tokens of 48 heads of 64).
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include "elem16.cuh"

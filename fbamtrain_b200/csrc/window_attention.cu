@@ -5,13 +5,13 @@
 //
 //   o_i = sum_j p_ij v_j,  p_ij = 2^(s_ij scale log2(e) - m_i) / l_i,  s = q k^T,  m the running maximum, l the running sum
 //
-// One thread block takes two tiles of queries of one key head.  A tile's 128 rows are TOKENS x the query heads that share the
+// One thread block takes one or two tiles of queries of one key head.  A tile's 128 rows are TOKENS x the query heads that share the
 // key head, so a key block is read once for all of them and one token of a shared head fills as many rows as there are heads.
 // Key blocks of 128 pass through a ring in shared memory, K and V in turn; only blocks that some row of the tiles sees are
 // visited (those of the first tokens, then those of the window).  Per block and tile: S = Q K^T into tensor memory
 // (tcgen05.mma); four softmax warps, one row a thread, read S, form the exponentials and write P over S as 16-bit values; the
 // second product takes P from tensor memory and adds P V to the tile's output there, which is rescaled only when a row's
-// maximum has grown by more than 2^8.  The two tiles take turns on the tensor cores.
+// maximum has grown by more than 2^8.  Two tiles take turns on the tensor cores.
 //
 // Over a cache the ring is filled page by page: the lanes of the loading warp each look up one page (or part of one of 128 slots
 // or more) and issue its copy.  Entries that are no page, slots behind the sequence and pages that nothing sees are filled with
@@ -52,15 +52,18 @@ struct FwdParams {
   int* status;
 };
 
-// TILES = 2: two tiles a thread block, one thread block a multiprocessor.  TILES = 1: one tile of one token with up to 16 heads, two
-// thread blocks a multiprocessor: such a tile has little to do for each key block that arrives, and two of them hide each other's waits.
-// Its Q keeps 16 rows a panel; what the product reads behind them are other buffers, in rows that nobody looks at.
-template <int D, int TILES>
-constexpr int kSlots = TILES == 2 ? (D == 64 ? 8 : 5) : (D == 64 ? 6 : 3);
-template <int TILES>
-constexpr int kQPanel = TILES == 2 ? kRows * 128 : 16 * 128;       // bytes of 64 channels of a tile
-template <int D, int TILES>
-constexpr int fwd_smem_bytes() { return TILES * (D / 64) * kQPanel<TILES> + kSlots<D, TILES> * kKeys * D * 2 + 256 + 1024; }
+// TILES = 2: two tiles a thread block, one thread block a multiprocessor: they share each key block.
+// TILES = 1: one tile a thread block, two thread blocks a multiprocessor, where all of them fit at once (296): 3 x 696 with a window
+// of 2, 8 heads of 128: 11.9 against 16.5 us; 8 x 1024, window 256, 16 heads of 64, where they do not: 65 against 48 us.
+// ONE: that tile is one token with up to 16 heads.  It has little to do for each key block that arrives, and two of them hide each
+// other's waits.  Its Q keeps 16 rows a panel; what the product reads behind them are other buffers, in rows that nobody looks at.
+constexpr int kResident = 296;
+template <int D, int TILES, bool ONE>
+constexpr int kSlots = TILES == 2 ? (D == 64 ? 8 : 5) : (D == 64 ? 6 : ONE ? 3 : 2);
+template <bool ONE>
+constexpr int kQPanel = ONE ? 16 * 128 : kRows * 128;              // bytes of 64 channels of a tile
+template <int D, int TILES, bool ONE>
+constexpr int fwd_smem_bytes() { return TILES * (D / 64) * kQPanel<ONE> + kSlots<D, TILES, ONE> * kKeys * D * 2 + 256 + 1024; }
 template <int TILES>
 constexpr int kFwdThreads = TILES * 128 + 128;                     // MMA issue, loads, two idle warps; four softmax warps a tile
 
@@ -81,20 +84,20 @@ __device__ __forceinline__ Span make_span(int i0, int i1, int base, int key_end,
   return s;
 }
 
-template <int D, bool PAGED, int TILES>
+template <int D, bool PAGED, int TILES, bool ONE>
 __global__ void __launch_bounds__(kFwdThreads<TILES>, TILES == 2 ? 1 : 2)
 window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
                   const __grid_constant__ CUtensorMap map_low, const __grid_constant__ FwdParams p) {
   constexpr int DP = D / 64;                 // 64-wide panels per row
-  constexpr int kQBytes = DP * kQPanel<TILES>;   // one tile
+  constexpr int kQBytes = DP * kQPanel<ONE>; // one tile
   constexpr int kKVBytes = kKeys * D * 2;
-  constexpr int NS = kSlots<D, TILES>;
+  constexpr int NS = kSlots<D, TILES, ONE>;
   constexpr uint32_t kTmemO = TILES * 128, kTmemCols = TILES * 256;   // S/P of each tile, 128 columns; then O of each, D
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                        // TILES tiles
-  uint8_t* sKV = sQ + TILES * kQBytes;           // NS slots: K and V of the blocks in turn
+  uint8_t* sKV = sQ + TILES * kQBytes;       // NS slots: K and V of the blocks in turn
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + NS * kKVBytes);
   uint64_t* q_full = bars;
   uint64_t* full = bars + 1;                 // [NS]
@@ -233,114 +236,114 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     else
       asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  if (warp == 1) {
-    // ---------------------------------------------------------------- loads
-    bool ok = true;
-    if (lane == 0) {
-      const int tiles = span[TILES - 1].hi >= 0 ? TILES : 1;
-      mbar_expect_tx(q_full, tiles * p.tile_tokens * p.group * D * 2);
-      for (int g = 0; g < tiles; ++g)
+    if (warp == 1) {
+      // ---------------------------------------------------------------- loads
+      bool ok = true;
+      if (lane == 0) {
+        const int tiles = span[TILES - 1].hi >= 0 ? TILES : 1;
+        mbar_expect_tx(q_full, tiles * p.tile_tokens * p.group * D * 2);
+        for (int g = 0; g < tiles; ++g)
 #pragma unroll
-        for (int j = 0; j < DP; ++j)           // rows beyond the tensor are filled with zeros
-          tma_load_4d(sQ + g * kQBytes + j * kQPanel<TILES>, &map_q, q_full, j * 64, kvh * p.group, row0 + tok0 + g * p.tile_tokens,
-                      PAGED ? 0 : b);
-    }
-    // the page (or part of it) that this lane fetches of a block; the number of pages where there is nothing to fetch
-    auto look_up = [&](int kb) {
-      const int key = kb * kKeys + lane * p.piece;
-      int id = -1;
-      if (lane * p.piece < kKeys && key < end && (key < sink_end || key + p.piece > near)) {
-        const int at = key / p.page;
-        if (at < p.max_pages) id = p.tables[b * p.t_sb + at];
+          for (int j = 0; j < DP; ++j)           // rows beyond the tensor are filled with zeros
+            tma_load_4d(sQ + g * kQBytes + j * kQPanel<ONE>, &map_q, q_full, j * 64, kvh * p.group, row0 + tok0 + g * p.tile_tokens,
+                        PAGED ? 0 : b);
       }
-      return id < 0 || id >= p.pages ? p.pages : id;
-    };
-    int next = 0;
-    if (PAGED) next = look_up(block_of(c0));
-    for (int c = c0; c < c1 && ok; ++c) {
-      const int kb = block_of(c), id = next;
-      if (PAGED && c + 1 < c1) next = look_up(block_of(c + 1));
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int f = 2 * (c - c0) + kv, s = f % NS;
-        if (f >= NS && !mbar_wait(&empty[s], (f / NS - 1) & 1)) { ok = false; break; }
-        const CUtensorMap* map = kv ? &map_v : &map_k;
-        if (lane == 0) mbar_expect_tx(&full[s], kKVBytes);
-        __syncwarp();
-        if constexpr (PAGED) {
-          if (lane * p.piece < kKeys) {
-            const int slot = (kb * kKeys + lane * p.piece) % p.page;
-#pragma unroll
-            for (int j = 0; j < DP; ++j)
-              tma_load_4d(sKV + s * kKVBytes + j * kKeys * 128 + lane * p.piece * 128, map, &full[s], j * 64, kvh, slot, id);
-          }
-        } else if (lane == 0) {
-#pragma unroll
-          for (int j = 0; j < DP; ++j) tma_load_4d(sKV + s * kKVBytes + j * kKeys * 128, map, &full[s], j * 64, kvh, kb * kKeys, b);
+      // the page (or part of it) that this lane fetches of a block; the number of pages where there is nothing to fetch
+      auto look_up = [&](int kb) {
+        const int key = kb * kKeys + lane * p.piece;
+        int id = -1;
+        if (lane * p.piece < kKeys && key < end && (key < sink_end || key + p.piece > near)) {
+          const int at = key / p.page;
+          if (at < p.max_pages) id = p.tables[b * p.t_sb + at];
         }
-      }
-    }
-    if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
-  } else if (warp == 0) {
-    // ---------------------------------------------------------------- products
-    if (elect_one()) {
-      const uint32_t idesc_s = make_idesc_f16kind(128, kKeys, false, false);
-      const uint32_t idesc_pv = make_idesc_f16kind(128, D, false, true);   // B = V is MN-major
-      auto wait_full = [&](int f) { return mbar_wait(&full[f % NS], (f / NS) & 1); };
-      const uint64_t kQ = k_major(smem_u32(sQ)), kKV = k_major(smem_u32(sKV)), mKV = mn_major(smem_u32(sKV));
-      auto issue_s = [&](int g, int f) {       // S_g = Q_g K^T
-        const uint64_t a = kQ + g * (kQBytes >> 4), bk = kKV + f % NS * (kKVBytes >> 4);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_f16_ss(tmem + g * 128, a + ((k / 4 * kQPanel<TILES> + k % 4 * 32) >> 4), bk + k_step(k), idesc_s, k != 0);
-        mma_commit(&s_full[g]);
+        return id < 0 || id >= p.pages ? p.pages : id;
       };
-      auto issue_pv = [&](int g, int f, bool first) {     // O_g (+)= P_g V
-        const uint64_t bv = mKV + f % NS * (kKVBytes >> 4);
-#pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          mma_f16_ts(tmem + kTmemO + g * D, tmem + g * 128 + k * 8, bv + mn_step(k), idesc_pv, !first || k != 0);
-        mma_commit(&pv_full[g]);
-      };
-      int done[TILES] = {};                    // blocks of each tile whose P V has been issued
-      bool ok = mbar_wait(q_full, 0) && wait_full(0);
-      if (ok) {
-        fence_after_sync();
-        const int kb = block_of(c0);
-        if (needed(span[0], kb)) issue_s(0, 0);
-        if (TILES == 2 && needed(span[TILES - 1], kb)) issue_s(TILES - 1, 0);
-        mma_commit(&empty[0]);
-      }
+      int next = 0;
+      if (PAGED) next = look_up(block_of(c0));
       for (int c = c0; c < c1 && ok; ++c) {
-        const int f = 2 * (c - c0), kb = block_of(c);
-        const bool more = c + 1 < c1;
-        const int kb1 = more ? block_of(c + 1) : -1;
-        if (!wait_full(f + 1)) { ok = false; break; }
-        auto step_pv = [&](int g) {
-          if (!needed(g == 0 ? span[0] : span[TILES - 1], kb)) return;
-          if (!mbar_wait(&p_ready[g], done[g] & 1)) { ok = false; return; }
-          fence_after_sync();
-          issue_pv(g, f + 1, done[g] == 0);
-          ++done[g];
-        };
-        step_pv(0);
-        if (!ok) break;
-        if (more) {
-          if (!wait_full(f + 2)) { ok = false; break; }
-          fence_after_sync();
-          if (needed(span[0], kb1)) issue_s(0, f + 2);   // S_0 of this block was read before p_ready[0] arrived
-        }
-        if (TILES == 2) step_pv(TILES - 1);
-        if (!ok) break;
-        mma_commit(&empty[(f + 1) % NS]);
-        if (more) {
-          if (TILES == 2 && needed(span[TILES - 1], kb1)) issue_s(TILES - 1, f + 2);
-          mma_commit(&empty[(f + 2) % NS]);
+        const int kb = block_of(c), id = next;
+        if (PAGED && c + 1 < c1) next = look_up(block_of(c + 1));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int f = 2 * (c - c0) + kv, s = f % NS;
+          if (f >= NS && !mbar_wait(&empty[s], (f / NS - 1) & 1)) { ok = false; break; }
+          const CUtensorMap* map = kv ? &map_v : &map_k;
+          if (lane == 0) mbar_expect_tx(&full[s], kKVBytes);
+          __syncwarp();
+          if constexpr (PAGED) {
+            if (lane * p.piece < kKeys) {
+              const int slot = (kb * kKeys + lane * p.piece) % p.page;
+#pragma unroll
+              for (int j = 0; j < DP; ++j)
+                tma_load_4d(sKV + s * kKVBytes + j * kKeys * 128 + lane * p.piece * 128, map, &full[s], j * 64, kvh, slot, id);
+            }
+          } else if (lane == 0) {
+#pragma unroll
+            for (int j = 0; j < DP; ++j) tma_load_4d(sKV + s * kKVBytes + j * kKeys * 128, map, &full[s], j * 64, kvh, kb * kKeys, b);
+          }
         }
       }
-      if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
+      if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
+    } else if (warp == 0) {
+      // ---------------------------------------------------------------- products
+      if (elect_one()) {
+        const uint32_t idesc_s = make_idesc_f16kind(128, kKeys, false, false);
+        const uint32_t idesc_pv = make_idesc_f16kind(128, D, false, true);   // B = V is MN-major
+        auto wait_full = [&](int f) { return mbar_wait(&full[f % NS], (f / NS) & 1); };
+        const uint64_t kQ = k_major(smem_u32(sQ)), kKV = k_major(smem_u32(sKV)), mKV = mn_major(smem_u32(sKV));
+        auto issue_s = [&](int g, int f) {       // S_g = Q_g K^T
+          const uint64_t a = kQ + g * (kQBytes >> 4), bk = kKV + f % NS * (kKVBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_f16_ss(tmem + g * 128, a + ((k / 4 * kQPanel<ONE> + k % 4 * 32) >> 4), bk + k_step(k), idesc_s, k != 0);
+          mma_commit(&s_full[g]);
+        };
+        auto issue_pv = [&](int g, int f, bool first) {     // O_g (+)= P_g V
+          const uint64_t bv = mKV + f % NS * (kKVBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            mma_f16_ts(tmem + kTmemO + g * D, tmem + g * 128 + k * 8, bv + mn_step(k), idesc_pv, !first || k != 0);
+          mma_commit(&pv_full[g]);
+        };
+        int done[TILES] = {};                    // blocks of each tile whose P V has been issued
+        bool ok = mbar_wait(q_full, 0) && wait_full(0);
+        if (ok) {
+          fence_after_sync();
+          const int kb = block_of(c0);
+          if (needed(span[0], kb)) issue_s(0, 0);
+          if (TILES == 2 && needed(span[TILES - 1], kb)) issue_s(TILES - 1, 0);
+          mma_commit(&empty[0]);
+        }
+        for (int c = c0; c < c1 && ok; ++c) {
+          const int f = 2 * (c - c0), kb = block_of(c);
+          const bool more = c + 1 < c1;
+          const int kb1 = more ? block_of(c + 1) : -1;
+          if (!wait_full(f + 1)) { ok = false; break; }
+          auto step_pv = [&](int g) {
+            if (!needed(g == 0 ? span[0] : span[TILES - 1], kb)) return;
+            if (!mbar_wait(&p_ready[g], done[g] & 1)) { ok = false; return; }
+            fence_after_sync();
+            issue_pv(g, f + 1, done[g] == 0);
+            ++done[g];
+          };
+          step_pv(0);
+          if (!ok) break;
+          if (more) {
+            if (!wait_full(f + 2)) { ok = false; break; }
+            fence_after_sync();
+            if (needed(span[0], kb1)) issue_s(0, f + 2);   // S_0 of this block was read before p_ready[0] arrived
+          }
+          if (TILES == 2) step_pv(TILES - 1);
+          if (!ok) break;
+          mma_commit(&empty[(f + 1) % NS]);
+          if (more) {
+            if (TILES == 2 && needed(span[TILES - 1], kb1)) issue_s(TILES - 1, f + 2);
+            mma_commit(&empty[(f + 2) % NS]);
+          }
+        }
+        if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
+      }
     }
-  }
   } else {
     if constexpr (TILES == 2)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -358,7 +361,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t lane_addr = uint32_t(lane_group * 32) << 16;
     const uint32_t tmem_s = tmem + g * 128, tmem_pv = tmem + kTmemO + g * D;
     const Span mine = g == 0 ? span[0] : span[TILES - 1];
-    const bool idle = TILES == 1 && lane_group * 32 >= p.group;   // rows that nobody looks at
+    const bool idle = ONE && lane_group * 32 >= p.group;   // rows that nobody looks at
     // m is the reference of the exponentials accumulated so far: p = 2^((s - m) scale).  It follows the running row maximum only
     // when that has moved by more than 2^8 past it, so that the output accumulator is rescaled on a few blocks only (values of p
     // stay below 2^8, far inside the 16-bit range; the final division by the row sum uses the same reference).
@@ -369,8 +372,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int kb = block_of(c);
       if (!needed(mine, kb)) continue;
       const int k0 = kb * kKeys;
+      if (!mbar_wait(&s_full[g], it & 1)) { ok = false; break; }
+      fence_after_sync();
       if (k0 + kKeys > end || (k0 < near && k0 + kKeys > sink_end)) {
-        // rows of V that no query of this block sees
+        // rows of V that no query of this block sees.  S of this block is there, so the block before has been used up: a wait on V's
+        // barrier any earlier could take the phase before for this one.
         const int f = 2 * (c - c0) + 1;
         if (!mbar_wait(&full[f % NS], (f / NS) & 1)) { ok = false; break; }
         const int key = k0 + row;
@@ -381,8 +387,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         fence_proxy_async_smem();
       }
-      if (!mbar_wait(&s_full[g], it & 1)) { ok = false; break; }
-      fence_after_sync();
       if (idle) {
         warp_arrive(&p_ready[g]);
         ++it;
@@ -532,7 +536,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                   hh[q] = ff2e2(o.x - rounded.x, o.y - rounded.y);
                 }
               }
-              *reinterpret_cast<uint4*>(sQ + g * kQBytes + d0 / 64 * kQPanel<TILES> + swz(row, d0 % 64 / 8 + d / 8)) = *reinterpret_cast<uint4*>(hh);
+              *reinterpret_cast<uint4*>(sQ + g * kQBytes + d0 / 64 * kQPanel<ONE> + swz(row, d0 % 64 / 8 + d / 8)) = *reinterpret_cast<uint4*>(hh);
             }
           }
           fence_proxy_async_smem();
@@ -540,7 +544,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (lane_group == 0 && tok0 + g * p.tile_tokens < p.T && elect_one()) {
 #pragma unroll
             for (int j = 0; j < DP; ++j)
-              tma_store_4d(pass ? &map_low : &map_out, sQ + g * kQBytes + j * kQPanel<TILES>, j * 64, kvh * p.group, tok0 + g * p.tile_tokens, b);
+              tma_store_4d(pass ? &map_low : &map_out, sQ + g * kQBytes + j * kQPanel<ONE>, j * 64, kvh * p.group, tok0 + g * p.tile_tokens, b);
             bulk_commit_group();
             bulk_wait_group_read<0>();
           }
@@ -553,7 +557,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (partial) {
           p.part_ml[(long long)split * p.T * heads + at] = make_float2(l > 0.0f ? m * p.scale_log2 : -INFINITY, l);
         } else if (!PAGED && p.lse != nullptr) {
-          p.lse[(((long long)b * p.kv_heads + kvh) * p.tiles + pair * 2 + g) * kRows + row] = l > 0.0f ? -(m * p.scale_log2 + log2f(l)) : 0.0f;
+          p.lse[(((long long)b * p.kv_heads + kvh) * p.tiles + pair * TILES + g) * kRows + row] = l > 0.0f ? -(m * p.scale_log2 + log2f(l)) : 0.0f;
         }
       }
     }
@@ -593,12 +597,12 @@ __global__ void __launch_bounds__(256) window_join_kernel(const float* part_o, c
   for (int v = 0; v < V; v += 2) *reinterpret_cast<elem2_t*>(dst + v) = ff2e2(o[v] * inv, o[v + 1] * inv);
 }
 
-template <int D, bool PAGED, int TILES>
+template <int D, bool PAGED, int TILES, bool ONE>
 int launch(dim3 grid, cudaStream_t s, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& out, const CUtensorMap& low,
            const FwdParams& p) {
-  constexpr int smem = fwd_smem_bytes<D, TILES>();
-  if (set_smem_once<window_fwd_kernel<D, PAGED, TILES>>(smem)) return 5;
-  window_fwd_kernel<D, PAGED, TILES><<<grid, kFwdThreads<TILES>, smem, s>>>(q, k, v, out, low, p);
+  constexpr int smem = fwd_smem_bytes<D, TILES, ONE>();
+  if (set_smem_once<window_fwd_kernel<D, PAGED, TILES, ONE>>(smem)) return 5;
+  window_fwd_kernel<D, PAGED, TILES, ONE><<<grid, kFwdThreads<TILES>, smem, s>>>(q, k, v, out, low, p);
   return 0;
 }
 
@@ -625,7 +629,10 @@ int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_s
   p.lse = lse;
   p.tiles = (T + p.tile_tokens - 1) / p.tile_tokens;
   p.status = status;
-  const long long pairs = (T + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens), blocks = pairs * B * kv_heads;
+  const long long tiles = (long long)p.tiles * B * kv_heads;
+  const bool one_tile = tiles <= kResident;
+  const int per = (one_tile ? 1 : 2) * p.tile_tokens;
+  const long long blocks = (long long)((T + per - 1) / per) * B * kv_heads;
   if (blocks > 0x7fffffffll) return 1;
   const int heads = kv_heads * group;
   const long long o_sb = (long long)T * heads * D;
@@ -637,8 +644,9 @@ int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_s
   if ((e = encode_heads(&mo, out, D, heads, T, B, D, heads * D, o_sb, group, p.tile_tokens))) return e;
   if ((e = encode_heads(&ml, lse != nullptr ? low : out, D, heads, T, B, D, heads * D, o_sb, group, p.tile_tokens))) return e;
   const unsigned grid = (unsigned)blocks;
-  if (D == 64 ? launch<64, false, 2>(grid, (cudaStream_t)stream, mq, mk, mv, mo, ml, p)
-              : launch<128, false, 2>(grid, (cudaStream_t)stream, mq, mk, mv, mo, ml, p))
+  cudaStream_t s = (cudaStream_t)stream;
+  if (one_tile ? (D == 64 ? launch<64, false, 1, false>(grid, s, mq, mk, mv, mo, ml, p) : launch<128, false, 1, false>(grid, s, mq, mk, mv, mo, ml, p))
+               : (D == 64 ? launch<64, false, 2, false>(grid, s, mq, mk, mv, mo, ml, p) : launch<128, false, 2, false>(grid, s, mq, mk, mv, mo, ml, p)))
     return 5;
   return cudaGetLastError() == cudaSuccess ? 0 : 5;
 }
@@ -674,8 +682,10 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   // pairs of tiles: one a sequence without offsets; with them, at most one that is not full of each sequence
   const bool single = offsets == nullptr && group <= 16;
   if (single) p.tile_tokens = 1;
-  const int per = 2 * p.tile_tokens;
-  const long long pairs = offsets == nullptr ? B : rows / per + (rows < B ? rows : B) + 1;
+  const long long spare = (rows < B ? rows : B) + 1;
+  const bool one_tile = !single && splits == 1 && (rows / p.tile_tokens + spare) * kv_heads <= kResident;
+  const int per = (one_tile ? 1 : 2) * p.tile_tokens;
+  const long long pairs = offsets == nullptr ? B : rows / per + spare;
   int e;
   CUtensorMap mq, mk, mv;
   if ((e = encode_heads(&mq, q, D, kv_heads * group, rows, 1, q_sh, q_st, (long long)rows * q_st, group, p.tile_tokens))) return e;
@@ -683,8 +693,9 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   if ((e = encode_heads(&mv, v_pages, D, kv_heads, page, pages, v_sh, v_ss, v_sp, 1, p.piece))) return e;
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)pairs, kv_heads, splits);
-  if (single ? (D == 64 ? launch<64, true, 1>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1>(grid, s, mq, mk, mv, mq, mq, p))
-             : (D == 64 ? launch<64, true, 2>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 2>(grid, s, mq, mk, mv, mq, mq, p)))
+  if (single     ? (D == 64 ? launch<64, true, 1, true>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, true>(grid, s, mq, mk, mv, mq, mq, p))
+      : one_tile ? (D == 64 ? launch<64, true, 1, false>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, false>(grid, s, mq, mk, mv, mq, mq, p))
+                 : (D == 64 ? launch<64, true, 2, false>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 2, false>(grid, s, mq, mk, mv, mq, mq, p)))
     return 5;
   if (splits > 1) {
     const long long all = (long long)rows * kv_heads * group;

@@ -331,138 +331,138 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   // Registers go where the scores are: four warps of 96, four of 144 and eight of 136 of the 128 a thread that the block was launched with.
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-  if (warp == 13) {
-    if (elect_one()) {
-      bool ok = true;
-      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int t) {
+    if (warp == 13) {
+      if (elect_one()) {
+        bool ok = true;
+        auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int t) {
 #pragma unroll
-        for (int j = 0; j < DP; ++j) tma_load_4d(dst + j * 128 * 128, map, bar, j * 64, head, t, b);
-      };
-      auto load_q = [&](int i) {
-        if (i >= 2 && !mbar_wait(&q_free[i & 1], ((i >> 1) - 1) & 1)) { ok = false; return; }
-        mbar_expect_tx(&q_full[i & 1], used * D * 2 + 512);
-        bulk_load(sL + (i & 1) * 128, p.lse + ((long long)bh * p.tiles + m0 + i) * kRows, 512, &q_full[i & 1]);
-        load(sQ + (i & 1) * kTile, &map_q, &q_full[i & 1], kvh * p.group, (m0 + i) * p.tile_tokens);
-      };
-      auto load_do = [&](int i) {
-        const int s = i % DOS;
-        if (i >= DOS && !mbar_wait(&do_free[s], (i / DOS - 1) & 1)) { ok = false; return; }
-        mbar_expect_tx(&do_full[s], used * D * 2 + 512);
-        bulk_load(sD + s * 128, p.delta + ((long long)bh * p.tiles + m0 + i) * kRows, 512, &do_full[s]);
-        load(sDO + s * kTile, &map_do, &do_full[s], kvh * p.group, (m0 + i) * p.tile_tokens);
-      };
-      mbar_expect_tx(kv_full, 2 * kTile);
-      load(sK, &map_k, kv_full, kvh, k0);
-      load_q(0);
-      load(sV, &map_v, kv_full, kvh, k0);
-      load_do(0);
-      if (n > 1) load_q(1);
-      for (int i = 1; i < n && ok; ++i) {
-        load_do(i);
-        if (ok && i + 1 < n) load_q(i + 1);
+          for (int j = 0; j < DP; ++j) tma_load_4d(dst + j * 128 * 128, map, bar, j * 64, head, t, b);
+        };
+        auto load_q = [&](int i) {
+          if (i >= 2 && !mbar_wait(&q_free[i & 1], ((i >> 1) - 1) & 1)) { ok = false; return; }
+          mbar_expect_tx(&q_full[i & 1], used * D * 2 + 512);
+          bulk_load(sL + (i & 1) * 128, p.lse + ((long long)bh * p.tiles + m0 + i) * kRows, 512, &q_full[i & 1]);
+          load(sQ + (i & 1) * kTile, &map_q, &q_full[i & 1], kvh * p.group, (m0 + i) * p.tile_tokens);
+        };
+        auto load_do = [&](int i) {
+          const int s = i % DOS;
+          if (i >= DOS && !mbar_wait(&do_free[s], (i / DOS - 1) & 1)) { ok = false; return; }
+          mbar_expect_tx(&do_full[s], used * D * 2 + 512);
+          bulk_load(sD + s * 128, p.delta + ((long long)bh * p.tiles + m0 + i) * kRows, 512, &do_full[s]);
+          load(sDO + s * kTile, &map_do, &do_full[s], kvh * p.group, (m0 + i) * p.tile_tokens);
+        };
+        mbar_expect_tx(kv_full, 2 * kTile);
+        load(sK, &map_k, kv_full, kvh, k0);
+        load_q(0);
+        load(sV, &map_v, kv_full, kvh, k0);
+        load_do(0);
+        if (n > 1) load_q(1);
+        for (int i = 1; i < n && ok; ++i) {
+          load_do(i);
+          if (ok && i + 1 < n) load_q(i + 1);
+        }
+        if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
       }
-      if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
-    }
-  } else if (warp == 12) {
-    if (elect_one()) {
-      bool ok = true;
-      const uint32_t id_s = make_idesc_f16kind(128, 128, false, false);   // S^T = K Q^T, dP^T = V dO^T
-      const uint32_t id_t = make_idesc_f16kind(128, D, false, true);      // dV = P^T dO, dK = dS^T Q (B MN-major)
-      const uint32_t id_q = make_idesc_f16kind(128, D, true, true);       // dQ = dS K (A, B MN-major)
-      const uint64_t kK = k_major(smem_u32(sK)), kV = k_major(smem_u32(sV)), kQ = k_major(smem_u32(sQ)), kDO = k_major(smem_u32(sDO));
-      const uint64_t mK = mn_major(smem_u32(sK)), mQ = mn_major(smem_u32(sQ)), mDO = mn_major(smem_u32(sDO));
-      const uint64_t kDS = k_major(smem_u32(sDS)), mDS = mn_major(smem_u32(sDS));
-      constexpr uint64_t kNext = kTile >> 4;                              // to the next stage
-      auto issue_s = [&](int i) {
-        if (!mbar_wait(&q_full[i & 1], (i >> 1) & 1)) { ok = false; return; }
-        fence_after_sync();
-        const uint64_t b = kQ + (i & 1) * kNext;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) mma_f16_ss(tm_s, kK + k_step(k), b + k_step(k), id_s, k != 0);
-        mma_commit(s_full);
-      };
-      auto issue_dp = [&](int i) {
-        if (!mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; return; }
-        fence_after_sync();
-        const uint64_t b = kDO + (i % DOS) * kNext;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) mma_f16_ss(tm_dp, kV + k_step(k), b + k_step(k), id_s, k != 0);
-        mma_commit(dp_full);
-      };
-      ok = mbar_wait(kv_full, 0) && mbar_wait(kv_clean, 0);
-      if (ok) issue_s(0);
-      if (ok) issue_dp(0);
-      for (int i = 0; i < n && ok; ++i) {
-        if (!mbar_wait(p_ready, i & 1) || !mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; break; }
-        fence_after_sync();
-        const uint64_t bDO = mDO + (i % DOS) * kNext, bQ = mQ + (i & 1) * kNext;
-#pragma unroll
-        for (int k = 0; k < 128 / 16; ++k)     // the 16-bit values of 64 queries lie in the first 32 columns of their scores
-          mma_f16_ts(tm_dv, tm_s + (k / 4) * 64 + (k % 4) * 8, bDO + mn_step(k), id_t, i != 0 || k != 0);
-        mma_commit(&do_free[i % DOS]);
-        if (ok && i + 1 < n) issue_s(i + 1);
-        if (!ok || !mbar_wait(ds_ready, i & 1)) { ok = false; break; }
-        fence_after_sync();
-        if (kOwnDq) {
-          if (i + 1 < n) issue_dp(i + 1);
-          if (!ok || (i > 0 && !mbar_wait(dq_read, (i - 1) & 1))) { ok = false; break; }
+    } else if (warp == 12) {
+      if (elect_one()) {
+        bool ok = true;
+        const uint32_t id_s = make_idesc_f16kind(128, 128, false, false);   // S^T = K Q^T, dP^T = V dO^T
+        const uint32_t id_t = make_idesc_f16kind(128, D, false, true);      // dV = P^T dO, dK = dS^T Q (B MN-major)
+        const uint32_t id_q = make_idesc_f16kind(128, D, true, true);       // dQ = dS K (A, B MN-major)
+        const uint64_t kK = k_major(smem_u32(sK)), kV = k_major(smem_u32(sV)), kQ = k_major(smem_u32(sQ)), kDO = k_major(smem_u32(sDO));
+        const uint64_t mK = mn_major(smem_u32(sK)), mQ = mn_major(smem_u32(sQ)), mDO = mn_major(smem_u32(sDO));
+        const uint64_t kDS = k_major(smem_u32(sDS)), mDS = mn_major(smem_u32(sDS));
+        constexpr uint64_t kNext = kTile >> 4;                              // to the next stage
+        auto issue_s = [&](int i) {
+          if (!mbar_wait(&q_full[i & 1], (i >> 1) & 1)) { ok = false; return; }
           fence_after_sync();
-        }
+          const uint64_t b = kQ + (i & 1) * kNext;
 #pragma unroll
-        for (int k = 0; k < 128 / 16; ++k)     // K dimension = keys; M = queries, two panels of 64
-          mma_f16_ss(tm_dq, mDS + mn_step(k), mK + mn_step(k), id_q, k != 0);
-        mma_commit(dq_full);
+          for (int k = 0; k < D / 16; ++k) mma_f16_ss(tm_s, kK + k_step(k), b + k_step(k), id_s, k != 0);
+          mma_commit(s_full);
+        };
+        auto issue_dp = [&](int i) {
+          if (!mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; return; }
+          fence_after_sync();
+          const uint64_t b = kDO + (i % DOS) * kNext;
 #pragma unroll
-        for (int k = 0; k < 128 / 16; ++k)     // K dimension = queries
-          mma_f16_ss(tm_dk, kDS + k_step(k), bQ + mn_step(k), id_t, i != 0 || k != 0);
-        mma_commit(dk_done);
-        mma_commit(&q_free[i & 1]);
-        if (!kOwnDq && i + 1 < n) {
-          if (!mbar_wait(dq_read, i & 1)) { ok = false; break; }
-          issue_dp(i + 1);
-        }
-      }
-      if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
-    }
-  } else if (warp >= 14) {
-    // ---------------------------------------------------------------- dQ to its tile's sum: every other tile that is not finished here
-    bool ok = true;
-    if (elect_one()) {
-      const int turn = warp - 14;
-      int nth = 0;                               // tiles of both turns so far
-      for (int i = 0; i < n && ok; ++i) {
-        int rank, last;
-        order(m0 + i, rank, last);
-        if (rank == last || (nth++ & 1) != turn) continue;
-        const long long tile = (long long)bh * p.tiles + m0 + i;
-        if (rank > 0) {
-          if (!reached(p.counters + tile, rank)) { ok = false; break; }
-          fence_proxy_async_all();
-        }
-        for (int c = 0; c < D / 16; ++c) {
-          if (!mbar_wait(&staged[turn * kStages + c % kStages], ((nth - 1 >> 1) * (D / 64) + c / kStages) & 1)) { ok = false; break; }
-          float* dst = p.sums + (tile * (D / 16) + c) * (kStage / 4);
-          const uint8_t* src = sStage + c % kStages * kStage;
-          if (rank == 0) bulk_store(dst, src, kStage); else bulk_add(dst, src, kStage);
-          bulk_commit_group();
-          if (c > 1) {                           // all copies but the last two have read their stages
-            bulk_wait_group_read<2>();
-            mbar_arrive(&stage_free[(c - 2) % kStages]);
+          for (int k = 0; k < D / 16; ++k) mma_f16_ss(tm_dp, kV + k_step(k), b + k_step(k), id_s, k != 0);
+          mma_commit(dp_full);
+        };
+        ok = mbar_wait(kv_full, 0) && mbar_wait(kv_clean, 0);
+        if (ok) issue_s(0);
+        if (ok) issue_dp(0);
+        for (int i = 0; i < n && ok; ++i) {
+          if (!mbar_wait(p_ready, i & 1) || !mbar_wait(&do_full[i % DOS], (i / DOS) & 1)) { ok = false; break; }
+          fence_after_sync();
+          const uint64_t bDO = mDO + (i % DOS) * kNext, bQ = mQ + (i & 1) * kNext;
+#pragma unroll
+          for (int k = 0; k < 128 / 16; ++k)     // the 16-bit values of 64 queries lie in the first 32 columns of their scores
+            mma_f16_ts(tm_dv, tm_s + (k / 4) * 64 + (k % 4) * 8, bDO + mn_step(k), id_t, i != 0 || k != 0);
+          mma_commit(&do_free[i % DOS]);
+          if (ok && i + 1 < n) issue_s(i + 1);
+          if (!ok || !mbar_wait(ds_ready, i & 1)) { ok = false; break; }
+          fence_after_sync();
+          if (kOwnDq) {
+            if (i + 1 < n) issue_dp(i + 1);
+            if (!ok || (i > 0 && !mbar_wait(dq_read, (i - 1) & 1))) { ok = false; break; }
+            fence_after_sync();
+          }
+#pragma unroll
+          for (int k = 0; k < 128 / 16; ++k)     // K dimension = keys; M = queries, two panels of 64
+            mma_f16_ss(tm_dq, mDS + mn_step(k), mK + mn_step(k), id_q, k != 0);
+          mma_commit(dq_full);
+#pragma unroll
+          for (int k = 0; k < 128 / 16; ++k)     // K dimension = queries
+            mma_f16_ss(tm_dk, kDS + k_step(k), bQ + mn_step(k), id_t, i != 0 || k != 0);
+          mma_commit(dk_done);
+          mma_commit(&q_free[i & 1]);
+          if (!kOwnDq && i + 1 < n) {
+            if (!mbar_wait(dq_read, i & 1)) { ok = false; break; }
+            issue_dp(i + 1);
           }
         }
-        if (!ok) break;
-        bulk_wait_group_read<1>();
-        mbar_arrive(&stage_free[kStages - 2]);
-        bulk_wait_group_read<0>();
-        mbar_arrive(&stage_free[kStages - 1]);
-        bulk_wait_group_all();
-        fence_proxy_async_all();
-        __threadfence();
-        store_release(p.counters + tile, rank + 1);
+        if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
       }
-      if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
+    } else if (warp >= 14) {
+      // ---------------------------------------------------------------- dQ to its tile's sum: every other tile that is not finished here
+      bool ok = true;
+      if (elect_one()) {
+        const int turn = warp - 14;
+        int nth = 0;                               // tiles of both turns so far
+        for (int i = 0; i < n && ok; ++i) {
+          int rank, last;
+          order(m0 + i, rank, last);
+          if (rank == last || (nth++ & 1) != turn) continue;
+          const long long tile = (long long)bh * p.tiles + m0 + i;
+          if (rank > 0) {
+            if (!reached(p.counters + tile, rank)) { ok = false; break; }
+            fence_proxy_async_all();
+          }
+          for (int c = 0; c < D / 16; ++c) {
+            if (!mbar_wait(&staged[turn * kStages + c % kStages], ((nth - 1 >> 1) * (D / 64) + c / kStages) & 1)) { ok = false; break; }
+            float* dst = p.sums + (tile * (D / 16) + c) * (kStage / 4);
+            const uint8_t* src = sStage + c % kStages * kStage;
+            if (rank == 0) bulk_store(dst, src, kStage); else bulk_add(dst, src, kStage);
+            bulk_commit_group();
+            if (c > 1) {                           // all copies but the last two have read their stages
+              bulk_wait_group_read<2>();
+              mbar_arrive(&stage_free[(c - 2) % kStages]);
+            }
+          }
+          if (!ok) break;
+          bulk_wait_group_read<1>();
+          mbar_arrive(&stage_free[kStages - 2]);
+          bulk_wait_group_read<0>();
+          mbar_arrive(&stage_free[kStages - 1]);
+          bulk_wait_group_all();
+          fence_proxy_async_all();
+          __threadfence();
+          store_release(p.counters + tile, rank + 1);
+        }
+        if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
+      }
     }
-  }
   } else if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     // ---------------------------------------------------------------- point-wise: 32 keys and 64 queries per warp
