@@ -64,28 +64,58 @@ template <bool ONE>
 constexpr int kQPanel = ONE ? 16 * 128 : kRows * 128;              // bytes of 64 channels of a tile
 template <int D, int TILES, bool ONE>
 constexpr int fwd_smem_bytes() { return TILES * (D / 64) * kQPanel<ONE> + kSlots<D, TILES, ONE> * kKeys * D * 2 + 256 + 1024; }
-template <int TILES>
-constexpr int kFwdThreads = TILES * 128 + 128;                     // MMA issue, loads, two idle warps; four softmax warps a tile
+// STEP: keys whose scores a softmax thread has at a time.  64: the next 64 are scored meanwhile, beside them, and less is scored that
+// the masks take away.  128: a product of 128 keys reads Q half as often, but the tensor memory has no room to score ahead; P V starts
+// with the first 96 keys, and some of the exponentials are formed by a polynomial.  With heads of 128 the products count where the keys
+// are many: 4 x 4096, 16 over 4 heads of 128, STEP 64 and 128: window 256 96 and 106 us, 1024 162 and 159, none 265 and 247; 2048 new
+// tokens of two sequences over 16384, 32 over 8 heads: 967 and 862.
+template <int TILES, int STEP>
+constexpr int kFwdThreads = TILES * 128 + (STEP == 128 ? 128 : 64);     // four softmax warps a tile; MMA issue; loads; for setmaxnreg two more
+constexpr int kMost = 96;                                               // STEP 128: keys whose P V starts early
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// 2^x for x <= 127, two at a time without the special-function units: x = n + f with |f| <= 1/2 (1.5 2^23 added and taken off again
+// rounds to the nearest n, and leaves n in the low bits), 2^f by the polynomial of degree five that has 1 at 0 and the least largest
+// relative error, 2^-22.6 in fp32, and n added to the exponent.  Below -127, where the sum would leave the exponent's range, x counts as -127,
+// whose result is 0; from there to -126 results are positive and below 2^-126.  NaN is not kept: the row's reference takes care of it.
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  x = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
+  const float2 t = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f));
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
+  float2 y = __ffma2_rn(make_float2(0.001326472731307149f, 0.001326472731307149f), f, make_float2(0.009671512991189957f, 0.009671512991189957f));
+  y = __ffma2_rn(y, f, make_float2(0.05550733581185341f, 0.05550733581185341f));
+  y = __ffma2_rn(y, f, make_float2(0.24022242426872253f, 0.24022242426872253f));
+  y = __ffma2_rn(y, f, make_float2(0.6931470036506653f, 0.6931470036506653f));
+  y = __ffma2_rn(y, f, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
 
 // Queries of one tile, or of both, as the kernel needs them: token numbers within the sequence's new tokens.
 struct Span {
   int p0, p1;      // positions of the first and the last valid query; p1 < p0: none
-  int lo, hi;      // key blocks of the window (first tokens apart)
+  int lo, hi;      // steps of keys of the window (first tokens apart)
 };
 
+template <int STEP>
 __device__ __forceinline__ Span make_span(int i0, int i1, int base, int key_end, int window) {
   Span s;
   s.p0 = max(0, base + i0);
   s.p1 = base + i1 - 1;
   const int end = min(s.p1 + 1, key_end);
   if (i1 <= i0 || end <= 0) { s.p1 = s.p0 - 1; s.lo = 0; s.hi = -1; return s; }
-  s.lo = max(0, s.p0 - window + 1) / kKeys;
-  s.hi = (end - 1) / kKeys;
+  s.lo = max(0, s.p0 - window + 1) / STEP;
+  s.hi = (end - 1) / STEP;
   return s;
 }
 
-template <int D, bool PAGED, int TILES, bool ONE>
-__global__ void __launch_bounds__(kFwdThreads<TILES>, TILES == 2 ? 1 : 2)
+template <int D, bool PAGED, int TILES, bool ONE, int STEP>
+__global__ void __launch_bounds__(kFwdThreads<TILES, STEP>, TILES == 2 ? 1 : 2)
 window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
                   const __grid_constant__ CUtensorMap map_low, const __grid_constant__ FwdParams p) {
@@ -94,6 +124,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   constexpr int kKVBytes = kKeys * D * 2;
   constexpr int NS = kSlots<D, TILES, ONE>;
   constexpr uint32_t kTmemO = TILES * 128, kTmemCols = TILES * 256;   // S/P of each tile, 128 columns; then O of each, D
+  constexpr int kMma = TILES * 4, kLoad = kMma + 1;   // warps
+  constexpr int AHEAD = kKeys / STEP;        // steps of a block: so many are scored ahead, in so many places
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                        // TILES tiles
@@ -102,10 +134,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* q_full = bars;
   uint64_t* full = bars + 1;                 // [NS]
   uint64_t* empty = full + NS;               // [NS]
-  uint64_t* s_full = empty + NS;             // [2]
-  uint64_t* p_ready = s_full + 2;            // [2]
-  uint64_t* pv_full = p_ready + 2;           // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_full + 2);
+  uint64_t* s_full = empty + NS;             // [tile][2]: of the steps in turn
+  uint64_t* p_ready = s_full + 2 * TILES;    // [tile][2]
+  uint64_t* pv_full = p_ready + 2 * TILES;   // [tile][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_full + 2 * TILES);
   int* found = reinterpret_cast<int*>(tmem_slot + 1);   // sequence, pair
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -178,26 +210,28 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   Span span[TILES];
 #pragma unroll
   for (int g = 0; g < TILES; ++g)
-    span[g] = make_span(tok0 + g * p.tile_tokens, min(tok0 + (g + 1) * p.tile_tokens, n_valid), base, key_end, p.window);
-  const Span both = make_span(tok0, min(tok0 + TILES * p.tile_tokens, n_valid), base, key_end, p.window);
+    span[g] = make_span<STEP>(tok0 + g * p.tile_tokens, min(tok0 + (g + 1) * p.tile_tokens, n_valid), base, key_end, p.window);
+  const Span both = make_span<STEP>(tok0, min(tok0 + TILES * p.tile_tokens, n_valid), base, key_end, p.window);
   const int near = max(0, both.p0 - p.window + 1), end = min(both.p1 + 1, key_end);       // what both tiles see together:
   const int sink_end = min(p.sinks, end);                                                  // [0, sink_end) and [near, end)
-  const int ns = both.hi < 0 ? 0 : min((p.sinks + kKeys - 1) / kKeys, both.hi + 1);        // blocks with first tokens
-  const int range0 = max(both.lo, ns);
-  const int listed = ns + max(0, both.hi - range0 + 1);                                    // a table may end in front of the window
+  const int lo = both.lo * STEP / kKeys, hi = both.hi < 0 ? -1 : both.hi * STEP / kKeys;  // blocks of its window
+  const int ns = min((p.sinks + kKeys - 1) / kKeys, hi + 1);                               // blocks with first tokens
+  const int range0 = max(lo, ns);
+  const int listed = ns + max(0, hi - range0 + 1);                                    // a table may end in front of the window
   int c0 = 0, c1 = listed;
   if (PAGED && p.splits > 1) {
     c0 = (int)((long long)listed * split / p.splits);
     c1 = (int)((long long)listed * (split + 1) / p.splits);
   }
   auto block_of = [&](int c) { return c < ns ? c : c - ns + range0; };
-  auto needed = [&](const Span& s, int kb) { return kb <= s.hi && (kb < ns || kb >= s.lo); };
+  const int sink_steps = (p.sinks + STEP - 1) / STEP;
+  auto needed = [&](const Span& s, int step) { return step <= s.hi && (step < sink_steps || step >= s.lo); };
 
   const bool partial = PAGED && p.splits > 1;
   if (c0 >= c1) {                              // no keys: zeros, or a part that adds nothing
     const int i1 = min(tok0 + TILES * p.tile_tokens, n_rows);
     const int per = p.group * (D / 8);
-    for (int i = threadIdx.x; i < (i1 - tok0) * per; i += kFwdThreads<TILES>) {
+    for (int i = threadIdx.x; i < (i1 - tok0) * per; i += kFwdThreads<TILES, STEP>) {
       const int t = tok0 + i / per, r = i % per;
       const long long row = (PAGED ? (long long)row0 : (long long)b * p.T) + t;
       const long long at = row * heads + kvh * p.group + r / (D / 8);
@@ -216,27 +250,23 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     prefetch_tensormap(&map_v);
     mbar_init(q_full, 1);
     for (int s = 0; s < NS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int g = 0; g < TILES; ++g) {
+    for (int g = 0; g < 2 * TILES; ++g) {
       mbar_init(&s_full[g], 1);
       mbar_init(&p_ready[g], 4);
       mbar_init(&pv_full[g], 1);
     }
     mbar_fence_init();
   }
-  if (warp == 0) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
+  if (warp == kMma) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
 
-  // Registers go where the scores are, four warps at a time: launched with 168 (TILES = 2) or 128 a thread, a softmax thread keeps a row of
-  // 128 scores.  With 168 for it a hundred bytes were spilled.
-  if (warp < 4) {
-    if constexpr (TILES == 2)
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    else
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 1) {
+  // With 128 scores a thread registers go where the scores are, four warps at a time (launched with 168 a thread).
+  if (warp >= kMma) {
+    if constexpr (STEP == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kLoad) {
       // ---------------------------------------------------------------- loads
       bool ok = true;
       if (lane == 0) {
@@ -284,73 +314,78 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
-    } else if (warp == 0) {
+    } else if (warp == kMma) {
       // ---------------------------------------------------------------- products
       if (elect_one()) {
-        const uint32_t idesc_s = make_idesc_f16kind(128, kKeys, false, false);
+        const uint32_t idesc_s = make_idesc_f16kind(128, STEP, false, false);
         const uint32_t idesc_pv = make_idesc_f16kind(128, D, false, true);   // B = V is MN-major
         auto wait_full = [&](int f) { return mbar_wait(&full[f % NS], (f / NS) & 1); };
         const uint64_t kQ = k_major(smem_u32(sQ)), kKV = k_major(smem_u32(sKV)), mKV = mn_major(smem_u32(sKV));
-        auto issue_s = [&](int g, int f) {       // S_g = Q_g K^T
-          const uint64_t a = kQ + g * (kQBytes >> 4), bk = kKV + f % NS * (kKVBytes >> 4);
+        int scored[TILES] = {}, added[TILES] = {};   // steps of each tile whose S, whose P V has been issued
+        auto issue_s = [&](int g, int t) {       // S_g = Q_g K^T, 64 keys
+          const int f = 2 * (t / AHEAD), turn = scored[g]++ % AHEAD;
+          const uint64_t a = kQ + g * (kQBytes >> 4), bk = kKV + ((f % NS * kKVBytes + t % AHEAD * (STEP * 128)) >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            mma_f16_ss(tmem + g * 128, a + ((k / 4 * kQPanel<ONE> + k % 4 * 32) >> 4), bk + k_step(k), idesc_s, k != 0);
-          mma_commit(&s_full[g]);
+            mma_f16_ss(tmem + g * 128 + turn * STEP, a + ((k / 4 * kQPanel<ONE> + k % 4 * 32) >> 4), bk + k_step(k), idesc_s, k != 0);
+          mma_commit(&s_full[2 * g + turn]);
         };
-        auto issue_pv = [&](int g, int f, bool first) {     // O_g (+)= P_g V
-          const uint64_t bv = mKV + f % NS * (kKVBytes >> 4);
+        auto issue_pv = [&](int g, int t) {      // O_g (+)= P_g V
+          const int f = 2 * (t / AHEAD) + 1, nth = added[g]++;
+          const uint64_t bv = mKV + (f % NS * kKVBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            mma_f16_ts(tmem + kTmemO + g * D, tmem + g * 128 + k * 8, bv + mn_step(k), idesc_pv, !first || k != 0);
-          mma_commit(&pv_full[g]);
+          for (int k = 0; k < (STEP == 128 ? kMost : STEP) / 16; ++k)
+            mma_f16_ts(tmem + kTmemO + g * D, tmem + g * 128 + nth % AHEAD * STEP + k * 8, bv + mn_step(t % AHEAD * (STEP / 16) + k), idesc_pv,
+                       nth != 0 || k != 0);
+          if constexpr (STEP == 128) {
+            if (!mbar_wait(&p_ready[2 * g + 1], nth & 1)) return false;
+            fence_after_sync();
+#pragma unroll
+            for (int k = kMost / 16; k < STEP / 16; ++k)
+              mma_f16_ts(tmem + kTmemO + g * D, tmem + g * 128 + k * 8, bv + mn_step(k), idesc_pv, true);
+          }
+          mma_commit(&pv_full[2 * g + nth % AHEAD]);
+          return true;
         };
-        int done[TILES] = {};                    // blocks of each tile whose P V has been issued
+        const int steps = AHEAD * (c1 - c0);
+        auto wants = [&](int g, int t) { return t < steps && needed(g == 0 ? span[0] : span[TILES - 1], block_of(c0 + t / AHEAD) * AHEAD + t % AHEAD); };
         bool ok = mbar_wait(q_full, 0) && wait_full(0);
         if (ok) {
           fence_after_sync();
-          const int kb = block_of(c0);
-          if (needed(span[0], kb)) issue_s(0, 0);
-          if (TILES == 2 && needed(span[TILES - 1], kb)) issue_s(TILES - 1, 0);
+          for (int t = 0; t < AHEAD; ++t)
+            for (int g = 0; g < TILES; ++g)
+              if (wants(g, t)) issue_s(g, t);
           mma_commit(&empty[0]);
         }
-        for (int c = c0; c < c1 && ok; ++c) {
-          const int f = 2 * (c - c0), kb = block_of(c);
-          const bool more = c + 1 < c1;
-          const int kb1 = more ? block_of(c + 1) : -1;
-          if (!wait_full(f + 1)) { ok = false; break; }
-          auto step_pv = [&](int g) {
-            if (!needed(g == 0 ? span[0] : span[TILES - 1], kb)) return;
-            if (!mbar_wait(&p_ready[g], done[g] & 1)) { ok = false; return; }
-            fence_after_sync();
-            issue_pv(g, f + 1, done[g] == 0);
-            ++done[g];
-          };
-          step_pv(0);
-          if (!ok) break;
-          if (more) {
-            if (!wait_full(f + 2)) { ok = false; break; }
-            fence_after_sync();
-            if (needed(span[0], kb1)) issue_s(0, f + 2);   // S_0 of this block was read before p_ready[0] arrived
+        // S of a tile's next step is there before the softmax is done with this one: two steps' scores lie beside each other.
+        for (int t = 0; t < steps && ok; ++t) {
+          const int f = 2 * (t / AHEAD);
+          if (t % AHEAD == 0 && !wait_full(f + 1)) { ok = false; break; }
+#pragma unroll
+          for (int g = 0; g < TILES; ++g) {
+            if (wants(g, t)) {
+              if (!mbar_wait(&p_ready[2 * g + added[g] % AHEAD], (added[g] / AHEAD) & 1)) { ok = false; break; }
+              fence_after_sync();
+              if (!issue_pv(g, t)) { ok = false; break; }
+            }
+            if (g == 0 && t % AHEAD == 0 && t + AHEAD < steps) {
+              if (!wait_full(f + 2)) { ok = false; break; }
+              fence_after_sync();
+            }
+            if (wants(g, t + AHEAD)) issue_s(g, t + AHEAD);      // over P of the step that has been added
           }
-          if (TILES == 2) step_pv(TILES - 1);
-          if (!ok) break;
-          mma_commit(&empty[(f + 1) % NS]);
-          if (more) {
-            if (TILES == 2 && needed(span[TILES - 1], kb1)) issue_s(TILES - 1, f + 2);
-            mma_commit(&empty[(f + 2) % NS]);
+          if (ok && t % AHEAD == AHEAD - 1) {
+            mma_commit(&empty[(f + 1) % NS]);
+            if (t + AHEAD < steps) mma_commit(&empty[(f + 2) % NS]);
           }
         }
         if (!ok) atomicExch(p.status, ATT_ERR_TIMEOUT);
       }
     }
   } else {
-    if constexpr (TILES == 2)
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    else
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if constexpr (STEP == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---------------------------------------------------------------- softmax / output threads of one tile
-    const int g = (warp - 4) >> 2;                   // tile of this warp group
+    const int g = warp >> 2;                         // tile of this warp group
     const int lane_group = warp & 3;                 // TMEM lane quarter this warp may access
     const int row = lane_group * 32 + lane;
     const int token = row / p.group;
@@ -359,7 +394,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const bool stored = token < p.tile_tokens && i < n_rows;
     const bool valid = stored && i < n_valid && pos >= 0;
     const uint32_t lane_addr = uint32_t(lane_group * 32) << 16;
-    const uint32_t tmem_s = tmem + g * 128, tmem_pv = tmem + kTmemO + g * D;
+    const uint32_t tmem_pv = tmem + kTmemO + g * D;
     const Span mine = g == 0 ? span[0] : span[TILES - 1];
     const bool idle = ONE && lane_group * 32 >= p.group;   // rows that nobody looks at
     // m is the reference of the exponentials accumulated so far: p = 2^((s - m) scale).  It follows the running row maximum only
@@ -368,50 +403,57 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     int it = 0;
-    for (int c = c0; c < c1; ++c) {
-      const int kb = block_of(c);
-      if (!needed(mine, kb)) continue;
-      const int k0 = kb * kKeys;
-      if (!mbar_wait(&s_full[g], it & 1)) { ok = false; break; }
+    for (int t = 0; t < AHEAD * (c1 - c0); ++t) {
+      const int step = block_of(c0 + t / AHEAD) * AHEAD + t % AHEAD;
+      if (!needed(mine, step)) continue;
+      const int k0 = step * STEP;
+      const uint32_t tmem_s = tmem + g * 128 + it % AHEAD * STEP;
+      if (!mbar_wait(&s_full[2 * g + it % AHEAD], (it / AHEAD) & 1)) { ok = false; break; }
       fence_after_sync();
-      if (k0 + kKeys > end || (k0 < near && k0 + kKeys > sink_end)) {
-        // rows of V that no query of this block sees.  S of this block is there, so the block before has been used up: a wait on V's
-        // barrier any earlier could take the phase before for this one.
-        const int f = 2 * (c - c0) + 1;
+      if ((k0 + STEP > end || (k0 < near && k0 + STEP > sink_end)) && (g == 0 || !needed(span[0], step))) {
+        // rows of V that no query of this block sees; the first tile's P V goes ahead of the second's.  S of this step is there, so V of
+        // the block before has been: a wait on V's barrier any earlier could take the phase before for this one.  Eight lanes a row:
+        // with a row a lane all lanes met in the same banks, 4 000 cycles a block.
+        const int f = 2 * (t / AHEAD) + 1;
         if (!mbar_wait(&full[f % NS], (f / NS) & 1)) { ok = false; break; }
-        const int key = k0 + row;
-        if (key >= end || (key < near && key >= sink_end)) {
-          uint8_t* at = sKV + f % NS * kKVBytes + row * 128;
 #pragma unroll
-          for (int j = 0; j < DP * 8; ++j) *reinterpret_cast<uint4*>(at + (j / 8) * kKeys * 128 + (j % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int at = 0; at < STEP / 4; at += 4) {
+          const int r = lane_group * (STEP / 4) + at + lane / 8, key = k0 + r;
+          if (key >= end || (key < near && key >= sink_end)) {
+#pragma unroll
+            for (int j = 0; j < DP; ++j)
+              *reinterpret_cast<uint4*>(sKV + f % NS * kKVBytes + (j * kKeys + t % AHEAD * STEP + r) * 128 + lane % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
         }
         fence_proxy_async_smem();
       }
       if (idle) {
-        warp_arrive(&p_ready[g]);
+        warp_arrive(&p_ready[2 * g + it % AHEAD]);
+        if (STEP == 128) warp_arrive(&p_ready[2 * g + 1]);
         ++it;
         continue;
       }
-      uint32_t r[kKeys];
+      uint32_t r[STEP];
 #pragma unroll
-      for (int j = 0; j < kKeys; j += 32) tmem_ld_32x32(tmem_s + lane_addr + j, *reinterpret_cast<uint32_t(*)[32]>(r + j));
+      for (int j = 0; j < STEP; j += 32) tmem_ld_32x32(tmem_s + lane_addr + j, *reinterpret_cast<uint32_t(*)[32]>(r + j));
       tmem_ld_wait();
-      // Masking is a pass of its own that only blocks on an edge take.
-      if (k0 + kKeys > min(mine.p0 + 1, key_end) || (k0 <= mine.p1 - p.window && k0 + kKeys > p.sinks)) {
+      // Masking is a pass of its own that only steps on an edge take.
+      if (k0 + STEP > min(mine.p0 + 1, key_end) || (k0 <= mine.p1 - p.window && k0 + STEP > p.sinks)) {
         const int hi = min(pos + 1, key_end) - k0, lo = pos - p.window + 1 - k0, first = p.sinks - k0;
         auto below = [](int c) { return c <= 0 ? 0u : c >= 32 ? 0xffffffffu : (1u << c) - 1u; };
 #pragma unroll
-        for (int w = 0; w < kKeys / 32; ++w) {
+        for (int w = 0; w < STEP / 32; ++w) {
           const uint32_t seen = below(hi - w * 32) & (~below(lo - w * 32) | below(first - w * 32));
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[w * 32 + j] = seen & (1u << j) ? r[w * 32 + j] : 0xff800000u;      // -inf
         }
       }
+      // The maximum is NaN where a score is: then the reference, and with it every exponential of the row, is NaN.
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < kKeys; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(r[j]));
-      const float m_blk = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-      const bool grow = (m_blk - m) * p.scale_log2 > 8.0f;      // true on the first block of any visible key
+      for (int j = 0; j < STEP; j += 2) mx4[j / 2 & 3] = max3_nan(mx4[j / 2 & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+      const float m_blk = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]);
+      const bool grow = !((m_blk - m) * p.scale_log2 <= 8.0f);      // true on the first block of any visible key
       float alpha = 1.0f;
       if (grow) {
         alpha = (m == -INFINITY) ? 0.0f : fast_exp2((m - m_blk) * p.scale_log2);
@@ -419,9 +461,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       const float m_use = (m == -INFINITY) ? 0.0f : m;
       if (it > 0 && __any_sync(0xffffffffu, grow)) {
-        // some row of this warp moved its reference: scale the accumulated output rows.  The product that adds the block before
-        // has completed (S of this block was issued after it); the wait makes that explicit and returns at once.
-        if (!mbar_wait(&pv_full[g], (it - 1) & 1)) { ok = false; break; }
+        // some row of this warp moved its reference: scale the accumulated output rows, once the step before has been added
+        if (!mbar_wait(&pv_full[2 * g + (it - 1) % AHEAD], ((it - 1) / AHEAD) & 1)) { ok = false; break; }
         fence_after_sync();
         const float2 a2 = make_float2(alpha, alpha);
 #pragma unroll 1
@@ -440,41 +481,46 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       // p = 2^(s scale - m scale): one packed multiply-add per pair, then the exponential; the row sum is taken over the fp32
       // values.  P is rounded to 16 bits as an operand of the second product (half a step of its type, relative to values whose
-      // largest is near 1).
+      // largest is near 1).  The special-function units form four exponentials a cycle and quarter of a multiprocessor: 1 024 cycles for
+      // 64 keys of two tiles, of the 1 900 that a step takes.  Of 128 scores a thread three pairs of eight are formed on the other units
+      // (30 011 tokens, window 2048: 543 -> 525 us); of 64 that gained nothing, the chain of the polynomial is too long for two warps.
       const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
       const float nm = -m_use * p.scale_log2;
       const float2 nm2 = make_float2(nm, nm);
       float2 rs2 = make_float2(0.0f, 0.0f), rs2b = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int part = 0; part < 4; ++part) {
+      for (int part = 0; part < STEP / 32; ++part) {
         uint32_t packed[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int at = part * 32 + 2 * j;
           const float2 e = __ffma2_rn(make_float2(__uint_as_float(r[at]), __uint_as_float(r[at + 1])), sc2, nm2);
-          const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+          const float2 pe = STEP == 128 && (j % 8 == 1 || j % 8 == 4 || j % 8 == 6) ? poly_exp2(e) : make_float2(fast_exp2(e.x), fast_exp2(e.y));
           if (j & 1) rs2b = __fadd2_rn(rs2b, pe); else rs2 = __fadd2_rn(rs2, pe);
           elem2_t h = f22e2(pe);
           packed[j] = *reinterpret_cast<uint32_t*>(&h);
         }
         tmem_st_32x16(tmem_s + lane_addr + part * 16, packed);
+        if (STEP == 128 && part == kMost / 32 - 1) {
+          tmem_st_wait();
+          fence_before_sync();
+          warp_arrive(&p_ready[2 * g]);
+        }
       }
       l = l * alpha + ((rs2.x + rs2.y) + (rs2b.x + rs2b.y));
       tmem_st_wait();
       fence_before_sync();
-      warp_arrive(&p_ready[g]);
+      warp_arrive(&p_ready[STEP == 128 ? 2 * g + 1 : 2 * g + it % AHEAD]);
       ++it;
     }
-    if (ok) {
-      // the last product completes the output rows in tensor memory: divide by the row sum and store
-      if (it > 0 && !mbar_wait(&pv_full[g], (it - 1) & 1)) ok = false;
-      fence_after_sync();
-    }
-    if (ok) {
+    // the last product completes the output rows in tensor memory: divide by the row sum and store
+    if (it > 0 && ok && !mbar_wait(&pv_full[2 * g + (it - 1) % AHEAD], ((it - 1) / AHEAD) & 1)) ok = false;
+    fence_after_sync();
+    {                                            // also after a wait that expired: the tile's warps meet below
       const long long at_row = (PAGED ? (long long)row0 : (long long)b * p.T) + i;
       const long long at = at_row * heads + kvh * p.group + (row - token * p.group);
       if (!valid) l = 0.0f;
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const float2 inv2 = make_float2(inv, inv);
       if constexpr (PAGED) {
 #pragma unroll 1
@@ -484,7 +530,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tmem_ld_32x32(tmem_pv + lane_addr + d0, r);
             tmem_ld_wait();
           }
-          if (it == 0 || !(l > 0.0f)) {          // nothing seen
+          if (it == 0 || l == 0.0f) {            // nothing seen
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0u;
           }
@@ -520,7 +566,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               tmem_ld_32x32(tmem_pv + lane_addr + d0, r);
               tmem_ld_wait();
             }
-            if (it == 0 || !(l > 0.0f)) {
+            if (it == 0 || l == 0.0f) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) r[j] = 0u;
             }
@@ -540,7 +586,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             }
           }
           fence_proxy_async_smem();
-          if (g == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");   // the tile's warps
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");   // the tile's warps
           if (lane_group == 0 && tok0 + g * p.tile_tokens < p.T && elect_one()) {
 #pragma unroll
             for (int j = 0; j < DP; ++j)
@@ -549,15 +595,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             bulk_wait_group_read<0>();
           }
           if (pass + 1 < passes) {
-            if (g == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
           }
         }
       }
       if (stored) {
         if (partial) {
-          p.part_ml[(long long)split * p.T * heads + at] = make_float2(l > 0.0f ? m * p.scale_log2 : -INFINITY, l);
+          p.part_ml[(long long)split * p.T * heads + at] = make_float2(l == 0.0f ? -INFINITY : m * p.scale_log2, l);
         } else if (!PAGED && p.lse != nullptr) {
-          p.lse[(((long long)b * p.kv_heads + kvh) * p.tiles + pair * TILES + g) * kRows + row] = l > 0.0f ? -(m * p.scale_log2 + log2f(l)) : 0.0f;
+          p.lse[(((long long)b * p.kv_heads + kvh) * p.tiles + pair * TILES + g) * kRows + row] = l == 0.0f ? 0.0f : -(m * p.scale_log2 + log2f(l));
         }
       }
     }
@@ -566,7 +612,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 0) { fence_after_sync(); tmem_dealloc(tmem, kTmemCols); }
+  if (warp == kMma) { fence_after_sync(); tmem_dealloc(tmem, kTmemCols); }
 }
 
 // Partial sums of a row's splits to its output: a warp a row.  With each split's reference m_s and total l_s,
@@ -584,27 +630,30 @@ __global__ void __launch_bounds__(256) window_join_kernel(const float* part_o, c
   for (int v = 0; v < V; ++v) o[v] = 0.0f;
   for (int s = 0; s < splits; ++s) {
     const float2 ml = part_ml[s * rows + row];
-    if (!(ml.y > 0.0f)) continue;              // also: sums that were not written
+    if (ml.y == 0.0f) continue;                // its sums were not written
     const float w = exp2f(ml.x - top);
     total += ml.y * w;
     const float* src = part_o + (s * rows + row) * D + lane * V;
 #pragma unroll
     for (int v = 0; v < V; ++v) o[v] += src[v] * w;
   }
-  const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   elem_t* dst = out + row * D + lane * V;
 #pragma unroll
   for (int v = 0; v < V; v += 2) *reinterpret_cast<elem2_t*>(dst + v) = ff2e2(o[v] * inv, o[v + 1] * inv);
 }
 
-template <int D, bool PAGED, int TILES, bool ONE>
+template <int D, bool PAGED, int TILES, bool ONE, int STEP>
 int launch(dim3 grid, cudaStream_t s, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& out, const CUtensorMap& low,
            const FwdParams& p) {
   constexpr int smem = fwd_smem_bytes<D, TILES, ONE>();
-  if (set_smem_once<window_fwd_kernel<D, PAGED, TILES, ONE>>(smem)) return 5;
-  window_fwd_kernel<D, PAGED, TILES, ONE><<<grid, kFwdThreads<TILES>, smem, s>>>(q, k, v, out, low, p);
+  if (set_smem_once<window_fwd_kernel<D, PAGED, TILES, ONE, STEP>>(smem)) return 5;
+  window_fwd_kernel<D, PAGED, TILES, ONE, STEP><<<grid, kFwdThreads<TILES, STEP>, smem, s>>>(q, k, v, out, low, p);
   return 0;
 }
+
+// STEP 128: by the keys that a pair of tiles sees at most.
+bool far_enough(long long keys, int D) { return D == 128 && keys >= 2048; }
 
 }  // namespace
 
@@ -645,8 +694,11 @@ int fbam_window_fwd(const void* q, long long q_sb, long long q_st, long long q_s
   if ((e = encode_heads(&ml, lse != nullptr ? low : out, D, heads, T, B, D, heads * D, o_sb, group, p.tile_tokens))) return e;
   const unsigned grid = (unsigned)blocks;
   cudaStream_t s = (cudaStream_t)stream;
-  if (one_tile ? (D == 64 ? launch<64, false, 1, false>(grid, s, mq, mk, mv, mo, ml, p) : launch<128, false, 1, false>(grid, s, mq, mk, mv, mo, ml, p))
-               : (D == 64 ? launch<64, false, 2, false>(grid, s, mq, mk, mv, mo, ml, p) : launch<128, false, 2, false>(grid, s, mq, mk, mv, mo, ml, p)))
+  const bool wide = far_enough((long long)p.window + per < T ? p.window + per : T, D);
+  if (one_tile ? (D == 64 ? launch<64, false, 1, false, 64>(grid, s, mq, mk, mv, mo, ml, p) : launch<128, false, 1, false, 64>(grid, s, mq, mk, mv, mo, ml, p))
+      : D == 64 ? launch<64, false, 2, false, 64>(grid, s, mq, mk, mv, mo, ml, p)
+      : wide    ? launch<128, false, 2, false, 128>(grid, s, mq, mk, mv, mo, ml, p)
+                : launch<128, false, 2, false, 64>(grid, s, mq, mk, mv, mo, ml, p))
     return 5;
   return cudaGetLastError() == cudaSuccess ? 0 : 5;
 }
@@ -693,9 +745,13 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   if ((e = encode_heads(&mv, v_pages, D, kv_heads, page, pages, v_sh, v_ss, v_sp, 1, p.piece))) return e;
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)pairs, kv_heads, splits);
-  if (single     ? (D == 64 ? launch<64, true, 1, true>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, true>(grid, s, mq, mk, mv, mq, mq, p))
-      : one_tile ? (D == 64 ? launch<64, true, 1, false>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, false>(grid, s, mq, mk, mv, mq, mq, p))
-                 : (D == 64 ? launch<64, true, 2, false>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 2, false>(grid, s, mq, mk, mv, mq, mq, p)))
+  const long long most = (long long)max_pages * page;
+  const bool wide = far_enough((long long)p.window + per < most ? p.window + per : most, D);
+  if (single     ? (D == 64 ? launch<64, true, 1, true, 64>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, true, 64>(grid, s, mq, mk, mv, mq, mq, p))
+      : one_tile ? (D == 64 ? launch<64, true, 1, false, 64>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, false, 64>(grid, s, mq, mk, mv, mq, mq, p))
+      : D == 64  ? launch<64, true, 2, false, 64>(grid, s, mq, mk, mv, mq, mq, p)
+      : wide     ? launch<128, true, 2, false, 128>(grid, s, mq, mk, mv, mq, mq, p)
+                 : launch<128, true, 2, false, 64>(grid, s, mq, mk, mv, mq, mq, p))
     return 5;
   if (splits > 1) {
     const long long all = (long long)rows * kv_heads * group;

@@ -225,3 +225,65 @@ def test_heads_of_more_than_2_31_values():
         oracle.within(g[-1:], *want[name])
         assert not g[:-1].any()
     nv.check_status(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("b,t,h,kv,d,win,sinks,padded", [
+    (3, 500, 32, 32, 64, 100, 3, True), (2, 700, 28, 28, 128, None, 0, False), (5, 333, 48, 24, 128, 64, 70, True),
+    (1, 2304, 17, 17, 128, None, 0, False), (2, 2200, 10, 10, 128, 2100, 5, True), (1, 2100, 20, 20, 64, 2000, 1, False)])
+def test_more_tiles_than_fit_at_once(b, t, h, kv, d, win, sinks, padded):
+    gen = _gen("waves", t, d)
+    qkv, dy = _randn(gen, b, t, h + 2 * kv, d), _randn(gen, b, t, h, d)
+    lengths = None
+    if padded:
+        lengths = torch.tensor([t - 129 * i for i in range(b)], device="cuda")
+        for i, n in enumerate(lengths.tolist()):
+            qkv[i, n:], dy[i, n:] = float("nan"), float("nan")
+    want = oracle.window(*qkv.split((h, kv, kv), 2), win, sinks, lengths, dy)
+    qkv.requires_grad_()
+    y = ops.window_attention_qkv(qkv, kv, win, sinks, lengths)
+    oracle.within(y, *want["y"])
+    with torch.no_grad():
+        assert torch.equal(ops.window_attention_qkv(qkv, kv, win, sinks, lengths), y)
+    grad, = torch.autograd.grad((y,), (qkv,), (dy,))
+    for part, name in zip(grad.split((h, kv, kv), 2), ("dq", "dk", "dv")):
+        oracle.within(part, *want[name])
+    nv.check_status(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("slots,most,h,kv,d,win,sinks", [(16, None, 32, 32, 64, None, 0), (64, 60, 32, 16, 128, 200, 9), (16, 200, 20, 20, 128, None, 0),
+                                                         (128, 30, 20, 20, 128, 2100, 2)])
+def test_new_tokens_in_waves(slots, most, h, kv, d, win, sinks):
+    gen = _gen("new in waves", h, d, most)
+    lengths, new = [700, 2400, 90, 33, 1000, 64, 2600], [300, 257, 90, 1, 129, 5, 700]
+    cache = _cache(gen, lengths, slots, kv, d, most)
+    q = _randn(gen, sum(new), h, d)
+    offsets = torch.tensor([0] + new, device="cuda").cumsum(0).to(I32)
+    want = oracle.cached(q, *cache, offsets, win, sinks)
+    y = ops.cache_attention(q, *cache, offsets, win, sinks)
+    oracle.within(y, *want)
+    for _ in range(5):
+        assert torch.equal(ops.cache_attention(q, *cache, offsets, win, sinks), y)
+    nv.check_status(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("t,h,kv,win", [(300, 2, 1, 90), (2200, 24, 24, None), (400, 40, 40, 64)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_what_is_not_a_number_shows(t, h, kv, win, d):
+    """NaN in a query or a key is in every row that sees it, and in no other."""
+    gen = _gen("nan", t)
+    q, k, v = _randn(gen, 1, t, h, d), _randn(gen, 1, t, kv, d), _randn(gen, 1, t, kv, d)
+    clean = ops.window_attention(q, k, v, win)
+    q[0, 40, 1, 5], k[0, t // 2, 0, 7] = float("nan"), float("nan")
+    y = ops.window_attention(q, k, v, win)
+    hurt = torch.zeros(t, h, dtype=torch.bool, device="cuda")
+    hurt[40, 1] = True
+    hurt[t // 2:t if win is None else t // 2 + win, :h // kv] = True
+    assert y[0][hurt].isnan().all() and torch.equal(y[0][~hurt], clean[0][~hurt])
+    pages, slots = -(-t // 16), 16
+    padded = [torch.nn.functional.pad(x[0], (0, 0, 0, 0, 0, pages * slots - t)).view(pages, slots, kv, d) for x in (k, v)]
+    tables, lengths = torch.arange(pages, dtype=I32, device="cuda")[None], torch.tensor([t], dtype=I32, device="cuda")
+    got = ops.cache_attention(q[0], *padded, tables, lengths, torch.tensor([0, t], dtype=I32, device="cuda"), win)
+    assert got[hurt].isnan().all() and got[~hurt].isfinite().all()
+    last = ops.cache_attention(q[0, t // 2:t // 2 + 1], *padded, tables, lengths - (t - t // 2 - 1), None, win)
+    assert last[0, :h // kv].isnan().all() and last[0, h // kv:].isfinite().all()
+    nv.check_status(torch.device("cuda", 0))
