@@ -66,9 +66,11 @@ template <int D, int TILES, bool ONE>
 constexpr int fwd_smem_bytes() { return TILES * (D / 64) * kQPanel<ONE> + kSlots<D, TILES, ONE> * kKeys * D * 2 + 256 + 1024; }
 // STEP: keys whose scores a softmax thread has at a time.  64: the next 64 are scored meanwhile, beside them, and less is scored that
 // the masks take away.  128: a product of 128 keys reads Q half as often, but the tensor memory has no room to score ahead; P V starts
-// with the first 96 keys, and some of the exponentials are formed by a polynomial.  With heads of 128 the products count where the keys
-// are many: 4 x 4096, 16 over 4 heads of 128, STEP 64 and 128: window 256 96 and 106 us, 1024 162 and 159, none 265 and 247; 2048 new
-// tokens of two sequences over 16384, 32 over 8 heads: 967 and 862.
+// with the first 96 keys.  With heads of 128 the products count where the keys are many: 4 x 4096, 16
+// over 4 heads of 128, STEP 64 and 128: window 256 97 and 109 us, 1024 163 and 164, none 265 and 247; 32 over 8 heads of 128: 512 new
+// tokens of eight sequences over 512 53 and 54, over 1024 70 and 68, over 2048 120 and 110, 2048 of two over 16384 893 and 777.
+// Single tokens (ONE) have one warp at work and wait for memory: the fewer steps the better (64 sequences of 16384 tokens, 32 over 4
+// heads of 128: 268 against 273 us; 100 of up to 2000, 16 over 4 heads of 64: 50 against 53).
 template <int TILES, int STEP>
 constexpr int kFwdThreads = TILES * 128 + (STEP == 128 ? 128 : 64);     // four softmax warps a tile; MMA issue; loads; for setmaxnreg two more
 constexpr int kMost = 96;                                               // STEP 128: keys whose P V starts early
@@ -77,23 +79,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float y;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
-}
-
-// 2^x for x <= 127, two at a time without the special-function units: x = n + f with |f| <= 1/2 (1.5 2^23 added and taken off again
-// rounds to the nearest n, and leaves n in the low bits), 2^f by the polynomial of degree five that has 1 at 0 and the least largest
-// relative error, 2^-22.6 in fp32, and n added to the exponent.  Below -127, where the sum would leave the exponent's range, x counts as -127,
-// whose result is 0; from there to -126 results are positive and below 2^-126.  NaN is not kept: the row's reference takes care of it.
-__device__ __forceinline__ float2 poly_exp2(float2 x) {
-  x = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
-  const float2 t = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f));
-  const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
-  const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
-  float2 y = __ffma2_rn(make_float2(0.001326472731307149f, 0.001326472731307149f), f, make_float2(0.009671512991189957f, 0.009671512991189957f));
-  y = __ffma2_rn(y, f, make_float2(0.05550733581185341f, 0.05550733581185341f));
-  y = __ffma2_rn(y, f, make_float2(0.24022242426872253f, 0.24022242426872253f));
-  y = __ffma2_rn(y, f, make_float2(0.6931470036506653f, 0.6931470036506653f));
-  y = __ffma2_rn(y, f, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
 
 // Queries of one tile, or of both, as the kernel needs them: token numbers within the sequence's new tokens.
@@ -263,9 +248,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
 
-  // With 128 scores a thread registers go where the scores are, four warps at a time (launched with 168 a thread).
+  // With 128 scores a thread registers go where the scores are, four warps at a time (launched with 168 a thread for
+  // two tiles, with 128 for one).
   if (warp >= kMma) {
-    if constexpr (STEP == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if constexpr (STEP == 128 && TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if constexpr (STEP == 128 && TILES == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == kLoad) {
       // ---------------------------------------------------------------- loads
       bool ok = true;
@@ -383,7 +370,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
     }
   } else {
-    if constexpr (STEP == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if constexpr (STEP == 128 && TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if constexpr (STEP == 128 && TILES == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ---------------------------------------------------------------- softmax / output threads of one tile
     const int g = warp >> 2;                         // tile of this warp group
     const int lane_group = warp & 3;                 // TMEM lane quarter this warp may access
@@ -481,9 +469,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       // p = 2^(s scale - m scale): one packed multiply-add per pair, then the exponential; the row sum is taken over the fp32
       // values.  P is rounded to 16 bits as an operand of the second product (half a step of its type, relative to values whose
-      // largest is near 1).  The special-function units form four exponentials a cycle and quarter of a multiprocessor: 1 024 cycles for
-      // 64 keys of two tiles, of the 1 900 that a step takes.  Of 128 scores a thread three pairs of eight are formed on the other units
-      // (30 011 tokens, window 2048: 543 -> 525 us); of 64 that gained nothing, the chain of the polynomial is too long for two warps.
+      // largest is near 1).  The special-function units form four exponentials a cycle and quarter of a
+      // multiprocessor: 1 024 cycles for 64 keys of two tiles, of the 1 900 that a step takes.  A part of them by a polynomial on the
+      // other units gained nothing with two warps a quarter, and where the power limit holds the clock it lost (3 420 against 3 120 us
+      // for 8192 tokens over 32768).
       const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
       const float nm = -m_use * p.scale_log2;
       const float2 nm2 = make_float2(nm, nm);
@@ -495,7 +484,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (int j = 0; j < 16; ++j) {
           const int at = part * 32 + 2 * j;
           const float2 e = __ffma2_rn(make_float2(__uint_as_float(r[at]), __uint_as_float(r[at + 1])), sc2, nm2);
-          const float2 pe = STEP == 128 && (j % 8 == 1 || j % 8 == 4 || j % 8 == 6) ? poly_exp2(e) : make_float2(fast_exp2(e.x), fast_exp2(e.y));
+          const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
           if (j & 1) rs2b = __fadd2_rn(rs2b, pe); else rs2 = __fadd2_rn(rs2, pe);
           elem2_t h = f22e2(pe);
           packed[j] = *reinterpret_cast<uint32_t*>(&h);
@@ -653,7 +642,7 @@ int launch(dim3 grid, cudaStream_t s, const CUtensorMap& q, const CUtensorMap& k
 }
 
 // STEP 128: by the keys that a pair of tiles sees at most.
-bool far_enough(long long keys, int D) { return D == 128 && keys >= 2048; }
+bool far_enough(long long keys, int D) { return D == 128 && keys >= 1536; }
 
 }  // namespace
 
@@ -747,7 +736,7 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   const dim3 grid((unsigned)pairs, kv_heads, splits);
   const long long most = (long long)max_pages * page;
   const bool wide = far_enough((long long)p.window + per < most ? p.window + per : most, D);
-  if (single     ? (D == 64 ? launch<64, true, 1, true, 64>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, true, 64>(grid, s, mq, mk, mv, mq, mq, p))
+  if (single     ? (D == 64 ? launch<64, true, 1, true, 128>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, true, 128>(grid, s, mq, mk, mv, mq, mq, p))
       : one_tile ? (D == 64 ? launch<64, true, 1, false, 64>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, false, 64>(grid, s, mq, mk, mv, mq, mq, p))
       : D == 64  ? launch<64, true, 2, false, 64>(grid, s, mq, mk, mv, mq, mq, p)
       : wide     ? launch<128, true, 2, false, 128>(grid, s, mq, mk, mv, mq, mq, p)

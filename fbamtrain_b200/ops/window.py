@@ -139,16 +139,17 @@ def window_attention_qkv(qkv, kv, window, sinks, lengths, scale):
 
 
 @functools.lru_cache(maxsize=1024)
-def _splits(units: int, blocks: int, slots: int) -> int:
+def _splits(units: int, blocks: int, slots: int, sums: float) -> int:
     """How many thread blocks share the keys of one tile (or pair of tiles) of queries, where ``units`` of them have up to ``blocks``
-    key blocks each and the machine holds ``slots`` thread blocks: what takes the least of (waves) x (key blocks of a share, and three
-    for a thread block's start and end), with eight for joining the shares (another launch, and on the host two more tensors).
-    Where the units alone fill the machine twice, shares would save nothing and their sums are large."""
+    key blocks each and the machine holds ``slots`` thread blocks.  In key blocks: the longer of one share and of all shares over all
+    slots, three a share for its start and end; half a share that the last ones are on their own; and where there are shares, eight for
+    joining them (another launch, and on the host two more tensors) and ``sums`` for each, which writes and reads them.  64 sequences of
+    16384 tokens, 4 key heads of 128 (256 units for 296 slots), shares of each: 1 303 us, 3 281, 5 268, 8 272, 24 315; 20 of up to 16000,
+    8 key heads: 1 228, 4 168, 8 167, 24 186; 100 of up to 2000, 4 key heads of 64: 1 50, 2 53, 4 63."""
     best, splits = None, 1
-    if units >= 2 * slots:
-        return 1
     for s in range(1, min(64, blocks) + 1):
-        cost = -(-units * s // slots) * (-(-blocks // s) + 3) + (8 if s > 1 else 0)
+        share = blocks / s + 3
+        cost = max(share, units * s * share / slots) + share / 2 + (8 + s * sums if s > 1 else 0)
         if best is None or cost < best:
             best, splits = cost, s
     return splits
@@ -165,7 +166,8 @@ def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks
     single = offsets is None and h // kv <= 16              # one token a sequence: two thread blocks a multiprocessor
     units = kv * (b if offsets is None else n // per + min(n, b))
     keys = most * page if window is None else min(most * page, window + per + sinks + 256)
-    splits = _splits(units, max(1, (keys + 127) // 128), 296 if single else 148)
+    slots = 296 if single else 148
+    splits = _splits(units, max(1, (keys + 127) // 128), slots, n * h / (64 * slots))
     part_o = part_ml = None
     if splits > 1:
         part_o = q.new_empty((splits, n, h, d), dtype=F32)
