@@ -53,8 +53,11 @@ struct FwdParams {
 };
 
 // TILES = 2: two tiles a thread block, one thread block a multiprocessor: they share each key block.
-// TILES = 1: one tile a thread block, two thread blocks a multiprocessor, where all of them fit at once (296): 3 x 696 with a window
-// of 2, 8 heads of 128: 11.9 against 16.5 us; 8 x 1024, window 256, 16 heads of 64, where they do not: 65 against 48 us.
+// TILES = 1: one tile a thread block, two thread blocks a multiprocessor, where all of them fit at once (296).  One tile and two: 3 x 696
+// with a window of 2, 8 heads of 64 8.8 and 10.9 us, of 128 10.7 and 12.4; 2 x 900, window 300, 8 over 4 heads of 64 10.6 and 12.6, of 128
+// 13.1 and 14.6; 8 x 1024, window 256, 16 heads of 64, where they do not fit, 59 and 43.  Over a cache heads of 128 have no room for a
+// page's way (two slots): 145 new tokens of ten sequences over 900, 8 over 4 heads of 64 16.6 and 19.6, of 128 26 and 23, which stay with
+// two tiles.
 // ONE: that tile is one token with up to 16 heads.  It has little to do for each key block that arrives, and two of them hide each
 // other's waits.  Its Q keeps 16 rows a panel; what the product reads behind them are other buffers, in rows that nobody looks at.
 constexpr int kResident = 296;
@@ -724,7 +727,7 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   const bool single = offsets == nullptr && group <= 16;
   if (single) p.tile_tokens = 1;
   const long long spare = (rows < B ? rows : B) + 1;
-  const bool one_tile = !single && splits == 1 && (rows / p.tile_tokens + spare) * kv_heads <= kResident;
+  const bool one_tile = D == 64 && !single && splits == 1 && (rows / p.tile_tokens + spare) * kv_heads <= kResident;
   const int per = (one_tile ? 1 : 2) * p.tile_tokens;
   const long long pairs = offsets == nullptr ? B : rows / per + spare;
   int e;
@@ -737,7 +740,7 @@ int fbam_cache_attention(const void* q, long long q_st, long long q_sh, const vo
   const long long most = (long long)max_pages * page;
   const bool wide = far_enough((long long)p.window + per < most ? p.window + per : most, D);
   if (single     ? (D == 64 ? launch<64, true, 1, true, 128>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, true, 128>(grid, s, mq, mk, mv, mq, mq, p))
-      : one_tile ? (D == 64 ? launch<64, true, 1, false, 64>(grid, s, mq, mk, mv, mq, mq, p) : launch<128, true, 1, false, 64>(grid, s, mq, mk, mv, mq, mq, p))
+      : one_tile ? launch<64, true, 1, false, 64>(grid, s, mq, mk, mv, mq, mq, p)
       : D == 64  ? launch<64, true, 2, false, 64>(grid, s, mq, mk, mv, mq, mq, p)
       : wide     ? launch<128, true, 2, false, 128>(grid, s, mq, mk, mv, mq, mq, p)
                  : launch<128, true, 2, false, 64>(grid, s, mq, mk, mv, mq, mq, p))

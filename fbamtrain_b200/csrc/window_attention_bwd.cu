@@ -60,7 +60,8 @@ struct BwdParams {
 };
 
 // delta, and what else has to be there before the main kernel: counters at zero, dQ of the rows behind a sequence's end.  D / 8 threads
-// a row, four rows a thread whose loads are on their way together.
+// a row, four rows a thread whose loads are on their way together; four of a row's threads place one of its sums each, since where they
+// go takes divisions.
 template <int D>
 __global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restrict__ o, const elem_t* __restrict__ low, const elem_t* __restrict__ d_o, long long do_sb, long long do_st, long long do_sh, float* __restrict__ delta, int* counters,
                                                            int n_counters, const BwdParams p) {
@@ -72,8 +73,18 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restr
   uint4 ov[kRowsEach], lv[kRowsEach], gv[kRowsEach];
   int h[kRowsEach], t[kRowsEach], b[kRowsEach];
   bool there[kRowsEach];
-  const long long bt = row0 / heads;                 // divided once: the next rows are counted on
-  int h_at = (int)(row0 - bt * heads), b_at = (int)(bt / p.T), t_at = (int)(bt - (long long)b_at * p.T);
+  int h_at, t_at, b_at;                              // divided once: the next rows are counted on
+  if (all < 0x80000000ll) {
+    const unsigned bt = (unsigned)row0 / (unsigned)heads;
+    h_at = (int)((unsigned)row0 - bt * heads);
+    b_at = (int)(bt / (unsigned)p.T);
+    t_at = (int)(bt - (unsigned)b_at * p.T);
+  } else {
+    const long long bt = row0 / heads;
+    h_at = (int)(row0 - bt * heads);
+    b_at = (int)(bt / p.T);
+    t_at = (int)(bt - (long long)b_at * p.T);
+  }
   const int step_t = kStep / heads, step_h = kStep - step_t * heads;
 #pragma unroll
   for (int u = 0; u < kRowsEach; ++u) {
@@ -102,6 +113,10 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restr
       gv[u] = *reinterpret_cast<const uint4*>(d_o + b[u] * do_sb + t[u] * do_st + h[u] * do_sh + part * 8);
     }
   }
+  static_assert(kLanes >= kRowsEach, "a lane a row");
+  float sum = 0.0f;
+  int h_of = 0, t_of = 0, b_of = 0;
+  bool placed = false;
 #pragma unroll
   for (int u = 0; u < kRowsEach; ++u) {
     float s = 0.0f;
@@ -117,9 +132,17 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restr
     }
 #pragma unroll
     for (int off = kLanes / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (there[u] && part == 0)
-      delta[(((long long)b[u] * p.kv_heads + (unsigned)h[u] / p.group) * p.tiles + (unsigned)t[u] / p.tile_tokens) * kRows +
-            (unsigned)t[u] % p.tile_tokens * p.group + (unsigned)h[u] % p.group] = -s;
+    if (part == u) {
+      sum = s;
+      h_of = h[u];
+      t_of = t[u];
+      b_of = b[u];
+      placed = there[u];
+    }
+  }
+  if (placed) {
+    const unsigned kvh = (unsigned)h_of / p.group, tile = (unsigned)t_of / p.tile_tokens;
+    delta[(((long long)b_of * p.kv_heads + kvh) * p.tiles + tile) * kRows + (t_of - tile * p.tile_tokens) * p.group + (h_of - kvh * p.group)] = -sum;
   }
 }
 
