@@ -15,6 +15,7 @@ from . import native as nv
 from .derivatives import first_only, tracked
 
 F32 = torch.float32
+_FAR = 2 ** 30 - 1                                        # windows beyond see everything
 
 
 def _usable(x: torch.Tensor) -> bool:
@@ -26,6 +27,11 @@ def _usable(x: torch.Tensor) -> bool:
 
 def _fetchable(x: torch.Tensor) -> torch.Tensor:
     return x if _usable(x) else x.clone(memory_format=torch.contiguous_format)
+
+
+def _reach(window, sinks):
+    """A window (0: none) and first tokens that fit the kernels' integers."""
+    return 0 if window is None or window > _FAR else window, min(sinks, _FAR)
 
 
 def _pairs(b, t, window):
@@ -45,7 +51,7 @@ def _forward(q, k, v, window, sinks, lengths, scale, keep):
         low = torch.empty_like(out)
         lse = q.new_empty((b, kv, (t + tokens - 1) // tokens, 128), dtype=F32)
     nv.check(nv.lib(q).fbam_window_fwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-                                       out.data_ptr(), nv.addr(low), nv.addr(lse), nv.addr(lengths), b, t, kv, h // kv, d, window or 0, sinks, scale,
+                                       out.data_ptr(), nv.addr(low), nv.addr(lse), nv.addr(lengths), b, t, kv, h // kv, d, *_reach(window, sinks), scale,
                                        nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_fwd")
     flops.add(4.0 * h * d * _pairs(b, t, window))
     return out, low, lse
@@ -58,13 +64,13 @@ def _backward(saved, d_out, into, window, sinks, scale):
     kv = k.shape[2]
     d_out = _fetchable(d_out)
     lib = nv.lib(q)
-    floats = lib.fbam_window_bwd_workspace(b, t, kv, h // kv, d, window or 0, sinks)
+    floats = lib.fbam_window_bwd_workspace(b, t, kv, h // kv, d, *_reach(window, sinks))
     work = lse.new_empty(floats)
     dq, dk, dv = into
     nv.check(lib.fbam_window_bwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
                                  out.data_ptr(), low.data_ptr(), d_out.data_ptr(), *d_out.stride()[:3], lse.data_ptr(), nv.addr(lengths),
                                  work.data_ptr(), floats, dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(),
-                                 *dv.stride()[:3], b, t, kv, h // kv, d, window or 0, sinks, scale,
+                                 *dv.stride()[:3], b, t, kv, h // kv, d, *_reach(window, sinks), scale,
                                  nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_bwd")
     flops.add(10.0 * h * d * _pairs(b, t, window))
 
@@ -175,6 +181,6 @@ def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks
     nv.check(lib.fbam_cache_attention(
         q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
         tables.data_ptr(), tables.stride(0), lengths.data_ptr(), nv.addr(offsets), out.data_ptr(), nv.addr(part_o), nv.addr(part_ml),
-        splits, n, b, most, page, pages, kv, h // kv, d, window or 0, sinks, d ** -0.5, nv.status_word(q.device).data_ptr(), nv.stream()),
+        splits, n, b, most, page, pages, kv, h // kv, d, *_reach(window, sinks), d ** -0.5, nv.status_word(q.device).data_ptr(), nv.stream()),
         "fbam_cache_attention")
     return out

@@ -287,3 +287,18 @@ def test_what_is_not_a_number_shows(t, h, kv, win, d):
     last = ops.cache_attention(q[0, t // 2:t // 2 + 1], *padded, tables, lengths - (t - t // 2 - 1), None, win)
     assert last[0, :h // kv].isnan().all() and last[0, h // kv:].isfinite().all()
     nv.check_status(torch.device("cuda", 0))
+
+
+def test_windows_beyond_the_kernels_integers():
+    gen = _gen("far windows")
+    qkv, dy = _randn(gen, 1, 300, 6, 64).requires_grad_(), _randn(gen, 1, 300, 2, 64)
+    cache = _cache(gen, [300, 200], 16, 2, 64)
+    q = _randn(gen, 2, 4, 64)
+
+    def everything(window, sinks):
+        y = ops.window_attention_qkv(qkv, 2, window, sinks)
+        return [y, *torch.autograd.grad((y,), (qkv,), (dy,)), ops.cache_attention(q, *cache, None, window, sinks)]
+
+    for window, sinks, same in ((2 ** 32 + 5, 3, (None, 0)), (2 ** 40, 2 ** 40, (None, 0)), (70, 2 ** 32 + 1, (70, 300))):
+        assert all(torch.equal(a, b) for a, b in zip(everything(window, sinks), everything(*same)))
+    nv.check_status(torch.device("cuda", 0))
