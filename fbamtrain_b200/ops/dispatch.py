@@ -442,9 +442,10 @@ def _check_cache(n, kv_heads, d, dtype, device, k_pages, v_pages, tables, length
         raise ValueError(f"without offsets there is one new token for each of {b} sequences, got {n}")
     if offsets is not None and (offsets.shape != (b + 1,) or offsets.dtype != torch.int32 or not offsets.is_contiguous()):
         raise ValueError(f"offsets are int32 ({b + 1},), got {offsets.dtype} {tuple(offsets.shape)}")
-    for name, x in (("key pages", k_pages), ("value pages", v_pages), ("page tables", tables), ("lengths", lengths), ("offsets", offsets)):
-        if x is not None and x.device != device:
-            raise ValueError(f"{name} are on {x.device}, the tokens on {device}")
+    if not (k_pages.device == v_pages.device == tables.device == lengths.device == device and (offsets is None or offsets.device == device)):
+        for name, x in (("key pages", k_pages), ("value pages", v_pages), ("page tables", tables), ("lengths", lengths), ("offsets", offsets)):
+            if x is not None and x.device != device:
+                raise ValueError(f"{name} are on {x.device}, the tokens on {device}")
 
 
 def _check_cache_native(d, k_pages, v_pages) -> None:
@@ -454,8 +455,8 @@ def _check_cache_native(d, k_pages, v_pages) -> None:
     if k_pages.shape[1] % 8:
         raise ValueError(f"pages have a multiple of 8 slots, got {k_pages.shape[1]}")
     for x in (k_pages, v_pages):
-        *outer, inner = x.stride()
-        if inner != 1 or x.data_ptr() % 16 or any(s % 8 or (s == 0 and n > 1) for s, n in zip(outer, x.shape)):
+        a, b, c, inner = x.stride()
+        if inner != 1 or x.data_ptr() % 16 or (a | b | c) % 8 or (0 in (a, b, c) and any(s == 0 and n > 1 for s, n in zip((a, b, c), x.shape))):
             raise ValueError("pages start at 16-byte boundaries, with 16-byte strides and channels side by side")
 
 

@@ -46,7 +46,8 @@ def _turned(x, positions, freqs, heads, interleaved, inverse):
         x = x.contiguous()
     y = x.new_empty((b, t, h, d))
     sb, st, sh, _ = x.stride()
-    pb, pt = positions.stride()
+    *rows, pt = positions.stride()
+    pb = rows[0] if rows and positions.shape[0] > 1 else 0          # one row of positions is everyone's
     nv.check(nv.lib(x).fbam_rotary(x.data_ptr(), sb, st, sh, y.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, pb, pt,
                                    freqs.table, len(freqs.turns), freqs.magnitude, interleaved, inverse, b, t, h, d, heads, nv.stream()),
              "fbam_rotary")
@@ -71,7 +72,6 @@ class _Rotary(torch.autograd.Function):
 def rotary(x, positions, freqs, heads, interleaved):
     if positions.device != x.device:
         raise ValueError(f"positions are on {positions.device}, the heads on {x.device}")
-    positions = positions.expand(x.shape[:2])
     if tracked(x):
         return _Rotary.apply(x, positions, freqs, heads, interleaved)
     return _turned(x, positions, freqs, heads, interleaved, False)
@@ -79,12 +79,14 @@ def rotary(x, positions, freqs, heads, interleaved):
 
 def cache_append(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interleaved, q_heads, kv_heads):
     n, _, d = qkv.shape
-    if qkv.stride(2) != 1 or qkv.stride(0) % 8 or qkv.stride(1) % 8 or qkv.data_ptr() % 16:
+    row, head, inner = qkv.stride()
+    if inner != 1 or (row | head) % 8 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
+        row, head, _ = qkv.stride()
     q = qkv.new_empty((n, q_heads, d))
     turns, pairs, magnitude = (None, 0, 1.0) if freqs is None else (freqs.table, len(freqs.turns), freqs.magnitude)
     nv.check(nv.lib(qkv).fbam_cache_append(
-        qkv.data_ptr(), qkv.stride(0), qkv.stride(1), q.data_ptr(), k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(),
+        qkv.data_ptr(), row, head, q.data_ptr(), k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(),
         *v_pages.stride()[:3], tables.data_ptr(), tables.stride(0), lengths.data_ptr(), nv.addr(offsets), turns, pairs, magnitude,
         interleaved, n, tables.shape[0], tables.shape[1], k_pages.shape[1], k_pages.shape[0], q_heads, kv_heads, d, nv.stream()),
         "fbam_cache_append")

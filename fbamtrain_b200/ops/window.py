@@ -22,7 +22,12 @@ def _usable(x: torch.Tensor) -> bool:
     """Whether the copy engine can fetch ``x`` ``(..., heads, channels)`` where it lies: channels side by side, a start and strides of 16
     bytes, nothing expanded."""
     *outer, inner = x.stride()
-    return inner == 1 and x.data_ptr() % 16 == 0 and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in zip(outer, x.shape))
+    if inner != 1 or x.data_ptr() % 16:
+        return False
+    for s, n in zip(outer, x.shape):
+        if s % 8 or (s == 0 and n > 1):
+            return False
+    return True
 
 
 def _fetchable(x: torch.Tensor) -> torch.Tensor:
@@ -40,46 +45,74 @@ def _pairs(b, t, window):
     return b * (w * (w + 1) // 2 + (t - w) * w)
 
 
-def _forward(q, k, v, window, sinks, lengths, scale, keep):
-    """``(out, low, lse)``; the last two with ``keep``: what the backward needs, ``low`` being what rounding took off ``out``."""
-    b, t, h, d = q.shape
-    kv = k.shape[2]
-    out = q.new_empty((b, t, h, d))
-    tokens = 128 // (h // kv)                            # of a tile of 128 rows
-    low = lse = None
+def _of(x):
+    """Where heads lie, as the entry points take them: the first one's address and the strides."""
+    return x.data_ptr(), x.stride()[:3]
+
+
+def _parts(qkv, kv):
+    """The query, key and value heads of a fused projection in this form (views of them would cost the host as much as the launch)."""
+    at, strides = _of(qkv)
+    step = strides[2] * 2                                # 16-bit values
+    heads = qkv.shape[2] - 2 * kv
+    return (at, strides), (at + heads * step, strides), (at + (heads + kv) * step, strides)
+
+
+def _forward(like, shape, q, k, v, window, sinks, lengths, scale, keep):
+    """``(out, kept)``; the latter with ``keep``, for the backward: an fp32 value for each row of each tile, and behind them, 16-bit,
+    what rounding took off ``out``."""
+    b, t, h, kv, d = shape
+    out = like.new_empty((b, t, h, d))
+    kept, lse, low = None, 0, 0
     if keep:
-        low = torch.empty_like(out)
-        lse = q.new_empty((b, kv, (t + tokens - 1) // tokens, 128), dtype=F32)
-    nv.check(nv.lib(q).fbam_window_fwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-                                       out.data_ptr(), nv.addr(low), nv.addr(lse), nv.addr(lengths), b, t, kv, h // kv, d, *_reach(window, sinks), scale,
-                                       nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_fwd")
+        rows = _lse_rows(shape)
+        kept = like.new_empty((rows + b * t * h * d // 2,), dtype=F32)
+        lse = kept.data_ptr()
+        low = lse + 4 * rows
+    (qp, qs), (kp, ks), (vp, vs) = q, k, v
+    nv.check(nv.lib(like).fbam_window_fwd(qp, *qs, kp, vp, *ks, *vs, out.data_ptr(), low, lse, nv.addr(lengths), b, t, kv, h // kv, d,
+                                          *_reach(window, sinks), scale, nv.status_word(like.device).data_ptr(), nv.stream()), "fbam_window_fwd")
     flops.add(4.0 * h * d * _pairs(b, t, window))
-    return out, low, lse
+    return out, kept
 
 
-def _backward(saved, d_out, into, window, sinks, scale):
-    """Fills ``into``: views for the gradients of the heads."""
-    q, k, v, out, low, lse, lengths = saved
-    b, t, h, d = q.shape
-    kv = k.shape[2]
+def _lse_rows(shape):
+    b, t, h, kv, _ = shape
+    tokens = 128 // (h // kv)                            # of a tile of 128 rows
+    return b * kv * ((t + tokens - 1) // tokens) * 128
+
+
+def _backward(shape, q, k, v, out, kept, lengths, d_out, dq, dk, dv, window, sinks, scale):
+    """Writes the gradients of the heads where ``dq``, ``dk`` and ``dv`` say."""
+    b, t, h, kv, d = shape
     d_out = _fetchable(d_out)
-    lib = nv.lib(q)
-    floats = lib.fbam_window_bwd_workspace(b, t, kv, h // kv, d, *_reach(window, sinks))
-    work = lse.new_empty(floats)
-    dq, dk, dv = into
-    nv.check(lib.fbam_window_bwd(q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-                                 out.data_ptr(), low.data_ptr(), d_out.data_ptr(), *d_out.stride()[:3], lse.data_ptr(), nv.addr(lengths),
-                                 work.data_ptr(), floats, dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(),
-                                 *dv.stride()[:3], b, t, kv, h // kv, d, *_reach(window, sinks), scale,
-                                 nv.status_word(q.device).data_ptr(), nv.stream()), "fbam_window_bwd")
+    lib = nv.lib(out)
+    how = (b, t, kv, h // kv, d, *_reach(window, sinks))
+    floats = lib.fbam_window_bwd_workspace(*how)
+    work = kept.new_empty(floats)
+    lse = kept.data_ptr()
+    (qp, qs), (kp, ks), (vp, vs), (dqp, dqs), (dkp, dks), (dvp, dvs) = q, k, v, dq, dk, dv
+    nv.check(lib.fbam_window_bwd(qp, *qs, kp, vp, *ks, *vs, out.data_ptr(), lse + 4 * _lse_rows(shape), d_out.data_ptr(), *d_out.stride()[:3], lse,
+                                 nv.addr(lengths), work.data_ptr(), floats, dqp, *dqs, dkp, *dks, dvp, *dvs, *how, scale,
+                                 nv.status_word(out.device).data_ptr(), nv.stream()), "fbam_window_bwd")
     flops.add(10.0 * h * d * _pairs(b, t, window))
+
+
+def _shape(q, k):
+    b, t, h, d = q.shape
+    return b, t, h, k.shape[2], d
+
+
+def _shape_qkv(qkv, kv):
+    b, t, all_heads, d = qkv.shape
+    return b, t, all_heads - 2 * kv, kv, d
 
 
 class _Window(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, lengths, scale):
-        out, low, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
-        ctx.save_for_backward(q, k, v, out, low, lse, lengths)
+        out, kept = _forward(q, _shape(q, k), _of(q), _of(k), _of(v), window, sinks, lengths, scale, True)
+        ctx.save_for_backward(q, k, v, out, kept, lengths)
         ctx.linked = ()
         ctx.how = (window, sinks, scale)
         return out
@@ -87,18 +120,17 @@ class _Window(torch.autograd.Function):
     @staticmethod
     @first_only("window_attention")
     def backward(ctx, d_out):
-        saved = ctx.saved_tensors
-        into = [x.new_empty(x.shape) for x in saved[:3]]
-        _backward(saved, d_out, into, *ctx.how)
-        return (*into, None, None, None, None)
+        q, k, v, out, kept, lengths = ctx.saved_tensors
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        _backward(_shape(q, k), _of(q), _of(k), _of(v), out, kept, lengths, d_out, _of(dq), _of(dk), _of(dv), *ctx.how)
+        return dq, dk, dv, None, None, None, None
 
 
 class _WindowQkv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, kv, window, sinks, lengths, scale):
-        q, k, v = _heads(qkv, kv)
-        out, low, lse = _forward(q, k, v, window, sinks, lengths, scale, True)
-        ctx.save_for_backward(qkv, out, low, lse, lengths)
+        out, kept = _forward(qkv, _shape_qkv(qkv, kv), *_parts(qkv, kv), window, sinks, lengths, scale, True)
+        ctx.save_for_backward(qkv, out, kept, lengths)
         ctx.linked = ()
         ctx.how = (window, sinks, scale)
         ctx.kv = kv
@@ -107,14 +139,11 @@ class _WindowQkv(torch.autograd.Function):
     @staticmethod
     @first_only("window_attention_qkv")
     def backward(ctx, d_out):
-        qkv, out, low, lse, lengths = ctx.saved_tensors
+        qkv, out, kept, lengths = ctx.saved_tensors
+        kv = ctx.kv
         grad = qkv.new_empty(qkv.shape)
-        _backward((*_heads(qkv, ctx.kv), out, low, lse, lengths), d_out, _heads(grad, ctx.kv), *ctx.how)
+        _backward(_shape_qkv(qkv, kv), *_parts(qkv, kv), out, kept, lengths, d_out, *_parts(grad, kv), *ctx.how)
         return grad, None, None, None, None, None
-
-
-def _heads(qkv, kv):
-    return qkv.split((qkv.shape[2] - 2 * kv, kv, kv), 2)
 
 
 def _lengths(lengths, like):
@@ -133,7 +162,7 @@ def window_attention(q, k, v, window, sinks, lengths, scale):
     q, k, v = _fetchable(q), _fetchable(k), _fetchable(v)
     if tracked(q, k, v):
         return _Window.apply(q, k, v, window, sinks, lengths, scale)
-    return _forward(q, k, v, window, sinks, lengths, scale, False)[0]
+    return _forward(q, _shape(q, k), _of(q), _of(k), _of(v), window, sinks, lengths, scale, False)[0]
 
 
 def window_attention_qkv(qkv, kv, window, sinks, lengths, scale):
@@ -141,7 +170,7 @@ def window_attention_qkv(qkv, kv, window, sinks, lengths, scale):
     qkv = _fetchable(qkv)
     if tracked(qkv):
         return _WindowQkv.apply(qkv, kv, window, sinks, lengths, scale)
-    return _forward(*_heads(qkv, kv), window, sinks, lengths, scale, False)[0]
+    return _forward(qkv, _shape_qkv(qkv, kv), *_parts(qkv, kv), window, sinks, lengths, scale, False)[0]
 
 
 @functools.lru_cache(maxsize=1024)
@@ -166,6 +195,7 @@ def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks
     b, most = tables.shape
     pages, page, kv, _ = k_pages.shape
     q = _fetchable(q)
+    q_row, q_head, _ = q.stride()
     out = q.new_empty((n, h, d))
     lib = nv.lib(q)
     per = 2 * (128 // (h // kv))
@@ -179,7 +209,7 @@ def cache_attention(q, k_pages, v_pages, tables, lengths, offsets, window, sinks
         part_o = q.new_empty((splits, n, h, d), dtype=F32)
         part_ml = part_o.new_empty((splits, n, h, 2))
     nv.check(lib.fbam_cache_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
+        q.data_ptr(), q_row, q_head, k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
         tables.data_ptr(), tables.stride(0), lengths.data_ptr(), nv.addr(offsets), out.data_ptr(), nv.addr(part_o), nv.addr(part_ml),
         splits, n, b, most, page, pages, kv, h // kv, d, *_reach(window, sinks), d ** -0.5, nv.status_word(q.device).data_ptr(), nv.stream()),
         "fbam_cache_attention")
