@@ -74,9 +74,9 @@ template <int D, int TILES, bool ONE>
 constexpr int fwd_smem_bytes() { return TILES * (D / 64) * kQPanel<ONE> + kSlots<D, TILES, ONE> * kKeys * D * 2 + 256 + 1024; }
 // STEP: keys whose scores a softmax thread has at a time.  64: the next 64 are scored meanwhile, beside them, and less is scored that
 // the masks take away.  128: a product of 128 keys reads Q half as often, but the tensor memory has no room to score ahead; P V starts
-// with the first 96 keys.  With heads of 128 the products count where the keys are many: 4 x 4096, 16
-// over 4 heads of 128, STEP 64 and 128: window 256 97 and 109 us, 1024 163 and 164, none 265 and 247; 32 over 8 heads of 128: 512 new
-// tokens of eight sequences over 512 53 and 54, over 1024 70 and 68, over 2048 120 and 110, 2048 of two over 16384 893 and 777.
+// with the first 96 keys.  With heads of 128 the products count where the keys are many: 4 x 4096, 16 over 4 heads of 128, STEP 64 and
+// 128: window 256 97 and 109 us, 1024 163 and 164, none 265 and 247; 32 over 8 heads of 128: 512 new tokens of eight sequences over 512
+// 53 and 54, over 1024 70 and 68, over 2048 120 and 110, 2048 of two over 16384 893 and 777.
 // Single tokens (ONE) have one warp at work and wait for memory: the fewer steps the better (64 sequences of 16384 tokens, 32 over 4
 // heads of 128: 268 against 273 us; 100 of up to 2000, 16 over 4 heads of 64: 50 against 53).
 template <int TILES, int STEP>
@@ -127,9 +127,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* q_full = bars;
   uint64_t* full = bars + 1;                 // [NS]
   uint64_t* empty = full + NS;               // [NS]
-  uint64_t* s_full = empty + NS;             // [tile][2]: of the steps in turn
-  uint64_t* p_ready = s_full + 2 * TILES;    // [tile][2]
-  uint64_t* pv_full = p_ready + 2 * TILES;   // [tile][2]
+  uint64_t* s_full = empty + NS;             // [tile][2]: of the steps in turn (STEP 128: the first)
+  uint64_t* p_ready = s_full + 2 * TILES;    // [tile][2]: of the steps in turn (STEP 128: of the first 96 keys, of all)
+  uint64_t* pv_full = p_ready + 2 * TILES;   // [tile][2]: as s_full
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_full + 2 * TILES);
   int* found = reinterpret_cast<int*>(tmem_slot + 1);   // sequence, pair
 
