@@ -50,7 +50,7 @@ struct BwdParams {
   const int* lengths;    // (B) or null
   float scale_log2, scale;
   const float* lse;      // (B, kv_heads, tile, 128): minus log2 of the sum of 2^(s scale log2(e))
-  const float* delta;    // the same: minus delta
+  const float* delta;    // the same: minus delta scale
   float* sums;           // (B, kv_heads, tile, D / 4, 128, 4) fp32: written before it is read
   int* counters;         // (B, kv_heads, tile): contributions that are in; zeroed
   int* ticket;           // zeroed
@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const elem_t* __restr
   }
   if (placed) {
     const unsigned kvh = (unsigned)h_of / p.group, tile = (unsigned)t_of / p.tile_tokens;
-    delta[(((long long)b_of * p.kv_heads + kvh) * p.tiles + tile) * kRows + (t_of - tile * p.tile_tokens) * p.group + (h_of - kvh * p.group)] = -sum;
+    delta[(((long long)b_of * p.kv_heads + kvh) * p.tiles + tile) * kRows + (t_of - tile * p.tile_tokens) * p.group + (h_of - kvh * p.group)] =
+        -sum * p.scale;
   }
 }
 
@@ -225,12 +226,12 @@ __device__ __forceinline__ void store_part(float4* sum, const uint32_t (&r)[N]) 
                                         __uint_as_float(r[4 * j + 3])));
 }
 template <int N>
-__device__ __forceinline__ void store_row(elem_t* dst, const uint32_t (&r)[N], float scale) {
+__device__ __forceinline__ void store_row(elem_t* dst, const uint32_t (&r)[N]) {
 #pragma unroll
   for (int j = 0; j < N; j += 8) {
     __align__(16) elem2_t hh[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j + 2 * q]) * scale, __uint_as_float(r[j + 2 * q + 1]) * scale);
+    for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j + 2 * q]), __uint_as_float(r[j + 2 * q + 1]));
     *reinterpret_cast<uint4*>(dst + j) = *reinterpret_cast<uint4*>(hh);
   }
 }
@@ -274,7 +275,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint8_t* sDS = sDO + DOS * kTile;
   uint8_t* sStage = sDS + kSq;                 // kStages
   float* sL = reinterpret_cast<float*>(sStage + kStages * kStage);   // two stages of 128: minus lse
-  float* sD = sL + 2 * 128;                    // DOS stages: minus delta
+  float* sD = sL + 2 * 128;                    // DOS stages: minus delta scale
   uint64_t* bars = reinterpret_cast<uint64_t*>(sD + DOS * 128);
   uint64_t* kv_full = bars;
   uint64_t* q_full = bars + 1;      // [2]
@@ -501,7 +502,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int lane_group = warp & 3, part = (warp - 4) >> 2;
     const int row = lane_group * 32 + lane;
     const uint32_t lane_addr = uint32_t(lane_group * 32) << 16;
-    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), scale2 = make_float2(p.scale, p.scale);
     uint8_t* dsPanel = sDS + part * 128 * 128;         // 64 queries
     const int my_row = lane_group * 32 + (lane >> 3 & 1) * 8 + (lane & 7), my_chunk = lane >> 4;   // as an address of store_matrices
     bool ok = true;
@@ -603,13 +604,14 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
         for (int h = 0; h < 2; ++h) tmem_ld_16x64(tm_dp + lane_addr + (uint32_t(h * 16) << 16) + part * 64, dp[h]);
         tmem_ld_wait();
-        // dS without the scale: dQ and dK are scaled once, at their ends
+        // dS with its scale, in one multiply-add a pair: P (dP - delta) alone is infinite in half 8 (D = 64) to 11.3 (D = 128) times
+        // earlier than dS.  In half dS itself has to be finite, and below 2^-14 it keeps an absolute error of 2^-25.
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float2 d = __fmul2_rn(make_float2(__uint_as_float(pr[h][j]), __uint_as_float(pr[h][j + 1])),
-                                        __fadd2_rn(make_float2(__uint_as_float(dp[h][j]), __uint_as_float(dp[h][j + 1])), ahead[j / 4]));
+                                        __ffma2_rn(make_float2(__uint_as_float(dp[h][j]), __uint_as_float(dp[h][j + 1])), scale2, ahead[j / 4]));
             pr[h][j] = __float_as_uint(d.x);
             pr[h][j + 1] = __float_as_uint(d.y);
           }
@@ -646,7 +648,6 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // through the stages of Q, which nothing reads any more, and out by the copy engine: as rows from registers they took 4 400
         // (D = 64) to 9 000 cycles of every thread block
         uint8_t* tile = sQ + part * kTile;
-        const float scale = part == 0 ? 1.0f : p.scale;
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t r[32];
@@ -656,7 +657,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           for (int j = 0; j < 4; ++j) {
             __align__(16) elem2_t hh[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j * 8 + 2 * q]) * scale, __uint_as_float(r[j * 8 + 2 * q + 1]) * scale);
+            for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j * 8 + 2 * q]), __uint_as_float(r[j * 8 + 2 * q + 1]));
             *reinterpret_cast<uint4*>(tile + c0 / 64 * 128 * 128 + swz(row, c0 % 64 / 8 + j)) = *reinterpret_cast<uint4*>(hh);
           }
         }
@@ -747,7 +748,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (half + 1 < D / 64) fetch(half + 1);
           if (token < p.tile_tokens && t_q < len) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) store_row(dst + half * 64 + c * 32, r[c], p.scale);
+            for (int c = 0; c < 2; ++c) store_row(dst + half * 64 + c * 32, r[c]);
           }
         }
       }
@@ -775,9 +776,8 @@ __global__ void __launch_bounds__(256) window_parts_kernel(const __grid_constant
     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
   }
   if (key >= p.T) return;
-  const float scale = which ? p.scale : 1.0f;
   elem_t* dst = which ? p.dk + b * p.k_sb + key * p.k_st + kvh * p.k_sh : p.dv + b * p.v_sb + key * p.v_st + kvh * p.v_sh;
-  __align__(8) elem2_t out[2] = {ff2e2(sum.x * scale, sum.y * scale), ff2e2(sum.z * scale, sum.w * scale)};
+  __align__(8) elem2_t out[2] = {ff2e2(sum.x, sum.y), ff2e2(sum.z, sum.w)};
   *reinterpret_cast<uint2*>(dst + piece * 4) = *reinterpret_cast<uint2*>(out);
 }
 

@@ -1,0 +1,58 @@
+"""Rotary positions, windowed attention and the paged cache on the kernels: what each call promises beyond ordinary inputs."""
+import zlib
+
+import pytest
+import torch
+
+import attention_oracle as oracle
+from fbamtrain_b200 import ops
+from fbamtrain_b200.ops import native as nv
+
+pytestmark = pytest.mark.gpu
+BF, HALF = torch.bfloat16, torch.float16
+I32 = torch.int32
+
+
+def _gen(*key):
+    return torch.Generator(device="cuda").manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def _randn(gen, *shape, dtype=BF, scale=1.0):
+    return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def _gradients(q, k, v, dy, window, sinks=0, lengths=None):
+    """All of a call against 64 bits; the gradients are returned."""
+    want = oracle.window(q, k, v, window, sinks, lengths, dy)
+    at = [x.clone().requires_grad_() for x in (q, k, v)]
+    y = ops.window_attention(*at, window, sinks, lengths)
+    oracle.within(y, *want["y"])
+    grads = torch.autograd.grad((y,), at, (dy,))
+    nv.check_status(q.device)
+    for g, name in zip(grads, ("dq", "dk", "dv")):
+        oracle.within(g, *want[name])
+    return grads
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# gradients of a scaled loss
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_gradients_in_half_are_finite_where_the_definition_is(d):
+    """Two equal scores, values of 1 and -1, a gradient of 4096 in all channels: the score's gradient is 32 d sqrt(d), 16 384 and
+    46 341, and before its scale 131 072 and 262 144, which half does not have."""
+    q, k, v = (torch.zeros(1, 2, 1, d, dtype=HALF, device="cuda") for _ in range(3))
+    q[..., 0] = 0.5
+    k[0, 0, 0, 1], k[0, 1, 0, 1] = 0.5, -0.5
+    v[0, 0], v[0, 1] = 1.0, -1.0
+    dy = torch.full((1, 2, 1, d), 4096.0, dtype=HALF, device="cuda")
+    dq, _, _ = _gradients(q, k, v, dy, None)
+    assert float(dq[0, 1, 0, 1]) == pytest.approx(2048.0 * d * d ** -0.5, rel=2.0 ** -10)
+
+
+@pytest.mark.parametrize("t,h,kv,d,win,sinks", [(70, 2, 1, 64, 2, 0), (300, 4, 2, 128, 3, 0), (200, 2, 2, 96, 2, 0)])
+def test_large_gradients_in_half(t, h, kv, d, win, sinks):
+    gen = _gen("large", t)
+    q, k = _randn(gen, 1, t, h, d, dtype=HALF, scale=0.25), _randn(gen, 1, t, kv, d, dtype=HALF, scale=0.25)
+    v, dy = _randn(gen, 1, t, kv, d, dtype=HALF), _randn(gen, 1, t, h, d, dtype=HALF, scale=10000.0)
+    _gradients(q, k, v, dy, win, sinks)
