@@ -90,4 +90,6 @@ def cache_append(qkv, k_pages, v_pages, tables, lengths, offsets, freqs, interle
         *v_pages.stride()[:3], tables.data_ptr(), tables.stride(0), lengths.data_ptr(), nv.addr(offsets), turns, pairs, magnitude,
         interleaved, n, tables.shape[0], tables.shape[1], k_pages.shape[1], k_pages.shape[0], q_heads, kv_heads, d, nv.stream()),
         "fbam_cache_append")
+    # written through pointers: a backward that saved the pages has to see it, as it sees the definition's stores
+    torch.autograd.graph.increment_version((k_pages, v_pages))
     return q

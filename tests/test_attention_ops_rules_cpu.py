@@ -1,0 +1,64 @@
+"""Rotary positions, windowed attention and the paged cache without a GPU: what each call promises beyond ordinary inputs."""
+import pytest
+import torch
+
+from fbamtrain_b200 import ops
+
+BF = torch.bfloat16
+I32 = torch.int32
+
+
+class Library:
+    """Takes the place of the kernels: every entry succeeds and does nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, entry):
+        return lambda *args: self.calls.append((entry, args)) or 0
+
+
+@pytest.fixture
+def library(monkeypatch):
+    from fbamtrain_b200.ops import native
+    fake = Library()
+    monkeypatch.setattr(native, "lib", lambda like=None: fake)
+    monkeypatch.setattr(native, "stream", lambda: 0)
+    monkeypatch.setattr(native, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    return fake
+
+
+def _small_cache(dtype=torch.float32):
+    k, v = torch.randn(3, 8, 1, 64).to(dtype), torch.randn(3, 8, 1, 64).to(dtype)
+    return k, v, torch.tensor([[0, 1]], dtype=I32), torch.tensor([5], dtype=I32)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# writes into the pages
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["definition", "kernels"])
+@pytest.mark.parametrize("page", [0, 1])
+def test_append_is_seen_by_a_backward_that_saved_the_pages(which, page, library):
+    cache = _small_cache(BF)
+    weight = torch.ones(64, dtype=BF, requires_grad=True)
+    loss = (cache[page] * weight).sum()                                 # saves the pages
+    qkv = torch.randn(1, 4, 64).to(BF)
+    if which == "definition":
+        ops.cache_append(qkv, *cache)
+    else:
+        from fbamtrain_b200.ops.positions import cache_append
+        cache_append(qkv, *cache, None, None, False, 2, 1)
+        assert [entry for entry, _ in library.calls] == ["fbam_cache_append"]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_append_to_pages_that_count_no_versions(library):
+    """Pages of inference mode, as a cache that is made there has them."""
+    from fbamtrain_b200.ops.positions import cache_append
+    with torch.inference_mode():
+        cache_append(torch.randn(1, 4, 64).to(BF), *_small_cache(BF), None, None, False, 2, 1)
+        ops.cache_append(torch.randn(1, 4, 64).to(BF), *_small_cache(BF))
+    cache = _small_cache(BF)
+    with torch.inference_mode():
+        cache_append(torch.randn(1, 4, 64).to(BF), *cache, None, None, False, 2, 1)

@@ -56,3 +56,23 @@ def test_large_gradients_in_half(t, h, kv, d, win, sinks):
     q, k = _randn(gen, 1, t, h, d, dtype=HALF, scale=0.25), _randn(gen, 1, t, kv, d, dtype=HALF, scale=0.25)
     v, dy = _randn(gen, 1, t, kv, d, dtype=HALF), _randn(gen, 1, t, h, d, dtype=HALF, scale=10000.0)
     _gradients(q, k, v, dy, win, sinks)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# the paged cache
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("page", [0, 1])
+@pytest.mark.parametrize("backend", ["auto", "torch"])
+def test_append_is_seen_by_a_backward_that_saved_the_pages(page, backend):
+    gen = _gen("versions")
+    cache = (_randn(gen, 3, 8, 1, 64), _randn(gen, 3, 8, 1, 64), torch.tensor([[0, 1]], dtype=I32, device="cuda"),
+             torch.tensor([5], dtype=I32, device="cuda"))
+    weight = torch.ones(64, dtype=BF, device="cuda", requires_grad=True)
+    loss = (cache[page] * weight).sum()
+    ops.set_backend(backend)
+    try:
+        ops.cache_append(_randn(gen, 1, 4, 64), *cache)
+    finally:
+        ops.set_backend("auto")
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
