@@ -631,47 +631,44 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         fetch(sL + ((i + 1) & 1) * 128);
       }
     }
-    // dV (part 0) and dK (part 1) of this key block
-    if (ok && mbar_wait(dk_done, (n - 1) & 1)) {
-      fence_after_sync();
-      const uint32_t src = part == 0 ? tm_dv : tm_dk;
-      if (last_part > 0) {
-        float4* to = p.kv_parts + (slot_of(p, bh, kb, part_at) * 2 + part) * (D / 4) * kKeys + row;
+    // dV (part 0) and dK (part 1) of this key block.  A wait may expire in some of a part's four warps only: they meet all the same.
+    ok = ok && mbar_wait(dk_done, (n - 1) & 1);
+    fence_after_sync();
+    const uint32_t src = part == 0 ? tm_dv : tm_dk;
+    if (last_part > 0) {
+      float4* to = p.kv_parts + (slot_of(p, bh, kb, part_at) * 2 + part) * (D / 4) * kKeys + row;
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32(src + lane_addr + c0, r);
-          tmem_ld_wait();
-          store_part<kKeys>(to + c0 / 4 * kKeys, r);
-        }
-      } else {
-        // through the stages of Q, which nothing reads any more, and out by the copy engine: as rows from registers they took 4 400
-        // (D = 64) to 9 000 cycles of every thread block
-        uint8_t* tile = sQ + part * kTile;
-#pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32(src + lane_addr + c0, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            __align__(16) elem2_t hh[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j * 8 + 2 * q]), __uint_as_float(r[j * 8 + 2 * q + 1]));
-            *reinterpret_cast<uint4*>(tile + c0 / 64 * 128 * 128 + swz(row, c0 % 64 / 8 + j)) = *reinterpret_cast<uint4*>(hh);
-          }
-        }
-        fence_proxy_async_smem();
-        if (part == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");   // four warps
-        if (lane_group == 0 && elect_one()) {
-#pragma unroll
-          for (int j = 0; j < DP; ++j) tma_store_4d(part == 0 ? &map_dv : &map_dk, tile + j * 128 * 128, j * 64, kvh, k0, b);   // rows behind T are cut
-          bulk_commit_group();
-          bulk_wait_group_read<0>();
-        }
+      for (int c0 = 0; ok && c0 < D; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32(src + lane_addr + c0, r);
+        tmem_ld_wait();
+        store_part<kKeys>(to + c0 / 4 * kKeys, r);
       }
     } else {
-      ok = false;
+      // through the stages of Q, which nothing reads any more, and out by the copy engine: as rows from registers they took 4 400
+      // (D = 64) to 9 000 cycles of every thread block
+      uint8_t* tile = sQ + part * kTile;
+#pragma unroll 1
+      for (int c0 = 0; ok && c0 < D; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32(src + lane_addr + c0, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __align__(16) elem2_t hh[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) hh[q] = ff2e2(__uint_as_float(r[j * 8 + 2 * q]), __uint_as_float(r[j * 8 + 2 * q + 1]));
+          *reinterpret_cast<uint4*>(tile + c0 / 64 * 128 * 128 + swz(row, c0 % 64 / 8 + j)) = *reinterpret_cast<uint4*>(hh);
+        }
+      }
+      fence_proxy_async_smem();
+      if (part == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");   // four warps
+      if (ok && lane_group == 0 && elect_one()) {
+#pragma unroll
+        for (int j = 0; j < DP; ++j) tma_store_4d(part == 0 ? &map_dv : &map_dk, tile + j * 128 * 128, j * 64, kvh, k0, b);   // rows behind T are cut
+        bulk_commit_group();
+        bulk_wait_group_read<0>();
+      }
     }
     if (!ok && lane == 0) atomicExch(p.status, ATT_ERR_TIMEOUT);
   } else {

@@ -1,7 +1,11 @@
 """Rotary positions, windowed attention and the paged cache without a GPU: what each call promises beyond ordinary inputs."""
+import os
+import re
+
 import pytest
 import torch
 
+import fbamtrain_b200
 from fbamtrain_b200 import ops
 
 BF = torch.bfloat16
@@ -62,3 +66,36 @@ def test_append_to_pages_that_count_no_versions(library):
     cache = _small_cache(BF)
     with torch.inference_mode():
         cache_append(torch.randn(1, 4, 64).to(BF), *cache, None, None, False, 2, 1)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# waits that run out
+# ------------------------------------------------------------------------------------------------------------------
+def _meetings(source):
+    """Of each named barrier in CUDA source: the headers of the blocks around it and the start of its own statement."""
+    code = re.sub(r"//[^\n]*", "", source)
+    code = re.sub(r"^\s*#[^\n]*", "", code, flags=re.M)
+    around, start, out, nested = [], 0, [], 0
+    for i, c in enumerate(code):
+        if code.startswith('"bar.sync', i):
+            out.append(around + [code[start:i]])
+        nested += (c == "(") - (c == ")")
+        if c == "{" and nested == 0:
+            around.append(code[start:i])
+        elif c == "}" and nested == 0:
+            around.pop()
+        if c in "{};" and nested == 0:
+            start = i + 1
+    assert not around
+    return out
+
+
+def test_warps_meet_whether_or_not_a_wait_of_theirs_expired():
+    """Warps that meet at a named barrier each have waited for themselves: one whose wait ran out has to come as well."""
+    for name in ("window_attention.cu", "window_attention_bwd.cu"):
+        with open(os.path.join(os.path.dirname(fbamtrain_b200.__file__), "csrc", name)) as f:
+            found = _meetings(f.read())
+        assert len(found) == 2
+        for around in found:
+            conditions = [h for h in around if re.search(r"\b(if|for|while)\b", h)]
+            assert conditions and not any(re.search(r"\bok\b|mbar_wait", h) for h in conditions), conditions
