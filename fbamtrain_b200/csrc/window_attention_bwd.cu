@@ -798,7 +798,7 @@ Plan make_plan(long long B, long long T, long long kv_heads, int group, int D, i
   const long long walk = a.tiles < reach ? a.tiles : reach;
   const long long steps = (((long long)a.blocks - a.firsts) * walk + (long long)a.firsts * a.tiles) * B * kv_heads / 148;
   auto divide = [](long long longest, long long share, int& parts, int& tiles) {
-    tiles = (int)(share < 8 ? 8 : share);
+    tiles = (int)(share < 8 ? 8 : share < longest ? share : longest);
     parts = (int)((longest + tiles - 1) / tiles);
   };
   divide(walk, steps / 2, a.parts, a.part_tiles);

@@ -99,3 +99,20 @@ def test_warps_meet_whether_or_not_a_wait_of_theirs_expired():
         for around in found:
             conditions = [h for h in around if re.search(r"\b(if|for|while)\b", h)]
             assert conditions and not any(re.search(r"\bok\b|mbar_wait", h) for h in conditions), conditions
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# plans
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t,kv,group", [(13_400_064, 232, 1), (11_783_936, 150, 2), (51_025_920, 4, 4), (2_000_000, 1, 1)])
+def test_workspace_of_walks_beyond_an_integer(t, kv, group):
+    """Where a multiprocessor has more tiles to do than an int holds, walks are not divided: the workspace is dQ's sums, counters and
+    delta only.  Where they are divided, by what one has to do."""
+    from fbamtrain_b200.ops import native
+    rows = 128 // group
+    tiles, blocks = -(-t // rows), -(-t // 128)
+    got = native.lib().fbam_window_bwd_workspace(1, t, kv, group, 64, 0, 0)
+    least = kv * tiles * 128 * 64 + (kv * tiles + 1 + 3) // 4 * 4 + kv * tiles * 128
+    parts = blocks * kv * 2 * 128 * 64
+    share = blocks * tiles * kv // 296
+    assert got == least + (0 if share >= tiles else -(-tiles // share) * parts)
