@@ -58,20 +58,24 @@ struct FwdParams {
 };
 
 // TILES = 2: two tiles a thread block, one thread block a multiprocessor: they share each key block.
-// TILES = 1: one tile a thread block, two thread blocks a multiprocessor, where all of them fit at once (296).  One tile and two: 3 x 696
-// with a window of 2, 8 heads of 64 8.8 and 10.9 us, of 128 10.7 and 12.4; 2 x 900, window 300, 8 over 4 heads of 64 10.6 and 12.6, of 128
-// 13.1 and 14.6; 8 x 1024, window 256, 16 heads of 64, where they do not fit, 59 and 43.  Over a cache heads of 128 have no room for a
-// page's way (two slots): 145 new tokens of ten sequences over 900, 8 over 4 heads of 64 16.6 and 19.6, of 128 26 and 23, which stay with
-// two tiles.
+// TILES = 1: one tile a thread block, two thread blocks a multiprocessor, where all of them fit at once (296).  One tile and two, heads of
+// 64: 3 x 696 with a window of 2, 8 heads, 8.8 and 10.9 us; 150 tiles, window 256, 11.2 and 13.7, no window 26.6 and 33.2; 296 tiles 14.0 and
+// 15.1, 18.6 and 22.5; 8 x 1024, window 256, 16 heads, where they do not fit, 59 and 43.  Heads of 128: 150 tiles 13.7 and 16.1, 33.4 and
+// 32.7; 296 tiles 17.1 and 18.4, 24.2 and 24.8.  (With six slots of 64 channels a multiprocessor took one of them: 20.5 us for 296 tiles,
+// window 256.)  Over a cache heads of 128 have no room for a page's way (two slots): 145 new tokens of ten sequences over 900, 16 over 8
+// heads of 64 22.1 and 37.3, 8 over 4 of 128 26 and 23, which stay with two tiles.
 // ONE: that tile is one token with up to 16 heads.  It has little to do for each key block that arrives, and two of them hide each
 // other's waits.  Its Q keeps 16 rows a panel; what the product reads behind them are other buffers, in rows that nobody looks at.
 constexpr int kResident = 296;
 template <int D, int TILES, bool ONE>
-constexpr int kSlots = TILES == 2 ? (D == 64 ? 8 : 5) : (D == 64 ? 6 : ONE ? 3 : 2);
+constexpr int kSlots = TILES == 2 ? (D == 64 ? 8 : 5) : (D == 64 ? (ONE ? 6 : 5) : ONE ? 3 : 2);
 template <bool ONE>
 constexpr int kQPanel = ONE ? 16 * 128 : kRows * 128;              // bytes of 64 channels of a tile
 template <int D, int TILES, bool ONE>
 constexpr int fwd_smem_bytes() { return TILES * (D / 64) * kQPanel<ONE> + kSlots<D, TILES, ONE> * kKeys * D * 2 + 256 + 1024; }
+// of a multiprocessor, which takes 1 KB for itself with each thread block
+template <int D, int TILES, bool ONE>
+constexpr bool kAllFit = (TILES == 2 ? 1 : 2) * (fwd_smem_bytes<D, TILES, ONE>() + 1024) <= 228 * 1024;
 // STEP: keys whose scores a softmax thread has at a time.  64: the next 64 are scored meanwhile, beside them, and less is scored that
 // the masks take away.  128: a product of 128 keys reads Q half as often, but the tensor memory has no room to score ahead; P V starts
 // with the first 96 keys.  With heads of 128 the products count where the keys are many: 4 x 4096, 16 over 4 heads of 128, STEP 64 and
@@ -644,6 +648,7 @@ template <int D, bool PAGED, int TILES, bool ONE, int STEP>
 int launch(dim3 grid, cudaStream_t s, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& out, const CUtensorMap& low,
            const FwdParams& p) {
   constexpr int smem = fwd_smem_bytes<D, TILES, ONE>();
+  static_assert(kAllFit<D, TILES, ONE>, "as many thread blocks a multiprocessor as the launch bounds say");
   if (set_smem_once<window_fwd_kernel<D, PAGED, TILES, ONE, STEP>>(smem)) return 5;
   window_fwd_kernel<D, PAGED, TILES, ONE, STEP><<<grid, kFwdThreads<TILES, STEP>, smem, s>>>(q, k, v, out, low, p);
   return 0;

@@ -76,3 +76,34 @@ def test_append_is_seen_by_a_backward_that_saved_the_pages(page, backend):
         ops.set_backend("auto")
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# one tile a thread block, two thread blocks a multiprocessor
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t,h,win,sinks", [(1300, 14, None, 0), (1100, 32, 700, 130), (640, 59, 64, 0)])
+@pytest.mark.parametrize("dtype", [BF, HALF])
+def test_as_many_tiles_as_thread_blocks_fit(t, h, win, sinks, dtype):
+    """150 to 296 tiles of heads of 64, whose ring of keys goes round more than once."""
+    assert 149 <= -(-t // 128) * h <= 296
+    gen = _gen("tiles", t)
+    _gradients(*(_randn(gen, 1, t, h, 64, dtype=dtype) for _ in range(4)), win, sinks)
+
+
+def _cache(gen, lengths, slots, kv, d, dtype=BF):
+    per = [-(-n // slots) for n in lengths]
+    tables = torch.full((len(lengths), max(per)), -1, dtype=I32, device="cuda")
+    order, at = torch.randperm(sum(per), generator=gen, device="cuda").to(I32), 0
+    for b, n in enumerate(per):
+        tables[b, :n] = order[at:at + n]
+        at += n
+    return (*(_randn(gen, sum(per), slots, kv, d, dtype=dtype) for _ in range(2)), tables, torch.tensor(lengths, dtype=I32, device="cuda"))
+
+
+@pytest.mark.parametrize("win,sinks", [(None, 0), (100, 20)])
+def test_as_many_tiles_over_a_cache_as_thread_blocks_fit(win, sinks):
+    gen = _gen("cached tiles")
+    cache = _cache(gen, [900] * 10, 16, 8, 64)
+    q, offsets = _randn(gen, 1450, 16, 64), (torch.arange(11, device="cuda") * 145).to(I32)
+    oracle.within(ops.cache_attention(q, *cache, offsets, win, sinks), *oracle.cached(q, *cache, offsets, win, sinks))
+    nv.check_status(q.device)
