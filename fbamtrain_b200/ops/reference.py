@@ -221,13 +221,13 @@ def _attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, at: torch.Tensor,
     kv, like = k.shape[1], q
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     j = torch.arange(k.shape[0], device=q.device)
-    there = (j < end).view(-1, 1, 1)
-    # what lies behind the end can hold anything
-    q = torch.where((at < end).view(-1, 1, 1), q.to(wide), 0.0)
-    k, v = torch.where(there, k.to(wide), 0.0), torch.where(there, v.to(wide), 0.0)
     seen = (j <= at.unsqueeze(1)) & (j < end) & (at.unsqueeze(1) < end)
     if window is not None:
         seen = seen & ((at.unsqueeze(1) - j < window) | (j < sinks))
+    # what lies behind the end, and keys and values that no query sees, can hold anything
+    q = torch.where((at < end).view(-1, 1, 1), q.to(wide), 0.0)
+    some = seen.any(0).view(-1, 1, 1)
+    k, v = torch.where(some, k.to(wide), 0.0), torch.where(some, v.to(wide), 0.0)
     s = torch.einsum("ngrd,mgd->grnm", q.reshape(n, kv, h // kv, d), k) * d ** -0.5
     nothing = ~seen.any(1)
     s = s.masked_fill(~seen & ~nothing.unsqueeze(1), float("-inf"))

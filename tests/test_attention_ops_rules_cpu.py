@@ -1,10 +1,12 @@
 """Rotary positions, windowed attention and the paged cache without a GPU: what each call promises beyond ordinary inputs."""
+import math
 import os
 import re
 
 import pytest
 import torch
 
+import attention_oracle as oracle
 import fbamtrain_b200
 from fbamtrain_b200 import ops
 
@@ -66,6 +68,24 @@ def test_append_to_pages_that_count_no_versions(library):
     cache = _small_cache(BF)
     with torch.inference_mode():
         cache_append(torch.randn(1, 4, 64).to(BF), *cache, None, None, False, 2, 1)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# slots that nobody sees
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,win,sinks", [(1, 10, 0), (1, 10, 5), (7, 10, 5), (20, 30, 17), (60, 3, 1), (3, None, 0)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_the_definition_of_cache_attention_reads_what_queries_see(new, win, sinks, value):
+    """Slots between the first tokens and the window, and behind the sequence, of pages that are still in the table."""
+    gen = torch.Generator().manual_seed(1)
+    k, v = torch.randn(10, 8, 2, 6, generator=gen), torch.randn(10, 8, 2, 6, generator=gen)
+    tables, lengths = torch.tensor([[3, 7, 1, 0, 9, 5, 2, 8]], dtype=I32), torch.tensor([60], dtype=I32)
+    offsets, q = torch.tensor([0, new], dtype=I32), torch.randn(new, 4, 6, generator=gen)
+    for j in range(64):
+        if j >= 60 or (win is not None and sinks <= j <= 60 - new - win):
+            k[tables[0, j // 8], j % 8] = v[tables[0, j // 8], j % 8] = value
+    y = ops.cache_attention(q, k, v, tables, lengths, offsets, win, sinks)
+    oracle.within(y, *oracle.cached(q, k, v, tables, lengths, offsets, win, sinks))
 
 
 # ------------------------------------------------------------------------------------------------------------------
