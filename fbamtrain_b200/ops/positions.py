@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple, Optional, Tuple
 
@@ -10,14 +11,22 @@ import torch
 from . import native as nv
 from .derivatives import first_only, tracked
 
-MAX_PAIRS = 128
 
-
-class RotaryFrequencies(NamedTuple):
-    """How far each pair of channels turns a position: fractions of a turn, times 2^64, and the factor on what is turned."""
+class _Frequencies(NamedTuple):
     turns: Tuple[int, ...]
     magnitude: float
-    table: C.Array                                      # ``turns`` as the kernels take them
+
+
+class RotaryFrequencies(_Frequencies):
+    """How far each pair of channels turns a position: fractions of a turn, times 2^64, and the factor on what is turned."""
+
+    @functools.cached_property
+    def table(self) -> C.Array:
+        """``turns`` as the kernels take them."""
+        return (C.c_ulonglong * max(1, len(self.turns)))(*self.turns)
+
+    def __reduce__(self):
+        return type(self), tuple(self)                  # without the table, which has no pickled form
 
     @property
     def dims(self) -> int:
@@ -37,7 +46,7 @@ def rotary_frequencies(dims: int, base: float, factor: float, context: Optional[
         turns.append(round(math.ldexp(theta / (2.0 * math.pi), 64)) % 2 ** 64)
     if factor > 1.0 and context is not None:
         magnitude = 1.0 + 0.1 * math.log(factor)
-    return RotaryFrequencies(tuple(turns), magnitude, (C.c_ulonglong * max(1, len(turns)))(*turns))
+    return RotaryFrequencies(tuple(turns), magnitude)
 
 
 def _turned(x, positions, freqs, heads, interleaved, inverse):

@@ -1,6 +1,9 @@
 """Rotary positions, windowed attention and the paged cache without a GPU: what each call promises beyond ordinary inputs."""
+import copy
+import io
 import math
 import os
+import pickle
 import re
 
 import pytest
@@ -86,6 +89,25 @@ def test_the_definition_of_cache_attention_reads_what_queries_see(new, win, sink
             k[tables[0, j // 8], j % 8] = v[tables[0, j // 8], j % 8] = value
     y = ops.cache_attention(q, k, v, tables, lengths, offsets, win, sinks)
     oracle.within(y, *oracle.cached(q, k, v, tables, lengths, offsets, win, sinks))
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# frequencies
+# ------------------------------------------------------------------------------------------------------------------
+def test_frequencies_and_a_model_that_has_them_are_pickled():
+    from fbamtrain_b200.models import AttentionDecoder
+    from fbamtrain_b200.models.init_utils import SeedSequence
+    freqs = ops.rotary_frequencies(64, factor=4.0, context=100)
+    for _ in range(2):
+        for other in (pickle.loads(pickle.dumps(freqs)), copy.deepcopy(freqs)):
+            assert other == freqs and other.dims == 64 and list(other.table) == list(freqs.turns)      # from here on with a table of its own
+    model = AttentionDecoder(frame_dim=8, dim=32, layers=1, heads=2, inner=16, vocab=5, dtype=torch.float32, seeds=SeedSequence(1))
+    file = io.BytesIO()
+    torch.save(model, file)
+    file.seek(0)
+    other = torch.load(file, weights_only=False)
+    args = torch.randn(1, 4, 8), torch.tensor([[-1, 2, 3, 1]]), torch.tensor([[2, 3, 1, 0]])
+    assert other.freqs == model.freqs and torch.equal(other(*args).logprob, model(*args).logprob)
 
 
 # ------------------------------------------------------------------------------------------------------------------
