@@ -6,8 +6,9 @@
 // behind them, and the heads behind the first `turned`, is copied.  The gradient is the same pass with −φ.
 //
 // Angles.  At position 10^6 an fp32 product position · θ is off by 0.03 of a radian.  A frequency is therefore kept as a 64-bit
-// fraction of a TURN a position: the product with the position modulo 2^64 is exact, what it drops are whole turns, and its top 32
-// bits are the angle to 2^-32 of a turn.  sin and cos are formed once for a (token, pair) and shared by all heads of the token.
+// fraction of a TURN a position: the product with the position modulo 2^64 is exact, and what it drops are whole turns.  Its top 32
+// bits go to sin and cos as fp32, which rounds them by up to 2^-26 of a turn, and the frequency's own rounding, 2^-65 of a turn, counts
+// once for every position.  sin and cos are formed once for a (token, pair) and shared by all heads of the token.
 //
 // The append form is the same pass of a serving step: the heads of new tokens come as (tokens, query + key + value heads, D);
 // turned queries go to a tensor, turned keys and the values into the pages of a cache.

@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+from decimal import Decimal, localcontext
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -33,19 +34,23 @@ class RotaryFrequencies(_Frequencies):
         return 2 * len(self.turns)
 
 
+_TWO_PI = 2 * Decimal("3.14159265358979323846264338327950288419716939937510")
+
+
 def rotary_frequencies(dims: int, base: float, factor: float, context: Optional[int], few: float, many: float) -> RotaryFrequencies:
-    turns, magnitude = [], 1.0
-    for i in range(dims // 2):
-        theta = base ** (-2.0 * i / dims)
-        if factor != 1.0:
-            kept = 0.0
-            if context is not None:
-                around = context * theta / (2.0 * math.pi)
-                kept = min(1.0, max(0.0, (around - few) / (many - few)))
-            theta *= kept + (1.0 - kept) / factor
-        turns.append(round(math.ldexp(theta / (2.0 * math.pi), 64)) % 2 ** 64)
-    if factor > 1.0 and context is not None:
-        magnitude = 1.0 + 0.1 * math.log(factor)
+    # in 50 digits: with the 53 bits of a double the last ones of a fraction of 64, which far positions bring up, would be anything
+    with localcontext(prec=50):
+        log_base, slower, least, most = Decimal(float(base)).ln(), Decimal(float(factor)), Decimal(float(few)), Decimal(float(many))
+        turns = []
+        for i in range(dims // 2):
+            turn = (log_base * (-2 * i) / dims).exp() / _TWO_PI
+            if factor != 1.0:
+                kept = Decimal(0)
+                if context is not None:
+                    kept = min(Decimal(1), max(Decimal(0), (context * turn - least) / (most - least)))
+                turn *= kept + (1 - kept) / slower
+            turns.append(int((turn * 2 ** 64).to_integral_value()) % 2 ** 64)
+    magnitude = 1.0 + 0.1 * math.log(factor) if factor > 1.0 and context is not None else 1.0
     return RotaryFrequencies(tuple(turns), magnitude)
 
 

@@ -197,10 +197,11 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], top: i
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, freqs, heads: int, interleaved: bool) -> torch.Tensor:
     """``x`` ``(B, T, H, D)``: the pairs of the first ``2 len(freqs.turns)`` channels of the first ``heads`` heads turned by
-    ``positions`` (broadcast to ``(B, T)``) times the frequencies; the angles in 64 bits."""
+    ``positions`` (broadcast to ``(B, T)``) times the frequencies; whole turns fall away as multiples of 2^64 do."""
     n = 2 * len(freqs.turns)
-    theta = torch.tensor([t * (2 * math.pi / 2 ** 64) for t in freqs.turns], dtype=torch.float64, device=x.device)
-    angle = (positions.expand(x.shape[:2]).double().unsqueeze(-1) * theta).unsqueeze(2)
+    turns = torch.tensor([t - (t >> 63 << 64) for t in freqs.turns], dtype=torch.int64, device=x.device)
+    part = positions.expand(x.shape[:2]).long().unsqueeze(-1) * turns
+    angle = (part.double() * (2 * math.pi / 2 ** 64)).unsqueeze(2)
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     cos, sin = (freqs.magnitude * angle.cos()).to(wide), (freqs.magnitude * angle.sin()).to(wide)
     r = x[:, :, :heads, :n].to(wide)

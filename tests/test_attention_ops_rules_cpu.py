@@ -5,6 +5,7 @@ import math
 import os
 import pickle
 import re
+from fractions import Fraction
 
 import pytest
 import torch
@@ -108,6 +109,45 @@ def test_frequencies_and_a_model_that_has_them_are_pickled():
     other = torch.load(file, weights_only=False)
     args = torch.randn(1, 4, 8), torch.tensor([[-1, 2, 3, 1]]), torch.tensor([[2, 3, 1, 0]])
     assert other.freqs == model.freqs and torch.equal(other(*args).logprob, model(*args).logprob)
+
+
+def _speeds(dims, digits=45):
+    """Of base 10^(dims / 2), whose pairs turn by 10^-i radians a position: that in turns, exact to ``digits``."""
+    def inverse_tangent(n):                                             # of 1 / n, by its series
+        total, term, i = 0, 10 ** digits // n, 1
+        while term:
+            total += term // i if i % 4 == 1 else -(term // i)
+            term //= n * n
+            i += 2
+        return total
+    pi = 4 * (4 * inverse_tangent(5) - inverse_tangent(239))            # Machin's formula
+    return [Fraction(10 ** digits, 2 * pi * 10 ** i) for i in range(dims // 2)]
+
+
+@pytest.mark.parametrize("settings", [{}, {"factor": 4.0}, {"factor": 8.0, "context": 512}, {"factor": 5.0, "context": 3000, "few": 2.0, "many": 40.0}])
+def test_frequencies_fill_their_64_bits(settings):
+    freqs = ops.rotary_frequencies(8, base=10000.0, **settings)
+    for got, turn in zip(freqs.turns, _speeds(8)):
+        factor = Fraction(settings.get("factor", 1))
+        if "context" in settings:
+            few, many = Fraction(settings.get("few", 1)), Fraction(settings.get("many", 32))
+            kept = min(Fraction(1), max(Fraction(0), (turn * settings["context"] - few) / (many - few)))
+            turn *= kept + (1 - kept) / factor
+        else:
+            turn /= factor
+        assert abs(got - turn * 2 ** 64) <= Fraction(1, 2) + Fraction(1, 10 ** 9)
+
+
+def test_the_definition_of_rotary_at_far_positions():
+    """In 64 bits: the angle is off by 2^-65 of a turn a position, and by the roundings of a double."""
+    positions = [1, 2 ** 31 - 1, 10 ** 12 + 7, -(2 ** 44) - 3, 2 ** 50 + 1]
+    x = torch.tensor([[1.0] * 4 + [0.0] * 4], dtype=torch.float64).expand(1, len(positions), 1, 8)
+    y = ops.rotary(x, torch.tensor([positions]), ops.rotary_frequencies(8))
+    for n, p in enumerate(positions):
+        for i, turn in enumerate(_speeds(8)):
+            angle = 2 * math.pi * float((p * turn) % 1)
+            bound = 2 * math.pi * (abs(p) * 2.0 ** -65) + 2.0 ** -48
+            assert abs(float(y[0, n, 0, i]) - math.cos(angle)) <= bound and abs(float(y[0, n, 0, 4 + i]) - math.sin(angle)) <= bound
 
 
 # ------------------------------------------------------------------------------------------------------------------

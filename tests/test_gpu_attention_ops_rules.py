@@ -1,4 +1,5 @@
 """Rotary positions, windowed attention and the paged cache on the kernels: what each call promises beyond ordinary inputs."""
+import math
 import zlib
 
 import pytest
@@ -107,3 +108,22 @@ def test_as_many_tiles_over_a_cache_as_thread_blocks_fit(win, sinks):
     q, offsets = _randn(gen, 1450, 16, 64), (torch.arange(11, device="cuda") * 145).to(I32)
     oracle.within(ops.cache_attention(q, *cache, offsets, win, sinks), *oracle.cached(q, *cache, offsets, win, sinks))
     nv.check_status(q.device)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# rotary positions
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("width", [64, 66])
+def test_rotary_at_far_positions(width, interleaved):
+    """Whole pieces and any, against the definition of the same frequencies in 64 bits."""
+    gen = _gen("far", width)
+    positions = torch.tensor([[0, 2 ** 31 - 1, 2 ** 38 + 5, -(2 ** 40) - 3, 2 ** 48 + 1]], device="cuda")
+    freqs = ops.rotary_frequencies(64)
+    x = _randn(gen, 1, 5, 3, width, dtype=HALF)
+    want = ops.rotary(x.double(), positions, freqs, interleaved=interleaved)
+    reach = x.double().abs().amax(-1, keepdim=True) * 2
+    # the angle (32 bits of a turn, rounded to 24), its sine and cosine and three roundings in fp32, one of the result
+    angle = 2 * math.pi * (2.0 ** -26 + 2.0 ** -32)
+    bound = oracle.UNIT[HALF] * want.abs() + oracle.FLOOR[HALF] + (angle + 2.0 ** -20) * reach
+    oracle.within(ops.rotary(x, positions, freqs, interleaved=interleaved), want, bound)
