@@ -20,6 +20,14 @@ def tracked(*tensors: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def wanted(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a derivative would have to pass through a call: a tensor requires a gradient where gradients are taken, or has a
+    tangent."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _First(torch.autograd.Function):
     @staticmethod
     def forward(ctx, name, grad, *of):

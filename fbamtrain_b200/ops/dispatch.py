@@ -7,7 +7,7 @@ import torch
 
 from . import native as nv
 from . import reference as ref
-from .derivatives import tracked
+from .derivatives import wanted
 
 import os
 
@@ -462,7 +462,7 @@ def _check_cache_native(d, k_pages, v_pages) -> None:
 
 
 def _no_gradient(name, *tensors) -> None:
-    if tracked(*tensors):
+    if wanted(*tensors):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train with window_attention")
 
 

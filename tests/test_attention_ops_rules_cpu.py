@@ -74,6 +74,26 @@ def test_append_to_pages_that_count_no_versions(library):
         cache_append(torch.randn(1, 4, 64).to(BF), *cache, None, None, False, 2, 1)
 
 
+def test_the_cache_operators_beside_tangents():
+    """A level of forward differentiation is no tangent: what has none passes, what has one is refused, without gradients too."""
+    from torch.autograd import forward_ad
+    cache, q, qkv = _small_cache(), torch.randn(1, 2, 64), torch.randn(1, 4, 64)
+
+    def dual(x):
+        return forward_ad.make_dual(x, torch.ones_like(x))
+
+    want = ops.cache_attention(q, *cache)
+    with forward_ad.dual_level():
+        assert torch.equal(ops.cache_append(qkv, *(x.clone() for x in cache)), qkv[:, :2])
+        assert torch.equal(ops.cache_attention(q, *cache), want)
+        for taken in (torch.enable_grad, torch.no_grad):
+            with taken():
+                for call in (lambda: ops.cache_attention(dual(q), *cache), lambda: ops.cache_append(dual(qkv), *cache),
+                             lambda: ops.cache_attention(q, cache[0], dual(cache[1]), *cache[2:])):
+                    with pytest.raises(RuntimeError, match="no gradient"):
+                        call()
+
+
 # ------------------------------------------------------------------------------------------------------------------
 # slots that nobody sees
 # ------------------------------------------------------------------------------------------------------------------
