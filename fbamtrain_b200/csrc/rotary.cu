@@ -73,7 +73,7 @@ __device__ __forceinline__ long long append_position(const RotaryParams& p, long
     }
     b = lo;
     first = p.offsets[lo];
-    count = p.offsets[lo + 1] - first;
+    count = min((long long)p.offsets[lo + 1], p.tokens) - first;
     if (n < first || n >= first + count) return -1;
   }
   return (long long)p.lengths[b] - count + (n - first);

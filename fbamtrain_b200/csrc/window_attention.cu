@@ -140,6 +140,20 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.kv_heads * p.group;
   int b, pair, kvh, split = 0;
+  const bool partial = PAGED && p.splits > 1;
+  // rows that see nothing: zeros, or a part that adds nothing
+  auto clear = [&](long long row0, int rows) {
+    const int per = p.group * (D / 8);
+    for (int i = threadIdx.x; i < rows * per; i += kFwdThreads<TILES, STEP>) {
+      const int r = i % per;
+      const long long at = (row0 + i / per) * heads + kvh * p.group + r / (D / 8);
+      if (partial) {
+        if (r % (D / 8) == 0) p.part_ml[(long long)split * p.T * heads + at] = make_float2(-INFINITY, 0.0f);
+      } else {
+        *reinterpret_cast<uint4*>(p.out + at * D + r % (D / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  };
   if constexpr (PAGED) {
     kvh = blockIdx.y;
     split = blockIdx.z;
@@ -147,6 +161,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       b = blockIdx.x;
       pair = 0;
     } else {
+      if (blockIdx.x == 0) {             // rows in front of the first sequence: none, as a rule
+        const int front = min(p.offsets[0], p.T);
+        for (int t = 0; t < front; t += kRows) clear(t, min(kRows, front - t));
+      }
       // which sequence this block's pair of tiles belongs to; the rows behind the last sequence count as one more, without keys
       if (warp == 0) {
         int before = 0, at = -1, which = 0;
@@ -224,20 +242,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int sink_steps = (p.sinks + STEP - 1) / STEP;
   auto needed = [&](const Span& s, int step) { return step <= s.hi && (step < sink_steps || step >= s.lo); };
 
-  const bool partial = PAGED && p.splits > 1;
-  if (c0 >= c1) {                              // no keys: zeros, or a part that adds nothing
-    const int i1 = min(tok0 + TILES * p.tile_tokens, n_rows);
-    const int per = p.group * (D / 8);
-    for (int i = threadIdx.x; i < (i1 - tok0) * per; i += kFwdThreads<TILES, STEP>) {
-      const int t = tok0 + i / per, r = i % per;
-      const long long row = (PAGED ? (long long)row0 : (long long)b * p.T) + t;
-      const long long at = row * heads + kvh * p.group + r / (D / 8);
-      if (partial) {
-        if (r % (D / 8) == 0) p.part_ml[(long long)split * p.T * heads + at] = make_float2(-INFINITY, 0.0f);
-      } else {
-        *reinterpret_cast<uint4*>(p.out + at * D + r % (D / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
+  if (c0 >= c1) {                              // no keys
+    clear((PAGED ? (long long)row0 : (long long)b * p.T) + tok0, min(tok0 + TILES * p.tile_tokens, n_rows) - tok0);
     return;
   }
 

@@ -474,8 +474,8 @@ def cache_append(qkv, k_pages, v_pages, tables, lengths, offsets=None, freqs=Non
 
     The new tokens are the last ones of their sequences.  Queries and keys are turned by their positions (``freqs``, ``interleaved`` as in
     :func:`rotary`; None: as they are), keys and values are written to their slots, and the queries are returned ``(N, H, D)``.  Rows
-    behind the last offset, and tokens that would lie in front of their sequence's start, give zeros and are not written; nor is a token
-    whose entry in the table is no page.  Sequences may share pages, but no two tokens of a call a slot."""
+    in front of the first offset or behind the last, and tokens that would lie in front of their sequence's start, give zeros and are not
+    written; nor is a token whose entry in the table is no page.  Sequences may share pages, but no two tokens of a call a slot."""
     if qkv.dim() != 3 or k_pages.dim() != 4:
         raise ValueError(f"new tokens are (tokens, heads, width) and pages (pages, slots, heads, width), got {tuple(qkv.shape)} and {tuple(k_pages.shape)}")
     n, all_heads, d = qkv.shape

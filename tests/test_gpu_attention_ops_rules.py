@@ -127,3 +127,50 @@ def test_rotary_at_far_positions(width, interleaved):
     angle = 2 * math.pi * (2.0 ** -26 + 2.0 ** -32)
     bound = oracle.UNIT[HALF] * want.abs() + oracle.FLOOR[HALF] + (angle + 2.0 ** -20) * reach
     oracle.within(ops.rotary(x, positions, freqs, interleaved=interleaved), want, bound)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# rows that belong to no sequence
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lengths,new,h,kv,d", [([300, 40], [2, 5], 4, 2, 64), ([2000, 900], [1, 1], 8, 2, 128), ([700, 300], [200, 90], 6, 2, 128),
+                                                ([260], [150], 40, 8, 64)])
+@pytest.mark.parametrize("front", [1, 130, 300])
+def test_rows_of_no_sequence_are_zeros(lengths, new, h, kv, d, front):
+    """In front of the first offset and behind the last, where memory held something else."""
+    gen = _gen("rows", lengths, front)
+    cache = _cache(gen, lengths, 16, kv, d)
+    n = front + sum(new) + 3
+    q = _randn(gen, n, h, d)
+    offsets = (front + torch.tensor([0] + new, device="cuda").cumsum(0)).to(I32)
+    for win in (None, 100):
+        want = oracle.cached(q, *cache, offsets, win, 0)
+        for _ in range(3):
+            spoilt = [torch.full(s, math.nan, dtype=BF, device="cuda") for s in ((n, h, d),) * 3]
+            del spoilt
+            y = ops.cache_attention(q, *cache, offsets, win)
+            oracle.within(y, *want)
+            assert not y[:front].any() and not y[front + sum(new):].any()
+    nv.check_status(q.device)
+
+
+def test_append_of_rows_that_offsets_go_beyond():
+    """Offsets behind the last row: the rows that are there are the last ones of their sequences, as the definition has it and as the
+    attention over them takes them."""
+    gen = _gen("beyond")
+    cache, qkv = _cache(gen, [40, 30], 16, 1, 64), _randn(gen, 5, 4, 64)
+    offsets = torch.tensor([1, 3, 9], dtype=I32, device="cuda")
+    freqs = ops.rotary_frequencies(64)
+    got, want = ([x.clone() for x in cache[:2]] for _ in range(2))
+    q = ops.cache_append(qkv, *got, *cache[2:], offsets, freqs)
+    y = ops.cache_attention(q, *got, *cache[2:], offsets)
+    ops.set_backend("torch")
+    try:
+        q_want = ops.cache_append(qkv, *want, *cache[2:], offsets, freqs)
+    finally:
+        ops.set_backend("auto")
+    for a, b in ((q, q_want), *zip(got, want)):        # one rounding each, of fp32 values that are 2^-20 of terms of size 8 apart
+        assert bool(((a.double() - b.double()).abs() <= 2 * oracle.UNIT[BF] * b.double().abs() + 2.0 ** -16).all())
+    for a, b, c in zip(got, want, cache):
+        assert torch.equal((a != c).any(-1), (b != c).any(-1))         # the same slots
+    oracle.within(y, *oracle.cached(q, *got, *cache[2:], offsets.clamp(max=5), None, 0))
+    assert not y[0].any() and not q[0].any()
