@@ -13,6 +13,7 @@ import torch
 from torch import nn
 
 from .. import ops
+from ..ops.dispatch import CACHE_WIDTHS, runs_native
 from .blocks import GatedMlp, Linear, RmsNorm, TokenEmbedding
 from .init_utils import SeedSequence, fill_uniform_fan_
 
@@ -121,7 +122,9 @@ class WindowBlock(nn.Module):
 class AttentionDecoder(nn.Module):
     """``frames (B, T, E)``: one vector per frame, as the frame head gives them; ``previous (B, T)``: the action taken before
     each frame, any id outside the vocabulary where there was none.  ``factor`` and ``context`` scale the positions for recordings
-    longer than those that the model was trained on (:func:`~fbamtrain_b200.ops.rotary_frequencies`)."""
+    longer than those that the model was trained on (:func:`~fbamtrain_b200.ops.rotary_frequencies`).
+
+    ``forward`` takes heads of any width.  The cache, on a GPU in 16 bits, takes heads of 64 or 128 channels: ``make_cache`` refuses others."""
 
     def __init__(self, frame_dim: int, dim: int, layers: int, heads: int, inner: int, vocab: int, dtype: torch.dtype, seeds: SeedSequence,
                  kv_heads: Optional[int] = None, window: Optional[int] = None, sinks: int = 0, bias: bool = True, eps: float = 1e-5,
@@ -162,12 +165,15 @@ class AttentionDecoder(nn.Module):
         """A cache for ``sequences`` recordings of up to ``most_tokens`` frames.  Without ``pages`` the pool holds all that they can need
         with single steps: with a window, of each the pages of the first tokens and of the window."""
         weight = self.head_weight
+        width = weight.shape[1] // self.heads
+        if width not in CACHE_WIDTHS and runs_native(weight, "mha"):
+            raise ValueError(f"the kernels keep heads of {' or '.join(map(str, CACHE_WIDTHS))} channels in a cache, this model's have {width}")
         if pages is None:
             each = -(-most_tokens // slots)
             if self.window is not None:
                 each = min(each, -(-self.sinks // slots) + -(-self.window // slots) + 1)
             pages = sequences * each
-        return PagedCache(len(self.block), pages, slots, self.kv_heads, weight.shape[1] // self.heads, sequences, most_tokens, weight.dtype,
+        return PagedCache(len(self.block), pages, slots, self.kv_heads, width, sequences, most_tokens, weight.dtype,
                           weight.device, self.window, self.sinks)
 
     @torch.no_grad()

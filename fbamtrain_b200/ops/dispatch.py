@@ -63,6 +63,11 @@ def _native(t: torch.Tensor, dtype: Optional[torch.dtype] = None, family: Option
     return use
 
 
+def runs_native(t: torch.Tensor, family: str) -> bool:
+    """Whether a call of the family on tensors like ``t`` runs on the kernels."""
+    return _native_inner(t, None, family)
+
+
 def _native_inner(t: torch.Tensor, dtype: Optional[torch.dtype], family: Optional[str]) -> bool:
     if not (t.is_cuda and _BACKEND == "auto"):
         return False
@@ -449,10 +454,13 @@ def _check_cache(n, kv_heads, d, dtype, device, k_pages, v_pages, tables, length
                 raise ValueError(f"{name} are on {x.device}, the tokens on {device}")
 
 
+CACHE_WIDTHS = (64, 128)
+
+
 def _check_cache_native(d, k_pages, v_pages) -> None:
     """What the kernels want of a cache beyond what the definition does: a call cannot lay pages out anew."""
-    if d not in (64, 128):
-        raise ValueError(f"the kernels keep heads of 64 or 128 channels in a cache, got {d}")
+    if d not in CACHE_WIDTHS:
+        raise ValueError(f"the kernels keep heads of {' or '.join(map(str, CACHE_WIDTHS))} channels in a cache, got {d}")
     if k_pages.shape[1] % 8:
         raise ValueError(f"pages have a multiple of 8 slots, got {k_pages.shape[1]}")
     for x in (k_pages, v_pages):

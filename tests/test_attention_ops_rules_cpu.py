@@ -218,3 +218,27 @@ def test_workspace_of_walks_beyond_an_integer(t, kv, group):
     parts = blocks * kv * 2 * 128 * 64
     share = blocks * tiles * kv // 296
     assert got == least + (0 if share >= tiles else -(-tiles // share) * parts)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# the decoder
+# ------------------------------------------------------------------------------------------------------------------
+def _decoder(heads=4, dim=256, **how):
+    from fbamtrain_b200.models import AttentionDecoder
+    from fbamtrain_b200.models.init_utils import SeedSequence
+    how = {"layers": 2, "kv_heads": 2, "window": 9, "sinks": 2, **how}
+    return AttentionDecoder(frame_dim=24, dim=dim, heads=heads, inner=32, vocab=37, dtype=torch.float32, seeds=SeedSequence(3), **how)
+
+
+@pytest.mark.parametrize("heads,dim,fits", [(4, 256, True), (2, 256, True), (4, 384, False), (4, 128, False)])
+def test_a_cache_that_the_kernels_do_not_take_is_refused_when_it_is_made(heads, dim, fits, monkeypatch):
+    """64 and 128 channels a head; 96 and 32, which train."""
+    from fbamtrain_b200.ops import dispatch
+    model = _decoder(heads, dim)
+    assert model.make_cache(2, 50).k.shape[-1] == dim // heads              # the definitions take any
+    monkeypatch.setattr(dispatch, "_native_inner", lambda t, dtype, family: True)
+    if fits:
+        model.make_cache(2, 50)
+    else:
+        with pytest.raises(ValueError, match="64 or 128"):
+            model.make_cache(2, 50)
