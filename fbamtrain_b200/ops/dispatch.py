@@ -397,8 +397,9 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, leng
     sees key ``j`` where ``j <= i`` and ``i - j < window`` or ``j < sinks``; scores are scaled by ``D ** -0.5``.
 
     ``lengths`` ``(B,)``: tokens of each sequence of a padded batch.  What lies behind them may hold anything, gives zeros and has
-    zero gradients.  Values within the sequences are finite.  Results and gradients do not vary from run to run.  Heads of up to
-    128 channels run on the kernels (as 64 or 128); wider ones take the PyTorch definition."""
+    zero gradients.  Values within the sequences are finite: one that is not shows, as 0 x inf, in rows that do not see it as well.
+    Results and gradients do not vary from run to run.  Heads of up to 128 channels run on the kernels (as 64 or 128); wider ones take
+    the PyTorch definition."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.shape[3] == 0:
         raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not go together")
     if not q.dtype == k.dtype == v.dtype:
@@ -506,10 +507,10 @@ def cache_append(qkv, k_pages, v_pages, tables, lengths, offsets=None, freqs=Non
 
 def cache_attention(q, k_pages, v_pages, tables, lengths, offsets=None, window: Optional[int] = None, sinks: int = 0):
     """Attention of new tokens ``q`` ``(N, H, D)`` over a paged cache that holds them already (arguments as in
-    :func:`cache_append`, mask as in :func:`window_attention`) → ``(N, H, D)``.  Slots that no query of a sequence sees may hold
-    anything and their pages may be gone from the table (-1) or belong to others; an entry that is no page where a query does see it
-    counts as keys and values of zero.  Rows of no sequence, or in front of one's start, give zeros.  Keys behind the table's width do
-    not exist."""
+    :func:`cache_append`, mask as in :func:`window_attention`) → ``(N, H, D)``.  Values that some query sees are finite, as
+    there.  Slots that no query of a sequence sees may hold anything and their pages may be gone from the table (-1) or belong to others;
+    an entry that is no page where a query does see it counts as keys and values of zero.  Rows of no sequence, or in front of one's
+    start, give zeros.  Keys behind the table's width do not exist."""
     if q.dim() != 3 or k_pages.dim() != 4:
         raise ValueError(f"new tokens are (tokens, heads, width) and pages (pages, slots, heads, width), got {tuple(q.shape)} and {tuple(k_pages.shape)}")
     n, heads, d = q.shape
