@@ -7,13 +7,14 @@ from a :class:`PagedCache`, whose size a window bounds for recordings of any len
 """
 from __future__ import annotations
 
+import operator
 from typing import List, Optional, Sequence
 
 import torch
 from torch import nn
 
 from .. import ops
-from ..ops.dispatch import CACHE_WIDTHS, runs_native
+from ..ops.dispatch import CACHE_WIDTHS, check_alternatives, runs_native
 from .blocks import GatedMlp, Linear, RmsNorm, TokenEmbedding
 from .init_utils import SeedSequence, fill_uniform_fan_
 
@@ -161,13 +162,16 @@ class AttentionDecoder(nn.Module):
         r = ops.token_logprobs(self.logits(self.features(frames, previous, lengths)), targets.reshape(-1), top, temperature)
         return ops.TokenLogprobs(*(None if v is None else v.view(*targets.shape, *v.shape[1:]) for v in r))
 
+    def _cache_width(self) -> int:
+        width = self.head_weight.shape[1] // self.heads
+        if width not in CACHE_WIDTHS and runs_native(self.head_weight, "mha"):
+            raise ValueError(f"the kernels keep heads of {' or '.join(map(str, CACHE_WIDTHS))} channels in a cache, this model's have {width}")
+        return width
+
     def make_cache(self, sequences: int, most_tokens: int, slots: int = 16, pages: Optional[int] = None) -> PagedCache:
         """A cache for ``sequences`` recordings of up to ``most_tokens`` frames.  Without ``pages`` the pool holds all that they can need
         with single steps: with a window, of each the pages of the first tokens and of the window."""
-        weight = self.head_weight
-        width = weight.shape[1] // self.heads
-        if width not in CACHE_WIDTHS and runs_native(weight, "mha"):
-            raise ValueError(f"the kernels keep heads of {' or '.join(map(str, CACHE_WIDTHS))} channels in a cache, this model's have {width}")
+        weight, width = self.head_weight, self._cache_width()
         if pages is None:
             each = -(-most_tokens // slots)
             if self.window is not None:
@@ -176,21 +180,39 @@ class AttentionDecoder(nn.Module):
         return PagedCache(len(self.block), pages, slots, self.kv_heads, width, sequences, most_tokens, weight.dtype,
                           weight.device, self.window, self.sinks)
 
+    def _check_cache(self, cache: PagedCache) -> None:
+        """A cache that does not go with this model would be found out with some layers written, or not at all."""
+        weight = self.head_weight
+        fits = (len(self.block), self.kv_heads, self._cache_width())
+        if (cache.k.shape[0], *cache.k.shape[3:]) != fits or cache.k.dtype != weight.dtype or cache.k.device != weight.device:
+            raise ValueError(f"the model has {fits[0]} layers of {fits[1]} key heads of {fits[2]}, {weight.dtype} on {weight.device}; the cache "
+                             f"{cache.k.shape[0]} of {cache.k.shape[3]} of {cache.k.shape[4]}, {cache.k.dtype} on {cache.k.device}")
+        if cache.window is not None and (self.window is None or cache.window < self.window or cache.sinks < self.sinks):
+            raise ValueError(f"the cache gives back what a window of {cache.window} and {cache.sinks} first tokens do not see, the model sees "
+                             f"{self.window} and {self.sinks}")
+
     @torch.no_grad()
     def extend(self, frames: torch.Tensor, previous: torch.Tensor, cache: PagedCache, new: Sequence[int], top: int = 1,
                temperature: float = 1.0) -> ops.TokenLogprobs:
         """New frames ``(N, E)``, ``new[b]`` of them of sequence ``b`` one after the other, with the actions before them ``(N,)``: the
         ``top`` most likely actions at each, with their log probabilities."""
+        new = [operator.index(n) for n in new]
         if sum(new) != frames.shape[0]:
             raise ValueError(f"{sum(new)} new frames are counted, {frames.shape[0]} given")
-        cache.make_room(new)
+        if previous.shape != (frames.shape[0],):
+            raise ValueError(f"the actions before {frames.shape[0]} frames are ({frames.shape[0]},), got {tuple(previous.shape)}")
+        self._check_cache(cache)
+        check_alternatives(self.vocab, top, temperature)
+        if frames.dtype != cache.k.dtype:
+            raise TypeError(f"the cache is {cache.k.dtype}, the frames {frames.dtype}")
+        x = self._inputs(frames, previous)
+        cache.make_room(new)                             # from here on the cache counts them
         offsets = None
         if any(n != 1 for n in new):
             starts = [0]
             for n in new:
                 starts.append(starts[-1] + n)
             offsets = torch.tensor(starts, dtype=torch.int32, device=frames.device)
-        x = self._inputs(frames, previous)
         for i, block in enumerate(self.block):
             x = block.extend(x, cache.k[i], cache.v[i], cache, offsets, self.freqs)
         return ops.token_logprobs(self.logits(self.ln_f(x)), None, top, temperature)

@@ -305,6 +305,14 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]
 
 
+def check_alternatives(vocab: int, top: int, temperature: float) -> None:
+    """What :func:`token_logprobs` takes of a vocabulary."""
+    if not 0 <= top <= min(MAX_ALTERNATIVES, vocab):
+        raise ValueError(f"between 0 and {min(MAX_ALTERNATIVES, vocab)} alternatives of {vocab} tokens, got {top}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"the temperature is above 0 and finite, got {temperature}")
+
+
 def token_logprobs(logits, targets=None, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
     """Of ``softmax(logits / temperature)`` over the last dimension: ``logprob (...)`` of ``targets (...)`` (None without),
     ``entropy (...)`` in nats and the ``top`` most likely tokens, ``top_logprobs`` and ``top_ids`` ``(..., top)`` (None for
@@ -317,10 +325,7 @@ def token_logprobs(logits, targets=None, top: int = 0, temperature: float = 1.0)
         raise ValueError(f"logits are (..., vocabulary), got {tuple(logits.shape)}")
     if targets is not None and (targets.shape != logits.shape[:-1] or targets.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"targets are int32 or int64 {tuple(logits.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
-    if not 0 <= top <= min(MAX_ALTERNATIVES, logits.shape[-1]):
-        raise ValueError(f"between 0 and {min(MAX_ALTERNATIVES, logits.shape[-1])} alternatives of {logits.shape[-1]} tokens, got {top}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"the temperature is above 0 and finite, got {temperature}")
+    check_alternatives(logits.shape[-1], top, temperature)
     if logits.is_cuda and _BACKEND == "auto" and logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
         from .logprobs import token_logprobs as f
         return TokenLogprobs(*f(logits, targets, top, temperature))

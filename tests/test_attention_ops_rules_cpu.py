@@ -235,10 +235,55 @@ def test_a_cache_that_the_kernels_do_not_take_is_refused_when_it_is_made(heads, 
     """64 and 128 channels a head; 96 and 32, which train."""
     from fbamtrain_b200.ops import dispatch
     model = _decoder(heads, dim)
-    assert model.make_cache(2, 50).k.shape[-1] == dim // heads              # the definitions take any
+    cache = model.make_cache(2, 50)
+    assert cache.k.shape[-1] == dim // heads                                # the definitions take any
     monkeypatch.setattr(dispatch, "_native_inner", lambda t, dtype, family: True)
     if fits:
         model.make_cache(2, 50)
-    else:
-        with pytest.raises(ValueError, match="64 or 128"):
-            model.make_cache(2, 50)
+        return
+    with pytest.raises(ValueError, match="64 or 128"):
+        model.make_cache(2, 50)
+    with pytest.raises(ValueError, match="64 or 128"):
+        model.step(torch.randn(2, 24), torch.tensor([1, 2]), cache)
+    assert cache.lengths.tolist() == [0, 0]
+
+
+def test_a_refused_step_leaves_the_cache_as_it_was():
+    """A call that raises has counted no tokens and taken no pages, so that it can be made again; with pages of another model, or of one
+    that looks further back, it is refused."""
+    from fbamtrain_b200.models import PagedCache
+    model, gen = _decoder(), torch.Generator().manual_seed(2)
+    cache = model.make_cache(2, 40, slots=8)
+    frames, previous = torch.randn(5, 24, generator=gen), torch.tensor([1, 2, 3, 4, 5])
+    model.extend(frames, previous, cache, [4, 1])
+
+    def state():
+        return [x.clone() for x in (cache.k, cache.v, cache.tables, cache.lengths)], list(cache._lengths), cache.free_pages
+
+    def same(a, b):
+        return all(torch.equal(x.nan_to_num(), y.nan_to_num()) for x, y in zip(a[0], b[0])) and a[1:] == b[1:]
+
+    before = state()
+    for bad in (dict(frames=frames[:, :23]), dict(previous=previous[:4]), dict(previous=previous.view(1, 5)), dict(previous=previous.float()),
+                dict(frames=frames.double()), dict(top=99), dict(top=-1), dict(temperature=0.0), dict(new=[6, -1]), dict(new=[2, 2]),
+                dict(new=[2.5, 2.5]), dict(new=[5]), dict(new=[5, 0, 0]), dict(new=[0, 5], frames=frames[:0])):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            model.extend(**{"frames": frames, "previous": previous, "cache": cache, "new": [2, 3], **bad})
+        assert same(state(), before), bad
+    got = model.extend(frames, previous, cache, torch.tensor([2, 3]))
+    assert got.entropy.shape == (5,) and cache.lengths.tolist() == [6, 4]
+
+    nothing = model.extend(frames[:0], previous[:0], cache, [0, 0])
+    assert nothing.entropy.shape == (0,) and nothing.top_ids.shape == (0, 1) and cache.lengths.tolist() == [6, 4]
+
+    def of(layers=2, kv=2, d=64, dtype=torch.float32, window=9, sinks=2):
+        return PagedCache(layers, 6, 8, kv, d, 2, 40, dtype, "cpu", window, sinks)
+
+    for fits in (of(), of(window=None), of(window=20, sinks=30), of(window=9, sinks=2)):
+        model.extend(frames, previous, fits, [2, 3])
+    for other in (of(layers=1), of(layers=3), of(kv=4), of(d=32), of(dtype=torch.float64), of(window=8), of(sinks=1)):
+        with pytest.raises(ValueError, match="model"):
+            model.extend(frames, previous, other, [2, 3])
+        assert other.lengths.tolist() == [0, 0]
+    with pytest.raises(ValueError, match="model"):
+        _decoder(window=None).extend(frames, previous, of(), [2, 3])

@@ -174,3 +174,35 @@ def test_append_of_rows_that_offsets_go_beyond():
         assert torch.equal((a != c).any(-1), (b != c).any(-1))         # the same slots
     oracle.within(y, *oracle.cached(q, *got, *cache[2:], offsets.clamp(max=5), None, 0))
     assert not y[0].any() and not q[0].any()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# the decoder
+# ------------------------------------------------------------------------------------------------------------------
+def test_a_refused_step_leaves_the_cache_as_it_was():
+    from fbamtrain_b200.models import AttentionDecoder, PagedCache
+    from fbamtrain_b200.models.init_utils import SeedSequence
+
+    def model(dim):
+        return AttentionDecoder(frame_dim=24, dim=dim, layers=2, heads=4, inner=32, vocab=37, dtype=BF, seeds=SeedSequence(3), kv_heads=2,
+                                window=9, sinks=2).cuda()
+
+    decoder, gen = model(256), _gen("decoder")
+    cache, frames, previous = decoder.make_cache(2, 40, slots=8), _randn(gen, 5, 24), torch.arange(5, device="cuda")
+    decoder.extend(frames, previous, cache, [4, 1])
+    before = [x.clone() for x in (cache.k, cache.v, cache.tables, cache.lengths)]
+    for bad in (dict(frames=frames[:, :23]), dict(frames=frames.half()), dict(frames=frames.cpu()), dict(previous=previous[:4]), dict(top=99),
+                dict(temperature=0.0), dict(new=[6, -1]), dict(new=[0, 5], previous=previous.cpu())):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            decoder.extend(**{"frames": frames, "previous": previous, "cache": cache, "new": [2, 3], **bad})
+        assert cache._lengths == [4, 1]
+    for a, b in zip(before, (cache.k, cache.v, cache.tables, cache.lengths)):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    other = model(384)                                    # 96 channels a head
+    with pytest.raises(ValueError, match="64 or 128"):
+        other.make_cache(2, 40)
+    by_hand = PagedCache(2, 9, 8, 2, 96, 2, 40, BF, "cuda", 9, 2)
+    with pytest.raises(ValueError, match="64 or 128"):
+        other.extend(frames, previous, by_hand, [2, 3])
+    assert by_hand.lengths.tolist() == [0, 0]
+    nv.check_status(frames.device)
