@@ -205,6 +205,9 @@ class AttentionDecoder(nn.Module):
         check_alternatives(self.vocab, top, temperature)
         if frames.dtype != cache.k.dtype:
             raise TypeError(f"the cache is {cache.k.dtype}, the frames {frames.dtype}")
+        if frames.shape[0] == 0:
+            cache.make_room(new)
+            return ops.token_logprobs(frames.new_empty((0, self.vocab)), None, top, temperature)
         x = self._inputs(frames, previous)
         cache.make_room(new)                             # from here on the cache counts them
         offsets = None

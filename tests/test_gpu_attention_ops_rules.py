@@ -206,3 +206,17 @@ def test_a_refused_step_leaves_the_cache_as_it_was():
         other.extend(frames, previous, by_hand, [2, 3])
     assert by_hand.lengths.tolist() == [0, 0]
     nv.check_status(frames.device)
+
+
+def test_a_step_without_frames():
+    from fbamtrain_b200.models import AttentionDecoder
+    from fbamtrain_b200.models.init_utils import SeedSequence
+    decoder = AttentionDecoder(frame_dim=24, dim=256, layers=2, heads=4, inner=32, vocab=37, dtype=BF, seeds=SeedSequence(3), window=9).cuda()
+    cache, frames, previous = decoder.make_cache(2, 40, slots=8), _randn(_gen("none"), 5, 24), torch.arange(5, device="cuda")
+    decoder.extend(frames, previous, cache, [4, 1])
+    nothing = decoder.extend(frames[:0], previous[:0], cache, [0, 0], top=3)
+    assert nothing.entropy.shape == (0,) and nothing.top_ids.shape == nothing.top_logprobs.shape == (0, 3)
+    assert cache.lengths.tolist() == [4, 1]
+    with pytest.raises(ValueError):
+        decoder.extend(frames[:0], previous[:0], cache, [0, 0, 0])
+    nv.check_status(frames.device)
