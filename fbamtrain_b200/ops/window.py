@@ -151,6 +151,8 @@ def _lengths(lengths, like):
         return None
     if lengths.device != like.device:
         raise ValueError(f"lengths are on {lengths.device}, the heads on {like.device}")
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, 2 ** 31 - 1)          # cut to 32 bits 2^32 + 3 would be 3
     return lengths.to(torch.int32).contiguous()
 
 

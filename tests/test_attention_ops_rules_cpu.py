@@ -203,6 +203,16 @@ def test_warps_meet_whether_or_not_a_wait_of_theirs_expired():
             assert conditions and not any(re.search(r"\bok\b|mbar_wait", h) for h in conditions), conditions
 
 
+@pytest.mark.parametrize("dtype", [I32, torch.int64])
+def test_lengths_reach_the_kernels_as_what_they_are(dtype):
+    """Beyond 32 bits too, where they are as good as the largest, or as none."""
+    from fbamtrain_b200.ops.window import _lengths
+    far = [2 ** 32 + 3, -2 ** 32 + 3, 2 ** 62, -2 ** 63] if dtype == torch.int64 else []
+    lengths = torch.tensor([0, 7, 2 ** 31 - 1, -5] + far, dtype=dtype)
+    got = _lengths(lengths, lengths)
+    assert got.dtype == I32 and [max(n, 0) for n in got.tolist()] == [0, 7, 2 ** 31 - 1, 0] + [2 ** 31 - 1, 0] * (len(far) // 2)
+
+
 # ------------------------------------------------------------------------------------------------------------------
 # plans
 # ------------------------------------------------------------------------------------------------------------------

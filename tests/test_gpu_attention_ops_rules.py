@@ -220,3 +220,14 @@ def test_a_step_without_frames():
     with pytest.raises(ValueError):
         decoder.extend(frames[:0], previous[:0], cache, [0, 0, 0])
     nv.check_status(frames.device)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# lengths
+# ------------------------------------------------------------------------------------------------------------------
+def test_lengths_beyond_32_bits():
+    gen = _gen("lengths")
+    heads = [_randn(gen, 4, 150, n, 64) for n in (2, 1, 1, 2)]
+    far = torch.tensor([2 ** 32 + 3, -2 ** 32 + 3, 150, 2 ** 62], device="cuda")
+    for lengths in (far, far.clamp(-1, 151).to(I32), torch.tensor([150, 0, 150, 150], device="cuda")):
+        _gradients(*heads, 40, 3, lengths)
