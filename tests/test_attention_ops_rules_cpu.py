@@ -214,6 +214,23 @@ def test_lengths_reach_the_kernels_as_what_they_are(dtype):
 
 
 # ------------------------------------------------------------------------------------------------------------------
+# nothing at all
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("b,t", [(0, 3), (2, 0), (0, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_gradients_of_no_tokens_are_empty(b, t, dtype):
+    q, k, v = (torch.randn(b, t, n, 8).to(dtype).requires_grad_() for n in (4, 2, 2))
+    lengths = torch.zeros(b, dtype=I32)
+    for how in ((None, 0, None), (3, 1, lengths)):
+        y = ops.window_attention(q, k, v, *how)
+        assert y.shape == q.shape and y.dtype == dtype
+        assert [g.shape for g in torch.autograd.grad((y.float().sum(),), (q, k, v))] == [q.shape, k.shape, v.shape]
+    qkv = torch.randn(b, t, 8, 8).to(dtype).requires_grad_()
+    for y in (ops.window_attention_qkv(qkv, 2, 3), ops.rotary(qkv, torch.arange(t), ops.rotary_frequencies(8))):
+        assert torch.autograd.grad((y.float().sum(),), (qkv,))[0].shape == qkv.shape
+
+
+# ------------------------------------------------------------------------------------------------------------------
 # plans
 # ------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("t,kv,group", [(13_400_064, 232, 1), (11_783_936, 150, 2), (51_025_920, 4, 4), (2_000_000, 1, 1)])
