@@ -59,6 +59,34 @@ def test_large_gradients_in_half(t, h, kv, d, win, sinks):
     _gradients(q, k, v, dy, win, sinks)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, HALF])
+def test_delta_has_what_rounding_took_off_the_output(d, dtype):
+    """Two equal scores over equal keys: the gradient of the query is nothing at all, the two scores' gradients cancel.  The values are
+    one step of the type apart, so that the output, half way between, loses as much in rounding as they differ by: with delta from the
+    rounded output alone the gradient is tens of times the bound."""
+    gen = _gen("residual", d)
+    t, h, kv, unit = 300, 4, 2, oracle.UNIT[dtype]
+    q, k = torch.zeros(1, t, h, d, dtype=dtype, device="cuda"), torch.ones(1, t, kv, d, dtype=dtype, device="cuda")
+    v = (1.0 + 2 * unit * torch.randint(0, 2, (1, t, kv, d), generator=gen, device="cuda")).to(dtype)
+    dy = _randn(gen, 1, t, h, d, dtype=dtype)
+    dy *= torch.arange(d, device="cuda") % (d // 8) == torch.arange(t, device="cuda").view(t, 1, 1) % (d // 8)     # eight channels a token
+    q.requires_grad_()
+    dq, = torch.autograd.grad((ops.window_attention(q, k, v, 2),), (q,), (dy,))
+    nv.check_status(q.device)
+    g, two = dy[0].double(), v[0].repeat_interleave(h // kv, 1).double()
+    two = torch.stack([two, torch.cat([two[:1], two[:-1]])])           # the token and the one before; the first sees itself only
+    out = two.mean(0)
+    dp, delta = (two * g).sum(-1), (out * g).sum(-1)
+    mass = (two * g).abs().sum(-1).amax(0)
+    # sums of eight products in fp32, delta from an output and a residual in 16 bits, dS rounded
+    wrong = (8 + 8) * 2.0 ** -24 * 2 * mass + unit ** 2 * mass + 2.0 ** -19 * (dp - delta).abs().amax(0)
+    wrong = d ** -0.5 * (wrong + unit * (dp - delta).abs().amax(0)) + 2 * oracle.FLOOR[dtype]
+    assert bool((dq[0].double().abs().amax(-1) <= wrong).all())
+    planted = d ** -0.5 * (dp - (out.to(dtype).double() * g).sum(-1)).mean(0).abs()
+    assert int((planted > 10 * wrong).sum()) > t * h // 2
+
+
 # ------------------------------------------------------------------------------------------------------------------
 # the paged cache
 # ------------------------------------------------------------------------------------------------------------------
