@@ -38,18 +38,20 @@ _TWO_PI = 2 * Decimal("3.14159265358979323846264338327950288419716939937510")
 
 
 def rotary_frequencies(dims: int, base: float, factor: float, context: Optional[int], few: float, many: float) -> RotaryFrequencies:
-    # in 50 digits: with the 53 bits of a double the last ones of a fraction of 64, which far positions bring up, would be anything
-    with localcontext(prec=50):
-        log_base, slower, least, most = Decimal(float(base)).ln(), Decimal(float(factor)), Decimal(float(few)), Decimal(float(many))
-        turns = []
-        for i in range(dims // 2):
-            turn = (log_base * (-2 * i) / dims).exp() / _TWO_PI
+    # in 40 digits: with the 53 bits of a double the last ones of a fraction of 64, which far positions bring up, would be anything
+    with localcontext(prec=40):
+        slower, least, most = Decimal(float(factor)), Decimal(float(few)), Decimal(float(many))
+        turns, turn, next_pair = [], 2 ** 64 / _TWO_PI, (Decimal(float(base)).ln() * -2 / max(dims, 1)).exp()
+        for _ in range(dims // 2):
+            scaled = turn
             if factor != 1.0:
                 kept = Decimal(0)
                 if context is not None:
-                    kept = min(Decimal(1), max(Decimal(0), (context * turn - least) / (most - least)))
-                turn *= kept + (1 - kept) / slower
-            turns.append(int((turn * 2 ** 64).to_integral_value()) % 2 ** 64)
+                    around = context * turn / 2 ** 64
+                    kept = min(Decimal(1), max(Decimal(0), (around - least) / (most - least)))
+                scaled = turn * kept + turn * (1 - kept) / slower
+            turns.append(int(scaled.to_integral_value()) % 2 ** 64)
+            turn *= next_pair
     magnitude = 1.0 + 0.1 * math.log(factor) if factor > 1.0 and context is not None else 1.0
     return RotaryFrequencies(tuple(turns), magnitude)
 
