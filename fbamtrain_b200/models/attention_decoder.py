@@ -3,7 +3,8 @@ with rotary positions → log probabilities.
 
 Beside :class:`~fbamtrain_b200.models.recurrent_decoder.RecurrentDecoder` this one keeps the last ``window`` frames and the first
 ``sinks`` of a recording as they were instead of a state.  ``forward`` scores whole sequences; ``extend`` and ``step`` answer new frames
-from a :class:`PagedCache`, whose size a window bounds for recordings of any length.  Query heads may share key heads.
+from a :class:`PagedCache`: a window bounds its pages, however long the recordings get (up to the tokens that its tables are made for).
+Query heads may share key heads.
 """
 from __future__ import annotations
 
