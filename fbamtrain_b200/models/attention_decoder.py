@@ -30,12 +30,13 @@ class PagedCache:
                  device, window: Optional[int] = None, sinks: int = 0):
         if slots < 1 or slots % 8:
             raise ValueError(f"pages have a multiple of 8 slots, got {slots}")
-        self.k = torch.empty(layers, pages, slots, kv_heads, head_dim, dtype=dtype, device=device)
-        self.v = torch.empty_like(self.k)
         self.slots, self.window, self.sinks = slots, window, sinks
         self.most = -(-most_tokens // slots)
-        self.tables = torch.full((sequences, self.most), -1, dtype=torch.int32, device=device)
-        self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):                # tensors made in that mode could not be written outside of it
+            self.k = torch.empty(layers, pages, slots, kv_heads, head_dim, dtype=dtype, device=device)
+            self.v = torch.empty_like(self.k)
+            self.tables = torch.full((sequences, self.most), -1, dtype=torch.int32, device=device)
+            self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
         self._lengths = [0] * sequences
         self._rows: List[dict] = [{} for _ in range(sequences)]      # page of each place in a sequence's row of the table
         self._free = list(range(pages - 1, -1, -1))

@@ -314,3 +314,20 @@ def test_a_refused_step_leaves_the_cache_as_it_was():
         assert other.lengths.tolist() == [0, 0]
     with pytest.raises(ValueError, match="model"):
         _decoder(window=None).extend(frames, previous, of(), [2, 3])
+
+
+def test_a_cache_serves_in_and_out_of_inference_mode():
+    """Wherever it was made."""
+    model, gen = _decoder(), torch.Generator().manual_seed(4)
+    frames, previous = torch.randn(5, 24, generator=gen), torch.tensor([1, 2, 3, 4, 5])
+    answers = []
+    for made in (True, False):
+        with torch.inference_mode(made):
+            cache = model.make_cache(2, 40, slots=8)
+        for mode in (True, False, True):
+            with torch.inference_mode(mode):
+                r = model.extend(frames, previous, cache, [2, 3])
+        cache.reset(0)
+        assert cache.lengths.tolist() == [0, 9]
+        answers.append(r.entropy)
+    assert torch.equal(*answers)
