@@ -4,7 +4,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
-from decimal import Decimal, localcontext
+from decimal import Context, Decimal, localcontext
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -34,12 +34,12 @@ class RotaryFrequencies(_Frequencies):
         return 2 * len(self.turns)
 
 
-_TWO_PI = 2 * Decimal("3.14159265358979323846264338327950288419716939937510")
+_TWO_PI = Decimal("6.28318530717958647692528676655900576839433879875")     # as it is written: a product would be rounded
 
 
 def rotary_frequencies(dims: int, base: float, factor: float, context: Optional[int], few: float, many: float) -> RotaryFrequencies:
     # in 40 digits: with the 53 bits of a double the last ones of a fraction of 64, which far positions bring up, would be anything
-    with localcontext(prec=40):
+    with localcontext(Context(prec=40)):
         slower, least, most = Decimal(float(factor)), Decimal(float(few)), Decimal(float(many))
         turns, turn, next_pair = [], 2 ** 64 / _TWO_PI, (Decimal(float(base)).ln() * -2 / max(dims, 1)).exp()
         for _ in range(dims // 2):

@@ -1,5 +1,6 @@
 """Rotary positions, windowed attention and the paged cache without a GPU: what each call promises beyond ordinary inputs."""
 import copy
+import decimal
 import io
 import math
 import os
@@ -156,6 +157,13 @@ def test_frequencies_fill_their_64_bits(settings):
         else:
             turn /= factor
         assert abs(got - turn * 2 ** 64) <= Fraction(1, 2) + Fraction(1, 10 ** 9)
+
+
+def test_frequencies_do_not_depend_on_the_callers_decimal_context():
+    want = ops.rotary_frequencies(64, factor=3.0, context=50)
+    with decimal.localcontext(prec=5, rounding=decimal.ROUND_UP) as around:
+        around.traps[decimal.Inexact] = True
+        assert ops.rotary_frequencies(64, factor=3.0, context=50) == want
 
 
 def test_the_definition_of_rotary_at_far_positions():
